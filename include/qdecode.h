@@ -44,6 +44,7 @@ extern "C" {
 
 #define QD_KV_F16 0           /* f16 KV cache (default) */
 #define QD_KV_F32 1           /* f32 KV cache, as the reference (cache_write.wgsl) */
+#define QD_KV_BF16 2          /* bf16: the paged operators and qd_sample_rows only */
 
 typedef struct qd_engine qd_engine;
 
@@ -361,6 +362,112 @@ int qd_gqa_decode(const float* q, const void* k_cache, const void* v_cache, int 
 int qd_gqa_decode_noalloc(const float* q, const void* k_cache, const void* v_cache, int kv_dtype,
                           float* y, uint32_t seq_len, uint32_t q_heads, uint32_t kv_heads,
                           uint32_t head_dim, void* stream);
+
+/* ---- paged key-value cache (device pointers) -------------------------------------
+ * No counterpart in the reference (one contiguous cache of 256 positions). A cache of
+ * pages, each page_size positions of every KV head; a block table names the page of
+ * every page_size positions of every sequence, so sequences of any length share one
+ * pool and grow page by page. The three calls below make one step over it: qd_paged_append,
+ * then qd_paged_attn_decode (one new token per sequence) or qd_paged_attn_prompt (a ragged
+ * batch of prompt chunks). All of them only enqueue, take every length from device memory
+ * (they can be captured into a graph and replayed with new lengths), and use no memory of
+ * the library's: calls on different streams with workspaces of their own may overlap.
+ *
+ * New tokens: row r of qkv / q / y belongs to the sequence b with
+ * q_starts[b] <= r < q_starts[b + 1] (q_starts: batch + 1 ascending device entries from 0),
+ * at position seq_lens[b] - (q_starts[b + 1] - r); rows from q_starts[batch] on (padding)
+ * are not read and what they would write is left as it was. q_starts NULL: one new token
+ * per sequence, row r = sequence r.
+ *
+ * Which keys: the query at position p sees key j when j <= p and (window == 0, or
+ * j > p - window, or j < sinks): with a window, the last `window` positions (its own
+ * included) and the first `sinks` ones. Only pages with a visible position are looked up
+ * in the table: others may be free (any entry). Cache rows that no query of the call sees,
+ * such as those behind a sequence's end or before every query's window, are never used,
+ * whatever they hold. A query that sees nothing (seq_lens[b] <= 0) gets zeros.
+ *
+ * A table entry outside [0, num_pages) where a position is visible, a length beyond
+ * table_width * page_size and a new token at a negative position (or, in the append, beyond
+ * the rotation tables) can only be seen on the device: the position is left out (not
+ * written, not attended to; the length is cut) and the bit is set in *status. */
+#define QD_PAGED_BAD_PAGE 1     /* status bits (or-ed; never cleared by the library) */
+#define QD_PAGED_BAD_LENGTH 2
+
+typedef struct qd_paged_kv {
+  void* k;                      /* [num_pages][kv_heads][page_size][head_dim] of dtype, 16-byte aligned */
+  void* v;                      /* the same shape */
+  int dtype;                    /* QD_KV_F16 or QD_KV_BF16 */
+  int num_pages;
+  int page_size;                /* a power of two, 16..256 */
+  int kv_heads;
+  int head_dim;                 /* 128 */
+  int batch;                    /* sequences, 0..4096 */
+  const int32_t* block_table;   /* [batch][table_stride], table_width entries of each row used */
+  int table_width, table_stride;
+  const int32_t* seq_lens;      /* [batch]: positions held, the new tokens included */
+  int32_t* status;              /* device word of QD_PAGED_* bits, or NULL */
+} qd_paged_kv;
+
+/* Head RMSNorm of q and k, rotary position, and the K and V rows written to their pages, in
+ * one pass over the projections' output: row r of qkv is [q_heads*128 | kv_heads*128 (k) |
+ * kv_heads*128 (v)], rows qkv_stride elements apart. For each head x of q and k:
+ *   x <- x * rsqrt(mean(x^2) + eps) * w    (w = q_norm / k_norm [128] f32; NULL: left out)
+ *   x[i], x[i+64] <- x[i] c - x[i+64] s, x[i+64] c + x[i] s,   i < 64,
+ * c = cos[position * rope_stride + i], s = sin[...] (f32 tables of rope_len entries each;
+ * both NULL: no rotation). q goes to q_out [rows][q_heads*128] (rows q_out_stride elements
+ * apart; q_out may be qkv itself, with its type and stride), k and v to the cache. All
+ * arithmetic in f32, rounded once to the output's type. qkv_dtype, q_out_dtype: QD_KV_F16,
+ * QD_KV_F32 or QD_KV_BF16; pointers 16-byte aligned, strides multiples of 8. Two rows of one
+ * call never share a position of the cache unless the block table does (then either wins).
+ * Replaces, for any number of rows, head_rms_norm.wgsl, rope.wgsl:14-31 and
+ * cache_write.wgsl. */
+int qd_paged_append(const qd_paged_kv* kv, const void* qkv, int qkv_dtype, int64_t qkv_stride, int rows,
+                    const int32_t* q_starts, int q_heads, const float* q_norm, const float* k_norm, float eps,
+                    const float* cos, const float* sin, int64_t rope_len, int64_t rope_stride, void* q_out,
+                    int q_out_dtype, int64_t q_out_stride, void* stream);
+
+/* Attention of one new token per sequence (rows = batch): y[b] = softmax(scale * q[b] k^T) v
+ * over the keys that position seq_lens[b] - 1 sees. q, y [batch][q_heads][128], rows q_stride /
+ * y_stride elements apart (multiples of 8), 16-byte aligned; dtype (of both) QD_KV_F32 or the
+ * cache's. q_heads is a multiple of kv_heads, at most 64 times it. The softmax and its sums
+ * are f32; with dtype QD_KV_F32 the products keep f32 accuracy (f16 cache) or 16 bits (bf16
+ * cache: both operands as a sum of two bf16). scale 0 means 1/sqrt(128). The workspace holds
+ * the joined parts' partial sums; nothing in it needs to start at zero. */
+size_t qd_paged_attn_decode_workspace_bytes(int batch, int q_heads);
+int qd_paged_attn_decode(const qd_paged_kv* kv, const void* q, int dtype, int64_t q_stride, int q_heads, int window,
+                         int sinks, float scale, void* y, int64_t y_stride, void* workspace, void* stream);
+
+/* The same for a ragged batch of new tokens (q_starts as above, not NULL): each row attends
+ * to the keys its own position sees, the call's own new tokens among them (append them
+ * first). q, y [rows][q_heads][128]. */
+size_t qd_paged_attn_prompt_workspace_bytes(int batch, int rows, int q_heads, int kv_heads);
+int qd_paged_attn_prompt(const qd_paged_kv* kv, const void* q, int dtype, int64_t q_stride, int rows,
+                         const int32_t* q_starts, int q_heads, int window, int sinks, float scale, void* y,
+                         int64_t y_stride, void* workspace, void* stream);
+
+/* ---- sampling of a batch of rows -------------------------------------------------- */
+
+/* One token per row of logits [rows][vocab] (device, dtype QD_KV_F32 / F16 / BF16, rows
+ * row_stride elements apart), every row with settings of its own (device arrays of `rows`
+ * entries; a NULL array stands for the value in brackets) and its own given random number:
+ *  - order: by value, ties (and -0 / +0) to the lower index, NaN below every number;
+ *  - w_i = exp((v_i - v_max) / temperature[r])   [1]; temperature <= 0 or NaN, or top_k == 1:
+ *    the first token of the order (greedy);
+ *  - top_k[r] [0]: the first top_k of the order; <= 0 or >= vocab: all;
+ *  - top_p[r] [1]: of those, the shortest prefix whose sum reaches top_p times their sum;
+ *    >= 1 or NaN: all of them, <= 0: the first;
+ *  - min_p[r] [0]: of those, the ones with w_i >= min_p (the first always stays); NaN: all;
+ *  - the token is the first kept one whose running sum exceeds u[r] times the kept sum
+ *    (u in [0, 1); the last kept one of non-zero weight if rounding leaves none).
+ * Weights and sums are exact to 2^-44 of the largest weight (64-bit fixed point: the result
+ * does not depend on the order of summation; a smaller weight counts as zero and is never
+ * drawn). A row whose largest value is infinite, or all NaN, is greedy. ids[r] receives the
+ * token, logprobs[r] (NULL: left out) the logarithm of its share of the kept sum (0 for a
+ * greedy row). Unlike qd_sample_logits there is no limit of 64 candidates. vocab at most
+ * 393216. Enqueues only; needs no workspace. */
+int qd_sample_rows(const void* logits, int dtype, int rows, uint32_t vocab, int64_t row_stride,
+                   const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                   const float* u, int32_t* ids, float* logprobs, void* stream);
 
 #ifdef __cplusplus
 }

@@ -20,6 +20,9 @@ QD_E_DEVICE = -6
 QD_E_TIMEOUT = -7
 QD_KV_F16 = 0
 QD_KV_F32 = 1
+QD_KV_BF16 = 2
+QD_PAGED_BAD_PAGE = 1
+QD_PAGED_BAD_LENGTH = 2
 
 # Every function include/qdecode.h declares (checked by the tests).
 EXPORTS = (
@@ -38,6 +41,8 @@ EXPORTS = (
     "qd_batch_shard_sync", "qd_engine_inject_stall", "qd_batch_inject_stall",
     "qd_run_kernel_benchmarks", "qd_run_full_decoder_stack_benchmark",
     "qd_generate_sample", "qd_sample_workspace_bytes", "qd_sample_logits",
+    "qd_paged_append", "qd_paged_attn_decode_workspace_bytes", "qd_paged_attn_decode",
+    "qd_paged_attn_prompt_workspace_bytes", "qd_paged_attn_prompt", "qd_sample_rows",
 )
 
 
@@ -61,6 +66,13 @@ class QdStats(C.Structure):
 
 class QdSampling(C.Structure):
     _fields_ = [("temperature", C.c_float), ("top_k", C.c_int), ("top_p", C.c_float), ("seed", C.c_uint64)]
+
+
+class QdPagedKv(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int), ("num_pages", C.c_int),
+                ("page_size", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("batch", C.c_int),
+                ("block_table", C.c_void_p), ("table_width", C.c_int), ("table_stride", C.c_int),
+                ("seq_lens", C.c_void_p), ("status", C.c_void_p)]
 
 
 class QdKernelBench(C.Structure):
@@ -198,6 +210,19 @@ def load(build_if_stale: bool = True):
     L.qd_sample_workspace_bytes.restype = C.c_size_t
     L.qd_sample_logits.argtypes = [vp, u32, C.POINTER(QdSampling), u32, vp, vp, vp]
     L.qd_sample_logits.restype = i32
+    i64, kv = C.c_int64, C.POINTER(QdPagedKv)
+    L.qd_paged_append.argtypes = [kv, vp, i32, i64, i32, vp, i32, vp, vp, f32, vp, vp, i64, i64, vp, i32, i64, vp]
+    L.qd_paged_append.restype = i32
+    L.qd_paged_attn_decode_workspace_bytes.argtypes = [i32, i32]
+    L.qd_paged_attn_decode_workspace_bytes.restype = C.c_size_t
+    L.qd_paged_attn_decode.argtypes = [kv, vp, i32, i64, i32, i32, i32, f32, vp, i64, vp, vp]
+    L.qd_paged_attn_decode.restype = i32
+    L.qd_paged_attn_prompt_workspace_bytes.argtypes = [i32, i32, i32, i32]
+    L.qd_paged_attn_prompt_workspace_bytes.restype = C.c_size_t
+    L.qd_paged_attn_prompt.argtypes = [kv, vp, i32, i64, i32, vp, i32, i32, i32, f32, vp, i64, vp, vp]
+    L.qd_paged_attn_prompt.restype = i32
+    L.qd_sample_rows.argtypes = [vp, i32, i32, u32, i64, vp, vp, vp, vp, vp, vp, vp, vp]
+    L.qd_sample_rows.restype = i32
     L.qd_run_kernel_benchmarks.argtypes = [vp, C.POINTER(QdKernelBench)]
     L.qd_run_kernel_benchmarks.restype = i32
     L.qd_run_full_decoder_stack_benchmark.argtypes = [vp, C.POINTER(QdStackBench)]

@@ -1,0 +1,186 @@
+// Host entries of the paged key-value cache operators (kernels: paged.cuh).
+#include <cmath>
+#include <string>
+
+#include "../../include/qdecode.h"
+#include "internal.cuh"
+#include "paged.cuh"
+
+namespace qd {
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static bool known_dtype(int d) { return d == QD_KV_F16 || d == QD_KV_F32 || d == QD_KV_BF16; }
+
+static void need(bool ok, const char* msg) {
+  if (!ok) throw QdError{QD_E_INVALID, msg};
+}
+
+static PagedArgs check_paged(const qd_paged_kv* kv) {
+  need(kv != nullptr, "paged cache: NULL pointer");
+  need(kv->dtype == QD_KV_F16 || kv->dtype == QD_KV_BF16, "paged cache: dtype must be QD_KV_F16 or QD_KV_BF16");
+  need(kv->head_dim == kHeadDim, "paged cache: head_dim must be 128");
+  need(kv->page_size >= 16 && kv->page_size <= 256 && (kv->page_size & (kv->page_size - 1)) == 0,
+       "paged cache: page_size must be a power of two from 16 to 256");
+  need(kv->kv_heads >= 1 && kv->kv_heads <= 1024, "paged cache: bad kv_heads");
+  need(kv->batch >= 0 && kv->batch <= 4096, "paged cache: batch must be 0..4096");
+  need(kv->num_pages >= 0 && kv->table_width >= 0 && kv->table_stride >= kv->table_width,
+       "paged cache: bad num_pages, table_width or table_stride");
+  need((long long)kv->table_width * kv->page_size <= 0x40000000LL, "paged cache: table_width * page_size beyond 2^30");
+  need(kv->batch == 0 || (kv->block_table && kv->seq_lens) , "paged cache: NULL block_table or seq_lens");
+  need(kv->num_pages == 0 || (kv->k && kv->v), "paged cache: NULL pool");
+  need(aligned16(kv->k) && aligned16(kv->v), "paged cache: pools must be 16-byte aligned");
+  PagedArgs a{};
+  a.k = kv->k;
+  a.v = kv->v;
+  a.num_pages = kv->num_pages;
+  while ((1 << a.page_shift) < kv->page_size) ++a.page_shift;
+  a.kv_heads = kv->kv_heads;
+  a.batch = kv->batch;
+  a.table = kv->block_table;
+  a.table_width = kv->table_width;
+  a.table_stride = kv->table_stride;
+  a.seq_lens = kv->seq_lens;
+  a.status = kv->status;
+  return a;
+}
+
+static PAttnArgs check_attn(const qd_paged_kv* kv, const void* q, int dtype, int64_t q_stride, int rows, int q_heads,
+                            int window, int sinks, float scale, void* y, int64_t y_stride) {
+  PAttnArgs a{};
+  a.kv = check_paged(kv);
+  need(rows >= 0, "paged attention: negative rows");
+  need(dtype == QD_KV_F32 || dtype == kv->dtype, "paged attention: q and y are QD_KV_F32 or of the cache's dtype");
+  need(q_heads >= 1 && q_heads % kv->kv_heads == 0 && q_heads / kv->kv_heads <= 64,
+       "paged attention: q_heads must be a multiple of kv_heads, at most 64 times it");
+  need(window >= 0 && sinks >= 0, "paged attention: window and sinks must not be negative");
+  need(std::isfinite(scale), "paged attention: scale must be finite");
+  need(rows == 0 || (q && y), "paged attention: NULL pointer");
+  need(aligned16(q) && aligned16(y), "paged attention: q and y must be 16-byte aligned");
+  need(q_stride >= (int64_t)q_heads * kHeadDim && y_stride >= (int64_t)q_heads * kHeadDim && q_stride % 8 == 0 &&
+           y_stride % 8 == 0,
+       "paged attention: row strides must be multiples of 8, at least q_heads * 128");
+  a.q = q;
+  a.q_stride = q_stride;
+  a.rows = rows;
+  a.q_heads = q_heads;
+  a.window = window;
+  a.sinks = sinks;
+  a.scale = scale == 0.0f ? 1.0f / std::sqrt((float)kHeadDim) : scale;
+  a.y = y;
+  a.dtype = dtype;
+  a.y_stride = y_stride;
+  return a;
+}
+
+static void launch_rows(const PAttnArgs& a, int kv_dtype, cudaStream_t s) {
+  const dim3 grid(a.rows, a.q_heads), block(128);
+  if (kv_dtype == QD_KV_F16) {
+    if (a.dtype == QD_KV_F32) launch_ex(k_paged_attn_rows<float, __half>, grid, block, 0, s, a);
+    else launch_ex(k_paged_attn_rows<__half, __half>, grid, block, 0, s, a);
+  } else {
+    if (a.dtype == QD_KV_F32) launch_ex(k_paged_attn_rows<float, __nv_bfloat16>, grid, block, 0, s, a);
+    else launch_ex(k_paged_attn_rows<__nv_bfloat16, __nv_bfloat16>, grid, block, 0, s, a);
+  }
+}
+
+}  // namespace qd
+
+using namespace qd;
+
+// Runs a checked body, turning every exception into the C status and message.
+template <typename F>
+static int guarded(F&& body) {
+  try {
+    body();
+  } catch (const QdError& err) {
+    set_thread_error(err.msg);
+    return err.code;
+  } catch (const std::exception& err) {
+    set_thread_error(err.what());
+    return QD_E_NOMEM;
+  }
+  return QD_OK;
+}
+
+extern "C" {
+
+int qd_paged_append(const qd_paged_kv* kv, const void* qkv, int qkv_dtype, int64_t qkv_stride, int rows,
+                    const int32_t* q_starts, int q_heads, const float* q_norm, const float* k_norm, float eps,
+                    const float* cos, const float* sin, int64_t rope_len, int64_t rope_stride, void* q_out,
+                    int q_out_dtype, int64_t q_out_stride, void* stream) {
+  return guarded([&] {
+    AppendArgs a{};
+    a.kv = check_paged(kv);
+    need(rows >= 0, "qd_paged_append: negative rows");
+    need(q_starts || rows == kv->batch, "qd_paged_append: without q_starts rows must equal the batch");
+    need(known_dtype(qkv_dtype) && known_dtype(q_out_dtype), "qd_paged_append: unknown dtype");
+    need(q_heads >= 0 && q_heads <= 65536, "qd_paged_append: bad q_heads");
+    const int64_t heads = (int64_t)q_heads + 2 * kv->kv_heads;
+    need(qkv_stride >= heads * kHeadDim && qkv_stride % 8 == 0,
+         "qd_paged_append: qkv_stride must be a multiple of 8, at least (q_heads + 2 kv_heads) * 128");
+    need(q_heads == 0 || (q_out_stride >= (int64_t)q_heads * kHeadDim && q_out_stride % 8 == 0),
+         "qd_paged_append: q_out_stride must be a multiple of 8, at least q_heads * 128");
+    need(std::isfinite(eps) && eps >= 0.0f, "qd_paged_append: eps must be finite and not negative");
+    need((cos == nullptr) == (sin == nullptr), "qd_paged_append: cos and sin go together");
+    need(!cos || (rope_len >= 0 && rope_stride >= 0 && rope_stride % 4 == 0),
+         "qd_paged_append: rope_stride must be a multiple of 4, not negative");
+    need(rows == 0 || (qkv && (q_out || q_heads == 0)), "qd_paged_append: NULL pointer");
+    need(aligned16(qkv) && aligned16(q_out) && aligned16(cos) && aligned16(sin) && aligned16(q_norm) &&
+             aligned16(k_norm),
+         "qd_paged_append: pointers must be 16-byte aligned");
+    if (rows == 0 || kv->batch == 0) return;
+    a.kv_dtype = kv->dtype;
+    a.qkv = qkv;
+    a.qkv_stride = qkv_stride;
+    a.rows = rows;
+    a.q_starts = q_starts;
+    a.q_heads = q_heads;
+    a.q_norm = q_norm;
+    a.k_norm = k_norm;
+    a.eps = eps;
+    a.cos_t = cos;
+    a.sin_t = sin;
+    a.rope_len = rope_len;
+    a.rope_stride = rope_stride;
+    a.q_out = q_out;
+    a.q_out_dtype = q_out_dtype;
+    a.q_out_stride = q_out_stride;
+    const long long warps = (long long)rows * ((heads + kAppendHeads - 1) / kAppendHeads);
+    need((warps + 7) / 8 <= 0x7fffffffLL, "qd_paged_append: too many rows");
+    const dim3 grid((unsigned)((warps + 7) / 8)), block(256);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (qkv_dtype == QD_KV_F32) launch_ex(k_paged_append<float>, grid, block, 0, s, a);
+    else if (qkv_dtype == QD_KV_F16) launch_ex(k_paged_append<__half>, grid, block, 0, s, a);
+    else launch_ex(k_paged_append<__nv_bfloat16>, grid, block, 0, s, a);
+  });
+}
+
+size_t qd_paged_attn_decode_workspace_bytes(int batch, int q_heads) { return 256; }
+
+int qd_paged_attn_decode(const qd_paged_kv* kv, const void* q, int dtype, int64_t q_stride, int q_heads, int window,
+                         int sinks, float scale, void* y, int64_t y_stride, void* workspace, void* stream) {
+  return guarded([&] {
+    need(kv != nullptr, "paged cache: NULL pointer");
+    PAttnArgs a = check_attn(kv, q, dtype, q_stride, kv->batch, q_heads, window, sinks, scale, y, y_stride);
+    if (a.rows == 0) return;
+    need(workspace != nullptr, "qd_paged_attn_decode: NULL workspace");
+    launch_rows(a, kv->dtype, static_cast<cudaStream_t>(stream));
+  });
+}
+
+size_t qd_paged_attn_prompt_workspace_bytes(int batch, int rows, int q_heads, int kv_heads) { return 256; }
+
+int qd_paged_attn_prompt(const qd_paged_kv* kv, const void* q, int dtype, int64_t q_stride, int rows,
+                         const int32_t* q_starts, int q_heads, int window, int sinks, float scale, void* y,
+                         int64_t y_stride, void* workspace, void* stream) {
+  return guarded([&] {
+    PAttnArgs a = check_attn(kv, q, dtype, q_stride, rows, q_heads, window, sinks, scale, y, y_stride);
+    if (rows == 0 || kv->batch == 0) return;
+    need(q_starts != nullptr, "qd_paged_attn_prompt: NULL q_starts");
+    need(workspace != nullptr, "qd_paged_attn_prompt: NULL workspace");
+    a.q_starts = q_starts;
+    launch_rows(a, kv->dtype, static_cast<cudaStream_t>(stream));
+  });
+}
+
+}  // extern "C"

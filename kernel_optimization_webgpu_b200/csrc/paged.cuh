@@ -1,0 +1,269 @@
+// Operators over a paged key-value cache: the fused head norm + rotation + append, and
+// attention of new tokens over the pages.
+//
+// Pools K, V: [page][kv_head][page_size][128]; the page_size rows of one (page, KV head) are
+// one contiguous range, which is what the attention kernels copy. Position p of sequence b
+// lives in page table[b][p / page_size], row p % page_size.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+
+namespace qd {
+
+struct PagedArgs {
+  void* k;
+  void* v;
+  int num_pages, page_shift;  // page_size = 1 << page_shift
+  int kv_heads, batch;
+  const int* table;
+  int table_width, table_stride;
+  const int* seq_lens;
+  int* status;
+};
+
+__device__ __forceinline__ void paged_flag(const PagedArgs& a, int bits) {
+  if (a.status) atomicOr(a.status, bits);
+}
+
+// Length of sequence b, cut to what its table row can name.
+__device__ __forceinline__ int paged_len(const PagedArgs& a, int b) {
+  return min(max(a.seq_lens[b], 0), a.table_width << a.page_shift);
+}
+
+// Page of position p (inside the table), or -1.
+__device__ __forceinline__ int paged_page(const PagedArgs& a, int b, int p) {
+  const int page = a.table[(long long)b * a.table_stride + (p >> a.page_shift)];
+  return (unsigned)page < (unsigned)a.num_pages ? page : -1;
+}
+
+// Sequence of row r: the b with q_starts[b] <= r < q_starts[b + 1], or -1 (padding rows).
+// Every lane of a warp calls it with the same r; 32 entries are compared per round trip.
+__device__ __forceinline__ int paged_find_seq(const int* q_starts, int batch, int r) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = batch;  // entries [lo, hi] bracket the answer: q_starts[lo] <= r
+  if (r < q_starts[0] || r >= q_starts[batch]) return -1;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) >> 5;
+    const int i = min(lo + (lane + 1) * step, hi);
+    const unsigned le = __ballot_sync(0xffffffffu, q_starts[i] <= r);
+    const int n = __popc(le);  // ascending entries: the lanes at or below r are a prefix
+    const int nlo = lo + n * step;
+    hi = min(nlo + step, hi);
+    lo = min(nlo, hi - 1);
+  }
+  return lo;
+}
+
+// Four consecutive elements as f32, and back with one rounding.
+template <typename T>
+__device__ __forceinline__ float4 load4(const void* base, long long e);
+template <>
+__device__ __forceinline__ float4 load4<float>(const void* base, long long e) {
+  return *reinterpret_cast<const float4*>(static_cast<const float*>(base) + e);
+}
+template <>
+__device__ __forceinline__ float4 load4<__half>(const void* base, long long e) {
+  const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __half*>(base) + e);
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+template <>
+__device__ __forceinline__ float4 load4<__nv_bfloat16>(const void* base, long long e) {
+  const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(base) + e);
+  return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                     __uint_as_float(u.y & 0xffff0000u));
+}
+
+__device__ __forceinline__ void store4(void* base, long long e, int dtype, float4 x) {
+  if (dtype == QD_KV_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(base) + e) = x;
+  } else if (dtype == QD_KV_F16) {
+    const __half2 a = __floats2half2_rn(x.x, x.y), b = __floats2half2_rn(x.z, x.w);
+    *reinterpret_cast<uint2*>(static_cast<__half*>(base) + e) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  } else {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(base) + e) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  }
+}
+
+// ---- head RMSNorm + rotation + append ------------------------------------------------
+struct AppendArgs {
+  PagedArgs kv;
+  int kv_dtype;
+  const void* qkv;
+  long long qkv_stride;
+  int rows;
+  const int* q_starts;
+  int q_heads;
+  const float* q_norm;
+  const float* k_norm;
+  float eps;
+  const float* cos_t;
+  const float* sin_t;
+  long long rope_len, rope_stride;
+  void* q_out;
+  int q_out_dtype;
+  long long q_out_stride;
+};
+
+// One warp per row and kAppendHeads consecutive heads of its [q | k | v]; lane l holds dims
+// 4l .. 4l+3, so the rotation's partner dims are 16 lanes away. The heads' loads are issued
+// first; the row's sequence and position are looked up under them.
+constexpr int kAppendHeads = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(256) k_paged_append(const __grid_constant__ AppendArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int heads = a.q_heads + 2 * a.kv.kv_heads;
+  const int per_row = (heads + kAppendHeads - 1) / kAppendHeads;
+  const long long w = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int r = (int)(w / per_row), h0 = (int)(w % per_row) * kAppendHeads;
+  if (r >= a.rows) return;
+  pdl_wait();
+  float4 x[kAppendHeads];
+#pragma unroll
+  for (int i = 0; i < kAppendHeads; ++i) {
+    const int h = min(h0 + i, heads - 1);
+    x[i] = load4<T>(a.qkv, r * a.qkv_stride + (long long)h * kHeadDim + 4 * lane);
+  }
+  int b = r, back = 1;
+  if (a.q_starts) {
+    b = paged_find_seq(a.q_starts, a.kv.batch, r);
+    if (b < 0) return;
+    back = a.q_starts[b + 1] - r;
+  }
+  const int p = a.kv.seq_lens[b] - back;
+  const long long t = (long long)p * a.rope_stride + 4 * (lane & 15);
+  const bool turned = a.cos_t != nullptr;
+  const bool live = p >= 0 && p < (a.kv.table_width << a.kv.page_shift) &&
+                    (!turned || (long long)p * a.rope_stride + kHeadDim / 2 <= a.rope_len);
+  if (!live) {
+    if (lane == 0) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
+    return;
+  }
+  float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (turned) {
+    c = *reinterpret_cast<const float4*>(a.cos_t + t);
+    s = *reinterpret_cast<const float4*>(a.sin_t + t);
+    if (lane < 16) s = make_float4(-s.x, -s.y, -s.z, -s.w);
+  }
+  int page = -1;
+  if (h0 + kAppendHeads > a.q_heads) {
+    page = paged_page(a.kv, b, p);
+    if (page < 0 && lane == 0) paged_flag(a.kv, QD_PAGED_BAD_PAGE);
+  }
+  const int ps = 1 << a.kv.page_shift;
+#pragma unroll
+  for (int i = 0; i < kAppendHeads; ++i) {
+    const int h = h0 + i;
+    if (h >= heads) break;
+    float4 y = x[i];
+    const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + a.kv.kv_heads;
+    if (!is_v) {
+      const float* wn = is_q ? a.q_norm : a.k_norm;
+      if (wn) {
+        const float ss = warp_sum(y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w);
+        const float f = rsqrtf(ss * (1.0f / kHeadDim) + a.eps);
+        const float4 n = *reinterpret_cast<const float4*>(wn + 4 * lane);
+        y = make_float4(y.x * f * n.x, y.y * f * n.y, y.z * f * n.z, y.w * f * n.w);
+      }
+      if (turned) {
+        const float4 o = make_float4(__shfl_xor_sync(0xffffffffu, y.x, 16), __shfl_xor_sync(0xffffffffu, y.y, 16),
+                                     __shfl_xor_sync(0xffffffffu, y.z, 16), __shfl_xor_sync(0xffffffffu, y.w, 16));
+        y = make_float4(y.x * c.x + o.x * s.x, y.y * c.y + o.y * s.y, y.z * c.z + o.z * s.z, y.w * c.w + o.w * s.w);
+      }
+    }
+    if (is_q) {
+      store4(a.q_out, r * a.q_out_stride + (long long)h * kHeadDim + 4 * lane, a.q_out_dtype, y);
+    } else if (page >= 0) {
+      const int g = h - a.q_heads - (is_v ? a.kv.kv_heads : 0);
+      const long long row = (((long long)page * a.kv.kv_heads + g) << a.kv.page_shift) + (p & (ps - 1));
+      store4(is_v ? a.kv.v : a.kv.k, row * kHeadDim + 4 * lane, a.kv_dtype, y);
+    }
+  }
+}
+
+// ---- attention of new tokens -----------------------------------------------------------
+struct PAttnArgs {
+  PagedArgs kv;
+  const void* q;
+  long long q_stride;
+  int rows;
+  const int* q_starts;
+  int q_heads;
+  int window, sinks;
+  float scale;
+  void* y;
+  int dtype;  // of q and y
+  long long y_stride;
+};
+
+// The plainest form: one CTA per (row, query head), four warps stepping over the visible keys
+// with a running maximum and sum each, joined at the end.
+template <typename TQ, typename TKV>
+__global__ void __launch_bounds__(128) k_paged_attn_rows(const __grid_constant__ PAttnArgs a) {
+  const int r = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = h / (a.q_heads / a.kv.kv_heads);
+  pdl_wait();
+  int b = r, back = 1;
+  if (a.q_starts) {
+    b = paged_find_seq(a.q_starts, a.kv.batch, r);
+    if (b < 0) return;
+    back = a.q_starts[b + 1] - r;
+  }
+  const int len = paged_len(a.kv, b);
+  const int asked = a.kv.seq_lens[b];
+  if (len < asked && lane == 0) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
+  const int p = asked - back;
+  const int end = min(p + 1, len);  // keys [0, end), minus what the window hides
+  const int lo = a.window > 0 ? max(0, p + 1 - a.window) : 0;
+  const int ns = min(min(a.sinks, lo), end);
+  float4 q = load4<TQ>(a.q, r * a.q_stride + (long long)h * kHeadDim + 4 * lane);
+  float m = -INFINITY, l = 0.0f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int n = ns + max(0, end - lo);
+  for (int i = warp; i < n; i += 4) {
+    const int j = i < ns ? i : lo + i - ns;
+    const int page = paged_page(a.kv, b, j);
+    if (page < 0) {
+      if (lane == 0) paged_flag(a.kv, QD_PAGED_BAD_PAGE);
+      continue;
+    }
+    const long long row = (((long long)page * a.kv.kv_heads + g) << a.kv.page_shift) + (j & ((1 << a.kv.page_shift) - 1));
+    const float4 k = load4<TKV>(a.kv.k, row * kHeadDim + 4 * lane);
+    const float4 v = load4<TKV>(a.kv.v, row * kHeadDim + 4 * lane);
+    const float s = warp_sum(q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w) * a.scale;
+    const float mn = fmaxf(m, s), f = m == -INFINITY ? 0.0f : expf(m - mn), w = mn == -INFINITY ? 0.0f : expf(s - mn);
+    l = l * f + w;
+    o = make_float4(o.x * f + w * v.x, o.y * f + w * v.y, o.z * f + w * v.z, o.w * f + w * v.w);
+    m = mn;
+  }
+  __shared__ float sm[4], sl[4];
+  __shared__ float4 so[4][32];
+  if (lane == 0) {
+    sm[warp] = m;
+    sl[warp] = l;
+  }
+  so[warp][lane] = o;
+  __syncthreads();
+  if (warp) return;
+  const float M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  float L = 0.0f;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < 4; ++i) {
+    const float f = sm[i] == -INFINITY ? 0.0f : expf(sm[i] - M);
+    const float4 t = so[i][lane];
+    L += sl[i] * f;
+    y = make_float4(y.x + t.x * f, y.y + t.y * f, y.z + t.z * f, y.w + t.w * f);
+  }
+  const float z = L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L);  // nothing seen: zeros
+  store4(a.y, r * a.y_stride + (long long)h * kHeadDim + 4 * lane, a.dtype,
+         make_float4(y.x * z, y.y * z, y.z * z, y.w * z));
+}
+
+}  // namespace qd

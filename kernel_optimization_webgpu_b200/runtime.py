@@ -589,6 +589,215 @@ def gqa_decode(q, k_cache, v_cache, seq_len: int, q_heads: int, kv_heads: int, y
     return y
 
 
+# ---- paged key-value cache and batched sampling (torch CUDA tensors) --------------------
+
+def _dtype_code(t, what: str) -> int:
+    import torch
+    code = {torch.float16: QD_KV_F16, torch.float32: QD_KV_F32, torch.bfloat16: _lib.QD_KV_BF16}.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what} must be float16, bfloat16 or float32, not {t.dtype}")
+    return code
+
+
+def _vector(t, n: Optional[int], dtype, device, what: str):
+    """Pointer of a contiguous 1-D tensor of n entries (None: NULL)."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.device != device or t.dim() != 1 or (n is not None and t.shape[0] != n) \
+            or (t.shape[0] > 1 and t.stride(0) != 1):
+        raise ValueError(f"{what} must be a contiguous {dtype} vector of {n if n is not None else 'n'} entries on {device}")
+    return t.data_ptr()
+
+
+def _rows(t, width: int, device, what: str) -> int:
+    """Row stride (elements) of a [rows, ...] tensor whose rows are `width` contiguous elements."""
+    if t.device != device:
+        raise ValueError(f"{what} must be on {device}")
+    inner = 1
+    for i in range(t.dim() - 1, 0, -1):
+        if t.shape[i] != 1 and t.stride(i) != inner:
+            raise ValueError(f"the rows of {what} must be contiguous")
+        inner *= t.shape[i]
+    if t.dim() < 1 or inner != width:
+        raise ValueError(f"{what} must have rows of {width} elements")
+    return t.stride(0) if t.shape[0] > 1 else width
+
+
+class _Launch:
+    """Makes a tensor's device and the given stream current, so that what the call allocates
+    belongs to the stream that uses it; gives the stream's handle."""
+
+    def __init__(self, device, stream):
+        import torch
+        if device.type != "cuda":
+            raise ValueError("tensors must be on a CUDA device")
+        if stream is not None and stream.device != device:
+            raise ValueError(f"the stream belongs to {stream.device}, the tensors to {device}")
+        self._with = None
+        if stream is not None:
+            self._with = torch.cuda.stream(stream)
+        elif device.index != torch.cuda.current_device():
+            self._with = torch.cuda.device(device)
+        self.handle = (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream
+
+    def __enter__(self):
+        if self._with is not None:
+            self._with.__enter__()
+        return self.handle
+
+    def __exit__(self, *exc):
+        if self._with is not None:
+            self._with.__exit__(*exc)
+
+
+def _paged_kv(k_pages, v_pages, block_table, seq_lens, status) -> "_lib.QdPagedKv":
+    import torch
+    dev = k_pages.device
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or not k_pages.is_contiguous() \
+            or not v_pages.is_contiguous() or v_pages.dtype != k_pages.dtype or v_pages.device != dev:
+        raise ValueError("k_pages and v_pages must be contiguous [pages][kv_heads][page_size][128] of one type and device")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.device != dev \
+            or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError("block_table must be int32 [batch][pages], its rows contiguous, beside the cache")
+    batch, width = block_table.shape
+    stride = block_table.stride(0) if batch > 1 else width
+    lens = _vector(seq_lens, batch, torch.int32, dev, "seq_lens")
+    pages, kv_heads, page_size, head_dim = k_pages.shape
+    return _lib.QdPagedKv(k_pages.data_ptr(), v_pages.data_ptr(), _dtype_code(k_pages, "the cache"), pages, page_size,
+                          kv_heads, head_dim, batch, block_table.data_ptr(), width, stride, lens,
+                          _vector(status, 1, torch.int32, dev, "status"))
+
+
+def paged_append(qkv, k_pages, v_pages, block_table, seq_lens, cos, sin, q_heads: int, q_norm=None, k_norm=None,
+                 eps: float = 1e-6, q_starts=None, q_out=None, rope_stride: Optional[int] = None, status=None,
+                 stream=None):
+    """Head RMSNorm + rotation of the new tokens' q and k, and their K/V rows into the pages
+    (qd_paged_append). qkv [rows][(q_heads + 2 kv_heads) * 128]; cache pools
+    [pages][kv_heads][page_size][128]; cos, sin f32 tables whose row for a position is
+    rope_stride elements after the previous one's (default: their own row stride; None, None:
+    no rotation); returns q [rows][q_heads * 128] (q_out, or a new tensor of qkv's type)."""
+    import torch
+    dev = qkv.device
+    kv = _paged_kv(k_pages, v_pages, block_table, seq_lens, status)
+    heads = q_heads + 2 * kv.kv_heads
+    stride, rows = _rows(qkv, heads * 128, dev, "qkv"), qkv.shape[0]
+    if k_pages.device != dev:
+        raise ValueError(f"the cache must be on {dev}")
+    rope_len = 0
+    for t in (cos, sin):
+        if t is not None and (t.dtype != torch.float32 or t.device != dev or not t.is_contiguous()):
+            raise ValueError(f"cos and sin must be contiguous float32 tables on {dev}")
+    if cos is not None and sin is not None:
+        rope_len = min(cos.numel(), sin.numel())
+        if rope_stride is None:
+            rope_stride = cos.stride(0) if cos.dim() > 1 else 64
+    with _Launch(dev, stream) as s:
+        if q_out is None:
+            q_out = torch.empty((rows, q_heads * 128), dtype=qkv.dtype, device=dev)
+        elif q_out.shape[0] != rows:
+            raise ValueError(f"q_out must have {rows} rows")
+        check(_lib.load().qd_paged_append(
+            kv, qkv.data_ptr(), _dtype_code(qkv, "qkv"), stride, rows,
+            _vector(q_starts, kv.batch + 1, torch.int32, dev, "q_starts"), q_heads,
+            _vector(q_norm, 128, torch.float32, dev, "q_norm"), _vector(k_norm, 128, torch.float32, dev, "k_norm"), eps,
+            None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(), rope_len,
+            rope_stride or 0, q_out.data_ptr(), _dtype_code(q_out, "q_out"),
+            _rows(q_out, q_heads * 128, dev, "q_out"), s))
+    return q_out
+
+
+def _attn_args(q, k_pages, v_pages, block_table, seq_lens, status):
+    kv = _paged_kv(k_pages, v_pages, block_table, seq_lens, status)
+    if k_pages.device != q.device:
+        raise ValueError(f"the cache must be on {q.device}")
+    width = 1
+    for n in q.shape[1:]:
+        width *= n
+    if q.dim() < 2 or width % 128:
+        raise ValueError("q must be [rows][q_heads][128] or [rows][q_heads * 128]")
+    return kv, width // 128, _rows(q, width, q.device, "q")
+
+
+def _attn_out(q, y):
+    import torch
+    if y is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if y.dtype != q.dtype or y.shape != q.shape:
+        raise ValueError("y must have q's type and shape")
+    return y
+
+
+def paged_attn_decode(q, k_pages, v_pages, block_table, seq_lens, window: int = 0, sinks: int = 0, scale: float = 0.0,
+                      y=None, workspace=None, status=None, stream=None):
+    """Attention of one new token per sequence over its pages (qd_paged_attn_decode): q
+    [batch][q_heads][128], the token at position seq_lens[b] - 1; window > 0: the last
+    `window` positions and the first `sinks`. workspace: a uint8 tensor of
+    paged_attn_decode_workspace bytes that no other stream uses meanwhile (default: a new one)."""
+    import torch
+    kv, heads, stride = _attn_args(q, k_pages, v_pages, block_table, seq_lens, status)
+    if q.shape[0] != kv.batch:
+        raise ValueError(f"q must have one row per sequence ({kv.batch})")
+    L = _lib.load()
+    with _Launch(q.device, stream) as s:
+        y = _attn_out(q, y)
+        n = L.qd_paged_attn_decode_workspace_bytes(kv.batch, heads)
+        ws = _workspace(workspace, n, q.device)
+        check(L.qd_paged_attn_decode(kv, q.data_ptr(), _dtype_code(q, "q"), stride, heads, window, sinks, scale,
+                                     y.data_ptr(), _rows(y, heads * 128, q.device, "y"), ws.data_ptr(), s))
+    return y
+
+
+def paged_attn_prompt(q, k_pages, v_pages, block_table, seq_lens, q_starts, window: int = 0, sinks: int = 0,
+                      scale: float = 0.0, y=None, workspace=None, status=None, stream=None):
+    """Causal attention of a ragged batch of new tokens over their pages (qd_paged_attn_prompt):
+    q [rows][q_heads][128], rows q_starts[b] .. q_starts[b + 1] - 1 being sequence b's newest
+    tokens (already appended). Rows from q_starts[batch] on are padding; y keeps what it held
+    there."""
+    import torch
+    kv, heads, stride = _attn_args(q, k_pages, v_pages, block_table, seq_lens, status)
+    L = _lib.load()
+    with _Launch(q.device, stream) as s:
+        y = _attn_out(q, y)
+        n = L.qd_paged_attn_prompt_workspace_bytes(kv.batch, q.shape[0], heads, kv.kv_heads)
+        ws = _workspace(workspace, n, q.device)
+        check(L.qd_paged_attn_prompt(kv, q.data_ptr(), _dtype_code(q, "q"), stride, q.shape[0],
+                                     _vector(q_starts, kv.batch + 1, torch.int32, q.device, "q_starts"), heads, window,
+                                     sinks, scale, y.data_ptr(), _rows(y, heads * 128, q.device, "y"), ws.data_ptr(), s))
+    return y
+
+
+def _workspace(given, n: int, device):
+    import torch
+    if given is None:
+        return torch.empty(n, dtype=torch.uint8, device=device)
+    if given.device != device or given.numel() * given.element_size() < n or not given.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous tensor of at least {n} bytes on {device}")
+    return given
+
+
+def sample_rows(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, ids=None, logprobs=None, stream=None):
+    """One token per row of logits [rows][vocab] (f32, f16 or bf16) from the given random
+    numbers u [rows] f32 in [0, 1), with per-row settings (f32 vectors; top_k int32; None: not
+    applied) as qd_sample_rows defines them. Returns (ids int32, logprobs f32)."""
+    import torch
+    if logits.dim() != 2:
+        raise ValueError("logits must be [rows][vocab]")
+    rows, vocab = logits.shape
+    dev = logits.device
+    stride = _rows(logits, vocab, dev, "logits")
+    f = [_vector(t, rows, torch.float32, dev, n) for t, n in
+         ((temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p"), (u, "u"))]
+    with _Launch(dev, stream) as s:
+        ids = torch.empty(rows, dtype=torch.int32, device=dev) if ids is None else ids
+        logprobs = torch.empty(rows, dtype=torch.float32, device=dev) if logprobs is None else logprobs
+        check(_lib.load().qd_sample_rows(logits.data_ptr(), _dtype_code(logits, "logits"), rows, vocab, stride, f[0],
+                                         _vector(top_k, rows, torch.int32, dev, "top_k"), f[1], f[2], f[3],
+                                         _vector(ids, rows, torch.int32, dev, "ids"),
+                                         _vector(logprobs, rows, torch.float32, dev, "logprobs"), s))
+    return ids, logprobs
+
+
 __all__ = ["Engine", "QdError", "createWebGpuContext", "runCustomQwenGreedyPrompt", "runKernelBenchmarks",
            "runFullDecoderStackBenchmark", "qwen_profile",
-           "qwenProfile", "q4_matvec", "lm_head_argmax", "gqa_decode", "LmHeadWorkspace"]
+           "qwenProfile", "q4_matvec", "lm_head_argmax", "gqa_decode", "LmHeadWorkspace",
+           "paged_append", "paged_attn_decode", "paged_attn_prompt", "sample_rows"]

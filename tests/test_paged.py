@@ -1,0 +1,521 @@
+"""The paged key-value cache operators (qd_paged_append, qd_paged_attn_decode,
+qd_paged_attn_prompt): refusals on the host (no GPU), and the CUDA path against plain
+64-bit evaluations at the sizes, masks and layouts where it can go wrong.
+
+Tolerances count roundings, relative to A = sum of |weight| |value| of an output:
+ - a score is a sum of 128 products: its error is at most S e_s, S = scale * sum |q| |k|,
+   e_s = 2^-19 for the f32 accumulation (8 steps of 16 products, one truncation of 2^-23
+   each, two operand parts) plus the operands' split (2^-21 for f32 as two f16, 2^-16 as two
+   bf16, 0 where q is 16-bit);
+ - a weight exp(s - m) is then off by 2 S e_s (score and maximum), plus 2^-20 for the
+   exponential and its rounded argument, plus its own rounding where it feeds a product in 16
+   bits (half a step: 2^-11, 2^-8) or as a sum of two parts (2^-21, 2^-16);
+ - sums over n keys in f32, in steps of 16 keys or fewer joins: n / 16 * 2^-23 + 2^-19;
+ - the output's own rounding, half a step of its type."""
+import ctypes as C
+import math
+
+import pytest
+
+from kernel_optimization_webgpu_b200 import _lib
+
+D = 128
+HALF_STEP = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+
+
+# ---- refusals (no GPU) -----------------------------------------------------------------
+
+def _kv(**kw):
+    d = dict(k=4096, v=8192, dtype=_lib.QD_KV_F16, num_pages=4, page_size=16, kv_heads=2, head_dim=128, batch=2,
+             block_table=4096, table_width=3, table_stride=3, seq_lens=4096, status=None)
+    d.update(kw)
+    return _lib.QdPagedKv(*(d[n] for n, _ in _lib.QdPagedKv._fields_))
+
+
+BAD_CACHES = [dict(dtype=_lib.QD_KV_F32), dict(dtype=7), dict(page_size=24), dict(page_size=8), dict(page_size=512),
+              dict(head_dim=64), dict(kv_heads=0), dict(batch=-1), dict(batch=4097), dict(num_pages=-1),
+              dict(table_stride=2), dict(table_width=-1, table_stride=0), dict(block_table=None), dict(seq_lens=None),
+              dict(k=None), dict(v=8200), dict(table_width=1 << 27, table_stride=1 << 27)]
+
+
+@pytest.mark.parametrize("bad", BAD_CACHES, ids=lambda d: ",".join(f"{k}={v}" for k, v in d.items()))
+def test_a_bad_cache_is_refused_by_every_entry(bad):
+    L = _lib.load()
+    kv = _kv(**bad)
+    assert L.qd_paged_append(kv, 4096, 1, 768, 2, None, 2, None, None, 1e-6, None, None, 0, 0, 4096, 1, 256,
+                             None) == _lib.QD_E_INVALID
+    assert L.qd_paged_attn_decode(kv, 4096, 1, 256, 2, 0, 0, 0.0, 4096, 256, 4096, None) == _lib.QD_E_INVALID
+    assert L.qd_paged_attn_prompt(kv, 4096, 1, 256, 2, 4096, 2, 0, 0, 0.0, 4096, 256, 4096, None) == _lib.QD_E_INVALID
+    assert L.qd_last_error(None).startswith(b"paged cache")
+
+
+def test_attention_arguments_are_refused():
+    L = _lib.load()
+    ok = dict(q=4096, dtype=1, stride=256, heads=2, window=0, sinks=0, scale=0.0, y=8192, y_stride=256, ws=4096)
+    bads = [dict(q=None), dict(y=None), dict(ws=None), dict(q=4104), dict(dtype=2), dict(dtype=9), dict(stride=248),
+            dict(stride=260), dict(y_stride=128), dict(heads=3), dict(heads=0), dict(heads=130), dict(window=-1),
+            dict(sinks=-1), dict(scale=math.inf), dict(scale=math.nan)]
+    for bad in bads:
+        c = {**ok, **bad}
+        if bad.get("heads") == 130:
+            c.update(stride=130 * 128, y_stride=130 * 128)
+        rc = L.qd_paged_attn_decode(_kv(), c["q"], c["dtype"], c["stride"], c["heads"], c["window"], c["sinks"],
+                                    c["scale"], c["y"], c["y_stride"], c["ws"], None)
+        assert rc == _lib.QD_E_INVALID, bad
+        rc = L.qd_paged_attn_prompt(_kv(), c["q"], c["dtype"], c["stride"], 5, 4096, c["heads"], c["window"], c["sinks"],
+                                    c["scale"], c["y"], c["y_stride"], c["ws"], None)
+        assert rc == _lib.QD_E_INVALID, bad
+    assert L.qd_paged_attn_decode(None, 4096, 1, 256, 2, 0, 0, 0.0, 4096, 256, 4096, None) == _lib.QD_E_INVALID
+    assert L.qd_paged_attn_prompt(_kv(), 4096, 1, 256, 5, None, 2, 0, 0, 0.0, 4096, 256, 4096,
+                                  None) == _lib.QD_E_INVALID
+    assert L.qd_paged_attn_prompt(_kv(), 4096, 1, 256, -1, 4096, 2, 0, 0, 0.0, 4096, 256, 4096,
+                                  None) == _lib.QD_E_INVALID
+    # nothing to do is not an error, and touches nothing
+    assert L.qd_paged_attn_prompt(_kv(), None, 1, 256, 0, None, 2, 0, 0, 0.0, None, 256, None, None) == _lib.QD_OK
+    assert L.qd_paged_attn_decode(_kv(batch=0), None, 1, 256, 2, 0, 0, 0.0, None, 256, None, None) == _lib.QD_OK
+
+
+def test_append_arguments_are_refused():
+    L = _lib.load()
+    ok = dict(qkv=4096, dtype=1, stride=768, rows=2, starts=None, heads=2, qn=None, kn=None, eps=1e-6, cos=4096, sin=4096,
+              rope_len=640, rope_stride=64, out=4096, out_dtype=1, out_stride=256)
+    bads = [dict(qkv=None), dict(out=None), dict(qkv=4100), dict(out=4104), dict(dtype=3), dict(out_dtype=-1),
+            dict(stride=760), dict(stride=770), dict(rows=-1), dict(rows=3), dict(heads=-1), dict(eps=-1.0),
+            dict(eps=math.nan), dict(sin=None), dict(cos=None), dict(rope_stride=2), dict(rope_stride=-64),
+            dict(rope_len=-1), dict(out_stride=128), dict(qn=4100), dict(kn=4100), dict(cos=4100)]
+    for bad in bads:
+        c = {**ok, **bad}
+        rc = L.qd_paged_append(_kv(), c["qkv"], c["dtype"], c["stride"], c["rows"], c["starts"], c["heads"], c["qn"],
+                               c["kn"], c["eps"], c["cos"], c["sin"], c["rope_len"], c["rope_stride"], c["out"],
+                               c["out_dtype"], c["out_stride"], None)
+        assert rc == _lib.QD_E_INVALID, bad
+    assert L.qd_paged_append(_kv(), None, 1, 768, 0, 4096, 2, None, None, 1e-6, None, None, 0, 0, None, 1, 256,
+                             None) == _lib.QD_OK
+
+
+def test_python_wrappers_refuse_before_they_enqueue():
+    torch = pytest.importorskip("torch")
+    from kernel_optimization_webgpu_b200 import runtime as R
+    k = torch.zeros(4, 2, 16, D, dtype=torch.float16)
+    table, lens = torch.zeros(2, 3, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    q = torch.zeros(2, 2, D)
+    for args in ((q, k, k[:3], table, lens), (q, k, k.bfloat16(), table, lens), (q, k.transpose(1, 2), k, table, lens),
+                 (q, k, k, table.long(), lens), (q, k, k, table, lens.long()), (q, k, k, table, lens[:1]),
+                 (q[:1], k, k, table, lens), (q[..., :64], k, k, table, lens), (q.transpose(0, 1), k, k, table, lens),
+                 (q.double(), k, k, table, lens), (q, k, k, table, lens)):   # the last: not CUDA tensors
+        with pytest.raises(ValueError):
+            R.paged_attn_decode(*args)
+    with pytest.raises(ValueError):
+        R.paged_append(torch.zeros(2, 700), k, k, table, lens, None, None, 2)
+
+
+# ---- the plain 64-bit forms -------------------------------------------------------------
+
+def _cuda():
+    torch = pytest.importorskip("torch")
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return torch
+
+
+def _types(torch):
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def make_cache(torch, totals, page, kv_heads, cache, seed=0, slack=0, fill=None, width=None):
+    """Pools of random rows, every page owned by one sequence or by none; a shuffled table.
+    fill: what every row that no sequence holds contains (NaN, for instance)."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    per = [-(-n // page) for n in totals]
+    pages = sum(per) + 2 + slack
+    order = torch.randperm(pages, generator=g, device="cuda").tolist()
+    width = width or max(per + [1])
+    table = torch.full((len(totals), width), -1, dtype=torch.int32)
+    T = _types(torch)[cache]
+    k, v = (torch.randn(pages, kv_heads, page, D, generator=g, device="cuda").to(T) for _ in "kv")
+    if fill is not None:
+        keep_k, keep_v = k.clone(), v.clone()
+        k.fill_(fill), v.fill_(fill)
+    at = 0
+    for b, n in enumerate(per):
+        for i in range(n):
+            pg = order[at]
+            at += 1
+            table[b, i] = pg
+            if fill is not None:
+                m = min(page, totals[b] - i * page)
+                k[pg, :, :m], v[pg, :, :m] = keep_k[pg, :, :m], keep_v[pg, :, :m]
+    return k, v, table.cuda(), torch.tensor(totals, dtype=torch.int32, device="cuda")
+
+
+def plain_attention(torch, q, k, v, table, lens, new, window, sinks, scale, io, cache):
+    """(y, tolerance) in 64 bits; new[b]: sequence b's new tokens (rows in order)."""
+    page, kvh = k.shape[2], k.shape[1]
+    H = q.shape[1]
+    ys, tols, first = [], [], 0
+    split = 0.0 if io != "f32" else (2.0 ** -21 if cache == "f16" else 2.0 ** -16)
+    weight = HALF_STEP[cache] if io != "f32" else split
+    for b, n in enumerate(new):
+        t = int(lens[b])
+        qs = q[first:first + n].double()
+        first += n
+        j = torch.arange(max(t, 1), device="cuda")[:max(t, 0)]
+        pg = table[b].long()[j // page]
+        p = torch.arange(t - n, t, device="cuda")[:, None]
+        seen = (j[None] <= p) & ((window == 0) | (j[None] > p - window) | (j[None] < sinks))
+        seen_any = seen.any(0)
+        pg = torch.where(seen_any, pg, torch.zeros_like(pg)) if t > 0 else pg
+        kk = torch.where(seen_any[:, None, None], k[pg, :, j % page].double(), 0.0).repeat_interleave(H // kvh, 1)
+        vv = torch.where(seen_any[:, None, None], v[pg, :, j % page].double(), 0.0).repeat_interleave(H // kvh, 1)
+        s = torch.einsum("nhd,jhd->nhj", qs, kk) * scale
+        size = torch.where(seen[:, None], torch.einsum("nhd,jhd->nhj", qs.abs(), kk.abs()) * abs(scale), 0.0)
+        s = s.masked_fill(~seen[:, None], -math.inf)
+        w = torch.exp(s - s.amax(-1, keepdim=True).clamp_min(-1e300)) if t > 0 else s
+        w = torch.where(seen[:, None], w, 0.0)
+        w = w / w.sum(-1, keepdim=True).clamp_min(1e-300)
+        y = torch.einsum("nhj,jhd->nhd", w, vv)
+        A = torch.einsum("nhj,jhd->nhd", w, vv.abs())
+        S = size.amax(-1)[..., None] if t > 0 else torch.zeros_like(y[..., :1])
+        eps = 2 * S * (2.0 ** -19 + split) + 2.0 ** -20 + weight + max(t, 0) / 16 * 2.0 ** -23 + 2.0 ** -19
+        ys.append(y)
+        tols.append(2 * A * eps + HALF_STEP[io] * y.abs() + (2.0 ** -25 if io == "f16" else 1e-30))
+    return torch.cat(ys), torch.cat(tols)
+
+
+def close(torch, got, want, tol):
+    off = (got.double() - want).abs()
+    assert bool((off <= tol).all()), f"off by {float((off / tol).nan_to_num(math.inf).max()):.3g} tolerances"
+
+
+# ---- attention of one new token ------------------------------------------------------------
+
+LENS = [[1], [31], [64, 65, 63], [0, 1, 0, 17, 0], [2049, 5, 700, 129], [1] * 70, [4000]]
+HEADS = [(16, 8), (8, 1), (4, 4), (10, 2), (12, 4), (18, 2)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", LENS, ids=lambda v: f"{len(v)}x{max(v)}")
+@pytest.mark.parametrize("heads", HEADS, ids=lambda h: f"{h[0]}q{h[1]}kv")
+@pytest.mark.parametrize("io,cache", [("f32", "f16"), ("f16", "f16"), ("bf16", "bf16"), ("f32", "bf16")])
+def test_decode_attention(lens, heads, io, cache):
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    page = [16, 32, 64, 256][(len(lens) + heads[0]) % 4]
+    # every row that is nobody's holds NaN: recycled and unwritten pages reach no result
+    k, v, table, n = make_cache(torch, lens, page, heads[1], cache, seed=len(lens), fill=math.nan)
+    q = (torch.randn(len(lens), heads[0], D, device="cuda") * 1.5).to(_types(torch)[io])
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    y = R.paged_attn_decode(q, k, v, table, n, status=status)
+    want, tol = plain_attention(torch, q, k, v, table, n, [1] * len(lens), 0, 0, D ** -0.5, io, cache)
+    close(torch, y, want, tol)
+    assert int(status) == 0
+    assert bool((y[n == 0] == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window,sinks", [(1, 0), (16, 0), (17, 4), (100, 64), (64, 65), (1000, 1), (5000, 7), (130, 3000)])
+@pytest.mark.parametrize("page", [16, 128])
+def test_decode_window_and_sinks_with_freed_pages(window, sinks, page):
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    lens = [1500, 3, 150, 64, 1]
+    k, v, table, n = make_cache(torch, lens, page, 2, "f16", fill=math.nan)
+    for b, t in enumerate(lens):   # a server frees the pages that no later query sees
+        for i in range(table.shape[1]):
+            lo, hi = i * page, min((i + 1) * page, t)
+            if hi <= lo or (hi <= t - window and lo >= sinks):
+                table[b, i] = -5 if i % 2 else 10 ** 6
+    q = torch.randn(len(lens), 8, D, device="cuda") * 1.5
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    y = R.paged_attn_decode(q, k, v, table, n, window=window, sinks=sinks, status=status)
+    want, tol = plain_attention(torch, q, k, v, table, n, [1] * 5, window, sinks, D ** -0.5, "f32", "f16")
+    close(torch, y, want, tol)
+    assert int(status) == 0
+
+
+@pytest.mark.gpu
+def test_decode_strides_scale_workspace_and_stream():
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    lens = [300, 7, 90]
+    k, v, table, n = make_cache(torch, lens, 32, 4, "f16", width=40)
+    wide = torch.randn(3, 8 * D + 64, device="cuda")
+    q = wide[:, :8 * D].unflatten(1, (8, D))
+    out = torch.full((3, 8 * D + 8), 7.0, device="cuda")
+    y = out[:, :8 * D].unflatten(1, (8, D))
+    ws = torch.full((_lib.load().qd_paged_attn_decode_workspace_bytes(3, 8),), 255, dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    got = R.paged_attn_decode(q, k, v, table, n, scale=0.25, y=y, workspace=ws, stream=stream)
+    stream.synchronize()
+    want, tol = plain_attention(torch, q, k, v, table, n, [1] * 3, 0, 0, 0.25, "f32", "f16")
+    close(torch, got, want, tol)
+    assert got.data_ptr() == out.data_ptr() and bool((out[:, 8 * D:] == 7).all())
+    flat = R.paged_attn_decode(q.reshape(3, -1), k, v, table[:, :12], n, scale=0.25)   # rows of a wider table
+    assert torch.equal(flat.view(3, 8, D), got)
+    with pytest.raises(ValueError):
+        R.paged_attn_decode(q, k, v, table, n, workspace=ws[:16])
+
+
+@pytest.mark.gpu
+def test_decode_is_the_same_every_time_and_replays_with_new_lengths():
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    lens = [900, 33, 2500, 1]
+    k, v, table, n = make_cache(torch, lens, 16, 2, "f16")
+    q = torch.randn(4, 16, D, device="cuda")
+    first = R.paged_attn_decode(q, k, v, table, n).clone()
+    for _ in range(3):
+        assert torch.equal(R.paged_attn_decode(q, k, v, table, n), first)
+    # two graphs of the same tensors with workspaces of their own
+    ws = [torch.empty(_lib.load().qd_paged_attn_decode_workspace_bytes(4, 16), dtype=torch.uint8, device="cuda")
+          for _ in range(2)]
+    y = [torch.zeros_like(q) for _ in range(2)]
+    graphs = []
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            R.paged_attn_decode(q, k, v, table, n, y=y[i], workspace=ws[i], window=1000 * i)
+        graphs.append(graph)
+    for shorter in ([900, 33, 2500, 1], [1, 32, 1200, 0]):
+        n.copy_(torch.tensor(shorter, dtype=torch.int32))
+        for i in range(2):
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            want, tol = plain_attention(torch, q, k, v, table, n, [1] * 4, 1000 * i, 0, D ** -0.5, "f32", "f16")
+            close(torch, y[i], want, tol)
+
+
+@pytest.mark.gpu
+def test_bad_pages_and_lengths_are_left_out_and_flagged():
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    k, v, table, n = make_cache(torch, [100, 40], 16, 2, "f16")
+    q = torch.randn(2, 4, D, device="cuda")
+    table[0, 2] = k.shape[0]       # one past the pool: positions 32..47 of sequence 0 are left out
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    y = R.paged_attn_decode(q, k, v, table, n, status=status)
+    assert int(status) == _lib.QD_PAGED_BAD_PAGE
+    keep = torch.cat([torch.arange(32), torch.arange(48, 100)]).cuda()
+    pg = table[0].long()[keep // 16]
+    kk, vv = (x[pg, :, keep % 16].double().repeat_interleave(2, 1) for x in (k, v))
+    w = torch.softmax(torch.einsum("hd,jhd->hj", q[0].double(), kk) / math.sqrt(D), -1)
+    assert float((y[0].double() - torch.einsum("hj,jhd->hd", w, vv)).abs().max()) < 1e-4
+    status.zero_()
+    y = R.paged_attn_prompt(q, k, v, table, n, torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda"), status=status)
+    assert int(status) == _lib.QD_PAGED_BAD_PAGE
+    assert float((y[0].double() - torch.einsum("hj,jhd->hd", w, vv)).abs().max()) < 1e-4
+    # a length beyond the table is cut to the table
+    status.zero_()
+    table[0, 2] = table[0, 1]
+    n[0] = 10 ** 9
+    y = R.paged_attn_decode(q, k, v, table, n, status=status)
+    assert int(status) == _lib.QD_PAGED_BAD_LENGTH and bool(torch.isfinite(y).all())
+    # a negative length holds nothing
+    status.zero_()
+    n[0] = -3
+    y = R.paged_attn_decode(q, k, v, table, n, status=status)
+    assert bool((y[0] == 0).all())
+
+
+# ---- attention of prompt chunks ------------------------------------------------------------
+
+CHUNKS = [([8], [8]), ([1], [1]), ([130], [130]), ([1, 0, 70, 5], [900, 40, 70, 6]), ([300, 17], [513, 1100]),
+          ([33] * 9, [33 + 40 * i for i in range(9)]), ([700], [1000]), ([0, 3, 0], [0, 3, 9])]
+
+
+def run_prompt(torch, new, totals, heads, page, io, cache, window, sinks, pad=3, fill=math.nan):
+    from kernel_optimization_webgpu_b200 import runtime as R
+    k, v, table, n = make_cache(torch, totals, page, heads[1], cache, seed=sum(new), fill=fill)
+    starts = torch.tensor([sum(new[:b]) for b in range(len(new) + 1)], dtype=torch.int32, device="cuda")
+    rows = sum(new) + pad
+    q = (torch.randn(rows, heads[0], D, device="cuda") * 1.5).to(_types(torch)[io])
+    q[sum(new):] = math.nan
+    y = torch.full_like(q, 5.0)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = R.paged_attn_prompt(q, k, v, table, n, starts, window=window, sinks=sinks, y=y, status=status)
+    assert bool((got[sum(new):] == 5.0).all()), "padding rows were written"
+    assert int(status) == 0
+    want, tol = plain_attention(torch, q, k, v, table, n, new, window, sinks, D ** -0.5, io, cache)
+    close(torch, got[:sum(new)], want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("chunk", CHUNKS, ids=lambda c: f"{len(c[0])}x{max(c[0])}of{max(c[1])}")
+@pytest.mark.parametrize("heads", HEADS, ids=lambda h: f"{h[0]}q{h[1]}kv")
+@pytest.mark.parametrize("io,cache", [("f32", "f16"), ("f16", "f16"), ("bf16", "bf16"), ("f32", "bf16")])
+def test_prompt_attention(chunk, heads, io, cache):
+    torch = _cuda()
+    run_prompt(torch, *chunk, heads, [16, 64, 128, 256][(len(chunk[0]) + heads[0]) % 4], io, cache, 0, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window,sinks", [(1, 0), (40, 0), (128, 4), (129, 130), (300, 1), (64, 700), (5000, 4)])
+@pytest.mark.parametrize("io,cache", [("f32", "f16"), ("bf16", "bf16")])
+def test_prompt_window_and_sinks(window, sinks, io, cache):
+    torch = _cuda()
+    run_prompt(torch, [400, 1, 70], [900, 300, 70], (8, 2), 16, io, cache, window, sinks)
+
+
+@pytest.mark.gpu
+def test_prompt_equals_decode_for_single_tokens():
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    lens = [70, 1, 515, 128]
+    k, v, table, n = make_cache(torch, lens, 32, 8, "f16")
+    q = torch.randn(4, 16, D, device="cuda")
+    starts = torch.arange(5, dtype=torch.int32, device="cuda")
+    a, b = R.paged_attn_prompt(q, k, v, table, n, starts), R.paged_attn_decode(q, k, v, table, n)
+    _, tol = plain_attention(torch, q, k, v, table, n, [1] * 4, 0, 0, D ** -0.5, "f32", "f16")
+    close(torch, a, b.double(), 2 * tol)
+
+
+@pytest.mark.gpu
+def test_a_causal_future_of_large_values_does_not_reach_the_past():
+    """Rows before a token see nothing of its K and V, however large these are."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    new = [150]
+    k, v, table, n = make_cache(torch, new, 16, 1, "f16")
+    starts = torch.tensor([0, 150], dtype=torch.int32, device="cuda")
+    q = torch.randn(150, 2, D, device="cuda").half()
+    before = R.paged_attn_prompt(q, k, v, table, n, starts).clone()
+    pg = table[0].long()
+    for p in range(140, 150):
+        k[pg[p // 16], :, p % 16] = 60000.0
+        v[pg[p // 16], :, p % 16] = -60000.0
+    after = R.paged_attn_prompt(q, k, v, table, n, starts)
+    assert torch.equal(before[:140], after[:140]) and bool(torch.isfinite(after).all())
+
+
+# ---- norm + rotation + append ----------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("io,cache,out", [("f32", "f16", "f32"), ("bf16", "bf16", "bf16"), ("f16", "f16", "f16"),
+                                          ("f32", "bf16", "bf16"), ("f32", "f16", "f16")])
+@pytest.mark.parametrize("new,totals", [([1], [9]), ([1, 1, 1], [5, 1, 700]), ([40, 0, 3, 129], [40, 7, 300, 129]),
+                                        ([1] * 200, list(range(1, 201)))], ids=["one", "three", "ragged", "many"])
+@pytest.mark.parametrize("heads", [(16, 8), (5, 1), (0, 2)], ids=lambda h: f"{h[0]}q{h[1]}kv")
+def test_append(io, cache, out, new, totals, heads):
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    T = _types(torch)
+    H, kvh = heads
+    k, v, table, n = make_cache(torch, totals, 16, kvh, cache)
+    rows, pad = sum(new), 2
+    qkv = torch.randn(rows + pad, (H + 2 * kvh) * D + 24, device="cuda").to(T[io])[:, :(H + 2 * kvh) * D]
+    qn, kn = torch.rand(D, device="cuda") + 0.5, torch.rand(D, device="cuda") + 0.5
+    angle = torch.rand(max(totals), 64, device="cuda") * 6.28
+    cos, sin = angle.cos(), angle.sin()
+    starts = torch.tensor([sum(new[:b]) for b in range(len(new) + 1)], dtype=torch.int32, device="cuda")
+    q_out = torch.full((rows + pad, H * D), 3.0, device="cuda").to(T[out])
+    k0, v0 = k.clone(), v.clone()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    R.paged_append(qkv, k, v, table, n, cos, sin, H, q_norm=qn, k_norm=kn, q_starts=starts, q_out=q_out, status=status)
+    assert int(status) == 0 and bool((q_out[rows:] == 3).all())
+    seq = torch.repeat_interleave(torch.arange(len(new)), torch.tensor(new)).cuda()
+    pos = torch.cat([torch.arange(t - m, t) for m, t in zip(new, totals)]).cuda()
+    x = qkv[:rows].double().unflatten(1, (-1, D))
+
+    def turned(h, w):
+        h = h / (h.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.double()
+        c, s = cos.double()[pos][:, None], sin.double()[pos][:, None]
+        a, b = h[..., :64], h[..., 64:]
+        # 128 squares (at most 9 roundings, halved by the root), the root (2 steps), two
+        # products with the weight and two with the rotation: under 16 half steps of f32
+        tol = 16 * 2.0 ** -24 * torch.cat([(a * c).abs() + (b * s).abs(), (b * c).abs() + (a * s).abs()], -1)
+        return torch.cat([a * c - b * s, b * c + a * s], -1), tol
+
+    want, tol = turned(x[:, :H], qn)
+    close(torch, q_out[:rows].unflatten(1, (-1, D)) if H else q_out[:rows].view(rows, 0, D), want,
+          tol + HALF_STEP[out] * want.abs() + 2.0 ** -25)
+    pg = table[seq].long().gather(1, (pos // 16)[:, None])[:, 0]
+    want, tol = turned(x[:, H:H + kvh], kn)
+    close(torch, k[pg, :, pos % 16], want, tol + HALF_STEP[cache] * want.abs() + 2.0 ** -25)
+    assert torch.equal(v[pg, :, pos % 16], qkv[:rows].float().unflatten(1, (-1, D))[:, H + kvh:].to(T[cache]))
+    untouched = torch.ones(k.shape[0], k.shape[2], dtype=torch.bool, device="cuda")
+    untouched[pg, pos % 16] = False
+    assert torch.equal(k.transpose(1, 2)[untouched], k0.transpose(1, 2)[untouched])
+    assert torch.equal(v.transpose(1, 2)[untouched], v0.transpose(1, 2)[untouched])
+
+
+@pytest.mark.gpu
+def test_append_in_place_without_norm_or_rotation_and_wider_table_rows():
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    k, v, table, n = make_cache(torch, [3, 20], 16, 2, "f16")
+    qkv = torch.randn(2, 8 * D, device="cuda")
+    x = qkv.clone()
+    q = R.paged_append(qkv, k, v, table, n, None, None, 4, q_out=qkv[:, :4 * D])      # plain append, in place
+    assert torch.equal(q, x[:, :4 * D])
+    assert torch.equal(k[table[1, 1].long(), :, 3], x[1, 4 * D:6 * D].view(2, D).half())
+    # rows of the table 128 apart, as the reference reads it (position p at row 2p)
+    cos, sin = torch.rand(40, 64, device="cuda"), torch.rand(40, 64, device="cuda")
+    a = R.paged_append(x, k, v, table, n, cos, sin, 4, rope_stride=128)
+    b = R.paged_append(x, k, v, table, n, cos[::2].contiguous(), sin[::2].contiguous(), 4)
+    assert torch.equal(a, b)
+    q2 = R.paged_append(x, k, v, table, n, cos, sin, 4, rope_stride=128, q_out=x[:, :4 * D])
+    assert torch.equal(q2, a)
+
+
+@pytest.mark.gpu
+def test_append_flags_what_has_no_place():
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    k, v, table, n = make_cache(torch, [16, 16, 16, 16], 16, 1, "f16")
+    n.copy_(torch.tensor([17, 0, 5, 9]))       # beyond the table; a new token at position -1; fine; bad page below
+    table[3, 0] = -1
+    k0 = k.clone()
+    cos = torch.rand(4, 64, device="cuda")       # tables end before position 4
+    x = torch.randn(4, 4 * D, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    R.paged_append(x, k, v, table, n, cos, cos, 2, status=status)
+    assert int(status) == _lib.QD_PAGED_BAD_LENGTH and torch.equal(k, k0)
+    status.zero_()
+    R.paged_append(x[3:], k, v, table[3:], n[3:], None, None, 2, status=status)
+    assert int(status) == _lib.QD_PAGED_BAD_PAGE and torch.equal(k, k0)
+
+
+# ---- the step as it is used -------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache,window", [("f16", 0), ("bf16", 24)])
+def test_prompt_then_decoding_steps_over_one_cache(cache, window):
+    """Three sequences: their prompts in two ragged chunks, then single tokens, then a draw:
+    the attention outputs equal those of a 64-bit evaluation over the rows that the appends
+    left in the cache, and the tokens are the definition's."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    torch.manual_seed(5)
+    H, kvh, page, sinks = 8, 2, 16, 4
+    T = _types(torch)[cache]
+    k, v = (torch.full((40, kvh, page, D), math.nan, device="cuda", dtype=T) for _ in "kv")
+    table = torch.randperm(40, device="cuda")[:36].to(torch.int32).view(3, 12)
+    a = torch.outer(torch.arange(192, device="cuda").double(), 1e6 ** (-torch.arange(64, device="cuda").double() / 64))
+    cos, sin = a.cos().float(), a.sin().float()
+    qn, kn = torch.rand(D, device="cuda") + 0.5, torch.rand(D, device="cuda") + 0.5
+    held = torch.zeros(3, dtype=torch.int32, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    head = torch.randn(H * D, 997, device="cuda") * 0.05
+    for new in ([70, 3, 33], [41, 1, 0], [1, 1, 1], [1, 1, 1]):
+        held += torch.tensor(new, dtype=torch.int32, device="cuda")
+        starts = torch.tensor([0, new[0], new[0] + new[1], sum(new)], dtype=torch.int32, device="cuda")
+        qkv = torch.randn(sum(new), (H + 2 * kvh) * D, device="cuda")
+        q = R.paged_append(qkv, k, v, table, held, cos, sin, H, q_norm=qn, k_norm=kn, q_starts=starts, status=status)
+        q = q.view(-1, H, D)
+        if max(new) > 1:
+            y = R.paged_attn_prompt(q, k, v, table, held, starts, window=window, sinks=sinks, status=status)
+        else:
+            y = R.paged_attn_decode(q, k, v, table, held, window=window, sinks=sinks, status=status)
+        want, tol = plain_attention(torch, q, k, v, table, held, new, window, sinks, D ** -0.5, "f32", cache)
+        close(torch, y, want, tol)
+    logits = y.reshape(3, -1) @ head
+    ids, logp = R.sample_rows(logits, torch.tensor([0.1, 0.5, 0.9], device="cuda"),
+                              temperature=torch.tensor([0.0, 1.0, 0.7], device="cuda"),
+                              top_k=torch.tensor([0, 1, 50], dtype=torch.int32, device="cuda"))
+    assert ids[:2].tolist() == logits[:2].argmax(-1).tolist()
+    w = torch.softmax(logits[2].double().topk(50).values / 0.7, 0)
+    rank = int((w.cumsum(0) <= 0.9).sum())
+    assert int(ids[2]) == int(logits[2].topk(50).indices[rank]) and abs(float(logp[2]) - math.log(float(w[rank]))) < 1e-5
+    assert int(status) == 0
