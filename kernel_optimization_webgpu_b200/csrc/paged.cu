@@ -1,10 +1,12 @@
 // Host entries of the paged key-value cache operators (kernels: paged.cuh).
+#include <algorithm>
 #include <cmath>
 #include <string>
 
 #include "../../include/qdecode.h"
 #include "internal.cuh"
 #include "paged.cuh"
+#include "paged_decode.cuh"
 
 namespace qd {
 
@@ -83,6 +85,19 @@ static void launch_rows(const PAttnArgs& a, int kv_dtype, cudaStream_t s) {
   }
 }
 
+template <typename T>
+static void launch_decode(const PAttnArgs& a, void* workspace, cudaStream_t s) {
+  static unsigned long long smem_set = 0;
+  allow_smem(k_paged_decode<T>, pd_smem(4096), smem_set);
+  const int nh = a.kv.kv_heads * ((a.q_heads / a.kv.kv_heads + 7) / 8);
+  // two CTAs an SM hold all of them at once; no more than there can be units
+  const long long most = (long long)a.kv.batch * nh * (((long long)a.kv.table_width << a.kv.page_shift) / kPdTile + 1);
+  if (most > 0x7fffffffLL) throw QdError{QD_E_RANGE, "qd_paged_attn_decode: batch * heads * table beyond 2^31 units"};
+  const int ctas = (int)std::max(1LL, std::min<long long>(most, std::min(2 * current_sms(), kPdMaxCtas)));
+  launch_ex(k_paged_decode<T>, dim3(ctas), dim3(kPdThreads), (size_t)pd_smem(a.kv.batch), s, a, workspace);
+  launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas);
+}
+
 }  // namespace qd
 
 using namespace qd;
@@ -155,7 +170,9 @@ int qd_paged_append(const qd_paged_kv* kv, const void* qkv, int qkv_dtype, int64
   });
 }
 
-size_t qd_paged_attn_decode_workspace_bytes(int batch, int q_heads) { return 256; }
+size_t qd_paged_attn_decode_workspace_bytes(int batch, int q_heads) {
+  return batch < 0 || q_heads < 0 ? 0 : pd_ws_bytes(batch);
+}
 
 int qd_paged_attn_decode(const qd_paged_kv* kv, const void* q, int dtype, int64_t q_stride, int q_heads, int window,
                          int sinks, float scale, void* y, int64_t y_stride, void* workspace, void* stream) {
@@ -164,7 +181,9 @@ int qd_paged_attn_decode(const qd_paged_kv* kv, const void* q, int dtype, int64_
     PAttnArgs a = check_attn(kv, q, dtype, q_stride, kv->batch, q_heads, window, sinks, scale, y, y_stride);
     if (a.rows == 0) return;
     need(workspace != nullptr, "qd_paged_attn_decode: NULL workspace");
-    launch_rows(a, kv->dtype, static_cast<cudaStream_t>(stream));
+    need(aligned16(workspace), "qd_paged_attn_decode: the workspace must be 16-byte aligned");
+    if (kv->dtype == QD_KV_F16) launch_decode<__half>(a, workspace, static_cast<cudaStream_t>(stream));
+    else launch_decode<__nv_bfloat16>(a, workspace, static_cast<cudaStream_t>(stream));
   });
 }
 

@@ -1,0 +1,491 @@
+// Attention of one new token per sequence over a paged cache, split over the cache's length.
+//
+// y = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s_j = scale q.k_j, over the visible keys. Each
+// key is read once and takes part in 4 * 128 flops per query head that shares it, far below
+// what the tensor cores do per byte: the kernel is bound by the bytes of K and V, so the
+// design is about keeping copies in flight on every SM from the first cycle to the last.
+//
+//  - Work is cut into units of 64 positions of one (sequence, KV head), and the flat list of all
+//    units into one run of equal length per CTA, whatever the lengths of the sequences. A run
+//    crosses from one sequence to the next without draining its copies. A (sequence, head) that
+//    one CTA holds whole is written by it; the others leave partial sums (at most two per CTA),
+//    which k_paged_decode_join adds in the order of the CTAs: no atomics, the same bits each time.
+//  - Warp w of a CTA owns positions 16w .. 16w+15 of every unit: its own ring of kPdStages slots
+//    filled by cp.async, its own running maximum and sum. No CTA barrier until a (sequence, head)
+//    ends. 16 positions lie in one page, so a slot needs one table entry, loaded a unit ahead.
+//    Rows that are not visible are filled with zeros instead of being read.
+//  - Products on mma.sync m16n8k16, 16 rows = up to 8 query heads twice: rows 0-7 hold the
+//    operand rounded to 16 bits, rows 8-15 what that rounding left. The two sums of a head meet
+//    in one thread (accumulator rows r and r + 8), so q and the weights keep twice 16 bits'
+//    precision at no extra instruction. (tcgen05 wants 64 rows or more; 56 of them would idle.)
+#pragma once
+
+#include "paged.cuh"
+
+namespace qd {
+
+constexpr int kPdThreads = 128;
+constexpr int kPdTile = 64;          // positions per unit
+constexpr int kPdStages = 3;
+constexpr int kPdSlot = 2 * 16 * 256;  // K and V rows of 16 positions
+constexpr int kPdMaxCtas = 320;
+constexpr float kPdLag = 8.0f;       // log2 a running maximum may fall behind before the sums are rescaled
+constexpr float kPdShift = 7.0f;     // weights are kept times 2^7: with the lag below 2^15 < 65504, and small
+                                     // weights stay in f16's normal range down to 2^-21 of the largest
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct PDecodeWs {
+  float* o;      // [2 * ctas][8][128]
+  float2* ml;    // [2 * ctas][8]
+  int* first;    // [batch + 1]: units of the sequences before b, one KV head's
+};
+__host__ __device__ inline size_t pd_ws_bytes(int batch) {
+  return (size_t)2 * kPdMaxCtas * 8 * (kHeadDim * 4 + 8) + (size_t)(batch + 1) * 4 + 256;
+}
+__host__ __device__ inline PDecodeWs pd_ws(void* p) {
+  PDecodeWs w;
+  w.o = static_cast<float*>(p);
+  w.ml = reinterpret_cast<float2*>(w.o + (size_t)2 * kPdMaxCtas * 8 * kHeadDim);
+  w.first = reinterpret_cast<int*>(w.ml + (size_t)2 * kPdMaxCtas * 8);
+  return w;
+}
+
+// The visible positions of a query at position asked - 1: [0, ns) and [lo, end), in tiles of
+// TILE positions: st of the sinks, then from w0 on.
+struct Visible {
+  int end, lo, ns, st, w0, tiles;
+  __device__ __forceinline__ bool at(int pos) const { return pos < end && (pos >= lo || pos < ns); }
+  __device__ __forceinline__ int tile(int i) const { return i < st ? i : w0 + (i - st); }
+};
+template <int TILE>
+__device__ __forceinline__ Visible visible(int asked, int len, int window, int sinks) {
+  Visible v;
+  v.end = len;
+  v.lo = window > 0 ? max(0, asked - window) : 0;
+  v.ns = min(min(sinks, v.lo), v.end);
+  v.st = (v.ns + TILE - 1) / TILE;
+  v.w0 = max(v.lo / TILE, v.st);
+  v.tiles = v.st + max(0, (v.end + TILE - 1) / TILE - v.w0);
+  return v;
+}
+
+__device__ __forceinline__ void cp_async16(unsigned dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1);
+template <>
+__device__ __forceinline__ void mma_16816<__half>(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&d)[4], const unsigned (&a)[4], unsigned b0,
+                                                         unsigned b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(unsigned addr, unsigned (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4_t(unsigned addr, unsigned (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+// hi = the pair rounded to 16 bits, lo = the rest, rounded again.
+template <typename T>
+__device__ __forceinline__ void split2(float x, float y, unsigned& hi, unsigned& lo);
+template <>
+__device__ __forceinline__ void split2<__half>(float x, float y, unsigned& hi, unsigned& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+  hi = *reinterpret_cast<const unsigned*>(&h);
+  lo = *reinterpret_cast<const unsigned*>(&l);
+}
+template <>
+__device__ __forceinline__ void split2<__nv_bfloat16>(float x, float y, unsigned& hi, unsigned& lo) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  const float2 f = __bfloat1622float2(h);
+  const __nv_bfloat162 l = __floats2bfloat162_rn(x - f.x, y - f.y);
+  hi = *reinterpret_cast<const unsigned*>(&h);
+  lo = *reinterpret_cast<const unsigned*>(&l);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float2 load2(const void* p, long long e, int dtype) {
+  if (dtype == QD_KV_F32) return *reinterpret_cast<const float2*>(static_cast<const float*>(p) + e);
+  const unsigned u = *reinterpret_cast<const unsigned*>(static_cast<const __half*>(p) + e);
+  if (dtype == QD_KV_F16) return __half22float2(*reinterpret_cast<const __half2*>(&u));
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+__device__ __forceinline__ void store2(void* p, long long e, int dtype, float x, float y) {
+  if (dtype == QD_KV_F32) {
+    *reinterpret_cast<float2*>(static_cast<float*>(p) + e) = make_float2(x, y);
+  } else if (dtype == QD_KV_F16) {
+    *reinterpret_cast<__half2*>(static_cast<__half*>(p) + e) = __floats2half2_rn(x, y);
+  } else {
+    *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(p) + e) = __floats2bfloat162_rn(x, y);
+  }
+}
+
+// Sum times the reciprocal of its weights; nothing seen gives zero.
+__device__ __forceinline__ float inv_sum(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+
+// A place in the flat list of units: unit t of sequence b's query group h (a KV head's heads,
+// eight at a time).
+struct PdCursor {
+  int b, h, t;
+  Visible v;
+};
+
+// Dynamic shared memory: 4 rings | the two halves' sums at a segment's end | units before b.
+__host__ __device__ constexpr int pd_smem(int batch) {
+  return 4 * kPdStages * kPdSlot + 2 * 8 * kHeadDim * 4 + 2 * 8 * 8 + (batch + 1) * 4;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_constant__ PAttnArgs a, void* workspace) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  unsigned char* ring = smem + warp * kPdStages * kPdSlot;
+  float* so = reinterpret_cast<float*>(smem + 4 * kPdStages * kPdSlot);  // [2][8][128]
+  float2* sml = reinterpret_cast<float2*>(so + 2 * 8 * kHeadDim);        // [2][8]
+  int* first = reinterpret_cast<int*>(sml + 16);
+  const int G = a.q_heads / a.kv.kv_heads, subs = (G + 7) >> 3, nh = a.kv.kv_heads * subs, B = a.kv.batch;
+  const PDecodeWs ws = pd_ws(workspace);
+  pdl_wait();
+  pdl_trigger();
+
+  // units before each sequence (an exclusive scan of the tile counts)
+  {
+    __shared__ int wsum[4];
+    const int per = (B + kPdThreads - 1) / kPdThreads;
+    const int b0 = min(tid * per, B), b1 = min(b0 + per, B);
+    int n = 0;
+    for (int b = b0; b < b1; ++b) {
+      const int t = visible<kPdTile>(a.kv.seq_lens[b], paged_len(a.kv, b), a.window, a.sinks).tiles;
+      first[b] = t;
+      n += t;
+    }
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    if (lane == 31) wsum[warp] = incl;
+    __syncthreads();
+    int at = incl - n;
+    for (int w = 0; w < warp; ++w) at += wsum[w];
+    for (int b = b0; b < b1; ++b) {
+      const int t = first[b];
+      first[b] = at;
+      at += t;
+    }
+    if (tid == kPdThreads - 1) first[B] = wsum[0] + wsum[1] + wsum[2] + wsum[3];
+    __syncthreads();
+  }
+  if (blockIdx.x == 0) {
+    for (int b = tid; b <= B; b += kPdThreads) ws.first[b] = first[b];
+    for (int b = tid; b < B; b += kPdThreads)
+      if (a.kv.seq_lens[b] > paged_len(a.kv, b) && a.kv.seq_lens[b] > 0) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
+  }
+  const long long U = (long long)first[B] * nh;
+  const int ctas = (int)min((long long)gridDim.x, U);  // none of them empty
+  if ((int)blockIdx.x >= ctas) return;
+  const int u0 = (int)(U * blockIdx.x / ctas), u1 = (int)(U * (blockIdx.x + 1) / ctas);
+
+  auto see = [&](PdCursor& c) {
+    c.v = visible<kPdTile>(a.kv.seq_lens[c.b], paged_len(a.kv, c.b), a.window, a.sinks);
+  };
+  auto step = [&](PdCursor& c) {  // to the next unit (there is one)
+    if (++c.t < c.v.tiles) return;
+    c.t = 0;
+    if (++c.h < nh) return;
+    c.h = 0;
+    do ++c.b;
+    while (first[c.b + 1] == first[c.b]);
+    see(c);
+  };
+  PdCursor cur;
+  {
+    int lo = 0, hi = B;  // the last sequence whose units start at or before u0
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if ((long long)first[mid] * nh <= u0) lo = mid;
+      else hi = mid;
+    }
+    cur.b = lo;
+    see(cur);
+    const int rest = u0 - first[lo] * nh;
+    cur.h = rest / cur.v.tiles;
+    cur.t = rest - cur.h * cur.v.tiles;
+  }
+  PdCursor pre = cur;  // the copies run ahead of the sums
+  const int n_units = u1 - u0;
+
+  // page of this warp's 16 positions of the unit at `pre`; -1: nothing visible there, -2: bad
+  auto page_of = [&](const PdCursor& c) {
+    const int p0 = c.v.tile(c.t) * kPdTile + 16 * warp;
+    const bool any = p0 < c.v.end && (p0 + 16 > c.v.lo || p0 < c.v.ns);
+    if (!any) return -1;
+    const int page = paged_page(a.kv, c.b, p0);
+    return page < 0 ? -2 : page;
+  };
+  int next_page = page_of(pre);
+  unsigned live_ring = 0;  // bit i: slot i holds rows
+  int issued = 0;
+  const int pmask = (1 << a.kv.page_shift) - 1;
+  const unsigned ring_s = (unsigned)__cvta_generic_to_shared(ring);
+  auto issue = [&]() {
+    const int slot = issued % kPdStages;
+    if (issued < n_units) {
+      const int page = next_page;
+      live_ring &= ~(1u << slot);
+      if (page >= 0) {
+        const int p0 = pre.v.tile(pre.t) * kPdTile + 16 * warp;
+        const long long row0 =
+            (((long long)page * a.kv.kv_heads + pre.h / subs) << a.kv.page_shift) + (p0 & pmask);
+        const char* ks = static_cast<const char*>(a.kv.k) + row0 * 256;
+        const char* vs = static_cast<const char*>(a.kv.v) + row0 * 256;
+        const unsigned dst = ring_s + slot * kPdSlot;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = 2 * i + (lane >> 4), c = lane & 15;
+          const bool ok = pre.v.at(p0 + r);
+          const unsigned off = r * 256 + ((c ^ (r & 7)) << 4);
+          cp_async16(dst + off, ks + r * 256 + c * 16, ok);
+          cp_async16(dst + 4096 + off, vs + r * 256 + c * 16, ok);
+        }
+        live_ring |= 1u << slot;
+      } else if (page == -2 && lane == 0) {
+        paged_flag(a.kv, QD_PAGED_BAD_PAGE);
+      }
+      ++issued;
+      if (issued < n_units) {
+        step(pre);
+        next_page = page_of(pre);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kPdStages - 1; ++i) issue();
+
+  const float qs = a.scale * kLog2e;
+  unsigned q[8][4];
+  float o[16][4], m = -INFINITY, l = 0.0f;
+  bool fresh = true;   // a new (sequence, head): load q, clear the sums
+  int seg = 0;         // segments finished by this CTA
+  bool from_start = cur.t == 0;
+  for (int i = 0; i < n_units; ++i) {
+    issue();
+    if (fresh) {
+      fresh = false;
+      const int hs = (cur.h % subs) * 8 + (lane >> 2);  // head within the KV head's group
+      const bool live = hs < G;
+      const long long base = cur.b * a.q_stride + ((long long)(cur.h / subs) * G + (live ? hs : 0)) * kHeadDim;
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) {
+        const int d = 16 * kk + 2 * (lane & 3);
+        const float2 x = load2(a.q, base + d, a.dtype), y = load2(a.q, base + d + 8, a.dtype);
+        const float f = live ? qs : 0.0f;
+        split2<T>(live ? x.x * f : 0.f, live ? x.y * f : 0.f, q[kk][0], q[kk][1]);
+        split2<T>(live ? y.x * f : 0.f, live ? y.y * f : 0.f, q[kk][2], q[kk][3]);
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+      m = -INFINITY;
+      l = 0.0f;
+    }
+    const int slot = i % kPdStages;
+    const bool rows = (live_ring >> slot) & 1u;
+    asm volatile("cp.async.wait_group %0;" ::"n"(kPdStages - 1) : "memory");
+    __syncwarp();
+    if (rows) {
+      const unsigned kb = ring_s + slot * kPdSlot, vb = kb + 4096;
+      float s[2][4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+      const int mi = lane >> 3, r8 = lane & 7;
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) {
+        unsigned b[4];
+        ldsm4(kb + (8 * (mi >> 1) + r8) * 256 + (((2 * kk + (mi & 1)) ^ r8) << 4), b);
+        mma_16816<T>(s[0], q[kk], b[0], b[1]);
+        mma_16816<T>(s[1], q[kk], b[2], b[3]);
+      }
+      const int p0 = cur.v.tile(cur.t) * kPdTile + 16 * warp;
+      float p[2][2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int pos = p0 + 8 * j + 2 * (lane & 3) + e;
+          p[j][e] = cur.v.at(pos) ? s[j][e] + s[j][2 + e] : -INFINITY;
+        }
+      float mt = fmaxf(fmaxf(p[0][0], p[0][1]), fmaxf(p[1][0], p[1][1]));
+      mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+      mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
+      if (__any_sync(0xffffffffu, mt > m + kPdLag)) {  // some head's maximum moved: rescale
+        const float mn = fmaxf(m, mt);
+        const float f = m == -INFINITY ? 0.0f : exp2_fast(m - mn);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          o[j][0] *= f;
+          o[j][1] *= f;
+          o[j][2] *= f;
+          o[j][3] *= f;
+        }
+      }
+      const float ref = m == -INFINITY ? 0.0f : m - kPdShift;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          p[j][e] = exp2_fast(p[j][e] - ref);
+          l += p[j][e];
+        }
+      unsigned w[4];
+      split2<T>(p[0][0], p[0][1], w[0], w[1]);
+      split2<T>(p[1][0], p[1][1], w[2], w[3]);
+#pragma unroll
+      for (int dn = 0; dn < 16; dn += 2) {
+        unsigned b[4];
+        ldsm4_t(vb + (r8 + 8 * (mi & 1)) * 256 + (((dn + (mi >> 1)) ^ r8) << 4), b);
+        mma_16816<T>(o[dn], w, b[0], b[1]);
+        mma_16816<T>(o[dn + 1], w, b[2], b[3]);
+      }
+    }
+    __syncwarp();  // the slot may be refilled
+    const bool last_t = cur.t + 1 == cur.v.tiles;
+    if (last_t || i + 1 == n_units) {
+      // The (sequence, head), or this CTA's part of it, ends: join the four warps.
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        o[j][0] += o[j][2];
+        o[j][1] += o[j][3];
+      }
+#pragma unroll
+      for (int half = 2; half >= 1; half >>= 1) {  // warps 2, 3 into 0, 1, then 1 into 0
+        if (warp >= half && warp < 2 * half) {
+          float* dst = so + (warp - half) * 8 * kHeadDim + (lane >> 2) * kHeadDim + 2 * (lane & 3);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) *reinterpret_cast<float2*>(dst + 8 * j) = make_float2(o[j][0], o[j][1]);
+          if ((lane & 3) == 0) sml[(warp - half) * 8 + (lane >> 2)] = make_float2(m, l);
+        }
+        __syncthreads();
+        if (warp < half) {
+          const float2 ml = sml[warp * 8 + (lane >> 2)];
+          const float mn = fmaxf(m, ml.x);
+          const float fa = m == -INFINITY ? 0.0f : exp2_fast(m - mn);
+          const float fb = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - mn);
+          const float* src = so + warp * 8 * kHeadDim + (lane >> 2) * kHeadDim + 2 * (lane & 3);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float2 x = *reinterpret_cast<const float2*>(src + 8 * j);
+            o[j][0] = o[j][0] * fa + x.x * fb;
+            o[j][1] = o[j][1] * fa + x.y * fb;
+          }
+          l = l * fa + ml.y * fb;
+          m = mn;
+        }
+        __syncthreads();
+      }
+      if (warp == 0) {
+        const int hs = (cur.h % subs) * 8 + (lane >> 2);
+        if (from_start && last_t) {
+          if (hs < G) {
+            const float z = inv_sum(l);
+            const long long base = cur.b * a.y_stride + ((long long)(cur.h / subs) * G + hs) * kHeadDim + 2 * (lane & 3);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) store2(a.y, base + 8 * j, a.dtype, o[j][0] * z, o[j][1] * z);
+          }
+        } else {
+          const long long slot8 = (2ll * blockIdx.x + (seg ? 1 : 0)) * 8 + (lane >> 2);
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            *reinterpret_cast<float2*>(ws.o + slot8 * kHeadDim + 8 * j + 2 * (lane & 3)) =
+                make_float2(o[j][0], o[j][1]);
+          if ((lane & 3) == 0) ws.ml[slot8] = make_float2(m, l);
+        }
+      }
+      ++seg;
+      fresh = true;
+    }
+    if (i + 1 < n_units) {
+      step(cur);
+      if (fresh) from_start = true;
+    }
+  }
+}
+
+// Joins the parts of each (sequence, query group) that several CTAs hold, and writes the zeros
+// of sequences without a visible key. Grid: batch * nh; warp w takes head w of the group.
+__global__ void __launch_bounds__(256) k_paged_decode_join(const __grid_constant__ PAttnArgs a, void* workspace,
+                                                           int grid) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int G = a.q_heads / a.kv.kv_heads, subs = (G + 7) >> 3, nh = a.kv.kv_heads * subs;
+  const int b = blockIdx.x / nh, h = blockIdx.x % nh, hs = (h % subs) * 8 + warp;
+  const PDecodeWs ws = pd_ws(workspace);
+  pdl_wait();
+  pdl_trigger();
+  if (hs >= G) return;
+  const int f0 = ws.first[b], tiles = ws.first[b + 1] - f0;
+  const long long base = b * a.y_stride + ((long long)(h / subs) * G + hs) * kHeadDim + 4 * lane;
+  if (tiles == 0) {
+    store4(a.y, base, a.dtype, make_float4(0.f, 0.f, 0.f, 0.f));
+    return;
+  }
+  const long long U = (long long)ws.first[a.kv.batch] * nh;
+  const int ctas = (int)min((long long)grid, U);
+  const long long v0 = (long long)f0 * nh + (long long)h * tiles, v1 = v0 + tiles;
+  const int c0 = (int)(((v0 + 1) * ctas - 1) / U), c1 = (int)((v1 * ctas - 1) / U);
+  if (c0 == c1) return;  // written whole
+  float M = -INFINITY, L = 0.0f;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c = c0; c <= c1; c += 32) {  // 32 parts at a time: their factors by lane, then the rows
+    const int n = min(32, c1 - c + 1);
+    long long slot = 0;
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (lane < n) {
+      const int cc = c + lane;
+      slot = (2ll * cc + (U * cc / ctas >= v0 ? 0 : 1)) * 8 + warp;
+      ml = ws.ml[slot];
+    }
+    const float mn = fmaxf(M, warp_max(ml.x));
+    const float fo = M == -INFINITY ? 0.0f : exp2_fast(M - mn);
+    const float f = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - mn);
+    L = L * fo + warp_sum(ml.y * f);
+    y = make_float4(y.x * fo, y.y * fo, y.z * fo, y.w * fo);
+    M = mn;
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) {
+      const float fk = __shfl_sync(0xffffffffu, f, k);
+      const long long sk = __shfl_sync(0xffffffffu, slot, k);
+      const float4 x = *reinterpret_cast<const float4*>(ws.o + sk * kHeadDim + 4 * lane);
+      y = make_float4(y.x + x.x * fk, y.y + x.y * fk, y.z + x.z * fk, y.w + x.w * fk);
+    }
+  }
+  const float z = inv_sum(L);
+  store4(a.y, base, a.dtype, make_float4(y.x * z, y.y * z, y.z * z, y.w * z));
+}
+
+}  // namespace qd
