@@ -131,39 +131,36 @@ __device__ __forceinline__ float2 load2(const void* p, long long e, int dtype) {
   if (dtype == QD_KV_F16) return __half22float2(*reinterpret_cast<const __half2*>(&u));
   return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
-__device__ __forceinline__ void store2(void* p, long long e, int dtype, float x, float y) {
-  if (dtype == QD_KV_F32) {
-    *reinterpret_cast<float2*>(static_cast<float*>(p) + e) = make_float2(x, y);
-  } else if (dtype == QD_KV_F16) {
-    *reinterpret_cast<__half2*>(static_cast<__half*>(p) + e) = __floats2half2_rn(x, y);
-  } else {
-    *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(p) + e) = __floats2bfloat162_rn(x, y);
-  }
+__device__ __forceinline__ void store1(void* p, long long e, int dtype, float x) {
+  if (dtype == QD_KV_F32) static_cast<float*>(p)[e] = x;
+  else if (dtype == QD_KV_F16) static_cast<__half*>(p)[e] = __float2half_rn(x);
+  else static_cast<__nv_bfloat16*>(p)[e] = __float2bfloat16_rn(x);
 }
 
 // Sum times the reciprocal of its weights; nothing seen gives zero.
 __device__ __forceinline__ float inv_sum(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
 
-// A place in the flat list of units: unit t of sequence b's query group h (a KV head's heads,
-// eight at a time).
+// A place in the flat list of units: unit t of sequence b, KV head g, and the sub-th eight of its
+// query heads.
 struct PdCursor {
-  int b, h, t;
+  int b, g, sub, t;
   Visible v;
 };
 
-// Dynamic shared memory: 4 rings | the two halves' sums at a segment's end | units before b.
-__host__ __device__ constexpr int pd_smem(int batch) {
-  return 4 * kPdStages * kPdSlot + 2 * 8 * kHeadDim * 4 + 2 * 8 * 8 + (batch + 1) * 4;
-}
+// Dynamic shared memory: 4 rings | units before each sequence. Where a (sequence, head) ends, each
+// warp's sums go to the ring slot it has just read, rows kPdSumRow floats apart (8 heads on
+// distinct banks).
+constexpr int kPdSumRow = 136;
+static_assert(8 * kPdSumRow * 4 <= kPdSlot, "a slot holds eight heads' sums");
+__host__ __device__ constexpr int pd_smem(int batch) { return 4 * kPdStages * kPdSlot + (batch + 1) * 4; }
 
 template <typename T>
 __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_constant__ PAttnArgs a, void* workspace) {
   extern __shared__ __align__(128) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   unsigned char* ring = smem + warp * kPdStages * kPdSlot;
-  float* so = reinterpret_cast<float*>(smem + 4 * kPdStages * kPdSlot);  // [2][8][128]
-  float2* sml = reinterpret_cast<float2*>(so + 2 * 8 * kHeadDim);        // [2][8]
-  int* first = reinterpret_cast<int*>(sml + 16);
+  int* first = reinterpret_cast<int*>(smem + 4 * kPdStages * kPdSlot);
+  __shared__ float2 sml[4][8];  // maximum and sum of each warp and head
   const int G = a.q_heads / a.kv.kv_heads, subs = (G + 7) >> 3, nh = a.kv.kv_heads * subs, B = a.kv.batch;
   const PDecodeWs ws = pd_ws(workspace);
   pdl_wait();
@@ -214,8 +211,10 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
   auto step = [&](PdCursor& c) {  // to the next unit (there is one)
     if (++c.t < c.v.tiles) return;
     c.t = 0;
-    if (++c.h < nh) return;
-    c.h = 0;
+    if (++c.sub < subs) return;
+    c.sub = 0;
+    if (++c.g < a.kv.kv_heads) return;
+    c.g = 0;
     do ++c.b;
     while (first[c.b + 1] == first[c.b]);
     see(c);
@@ -231,8 +230,10 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
     cur.b = lo;
     see(cur);
     const int rest = u0 - first[lo] * nh;
-    cur.h = rest / cur.v.tiles;
-    cur.t = rest - cur.h * cur.v.tiles;
+    const int h = rest / cur.v.tiles;
+    cur.t = rest - h * cur.v.tiles;
+    cur.g = h / subs;
+    cur.sub = h - cur.g * subs;
   }
   PdCursor pre = cur;  // the copies run ahead of the sums
   const int n_units = u1 - u0;
@@ -247,34 +248,47 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
   };
   int next_page = page_of(pre);
   unsigned live_ring = 0;  // bit i: slot i holds rows
-  int issued = 0;
+  int issued = 0, in_slot = 0;
   const int pmask = (1 << a.kv.page_shift) - 1;
   const unsigned ring_s = (unsigned)__cvta_generic_to_shared(ring);
+  // lane -> 16-byte chunk lane % 16 of rows 2i + lane / 16; chunk c of row r sits at c ^ (r % 8)
+  unsigned to[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 2 * i + (lane >> 4);
+    to[i] = ring_s + r * 256 + (((lane & 15) ^ r) << 4);
+  }
   auto issue = [&]() {
-    const int slot = issued % kPdStages;
     if (issued < n_units) {
       const int page = next_page;
-      live_ring &= ~(1u << slot);
+      live_ring &= ~(1u << in_slot);
       if (page >= 0) {
         const int p0 = pre.v.tile(pre.t) * kPdTile + 16 * warp;
-        const long long row0 =
-            (((long long)page * a.kv.kv_heads + pre.h / subs) << a.kv.page_shift) + (p0 & pmask);
-        const char* ks = static_cast<const char*>(a.kv.k) + row0 * 256;
-        const char* vs = static_cast<const char*>(a.kv.v) + row0 * 256;
-        const unsigned dst = ring_s + slot * kPdSlot;
+        const long long row0 = (((long long)page * a.kv.kv_heads + pre.g) << a.kv.page_shift) + (p0 & pmask);
+        const char* ks = static_cast<const char*>(a.kv.k) + row0 * 256 + lane * 16;
+        const char* vs = static_cast<const char*>(a.kv.v) + row0 * 256 + lane * 16;
+        const unsigned dst = in_slot * kPdSlot;
+        const bool all = p0 + 16 <= pre.v.end && (p0 >= pre.v.lo || p0 + 16 <= pre.v.ns);
+        if (all) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = 2 * i + (lane >> 4), c = lane & 15;
-          const bool ok = pre.v.at(p0 + r);
-          const unsigned off = r * 256 + ((c ^ (r & 7)) << 4);
-          cp_async16(dst + off, ks + r * 256 + c * 16, ok);
-          cp_async16(dst + 4096 + off, vs + r * 256 + c * 16, ok);
+          for (int i = 0; i < 8; ++i) {
+            cp_async16(to[i & 3] + dst + (i >> 2) * 2048, ks + i * 512, true);
+            cp_async16(to[i & 3] + dst + (i >> 2) * 2048 + 4096, vs + i * 512, true);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const bool ok = pre.v.at(p0 + 2 * i + (lane >> 4));
+            cp_async16(to[i & 3] + dst + (i >> 2) * 2048, ks + i * 512, ok);
+            cp_async16(to[i & 3] + dst + (i >> 2) * 2048 + 4096, vs + i * 512, ok);
+          }
         }
-        live_ring |= 1u << slot;
+        live_ring |= 1u << in_slot;
       } else if (page == -2 && lane == 0) {
         paged_flag(a.kv, QD_PAGED_BAD_PAGE);
       }
       ++issued;
+      in_slot = in_slot + 1 == kPdStages ? 0 : in_slot + 1;
       if (issued < n_units) {
         step(pre);
         next_page = page_of(pre);
@@ -285,58 +299,77 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
 #pragma unroll
   for (int i = 0; i < kPdStages - 1; ++i) issue();
 
+  // The queries of a (sequence, head): lane -> head lane / 4, dims 16 kk + 2 (lane % 4) + {0, 1, 8, 9}.
+  // They are fetched a unit before they are needed.
   const float qs = a.scale * kLog2e;
+  float2 qn[16];
+  auto fetch_q = [&](const PdCursor& c) {
+    const int hs = c.sub * 8 + (lane >> 2);
+    const bool live = hs < G;
+    const long long base = c.b * a.q_stride + ((long long)c.g * G + (live ? hs : 0)) * kHeadDim + 2 * (lane & 3);
+#pragma unroll
+    for (int kk = 0; kk < 16; ++kk) qn[kk] = load2(a.q, base + 8 * kk, a.dtype);
+    if (!live) {
+#pragma unroll
+      for (int kk = 0; kk < 16; ++kk) qn[kk] = make_float2(0.f, 0.f);
+    }
+  };
+  fetch_q(cur);
   unsigned q[8][4];
   float o[16][4], m = -INFINITY, l = 0.0f;
-  bool fresh = true;   // a new (sequence, head): load q, clear the sums
+  bool fresh = true;   // a new (sequence, head): take its q, clear the sums
   int seg = 0;         // segments finished by this CTA
   bool from_start = cur.t == 0;
+  int slot = 0;
   for (int i = 0; i < n_units; ++i) {
     issue();
     if (fresh) {
       fresh = false;
-      const int hs = (cur.h % subs) * 8 + (lane >> 2);  // head within the KV head's group
-      const bool live = hs < G;
-      const long long base = cur.b * a.q_stride + ((long long)(cur.h / subs) * G + (live ? hs : 0)) * kHeadDim;
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) {
-        const int d = 16 * kk + 2 * (lane & 3);
-        const float2 x = load2(a.q, base + d, a.dtype), y = load2(a.q, base + d + 8, a.dtype);
-        const float f = live ? qs : 0.0f;
-        split2<T>(live ? x.x * f : 0.f, live ? x.y * f : 0.f, q[kk][0], q[kk][1]);
-        split2<T>(live ? y.x * f : 0.f, live ? y.y * f : 0.f, q[kk][2], q[kk][3]);
+        split2<T>(qn[2 * kk].x * qs, qn[2 * kk].y * qs, q[kk][0], q[kk][1]);
+        split2<T>(qn[2 * kk + 1].x * qs, qn[2 * kk + 1].y * qs, q[kk][2], q[kk][3]);
       }
 #pragma unroll
       for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
       m = -INFINITY;
       l = 0.0f;
     }
-    const int slot = i % kPdStages;
+    const bool last_t = cur.t + 1 == cur.v.tiles, more = i + 1 < n_units;
+    PdCursor nxt = cur;
+    if (more) {
+      step(nxt);
+      if (last_t) fetch_q(nxt);
+    }
     const bool rows = (live_ring >> slot) & 1u;
     asm volatile("cp.async.wait_group %0;" ::"n"(kPdStages - 1) : "memory");
     __syncwarp();
     if (rows) {
       const unsigned kb = ring_s + slot * kPdSlot, vb = kb + 4096;
-      float s[2][4];
+      float s[4][4];  // two key halves, each in two chains of products (even and odd steps)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+      for (int j = 0; j < 4; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
       const int mi = lane >> 3, r8 = lane & 7;
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) {
         unsigned b[4];
         ldsm4(kb + (8 * (mi >> 1) + r8) * 256 + (((2 * kk + (mi & 1)) ^ r8) << 4), b);
-        mma_16816<T>(s[0], q[kk], b[0], b[1]);
-        mma_16816<T>(s[1], q[kk], b[2], b[3]);
+        mma_16816<T>(s[2 * (kk & 1)], q[kk], b[0], b[1]);
+        mma_16816<T>(s[2 * (kk & 1) + 1], q[kk], b[2], b[3]);
       }
       const int p0 = cur.v.tile(cur.t) * kPdTile + 16 * warp;
       float p[2][2];
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int pos = p0 + 8 * j + 2 * (lane & 3) + e;
-          p[j][e] = cur.v.at(pos) ? s[j][e] + s[j][2 + e] : -INFINITY;
-        }
+        for (int e = 0; e < 2; ++e) p[j][e] = (s[j][e] + s[2 + j][e]) + (s[j][2 + e] + s[2 + j][2 + e]);
+      if (!(p0 + 16 <= cur.v.end && (p0 >= cur.v.lo || p0 + 16 <= cur.v.ns))) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (!cur.v.at(p0 + 8 * j + 2 * (lane & 3) + e)) p[j][e] = -INFINITY;
+      }
       float mt = fmaxf(fmaxf(p[0][0], p[0][1]), fmaxf(p[1][0], p[1][1]));
       mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
       mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
@@ -373,119 +406,120 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
       }
     }
     __syncwarp();  // the slot may be refilled
-    const bool last_t = cur.t + 1 == cur.v.tiles;
-    if (last_t || i + 1 == n_units) {
+    if (last_t || !more) {
       // The (sequence, head), or this CTA's part of it, ends: join the four warps.
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
+      float* mine = reinterpret_cast<float*>(ring + slot * kPdSlot) + (lane >> 2) * kPdSumRow + 2 * (lane & 3);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        o[j][0] += o[j][2];
-        o[j][1] += o[j][3];
-      }
+      for (int j = 0; j < 16; ++j)
+        *reinterpret_cast<float2*>(mine + 8 * j) = make_float2(o[j][0] + o[j][2], o[j][1] + o[j][3]);
+      if ((lane & 3) == 0) sml[warp][lane >> 2] = make_float2(m, l);
+      __syncthreads();
+      const int live = min(8, G - cur.sub * 8);
+      const bool whole = from_start && last_t;
+      const long long out = cur.b * a.y_stride + ((long long)cur.g * G + cur.sub * 8) * kHeadDim + tid;
+      const long long part = (2ll * blockIdx.x + (seg ? 1 : 0)) * 8;
+      for (int h = 0; h < live; ++h) {  // thread tid: dim tid
+        const float M = fmaxf(fmaxf(sml[0][h].x, sml[1][h].x), fmaxf(sml[2][h].x, sml[3][h].x));
+        float L = 0.0f, x = 0.0f;
 #pragma unroll
-      for (int half = 2; half >= 1; half >>= 1) {  // warps 2, 3 into 0, 1, then 1 into 0
-        if (warp >= half && warp < 2 * half) {
-          float* dst = so + (warp - half) * 8 * kHeadDim + (lane >> 2) * kHeadDim + 2 * (lane & 3);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) *reinterpret_cast<float2*>(dst + 8 * j) = make_float2(o[j][0], o[j][1]);
-          if ((lane & 3) == 0) sml[(warp - half) * 8 + (lane >> 2)] = make_float2(m, l);
+        for (int w = 0; w < 4; ++w) {
+          const float f = sml[w][h].x == -INFINITY ? 0.0f : exp2_fast(sml[w][h].x - M);
+          L += sml[w][h].y * f;
+          x += reinterpret_cast<const float*>(smem + (w * kPdStages + slot) * kPdSlot)[h * kPdSumRow + tid] * f;
         }
-        __syncthreads();
-        if (warp < half) {
-          const float2 ml = sml[warp * 8 + (lane >> 2)];
-          const float mn = fmaxf(m, ml.x);
-          const float fa = m == -INFINITY ? 0.0f : exp2_fast(m - mn);
-          const float fb = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - mn);
-          const float* src = so + warp * 8 * kHeadDim + (lane >> 2) * kHeadDim + 2 * (lane & 3);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float2 x = *reinterpret_cast<const float2*>(src + 8 * j);
-            o[j][0] = o[j][0] * fa + x.x * fb;
-            o[j][1] = o[j][1] * fa + x.y * fb;
-          }
-          l = l * fa + ml.y * fb;
-          m = mn;
-        }
-        __syncthreads();
-      }
-      if (warp == 0) {
-        const int hs = (cur.h % subs) * 8 + (lane >> 2);
-        if (from_start && last_t) {
-          if (hs < G) {
-            const float z = inv_sum(l);
-            const long long base = cur.b * a.y_stride + ((long long)(cur.h / subs) * G + hs) * kHeadDim + 2 * (lane & 3);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) store2(a.y, base + 8 * j, a.dtype, o[j][0] * z, o[j][1] * z);
-          }
+        if (whole) {
+          store1(a.y, out + h * kHeadDim, a.dtype, x * inv_sum(L));
         } else {
-          const long long slot8 = (2ll * blockIdx.x + (seg ? 1 : 0)) * 8 + (lane >> 2);
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            *reinterpret_cast<float2*>(ws.o + slot8 * kHeadDim + 8 * j + 2 * (lane & 3)) =
-                make_float2(o[j][0], o[j][1]);
-          if ((lane & 3) == 0) ws.ml[slot8] = make_float2(m, l);
+          ws.o[(part + h) * kHeadDim + tid] = x;
+          if (tid == 0) ws.ml[part + h] = make_float2(M, L);
         }
       }
+      __syncthreads();  // before the slots are refilled
       ++seg;
       fresh = true;
+      from_start = true;
     }
-    if (i + 1 < n_units) {
-      step(cur);
-      if (fresh) from_start = true;
-    }
+    cur = nxt;
+    slot = slot + 1 == kPdStages ? 0 : slot + 1;
   }
 }
 
 // Joins the parts of each (sequence, query group) that several CTAs hold, and writes the zeros
-// of sequences without a visible key. Grid: batch * nh; warp w takes head w of the group.
+// of sequences without a visible key. Grid: batch * nh. Warp w takes head w / per of the group
+// and every per-th part (per = 8 / heads, a power of two): each lane's loads of up to eight
+// parts are in flight together (with one warp per head, 37 parts took 6 us).
 __global__ void __launch_bounds__(256) k_paged_decode_join(const __grid_constant__ PAttnArgs a, void* workspace,
                                                            int grid) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int G = a.q_heads / a.kv.kv_heads, subs = (G + 7) >> 3, nh = a.kv.kv_heads * subs;
-  const int b = blockIdx.x / nh, h = blockIdx.x % nh, hs = (h % subs) * 8 + warp;
+  const int b = blockIdx.x / nh, h = blockIdx.x % nh, heads = min(8, G - (h % subs) * 8);
   const PDecodeWs ws = pd_ws(workspace);
   pdl_wait();
   pdl_trigger();
-  if (hs >= G) return;
   const int f0 = ws.first[b], tiles = ws.first[b + 1] - f0;
-  const long long base = b * a.y_stride + ((long long)(h / subs) * G + hs) * kHeadDim + 4 * lane;
-  if (tiles == 0) {
-    store4(a.y, base, a.dtype, make_float4(0.f, 0.f, 0.f, 0.f));
-    return;
-  }
   const long long U = (long long)ws.first[a.kv.batch] * nh;
   const int ctas = (int)min((long long)grid, U);
   const long long v0 = (long long)f0 * nh + (long long)h * tiles, v1 = v0 + tiles;
-  const int c0 = (int)(((v0 + 1) * ctas - 1) / U), c1 = (int)((v1 * ctas - 1) / U);
-  if (c0 == c1) return;  // written whole
+  int c0 = 0, c1 = -1;
+  if (tiles > 0) {
+    c0 = (int)(((v0 + 1) * ctas - 1) / U);
+    c1 = (int)((v1 * ctas - 1) / U);
+    if (c0 == c1) return;  // written whole
+  }
+  const int lg = heads > 4 ? 0 : heads > 2 ? 1 : heads > 1 ? 2 : 3, per = 1 << lg;
+  const int hw = warp >> lg, k0 = warp & (per - 1);
   float M = -INFINITY, L = 0.0f;
   float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c = c0; c <= c1; c += 32) {  // 32 parts at a time: their factors by lane, then the rows
-    const int n = min(32, c1 - c + 1);
-    long long slot = 0;
-    float2 ml = make_float2(-INFINITY, 0.0f);
-    if (lane < n) {
-      const int cc = c + lane;
-      slot = (2ll * cc + (U * cc / ctas >= v0 ? 0 : 1)) * 8 + warp;
-      ml = ws.ml[slot];
-    }
-    const float mn = fmaxf(M, warp_max(ml.x));
-    const float fo = M == -INFINITY ? 0.0f : exp2_fast(M - mn);
-    const float f = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - mn);
-    L = L * fo + warp_sum(ml.y * f);
-    y = make_float4(y.x * fo, y.y * fo, y.z * fo, y.w * fo);
-    M = mn;
-#pragma unroll 4
-    for (int k = 0; k < n; ++k) {
-      const float fk = __shfl_sync(0xffffffffu, f, k);
-      const long long sk = __shfl_sync(0xffffffffu, slot, k);
-      const float4 x = *reinterpret_cast<const float4*>(ws.o + sk * kHeadDim + 4 * lane);
-      y = make_float4(y.x + x.x * fk, y.y + x.y * fk, y.z + x.z * fk, y.w + x.w * fk);
+  if (hw < heads) {
+    for (int c = c0 + k0; c <= c1; c += 8 * per) {
+      float2 ml[8];
+      float4 x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int cc = c + k * per;
+        ml[k] = make_float2(-INFINITY, 0.0f);
+        x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (cc <= c1) {
+          const long long slot = (2ll * cc + (U * cc / ctas >= v0 ? 0 : 1)) * 8 + hw;
+          ml[k] = ws.ml[slot];
+          x[k] = *reinterpret_cast<const float4*>(ws.o + slot * kHeadDim + 4 * lane);
+        }
+      }
+      float mn = M;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mn = fmaxf(mn, ml[k].x);
+      const float fo = M == -INFINITY ? 0.0f : exp2_fast(M - mn);
+      L *= fo;
+      y = make_float4(y.x * fo, y.y * fo, y.z * fo, y.w * fo);
+      M = mn;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float f = ml[k].x == -INFINITY ? 0.0f : exp2_fast(ml[k].x - M);
+        L += ml[k].y * f;
+        y = make_float4(y.x + x[k].x * f, y.y + x[k].y * f, y.z + x[k].z * f, y.w + x[k].w * f);
+      }
     }
   }
+  __shared__ float2 sml[8];
+  __shared__ float4 so[8][32];
+  if (lane == 0) sml[warp] = make_float2(M, L);
+  so[warp][lane] = y;
+  __syncthreads();
+  if (hw >= heads || k0) return;
+  for (int w = 1; w < per; ++w) {
+    const float2 ml = sml[warp + w];
+    const float4 x = so[warp + w][lane];
+    const float mn = fmaxf(M, ml.x);
+    const float fa = M == -INFINITY ? 0.0f : exp2_fast(M - mn), fb = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - mn);
+    L = L * fa + ml.y * fb;
+    y = make_float4(y.x * fa + x.x * fb, y.y * fa + x.y * fb, y.z * fa + x.z * fb, y.w * fa + x.w * fb);
+    M = mn;
+  }
   const float z = inv_sum(L);
-  store4(a.y, base, a.dtype, make_float4(y.x * z, y.y * z, y.z * z, y.w * z));
+  store4(a.y, b * a.y_stride + ((long long)(h / subs) * G + (h % subs) * 8 + hw) * kHeadDim + 4 * lane, a.dtype,
+         make_float4(y.x * z, y.y * z, y.z * z, y.w * z));
 }
 
 }  // namespace qd
