@@ -392,6 +392,7 @@ int qd_gqa_decode_noalloc(const float* q, const void* k_cache, const void* v_cac
  * written, not attended to; the length is cut) and the bit is set in *status. */
 #define QD_PAGED_BAD_PAGE 1     /* status bits (or-ed; never cleared by the library) */
 #define QD_PAGED_BAD_LENGTH 2
+#define QD_PAGED_TIMEOUT 4      /* a device-side wait of qd_paged_attn_prompt expired: its results are void */
 
 typedef struct qd_paged_kv {
   void* k;                      /* [num_pages][kv_heads][page_size][head_dim] of dtype, 16-byte aligned */

@@ -23,6 +23,7 @@ QD_KV_F32 = 1
 QD_KV_BF16 = 2
 QD_PAGED_BAD_PAGE = 1
 QD_PAGED_BAD_LENGTH = 2
+QD_PAGED_TIMEOUT = 4
 
 # Every function include/qdecode.h declares (checked by the tests).
 EXPORTS = (

@@ -15,7 +15,7 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libqdecode.so")
 SOURCES = ["engine.cu", "batch.cu", "noalloc.cu", "bench_api.cu", "sample.cu", "paged.cu", "sample_rows.cu"]
-DEPS = SOURCES + ["kernels.cuh", "persist.cuh", "gemm_tc.cuh", "batch.cuh", "paged.cuh", "paged_decode.cuh", "internal.cuh", "tma.cuh", "common.cuh", "json.hpp"]
+DEPS = SOURCES + ["kernels.cuh", "persist.cuh", "gemm_tc.cuh", "batch.cuh", "paged.cuh", "paged_decode.cuh", "paged_prompt.cuh", "internal.cuh", "tma.cuh", "common.cuh", "json.hpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -7,6 +7,7 @@
 #include "internal.cuh"
 #include "paged.cuh"
 #include "paged_decode.cuh"
+#include "paged_prompt.cuh"
 
 namespace qd {
 
@@ -65,24 +66,13 @@ static PAttnArgs check_attn(const qd_paged_kv* kv, const void* q, int dtype, int
   a.q_stride = q_stride;
   a.rows = rows;
   a.q_heads = q_heads;
-  a.window = window;
-  a.sinks = sinks;
+  a.window = std::min(window, 1 << 30);  // positions end at 2^30: the same keys, and no overflow
+  a.sinks = std::min(sinks, 1 << 30);
   a.scale = scale == 0.0f ? 1.0f / std::sqrt((float)kHeadDim) : scale;
   a.y = y;
   a.dtype = dtype;
   a.y_stride = y_stride;
   return a;
-}
-
-static void launch_rows(const PAttnArgs& a, int kv_dtype, cudaStream_t s) {
-  const dim3 grid(a.rows, a.q_heads), block(128);
-  if (kv_dtype == QD_KV_F16) {
-    if (a.dtype == QD_KV_F32) launch_ex(k_paged_attn_rows<float, __half>, grid, block, 0, s, a);
-    else launch_ex(k_paged_attn_rows<__half, __half>, grid, block, 0, s, a);
-  } else {
-    if (a.dtype == QD_KV_F32) launch_ex(k_paged_attn_rows<float, __nv_bfloat16>, grid, block, 0, s, a);
-    else launch_ex(k_paged_attn_rows<__nv_bfloat16, __nv_bfloat16>, grid, block, 0, s, a);
-  }
 }
 
 template <typename T>
@@ -96,6 +86,46 @@ static void launch_decode(const PAttnArgs& a, void* workspace, cudaStream_t s) {
   const int ctas = (int)std::max(1LL, std::min<long long>(most, std::min(2 * current_sms(), kPdMaxCtas)));
   launch_ex(k_paged_decode<T>, dim3(ctas), dim3(kPdThreads), (size_t)pd_smem(a.kv.batch), s, a, workspace);
   launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas);
+}
+
+// Row tiles of a call (at most), and the parts that their keys are split into: enough to give
+// every SM a CTA, none where the row tiles alone do.
+static int prompt_items(int batch, int rows, int group) {
+  return (int)((long long)rows * group / kPpRows) + std::min(batch, rows);
+}
+static int prompt_splits(int items, int kv_heads) {
+  const long long n = (long long)items * kv_heads;
+  return n == 0 ? 1 : (int)std::max(1LL, std::min<long long>(kPpMaxSplits, current_sms() / n));
+}
+
+template <typename T, bool SPLIT>
+static void launch_prompt(const PAttnArgs& a, const void* q_any, void* workspace, cudaStream_t s) {
+  const int G = a.q_heads / a.kv.kv_heads, items = prompt_items(a.kv.batch, a.rows, G);
+  PPromptArgs p{};
+  p.a = a;
+  p.splits = prompt_splits(items, a.kv.kv_heads);
+  p.po = static_cast<float*>(workspace);
+  p.pml = reinterpret_cast<float2*>(p.po + (size_t)items * a.kv.kv_heads * p.splits * kPpRows * kHeadDim);
+  // a table that holds few tiles never splits them into more parts than this
+  const long long tiles = (((long long)a.kv.table_width << a.kv.page_shift) + kPpKeys - 1) / kPpKeys;
+  p.splits = (int)std::max(1LL, std::min<long long>(p.splits, tiles / 2));
+  const long long grid = (long long)items * a.kv.kv_heads * p.splits;
+  if (grid * 32 > 0x7fffffffLL) throw QdError{QD_E_RANGE, "qd_paged_attn_prompt: too many rows"};
+  const CUtensorMapDataType type =
+      std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const unsigned box = std::min(1 << a.kv.page_shift, kPpKeys);
+  // (an empty pool has no page that could be copied: any address will do)
+  const uint64_t pool = std::max<uint64_t>((uint64_t)a.kv.num_pages * a.kv.kv_heads << a.kv.page_shift, box);
+  std::string err;
+  if (!make_tmap_2d(&p.tk, a.kv.num_pages ? a.kv.k : q_any, type, kHeadDim, pool, kHeadDim * 2, 64, box,
+                    CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
+      !make_tmap_2d(&p.tv, a.kv.num_pages ? a.kv.v : q_any, type, kHeadDim, pool, kHeadDim * 2, 64, box,
+                    CU_TENSOR_MAP_SWIZZLE_128B, &err))
+    throw QdError{QD_E_CUDA, err};
+  static unsigned long long smem_set = 0;
+  allow_smem(k_paged_prompt<T, SPLIT>, pp_smem<SPLIT>(), smem_set);
+  launch_ex(k_paged_prompt<T, SPLIT>, dim3((unsigned)grid), dim3(kPpThreads), (size_t)pp_smem<SPLIT>(), s, p);
+  if (p.splits > 1) launch_ex(k_paged_prompt_join, dim3(items * a.kv.kv_heads * 32), dim3(256), 0, s, p);
 }
 
 }  // namespace qd
@@ -187,7 +217,11 @@ int qd_paged_attn_decode(const qd_paged_kv* kv, const void* q, int dtype, int64_
   });
 }
 
-size_t qd_paged_attn_prompt_workspace_bytes(int batch, int rows, int q_heads, int kv_heads) { return 256; }
+size_t qd_paged_attn_prompt_workspace_bytes(int batch, int rows, int q_heads, int kv_heads) {
+  if (batch < 0 || rows < 0 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads) return 0;
+  const int items = prompt_items(batch, rows, q_heads / kv_heads), splits = prompt_splits(items, kv_heads);
+  return splits == 1 ? 256 : (size_t)items * kv_heads * splits * kPpRows * (kHeadDim * 4 + 8);
+}
 
 int qd_paged_attn_prompt(const qd_paged_kv* kv, const void* q, int dtype, int64_t q_stride, int rows,
                          const int32_t* q_starts, int q_heads, int window, int sinks, float scale, void* y,
@@ -198,7 +232,15 @@ int qd_paged_attn_prompt(const qd_paged_kv* kv, const void* q, int dtype, int64_
     need(q_starts != nullptr, "qd_paged_attn_prompt: NULL q_starts");
     need(workspace != nullptr, "qd_paged_attn_prompt: NULL workspace");
     a.q_starts = q_starts;
-    launch_rows(a, kv->dtype, static_cast<cudaStream_t>(stream));
+    need(aligned16(workspace), "qd_paged_attn_prompt: the workspace must be 16-byte aligned");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (kv->dtype == QD_KV_F16) {
+      if (dtype == QD_KV_F32) launch_prompt<__half, true>(a, q, workspace, s);
+      else launch_prompt<__half, false>(a, q, workspace, s);
+    } else {
+      if (dtype == QD_KV_F32) launch_prompt<__nv_bfloat16, true>(a, q, workspace, s);
+      else launch_prompt<__nv_bfloat16, false>(a, q, workspace, s);
+    }
   });
 }
 

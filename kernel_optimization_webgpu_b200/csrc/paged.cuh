@@ -203,67 +203,4 @@ struct PAttnArgs {
   long long y_stride;
 };
 
-// The plainest form: one CTA per (row, query head), four warps stepping over the visible keys
-// with a running maximum and sum each, joined at the end.
-template <typename TQ, typename TKV>
-__global__ void __launch_bounds__(128) k_paged_attn_rows(const __grid_constant__ PAttnArgs a) {
-  const int r = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = h / (a.q_heads / a.kv.kv_heads);
-  pdl_wait();
-  int b = r, back = 1;
-  if (a.q_starts) {
-    b = paged_find_seq(a.q_starts, a.kv.batch, r);
-    if (b < 0) return;
-    back = a.q_starts[b + 1] - r;
-  }
-  const int len = paged_len(a.kv, b);
-  const int asked = a.kv.seq_lens[b];
-  if (len < asked && lane == 0) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
-  const int p = asked - back;
-  const int end = min(p + 1, len);  // keys [0, end), minus what the window hides
-  const int lo = a.window > 0 ? max(0, p + 1 - a.window) : 0;
-  const int ns = min(min(a.sinks, lo), end);
-  float4 q = load4<TQ>(a.q, r * a.q_stride + (long long)h * kHeadDim + 4 * lane);
-  float m = -INFINITY, l = 0.0f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int n = ns + max(0, end - lo);
-  for (int i = warp; i < n; i += 4) {
-    const int j = i < ns ? i : lo + i - ns;
-    const int page = paged_page(a.kv, b, j);
-    if (page < 0) {
-      if (lane == 0) paged_flag(a.kv, QD_PAGED_BAD_PAGE);
-      continue;
-    }
-    const long long row = (((long long)page * a.kv.kv_heads + g) << a.kv.page_shift) + (j & ((1 << a.kv.page_shift) - 1));
-    const float4 k = load4<TKV>(a.kv.k, row * kHeadDim + 4 * lane);
-    const float4 v = load4<TKV>(a.kv.v, row * kHeadDim + 4 * lane);
-    const float s = warp_sum(q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w) * a.scale;
-    const float mn = fmaxf(m, s), f = m == -INFINITY ? 0.0f : expf(m - mn), w = mn == -INFINITY ? 0.0f : expf(s - mn);
-    l = l * f + w;
-    o = make_float4(o.x * f + w * v.x, o.y * f + w * v.y, o.z * f + w * v.z, o.w * f + w * v.w);
-    m = mn;
-  }
-  __shared__ float sm[4], sl[4];
-  __shared__ float4 so[4][32];
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
-  }
-  so[warp][lane] = o;
-  __syncthreads();
-  if (warp) return;
-  const float M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  float L = 0.0f;
-  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = 0; i < 4; ++i) {
-    const float f = sm[i] == -INFINITY ? 0.0f : expf(sm[i] - M);
-    const float4 t = so[i][lane];
-    L += sl[i] * f;
-    y = make_float4(y.x + t.x * f, y.y + t.y * f, y.z + t.z * f, y.w + t.w * f);
-  }
-  const float z = L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L);  // nothing seen: zeros
-  store4(a.y, r * a.y_stride + (long long)h * kHeadDim + 4 * lane, a.dtype,
-         make_float4(y.x * z, y.y * z, y.z * z, y.w * z));
-}
-
 }  // namespace qd

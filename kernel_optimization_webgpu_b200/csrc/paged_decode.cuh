@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
       mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
       mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
       if (__any_sync(0xffffffffu, mt > m + kPdLag)) {  // some head's maximum moved: rescale
-        const float mn = fmaxf(m, mt);
+        const float mn = mt > m + kPdLag ? mt : m;
         const float f = m == -INFINITY ? 0.0f : exp2_fast(m - mn);
         m = mn;
         l *= f;

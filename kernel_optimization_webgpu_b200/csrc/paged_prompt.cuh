@@ -1,0 +1,590 @@
+// Attention of a ragged batch of prompt chunks over a paged cache, on the tcgen05 tensor cores.
+//
+// Rows: the (token, query head) pairs of one sequence and KV head, token-major, so that all the
+// query heads that share a KV head share its tiles whatever their number. A CTA takes 256
+// consecutive rows as two M = 128 tiles and walks the 128-key tiles that any of its rows sees:
+//   S = Q K^T      -> TMEM (f32)                     M 128, N 128 keys, K 128 dims
+//   P = exp2(S c - m)   one thread per row: maximum, weights, their sum, all in f32
+//   O += P V       -> TMEM (f32), P read from TMEM   M 128, N 128 dims, K 128 keys
+// The two tiles alternate: while one's softmax runs, the tensor cores work for the other. P
+// replaces its S in TMEM (S0 S1 O0 O1 = 512 columns); the MMAs of one issuer run in order, so
+// S of the next key tile may be issued right behind the product that reads P.
+//
+// O is rescaled only when a row's maximum has grown by more than 2^kPpLag since the last time
+// (weights then stay below 2^(kPpLag + kPpShift), inside f16); the final division makes up for
+// it, so the result is exact to rounding. P is rounded to the cache's 16-bit type (half a step
+// relative, as the tensor cores take 16-bit operands); its sum is taken in f32 before that.
+// With f32 queries (SPLIT) q and P are each a sum of two 16-bit operands and every product is
+// issued twice, which keeps f32 accuracy on an f16 cache.
+//
+// K and V come page by page by TMA (128-byte swizzle; rows of a page and head are contiguous)
+// into a ring of 32 KB tiles. V rows that no query of the CTA sees are cleared in shared memory:
+// their weight is 0, but 0 times what a recycled page holds could be NaN.
+//
+// Few rows over a long cache (a chunk behind a long context): the key tiles of a CTA's rows are
+// split over gridDim parts whose sums k_paged_prompt_join adds in order.
+#pragma once
+
+#include <climits>
+#include <type_traits>
+
+#include "gemm_tc.cuh"
+#include "paged_decode.cuh"
+
+namespace qd {
+
+constexpr int kPpThreads = 384;    // 2 x 128 softmax threads; the MMA warp, the copy warp and two idle ones
+// Registers: 168 a thread at launch (64512 in all); the softmax threads hold a row of 128 scores, so
+// the third warpgroup gives its share up: 2 * 128 * 224 + 128 * 56 = 64512.
+constexpr int kPpRegsMany = 224, kPpRegsFew = 56;
+constexpr int kPpRows = 256;
+constexpr int kPpKeys = 128;
+constexpr int kPpTileBytes = 128 * 256;  // a 128 x 128 tile of 16-bit elements
+constexpr int kPpMaxSplits = 32;
+constexpr float kPpLag = 8.0f, kPpShift = 7.0f;
+
+struct PPromptArgs {
+  CUtensorMap tk, tv;
+  PAttnArgs a;
+  int splits;
+  float* po;     // [item][split][256][128] unnormalised
+  float2* pml;   // [item][split][256]
+};
+
+template <bool SPLIT>
+__host__ __device__ constexpr int pp_slots() { return SPLIT ? 3 : 5; }
+template <bool SPLIT>
+__host__ __device__ constexpr int pp_smem() {
+  return ((SPLIT ? 4 : 2) + pp_slots<SPLIT>()) * kPpTileBytes + 1024;
+}
+
+// The item-th tile of rows, counted from the last (the latest rows of a prompt see the most keys
+// and start first): its sequence and tile, or false. Called by whole warps.
+__device__ __forceinline__ bool pp_item(const PAttnArgs& a, int G, int item, int& seq, int& tile) {
+  const int lane = threadIdx.x & 31, B = a.kv.batch;
+  int total = 0;
+  for (int b0 = 0; b0 < B; b0 += 32) {
+    const int b = b0 + lane;
+    const int n = b < B ? max(a.q_starts[b + 1] - a.q_starts[b], 0) : 0;
+    int t = (n * G + kPpRows - 1) / kPpRows;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    total += t;
+  }
+  int want = total - 1 - item;
+  if (want < 0) return false;
+  for (int b0 = 0; b0 < B; b0 += 32) {
+    const int b = b0 + lane;
+    const int n = b < B ? max(a.q_starts[b + 1] - a.q_starts[b], 0) : 0;
+    const int t = (n * G + kPpRows - 1) / kPpRows;
+    int incl = t;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, incl > want);
+    if (past) {
+      const int src = __ffs(past) - 1;
+      seq = b0 + src;
+      tile = want - __shfl_sync(0xffffffffu, incl - t, src);
+      return true;
+    }
+    want -= __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return false;
+}
+
+// What the rows of an item are: first token, positions, and the keys that any of them sees.
+struct PpItem {
+  int tok0, n_rows, pos0, len, asked;  // row r: token tok0 + r / G at position pos0 + r / G
+  Visible v;
+};
+__device__ __forceinline__ PpItem pp_rows(const PAttnArgs& a, int G, int seq, int tile) {
+  PpItem it;
+  const int s0 = a.q_starts[seq], n = a.q_starts[seq + 1] - s0;
+  it.asked = a.kv.seq_lens[seq];
+  it.len = paged_len(a.kv, seq);
+  it.tok0 = s0;
+  it.pos0 = it.asked - n;
+  it.n_rows = n * G;
+  const int r0 = tile * kPpRows, r1 = min(r0 + kPpRows, it.n_rows);
+  const int plo = it.pos0 + r0 / G, phi = it.pos0 + (r1 - 1) / G;
+  Visible& v = it.v;
+  v.end = max(0, min(phi + 1, it.len));
+  v.lo = a.window > 0 ? max(0, plo + 1 - a.window) : 0;
+  v.ns = min(min(a.sinks, v.lo), v.end);
+  v.st = (v.ns + kPpKeys - 1) / kPpKeys;
+  v.w0 = max(v.lo / kPpKeys, v.st);
+  v.tiles = v.st + max(0, (v.end + kPpKeys - 1) / kPpKeys - v.w0);
+  return it;
+}
+// Bits 0 .. n - 1.
+__device__ __forceinline__ unsigned pp_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+// Parts that an item's key tiles are really split into: at least two tiles each.
+__device__ __forceinline__ int pp_parts(int tiles, int splits) { return min(splits, max(1, tiles >> 1)); }
+
+// Bounded wait that gives up at once where another role already has.
+__device__ __forceinline__ bool pp_wait(unsigned long long* bar, unsigned parity, volatile int* failed) {
+  if (tc_mbar_test(bar, parity)) return true;
+  const unsigned long long t0 = tc_now();
+  while (!tc_mbar_test(bar, parity)) {
+    if (*failed) return false;
+    if (tc_now() - t0 > kTcWaitNs) {
+      *failed = 1;
+      return false;
+    }
+  }
+  return true;
+}
+__device__ __forceinline__ void pp_arrive(unsigned long long* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc_smem(bar)) : "memory");
+}
+
+// B operand with its N index (dims) contiguous: 64-dim rows of 128 bytes, 128-byte swizzle; the
+// next 64 dims kPpTileBytes / 2 on, the next 8 keys 1024 bytes on.
+__device__ __forceinline__ unsigned long long umma_desc_mn_sw128(unsigned smem_addr) {
+  return (unsigned long long)((smem_addr >> 4) & 0x3FFFu) | ((unsigned long long)(kPpTileBytes / 2 >> 4) << 16) |
+         ((unsigned long long)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// f32 accumulator, 16-bit operands (f16 or bf16), B with N contiguous where mn.
+template <typename T>
+__device__ __forceinline__ unsigned pp_idesc(bool mn) {
+  const unsigned fmt = sizeof(T) == 2 && !std::is_same<T, __half>::value ? 1u : 0u;
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | (mn ? 1u << 16 : 0u) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+}
+// D += A B with A in TMEM.
+__device__ __forceinline__ void umma_f16_ts(unsigned d_tmem, unsigned a_tmem, unsigned long long b, unsigned idesc,
+                                            bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b), "r"(idesc), "r"((unsigned)accumulate)
+      : "memory");
+}
+#define PP_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+// 64 consecutive TMEM columns of this warp's lanes.
+__device__ __forceinline__ void tmem_ld64(unsigned taddr, unsigned* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : PP_R8(r, 0), PP_R8(r, 8), PP_R8(r, 16), PP_R8(r, 24), PP_R8(r, 32), PP_R8(r, 40), PP_R8(r, 48), PP_R8(r, 56)
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(unsigned taddr, unsigned* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : PP_R8(r, 0), PP_R8(r, 8)
+      : "r"(taddr)
+      : "memory");
+}
+#undef PP_R8
+#define PP_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+__device__ __forceinline__ void tmem_st16(unsigned taddr, const unsigned* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::PP_W8(r, 0),
+      PP_W8(r, 8), "r"(taddr)
+      : "memory");
+}
+#undef PP_W8
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <typename T>
+__device__ __forceinline__ unsigned pack2(float x, float y);
+template <>
+__device__ __forceinline__ unsigned pack2<__half>(float x, float y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+template <>
+__device__ __forceinline__ unsigned pack2<__nv_bfloat16>(float x, float y) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+
+template <typename T, bool SPLIT>
+__global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_constant__ PPromptArgs pa) {
+  const PAttnArgs& a = pa.a;
+  constexpr int S = pp_slots<SPLIT>();
+  constexpr int kQTile = (SPLIT ? 2 : 1) * kPpTileBytes;  // hi (and lo) of 128 rows
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* qs =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* ring = qs + 2 * kQTile;
+  __shared__ unsigned long long full[S], raw, empty[S], s_full[2], p_full[2], o_done[2], drain;
+  __shared__ unsigned bad_rows[8];  // of key tile j: bit i set where 16-key chunk i has no usable page
+  __shared__ unsigned tmem_base;
+  __shared__ int failed;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int kvh = a.kv.kv_heads, G = a.q_heads / kvh;
+  const int g = blockIdx.x % kvh, z = (blockIdx.x / kvh) % pa.splits, item = blockIdx.x / (kvh * pa.splits);
+  pdl_wait();
+  pdl_trigger();
+  int seq = 0, tile = 0;
+  if (!pp_item(a, G, item, seq, tile)) return;
+  const PpItem it = pp_rows(a, G, seq, tile);
+  if (it.asked > it.len && it.asked > 0 && tid == 0) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
+  const int parts = pp_parts(it.v.tiles, pa.splits);
+  if (z >= parts) return;
+  const int t0 = (int)((long long)it.v.tiles * z / parts), nk = (int)((long long)it.v.tiles * (z + 1) / parts) - t0;
+  const int row0 = tile * kPpRows;
+  const int halves = it.n_rows - row0 > 128 ? 2 : 1;
+
+  // this thread's row (softmax threads)
+  const int row = row0 + tid;
+  const int tok = row / G, hs = row - tok * G;
+  const bool live = tid < kPpRows && row < it.n_rows && (unsigned)(it.tok0 + tok) < (unsigned)a.rows;
+
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(&tmem_base)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid == 0) {
+    for (int i = 0; i < S; ++i) {
+      tc_mbar_init(&full[i]);
+      tc_mbar_init(&empty[i]);
+    }
+    tc_mbar_init(&raw);
+    tc_mbar_init(&drain);
+    for (int i = 0; i < 2; ++i) {
+      tc_mbar_init(&s_full[i]);
+      tc_mbar_init(&o_done[i]);
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 128;" ::"r"(tc_smem(&p_full[i])) : "memory");
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    failed = 0;
+  }
+  // Q: one row per thread, K-major with the 128-byte swizzle; dead rows are zero. A negative scale
+  // changes the sign of q, so that the softmax always has a positive one.
+  if (tid < kPpRows && nk > 0) {
+    const int r = tid & 127;
+    unsigned char* dst = qs + (tid >> 7) * kQTile + r * 128;
+    const long long base = (long long)(it.tok0 + (live ? tok : 0)) * a.q_stride + ((long long)g * G + hs) * kHeadDim;
+    if constexpr (SPLIT) {
+#pragma unroll 4
+      for (int c = 0; c < 16; ++c) {
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+        if (live) {
+          x = load4<float>(a.q, base + 8 * c);
+          y = load4<float>(a.q, base + 8 * c + 4);
+          if (a.scale < 0.0f) {
+            x = make_float4(-x.x, -x.y, -x.z, -x.w);
+            y = make_float4(-y.x, -y.y, -y.z, -y.w);
+          }
+        }
+        uint4 h, l;
+        split2<T>(x.x, x.y, h.x, l.x);
+        split2<T>(x.z, x.w, h.y, l.y);
+        split2<T>(y.x, y.y, h.z, l.z);
+        split2<T>(y.z, y.w, h.w, l.w);
+        const unsigned off = (c >> 3) * (kPpTileBytes / 2) + (((c ^ r) & 7) << 4);
+        *reinterpret_cast<uint4*>(dst + off) = h;
+        *reinterpret_cast<uint4*>(dst + kPpTileBytes + off) = l;
+      }
+    } else {
+      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + base);
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        uint4 x = live ? src[c] : make_uint4(0, 0, 0, 0);
+        if (a.scale < 0.0f)
+          x = make_uint4(x.x ^ 0x80008000u, x.y ^ 0x80008000u, x.z ^ 0x80008000u, x.w ^ 0x80008000u);
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * (kPpTileBytes / 2) + (((c ^ r) & 7) << 4)) = x;
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const unsigned tmem = tmem_base;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPpRegsFew));
+  if (warp == 9 && nk > 0) {
+    // ---- copies: K and V tiles alternate through the ring ----
+    const int ps = 1 << a.kv.page_shift, box = min(ps, kPpKeys), boxes = kPpKeys / box;
+    unsigned raw_phase = 0;
+    int issued_to = -1;
+    bool ok = true;
+    for (int i = 0; i < 2 * nk && ok; ++i) {
+      const int j = i >> 1, slot = i % S;
+      const bool is_v = i & 1;
+      const int k0 = it.v.tile(t0 + j) * kPpKeys;
+      // lane n: the page of the n-th box, if any row of the CTA sees it
+      int page = -1;
+      const int p0 = k0 + lane * box;
+      const bool any = lane < boxes && p0 < it.v.end && (p0 + box > it.v.lo || p0 < it.v.ns);
+      if (any) page = paged_page(a.kv, seq, p0);
+      const unsigned seen = __ballot_sync(0xffffffffu, any), good = __ballot_sync(0xffffffffu, page >= 0);
+      if (i >= S) ok = pp_wait(&empty[slot], (unsigned)(i / S - 1) & 1u, &failed);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const bool partial = !(k0 + kPpKeys <= it.v.end && (k0 >= it.v.lo || k0 + kPpKeys <= it.v.ns)) || good != seen;
+      const bool clear = is_v && partial;
+      unsigned char* dst = ring + slot * kPpTileBytes;
+      unsigned long long* bar = clear ? &raw : &full[slot];
+      if (lane == 0) {
+        if (!is_v) {
+          unsigned bad = 0;
+          for (int n = 0; n < boxes; ++n)
+            if (((seen & ~good) >> n) & 1u) bad |= ((1u << (box / 16)) - 1u) << (n * (box / 16));
+          bad_rows[j & 7] = bad;
+          if (bad) paged_flag(a.kv, QD_PAGED_BAD_PAGE);
+        }
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc_smem(bar)),
+                     "r"(__popc(good) * box * 256)
+                     : "memory");
+      }
+      __syncwarp();
+      if (page >= 0) {
+        const int y = (page * kvh + g) * ps + (p0 & (ps - 1));
+        unsigned char* d = dst + lane * box * 128;
+        tma_load_2d(d, is_v ? &pa.tv : &pa.tk, 0, y, bar);
+        tma_load_2d(d + kPpTileBytes / 2, is_v ? &pa.tv : &pa.tk, 64, y, bar);
+      }
+      if (clear) {
+        ok = pp_wait(&raw, raw_phase, &failed);
+        ok = __all_sync(0xffffffffu, ok);
+        raw_phase ^= 1u;
+        for (int e = lane; e < kPpKeys * 16; e += 32) {
+          const int r = e >> 4, c = e & 15, pos = k0 + r;
+          const bool keep = it.v.at(pos) && ((good >> (r / box)) & 1u);
+          if (!keep) *reinterpret_cast<uint4*>(dst + (c >> 3) * (kPpTileBytes / 2) + r * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) pp_arrive(&full[slot]);
+      }
+      issued_to = i;
+    }
+    // nothing may still be landing when the CTA ends
+    for (int i = max(0, issued_to - S + 1); i <= issued_to; ++i)
+      (void)tc_mbar_wait(&full[i % S], (unsigned)(i / S) & 1u);
+  } else if (warp == 8 && nk > 0) {
+    // ---- MMA issue (one lane) ----
+    if (lane == 0) {
+      const unsigned id_s = pp_idesc<T>(false), id_o = pp_idesc<T>(true);
+      auto scores = [&](int t, int slot) {  // S_t = Q_t K^T
+        const unsigned qb = tc_smem(qs + t * kQTile), kb = tc_smem(ring + slot * kPpTileBytes);
+#pragma unroll
+        for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {
+            const unsigned off = (ks >> 2) * (kPpTileBytes / 2) + (ks & 3) * 32;
+            umma_f16(tmem + t * 128, umma_desc_k_sw128(qb + part * kPpTileBytes + off), umma_desc_k_sw128(kb + off), id_s,
+                     part > 0 || ks > 0);
+          }
+        umma_commit(&s_full[t]);
+      };
+      bool ok = pp_wait(&full[0], 0, &failed);
+      if (ok) {
+        tc_fence_after();
+        for (int t = 0; t < halves; ++t) scores(t, 0);
+        umma_commit(&empty[0]);
+      }
+      for (int j = 0; j < nk && ok; ++j) {
+        const int vi = 2 * j + 1, vs = vi % S, ki = 2 * j + 2, ks_slot = ki % S;
+        ok = pp_wait(&full[vs], (unsigned)(vi / S) & 1u, &failed);
+        if (ok && j + 1 < nk) ok = pp_wait(&full[ks_slot], (unsigned)(ki / S) & 1u, &failed);
+        for (int t = 0; t < halves && ok; ++t) {
+          ok = pp_wait(&p_full[t], (unsigned)j & 1u, &failed);
+          if (!ok) break;
+          tc_fence_after();
+          const unsigned vb = tc_smem(ring + vs * kPpTileBytes);
+#pragma unroll
+          for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks)
+              umma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + part * 64 + ks * 8, umma_desc_mn_sw128(vb + ks * 2048),
+                          id_o, j > 0 || part > 0 || ks > 0);
+          umma_commit(&o_done[t]);
+          if (t == halves - 1) umma_commit(&empty[vs]);
+          if (j + 1 < nk) {
+            scores(t, ks_slot);
+            if (t == halves - 1) umma_commit(&empty[ks_slot]);
+          }
+        }
+      }
+      if (!ok) {  // given up: let what was issued finish before the CTA ends
+        umma_commit(&drain);
+        (void)tc_mbar_wait(&drain, 0);
+      }
+    }
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPpRegsMany));
+  if ((warp >> 2) < halves && nk > 0) {
+    // ---- softmax: one row per thread ----
+    float m = -INFINITY, l = 0.0f;
+    const int t = warp >> 2;
+    const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
+    const unsigned ts = tmem + t * 128 + lanes, to = tmem + 256 + t * 128 + lanes;
+    const float c = fabsf(a.scale) * kLog2e;
+    const int p = live ? it.pos0 + tok : -1;
+    const int pmax = min(p, it.len - 1);
+    const int phi = a.window > 0 ? p - a.window : -2;  // keys up to here are hidden, unless sinks
+    // positions of the warp's first and last live rows
+    const unsigned lv = __ballot_sync(0xffffffffu, live);
+    const int pw0 = __shfl_sync(0xffffffffu, p, 0), pw1 = __shfl_sync(0xffffffffu, p, lv ? 31 - __clz(lv) : 0);
+    bool ok = true;
+    for (int j = 0; j < nk; ++j) {
+      ok = pp_wait(&s_full[t], (unsigned)j & 1u, &failed);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      unsigned sr[128];
+      tmem_ld64(ts, sr);
+      tmem_ld64(ts + 64, sr + 64);
+      const int k0 = it.v.tile(t0 + j) * kPpKeys;
+      const unsigned bad = bad_rows[j & 7];
+      const bool inside = lv == 0xffffffffu && bad == 0 && k0 + kPpKeys - 1 <= min(pw0, it.len - 1) &&
+                          (a.window == 0 || k0 > pw1 - a.window || k0 + kPpKeys <= a.sinks);
+      if (!inside) {
+        // bit i of a word: key k0 + 32 w + i is visible to this row
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int at = k0 + 32 * w;
+          unsigned see = pp_below(pmax + 1 - at) & (~pp_below(phi + 1 - at) | pp_below(a.sinks - at));
+          if ((bad >> (2 * w)) & 1u) see &= 0xffff0000u;
+          if ((bad >> (2 * w)) & 2u) see &= 0x0000ffffu;
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!((see >> i) & 1u)) sr[32 * w + i] = 0xff800000u;
+        }
+      }
+      float mx[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx[i] = fmaxf(__uint_as_float(sr[i]), __uint_as_float(sr[i + 4]));
+#pragma unroll
+      for (int i = 8; i < 128; i += 4)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(sr[i + e]));
+      const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+      if (__any_sync(0xffffffffu, mt > m + kPpLag)) {
+        // each row by its own maximum (a factor of 1 where it has not moved), so that a row's result
+        // does not depend on the rows beside it
+        const float mn = mt > m + kPpLag ? mt : m;
+        const float f = m == -INFINITY ? 0.0f : exp2_fast(m - mn);
+        m = mn;
+        l *= f;
+        if (j > 0) {  // the product of the tile before must have reached O
+          ok = pp_wait(&o_done[t], (unsigned)(j - 1) & 1u, &failed);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int h = 0; h < 8; ++h) {
+            unsigned o[16];
+            tmem_ld16(to + 16 * h, o);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st16(to + 16 * h, o);
+          }
+        }
+      }
+      const float ref = m == -INFINITY ? 0.0f : kPpShift - m;
+      float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {  // 32 keys: 16 packed columns
+        unsigned w[16], wl[SPLIT ? 16 : 1];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float s0 = __uint_as_float(sr[32 * h + 2 * i]), s1 = __uint_as_float(sr[32 * h + 2 * i + 1]);
+          float2 e = __ffma2_rn(make_float2(s0, s1), make_float2(c, c), make_float2(ref, ref));
+          e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+          sum = __fadd2_rn(sum, e);
+          if constexpr (SPLIT) split2<T>(e.x, e.y, w[i], wl[i]);
+          else w[i] = pack2<T>(e.x, e.y);
+        }
+        tmem_st16(ts + 16 * h, w);
+        if constexpr (SPLIT) tmem_st16(ts + 64 + 16 * h, wl);
+      }
+      l += sum.x + sum.y;
+      tmem_wait_st();
+      tc_fence_before();
+      pp_arrive(&p_full[t]);
+    }
+    if (ok) {
+      ok = pp_wait(&o_done[t], (unsigned)(nk - 1) & 1u, &failed);
+      ok = __all_sync(0xffffffffu, ok);
+    }
+    if (ok) {
+      tc_fence_after();
+      const bool whole = parts == 1;
+      const float f = whole ? inv_sum(l) : 1.0f;
+      const long long prow = (((long long)item * kvh + g) * pa.splits + z) * kPpRows + tid;
+      const long long base = (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + hs) * kHeadDim;
+      if (!whole) pa.pml[prow] = make_float2(m, l);
+#pragma unroll 1
+      for (int h = 0; h < 4; ++h) {
+        float o[32];
+        tmem_ld32(to + 32 * h, o);
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(pa.po + prow * kHeadDim + 32 * h + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        } else if (live) {
+          if constexpr (SPLIT) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(static_cast<float*>(a.y) + base + 32 * h + i) =
+                  make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+              *reinterpret_cast<uint4*>(static_cast<T*>(a.y) + base + 32 * h + i) =
+                  make_uint4(pack2<T>(o[i] * f, o[i + 1] * f), pack2<T>(o[i + 2] * f, o[i + 3] * f),
+                             pack2<T>(o[i + 4] * f, o[i + 5] * f), pack2<T>(o[i + 6] * f, o[i + 7] * f));
+          }
+        }
+      }
+    }
+  }
+  }
+  if (nk == 0 && live) {  // no key is visible to any row
+    const long long base = (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + hs) * kHeadDim;
+    for (int i = 0; i < kHeadDim; i += 4) store4(a.y, base + i, a.dtype, make_float4(0.f, 0.f, 0.f, 0.f));
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && failed) paged_flag(a.kv, QD_PAGED_TIMEOUT);
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// Adds the parts of rows whose key tiles were split. One warp per row; grid: items * kv_heads * 32.
+__global__ void __launch_bounds__(256) k_paged_prompt_join(const __grid_constant__ PPromptArgs pa) {
+  const PAttnArgs& a = pa.a;
+  const int kvh = a.kv.kv_heads, G = a.q_heads / kvh, lane = threadIdx.x & 31;
+  const int r = (blockIdx.x & 31) * 8 + (threadIdx.x >> 5), ig = blockIdx.x >> 5, g = ig % kvh, item = ig / kvh;
+  pdl_wait();
+  pdl_trigger();
+  int seq = 0, tile = 0;
+  if (!pp_item(a, G, item, seq, tile)) return;
+  const PpItem it = pp_rows(a, G, seq, tile);
+  const int parts = pp_parts(it.v.tiles, pa.splits), row = tile * kPpRows + r, tok = row / G;
+  if (parts == 1 || row >= it.n_rows || (unsigned)(it.tok0 + tok) >= (unsigned)a.rows) return;
+  const long long p0 = ((long long)item * kvh + g) * pa.splits * kPpRows + r;
+  const float2 ml = lane < parts ? pa.pml[p0 + (long long)lane * kPpRows] : make_float2(-INFINITY, 0.0f);
+  const float M = warp_max(ml.x);
+  const float f = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - M);
+  const float L = warp_sum(ml.y * f);
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int k = 0; k < parts; ++k) {
+    const float fk = __shfl_sync(0xffffffffu, f, k);
+    const float4 x = *reinterpret_cast<const float4*>(pa.po + (p0 + (long long)k * kPpRows) * kHeadDim + 4 * lane);
+    y = make_float4(y.x + x.x * fk, y.y + x.y * fk, y.z + x.z * fk, y.w + x.w * fk);
+  }
+  const float zf = inv_sum(L);
+  store4(a.y, (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + row % G) * kHeadDim + 4 * lane, a.dtype,
+         make_float4(y.x * zf, y.y * zf, y.z * zf, y.w * zf));
+}
+
+}  // namespace qd
