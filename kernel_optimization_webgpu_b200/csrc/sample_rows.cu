@@ -8,19 +8,23 @@
 // summed as 64-bit integers: exact, so the answer does not depend on the order of summation, and
 // a border is misplaced only where the random number falls within about 2^-40 of it.
 //
-// One thread-block cluster per row. The row is read once, into the CTAs' shared memory; what is
-// bound is then the latency of a few passes over it, so the work of a pass is spread over the
-// cluster and the passes are few:
+// One thread-block cluster per row. The row is read once, into the CTAs' shared memory; what bounds
+// it is then the latency of a few passes and cluster barriers and, with many rows, the
+// instructions per token, so the passes are few and the work of each is spread over the cluster:
 //  1. maximum and minimum;
-//  2. histogram over kRowsBins equal steps of value between them (or 31 T nats, beyond which a
-//     weight is zero): counts, and sums of weights where a cut needs them, by integer atomics in
-//     shared memory. Steps are monotone in the value, so every border lies in a known step;
-//  3. the steps that hold all tokens that can be kept, when these are at most kRowsList, are
-//     gathered into the first CTA, sorted, and all cuts and the draw are done there.
-// Otherwise (a large nucleus, the whole vocabulary) each border is resolved alone: the tokens of
-// its step are gathered and sorted, a step with too many is cut into finer ones by key, and where
-// all of them are equal their order is their index. The first CTA of the cluster leads: it
-// tells the others what to do next and ends them.
+//  2. histogram over kRowsBins equal steps of value between them (or 32 T nats, beyond which a
+//     weight is zero): counts, and the sums of the places within a step, by 32-bit atomics in
+//     shared memory. Steps are monotone in the value. Count times the weight at the mean place
+//     is a step's sum of weights to within s^2 / 8 + 1e-5 of itself, s the step in nats (the
+//     exponential's curvature over one step, and f32 roundings), which tells for every border
+//     in which few steps it must lie;
+//  3. the tokens of those steps are gathered into the first CTA; in the same pass the exact
+//     weights of all tokens, and of those above each such range, are summed in registers. The
+//     leader sorts the gathered ones and finds the borders exactly.
+// Where a range holds more than kRowsList tokens (long classes of equal values, a large top-k), each border
+// is resolved alone: exact sums by step, the tokens of one step gathered and sorted, a step with
+// too many cut into finer ones by key, and where all of them are equal their order is their
+// index. The first CTA of the cluster leads: it tells the others what to do next and ends them.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -41,13 +45,15 @@ constexpr int kRowsThreads = 512;
 constexpr int kRowsWarps = kRowsThreads / 32;
 constexpr int kRowsMaxVocab = 393216;
 constexpr int kRowsMaxCluster = 8;
-constexpr int kRowsBins = 1024;   // two a thread of the leader
+constexpr int kRowsMaxPer = kRowsMaxVocab / kRowsMaxCluster;  // tokens a CTA takes: its 32-bit sums of 16 bits fit
+constexpr int kRowsBins = 2048;       // four a thread of the leader; 1024 left 40 of 64 rows above a list's size
+constexpr int kRowsExact = kRowsBins / 2;  // bins of an exact histogram (twice the words a bin)
 constexpr int kRowsList = 1024;
 constexpr double kRowsOne = 17592186044416.0;  // weight 1 = 2^44
 
 struct SampleRowsArgs {
   const void* logits;
-  int vocab, per;  // per: tokens a CTA holds
+  int vocab, per;  // per: tokens a CTA takes, a multiple of 8
   long long row_stride;
   const float* temperature;
   const int* top_k;
@@ -58,8 +64,9 @@ struct SampleRowsArgs {
   float* logprobs;
 };
 
-// Larger value, larger key.
+// Larger value, larger key; NaN lowest.
 __device__ __forceinline__ uint32_t row_key(float v) {
+  if (v != v) return 0u;
   const uint32_t u = __float_as_uint(v + 0.0f);  // -0 as +0
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
@@ -71,10 +78,12 @@ __device__ __forceinline__ float row_key_value(uint32_t k) {
 enum RowsOp : int { kOpEnd = 0, kOpHist, kOpGather, kOpRange, kOpMass, kOpCount, kOpPick };
 struct RowsCmd {
   int op;
-  int by_bin;         // members: bins [lo, hi] of the first histogram; else keys [lo, hi]
+  int by_bin;         // members: bins [lo, hi] (2: of the exact histogram), else keys [lo, hi]
   uint32_t lo, hi;
   int shift;          // kOpHist by key: bin = (hi - key) >> shift
   int rank, n;        // kOpPick: CTA `rank` finds its n-th member by index
+  int sums;           // kOpGather: also the weights of all tokens, and of those in bins below lo and lo2
+  uint32_t lo2, hi2;  // kOpGather by bin: a second range of members (lo2 > hi2: none)
 };
 // A prefix of the row's order: every key above `key` and the first `ties` of those equal to it.
 struct RowsPrefix {
@@ -83,18 +92,24 @@ struct RowsPrefix {
   u64 mass;
 };
 
+// A bin, its tokens, and the tokens and weight before it.
+struct RowsAt {
+  int bin, count, before;
+  u64 mass;
+};
+
 struct RowsShared {
   RowsCmd cmd;
   float mx[kRowsMaxCluster], mn[kRowsMaxCluster];
   u64 part[kRowsMaxCluster];      // per-CTA sums for the leader
+  u64 above[3][kRowsMaxCluster];  // kOpGather with sums: all, below lo, below lo2
+  int taken;                      // entries of this CTA's own list
   uint32_t key_min, key_max;      // leader
   int found;                      // leader: an index
-  int listed;                     // leader: entries of the list
   u64 red[kRowsWarps];
-  u64 pick_mass;                  // results of searches over the leader's threads
-  int pick_bin, pick_at;
-  u64 pick_base;
-  int pick_count;
+  RowsAt at[4];                   // results of searches over the leader's threads
+  int pick_at, upto;
+  u64 whole;
 };
 
 template <typename T>
@@ -108,22 +123,74 @@ __device__ __forceinline__ float rows_value(const void* p, long long i) {
 struct RowsCta {
   cg::cluster_group cl;
   RowsShared* sh;
-  float* val;      // [per], NaN as -inf
-  uint4* hist;     // [kRowsBins] {count, weights in three 32-bit sums of 16 + 14 + 14 bits}
+  float* val;       // this CTA's tokens, filled up to a multiple of 4 with NaN
+  uint32_t* hist;   // [2][kRowsBins]: counts, places; or [4][kRowsExact]: counts, and weights in three sums
+  const double* pow2;  // 2^(i / 128)
   u64* list;       // leader: {~key, index}
-  int n, base, C, rank;
-  float vmax, scale;
-  double inv_t;
+  int n, base, C, lg, rank;  // C = 1 << lg CTAs
+  float vmax, scale, range;  // scale: places per unit of value
+  double inv_t, z_scale;  // 1 / T and 128 log2(e) / T
+  float step;             // width of a bin in the weight's logarithm to base 2
 
-  __device__ __forceinline__ int bin(float v) const {  // ascending as v descends
-    return v == -INFINITY ? kRowsBins - 1 : (int)fminf((vmax - v) * scale, (float)(kRowsBins - 1));
+  // A value's place: 4096ths of a bin below the maximum, rounded by an addition of 2^23 (conversions
+  // run at an eighth of its rate). Ascending as v descends. kNoPlace for what has no weight: NaN,
+  // -inf, beyond the range; those are the last bin.
+  static constexpr uint32_t kNoPlace = (kRowsBins - 1) << 12;
+  __device__ __forceinline__ uint32_t place(float v) const {
+    const float d = vmax - v;
+    const uint32_t u = __float_as_uint(fminf(fmaf(d, scale, 8388608.0f), 8388608.0f + (float)(kNoPlace - 1))) & 0x7fffffu;
+    return d <= range ? u : kNoPlace;
+  }
+  __device__ __forceinline__ int bin(float v) const { return (int)(place(v) >> 12); }
+  __device__ __forceinline__ int exact_bin(float v) const { return (int)(place(v) >> 13); }
+  // exp((v - v_max) / T) * 2^44, rounded: with z = 128 log2(e) (v - v_max) / T = 128 e + i + r, it is
+  // 2^(44 + e) 2^(i / 128) 2^(r / 128), |r| <= 1 / 2, the last factor by its Taylor sum to the fourth
+  // power (the rest is below 2^-49): table-driven, after Tang, ACM TOMS 15 (1989). Roundings to
+  // an integer are additions of 1.5 * 2^52 and 2^52.
+  __device__ __forceinline__ double raw_weight(float v) const {  // before the last rounding, v within the range
+    const double d = (double)v - (double)vmax;
+    const double near = fma(d, z_scale, 6755399441055744.0);
+    const int k = __double2loint(near);
+    const double r = fma(d, z_scale, 6755399441055744.0 - near);
+    constexpr double c = 0.6931471805599453 / 128.0;
+    const double p = fma(fma(fma(fma(c * c * c * c / 24.0, r, c * c * c / 6.0), r, c * c / 2.0), r, c), r, 1.0);
+    const double w = p * pow2[k & 127];
+    return __hiloint2double(__double2hiint(w) + (((k >> 7) + 44) << 20), __double2loint(w));
   }
   __device__ __forceinline__ u64 weight(float v) const {
-    return v == -INFINITY ? 0ull : (u64)__double2ll_rn(exp(((double)v - (double)vmax) * inv_t) * kRowsOne);
+    if (!(vmax - v <= range)) return 0ull;
+    return (u64)__double_as_longlong(raw_weight(v) + 4503599627370496.0) & 0xfffffffffffffull;
+  }
+  // f(values, index of the first) for every four tokens of this CTA, the last ones filled up with NaN
+  // (which has no weight and sorts last), two loads before their work.
+  template <typename F>
+  __device__ __forceinline__ void each4(F&& f) const {
+    int i = 4 * threadIdx.x;
+    for (; i + 4 * kRowsThreads < n; i += 8 * kRowsThreads) {
+      const float4 x = *reinterpret_cast<const float4*>(val + i);
+      const float4 y = *reinterpret_cast<const float4*>(val + i + 4 * kRowsThreads);
+      const float v[4] = {x.x, x.y, x.z, x.w}, w[4] = {y.x, y.y, y.z, y.w};
+      f(v, i);
+      f(w, i + 4 * kRowsThreads);
+    }
+    if (i < n) {
+      const float4 x = *reinterpret_cast<const float4*>(val + i);
+      const float v[4] = {x.x, x.y, x.z, x.w};
+      f(v, i);
+    }
+  }
+  // f(value, index) for every token.
+  template <typename F>
+  __device__ __forceinline__ void each(F&& f) const {
+    each4([&](const float (&v)[4], int i) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i + k < n) f(v[k], i + k);
+    });
   }
   __device__ __forceinline__ bool member(const RowsCmd& c, float v) const {
     if (c.by_bin) {
-      const uint32_t b = (uint32_t)bin(v);
+      const uint32_t b = (uint32_t)(c.by_bin == 2 ? exact_bin(v) : bin(v));
       return b >= c.lo && b <= c.hi;
     }
     const uint32_t k = row_key(v);
@@ -141,41 +208,76 @@ struct RowsCta {
     return t;
   }
 
-  // Histogram of the members; afterwards this CTA's share of the bins holds the whole row's sums
-  // as {count, weight low, weight high, -}.
-  __device__ void histogram(const RowsCmd& c, bool mass) {
-    for (int i = threadIdx.x; i < kRowsBins; i += kRowsThreads) hist[i] = make_uint4(0, 0, 0, 0);
+  // Histogram of the members; afterwards this CTA's share of the bins holds the whole row's sums:
+  // the count, and the sum of weights (kExact) or of places (kPlaces) as two words.
+  enum HistKind : int { kCounts, kPlaces, kExact };
+  __device__ void histogram(const RowsCmd& c, HistKind kind) {
+    const int nb = kind == kExact ? kRowsExact : kRowsBins;
+    for (int i = threadIdx.x; i < kRowsBins / 2; i += kRowsThreads)
+      reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kRowsThreads) {
-      const float v = val[i];
-      int b;
-      if (c.by_bin) {
-        b = bin(v);
-      } else {
-        const uint32_t k = row_key(v);
-        if (k < c.lo || k > c.hi) continue;
-        b = (int)((c.hi - k) >> c.shift);
-      }
-      atomicAdd(&hist[b].x, 1u);
-      if (mass) {
+    if (kind == kCounts) {
+      each4([&](const float (&v)[4], int) {
+        int b[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) b[k] = bin(v[k]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) atomicAdd(&hist[b[k]], 1u);
+      });
+    } else if (kind == kPlaces) {
+      each4([&](const float (&v)[4], int) {
+        uint32_t u[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) u[k] = place(v[k]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          atomicAdd(&hist[u[k] >> 12], 1u);
+          atomicAdd(&hist[kRowsBins + (u[k] >> 12)], u[k] & 4095u);
+        }
+      });
+    } else {
+      each([&](float v, int) {
+        int b;
+        if (c.by_bin) {
+          b = exact_bin(v);
+        } else {
+          const uint32_t k = row_key(v);
+          if (k < c.lo || k > c.hi) return;
+          b = (int)((c.hi - k) >> c.shift);
+        }
+        atomicAdd(&hist[b], 1u);
         const u64 w = weight(v);
-        atomicAdd(&hist[b].y, (uint32_t)w & 0xffffu);
-        atomicAdd(&hist[b].z, (uint32_t)(w >> 16) & 0x3fffu);
-        atomicAdd(&hist[b].w, (uint32_t)(w >> 30));
-      }
+        const uint32_t low = (uint32_t)w & 0x3fffu, mid = (uint32_t)(w >> 14) & 0x3fffu, high = (uint32_t)(w >> 28);
+        if (low) atomicAdd(&hist[nb + b], low);
+        if (mid) atomicAdd(&hist[2 * nb + b], mid);
+        if (high) atomicAdd(&hist[3 * nb + b], high);
+      });
     }
     cl.sync();
-    const int share = kRowsBins / C;
+    const int share = nb >> lg;
     for (int i = threadIdx.x; i < share; i += kRowsThreads) {
       const int b = rank * share + i;
+      uint32_t h[4][kRowsMaxCluster];
+      const int fields = kind == kCounts ? 1 : kind == kPlaces ? 2 : 4;
+#pragma unroll
+      for (int f = 0; f < 4; ++f)
+#pragma unroll
+        for (int r = 0; r < kRowsMaxCluster; ++r)  // all loads in flight together
+          h[f][r] = f < fields && r < C ? cl.map_shared_rank(hist, r)[f * nb + b] : 0u;
       uint32_t count = 0;
       u64 w = 0;
-      for (int r = 0; r < C; ++r) {
-        const uint4 h = *cl.map_shared_rank(&hist[b], r);
-        count += h.x;
-        w += (u64)h.y + ((u64)h.z << 16) + ((u64)h.w << 30);
+#pragma unroll
+      for (int r = 0; r < kRowsMaxCluster; ++r) {
+        count += h[0][r];
+        w += (u64)h[1][r] + ((u64)h[2][r] << 14) + ((u64)h[3][r] << 28);
       }
-      hist[b] = make_uint4(count, (uint32_t)w, (uint32_t)(w >> 32), 0);
+      hist[b] = count;
+      if (kind == kPlaces) {  // (a row's sum of places fits: at most 393216 times 4095)
+        hist[kRowsBins + b] = (uint32_t)w;
+      } else if (kind == kExact) {
+        hist[nb + b] = (uint32_t)w;
+        hist[2 * nb + b] = (uint32_t)(w >> 32);
+      }
     }
   }
 
@@ -184,29 +286,71 @@ struct RowsCta {
     RowsShared* lead = cl.map_shared_rank(sh, 0);
     const int lane = threadIdx.x & 31;
     if (c.op == kOpHist) {
-      histogram(c, true);
-    } else if (c.op == kOpGather) {
-      u64* out = cl.map_shared_rank(list, 0);
-      for (int i0 = 0; i0 < n; i0 += kRowsThreads) {
-        const int i = i0 + threadIdx.x;
-        const float v = i < n ? val[i] : 0.0f;
-        const bool in = i < n && member(c, v);
-        const unsigned who = __ballot_sync(0xffffffffu, in);
-        if (who) {
-          int at = 0;
-          if (lane == 0) at = atomicAdd(&lead->listed, __popc(who));
-          at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
-          if (in && at < kRowsList) out[at] = ((u64)~row_key(v) << 32) | (unsigned)(base + i);
+      histogram(c, kExact);
+    } else if (c.op == kOpGather) {  // into this CTA's own list; the leader collects them
+      if (threadIdx.x == 0) sh->taken = 0;
+      __syncthreads();
+      auto keep = [&](float v, int i) {
+        const int at = atomicAdd(&sh->taken, 1);
+        if (at < kRowsList) list[at] = ((u64)~row_key(v) << 32) | (unsigned)(base + i);
+      };
+      if (c.sums) {  // by bin
+        // Each thread adds at most 96 weights below 2^45 to 2^52: additions there round every weight to an
+        // integer and are exact otherwise.
+        double sum[3] = {4503599627370496.0, 4503599627370496.0, 4503599627370496.0};
+        const uint32_t lo = c.lo << 12, span = ((c.hi + 1) << 12) - lo, lo2 = c.lo2 << 12;
+        const uint32_t span2 = c.lo2 <= c.hi2 ? ((c.hi2 + 1) << 12) - lo2 : 0u;
+        each4([&](const float (&v)[4], int i) {
+          bool any = false;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t u = place(v[k]);
+            const double w = u < kNoPlace ? raw_weight(v[k]) : 0.0;
+            sum[0] += w;
+            sum[1] += u < lo ? w : 0.0;
+            if (span2) sum[2] += u < lo2 ? w : 0.0;
+            any = any || u - lo < span || u - lo2 < span2;
+          }
+          if (any) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t u = place(v[k]);
+              if ((u - lo < span || u - lo2 < span2) && i + k < n) keep(v[k], i + k);
+            }
+          }
+        });
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          const u64 all = block_sum64((u64)__double_as_longlong(sum[k]) & 0xfffffffffffffull);
+          if (threadIdx.x == 0) lead->above[k][rank] = all;
         }
+      } else if (c.by_bin == 1) {
+        const uint32_t lo = c.lo << 12, span = ((c.hi + 1) << 12) - lo;
+        each4([&](const float (&v)[4], int i) {
+          bool in[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) in[k] = place(v[k]) - lo < span;
+          if (in[0] || in[1] || in[2] || in[3]) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (in[k] && i + k < n) keep(v[k], i + k);
+          }
+        });
+      } else {
+        each([&](float v, int i) {
+          if (member(c, v)) keep(v, i);
+        });
       }
+      __syncthreads();
+      if (threadIdx.x == 0) lead->part[rank] = (u64)min(sh->taken, kRowsList);
     } else if (c.op == kOpRange) {
       uint32_t lo = 0xffffffffu, hi = 0u;
-      for (int i = threadIdx.x; i < n; i += kRowsThreads)
-        if (member(c, val[i])) {
-          const uint32_t k = row_key(val[i]);
-          lo = min(lo, k);
-          hi = max(hi, k);
+      each([&](float v, int) {
+        if (member(c, v)) {
+          lo = min(lo, row_key(v));
+          hi = max(hi, row_key(v));
         }
+      });
       lo = __reduce_min_sync(0xffffffffu, lo);
       hi = __reduce_max_sync(0xffffffffu, hi);
       if (lane == 0 && lo <= hi) {
@@ -215,8 +359,9 @@ struct RowsCta {
       }
     } else if (c.op == kOpMass || c.op == kOpCount) {
       u64 s = 0;
-      for (int i = threadIdx.x; i < n; i += kRowsThreads)
-        if (member(c, val[i])) s += c.op == kOpMass ? weight(val[i]) : 1ull;
+      each([&](float v, int) {
+        if (member(c, v)) s += c.op == kOpMass ? weight(v) : 1ull;
+      });
       s = block_sum64(s);
       if (threadIdx.x == 0) lead->part[rank] = s;
     } else if (c.op == kOpPick && c.rank == rank) {
@@ -245,13 +390,15 @@ struct RowsCta {
   __device__ void command(const RowsCmd& c) {
     __syncthreads();
     if ((int)threadIdx.x < C) *cl.map_shared_rank(&sh->cmd, threadIdx.x) = c;
-    if (threadIdx.x == 0 && c.op == kOpGather) sh->listed = 0;
     if (threadIdx.x == 0 && c.op == kOpRange) {
       sh->key_min = 0xffffffffu;
       sh->key_max = 0u;
     }
+    if (c.op == kOpEnd) {  // nothing more passes between the CTAs: the leader need not wait
+      (void)cl.barrier_arrive();
+      return;
+    }
     cl.sync();
-    if (c.op == kOpEnd) return;
     perform(c);
     cl.sync();
   }
@@ -262,7 +409,7 @@ struct RowsCta {
     return s;
   }
   __device__ int index_of(uint32_t key, int nth) {  // the nth token (from 0) of that key
-    RowsCmd c{kOpCount, 0, key, key, 0, 0, 0};
+    RowsCmd c{kOpCount, 0, key, key, 0, 0, 0, 0, 1, 0};
     command(c);
     c.op = kOpPick;
     c.n = nth;
@@ -271,23 +418,39 @@ struct RowsCta {
     return sh->found;
   }
 
-  // This thread's two bins of the reduced histogram, and inclusive running sums at their ends.
+  // This thread's bins of the reduced histogram (four neighbours; two of an exact one), and running
+  // sums up to and with each. Weights are exact after kExact, estimates after kPlaces.
   struct Bins {
-    uint32_t count[2], run[2];
-    u64 mass[2], mrun[2];
+    int per;
+    uint32_t count[4], run[4];
+    u64 mass[4], mrun[4];
   };
-  __device__ Bins read_bins() {
+  __device__ Bins read_bins(HistKind kind) {
     Bins b;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nb = kind == kExact ? kRowsExact : kRowsBins;
+    b.per = kind == kExact ? 2 : 4;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int i = 2 * threadIdx.x + e;
-      const uint4 h = *cl.map_shared_rank(&hist[i], i / (kRowsBins / C));
-      b.count[e] = h.x;
-      b.mass[e] = (u64)h.y | ((u64)h.z << 32);
+    for (int e = 0; e < 4; ++e) {
+      b.count[e] = 0;
+      b.mass[e] = 0;
+      if (e >= b.per) continue;
+      const int i = b.per * threadIdx.x + e;
+      const uint32_t* h = cl.map_shared_rank(hist, i / (nb >> lg)) + i;
+      b.count[e] = h[0];
+      if (kind == kExact) {
+        b.mass[e] = (u64)h[nb] | ((u64)h[2 * nb] << 32);
+      } else if (kind == kPlaces && b.count[e] && i < kRowsBins - 1) {
+        const float at = (float)i + (float)h[nb] / (4096.0f * (float)b.count[e]);
+        b.mass[e] = (u64)((float)b.count[e] * exp2f(44.0f - at * step));
+      }
     }
-    uint32_t c = b.count[0] + b.count[1];
-    u64 m = b.mass[0] + b.mass[1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      b.run[e] = (e ? b.run[e - 1] : 0u) + b.count[e];
+      b.mrun[e] = (e ? b.mrun[e - 1] : 0ull) + b.mass[e];
+    }
+    uint32_t c = b.run[3];
+    u64 m = b.mrun[3];
     const uint32_t c0 = c;
     const u64 m0 = m;
 #pragma unroll
@@ -311,62 +474,103 @@ struct RowsCta {
       c += wc[w];
       m += wm[w];
     }
-    b.run[0] = c - c0 + b.count[0];
-    b.run[1] = c;
-    b.mrun[0] = m - m0 + b.mass[0];
-    b.mrun[1] = m;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      b.run[e] += c - c0;
+      b.mrun[e] += m - m0;
+    }
     return b;
   }
-  // The bin at which the running count (by_count) or weight first reaches goal: its number, size
-  // and what comes before it, in sh->pick_*. (goal lies within the whole sum.)
-  __device__ void find_bin(const Bins& b, u64 goal, bool by_count) {
-    __syncthreads();
-    if (threadIdx.x == 0) sh->pick_bin = -1;
+  // For each goal: the bin at which the running count (by_count) or weight first reaches it, and the
+  // tokens and weight before it, in sh->at. (A goal lies within the whole sum.)
+  __device__ void find_bins(const Bins& b, const u64* goal, int n_goals, bool by_count) {
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int e = 0; e < 4; ++e) {
       const u64 hi = by_count ? b.run[e] : b.mrun[e], own = by_count ? b.count[e] : b.mass[e];
-      if (hi >= goal && hi - own < goal) {
-        sh->pick_bin = 2 * threadIdx.x + e;
-        sh->pick_count = (int)b.count[e];
-        sh->pick_base = b.run[e] - b.count[e];
-        sh->pick_mass = b.mrun[e] - b.mass[e];
-      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k < n_goals && hi >= goal[k] && hi - own < goal[k])
+          sh->at[k] = RowsAt{b.per * (int)threadIdx.x + e, (int)b.count[e], (int)(b.run[e] - b.count[e]), b.mrun[e] - b.mass[e]};
     }
     __syncthreads();
   }
 
-  // Sorts the gathered list (value descending, then index) and leaves its running weights in
-  // cum (over the leader's histogram, whose bins were read before).
-  __device__ int sort_list(u64* cum) {
-    const int m = min(sh->listed, kRowsList);
-    int p2 = 64;
-    while (p2 < m) p2 <<= 1;
-    for (int i = m + threadIdx.x; i < p2; i += kRowsThreads) list[i] = ~0ull;
+  // Collects the CTAs' lists behind the leader's own.
+  __device__ int collect() {
+    int off[kRowsMaxCluster + 1];
+    off[0] = 0;
+#pragma unroll
+    for (int r = 0; r < kRowsMaxCluster; ++r) off[r + 1] = off[r] + (r < C ? (int)sh->part[r] : 0);
+    const int m = min(off[kRowsMaxCluster], kRowsList);
+    for (int i = off[1] + threadIdx.x; i < m; i += kRowsThreads) {
+      int r = 1;
+#pragma unroll
+      for (int k = 2; k < kRowsMaxCluster; ++k) r += i >= off[k];
+      int at = 0;
+#pragma unroll
+      for (int k = 1; k < kRowsMaxCluster; ++k)
+        if (r == k) at = i - off[k];
+      list[i] = cl.map_shared_rank(list, r)[at];
+    }
     __syncthreads();
+    return m;
+  }
+  // Bitonic sort of the list padded to kRowsList: each warp keeps 64 neighbours in registers (two a
+  // lane, 32 apart) and exchanges by shuffles; only distances of 64 and more go through shared memory
+  // (10 steps with a barrier instead of 55).
+  __device__ void sort_all(int m) {
+    const int lane = threadIdx.x & 31, i0 = (threadIdx.x >> 5) * 64 + lane;
+    u64 x = i0 < m ? list[i0] : ~0ull, y = i0 + 32 < m ? list[i0 + 32] : ~0ull;
+    auto order = [](u64& a, u64& b, bool up) {
+      if ((a > b) == up) {
+        const u64 t = a;
+        a = b;
+        b = t;
+      }
+    };
+    auto swap = [&](u64& a, int j, bool up) {  // against the lane j away; `up`: the lower index keeps the smaller
+      const u64 o = __shfl_xor_sync(0xffffffffu, a, j);
+      if ((a > o) == (((lane & j) == 0) == up)) a = o;
+    };
+    for (int k = 2; k <= kRowsList; k <<= 1) {
+      for (int j = k >> 1; j >= 64; j >>= 1) {
+        __syncthreads();
+        list[i0] = x;
+        list[i0 + 32] = y;
+        __syncthreads();
+        const bool up = ((i0 & k) == 0) == ((i0 & j) == 0);
+        const u64 ox = list[i0 ^ j], oy = list[(i0 + 32) ^ j];
+        if ((x > ox) == up) x = ox;
+        if ((y > oy) == up) y = oy;
+      }
+      if (k >= 64) order(x, y, (i0 & k) == 0);
+      for (int j = min(k >> 1, 16); j > 0; j >>= 1) {
+        swap(x, j, (i0 & k) == 0);
+        swap(y, j, ((i0 + 32) & k) == 0);
+      }
+    }
+    __syncthreads();
+    list[i0] = x;
+    list[i0 + 32] = y;
+    __syncthreads();
+  }
+  // Sorts the collected list (value descending, then index) and leaves its running weights in
+  // cum (over the leader's histogram, whose bins were read before).
+  __device__ void sort_list(u64* cum, int m) {
     if (m <= 256) {  // rank by counting
       u64 x = 0;
       int r = 0;
       if ((int)threadIdx.x < m) {
         x = list[threadIdx.x];
+#pragma unroll 8
         for (int i = 0; i < m; ++i) r += list[i] < x;
       }
       __syncthreads();
       if ((int)threadIdx.x < m) list[r] = x;
       __syncthreads();
     } else {
-      for (int k = 2; k <= p2; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-          for (int i = threadIdx.x; i < p2 / 2; i += kRowsThreads) {
-            const int a = ((i & ~(j - 1)) << 1) | (i & (j - 1)), b = a | j;
-            const u64 x = list[a], y = list[b];
-            if ((x > y) == ((a & k) == 0)) {
-              list[a] = y;
-              list[b] = x;
-            }
-          }
-          __syncthreads();
-        }
+      sort_all(m);
     }
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i0 = 2 * threadIdx.x;
     const u64 w0 = i0 < m ? weight(entry_value(list[i0])) : 0ull, w1 = i0 + 1 < m ? weight(entry_value(list[i0 + 1])) : 0ull;
@@ -383,7 +587,6 @@ struct RowsCta {
     if (i0 < m) cum[i0] = s - w1;
     if (i0 + 1 < m) cum[i0 + 1] = s;
     __syncthreads();
-    return m;
   }
   __device__ __forceinline__ static float entry_value(u64 e) { return row_key_value(~(uint32_t)(e >> 32)); }
   // First entry whose running weight reaches goal (goal <= cum[m - 1]), in every thread.
@@ -401,10 +604,11 @@ struct RowsCta {
   // The prefix at whose end the running count or weight first reaches goal, and (want_index) the
   // token that ends it. b: the row's first histogram.
   __device__ RowsPrefix resolve(const Bins& first, u64 goal, bool by_count, bool want_index, int* index) {
-    find_bin(first, goal, by_count);
-    u64 before = sh->pick_base, mass = sh->pick_mass;
-    int count = sh->pick_count;
-    RowsCmd c{kOpGather, 1, (uint32_t)sh->pick_bin, (uint32_t)sh->pick_bin, 0, 0, 0};
+    u64 goals[4] = {goal, 0, 0, 0};
+    find_bins(first, goals, 1, by_count);
+    u64 before = sh->at[0].before, mass = sh->at[0].mass;
+    int count = sh->at[0].count;
+    RowsCmd c{kOpGather, 2, (uint32_t)sh->at[0].bin, (uint32_t)sh->at[0].bin, 0, 0, 0, 0, 1, 0};
     // (32 bits of key, ten a round: five rounds always reach a single key)
     for (int round = 0; round < 6 && count > kRowsList; ++round) {
       if (c.by_bin) {
@@ -417,14 +621,15 @@ struct RowsCta {
       if (c.lo == c.hi) break;
       c.op = kOpHist;
       c.shift = 0;
-      while (((c.hi - c.lo) >> c.shift) >= (uint32_t)kRowsBins) ++c.shift;
+      while (((c.hi - c.lo) >> c.shift) >= (uint32_t)kRowsExact) ++c.shift;
       command(c);
-      const Bins b = read_bins();
-      find_bin(b, goal - (by_count ? before : mass), by_count);
-      before += sh->pick_base;
-      mass += sh->pick_mass;
-      count = sh->pick_count;
-      const uint32_t top = c.hi - ((uint32_t)sh->pick_bin << c.shift), span = (1u << c.shift) - 1u;
+      const Bins b = read_bins(kExact);
+      goals[0] = goal - (by_count ? before : mass);
+      find_bins(b, goals, 1, by_count);
+      before += sh->at[0].before;
+      mass += sh->at[0].mass;
+      count = sh->at[0].count;
+      const uint32_t top = c.hi - ((uint32_t)sh->at[0].bin << c.shift), span = (1u << c.shift) - 1u;
       c.lo = max(c.lo, top - min(top, span));
       c.hi = top;
     }
@@ -440,7 +645,8 @@ struct RowsCta {
     c.op = kOpGather;
     command(c);
     u64* cum = reinterpret_cast<u64*>(hist);
-    const int m = sort_list(cum);
+    const int m = collect();
+    sort_list(cum, m);
     const int at = by_count ? (int)(goal - before) - 1 : find_entry(cum, m, goal - mass);
     p.key = ~(uint32_t)(list[at] >> 32);
     p.mass = mass + cum[at];
@@ -462,17 +668,21 @@ template <typename T>
 __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_constant__ SampleRowsArgs a) {
   extern __shared__ __align__(16) unsigned char rows_smem[];
   __shared__ RowsShared sh;
+  __shared__ double pow2[128];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   RowsCta x{cg::this_cluster()};
   x.sh = &sh;
   x.C = (int)x.cl.num_blocks();
   x.rank = (int)x.cl.block_rank();
-  x.hist = reinterpret_cast<uint4*>(rows_smem);
-  x.list = reinterpret_cast<u64*>(rows_smem + kRowsBins * 16);
-  x.val = reinterpret_cast<float*>(rows_smem + kRowsBins * 16 + kRowsList * 8);
+  x.lg = 31 - __clz(x.C);
+  x.hist = reinterpret_cast<uint32_t*>(rows_smem);
+  x.list = reinterpret_cast<u64*>(rows_smem + kRowsBins * 8);
+  x.val = reinterpret_cast<float*>(rows_smem + kRowsBins * 8 + kRowsList * 8);
   const int r = blockIdx.x / x.C;
   x.base = x.rank * a.per;
   x.n = max(0, min(a.per, a.vocab - x.base));
+  x.pow2 = pow2;
+  if (tid < 128) pow2[tid] = exp2(tid / 128.0);
   auto started = x.cl.barrier_arrive();  // waited for before the first access to another CTA's memory
   pdl_wait();
   pdl_trigger();
@@ -487,30 +697,37 @@ __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_co
   const char* row = static_cast<const char*>(a.logits) + (r * a.row_stride + x.base) * (long long)sizeof(T);
   float mx = -INFINITY, mn = INFINITY;
   auto take = [&](float v) {
-    if (!(v == v)) v = -INFINITY;
     mx = fmaxf(mx, v);
-    if (v > -INFINITY) mn = fminf(mn, v);
-    return v;
+    mn = fminf(mn, v > -INFINITY ? v : INFINITY);
   };
-  constexpr int V16 = 16 / sizeof(T);
+  constexpr int V = 16 / sizeof(T);
   int done = 0;
   if ((reinterpret_cast<uintptr_t>(row) & 15) == 0) {
-    const int chunks = x.n / V16;
-#pragma unroll 4
+    const uint4* src = reinterpret_cast<const uint4*>(row);
+    const int chunks = x.n / V;
+#pragma unroll 5
     for (int i = tid; i < chunks; i += kRowsThreads) {
-      const uint4 q = ld_stream(reinterpret_cast<const uint4*>(row) + i);
-      T t[V16];
+      const uint4 q = ld_stream(src + i);
+      T t[V];
       memcpy(t, &q, 16);
-      float f[V16];
 #pragma unroll
-      for (int e = 0; e < V16; ++e) f[e] = take(rows_value<T>(t, e));
-#pragma unroll
-      for (int e = 0; e < V16; e += 4)
-        *reinterpret_cast<float4*>(x.val + i * V16 + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+      for (int k = 0; k < V; k += 4) {
+        const float4 f = make_float4(rows_value<T>(t, k), rows_value<T>(t, k + 1), rows_value<T>(t, k + 2), rows_value<T>(t, k + 3));
+        take(f.x);
+        take(f.y);
+        take(f.z);
+        take(f.w);
+        *reinterpret_cast<float4*>(x.val + i * V + k) = f;
+      }
     }
-    done = chunks * V16;
+    done = chunks * V;
   }
-  for (int i = done + tid; i < x.n; i += kRowsThreads) x.val[i] = take(rows_value<T>(row, i));
+  for (int i = done + tid; i < x.n; i += kRowsThreads) {
+    const float v = rows_value<T>(row, i);
+    take(v);
+    x.val[i] = v;
+  }
+  if (tid < ((4 - x.n % 4) & 3)) x.val[x.n + tid] = __int_as_float(0x7fc00000);
   mx = warp_max(mx);
   mn = -warp_max(-mn);
   if (lane == 0) {
@@ -538,10 +755,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_co
   if (!(temperature > 0.0f) || top_k == 1 || !(fabsf(mx) < INFINITY)) {
     // greedy: the first token of the largest value; where all are -inf or NaN the first that is not NaN
     int at = 0x7fffffff;
-    for (int i = tid; i < x.n; i += kRowsThreads) {
-      const bool is = mx > -INFINITY ? x.val[i] == mx : !isnan(rows_value<T>(row, i));
-      if (is) at = min(at, x.base + i);
-    }
+    x.each([&](float v, int i) {
+      if (mx > -INFINITY ? v == mx : !isnan(v)) at = min(at, x.base + i);
+    });
     at = __reduce_min_sync(0xffffffffu, at);
     if (lane == 0) atomicMin(&x.cl.map_shared_rank(&sh, 0)->found, at);
     x.cl.sync();
@@ -552,14 +768,16 @@ __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_co
     return;
   }
   x.inv_t = 1.0 / (double)temperature;
-  const float range = fminf(31.0f * temperature, mx - mn);
-  x.scale = range > 0.0f ? fminf((float)(kRowsBins - 1) / range, 3.0e38f) : 0.0f;
+  x.z_scale = x.inv_t * (128.0 * 1.4426950408889634);
+  // 32 T: 2^44 exp(-32) < 1/2, so that what lies beyond weighs nothing
+  x.range = fminf(32.0f * temperature, mx - mn);
+  x.scale = x.range > 0.0f ? fminf((float)(RowsCta::kNoPlace) / x.range, 3.0e38f) : 0.0f;
+  x.step = x.scale > 0.0f ? (float)(x.z_scale * (4096.0 / 128.0) / (double)x.scale) : 0.0f;
 
-  // weights are summed at once where a cut or the draw will need them; a top-k cut, or a min-p cut
-  // without a top-p one, usually leaves a short list that does not
+  // weights matter unless a top-k cut (or a min-p cut without a top-p one) leaves a short list
   const bool cut_p = top_p < 1.0f, cut_m = min_p > 0.0f;
-  bool mass = !few && (cut_p || !cut_m);
-  x.histogram(RowsCmd{kOpHist, 1, 0, kRowsBins - 1, 0, 0, 0}, mass);
+  const RowsCta::HistKind kind = few || (cut_m && !cut_p) ? RowsCta::kCounts : RowsCta::kPlaces;
+  x.histogram(RowsCmd{}, kind);
   x.cl.sync();
   if (x.rank != 0) {
     for (;;) {
@@ -572,33 +790,46 @@ __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_co
   }
 
   // ---- the leader ----
-  const RowsCmd end{kOpEnd, 0, 0, 0, 0, 0, 0};
-  RowsCta::Bins bins = x.read_bins();
+  const RowsCmd all_bins{kOpHist, 2, 0, kRowsExact - 1, 0, 0, 0, 0, 1, 0}, end{};
+  RowsCta::Bins bins = x.read_bins(kind);
   const uint32_t kmin = cut_m ? rows_min_key(min_p, mx, (double)temperature) : 0u;
-  // the last step that can hold a kept token, and how many tokens there are up to it
-  int last = kRowsBins - 1, upto = a.vocab;
-  if (few) {
-    x.find_bin(bins, (u64)top_k, true);
-    last = sh.pick_bin;
-    upto = (int)sh.pick_base + sh.pick_count;
-  } else if (cut_p) {
-    if (tid == kRowsThreads - 1) sh.part[0] = bins.mrun[1];
-    __syncthreads();
-    x.find_bin(bins, max((u64)ceil(fmax((double)top_p, 0.0) * (double)sh.part[0]), 1ull), false);
-    last = sh.pick_bin;
-    upto = (int)sh.pick_base + sh.pick_count;
-  }
-  if (cut_m && !(few && cut_p)) {  // (top-p after top-k needs the whole top-k's sum)
-    const int mb = x.bin(row_key_value(kmin));
-    if (mb < last) {
-      last = mb;
-      __syncthreads();
+  const double p_share = fmax((double)top_p, 0.0);
+  const int mbin = cut_m ? x.bin(row_key_value(kmin)) : kRowsBins - 1;
+  if (tid == kRowsThreads - 1) sh.whole = bins.mrun[3];
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if (2 * tid + e == mb) sh.pick_count = (int)bins.run[e];
-      __syncthreads();
-      upto = sh.pick_count;
-    }
+  for (int e = 0; e < 4; ++e)
+    if (4 * tid + e == mbin) sh.upto = (int)bins.run[e];
+  __syncthreads();
+  // Where the top-p border and the draw must lie, by the estimated running weights (kPlaces).
+  const double about = (double)sh.whole, nats = (double)x.step * 0.6931471805599453;
+  const double slack = 3.0 * (nats * nats / 8.0 + 1.0e-5);
+  const double p_goal = cut_p ? p_share * about : about, uu = fmin(fmax((double)u, 0.0), 1.0);
+  // (the token that reaches the top-p border is kept whole: at most one weight more)
+  const double d_lo_goal = uu * (cut_p ? p_goal * (1.0 - slack) : about),
+               d_hi_goal = uu * (cut_p ? p_goal * (1.0 + slack) + kRowsOne : about);
+  u64 goals[4];
+  goals[0] = few ? (u64)top_k : (u64)fmin(fmax(p_goal * (1.0 + slack), 1.0), about);
+  goals[1] = (u64)fmin(fmax(p_goal * (1.0 - slack), 1.0), about);
+  goals[2] = (u64)fmin(fmax(d_hi_goal * (1.0 + slack) + 1.0, 1.0), about);
+  goals[3] = (u64)fmin(fmax(d_lo_goal * (1.0 - slack), 1.0), about);
+  if (kind == RowsCta::kPlaces || few) x.find_bins(bins, goals, few ? 1 : 4, few);
+  // the last bin that can hold a kept token, and the tokens up to it
+  int last = kRowsBins - 1, upto = a.vocab;
+  if (few || cut_p) {
+    last = sh.at[0].bin;
+    upto = sh.at[0].before + sh.at[0].count;
+  }
+  if (cut_m && !(few && cut_p) && mbin < last) {  // (top-p after top-k needs the whole top-k's sum)
+    last = mbin;
+    upto = sh.upto;
+  }
+  // without a top-k or min-p cut: the ranges of bins of the border and of the draw, if short enough
+  const int p_lo = sh.at[1].bin, p_hi = last, d_lo = min(sh.at[3].bin, last), d_hi = min(sh.at[2].bin, last);
+  bool ranges = upto > kRowsList && kind == RowsCta::kPlaces && !cut_m;
+  if (ranges) {
+    int found = sh.at[2].before + sh.at[2].count - sh.at[3].before;
+    if (cut_p) found += upto - sh.at[1].before;
+    ranges = found <= kRowsList;
   }
   u64 total = 0;
   int id = 0;
@@ -606,18 +837,20 @@ __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_co
   auto share = [&](uint32_t key) {
     return (float)(((double)row_key_value(key) - (double)mx) * x.inv_t - log((double)total / kRowsOne));
   };
+  u64* cum = reinterpret_cast<u64*>(x.hist);
+  bool settled = false;
   if (upto <= kRowsList) {
-    u64 all = 0;
-    if (!few && cut_p) all = sh.part[0];
-    __syncthreads();
-    x.command(RowsCmd{kOpGather, 1, 0, (uint32_t)last, 0, 0, 0});
+    x.command(RowsCmd{kOpGather, 1, 0, (uint32_t)last, 0, 0, 0, cut_p && !few, 1, 0});
+    int m = x.collect();
     x.command(end);
-    u64* cum = reinterpret_cast<u64*>(x.hist);
-    int m = x.sort_list(cum);
+    x.sort_list(cum, m);
     if (few) m = min(m, top_k);
     if (cut_p) {
-      const u64 sum = few ? cum[m - 1] : all;
-      m = min(m, x.find_entry(cum, m, min(max((u64)ceil(fmax((double)top_p, 0.0) * (double)sum), 1ull), cum[m - 1])) + 1);
+      u64 sum = 0;
+      if (few) sum = cum[m - 1];
+      else
+        for (int c = 0; c < x.C; ++c) sum += sh.above[0][c];
+      m = min(m, x.find_entry(cum, m, min(max((u64)ceil(p_share * (double)sum), 1ull), cum[m - 1])) + 1);
     }
     if (cut_m) {
       __syncthreads();
@@ -637,25 +870,83 @@ __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_co
     const int at = x.find_entry(cum, m, min((u64)floor((double)u * (double)total), total - 1) + 1);
     id = (int)(uint32_t)x.list[at];
     logp = share(~(uint32_t)(x.list[at] >> 32));
-  } else {
-    if (!mass) {
-      x.command(RowsCmd{kOpHist, 1, 0, kRowsBins - 1, 0, 0, 0});
-      bins = x.read_bins();
+    settled = true;
+  } else if (ranges) {
+    // Both ranges in one list, in order: the draw's tokens lie at or before the border's. Where the
+    // ranges overlap they are one. Running weights: exact, from those above each range.
+    RowsCmd c{kOpGather, 1, (uint32_t)d_lo, (uint32_t)d_hi, 0, 0, 0, 1, 1, 0};
+    if (cut_p) {
+      if (p_lo <= d_hi + 1) {
+        c.hi = (uint32_t)p_hi;
+      } else {
+        c.lo2 = (uint32_t)p_lo;
+        c.hi2 = (uint32_t)p_hi;
+      }
     }
-    if (tid == kRowsThreads - 1) sh.pick_mass = bins.mrun[1];
+    x.command(c);
+    const int m = x.collect();
+    u64 all = 0, above = 0, above2 = 0;
+    for (int k = 0; k < x.C; ++k) {
+      all += sh.above[0][k];
+      above += sh.above[1][k];
+      above2 += sh.above[2][k];
+    }
+    const bool split = c.lo2 <= c.hi2;
+    x.sort_list(cum, m);
+    // entries of the first range, then what the second one's running weights lack
+    int m1 = m;
+    if (split) {
+      __syncthreads();
+      if (tid == 0) sh.pick_at = 0;
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = 2 * tid + e;
+        if (i < m && x.bin(x.entry_value(x.list[i])) <= d_hi && (i + 1 == m || x.bin(x.entry_value(x.list[i + 1])) > d_hi))
+          sh.pick_at = i + 1;
+      }
+      __syncthreads();
+      m1 = sh.pick_at;
+    }
+    const u64 first = m1 > 0 ? cum[m1 - 1] : 0ull;
+    const u64 lift = split ? above2 - above - first : 0ull;  // weights between the ranges
+    const u64 span = m > 0 ? above + cum[m - 1] + lift : 0ull;
+    total = all;
+    bool ok = m > 0;
+    if (cut_p && ok) {
+      const u64 goal = max((u64)ceil(p_share * (double)all), 1ull);
+      const u64 from = split ? above + first + lift : above;  // before the border's range
+      ok = goal > from && goal <= span;
+      if (ok) total = above + lift + cum[x.find_entry(cum, m, goal - above - lift)];
+    }
+    if (ok) {
+      const u64 goal = min((u64)floor((double)u * (double)total), total - 1) + 1;
+      ok = m1 > 0 && goal > above && goal <= above + first;
+      if (ok) {
+        const int at = x.find_entry(cum, m1, goal - above);
+        id = (int)(uint32_t)x.list[at];
+        logp = share(~(uint32_t)(x.list[at] >> 32));
+        settled = true;
+        x.command(end);
+      }
+    }
+  }
+  if (!settled) {
+    x.command(all_bins);
+    bins = x.read_bins(RowsCta::kExact);
+    if (tid == kRowsThreads - 1) sh.whole = bins.mrun[3];
     __syncthreads();
-    RowsPrefix keep{0u, a.vocab, sh.pick_mass};
+    RowsPrefix keep{0u, a.vocab, sh.whole};
     int unused;
     if (few) keep = x.resolve(bins, (u64)top_k, true, false, &unused);
     if (cut_p) {
-      const RowsPrefix p =
-          x.resolve(bins, max((u64)ceil(fmax((double)top_p, 0.0) * (double)keep.mass), 1ull), false, false, &unused);
+      const RowsPrefix p = x.resolve(bins, max((u64)ceil(p_share * (double)keep.mass), 1ull), false, false, &unused);
       if (p.key > keep.key || (p.key == keep.key && p.ties < keep.ties)) keep = p;
     }
     if (min_p > 1.0f) {
       keep.mass = x.weight(mx);
     } else if (cut_m && kmin > keep.key) {
-      keep.mass = x.total_of(RowsCmd{kOpMass, 0, kmin, 0xffffffffu, 0, 0, 0});
+      keep.mass = x.total_of(RowsCmd{kOpMass, 0, kmin, 0xffffffffu, 0, 0, 0, 0, 1, 0});
     }
     total = keep.mass;
     const RowsPrefix p = x.resolve(bins, min((u64)floor((double)u * (double)total), total - 1) + 1, false, true, &id);
@@ -670,16 +961,17 @@ __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_co
 
 template <typename T>
 static void launch_sample_rows(SampleRowsArgs a, int rows, cudaStream_t s) {
-  // CTAs per row: enough that a CTA holds at most 20480 tokens (two CTAs an SM) and, with few rows,
-  // that the SMs are used; a CTA below 2048 tokens gains nothing any more.
+  // CTAs per row: enough that a CTA holds at most 20480 tokens (two CTAs an SM; without a copy in shared
+  // memory, passes over L1 and L2 took 1.2 to 1.5 times as long) and, with few rows, that the SMs are
+  // used; a CTA below 2048 tokens gains nothing any more.
   int C = 1;
   while (C < kRowsMaxCluster && ((a.vocab + C - 1) / C > 20480 ||
                                  ((long long)rows * C < 2 * current_sms() && (a.vocab + C - 1) / C > 2048)))
     C *= 2;
   a.per = ((a.vocab + C - 1) / C + 7) / 8 * 8;
-  const size_t smem = kRowsBins * 16 + kRowsList * 8 + (size_t)a.per * 4;
+  const size_t smem = kRowsBins * 8 + kRowsList * 8 + (size_t)a.per * 4;
   static unsigned long long smem_set = 0;
-  allow_smem(k_sample_rows<T>, kRowsBins * 16 + kRowsList * 8 + (size_t)(kRowsMaxVocab / kRowsMaxCluster + 8) * 4, smem_set);
+  allow_smem(k_sample_rows<T>, kRowsBins * 8 + kRowsList * 8 + (size_t)kRowsMaxPer * 4, smem_set);
   if ((long long)rows * C > 0x7fffffffLL) throw QdError{QD_E_RANGE, "qd_sample_rows: too many rows"};
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * C));
