@@ -590,82 +590,94 @@ def gqa_decode(q, k_cache, v_cache, seq_len: int, q_heads: int, kv_heads: int, y
 
 
 # ---- paged key-value cache and batched sampling (torch CUDA tensors) --------------------
+# These calls are made per layer or per token, so their host side is kept short: one test of
+# everything that may be wrong, with the message looked for only when it fails.
 
-def _dtype_code(t, what: str) -> int:
-    import torch
-    code = {torch.float16: QD_KV_F16, torch.float32: QD_KV_F32, torch.bfloat16: _lib.QD_KV_BF16}.get(t.dtype)
+class _Torch:
+    """torch's names used below, looked up once (torch is imported on first use)."""
+    ready = False
+
+    @classmethod
+    def load(cls):
+        import torch
+        cls.torch, cls.empty, cls.empty_like = torch, torch.empty, torch.empty_like
+        cls.i32, cls.f32, cls.u8 = torch.int32, torch.float32, torch.uint8
+        cls.code = {torch.float16: QD_KV_F16, torch.float32: QD_KV_F32, torch.bfloat16: _lib.QD_KV_BF16}
+        if torch.cuda.is_available():
+            torch.cuda.init()
+            cls.device, cls.stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+        cls.lib = _lib.load()
+        cls.ready = True
+
+
+def _elsewhere(dev: int, stream):
+    """None where the call can go on as it is; else a context that makes the tensors' device and
+    the stream current (what the call allocates then belongs to the stream that uses it)."""
+    t = _Torch
+    if dev < 0:
+        raise ValueError("tensors must be on a CUDA device")
+    if stream is not None:
+        if stream.device.index != dev:
+            raise ValueError(f"the stream belongs to {stream.device}, the tensors to cuda:{dev}")
+        return t.torch.cuda.stream(stream)
+    return None if t.device() == dev else t.torch.cuda.device(dev)
+
+
+def _vector(x, n: int, dtype, dev: int, what: str):
+    """Pointer of a contiguous vector of n entries (None: NULL)."""
+    if x is None:
+        return None
+    if x.dtype is not dtype or x.shape != (n,) or not x.is_contiguous() or x.get_device() != dev:
+        raise ValueError(f"{what} must be a contiguous {dtype} vector of {n} entries on cuda:{dev}")
+    return x.data_ptr()
+
+
+def _row_stride(x, width: int, what: str) -> int:
+    """Row stride (elements) of a [rows, ...] tensor whose rows are `width` contiguous elements."""
+    if x.is_contiguous() and x.dim() and x.shape[0] * width == x.numel():
+        return width
+    inner = 1
+    for i in range(x.dim() - 1, 0, -1):
+        if x.shape[i] != 1 and x.stride(i) != inner:
+            raise ValueError(f"the rows of {what} must be contiguous")
+        inner *= x.shape[i]
+    if x.dim() < 1 or inner != width:
+        raise ValueError(f"{what} must have rows of {width} elements")
+    return x.stride(0) if x.shape[0] > 1 else width
+
+
+def _code(x, what: str) -> int:
+    code = _Torch.code.get(x.dtype)
     if code is None:
-        raise ValueError(f"{what} must be float16, bfloat16 or float32, not {t.dtype}")
+        raise ValueError(f"{what} must be float16, bfloat16 or float32, not {x.dtype}")
     return code
 
 
-def _vector(t, n: Optional[int], dtype, device, what: str):
-    """Pointer of a contiguous 1-D tensor of n entries (None: NULL)."""
-    if t is None:
-        return None
-    if t.dtype != dtype or t.device != device or t.dim() != 1 or (n is not None and t.shape[0] != n) \
-            or (t.shape[0] > 1 and t.stride(0) != 1):
-        raise ValueError(f"{what} must be a contiguous {dtype} vector of {n if n is not None else 'n'} entries on {device}")
-    return t.data_ptr()
+def _paged_kv(k, v, table, seq_lens, status, dev: int) -> "_lib.QdPagedKv":
+    t, shape = _Torch, k.shape
+    if len(shape) != 4 or v.shape != shape or v.dtype is not k.dtype or not k.is_contiguous() or not v.is_contiguous() \
+            or k.get_device() != dev or v.get_device() != dev:
+        raise ValueError("k_pages and v_pages must be contiguous [pages][kv_heads][page_size][128] of one type, "
+                         "on the device of the other tensors")
+    if table.dtype is not t.i32 or table.dim() != 2 or table.get_device() != dev:
+        raise ValueError(f"block_table must be int32 [batch][pages] on cuda:{dev}")
+    batch, width = table.shape
+    stride = width
+    if not table.is_contiguous():
+        if width > 1 and table.stride(1) != 1:
+            raise ValueError("the rows of block_table must be contiguous")
+        stride = table.stride(0) if batch > 1 else width
+    return _lib.QdPagedKv(k.data_ptr(), v.data_ptr(), _code(k, "the cache"), shape[0], shape[2], shape[1], shape[3],
+                          batch, table.data_ptr(), width, stride, _vector(seq_lens, batch, t.i32, dev, "seq_lens"),
+                          None if status is None else _vector(status, 1, t.i32, dev, "status"))
 
 
-def _rows(t, width: int, device, what: str) -> int:
-    """Row stride (elements) of a [rows, ...] tensor whose rows are `width` contiguous elements."""
-    if t.device != device:
-        raise ValueError(f"{what} must be on {device}")
-    inner = 1
-    for i in range(t.dim() - 1, 0, -1):
-        if t.shape[i] != 1 and t.stride(i) != inner:
-            raise ValueError(f"the rows of {what} must be contiguous")
-        inner *= t.shape[i]
-    if t.dim() < 1 or inner != width:
-        raise ValueError(f"{what} must have rows of {width} elements")
-    return t.stride(0) if t.shape[0] > 1 else width
-
-
-class _Launch:
-    """Makes a tensor's device and the given stream current, so that what the call allocates
-    belongs to the stream that uses it; gives the stream's handle."""
-
-    def __init__(self, device, stream):
-        import torch
-        if device.type != "cuda":
-            raise ValueError("tensors must be on a CUDA device")
-        if stream is not None and stream.device != device:
-            raise ValueError(f"the stream belongs to {stream.device}, the tensors to {device}")
-        self._with = None
-        if stream is not None:
-            self._with = torch.cuda.stream(stream)
-        elif device.index != torch.cuda.current_device():
-            self._with = torch.cuda.device(device)
-        self.handle = (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream
-
-    def __enter__(self):
-        if self._with is not None:
-            self._with.__enter__()
-        return self.handle
-
-    def __exit__(self, *exc):
-        if self._with is not None:
-            self._with.__exit__(*exc)
-
-
-def _paged_kv(k_pages, v_pages, block_table, seq_lens, status) -> "_lib.QdPagedKv":
-    import torch
-    dev = k_pages.device
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or not k_pages.is_contiguous() \
-            or not v_pages.is_contiguous() or v_pages.dtype != k_pages.dtype or v_pages.device != dev:
-        raise ValueError("k_pages and v_pages must be contiguous [pages][kv_heads][page_size][128] of one type and device")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.device != dev \
-            or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError("block_table must be int32 [batch][pages], its rows contiguous, beside the cache")
-    batch, width = block_table.shape
-    stride = block_table.stride(0) if batch > 1 else width
-    lens = _vector(seq_lens, batch, torch.int32, dev, "seq_lens")
-    pages, kv_heads, page_size, head_dim = k_pages.shape
-    return _lib.QdPagedKv(k_pages.data_ptr(), v_pages.data_ptr(), _dtype_code(k_pages, "the cache"), pages, page_size,
-                          kv_heads, head_dim, batch, block_table.data_ptr(), width, stride, lens,
-                          _vector(status, 1, torch.int32, dev, "status"))
+def _workspace(given, n: int, dev: int):
+    if given is None:
+        return _Torch.empty(n, dtype=_Torch.u8, device=dev)
+    if given.get_device() != dev or given.numel() * given.element_size() < n or not given.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous tensor of at least {n} bytes on cuda:{dev}")
+    return given
 
 
 def paged_append(qkv, k_pages, v_pages, block_table, seq_lens, cos, sin, q_heads: int, q_norm=None, k_norm=None,
@@ -676,74 +688,86 @@ def paged_append(qkv, k_pages, v_pages, block_table, seq_lens, cos, sin, q_heads
     [pages][kv_heads][page_size][128]; cos, sin f32 tables whose row for a position is
     rope_stride elements after the previous one's (default: their own row stride; None, None:
     no rotation); returns q [rows][q_heads * 128] (q_out, or a new tensor of qkv's type)."""
-    import torch
-    dev = qkv.device
-    kv = _paged_kv(k_pages, v_pages, block_table, seq_lens, status)
-    heads = q_heads + 2 * kv.kv_heads
-    stride, rows = _rows(qkv, heads * 128, dev, "qkv"), qkv.shape[0]
-    if k_pages.device != dev:
-        raise ValueError(f"the cache must be on {dev}")
+    t = _Torch
+    if not t.ready:
+        t.load()
+    dev = qkv.get_device()
+    kv = _paged_kv(k_pages, v_pages, block_table, seq_lens, status, dev)
+    stride, rows = _row_stride(qkv, (q_heads + 2 * kv.kv_heads) * 128, "qkv"), qkv.shape[0]
     rope_len = 0
-    for t in (cos, sin):
-        if t is not None and (t.dtype != torch.float32 or t.device != dev or not t.is_contiguous()):
-            raise ValueError(f"cos and sin must be contiguous float32 tables on {dev}")
+    for x in (cos, sin):
+        if x is not None and (x.dtype is not t.f32 or x.get_device() != dev or not x.is_contiguous()):
+            raise ValueError(f"cos and sin must be contiguous float32 tables on cuda:{dev}")
     if cos is not None and sin is not None:
         rope_len = min(cos.numel(), sin.numel())
         if rope_stride is None:
             rope_stride = cos.stride(0) if cos.dim() > 1 else 64
-    with _Launch(dev, stream) as s:
-        if q_out is None:
-            q_out = torch.empty((rows, q_heads * 128), dtype=qkv.dtype, device=dev)
-        elif q_out.shape[0] != rows:
-            raise ValueError(f"q_out must have {rows} rows")
-        check(_lib.load().qd_paged_append(
-            kv, qkv.data_ptr(), _dtype_code(qkv, "qkv"), stride, rows,
-            _vector(q_starts, kv.batch + 1, torch.int32, dev, "q_starts"), q_heads,
-            _vector(q_norm, 128, torch.float32, dev, "q_norm"), _vector(k_norm, 128, torch.float32, dev, "k_norm"), eps,
-            None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(), rope_len,
-            rope_stride or 0, q_out.data_ptr(), _dtype_code(q_out, "q_out"),
-            _rows(q_out, q_heads * 128, dev, "q_out"), s))
+    there = _elsewhere(dev, stream)
+    if there is not None:
+        with there:
+            return paged_append(qkv, k_pages, v_pages, block_table, seq_lens, cos, sin, q_heads, q_norm, k_norm, eps,
+                                q_starts, q_out, rope_stride, status)
+    if q_out is None:
+        q_out = t.empty((rows, q_heads * 128), dtype=qkv.dtype, device=dev)
+        out_stride = q_heads * 128
+    elif q_out.get_device() != dev or q_out.shape[0] != rows:
+        raise ValueError(f"q_out must have {rows} rows on cuda:{dev}")
+    else:
+        out_stride = _row_stride(q_out, q_heads * 128, "q_out")
+    rc = t.lib.qd_paged_append(
+        kv, qkv.data_ptr(), _code(qkv, "qkv"), stride, rows,
+        None if q_starts is None else _vector(q_starts, kv.batch + 1, t.i32, dev, "q_starts"), q_heads,
+        _vector(q_norm, 128, t.f32, dev, "q_norm"), _vector(k_norm, 128, t.f32, dev, "k_norm"), eps,
+        None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(), rope_len, rope_stride or 0,
+        q_out.data_ptr(), _code(q_out, "q_out"), out_stride, t.stream(dev))
+    if rc:
+        check(rc)
     return q_out
 
 
-def _attn_args(q, k_pages, v_pages, block_table, seq_lens, status):
-    kv = _paged_kv(k_pages, v_pages, block_table, seq_lens, status)
-    if k_pages.device != q.device:
-        raise ValueError(f"the cache must be on {q.device}")
-    width = 1
-    for n in q.shape[1:]:
-        width *= n
-    if q.dim() < 2 or width % 128:
+def _attn(q, k_pages, v_pages, block_table, seq_lens, status):
+    """(cache, query heads, q's row stride, elements a row) of an attention call."""
+    kv = _paged_kv(k_pages, v_pages, block_table, seq_lens, status, q.get_device())
+    shape = q.shape
+    width = shape[1] * shape[2] if len(shape) == 3 else shape[1] if len(shape) == 2 else 1
+    if width % 128:
         raise ValueError("q must be [rows][q_heads][128] or [rows][q_heads * 128]")
-    return kv, width // 128, _rows(q, width, q.device, "q")
+    return kv, width // 128, _row_stride(q, width, "q"), width
 
 
-def _attn_out(q, y):
-    import torch
+def _attn_out(q, y, width: int):
     if y is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if y.dtype != q.dtype or y.shape != q.shape:
-        raise ValueError("y must have q's type and shape")
-    return y
+        if q.is_contiguous():
+            return _Torch.empty_like(q), width
+        return _Torch.empty(q.shape, dtype=q.dtype, device=q.device), width
+    if y.dtype is not q.dtype or y.shape != q.shape or y.get_device() != q.get_device():
+        raise ValueError("y must have q's type, shape and device")
+    return y, _row_stride(y, width, "y")
 
 
 def paged_attn_decode(q, k_pages, v_pages, block_table, seq_lens, window: int = 0, sinks: int = 0, scale: float = 0.0,
                       y=None, workspace=None, status=None, stream=None):
     """Attention of one new token per sequence over its pages (qd_paged_attn_decode): q
     [batch][q_heads][128], the token at position seq_lens[b] - 1; window > 0: the last
-    `window` positions and the first `sinks`. workspace: a uint8 tensor of
-    paged_attn_decode_workspace bytes that no other stream uses meanwhile (default: a new one)."""
-    import torch
-    kv, heads, stride = _attn_args(q, k_pages, v_pages, block_table, seq_lens, status)
+    `window` positions and the first `sinks`. workspace: a tensor of at least
+    qd_paged_attn_decode_workspace_bytes that no other stream uses meanwhile (default: a new one)."""
+    t = _Torch
+    if not t.ready:
+        t.load()
+    kv, heads, stride, width = _attn(q, k_pages, v_pages, block_table, seq_lens, status)
     if q.shape[0] != kv.batch:
         raise ValueError(f"q must have one row per sequence ({kv.batch})")
-    L = _lib.load()
-    with _Launch(q.device, stream) as s:
-        y = _attn_out(q, y)
-        n = L.qd_paged_attn_decode_workspace_bytes(kv.batch, heads)
-        ws = _workspace(workspace, n, q.device)
-        check(L.qd_paged_attn_decode(kv, q.data_ptr(), _dtype_code(q, "q"), stride, heads, window, sinks, scale,
-                                     y.data_ptr(), _rows(y, heads * 128, q.device, "y"), ws.data_ptr(), s))
+    dev = q.get_device()
+    there = _elsewhere(dev, stream)
+    if there is not None:
+        with there:
+            return paged_attn_decode(q, k_pages, v_pages, block_table, seq_lens, window, sinks, scale, y, workspace, status)
+    y, y_stride = _attn_out(q, y, width)
+    ws = _workspace(workspace, t.lib.qd_paged_attn_decode_workspace_bytes(kv.batch, heads), dev)
+    rc = t.lib.qd_paged_attn_decode(kv, q.data_ptr(), _code(q, "q"), stride, heads, window, sinks, scale, y.data_ptr(),
+                                    y_stride, ws.data_ptr(), t.stream(dev))
+    if rc:
+        check(rc)
     return y
 
 
@@ -753,47 +777,55 @@ def paged_attn_prompt(q, k_pages, v_pages, block_table, seq_lens, q_starts, wind
     q [rows][q_heads][128], rows q_starts[b] .. q_starts[b + 1] - 1 being sequence b's newest
     tokens (already appended). Rows from q_starts[batch] on are padding; y keeps what it held
     there."""
-    import torch
-    kv, heads, stride = _attn_args(q, k_pages, v_pages, block_table, seq_lens, status)
-    L = _lib.load()
-    with _Launch(q.device, stream) as s:
-        y = _attn_out(q, y)
-        n = L.qd_paged_attn_prompt_workspace_bytes(kv.batch, q.shape[0], heads, kv.kv_heads)
-        ws = _workspace(workspace, n, q.device)
-        check(L.qd_paged_attn_prompt(kv, q.data_ptr(), _dtype_code(q, "q"), stride, q.shape[0],
-                                     _vector(q_starts, kv.batch + 1, torch.int32, q.device, "q_starts"), heads, window,
-                                     sinks, scale, y.data_ptr(), _rows(y, heads * 128, q.device, "y"), ws.data_ptr(), s))
+    t = _Torch
+    if not t.ready:
+        t.load()
+    kv, heads, stride, width = _attn(q, k_pages, v_pages, block_table, seq_lens, status)
+    dev = q.get_device()
+    there = _elsewhere(dev, stream)
+    if there is not None:
+        with there:
+            return paged_attn_prompt(q, k_pages, v_pages, block_table, seq_lens, q_starts, window, sinks, scale, y,
+                                     workspace, status)
+    y, y_stride = _attn_out(q, y, width)
+    rows = q.shape[0]
+    ws = _workspace(workspace, t.lib.qd_paged_attn_prompt_workspace_bytes(kv.batch, rows, heads, kv.kv_heads), dev)
+    rc = t.lib.qd_paged_attn_prompt(kv, q.data_ptr(), _code(q, "q"), stride, rows,
+                                    _vector(q_starts, kv.batch + 1, t.i32, dev, "q_starts"), heads, window, sinks, scale,
+                                    y.data_ptr(), y_stride, ws.data_ptr(), t.stream(dev))
+    if rc:
+        check(rc)
     return y
-
-
-def _workspace(given, n: int, device):
-    import torch
-    if given is None:
-        return torch.empty(n, dtype=torch.uint8, device=device)
-    if given.device != device or given.numel() * given.element_size() < n or not given.is_contiguous():
-        raise ValueError(f"workspace must be a contiguous tensor of at least {n} bytes on {device}")
-    return given
 
 
 def sample_rows(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, ids=None, logprobs=None, stream=None):
     """One token per row of logits [rows][vocab] (f32, f16 or bf16) from the given random
     numbers u [rows] f32 in [0, 1), with per-row settings (f32 vectors; top_k int32; None: not
     applied) as qd_sample_rows defines them. Returns (ids int32, logprobs f32)."""
-    import torch
+    t = _Torch
+    if not t.ready:
+        t.load()
     if logits.dim() != 2:
         raise ValueError("logits must be [rows][vocab]")
     rows, vocab = logits.shape
-    dev = logits.device
-    stride = _rows(logits, vocab, dev, "logits")
-    f = [_vector(t, rows, torch.float32, dev, n) for t, n in
-         ((temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p"), (u, "u"))]
-    with _Launch(dev, stream) as s:
-        ids = torch.empty(rows, dtype=torch.int32, device=dev) if ids is None else ids
-        logprobs = torch.empty(rows, dtype=torch.float32, device=dev) if logprobs is None else logprobs
-        check(_lib.load().qd_sample_rows(logits.data_ptr(), _dtype_code(logits, "logits"), rows, vocab, stride, f[0],
-                                         _vector(top_k, rows, torch.int32, dev, "top_k"), f[1], f[2], f[3],
-                                         _vector(ids, rows, torch.int32, dev, "ids"),
-                                         _vector(logprobs, rows, torch.float32, dev, "logprobs"), s))
+    dev = logits.get_device()
+    stride = _row_stride(logits, vocab, "logits")
+    there = _elsewhere(dev, stream)
+    if there is not None:
+        with there:
+            return sample_rows(logits, u, temperature, top_k, top_p, min_p, ids, logprobs)
+    if ids is None:
+        ids = t.empty(rows, dtype=t.i32, device=dev)
+    if logprobs is None:
+        logprobs = t.empty(rows, dtype=t.f32, device=dev)
+    rc = t.lib.qd_sample_rows(logits.data_ptr(), _code(logits, "logits"), rows, vocab, stride,
+                              _vector(temperature, rows, t.f32, dev, "temperature"),
+                              _vector(top_k, rows, t.i32, dev, "top_k"), _vector(top_p, rows, t.f32, dev, "top_p"),
+                              _vector(min_p, rows, t.f32, dev, "min_p"), _vector(u, rows, t.f32, dev, "u"),
+                              _vector(ids, rows, t.i32, dev, "ids"), _vector(logprobs, rows, t.f32, dev, "logprobs"),
+                              t.stream(dev))
+    if rc:
+        check(rc)
     return ids, logprobs
 
 
