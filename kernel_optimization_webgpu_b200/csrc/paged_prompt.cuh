@@ -119,6 +119,12 @@ __device__ __forceinline__ PpItem pp_rows(const PAttnArgs& a, int G, int seq, in
   v.tiles = v.st + max(0, (v.end + kPpKeys - 1) / kPpKeys - v.w0);
   return it;
 }
+// Largest of three, NaN if one of them is.
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
 // Bits 0 .. n - 1.
 __device__ __forceinline__ unsigned pp_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 // Parts that an item's key tiles are really split into: at least two tiles each.
@@ -216,7 +222,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
   unsigned char* qs =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* ring = qs + 2 * kQTile;
-  __shared__ unsigned long long full[S], raw, empty[S], s_full[2], p_full[2], o_done[2], drain;
+  __shared__ unsigned long long full[S], raw, empty[S], s_full[2], p_full[2], o_done[2], q_full[2], drain;
   __shared__ unsigned bad_rows[8];  // of key tile j: bit i set where 16-key chunk i has no usable page
   __shared__ unsigned tmem_base;
   __shared__ int failed;
@@ -257,48 +263,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       tc_mbar_init(&s_full[i]);
       tc_mbar_init(&o_done[i]);
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 128;" ::"r"(tc_smem(&p_full[i])) : "memory");
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 128;" ::"r"(tc_smem(&q_full[i])) : "memory");
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     failed = 0;
-  }
-  // Q: one row per thread, K-major with the 128-byte swizzle; dead rows are zero. A negative scale
-  // changes the sign of q, so that the softmax always has a positive one.
-  if (tid < kPpRows && nk > 0) {
-    const int r = tid & 127;
-    unsigned char* dst = qs + (tid >> 7) * kQTile + r * 128;
-    const long long base = (long long)(it.tok0 + (live ? tok : 0)) * a.q_stride + ((long long)g * G + hs) * kHeadDim;
-    if constexpr (SPLIT) {
-#pragma unroll 4
-      for (int c = 0; c < 16; ++c) {
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-        if (live) {
-          x = load4<float>(a.q, base + 8 * c);
-          y = load4<float>(a.q, base + 8 * c + 4);
-          if (a.scale < 0.0f) {
-            x = make_float4(-x.x, -x.y, -x.z, -x.w);
-            y = make_float4(-y.x, -y.y, -y.z, -y.w);
-          }
-        }
-        uint4 h, l;
-        split2<T>(x.x, x.y, h.x, l.x);
-        split2<T>(x.z, x.w, h.y, l.y);
-        split2<T>(y.x, y.y, h.z, l.z);
-        split2<T>(y.z, y.w, h.w, l.w);
-        const unsigned off = (c >> 3) * (kPpTileBytes / 2) + (((c ^ r) & 7) << 4);
-        *reinterpret_cast<uint4*>(dst + off) = h;
-        *reinterpret_cast<uint4*>(dst + kPpTileBytes + off) = l;
-      }
-    } else {
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + base);
-#pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        uint4 x = live ? src[c] : make_uint4(0, 0, 0, 0);
-        if (a.scale < 0.0f)
-          x = make_uint4(x.x ^ 0x80008000u, x.y ^ 0x80008000u, x.z ^ 0x80008000u, x.w ^ 0x80008000u);
-        *reinterpret_cast<uint4*>(dst + (c >> 3) * (kPpTileBytes / 2) + (((c ^ r) & 7) << 4)) = x;
-      }
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
@@ -384,11 +352,12 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         umma_commit(&s_full[t]);
       };
       bool ok = pp_wait(&full[0], 0, &failed);
-      if (ok) {
+      for (int t = 0; t < halves && ok; ++t) {
+        ok = pp_wait(&q_full[t], 0, &failed);
         tc_fence_after();
-        for (int t = 0; t < halves; ++t) scores(t, 0);
-        umma_commit(&empty[0]);
+        if (ok) scores(t, 0);
       }
+      if (ok) umma_commit(&empty[0]);
       for (int j = 0; j < nk && ok; ++j) {
         const int vi = 2 * j + 1, vs = vi % S, ki = 2 * j + 2, ks_slot = ki % S;
         ok = pp_wait(&full[vs], (unsigned)(vi / S) & 1u, &failed);
@@ -424,6 +393,46 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
     // ---- softmax: one row per thread ----
     float m = -INFINITY, l = 0.0f;
     const int t = warp >> 2;
+    // Q: one row per thread, K-major with the 128-byte swizzle; dead rows are zero. A negative scale
+    // changes the sign of q, so that the softmax always has a positive one.
+    {
+    const int r = tid & 127;
+    unsigned char* dst = qs + (tid >> 7) * kQTile + r * 128;
+    const long long base = (long long)(it.tok0 + (live ? tok : 0)) * a.q_stride + ((long long)g * G + hs) * kHeadDim;
+    if constexpr (SPLIT) {
+#pragma unroll 8
+      for (int c = 0; c < 16; ++c) {
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+        if (live) {
+          x = load4<float>(a.q, base + 8 * c);
+          y = load4<float>(a.q, base + 8 * c + 4);
+          if (a.scale < 0.0f) {
+            x = make_float4(-x.x, -x.y, -x.z, -x.w);
+            y = make_float4(-y.x, -y.y, -y.z, -y.w);
+          }
+        }
+        uint4 h, l;
+        split2<T>(x.x, x.y, h.x, l.x);
+        split2<T>(x.z, x.w, h.y, l.y);
+        split2<T>(y.x, y.y, h.z, l.z);
+        split2<T>(y.z, y.w, h.w, l.w);
+        const unsigned off = (c >> 3) * (kPpTileBytes / 2) + (((c ^ r) & 7) << 4);
+        *reinterpret_cast<uint4*>(dst + off) = h;
+        *reinterpret_cast<uint4*>(dst + kPpTileBytes + off) = l;
+      }
+    } else {
+      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + base);
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        uint4 x = live ? src[c] : make_uint4(0, 0, 0, 0);
+        if (a.scale < 0.0f)
+          x = make_uint4(x.x ^ 0x80008000u, x.y ^ 0x80008000u, x.z ^ 0x80008000u, x.w ^ 0x80008000u);
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * (kPpTileBytes / 2) + (((c ^ r) & 7) << 4)) = x;
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+    pp_arrive(&q_full[t]);
     const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
     const unsigned ts = tmem + t * 128 + lanes, to = tmem + 256 + t * 128 + lanes;
     const float c = fabsf(a.scale) * kLog2e;
@@ -461,12 +470,14 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       }
       float mx[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mx[i] = fmaxf(__uint_as_float(sr[i]), __uint_as_float(sr[i + 4]));
+      for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(sr[e]);
 #pragma unroll
-      for (int i = 8; i < 128; i += 4)
+      for (int i = 4; i < 124; i += 8)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(sr[i + e]));
-      const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sr[i + e]), __uint_as_float(sr[i + 4 + e]));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sr[124 + e]), -INFINITY);
+      const float mt = max3(max3(mx[0], mx[1], mx[2]), mx[3], -INFINITY) * c;  // NaN where a score is
       if (__any_sync(0xffffffffu, mt > m + kPpLag)) {
         // each row by its own maximum (a factor of 1 where it has not moved), so that a row's result
         // does not depend on the rows beside it
