@@ -4,9 +4,11 @@
 // query heads that share a KV head share its tiles whatever their number. A CTA takes 256
 // consecutive rows as two M = 128 tiles and walks the 128-key tiles that any of its rows sees:
 //   S = Q K^T      -> TMEM (f32)                     M 128, N 128 keys, K 128 dims
-//   P = exp2(S c - m)   one thread per row: maximum, weights, their sum, all in f32
+//   P = exp2(S c - m)   two threads per row: maximum, weights, their sum, all in f32
 //   O += P V       -> TMEM (f32), P read from TMEM   M 128, N 128 dims, K 128 keys
 // The two tiles alternate: while one's softmax runs, the tensor cores work for the other. P
+// (One thread per row left a single softmax warp of a tile on each scheduler, and its chain of
+// dependent instructions set the pace: 1 x 8192 301 us against TODO us with two.) P
 // replaces its S in TMEM (S0 S1 O0 O1 = 512 columns); the MMAs of one issuer run in order, so
 // S of the next key tile may be issued right behind the product that reads P.
 //
@@ -33,10 +35,11 @@
 
 namespace qd {
 
-constexpr int kPpThreads = 384;    // 2 x 128 softmax threads; the MMA warp, the copy warp and two idle ones
-// Registers: 168 a thread at launch (64512 in all); the softmax threads hold a row of 128 scores, so
-// the third warpgroup gives its share up: 2 * 128 * 224 + 128 * 56 = 64512.
-constexpr int kPpRegsMany = 224, kPpRegsFew = 56;
+constexpr int kPpSoftmax = 512;    // softmax threads: two a row, 64 keys of a tile each
+constexpr int kPpThreads = 640;    // and the MMA warp, the copy warp and two idle ones
+// Registers: 96 a thread at launch (61440 in all); a softmax thread holds 64 scores, so the last
+// warpgroup gives some of its share up: 512 * 104 + 128 * 64 = 61440.
+constexpr int kPpRegsMany = 104, kPpRegsFew = 64;
 constexpr int kPpRows = 256;
 constexpr int kPpKeys = 128;
 constexpr int kPpTileBytes = 128 * 256;  // a 128 x 128 tile of 16-bit elements
@@ -125,6 +128,18 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
   return r;
 }
+// Whether any of a pair of warps says so, and their plain meeting.
+__device__ __forceinline__ bool pp_any(int barrier, bool mine) {
+  unsigned r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbarrier.cta.red.or.pred p, %2, 64, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)
+      : "r"((unsigned)mine), "r"(barrier)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void pp_meet(int barrier) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(barrier) : "memory"); }
 // Bits 0 .. n - 1.
 __device__ __forceinline__ unsigned pp_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 // Parts that an item's key tiles are really split into: at least two tiles each.
@@ -159,13 +174,30 @@ __device__ __forceinline__ unsigned pp_idesc(bool mn) {
   const unsigned fmt = sizeof(T) == 2 && !std::is_same<T, __half>::value ? 1u : 0u;
   return (1u << 4) | (fmt << 7) | (fmt << 10) | (mn ? 1u << 16 : 0u) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
 }
-// D += A B with A in TMEM.
-__device__ __forceinline__ void umma_f16_ts(unsigned d_tmem, unsigned a_tmem, unsigned long long b, unsigned idesc,
-                                            bool accumulate) {
+// D (+)= A B, issued by the lane whose `leader` is set: A from shared memory, or from TMEM.
+template <bool kAccumulate>
+__device__ __forceinline__ void pp_mma_ss(unsigned d_tmem, unsigned long long a, unsigned long long b, unsigned idesc,
+                                          unsigned leader) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b), "r"(idesc), "r"((unsigned)accumulate)
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 e, %4, 0;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a), "l"(b), "r"(idesc), "r"(leader), "n"(kAccumulate ? 1 : 0)
+      : "memory");
+}
+__device__ __forceinline__ void pp_mma_ts(unsigned d_tmem, unsigned a_tmem, unsigned long long b, unsigned idesc,
+                                          bool accumulate, unsigned leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 e, %4, 0;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b), "r"(idesc), "r"(leader), "r"((unsigned)accumulate)
+      : "memory");
+}
+// All products issued so far by that lane arrive on the barrier when they are done.
+__device__ __forceinline__ void pp_commit(unsigned long long* bar, unsigned leader) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(tc_smem(bar)),
+      "r"(leader)
       : "memory");
 }
 #define PP_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
@@ -225,8 +257,11 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
   __shared__ unsigned long long full[S], raw, empty[S], s_full[2], p_full[2], o_done[2], q_full[2], drain;
   __shared__ unsigned bad_rows[8];  // of key tile j: bit i set where 16-key chunk i has no usable page
   __shared__ unsigned tmem_base;
+  __shared__ float shared_row[kPpRows];  // between a row's two threads: a maximum (NaN: given up), then a sum
   __shared__ int failed;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // (values read back from lane 0 are warp-uniform to the compiler: the MMA warp's operands then live
+  // in uniform registers)
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int kvh = a.kv.kv_heads, G = a.q_heads / kvh;
   const int g = blockIdx.x % kvh, z = (blockIdx.x / kvh) % pa.splits, item = blockIdx.x / (kvh * pa.splits);
   pdl_wait();
@@ -237,16 +272,18 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
   if (it.asked > it.len && it.asked > 0 && tid == 0) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
   const int parts = pp_parts(it.v.tiles, pa.splits);
   if (z >= parts) return;
-  const int t0 = (int)((long long)it.v.tiles * z / parts), nk = (int)((long long)it.v.tiles * (z + 1) / parts) - t0;
+  const int t0 = (int)((long long)it.v.tiles * z / parts);
+  const int nk = __shfl_sync(0xffffffffu, (int)((long long)it.v.tiles * (z + 1) / parts) - t0, 0);
   const int row0 = tile * kPpRows;
-  const int halves = it.n_rows - row0 > 128 ? 2 : 1;
+  const int halves = __shfl_sync(0xffffffffu, it.n_rows - row0 > 128 ? 2 : 1, 0);
 
-  // this thread's row (softmax threads)
-  const int row = row0 + tid;
+  // this thread's row and half of a row's keys and dims (softmax threads)
+  const int t = (tid >> 8) & 1, hf = (tid >> 7) & 1, lr = t * 128 + (tid & 127);
+  const int row = row0 + lr;
   const int tok = row / G, hs = row - tok * G;
-  const bool live = tid < kPpRows && row < it.n_rows && (unsigned)(it.tok0 + tok) < (unsigned)a.rows;
+  const bool live = tid < kPpSoftmax && row < it.n_rows && (unsigned)(it.tok0 + tok) < (unsigned)a.rows;
 
-  if (warp == 8) {
+  if (warp == kPpSoftmax / 32) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(&tmem_base)),
                  "r"(512)
                  : "memory");
@@ -262,8 +299,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
     for (int i = 0; i < 2; ++i) {
       tc_mbar_init(&s_full[i]);
       tc_mbar_init(&o_done[i]);
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 128;" ::"r"(tc_smem(&p_full[i])) : "memory");
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 128;" ::"r"(tc_smem(&q_full[i])) : "memory");
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 256;" ::"r"(tc_smem(&p_full[i])) : "memory");
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 256;" ::"r"(tc_smem(&q_full[i])) : "memory");
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     failed = 0;
@@ -271,11 +308,11 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const unsigned tmem = tmem_base;
+  const unsigned tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
 
-  if (warp >= 8) {
+  if (warp >= kPpSoftmax / 32) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPpRegsFew));
-  if (warp == 9 && nk > 0) {
+    if (warp == kPpSoftmax / 32 + 1 && nk > 0) {
     // ---- copies: K and V tiles alternate through the ring ----
     const int ps = 1 << a.kv.page_shift, box = min(ps, kPpKeys), boxes = kPpKeys / box;
     unsigned raw_phase = 0;
@@ -335,238 +372,264 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
     // nothing may still be landing when the CTA ends
     for (int i = max(0, issued_to - S + 1); i <= issued_to; ++i)
       (void)tc_mbar_wait(&full[i % S], (unsigned)(i / S) & 1u);
-  } else if (warp == 8 && nk > 0) {
-    // ---- MMA issue (one lane) ----
-    if (lane == 0) {
-      const unsigned id_s = pp_idesc<T>(false), id_o = pp_idesc<T>(true);
-      auto scores = [&](int t, int slot) {  // S_t = Q_t K^T
-        const unsigned qb = tc_smem(qs + t * kQTile), kb = tc_smem(ring + slot * kPpTileBytes);
+  } else if (warp == kPpSoftmax / 32 && nk > 0) {
+    // ---- MMA issue ----
+    // The whole warp runs the loop, so that the descriptors are warp-uniform values, and one lane issues.
+    // (Under `if (lane == 0)` each of the 16 products of a tile and its operands took 90 cycles to issue,
+    // more than the 64 that it runs.)
+    const unsigned id_s = pp_idesc<T>(false), id_o = pp_idesc<T>(true), leader = lane == 0;
+    const unsigned long long dq = umma_desc_k_sw128(tc_smem(qs)), dk = umma_desc_k_sw128(tc_smem(ring));
+    const unsigned long long dv = umma_desc_mn_sw128(tc_smem(ring));
+    auto scores = [&](int t, int slot) {  // S_t = Q_t K^T
+      const unsigned long long q0 = dq + (unsigned)(t * (kQTile >> 4)), k0 = dk + (unsigned)(slot * (kPpTileBytes >> 4));
+#pragma unroll
+      for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          const unsigned off = ((ks >> 2) * (kPpTileBytes / 2) + (ks & 3) * 32) >> 4;
+          if (part == 0 && ks == 0) pp_mma_ss<false>(tmem + t * 128, q0, k0, id_s, leader);
+          else pp_mma_ss<true>(tmem + t * 128, q0 + part * (kPpTileBytes >> 4) + off, k0 + off, id_s, leader);
+        }
+      pp_commit(&s_full[t], leader);
+    };
+    bool ok = __all_sync(0xffffffffu, pp_wait(&full[0], 0, &failed));
+    for (int t = 0; t < halves && ok; ++t) {
+      ok = __all_sync(0xffffffffu, pp_wait(&q_full[t], 0, &failed));
+      tc_fence_after();
+      if (ok) scores(t, 0);
+    }
+    if (ok) pp_commit(&empty[0], leader);
+    int vs = 1 % S, ks_slot = 2 % S;       // ring slots of V of tile j and K of tile j + 1,
+    unsigned vph = 0, kph = 2 / S & 1u;    // and their phases
+    for (int j = 0; j < nk && ok; ++j) {
+      ok = pp_wait(&full[vs], vph, &failed);
+      if (j + 1 < nk) ok = pp_wait(&full[ks_slot], kph, &failed) && ok;
+      ok = __all_sync(0xffffffffu, ok);
+      for (int t = 0; t < halves && ok; ++t) {
+        ok = __all_sync(0xffffffffu, pp_wait(&p_full[t], (unsigned)j & 1u, &failed));
+        if (!ok) break;
+        tc_fence_after();
+        const unsigned long long v0 = dv + (unsigned)(vs * (kPpTileBytes >> 4));
+        const unsigned od = tmem + 256 + t * 128, pd = tmem + t * 128;
 #pragma unroll
         for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks) {
-            const unsigned off = (ks >> 2) * (kPpTileBytes / 2) + (ks & 3) * 32;
-            umma_f16(tmem + t * 128, umma_desc_k_sw128(qb + part * kPpTileBytes + off), umma_desc_k_sw128(kb + off), id_s,
-                     part > 0 || ks > 0);
+            if (part == 0 && ks == 0) pp_mma_ts(od, pd, v0, id_o, j > 0, leader);
+            else pp_mma_ts(od, pd + part * 64 + ks * 8, v0 + ks * (2048 >> 4), id_o, true, leader);
           }
-        umma_commit(&s_full[t]);
-      };
-      bool ok = pp_wait(&full[0], 0, &failed);
-      for (int t = 0; t < halves && ok; ++t) {
-        ok = pp_wait(&q_full[t], 0, &failed);
-        tc_fence_after();
-        if (ok) scores(t, 0);
-      }
-      if (ok) umma_commit(&empty[0]);
-      for (int j = 0; j < nk && ok; ++j) {
-        const int vi = 2 * j + 1, vs = vi % S, ki = 2 * j + 2, ks_slot = ki % S;
-        ok = pp_wait(&full[vs], (unsigned)(vi / S) & 1u, &failed);
-        if (ok && j + 1 < nk) ok = pp_wait(&full[ks_slot], (unsigned)(ki / S) & 1u, &failed);
-        for (int t = 0; t < halves && ok; ++t) {
-          ok = pp_wait(&p_full[t], (unsigned)j & 1u, &failed);
-          if (!ok) break;
-          tc_fence_after();
-          const unsigned vb = tc_smem(ring + vs * kPpTileBytes);
-#pragma unroll
-          for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks)
-              umma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + part * 64 + ks * 8, umma_desc_mn_sw128(vb + ks * 2048),
-                          id_o, j > 0 || part > 0 || ks > 0);
-          umma_commit(&o_done[t]);
-          if (t == halves - 1) umma_commit(&empty[vs]);
-          if (j + 1 < nk) {
-            scores(t, ks_slot);
-            if (t == halves - 1) umma_commit(&empty[ks_slot]);
-          }
+        pp_commit(&o_done[t], leader);
+        if (t == halves - 1) pp_commit(&empty[vs], leader);
+        if (j + 1 < nk) {
+          scores(t, ks_slot);
+          if (t == halves - 1) pp_commit(&empty[ks_slot], leader);
         }
       }
-      if (!ok) {  // given up: let what was issued finish before the CTA ends
-        umma_commit(&drain);
-        (void)tc_mbar_wait(&drain, 0);
-      }
+      vs += 2;
+      if (vs >= S) vs -= S, vph ^= 1u;
+      ks_slot += 2;
+      if (ks_slot >= S) ks_slot -= S, kph ^= 1u;
+    }
+    if (!ok) {  // given up: let what was issued finish before the CTA ends
+      pp_commit(&drain, leader);
+      (void)tc_mbar_wait(&drain, 0);
     }
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPpRegsMany));
-  if ((warp >> 2) < halves && nk > 0) {
-    // ---- softmax: one row per thread ----
-    float m = -INFINITY, l = 0.0f;
-    const int t = warp >> 2;
-    // Q: one row per thread, K-major with the 128-byte swizzle; dead rows are zero. A negative scale
-    // changes the sign of q, so that the softmax always has a positive one.
-    {
-    const int r = tid & 127;
-    unsigned char* dst = qs + (tid >> 7) * kQTile + r * 128;
-    const long long base = (long long)(it.tok0 + (live ? tok : 0)) * a.q_stride + ((long long)g * G + hs) * kHeadDim;
-    if constexpr (SPLIT) {
-#pragma unroll 8
-      for (int c = 0; c < 16; ++c) {
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-        if (live) {
-          x = load4<float>(a.q, base + 8 * c);
-          y = load4<float>(a.q, base + 8 * c + 4);
-          if (a.scale < 0.0f) {
-            x = make_float4(-x.x, -x.y, -x.z, -x.w);
-            y = make_float4(-y.x, -y.y, -y.z, -y.w);
+    if (t < halves && nk > 0) {
+      // ---- softmax: half a row per thread ----
+      // Q: K-major with the 128-byte swizzle; dead rows are zero. A negative scale changes the sign of q,
+      // so that the softmax always has a positive one.
+      {
+        const int r = tid & 127;
+        unsigned char* dst = qs + t * kQTile + hf * (kPpTileBytes / 2) + r * 128;
+        const long long base =
+            (long long)(it.tok0 + (live ? tok : 0)) * a.q_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf;
+        if constexpr (SPLIT) {
+#pragma unroll 4
+          for (int c = 0; c < 8; ++c) {
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+            if (live) {
+              x = load4<float>(a.q, base + 8 * c);
+              y = load4<float>(a.q, base + 8 * c + 4);
+              if (a.scale < 0.0f) {
+                x = make_float4(-x.x, -x.y, -x.z, -x.w);
+                y = make_float4(-y.x, -y.y, -y.z, -y.w);
+              }
+            }
+            uint4 hi, lo;
+            split2<T>(x.x, x.y, hi.x, lo.x);
+            split2<T>(x.z, x.w, hi.y, lo.y);
+            split2<T>(y.x, y.y, hi.z, lo.z);
+            split2<T>(y.z, y.w, hi.w, lo.w);
+            const unsigned off = ((c ^ r) & 7) << 4;
+            *reinterpret_cast<uint4*>(dst + off) = hi;
+            *reinterpret_cast<uint4*>(dst + kPpTileBytes + off) = lo;
+          }
+        } else {
+          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + base);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint4 x = live ? src[c] : make_uint4(0, 0, 0, 0);
+            if (a.scale < 0.0f)
+              x = make_uint4(x.x ^ 0x80008000u, x.y ^ 0x80008000u, x.z ^ 0x80008000u, x.w ^ 0x80008000u);
+            *reinterpret_cast<uint4*>(dst + (((c ^ r) & 7) << 4)) = x;
           }
         }
-        uint4 h, l;
-        split2<T>(x.x, x.y, h.x, l.x);
-        split2<T>(x.z, x.w, h.y, l.y);
-        split2<T>(y.x, y.y, h.z, l.z);
-        split2<T>(y.z, y.w, h.w, l.w);
-        const unsigned off = (c >> 3) * (kPpTileBytes / 2) + (((c ^ r) & 7) << 4);
-        *reinterpret_cast<uint4*>(dst + off) = h;
-        *reinterpret_cast<uint4*>(dst + kPpTileBytes + off) = l;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
-    } else {
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + base);
+      pp_arrive(&q_full[t]);
+      float m = -INFINITY, l = 0.0f;
+      const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
+      const unsigned ts = tmem + t * 128 + lanes, to = tmem + 256 + t * 128 + 64 * hf + lanes;
+      const int pair = 1 + t * 4 + (warp & 3);  // named barrier of the two warps that share 32 rows
+      const float c = fabsf(a.scale) * kLog2e;
+      const int p = live ? it.pos0 + tok : -1;
+      const int pmax = min(p, it.len - 1);
+      const int phi = a.window > 0 ? p - a.window : -2;  // keys up to here are hidden, unless sinks
+      // positions of the warp's first and last live rows
+      const unsigned lv = __ballot_sync(0xffffffffu, live);
+      const int pw0 = __shfl_sync(0xffffffffu, p, 0), pw1 = __shfl_sync(0xffffffffu, p, lv ? 31 - __clz(lv) : 0);
+      bool ok = true;  // (a warp that has given up still meets its partner at their barriers, where both end)
+      for (int j = 0; j < nk; ++j) {
+        ok = ok && __all_sync(0xffffffffu, pp_wait(&s_full[t], (unsigned)j & 1u, &failed));
+        tc_fence_after();
+        unsigned sr[64];
+        tmem_ld64(ts + 64 * hf, sr);
+        const int k0 = it.v.tile(t0 + j) * kPpKeys;
+        const unsigned bad = bad_rows[j & 7];
+        const bool inside = lv == 0xffffffffu && bad == 0 && k0 + kPpKeys - 1 <= min(pw0, it.len - 1) &&
+                            (a.window == 0 || k0 > pw1 - a.window || k0 + kPpKeys <= a.sinks);
+        if (!inside) {
+          // bit i of a word: key at + i is visible to this row
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        uint4 x = live ? src[c] : make_uint4(0, 0, 0, 0);
-        if (a.scale < 0.0f)
-          x = make_uint4(x.x ^ 0x80008000u, x.y ^ 0x80008000u, x.z ^ 0x80008000u, x.w ^ 0x80008000u);
-        *reinterpret_cast<uint4*>(dst + (c >> 3) * (kPpTileBytes / 2) + (((c ^ r) & 7) << 4)) = x;
-      }
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  }
-    pp_arrive(&q_full[t]);
-    const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
-    const unsigned ts = tmem + t * 128 + lanes, to = tmem + 256 + t * 128 + lanes;
-    const float c = fabsf(a.scale) * kLog2e;
-    const int p = live ? it.pos0 + tok : -1;
-    const int pmax = min(p, it.len - 1);
-    const int phi = a.window > 0 ? p - a.window : -2;  // keys up to here are hidden, unless sinks
-    // positions of the warp's first and last live rows
-    const unsigned lv = __ballot_sync(0xffffffffu, live);
-    const int pw0 = __shfl_sync(0xffffffffu, p, 0), pw1 = __shfl_sync(0xffffffffu, p, lv ? 31 - __clz(lv) : 0);
-    bool ok = true;
-    for (int j = 0; j < nk; ++j) {
-      ok = pp_wait(&s_full[t], (unsigned)j & 1u, &failed);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tc_fence_after();
-      unsigned sr[128];
-      tmem_ld64(ts, sr);
-      tmem_ld64(ts + 64, sr + 64);
-      const int k0 = it.v.tile(t0 + j) * kPpKeys;
-      const unsigned bad = bad_rows[j & 7];
-      const bool inside = lv == 0xffffffffu && bad == 0 && k0 + kPpKeys - 1 <= min(pw0, it.len - 1) &&
-                          (a.window == 0 || k0 > pw1 - a.window || k0 + kPpKeys <= a.sinks);
-      if (!inside) {
-        // bit i of a word: key k0 + 32 w + i is visible to this row
+          for (int w = 0; w < 2; ++w) {
+            const int at = k0 + 64 * hf + 32 * w, b = bad >> (4 * hf + 2 * w);
+            unsigned see = pp_below(pmax + 1 - at) & (~pp_below(phi + 1 - at) | pp_below(a.sinks - at));
+            if (b & 1) see &= 0xffff0000u;
+            if (b & 2) see &= 0x0000ffffu;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const int at = k0 + 32 * w;
-          unsigned see = pp_below(pmax + 1 - at) & (~pp_below(phi + 1 - at) | pp_below(a.sinks - at));
-          if ((bad >> (2 * w)) & 1u) see &= 0xffff0000u;
-          if ((bad >> (2 * w)) & 2u) see &= 0x0000ffffu;
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!((see >> i) & 1u)) sr[32 * w + i] = 0xff800000u;
+            for (int i = 0; i < 32; ++i)
+              if (!((see >> i) & 1u)) sr[32 * w + i] = 0xff800000u;
+          }
         }
-      }
-      float mx[4];
+        float mx[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(sr[e]);
+        for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(sr[e]);
 #pragma unroll
-      for (int i = 4; i < 124; i += 8)
+        for (int i = 4; i < 60; i += 8)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sr[i + e]), __uint_as_float(sr[i + 4 + e]));
+          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sr[i + e]), __uint_as_float(sr[i + 4 + e]));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sr[124 + e]), -INFINITY);
-      const float mt = max3(max3(mx[0], mx[1], mx[2]), mx[3], -INFINITY) * c;  // NaN where a score is
-      if (__any_sync(0xffffffffu, mt > m + kPpLag)) {
-        // each row by its own maximum (a factor of 1 where it has not moved), so that a row's result
-        // does not depend on the rows beside it
-        const float mn = mt > m + kPpLag ? mt : m;
-        const float f = m == -INFINITY ? 0.0f : exp2_fast(m - mn);
-        m = mn;
-        l *= f;
-        if (j > 0) {  // the product of the tile before must have reached O
-          ok = pp_wait(&o_done[t], (unsigned)(j - 1) & 1u, &failed);
-          ok = __all_sync(0xffffffffu, ok);
+        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sr[60 + e]), -INFINITY);
+        float mt = max3(max3(mx[0], mx[1], mx[2]), mx[3], -INFINITY) * c;  // NaN where a score is
+        // This barrier also stands between every read of S and the writes of P over it.
+        if (pp_any(pair, !ok || mt > m + kPpLag)) {
+          // The first thread's maximum to the second, the larger one back. (A NaN maximum moves nothing: its
+          // row becomes NaN by its weights.)
+          const float gone = __int_as_float(0x7fffffff);
+          if (!(mt == mt)) mt = -INFINITY;
+          if (hf == 0) shared_row[lr] = ok ? mt : gone;
+          pp_meet(pair);
+          if (hf == 1) {
+            const float other = shared_row[lr];
+            shared_row[lr] = ok && other == other ? fmaxf(mt, other) : gone;
+          }
+          pp_meet(pair);
+          mt = shared_row[lr];
+          ok = __all_sync(0xffffffffu, mt == mt);
           if (!ok) break;
-          tc_fence_after();
+          // each row by its own maximum (a factor of 1 where it has not moved), so that a row's result
+          // does not depend on the rows beside it
+          const float mn = mt > m + kPpLag ? mt : m;
+          const float f = m == -INFINITY ? 0.0f : exp2_fast(m - mn);
+          m = mn;
+          l *= f;
+          if (j > 0) {  // the product of the tile before must have reached O
+            ok = __all_sync(0xffffffffu, pp_wait(&o_done[t], (unsigned)(j - 1) & 1u, &failed));
+            tc_fence_after();
 #pragma unroll 1
-          for (int h = 0; h < 8; ++h) {
-            unsigned o[16];
-            tmem_ld16(to + 16 * h, o);
+            for (int h = 0; h < 4; ++h) {
+              unsigned o[16];
+              tmem_ld16(to + 16 * h, o);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_st16(to + 16 * h, o);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st16(to + 16 * h, o);
+            }
           }
         }
-      }
-      const float ref = m == -INFINITY ? 0.0f : kPpShift - m;
-      float2 sum = make_float2(0.f, 0.f);
+        const float ref = m == -INFINITY ? 0.0f : kPpShift - m;
+        float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {  // 32 keys: 16 packed columns
-        unsigned w[16], wl[SPLIT ? 16 : 1];
+        for (int h = 0; h < 2; ++h) {  // 32 keys: 16 packed columns
+          unsigned w[16], wl[SPLIT ? 16 : 1];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float s0 = __uint_as_float(sr[32 * h + 2 * i]), s1 = __uint_as_float(sr[32 * h + 2 * i + 1]);
-          float2 e = __ffma2_rn(make_float2(s0, s1), make_float2(c, c), make_float2(ref, ref));
-          e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-          sum = __fadd2_rn(sum, e);
-          if constexpr (SPLIT) split2<T>(e.x, e.y, w[i], wl[i]);
-          else w[i] = pack2<T>(e.x, e.y);
+          for (int i = 0; i < 16; ++i) {
+            const float s0 = __uint_as_float(sr[32 * h + 2 * i]), s1 = __uint_as_float(sr[32 * h + 2 * i + 1]);
+            float2 e = __ffma2_rn(make_float2(s0, s1), make_float2(c, c), make_float2(ref, ref));
+            e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+            sum = __fadd2_rn(sum, e);
+            if constexpr (SPLIT) split2<T>(e.x, e.y, w[i], wl[i]);
+            else w[i] = pack2<T>(e.x, e.y);
+          }
+          tmem_st16(ts + 32 * hf + 16 * h, w);
+          if constexpr (SPLIT) tmem_st16(ts + 64 + 32 * hf + 16 * h, wl);
         }
-        tmem_st16(ts + 16 * h, w);
-        if constexpr (SPLIT) tmem_st16(ts + 64 + 16 * h, wl);
+        l += sum.x + sum.y;
+        tmem_wait_st();
+        tc_fence_before();
+        if (ok) pp_arrive(&p_full[t]);
       }
-      l += sum.x + sum.y;
-      tmem_wait_st();
-      tc_fence_before();
-      pp_arrive(&p_full[t]);
-    }
-    if (ok) {
-      ok = pp_wait(&o_done[t], (unsigned)(nk - 1) & 1u, &failed);
-      ok = __all_sync(0xffffffffu, ok);
-    }
-    if (ok) {
-      tc_fence_after();
-      const bool whole = parts == 1;
-      const float f = whole ? inv_sum(l) : 1.0f;
-      const long long prow = (((long long)item * kvh + g) * pa.splits + z) * kPpRows + tid;
-      const long long base = (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + hs) * kHeadDim;
-      if (!whole) pa.pml[prow] = make_float2(m, l);
+      pp_meet(pair);  // (the last maximum has been read)
+      if (hf == 0) shared_row[lr] = l;
+      pp_meet(pair);
+      if (hf == 1) shared_row[lr] += l;
+      pp_meet(pair);
+      l = shared_row[lr];
+      if (ok) ok = __all_sync(0xffffffffu, pp_wait(&o_done[t], (unsigned)(nk - 1) & 1u, &failed));
+      if (ok) {
+        tc_fence_after();
+        const bool whole = parts == 1;
+        const float f = whole ? inv_sum(l) : 1.0f;
+        const long long prow = (((long long)item * kvh + g) * pa.splits + z) * kPpRows + lr;
+        const long long base = (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf;
+        if (!whole && hf == 0) pa.pml[prow] = make_float2(m, l);
 #pragma unroll 1
-      for (int h = 0; h < 4; ++h) {
-        float o[32];
-        tmem_ld32(to + 32 * h, o);
-        if (!whole) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4*>(pa.po + prow * kHeadDim + 32 * h + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-        } else if (live) {
-          if constexpr (SPLIT) {
+        for (int h = 0; h < 2; ++h) {
+          float o[32];
+          tmem_ld32(to + 32 * h, o);
+          if (!whole) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<float4*>(static_cast<float*>(a.y) + base + 32 * h + i) =
-                  make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f);
-          } else {
+              *reinterpret_cast<float4*>(pa.po + prow * kHeadDim + 64 * hf + 32 * h + i) =
+                  make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          } else if (live) {
+            if constexpr (SPLIT) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 8)
-              *reinterpret_cast<uint4*>(static_cast<T*>(a.y) + base + 32 * h + i) =
-                  make_uint4(pack2<T>(o[i] * f, o[i + 1] * f), pack2<T>(o[i + 2] * f, o[i + 3] * f),
-                             pack2<T>(o[i + 4] * f, o[i + 5] * f), pack2<T>(o[i + 6] * f, o[i + 7] * f));
+              for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<float4*>(static_cast<float*>(a.y) + base + 32 * h + i) =
+                    make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; i += 8)
+                *reinterpret_cast<uint4*>(static_cast<T*>(a.y) + base + 32 * h + i) =
+                    make_uint4(pack2<T>(o[i] * f, o[i + 1] * f), pack2<T>(o[i + 2] * f, o[i + 3] * f),
+                               pack2<T>(o[i + 4] * f, o[i + 5] * f), pack2<T>(o[i + 6] * f, o[i + 7] * f));
+            }
           }
         }
       }
     }
   }
-  }
   if (nk == 0 && live) {  // no key is visible to any row
-    const long long base = (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + hs) * kHeadDim;
-    for (int i = 0; i < kHeadDim; i += 4) store4(a.y, base + i, a.dtype, make_float4(0.f, 0.f, 0.f, 0.f));
+    const long long base = (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf;
+    for (int i = 0; i < kHeadDim / 2; i += 4) store4(a.y, base + i, a.dtype, make_float4(0.f, 0.f, 0.f, 0.f));
   }
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && failed) paged_flag(a.kv, QD_PAGED_TIMEOUT);
-  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (warp == kPpSoftmax / 32) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 // Adds the parts of rows whose key tiles were split. One warp per row; grid: items * kv_heads * 32.
