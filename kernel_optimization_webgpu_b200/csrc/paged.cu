@@ -116,10 +116,13 @@ static void launch_prompt(const PAttnArgs& a, const void* q_any, void* workspace
   const unsigned box = std::min(1 << a.kv.page_shift, kPpKeys);
   // (an empty pool has no page that could be copied: any address will do)
   const uint64_t pool = std::max<uint64_t>((uint64_t)a.kv.num_pages * a.kv.kv_heads << a.kv.page_shift, box);
+  if (pool > 0x7fffffffULL) throw QdError{QD_E_RANGE, "qd_paged_attn_prompt: a pool beyond 2^31 rows"};
   std::string err;
   if (!make_tmap_2d(&p.tk, a.kv.num_pages ? a.kv.k : q_any, type, kHeadDim, pool, kHeadDim * 2, 64, box,
                     CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
       !make_tmap_2d(&p.tv, a.kv.num_pages ? a.kv.v : q_any, type, kHeadDim, pool, kHeadDim * 2, 64, box,
+                    CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
+      !make_tmap_2d(&p.tv16, a.kv.num_pages ? a.kv.v : q_any, type, kHeadDim, pool, kHeadDim * 2, 64, 16,
                     CU_TENSOR_MAP_SWIZZLE_128B, &err))
     throw QdError{QD_E_CUDA, err};
   static unsigned long long smem_set = 0;

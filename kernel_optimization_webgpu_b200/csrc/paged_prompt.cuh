@@ -20,8 +20,8 @@
 // issued twice, which keeps f32 accuracy on an f16 cache.
 //
 // K and V come page by page by TMA (128-byte swizzle; rows of a page and head are contiguous)
-// into a ring of 32 KB tiles. V rows that no query of the CTA sees are cleared in shared memory:
-// their weight is 0, but 0 times what a recycled page holds could be NaN.
+// into a ring of 32 KB tiles. V rows that no query of the CTA sees are zeros in shared memory: their
+// weight is 0, but 0 times what a recycled page holds could be NaN.
 //
 // Few rows over a long cache (a chunk behind a long context): the key tiles of a CTA's rows are
 // split over gridDim parts whose sums k_paged_prompt_join adds in order.
@@ -47,7 +47,7 @@ constexpr int kPpMaxSplits = 32;
 constexpr float kPpLag = 8.0f, kPpShift = 7.0f;
 
 struct PPromptArgs {
-  CUtensorMap tk, tv;
+  CUtensorMap tk, tv, tv16;  // boxes of a page (at most 128 rows), and of 16 rows
   PAttnArgs a;
   int splits;
   float* po;     // [item][split][256][128] unnormalised
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
   unsigned char* qs =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* ring = qs + 2 * kQTile;
-  __shared__ unsigned long long full[S], raw, empty[S], s_full[2], p_full[2], o_done[2], q_full[2], drain;
+  __shared__ unsigned long long full[S], empty[S], s_full[2], p_full[2], o_done[2], q_full[2], drain;
   __shared__ unsigned bad_rows[8];  // of key tile j: bit i set where 16-key chunk i has no usable page
   __shared__ unsigned tmem_base;
   __shared__ float shared_row[kPpRows];  // between a row's two threads: a maximum (NaN: given up), then a sum
@@ -294,7 +294,6 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       tc_mbar_init(&full[i]);
       tc_mbar_init(&empty[i]);
     }
-    tc_mbar_init(&raw);
     tc_mbar_init(&drain);
     for (int i = 0; i < 2; ++i) {
       tc_mbar_init(&s_full[i]);
@@ -315,7 +314,6 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
     if (warp == kPpSoftmax / 32 + 1 && nk > 0) {
     // ---- copies: K and V tiles alternate through the ring ----
     const int ps = 1 << a.kv.page_shift, box = min(ps, kPpKeys), boxes = kPpKeys / box;
-    unsigned raw_phase = 0;
     int issued_to = -1;
     bool ok = true;
     for (int i = 0; i < 2 * nk && ok; ++i) {
@@ -332,39 +330,65 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       const bool partial = !(k0 + kPpKeys <= it.v.end && (k0 >= it.v.lo || k0 + kPpKeys <= it.v.ns)) || good != seen;
-      const bool clear = is_v && partial;
       unsigned char* dst = ring + slot * kPpTileBytes;
-      unsigned long long* bar = clear ? &raw : &full[slot];
-      if (lane == 0) {
-        if (!is_v) {
-          unsigned bad = 0;
-          for (int n = 0; n < boxes; ++n)
-            if (((seen & ~good) >> n) & 1u) bad |= ((1u << (box / 16)) - 1u) << (n * (box / 16));
-          bad_rows[j & 7] = bad;
-          if (bad) paged_flag(a.kv, QD_PAGED_BAD_PAGE);
-        }
-        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc_smem(bar)),
-                     "r"(__popc(good) * box * 256)
-                     : "memory");
+      if (lane == 0 && !is_v) {
+        unsigned bad = 0;
+        for (int n = 0; n < boxes; ++n)
+          if (((seen & ~good) >> n) & 1u) bad |= ((1u << (box / 16)) - 1u) << (n * (box / 16));
+        bad_rows[j & 7] = bad;
+        if (bad) paged_flag(a.kv, QD_PAGED_BAD_PAGE);
       }
-      __syncwarp();
-      if (page >= 0) {
-        const int y = (page * kvh + g) * ps + (p0 & (ps - 1));
-        unsigned char* d = dst + lane * box * 128;
-        tma_load_2d(d, is_v ? &pa.tv : &pa.tk, 0, y, bar);
-        tma_load_2d(d + kPpTileBytes / 2, is_v ? &pa.tv : &pa.tk, 64, y, bar);
-      }
-      if (clear) {
-        ok = pp_wait(&raw, raw_phase, &failed);
-        ok = __all_sync(0xffffffffu, ok);
-        raw_phase ^= 1u;
-        for (int e = lane; e < kPpKeys * 16; e += 32) {
-          const int r = e >> 4, c = e & 15, pos = k0 + r;
-          const bool keep = it.v.at(pos) && ((good >> (r / box)) & 1u);
-          if (!keep) *reinterpret_cast<uint4*>(dst + (c >> 3) * (kPpTileBytes / 2) + r * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (!(is_v && partial)) {  // whole boxes (what they hold of hidden keys gives scores that are masked)
+        if (lane == 0)
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc_smem(&full[slot])),
+                       "r"(__popc(good) * box * 256)
+                       : "memory");
         __syncwarp();
+        if (page >= 0) {
+          const int y = (page * kvh + g) * ps + (p0 & (ps - 1));
+          unsigned char* d = dst + lane * box * 128;
+          tma_load_2d(d, is_v ? &pa.tv : &pa.tk, 0, y, &full[slot]);
+          tma_load_2d(d + kPpTileBytes / 2, is_v ? &pa.tv : &pa.tk, 64, y, &full[slot]);
+        }
+      } else {
+        // V of a tile with hidden rows, by groups of 16: TMA copies a group that is wholly visible and, from
+        // outside the tensor, the zeros of one that is wholly hidden; the rows of a group with both
+        // are copied or cleared one by one. (Clearing after the copy, row by row, cost 33 of 158 us
+        // where every row has a window: 5 ragged chunks of up to 1500 tokens.)
+        const int g0 = k0 + 16 * lane, gpage = __shfl_sync(0xffffffffu, page, (16 * (lane & 7)) / box);
+        bool all = lane < 8 && gpage >= 0, some = false;
+        if (all) {
+          some = g0 < it.v.end && (g0 + 16 > it.v.lo || g0 < it.v.ns);
+          all = g0 + 16 <= it.v.end && (g0 >= it.v.lo || g0 + 16 <= it.v.ns);
+        }
+        const unsigned edge = __ballot_sync(0xffffffffu, some && !all);
+        if (lane == 0)
+          asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(tc_smem(&full[slot])),
+                       "r"((8 - __popc(edge)) * 4096)
+                       : "memory");
+        __syncwarp();
+        if (lane < 8 && !((edge >> lane) & 1u)) {
+          const int y = all ? (gpage * kvh + g) * ps + (g0 & (ps - 1)) : -16;
+          unsigned char* d = dst + lane * 16 * 128;
+          tma_load_2d(d, &pa.tv16, 0, y, &full[slot]);
+          tma_load_2d(d + kPpTileBytes / 2, &pa.tv16, 64, y, &full[slot]);
+        }
+        for (unsigned left = edge; left; left &= left - 1) {
+          const int n = __ffs(left) - 1, q0 = k0 + 16 * n;
+          const long long row = ((long long)__shfl_sync(0xffffffffu, gpage, n) * kvh + g) * ps + (q0 & (ps - 1));
+          const char* src = static_cast<const char*>(a.kv.v) + row * 256 + (lane & 15) * 16;
+          const unsigned d = tc_smem(dst) + ((lane & 15) >> 3) * (kPpTileBytes / 2) + n * 16 * 128;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int r = 2 * e + (lane >> 4);
+            cp_async16(d + r * 128 + (((lane ^ r) & 7) << 4), src + r * 256, it.v.at(q0 + r));
+          }
+        }
+        if (edge) {
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
         if (lane == 0) pp_arrive(&full[slot]);
       }
       issued_to = i;
