@@ -176,7 +176,7 @@ def run(s):
         if op == "append":
             q = R.paged_append(s["qkv"], s["k"], s["v"], s["table"], s["lens"], s["cos"], s["sin"], c["q_heads"],
                                q_norm=s["q_norm"], k_norm=s["k_norm"], q_starts=s["starts"])
-            return q, s["k"], s["v"]
+            return q.view(s["rows"], c["q_heads"], D), s["k"], s["v"]
         if op == "decode":
             return R.paged_attn_decode(s["q"], s["k"], s["v"], s["table"], s["lens"], window=c["window"],
                                        sinks=c["sinks"])
