@@ -75,37 +75,41 @@ static PAttnArgs check_attn(const qd_paged_kv* kv, const void* q, int dtype, int
   return a;
 }
 
-template <typename T>
+template <typename T, bool THREE>
 static void launch_decode(const PAttnArgs& a, void* workspace, cudaStream_t s) {
   static unsigned long long smem_set = 0;
-  allow_smem(k_paged_decode<T>, pd_smem(4096), smem_set);
+  allow_smem(k_paged_decode<T, THREE>, pd_smem(4096), smem_set);
   const int nh = a.kv.kv_heads * ((a.q_heads / a.kv.kv_heads + 7) / 8);
   // two CTAs an SM hold all of them at once; no more than there can be units
   const long long most = (long long)a.kv.batch * nh * (((long long)a.kv.table_width << a.kv.page_shift) / kPdTile + 1);
   if (most > 0x7fffffffLL) throw QdError{QD_E_RANGE, "qd_paged_attn_decode: batch * heads * table beyond 2^31 units"};
   const int ctas = (int)std::max(1LL, std::min<long long>(most, std::min(2 * current_sms(), kPdMaxCtas)));
-  launch_ex(k_paged_decode<T>, dim3(ctas), dim3(kPdThreads), (size_t)pd_smem(a.kv.batch), s, a, workspace);
-  launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas);
+  launch_ex(k_paged_decode<T, THREE>, dim3(ctas), dim3(kPdThreads), (size_t)pd_smem(a.kv.batch), s, a, workspace);
+  // (a table of one unit leaves nothing to join)
+  if ((a.kv.table_width << a.kv.page_shift) > kPdTile)
+    launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas);
 }
 
 // Row tiles of a call (at most), and the parts that their keys are split into: enough to give
 // every SM a CTA, none where the row tiles alone do.
-static int prompt_items(int batch, int rows, int group) {
-  return (int)((long long)rows * group / kPpRows) + std::min(batch, rows);
+static int prompt_items(int batch, int rows, int group, int cta_rows) {
+  return (int)((long long)rows * group / cta_rows) + std::min(batch, rows);
 }
 static int prompt_splits(int items, int kv_heads) {
   const long long n = (long long)items * kv_heads;
   return n == 0 ? 1 : (int)std::max(1LL, std::min<long long>(kPpMaxSplits, current_sms() / n));
 }
 
-template <typename T, bool SPLIT>
+template <typename T, int PARTS>
 static void launch_prompt(const PAttnArgs& a, const void* q_any, void* workspace, cudaStream_t s) {
-  const int G = a.q_heads / a.kv.kv_heads, items = prompt_items(a.kv.batch, a.rows, G);
+  constexpr int kRows = 128 * pp_tiles<PARTS>();
+  const int G = a.q_heads / a.kv.kv_heads, items = prompt_items(a.kv.batch, a.rows, G, kRows);
   PPromptArgs p{};
   p.a = a;
+  p.cta_rows = kRows;
   p.splits = prompt_splits(items, a.kv.kv_heads);
   p.po = static_cast<float*>(workspace);
-  p.pml = reinterpret_cast<float2*>(p.po + (size_t)items * a.kv.kv_heads * p.splits * kPpRows * kHeadDim);
+  p.pml = reinterpret_cast<float2*>(p.po + (size_t)items * a.kv.kv_heads * p.splits * kRows * kHeadDim);
   // a table that holds few tiles never splits them into more parts than this
   const long long tiles = (((long long)a.kv.table_width << a.kv.page_shift) + kPpKeys - 1) / kPpKeys;
   p.splits = (int)std::max(1LL, std::min<long long>(p.splits, tiles / 2));
@@ -126,9 +130,9 @@ static void launch_prompt(const PAttnArgs& a, const void* q_any, void* workspace
                     CU_TENSOR_MAP_SWIZZLE_128B, &err))
     throw QdError{QD_E_CUDA, err};
   static unsigned long long smem_set = 0;
-  allow_smem(k_paged_prompt<T, SPLIT>, pp_smem<SPLIT>(), smem_set);
-  launch_ex(k_paged_prompt<T, SPLIT>, dim3((unsigned)grid), dim3(kPpThreads), (size_t)pp_smem<SPLIT>(), s, p);
-  if (p.splits > 1) launch_ex(k_paged_prompt_join, dim3(items * a.kv.kv_heads * 32), dim3(256), 0, s, p);
+  allow_smem(k_paged_prompt<T, PARTS>, pp_smem<PARTS>(), smem_set);
+  launch_ex(k_paged_prompt<T, PARTS>, dim3((unsigned)grid), dim3(kPpThreads), (size_t)pp_smem<PARTS>(), s, p);
+  if (p.splits > 1) launch_ex(k_paged_prompt_join, dim3(items * a.kv.kv_heads * (kRows / 8)), dim3(256), 0, s, p);
 }
 
 }  // namespace qd
@@ -215,15 +219,21 @@ int qd_paged_attn_decode(const qd_paged_kv* kv, const void* q, int dtype, int64_
     if (a.rows == 0) return;
     need(workspace != nullptr, "qd_paged_attn_decode: NULL workspace");
     need(aligned16(workspace), "qd_paged_attn_decode: the workspace must be 16-byte aligned");
-    if (kv->dtype == QD_KV_F16) launch_decode<__half>(a, workspace, static_cast<cudaStream_t>(stream));
-    else launch_decode<__nv_bfloat16>(a, workspace, static_cast<cudaStream_t>(stream));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (kv->dtype == QD_KV_F16) launch_decode<__half, false>(a, workspace, s);
+    else if (dtype == QD_KV_F32) launch_decode<__nv_bfloat16, true>(a, workspace, s);
+    else launch_decode<__nv_bfloat16, false>(a, workspace, s);
   });
 }
 
 size_t qd_paged_attn_prompt_workspace_bytes(int batch, int rows, int q_heads, int kv_heads) {
   if (batch < 0 || rows < 0 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads) return 0;
-  const int items = prompt_items(batch, rows, q_heads / kv_heads), splits = prompt_splits(items, kv_heads);
-  return splits == 1 ? 256 : (size_t)items * kv_heads * splits * kPpRows * (kHeadDim * 4 + 8);
+  size_t most = 256;
+  for (const int cta_rows : {128, 256}) {  // (a CTA's rows depend on the types)
+    const int items = prompt_items(batch, rows, q_heads / kv_heads, cta_rows), splits = prompt_splits(items, kv_heads);
+    if (splits > 1) most = std::max(most, (size_t)items * kv_heads * splits * cta_rows * (kHeadDim * 4 + 8));
+  }
+  return most;
 }
 
 int qd_paged_attn_prompt(const qd_paged_kv* kv, const void* q, int dtype, int64_t q_stride, int rows,
@@ -238,11 +248,11 @@ int qd_paged_attn_prompt(const qd_paged_kv* kv, const void* q, int dtype, int64_
     need(aligned16(workspace), "qd_paged_attn_prompt: the workspace must be 16-byte aligned");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (kv->dtype == QD_KV_F16) {
-      if (dtype == QD_KV_F32) launch_prompt<__half, true>(a, q, workspace, s);
-      else launch_prompt<__half, false>(a, q, workspace, s);
+      if (dtype == QD_KV_F32) launch_prompt<__half, 2>(a, q, workspace, s);
+      else launch_prompt<__half, 1>(a, q, workspace, s);
     } else {
-      if (dtype == QD_KV_F32) launch_prompt<__nv_bfloat16, true>(a, q, workspace, s);
-      else launch_prompt<__nv_bfloat16, false>(a, q, workspace, s);
+      if (dtype == QD_KV_F32) launch_prompt<__nv_bfloat16, 3>(a, q, workspace, s);
+      else launch_prompt<__nv_bfloat16, 1>(a, q, workspace, s);
     }
   });
 }

@@ -18,7 +18,11 @@
 //    operand rounded to 16 bits, rows 8-15 what that rounding left. The two sums of a head meet
 //    in one thread (accumulator rows r and r + 8), so q and the weights keep twice 16 bits'
 //    precision at no extra instruction. (tcgen05 wants 64 rows or more; 56 of them would idle.)
+//    Two bf16 hold only 16 of f32's 24 bits (results were 5e-6 off): with f32 queries on a bf16
+//    cache a second set of products takes the rest of both operands (THREE).
 #pragma once
+
+#include <type_traits>
 
 #include "paged.cuh"
 
@@ -119,6 +123,16 @@ __device__ __forceinline__ void split2<__nv_bfloat16>(float x, float y, unsigned
   hi = *reinterpret_cast<const unsigned*>(&h);
   lo = *reinterpret_cast<const unsigned*>(&l);
 }
+// The pair rounded to 16 bits, and the rest.
+template <typename T>
+__device__ __forceinline__ float2 split2_rest(float x, float y, unsigned& hi) {
+  unsigned lo;
+  split2<T>(x, y, hi, lo);
+  const float2 f = std::is_same<T, __half>::value
+                       ? __half22float2(*reinterpret_cast<const __half2*>(&hi))
+                       : make_float2(__uint_as_float(hi << 16), __uint_as_float(hi & 0xffff0000u));
+  return make_float2(x - f.x, y - f.y);
+}
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -154,7 +168,7 @@ constexpr int kPdSumRow = 136;
 static_assert(8 * kPdSumRow * 4 <= kPdSlot, "a slot holds eight heads' sums");
 __host__ __device__ constexpr int pd_smem(int batch) { return 4 * kPdStages * kPdSlot + (batch + 1) * 4; }
 
-template <typename T>
+template <typename T, bool THREE>
 __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_constant__ PAttnArgs a, void* workspace) {
   extern __shared__ __align__(128) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -200,6 +214,9 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
     for (int b = tid; b < B; b += kPdThreads)
       if (a.kv.seq_lens[b] > paged_len(a.kv, b) && a.kv.seq_lens[b] > 0) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
   }
+  for (int b = blockIdx.x; b < B; b += gridDim.x)  // nothing visible: zeros
+    if (first[b + 1] == first[b])
+      for (int i = tid; i < a.q_heads * kHeadDim; i += kPdThreads) store1(a.y, b * a.y_stride + i, a.dtype, 0.0f);
   const long long U = (long long)first[B] * nh;
   const int ctas = (int)min((long long)gridDim.x, U);  // none of them empty
   if ((int)blockIdx.x >= ctas) return;
@@ -315,7 +332,7 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
     }
   };
   fetch_q(cur);
-  unsigned q[8][4];
+  unsigned q[8][4], q3[THREE ? 8 : 1][2];
   float o[16][4], m = -INFINITY, l = 0.0f;
   bool fresh = true;   // a new (sequence, head): take its q, clear the sums
   int seg = 0;         // segments finished by this CTA
@@ -327,8 +344,15 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
       fresh = false;
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) {
-        split2<T>(qn[2 * kk].x * qs, qn[2 * kk].y * qs, q[kk][0], q[kk][1]);
-        split2<T>(qn[2 * kk + 1].x * qs, qn[2 * kk + 1].y * qs, q[kk][2], q[kk][3]);
+        if constexpr (THREE) {
+          const float2 x = split2_rest<T>(qn[2 * kk].x * qs, qn[2 * kk].y * qs, q[kk][0]);
+          const float2 y = split2_rest<T>(qn[2 * kk + 1].x * qs, qn[2 * kk + 1].y * qs, q[kk][2]);
+          split2<T>(x.x, x.y, q[kk][1], q3[kk][0]);
+          split2<T>(y.x, y.y, q[kk][3], q3[kk][1]);
+        } else {
+          split2<T>(qn[2 * kk].x * qs, qn[2 * kk].y * qs, q[kk][0], q[kk][1]);
+          split2<T>(qn[2 * kk + 1].x * qs, qn[2 * kk + 1].y * qs, q[kk][2], q[kk][3]);
+        }
       }
 #pragma unroll
       for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
@@ -356,6 +380,11 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
         ldsm4(kb + (8 * (mi >> 1) + r8) * 256 + (((2 * kk + (mi & 1)) ^ r8) << 4), b);
         mma_16816<T>(s[2 * (kk & 1)], q[kk], b[0], b[1]);
         mma_16816<T>(s[2 * (kk & 1) + 1], q[kk], b[2], b[3]);
+        if constexpr (THREE) {
+          const unsigned q2[4] = {q3[kk][0], 0u, q3[kk][1], 0u};
+          mma_16816<T>(s[2 * (kk & 1)], q2, b[0], b[1]);
+          mma_16816<T>(s[2 * (kk & 1) + 1], q2, b[2], b[3]);
+        }
       }
       const int p0 = cur.v.tile(cur.t) * kPdTile + 16 * warp;
       float p[2][2];
@@ -394,15 +423,25 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
           p[j][e] = exp2_fast(p[j][e] - ref);
           l += p[j][e];
         }
-      unsigned w[4];
-      split2<T>(p[0][0], p[0][1], w[0], w[1]);
-      split2<T>(p[1][0], p[1][1], w[2], w[3]);
+      unsigned w[4], w3[4] = {0u, 0u, 0u, 0u};
+      if constexpr (THREE) {
+        const float2 x = split2_rest<T>(p[0][0], p[0][1], w[0]), y = split2_rest<T>(p[1][0], p[1][1], w[2]);
+        split2<T>(x.x, x.y, w[1], w3[0]);
+        split2<T>(y.x, y.y, w[3], w3[2]);
+      } else {
+        split2<T>(p[0][0], p[0][1], w[0], w[1]);
+        split2<T>(p[1][0], p[1][1], w[2], w[3]);
+      }
 #pragma unroll
       for (int dn = 0; dn < 16; dn += 2) {
         unsigned b[4];
         ldsm4_t(vb + (r8 + 8 * (mi & 1)) * 256 + (((dn + (mi >> 1)) ^ r8) << 4), b);
         mma_16816<T>(o[dn], w, b[0], b[1]);
         mma_16816<T>(o[dn + 1], w, b[2], b[3]);
+        if constexpr (THREE) {
+          mma_16816<T>(o[dn], w3, b[0], b[1]);
+          mma_16816<T>(o[dn + 1], w3, b[2], b[3]);
+        }
       }
     }
     __syncwarp();  // the slot may be refilled
@@ -446,8 +485,7 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
   }
 }
 
-// Joins the parts of each (sequence, query group) that several CTAs hold, and writes the zeros
-// of sequences without a visible key. Grid: batch * nh. Warp w takes head w / per of the group
+// Joins the parts of each (sequence, query group) that several CTAs hold. Grid: batch * nh. Warp w takes head w / per of the group
 // and every per-th part (per = 8 / heads, a power of two): each lane's loads of up to eight
 // parts are in flight together (with one warp per head, 37 parts took 6 us).
 __global__ void __launch_bounds__(256) k_paged_decode_join(const __grid_constant__ PAttnArgs a, void* workspace,
@@ -462,12 +500,9 @@ __global__ void __launch_bounds__(256) k_paged_decode_join(const __grid_constant
   const long long U = (long long)ws.first[a.kv.batch] * nh;
   const int ctas = (int)min((long long)grid, U);
   const long long v0 = (long long)f0 * nh + (long long)h * tiles, v1 = v0 + tiles;
-  int c0 = 0, c1 = -1;
-  if (tiles > 0) {
-    c0 = (int)(((v0 + 1) * ctas - 1) / U);
-    c1 = (int)((v1 * ctas - 1) / U);
-    if (c0 == c1) return;  // written whole
-  }
+  if (tiles == 0) return;
+  const int c0 = (int)(((v0 + 1) * ctas - 1) / U), c1 = (int)((v1 * ctas - 1) / U);
+  if (c0 == c1) return;  // written whole
   const int lg = heads > 4 ? 0 : heads > 2 ? 1 : heads > 1 ? 2 : 3, per = 1 << lg;
   const int hw = warp >> lg, k0 = warp & (per - 1);
   float M = -INFINITY, L = 0.0f;

@@ -16,8 +16,9 @@
 // (weights then stay below 2^(kPpLag + kPpShift), inside f16); the final division makes up for
 // it, so the result is exact to rounding. P is rounded to the cache's 16-bit type (half a step
 // relative, as the tensor cores take 16-bit operands); its sum is taken in f32 before that.
-// With f32 queries (SPLIT) q and P are each a sum of two 16-bit operands and every product is
-// issued twice, which keeps f32 accuracy on an f16 cache.
+// With f32 queries q and P are each a sum of PARTS 16-bit operands, and every product is issued that
+// many times: two f16 keep 22 bits, two bf16 only 16 (the results were 5e-6 off), so a bf16 cache
+// takes three. Three parts of P do not fit over S in TMEM, so such a CTA has one row tile.
 //
 // K and V come page by page by TMA (128-byte swizzle; rows of a page and head are contiguous)
 // into a ring of 32 KB tiles. V rows that no query of the CTA sees are zeros in shared memory: their
@@ -40,7 +41,6 @@ constexpr int kPpThreads = 640;    // and the MMA warp, the copy warp and two id
 // Registers: 96 a thread at launch (61440 in all); a softmax thread holds 64 scores, so the last
 // warpgroup gives some of its share up: 512 * 104 + 128 * 64 = 61440.
 constexpr int kPpRegsMany = 104, kPpRegsFew = 64;
-constexpr int kPpRows = 256;
 constexpr int kPpKeys = 128;
 constexpr int kPpTileBytes = 128 * 256;  // a 128 x 128 tile of 16-bit elements
 constexpr int kPpMaxSplits = 32;
@@ -50,26 +50,29 @@ struct PPromptArgs {
   CUtensorMap tk, tv, tv16;  // boxes of a page (at most 128 rows), and of 16 rows
   PAttnArgs a;
   int splits;
-  float* po;     // [item][split][256][128] unnormalised
-  float2* pml;   // [item][split][256]
+  int cta_rows;  // 128 times the row tiles of a CTA
+  float* po;     // [item][KV head][split][cta_rows][128] unnormalised
+  float2* pml;   // [item][KV head][split][cta_rows]
 };
 
-template <bool SPLIT>
-__host__ __device__ constexpr int pp_slots() { return SPLIT ? 3 : 5; }
-template <bool SPLIT>
+template <int PARTS>
+__host__ __device__ constexpr int pp_tiles() { return PARTS == 3 ? 1 : 2; }  // row tiles of a CTA
+template <int PARTS>
+__host__ __device__ constexpr int pp_slots() { return PARTS == 1 ? 5 : PARTS == 2 ? 3 : 4; }
+template <int PARTS>
 __host__ __device__ constexpr int pp_smem() {
-  return ((SPLIT ? 4 : 2) + pp_slots<SPLIT>()) * kPpTileBytes + 1024;
+  return (pp_tiles<PARTS>() * PARTS + pp_slots<PARTS>()) * kPpTileBytes + 1024;
 }
 
 // The item-th tile of rows, counted from the last (the latest rows of a prompt see the most keys
 // and start first): its sequence and tile, or false. Called by whole warps.
-__device__ __forceinline__ bool pp_item(const PAttnArgs& a, int G, int item, int& seq, int& tile) {
+__device__ __forceinline__ bool pp_item(const PAttnArgs& a, int G, int cta_rows, int item, int& seq, int& tile) {
   const int lane = threadIdx.x & 31, B = a.kv.batch;
   int total = 0;
   for (int b0 = 0; b0 < B; b0 += 32) {
     const int b = b0 + lane;
     const int n = b < B ? max(a.q_starts[b + 1] - a.q_starts[b], 0) : 0;
-    int t = (n * G + kPpRows - 1) / kPpRows;
+    int t = (n * G + cta_rows - 1) / cta_rows;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
     total += t;
@@ -79,7 +82,7 @@ __device__ __forceinline__ bool pp_item(const PAttnArgs& a, int G, int item, int
   for (int b0 = 0; b0 < B; b0 += 32) {
     const int b = b0 + lane;
     const int n = b < B ? max(a.q_starts[b + 1] - a.q_starts[b], 0) : 0;
-    const int t = (n * G + kPpRows - 1) / kPpRows;
+    const int t = (n * G + cta_rows - 1) / cta_rows;
     int incl = t;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -103,7 +106,7 @@ struct PpItem {
   int tok0, n_rows, pos0, len, asked;  // row r: token tok0 + r / G at position pos0 + r / G
   Visible v;
 };
-__device__ __forceinline__ PpItem pp_rows(const PAttnArgs& a, int G, int seq, int tile) {
+__device__ __forceinline__ PpItem pp_rows(const PAttnArgs& a, int G, int cta_rows, int seq, int tile) {
   PpItem it;
   const int s0 = a.q_starts[seq], n = a.q_starts[seq + 1] - s0;
   it.asked = a.kv.seq_lens[seq];
@@ -111,7 +114,7 @@ __device__ __forceinline__ PpItem pp_rows(const PAttnArgs& a, int G, int seq, in
   it.tok0 = s0;
   it.pos0 = it.asked - n;
   it.n_rows = n * G;
-  const int r0 = tile * kPpRows, r1 = min(r0 + kPpRows, it.n_rows);
+  const int r0 = tile * cta_rows, r1 = min(r0 + cta_rows, it.n_rows);
   const int plo = it.pos0 + r0 / G, phi = it.pos0 + (r1 - 1) / G;
   Visible& v = it.v;
   v.end = max(0, min(phi + 1, it.len));
@@ -245,19 +248,34 @@ __device__ __forceinline__ unsigned pack2<__nv_bfloat16>(float x, float y) {
   return *reinterpret_cast<const unsigned*>(&h);
 }
 
-template <typename T, bool SPLIT>
+// x, y as the sum of PARTS packed pairs, each the rounded rest of those before.
+template <typename T, int PARTS>
+__device__ __forceinline__ void split_parts(float x, float y, unsigned (&u)[PARTS]) {
+  if constexpr (PARTS == 1) {
+    u[0] = pack2<T>(x, y);
+  } else if constexpr (PARTS == 2) {
+    split2<T>(x, y, u[0], u[1]);
+  } else {
+    const float2 rest = split2_rest<T>(x, y, u[0]);
+    split2<T>(rest.x, rest.y, u[1], u[2]);
+  }
+}
+
+template <typename T, int PARTS>
 __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_constant__ PPromptArgs pa) {
   const PAttnArgs& a = pa.a;
-  constexpr int S = pp_slots<SPLIT>();
-  constexpr int kQTile = (SPLIT ? 2 : 1) * kPpTileBytes;  // hi (and lo) of 128 rows
+  constexpr int S = pp_slots<PARTS>(), kTiles = pp_tiles<PARTS>(), kRows = 128 * kTiles;
+  constexpr int kQTile = PARTS * kPpTileBytes;  // the parts of 128 rows
+  // TMEM columns: S_t | O_t with P over S, or S | P (three parts) | O
+  constexpr unsigned kColP = kTiles == 2 ? 0 : 128, kColO = kTiles == 2 ? 256 : 384;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* qs =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  unsigned char* ring = qs + 2 * kQTile;
+  unsigned char* ring = qs + kTiles * kQTile;
   __shared__ unsigned long long full[S], empty[S], s_full[2], p_full[2], o_done[2], q_full[2], drain;
   __shared__ unsigned bad_rows[8];  // of key tile j: bit i set where 16-key chunk i has no usable page
   __shared__ unsigned tmem_base;
-  __shared__ float shared_row[kPpRows];  // between a row's two threads: a maximum (NaN: given up), then a sum
+  __shared__ float shared_row[256];  // between a row's two threads: a maximum (NaN: given up), then a sum
   __shared__ int failed;
   // (values read back from lane 0 are warp-uniform to the compiler: the MMA warp's operands then live
   // in uniform registers)
@@ -267,21 +285,21 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
   pdl_wait();
   pdl_trigger();
   int seq = 0, tile = 0;
-  if (!pp_item(a, G, item, seq, tile)) return;
-  const PpItem it = pp_rows(a, G, seq, tile);
+  if (!pp_item(a, G, kRows, item, seq, tile)) return;
+  const PpItem it = pp_rows(a, G, kRows, seq, tile);
   if (it.asked > it.len && it.asked > 0 && tid == 0) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
   const int parts = pp_parts(it.v.tiles, pa.splits);
   if (z >= parts) return;
   const int t0 = (int)((long long)it.v.tiles * z / parts);
   const int nk = __shfl_sync(0xffffffffu, (int)((long long)it.v.tiles * (z + 1) / parts) - t0, 0);
-  const int row0 = tile * kPpRows;
-  const int halves = __shfl_sync(0xffffffffu, it.n_rows - row0 > 128 ? 2 : 1, 0);
+  const int row0 = tile * kRows;
+  const int halves = __shfl_sync(0xffffffffu, kTiles == 2 && it.n_rows - row0 > 128 ? 2 : 1, 0);
 
   // this thread's row and half of a row's keys and dims (softmax threads)
   const int t = (tid >> 8) & 1, hf = (tid >> 7) & 1, lr = t * 128 + (tid & 127);
   const int row = row0 + lr;
   const int tok = row / G, hs = row - tok * G;
-  const bool live = tid < kPpSoftmax && row < it.n_rows && (unsigned)(it.tok0 + tok) < (unsigned)a.rows;
+  const bool live = tid < kPpSoftmax && lr < kRows && row < it.n_rows && (unsigned)(it.tok0 + tok) < (unsigned)a.rows;
 
   if (warp == kPpSoftmax / 32) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(&tmem_base)),
@@ -407,7 +425,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
     auto scores = [&](int t, int slot) {  // S_t = Q_t K^T
       const unsigned long long q0 = dq + (unsigned)(t * (kQTile >> 4)), k0 = dk + (unsigned)(slot * (kPpTileBytes >> 4));
 #pragma unroll
-      for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+      for (int part = 0; part < PARTS; ++part)
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
           const unsigned off = ((ks >> 2) * (kPpTileBytes / 2) + (ks & 3) * 32) >> 4;
@@ -434,9 +452,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         if (!ok) break;
         tc_fence_after();
         const unsigned long long v0 = dv + (unsigned)(vs * (kPpTileBytes >> 4));
-        const unsigned od = tmem + 256 + t * 128, pd = tmem + t * 128;
+        const unsigned od = tmem + kColO + t * 128, pd = tmem + kColP + t * 128;
 #pragma unroll
-        for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+        for (int part = 0; part < PARTS; ++part)
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks) {
             if (part == 0 && ks == 0) pp_mma_ts(od, pd, v0, id_o, j > 0, leader);
@@ -470,7 +488,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         unsigned char* dst = qs + t * kQTile + hf * (kPpTileBytes / 2) + r * 128;
         const long long base =
             (long long)(it.tok0 + (live ? tok : 0)) * a.q_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf;
-        if constexpr (SPLIT) {
+        if constexpr (PARTS > 1) {
 #pragma unroll 4
           for (int c = 0; c < 8; ++c) {
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
@@ -482,14 +500,16 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                 y = make_float4(-y.x, -y.y, -y.z, -y.w);
               }
             }
-            uint4 hi, lo;
-            split2<T>(x.x, x.y, hi.x, lo.x);
-            split2<T>(x.z, x.w, hi.y, lo.y);
-            split2<T>(y.x, y.y, hi.z, lo.z);
-            split2<T>(y.z, y.w, hi.w, lo.w);
+            unsigned u[4][PARTS];
+            split_parts<T, PARTS>(x.x, x.y, u[0]);
+            split_parts<T, PARTS>(x.z, x.w, u[1]);
+            split_parts<T, PARTS>(y.x, y.y, u[2]);
+            split_parts<T, PARTS>(y.z, y.w, u[3]);
             const unsigned off = ((c ^ r) & 7) << 4;
-            *reinterpret_cast<uint4*>(dst + off) = hi;
-            *reinterpret_cast<uint4*>(dst + kPpTileBytes + off) = lo;
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part)
+              *reinterpret_cast<uint4*>(dst + part * kPpTileBytes + off) =
+                  make_uint4(u[0][part], u[1][part], u[2][part], u[3][part]);
           }
         } else {
           const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + base);
@@ -506,7 +526,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       pp_arrive(&q_full[t]);
       float m = -INFINITY, l = 0.0f;
       const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
-      const unsigned ts = tmem + t * 128 + lanes, to = tmem + 256 + t * 128 + 64 * hf + lanes;
+      const unsigned ts = tmem + t * 128 + lanes, tp = tmem + kColP + t * 128 + 32 * hf + lanes;
+      const unsigned to = tmem + kColO + t * 128 + 64 * hf + lanes;
       const int pair = 1 + t * 4 + (warp & 3);  // named barrier of the two warps that share 32 rows
       const float c = fabsf(a.scale) * kLog2e;
       const int p = live ? it.pos0 + tok : -1;
@@ -587,18 +608,20 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {  // 32 keys: 16 packed columns
-          unsigned w[16], wl[SPLIT ? 16 : 1];
+          unsigned w[PARTS][16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float s0 = __uint_as_float(sr[32 * h + 2 * i]), s1 = __uint_as_float(sr[32 * h + 2 * i + 1]);
             float2 e = __ffma2_rn(make_float2(s0, s1), make_float2(c, c), make_float2(ref, ref));
             e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
             sum = __fadd2_rn(sum, e);
-            if constexpr (SPLIT) split2<T>(e.x, e.y, w[i], wl[i]);
-            else w[i] = pack2<T>(e.x, e.y);
+            unsigned u[PARTS];
+            split_parts<T, PARTS>(e.x, e.y, u);
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) w[part][i] = u[part];
           }
-          tmem_st16(ts + 32 * hf + 16 * h, w);
-          if constexpr (SPLIT) tmem_st16(ts + 64 + 32 * hf + 16 * h, wl);
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part) tmem_st16(tp + 64 * part + 16 * h, w[part]);
         }
         l += sum.x + sum.y;
         tmem_wait_st();
@@ -616,7 +639,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         tc_fence_after();
         const bool whole = parts == 1;
         const float f = whole ? inv_sum(l) : 1.0f;
-        const long long prow = (((long long)item * kvh + g) * pa.splits + z) * kPpRows + lr;
+        const long long prow = (((long long)item * kvh + g) * pa.splits + z) * kRows + lr;
         const long long base = (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf;
         if (!whole && hf == 0) pa.pml[prow] = make_float2(m, l);
 #pragma unroll 1
@@ -629,7 +652,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
               *reinterpret_cast<float4*>(pa.po + prow * kHeadDim + 64 * hf + 32 * h + i) =
                   make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           } else if (live) {
-            if constexpr (SPLIT) {
+            if constexpr (PARTS > 1) {
 #pragma unroll
               for (int i = 0; i < 32; i += 4)
                 *reinterpret_cast<float4*>(static_cast<float*>(a.y) + base + 32 * h + i) =
@@ -656,20 +679,21 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
   if (warp == kPpSoftmax / 32) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
-// Adds the parts of rows whose key tiles were split. One warp per row; grid: items * kv_heads * 32.
+// Adds the parts of rows whose key tiles were split. One warp per row; grid: items * kv_heads * cta_rows / 8.
 __global__ void __launch_bounds__(256) k_paged_prompt_join(const __grid_constant__ PPromptArgs pa) {
   const PAttnArgs& a = pa.a;
   const int kvh = a.kv.kv_heads, G = a.q_heads / kvh, lane = threadIdx.x & 31;
-  const int r = (blockIdx.x & 31) * 8 + (threadIdx.x >> 5), ig = blockIdx.x >> 5, g = ig % kvh, item = ig / kvh;
+  const int R = pa.cta_rows, per = R >> 3;
+  const int r = (blockIdx.x % per) * 8 + (threadIdx.x >> 5), ig = blockIdx.x / per, g = ig % kvh, item = ig / kvh;
   pdl_wait();
   pdl_trigger();
   int seq = 0, tile = 0;
-  if (!pp_item(a, G, item, seq, tile)) return;
-  const PpItem it = pp_rows(a, G, seq, tile);
-  const int parts = pp_parts(it.v.tiles, pa.splits), row = tile * kPpRows + r, tok = row / G;
+  if (!pp_item(a, G, R, item, seq, tile)) return;
+  const PpItem it = pp_rows(a, G, R, seq, tile);
+  const int parts = pp_parts(it.v.tiles, pa.splits), row = tile * R + r, tok = row / G;
   if (parts == 1 || row >= it.n_rows || (unsigned)(it.tok0 + tok) >= (unsigned)a.rows) return;
-  const long long p0 = ((long long)item * kvh + g) * pa.splits * kPpRows + r;
-  const float2 ml = lane < parts ? pa.pml[p0 + (long long)lane * kPpRows] : make_float2(-INFINITY, 0.0f);
+  const long long p0 = ((long long)item * kvh + g) * pa.splits * R + r;
+  const float2 ml = lane < parts ? pa.pml[p0 + (long long)lane * R] : make_float2(-INFINITY, 0.0f);
   const float M = warp_max(ml.x);
   const float f = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - M);
   const float L = warp_sum(ml.y * f);
@@ -677,7 +701,7 @@ __global__ void __launch_bounds__(256) k_paged_prompt_join(const __grid_constant
 #pragma unroll 8
   for (int k = 0; k < parts; ++k) {
     const float fk = __shfl_sync(0xffffffffu, f, k);
-    const float4 x = *reinterpret_cast<const float4*>(pa.po + (p0 + (long long)k * kPpRows) * kHeadDim + 4 * lane);
+    const float4 x = *reinterpret_cast<const float4*>(pa.po + (p0 + (long long)k * R) * kHeadDim + 4 * lane);
     y = make_float4(y.x + x.x * fk, y.y + x.y * fk, y.z + x.z * fk, y.w + x.w * fk);
   }
   const float zf = inv_sum(L);
