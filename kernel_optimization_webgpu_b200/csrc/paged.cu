@@ -75,6 +75,16 @@ static PAttnArgs check_attn(const qd_paged_kv* kv, const void* q, int dtype, int
   return a;
 }
 
+template <int HEADS>
+static void launch_append(const AppendArgs& a, int qkv_dtype, long long heads, cudaStream_t s) {
+  const long long warps = a.rows * ((heads + HEADS - 1) / HEADS);
+  need(warps <= 0x7fffffffLL, "qd_paged_append: too many rows");
+  const dim3 grid((unsigned)((warps + 7) / 8)), block(256);
+  if (qkv_dtype == QD_KV_F32) launch_ex(k_paged_append<float, HEADS>, grid, block, 0, s, a);
+  else if (qkv_dtype == QD_KV_F16) launch_ex(k_paged_append<__half, HEADS>, grid, block, 0, s, a);
+  else launch_ex(k_paged_append<__nv_bfloat16, HEADS>, grid, block, 0, s, a);
+}
+
 template <typename T, bool THREE>
 static void launch_decode(const PAttnArgs& a, void* workspace, cudaStream_t s) {
   static unsigned long long smem_set = 0;
@@ -197,13 +207,10 @@ int qd_paged_append(const qd_paged_kv* kv, const void* qkv, int qkv_dtype, int64
     a.q_out = q_out;
     a.q_out_dtype = q_out_dtype;
     a.q_out_stride = q_out_stride;
-    const long long warps = (long long)rows * ((heads + kAppendHeads - 1) / kAppendHeads);
-    need((warps + 7) / 8 <= 0x7fffffffLL, "qd_paged_append: too many rows");
-    const dim3 grid((unsigned)((warps + 7) / 8)), block(256);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (qkv_dtype == QD_KV_F32) launch_ex(k_paged_append<float>, grid, block, 0, s, a);
-    else if (qkv_dtype == QD_KV_F16) launch_ex(k_paged_append<__half>, grid, block, 0, s, a);
-    else launch_ex(k_paged_append<__nv_bfloat16>, grid, block, 0, s, a);
+    // four heads a warp once that gives every SM four CTAs, else two
+    if (rows * ((heads + 3) / 4) >= 32LL * current_sms()) launch_append<4>(a, qkv_dtype, heads, s);
+    else launch_append<2>(a, qkv_dtype, heads, s);
   });
 }
 

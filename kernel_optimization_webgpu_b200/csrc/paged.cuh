@@ -111,26 +111,26 @@ struct AppendArgs {
   long long q_out_stride;
 };
 
-// One warp per row and kAppendHeads consecutive heads of its [q | k | v]; lane l holds dims
-// 4l .. 4l+3, so the rotation's partner dims are 16 lanes away. The heads' loads are issued
-// first; the row's sequence and position are looked up under them.
-constexpr int kAppendHeads = 4;
-
-template <typename T>
-__global__ void __launch_bounds__(256) k_paged_append(const __grid_constant__ AppendArgs a) {
+// One warp per row and HEADS consecutive heads of its [q | k | v]; lane l holds dims 4l .. 4l+3, so
+// the rotation's partner dims are 16 lanes away. What it has to move bounds it (per row and head 512
+// bytes of f32 in, 512 or 256 out), so the heads' loads go out first, and the row's sequence,
+// position and page are looked up under them; the heads' sums of squares then run side by side.
+// HEADS: 4 keep 2 KB in flight per warp at 40 warps an SM (16384 rows of 16 + 8 + 8 heads, f32, 470 MB:
+// 82 us = 5.7 TB/s, 88 with 8); with few rows 2 spread the work over more warps (1 row: 2.5 us, 3.2
+// with 4).
+template <typename T, int HEADS>
+__global__ void __launch_bounds__(256, HEADS == 4 ? 5 : 6) k_paged_append(const __grid_constant__ AppendArgs a) {
   const int lane = threadIdx.x & 31;
   const int heads = a.q_heads + 2 * a.kv.kv_heads;
-  const int per_row = (heads + kAppendHeads - 1) / kAppendHeads;
-  const long long w = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int r = (int)(w / per_row), h0 = (int)(w % per_row) * kAppendHeads;
+  const unsigned per_row = (unsigned)(heads + HEADS - 1) / HEADS;
+  const unsigned w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int r = (int)(w / per_row), h0 = (int)(w % per_row) * HEADS;
   if (r >= a.rows) return;
   pdl_wait();
-  float4 x[kAppendHeads];
+  float4 x[HEADS];
 #pragma unroll
-  for (int i = 0; i < kAppendHeads; ++i) {
-    const int h = min(h0 + i, heads - 1);
-    x[i] = load4<T>(a.qkv, r * a.qkv_stride + (long long)h * kHeadDim + 4 * lane);
-  }
+  for (int i = 0; i < HEADS; ++i)
+    x[i] = load4<T>(a.qkv, r * a.qkv_stride + (long long)min(h0 + i, heads - 1) * kHeadDim + 4 * lane);
   int b = r, back = 1;
   if (a.q_starts) {
     b = paged_find_seq(a.q_starts, a.kv.batch, r);
@@ -153,22 +153,28 @@ __global__ void __launch_bounds__(256) k_paged_append(const __grid_constant__ Ap
     if (lane < 16) s = make_float4(-s.x, -s.y, -s.z, -s.w);
   }
   int page = -1;
-  if (h0 + kAppendHeads > a.q_heads) {
+  if (h0 + HEADS > a.q_heads) {
     page = paged_page(a.kv, b, p);
     if (page < 0 && lane == 0) paged_flag(a.kv, QD_PAGED_BAD_PAGE);
   }
-  const int ps = 1 << a.kv.page_shift;
+  const int k0 = a.q_heads, v0 = a.q_heads + a.kv.kv_heads;
+  float ss[HEADS];
 #pragma unroll
-  for (int i = 0; i < kAppendHeads; ++i) {
+  for (int i = 0; i < HEADS; ++i) ss[i] = x[i].x * x[i].x + x[i].y * x[i].y + x[i].z * x[i].z + x[i].w * x[i].w;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) ss[i] += __shfl_xor_sync(0xffffffffu, ss[i], o);
+  const int in_page = p & ((1 << a.kv.page_shift) - 1);
+#pragma unroll
+  for (int i = 0; i < HEADS; ++i) {
     const int h = h0 + i;
     if (h >= heads) break;
     float4 y = x[i];
-    const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + a.kv.kv_heads;
-    if (!is_v) {
-      const float* wn = is_q ? a.q_norm : a.k_norm;
+    if (h < v0) {
+      const float* wn = h < k0 ? a.q_norm : a.k_norm;
       if (wn) {
-        const float ss = warp_sum(y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w);
-        const float f = rsqrtf(ss * (1.0f / kHeadDim) + a.eps);
+        const float f = rsqrtf(ss[i] * (1.0f / kHeadDim) + a.eps);
         const float4 n = *reinterpret_cast<const float4*>(wn + 4 * lane);
         y = make_float4(y.x * f * n.x, y.y * f * n.y, y.z * f * n.z, y.w * f * n.w);
       }
@@ -178,12 +184,12 @@ __global__ void __launch_bounds__(256) k_paged_append(const __grid_constant__ Ap
         y = make_float4(y.x * c.x + o.x * s.x, y.y * c.y + o.y * s.y, y.z * c.z + o.z * s.z, y.w * c.w + o.w * s.w);
       }
     }
-    if (is_q) {
+    if (h < k0) {
       store4(a.q_out, r * a.q_out_stride + (long long)h * kHeadDim + 4 * lane, a.q_out_dtype, y);
     } else if (page >= 0) {
-      const int g = h - a.q_heads - (is_v ? a.kv.kv_heads : 0);
-      const long long row = (((long long)page * a.kv.kv_heads + g) << a.kv.page_shift) + (p & (ps - 1));
-      store4(is_v ? a.kv.v : a.kv.k, row * kHeadDim + 4 * lane, a.kv_dtype, y);
+      const int g = h < v0 ? h - k0 : h - v0;
+      const long long row = (((long long)page * a.kv.kv_heads + g) << a.kv.page_shift) + in_page;
+      store4(h < v0 ? a.kv.k : a.kv.v, row * kHeadDim + 4 * lane, a.kv_dtype, y);
     }
   }
 }

@@ -307,8 +307,8 @@ struct RowsCta {
             const uint32_t u = place(v[k]);
             const double w = u < kNoPlace ? raw_weight(v[k]) : 0.0;
             sum[0] += w;
-            sum[1] += u < lo ? w : 0.0;
-            if (span2) sum[2] += u < lo2 ? w : 0.0;
+            if (u < lo) sum[1] += w;
+            if (u < lo2) sum[2] += w;
             any = any || u - lo < span || u - lo2 < span2;
           }
           if (any) {
