@@ -1,14 +1,18 @@
 """Build recipe for the in-tree CUDA library (libqdecode.so, sm_100a).
 
 The library is compiled with nvcc directly (no torch extension machinery): it is
-a plain C-ABI shared object that JavaScript, C or Python can load.
+a plain C-ABI shared object that JavaScript, C or Python can load. Beside it, where
+torch is installed, _torch_calls.so: the Python module through which runtime.py's paged
+operators and batched sampler take torch tensors (csrc/torch_calls.cpp).
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -16,6 +20,8 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libqdecode.so")
 SOURCES = ["engine.cu", "batch.cu", "noalloc.cu", "bench_api.cu", "sample.cu", "paged.cu", "sample_rows.cu"]
 DEPS = SOURCES + ["kernels.cuh", "persist.cuh", "gemm_tc.cuh", "batch.cuh", "paged.cuh", "paged_decode.cuh", "paged_prompt.cuh", "internal.cuh", "tma.cuh", "common.cuh", "json.hpp"]
+CALLS = os.path.join(PKG, "_torch_calls.so")
+CALLS_SOURCE = "torch_calls.cpp"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -36,6 +42,7 @@ def _stale() -> bool:
 
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not _stale():
+        build_calls()
         return LIB
     obj_dir = os.path.join(PKG, "_build")
     os.makedirs(obj_dir, exist_ok=True)
@@ -65,7 +72,30 @@ def build(force: bool = False, verbose: bool = False) -> str:
         sys.stderr.write(res.stdout + res.stderr)
         raise RuntimeError("nvcc failed linking libqdecode.so")
     os.replace(LIB + ".tmp", LIB)
+    build_calls(force)
     return LIB
+
+
+def build_calls(force: bool = False) -> str:
+    """_torch_calls.so against the installed torch (nothing where there is none)."""
+    torch = importlib.util.find_spec("torch")  # found, not imported
+    if torch is None:
+        return ""
+    src, header = os.path.join(CSRC, CALLS_SOURCE), os.path.join(ROOT, "include", "qdecode.h")
+    if not force and os.path.exists(CALLS) and all(os.path.getmtime(p) <= os.path.getmtime(CALLS) for p in (src, header)):
+        return CALLS
+    home = torch.submodule_search_locations[0]
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", src, "-o", CALLS + ".tmp",
+           "-I", os.path.join(home, "include"), "-I", os.path.join(home, "include", "torch", "csrc", "api", "include"),
+           "-I", sysconfig.get_paths()["include"], "-I", os.path.join(cuda, "include"), "-L", os.path.join(home, "lib"),
+           "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda", "-L", PKG, "-lqdecode", "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError("g++ failed building _torch_calls.so")
+    os.replace(CALLS + ".tmp", CALLS)
+    return CALLS
 
 
 if __name__ == "__main__":

@@ -590,94 +590,28 @@ def gqa_decode(q, k_cache, v_cache, seq_len: int, q_heads: int, kv_heads: int, y
 
 
 # ---- paged key-value cache and batched sampling (torch CUDA tensors) --------------------
-# These calls are made per layer or per token, so their host side is kept short: one test of
-# everything that may be wrong, with the message looked for only when it fails.
+# Checks, outputs and launches are in csrc/torch_calls.cpp (ValueError for tensors that do not fit
+# together, QdError for what the C ABI refuses). A tensor's own device is made current for the call.
 
-class _Torch:
-    """torch's names used below, looked up once (torch is imported on first use)."""
-    ready = False
-
-    @classmethod
-    def load(cls):
-        import torch
-        cls.torch, cls.empty, cls.empty_like = torch, torch.empty, torch.empty_like
-        cls.i32, cls.f32, cls.u8 = torch.int32, torch.float32, torch.uint8
-        cls.code = {torch.float16: QD_KV_F16, torch.float32: QD_KV_F32, torch.bfloat16: _lib.QD_KV_BF16}
-        if torch.cuda.is_available():
-            torch.cuda.init()
-            cls.device, cls.stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
-        cls.lib = _lib.load()
-        cls.ready = True
+_calls_module = None
 
 
-def _elsewhere(dev: int, stream):
-    """None where the call can go on as it is; else a context that makes the tensors' device and
-    the stream current (what the call allocates then belongs to the stream that uses it)."""
-    t = _Torch
-    if dev < 0:
-        raise ValueError("tensors must be on a CUDA device")
-    if stream is not None:
-        if stream.device.index != dev:
-            raise ValueError(f"the stream belongs to {stream.device}, the tensors to cuda:{dev}")
-        return t.torch.cuda.stream(stream)
-    return None if t.device() == dev else t.torch.cuda.device(dev)
+def _calls():
+    global _calls_module
+    if _calls_module is None:
+        import torch  # noqa: F401  (the module uses torch's libraries)
+        _lib.load()
+        from . import _torch_calls
+        _calls_module = _torch_calls
+    return _calls_module
 
 
-def _vector(x, n: int, dtype, dev: int, what: str):
-    """Pointer of a contiguous vector of n entries (None: NULL)."""
-    if x is None:
-        return None
-    if x.dtype is not dtype or x.shape != (n,) or not x.is_contiguous() or x.get_device() != dev:
-        raise ValueError(f"{what} must be a contiguous {dtype} vector of {n} entries on cuda:{dev}")
-    return x.data_ptr()
-
-
-def _row_stride(x, width: int, what: str) -> int:
-    """Row stride (elements) of a [rows, ...] tensor whose rows are `width` contiguous elements."""
-    if x.is_contiguous() and x.dim() and x.shape[0] * width == x.numel():
-        return width
-    inner = 1
-    for i in range(x.dim() - 1, 0, -1):
-        if x.shape[i] != 1 and x.stride(i) != inner:
-            raise ValueError(f"the rows of {what} must be contiguous")
-        inner *= x.shape[i]
-    if x.dim() < 1 or inner != width:
-        raise ValueError(f"{what} must have rows of {width} elements")
-    return x.stride(0) if x.shape[0] > 1 else width
-
-
-def _code(x, what: str) -> int:
-    code = _Torch.code.get(x.dtype)
-    if code is None:
-        raise ValueError(f"{what} must be float16, bfloat16 or float32, not {x.dtype}")
-    return code
-
-
-def _paged_kv(k, v, table, seq_lens, status, dev: int) -> "_lib.QdPagedKv":
-    t, shape = _Torch, k.shape
-    if len(shape) != 4 or v.shape != shape or v.dtype is not k.dtype or not k.is_contiguous() or not v.is_contiguous() \
-            or k.get_device() != dev or v.get_device() != dev:
-        raise ValueError("k_pages and v_pages must be contiguous [pages][kv_heads][page_size][128] of one type, "
-                         "on the device of the other tensors")
-    if table.dtype is not t.i32 or table.dim() != 2 or table.get_device() != dev:
-        raise ValueError(f"block_table must be int32 [batch][pages] on cuda:{dev}")
-    batch, width = table.shape
-    stride = width
-    if not table.is_contiguous():
-        if width > 1 and table.stride(1) != 1:
-            raise ValueError("the rows of block_table must be contiguous")
-        stride = table.stride(0) if batch > 1 else width
-    return _lib.QdPagedKv(k.data_ptr(), v.data_ptr(), _code(k, "the cache"), shape[0], shape[2], shape[1], shape[3],
-                          batch, table.data_ptr(), width, stride, _vector(seq_lens, batch, t.i32, dev, "seq_lens"),
-                          None if status is None else _vector(status, 1, t.i32, dev, "status"))
-
-
-def _workspace(given, n: int, dev: int):
-    if given is None:
-        return _Torch.empty(n, dtype=_Torch.u8, device=dev)
-    if given.get_device() != dev or given.numel() * given.element_size() < n or not given.is_contiguous():
-        raise ValueError(f"workspace must be a contiguous tensor of at least {n} bytes on cuda:{dev}")
-    return given
+def _on(stream, x):
+    """Makes the given stream current: what a call allocates then belongs to it."""
+    import torch
+    if stream.device != x.device:
+        raise ValueError(f"the stream belongs to {stream.device}, the tensors to {x.device}")
+    return torch.cuda.stream(stream)
 
 
 def paged_append(qkv, k_pages, v_pages, block_table, seq_lens, cos, sin, q_heads: int, q_norm=None, k_norm=None,
@@ -688,61 +622,12 @@ def paged_append(qkv, k_pages, v_pages, block_table, seq_lens, cos, sin, q_heads
     [pages][kv_heads][page_size][128]; cos, sin f32 tables whose row for a position is
     rope_stride elements after the previous one's (default: their own row stride; None, None:
     no rotation); returns q [rows][q_heads * 128] (q_out, or a new tensor of qkv's type)."""
-    t = _Torch
-    if not t.ready:
-        t.load()
-    dev = qkv.get_device()
-    kv = _paged_kv(k_pages, v_pages, block_table, seq_lens, status, dev)
-    stride, rows = _row_stride(qkv, (q_heads + 2 * kv.kv_heads) * 128, "qkv"), qkv.shape[0]
-    rope_len = 0
-    for x in (cos, sin):
-        if x is not None and (x.dtype is not t.f32 or x.get_device() != dev or not x.is_contiguous()):
-            raise ValueError(f"cos and sin must be contiguous float32 tables on cuda:{dev}")
-    if cos is not None and sin is not None:
-        rope_len = min(cos.numel(), sin.numel())
-        if rope_stride is None:
-            rope_stride = cos.stride(0) if cos.dim() > 1 else 64
-    there = _elsewhere(dev, stream)
-    if there is not None:
-        with there:
+    if stream is not None:
+        with _on(stream, qkv):
             return paged_append(qkv, k_pages, v_pages, block_table, seq_lens, cos, sin, q_heads, q_norm, k_norm, eps,
                                 q_starts, q_out, rope_stride, status)
-    if q_out is None:
-        q_out = t.empty((rows, q_heads * 128), dtype=qkv.dtype, device=dev)
-        out_stride = q_heads * 128
-    elif q_out.get_device() != dev or q_out.shape[0] != rows:
-        raise ValueError(f"q_out must have {rows} rows on cuda:{dev}")
-    else:
-        out_stride = _row_stride(q_out, q_heads * 128, "q_out")
-    rc = t.lib.qd_paged_append(
-        kv, qkv.data_ptr(), _code(qkv, "qkv"), stride, rows,
-        None if q_starts is None else _vector(q_starts, kv.batch + 1, t.i32, dev, "q_starts"), q_heads,
-        _vector(q_norm, 128, t.f32, dev, "q_norm"), _vector(k_norm, 128, t.f32, dev, "k_norm"), eps,
-        None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(), rope_len, rope_stride or 0,
-        q_out.data_ptr(), _code(q_out, "q_out"), out_stride, t.stream(dev))
-    if rc:
-        check(rc)
-    return q_out
-
-
-def _attn(q, k_pages, v_pages, block_table, seq_lens, status):
-    """(cache, query heads, q's row stride, elements a row) of an attention call."""
-    kv = _paged_kv(k_pages, v_pages, block_table, seq_lens, status, q.get_device())
-    shape = q.shape
-    width = shape[1] * shape[2] if len(shape) == 3 else shape[1] if len(shape) == 2 else 1
-    if width % 128:
-        raise ValueError("q must be [rows][q_heads][128] or [rows][q_heads * 128]")
-    return kv, width // 128, _row_stride(q, width, "q"), width
-
-
-def _attn_out(q, y, width: int):
-    if y is None:
-        if q.is_contiguous():
-            return _Torch.empty_like(q), width
-        return _Torch.empty(q.shape, dtype=q.dtype, device=q.device), width
-    if y.dtype is not q.dtype or y.shape != q.shape or y.get_device() != q.get_device():
-        raise ValueError("y must have q's type, shape and device")
-    return y, _row_stride(y, width, "y")
+    return (_calls_module or _calls()).paged_append(qkv, k_pages, v_pages, block_table, seq_lens, cos, sin, q_heads,
+                                                    q_norm, k_norm, eps, q_starts, q_out, rope_stride, status)
 
 
 def paged_attn_decode(q, k_pages, v_pages, block_table, seq_lens, window: int = 0, sinks: int = 0, scale: float = 0.0,
@@ -751,24 +636,11 @@ def paged_attn_decode(q, k_pages, v_pages, block_table, seq_lens, window: int = 
     [batch][q_heads][128], the token at position seq_lens[b] - 1; window > 0: the last
     `window` positions and the first `sinks`. workspace: a tensor of at least
     qd_paged_attn_decode_workspace_bytes that no other stream uses meanwhile (default: a new one)."""
-    t = _Torch
-    if not t.ready:
-        t.load()
-    kv, heads, stride, width = _attn(q, k_pages, v_pages, block_table, seq_lens, status)
-    if q.shape[0] != kv.batch:
-        raise ValueError(f"q must have one row per sequence ({kv.batch})")
-    dev = q.get_device()
-    there = _elsewhere(dev, stream)
-    if there is not None:
-        with there:
+    if stream is not None:
+        with _on(stream, q):
             return paged_attn_decode(q, k_pages, v_pages, block_table, seq_lens, window, sinks, scale, y, workspace, status)
-    y, y_stride = _attn_out(q, y, width)
-    ws = _workspace(workspace, t.lib.qd_paged_attn_decode_workspace_bytes(kv.batch, heads), dev)
-    rc = t.lib.qd_paged_attn_decode(kv, q.data_ptr(), _code(q, "q"), stride, heads, window, sinks, scale, y.data_ptr(),
-                                    y_stride, ws.data_ptr(), t.stream(dev))
-    if rc:
-        check(rc)
-    return y
+    return (_calls_module or _calls()).paged_attn_decode(q, k_pages, v_pages, block_table, seq_lens, window, sinks, scale,
+                                                         y, workspace, status)
 
 
 def paged_attn_prompt(q, k_pages, v_pages, block_table, seq_lens, q_starts, window: int = 0, sinks: int = 0,
@@ -777,56 +649,22 @@ def paged_attn_prompt(q, k_pages, v_pages, block_table, seq_lens, q_starts, wind
     q [rows][q_heads][128], rows q_starts[b] .. q_starts[b + 1] - 1 being sequence b's newest
     tokens (already appended). Rows from q_starts[batch] on are padding; y keeps what it held
     there."""
-    t = _Torch
-    if not t.ready:
-        t.load()
-    kv, heads, stride, width = _attn(q, k_pages, v_pages, block_table, seq_lens, status)
-    dev = q.get_device()
-    there = _elsewhere(dev, stream)
-    if there is not None:
-        with there:
+    if stream is not None:
+        with _on(stream, q):
             return paged_attn_prompt(q, k_pages, v_pages, block_table, seq_lens, q_starts, window, sinks, scale, y,
                                      workspace, status)
-    y, y_stride = _attn_out(q, y, width)
-    rows = q.shape[0]
-    ws = _workspace(workspace, t.lib.qd_paged_attn_prompt_workspace_bytes(kv.batch, rows, heads, kv.kv_heads), dev)
-    rc = t.lib.qd_paged_attn_prompt(kv, q.data_ptr(), _code(q, "q"), stride, rows,
-                                    _vector(q_starts, kv.batch + 1, t.i32, dev, "q_starts"), heads, window, sinks, scale,
-                                    y.data_ptr(), y_stride, ws.data_ptr(), t.stream(dev))
-    if rc:
-        check(rc)
-    return y
+    return (_calls_module or _calls()).paged_attn_prompt(q, k_pages, v_pages, block_table, seq_lens, q_starts, window,
+                                                         sinks, scale, y, workspace, status)
 
 
 def sample_rows(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, ids=None, logprobs=None, stream=None):
     """One token per row of logits [rows][vocab] (f32, f16 or bf16) from the given random
     numbers u [rows] f32 in [0, 1), with per-row settings (f32 vectors; top_k int32; None: not
     applied) as qd_sample_rows defines them. Returns (ids int32, logprobs f32)."""
-    t = _Torch
-    if not t.ready:
-        t.load()
-    if logits.dim() != 2:
-        raise ValueError("logits must be [rows][vocab]")
-    rows, vocab = logits.shape
-    dev = logits.get_device()
-    stride = _row_stride(logits, vocab, "logits")
-    there = _elsewhere(dev, stream)
-    if there is not None:
-        with there:
+    if stream is not None:
+        with _on(stream, logits):
             return sample_rows(logits, u, temperature, top_k, top_p, min_p, ids, logprobs)
-    if ids is None:
-        ids = t.empty(rows, dtype=t.i32, device=dev)
-    if logprobs is None:
-        logprobs = t.empty(rows, dtype=t.f32, device=dev)
-    rc = t.lib.qd_sample_rows(logits.data_ptr(), _code(logits, "logits"), rows, vocab, stride,
-                              _vector(temperature, rows, t.f32, dev, "temperature"),
-                              _vector(top_k, rows, t.i32, dev, "top_k"), _vector(top_p, rows, t.f32, dev, "top_p"),
-                              _vector(min_p, rows, t.f32, dev, "min_p"), _vector(u, rows, t.f32, dev, "u"),
-                              _vector(ids, rows, t.i32, dev, "ids"), _vector(logprobs, rows, t.f32, dev, "logprobs"),
-                              t.stream(dev))
-    if rc:
-        check(rc)
-    return ids, logprobs
+    return (_calls_module or _calls()).sample_rows(logits, u, temperature, top_k, top_p, min_p, ids, logprobs)
 
 
 __all__ = ["Engine", "QdError", "createWebGpuContext", "runCustomQwenGreedyPrompt", "runKernelBenchmarks",
