@@ -442,7 +442,7 @@ int qd_paged_attn_decode(const qd_paged_kv* kv, const void* q, int dtype, int64_
 /* The same for a ragged batch of new tokens (q_starts as above, not NULL): each row attends
  * to the keys its own position sees, the call's own new tokens among them (append them
  * first). q, y [rows][q_heads][128]. */
-size_t qd_paged_attn_prompt_workspace_bytes(int batch, int rows, int q_heads, int kv_heads);
+size_t qd_paged_attn_prompt_workspace_bytes(int batch, int rows, int q_heads, int kv_heads, int dtype);
 int qd_paged_attn_prompt(const qd_paged_kv* kv, const void* q, int dtype, int64_t q_stride, int rows,
                          const int32_t* q_starts, int q_heads, int window, int sinks, float scale, void* y,
                          int64_t y_stride, void* workspace, void* stream);

@@ -218,7 +218,7 @@ def load(build_if_stale: bool = True):
     L.qd_paged_attn_decode_workspace_bytes.restype = C.c_size_t
     L.qd_paged_attn_decode.argtypes = [kv, vp, i32, i64, i32, i32, i32, f32, vp, i64, vp, vp]
     L.qd_paged_attn_decode.restype = i32
-    L.qd_paged_attn_prompt_workspace_bytes.argtypes = [i32, i32, i32, i32]
+    L.qd_paged_attn_prompt_workspace_bytes.argtypes = [i32, i32, i32, i32, i32]
     L.qd_paged_attn_prompt_workspace_bytes.restype = C.c_size_t
     L.qd_paged_attn_prompt.argtypes = [kv, vp, i32, i64, i32, vp, i32, i32, i32, f32, vp, i64, vp, vp]
     L.qd_paged_attn_prompt.restype = i32

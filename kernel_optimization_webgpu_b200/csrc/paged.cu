@@ -118,8 +118,8 @@ static void launch_prompt(const PAttnArgs& a, const void* q_any, void* workspace
   p.a = a;
   p.cta_rows = kRows;
   p.splits = prompt_splits(items, a.kv.kv_heads);
-  p.po = static_cast<float*>(workspace);
-  p.pml = reinterpret_cast<float2*>(p.po + (size_t)items * a.kv.kv_heads * p.splits * kRows * kHeadDim);
+  p.po = static_cast<float4*>(workspace);
+  p.pml = reinterpret_cast<float2*>(p.po + (size_t)items * a.kv.kv_heads * p.splits * kRows * (kHeadDim / 4));
   // a table that holds few tiles never splits them into more parts than this
   const long long tiles = (((long long)a.kv.table_width << a.kv.page_shift) + kPpKeys - 1) / kPpKeys;
   p.splits = (int)std::max(1LL, std::min<long long>(p.splits, tiles / 2));
@@ -233,12 +233,13 @@ int qd_paged_attn_decode(const qd_paged_kv* kv, const void* q, int dtype, int64_
   });
 }
 
-size_t qd_paged_attn_prompt_workspace_bytes(int batch, int rows, int q_heads, int kv_heads) {
+size_t qd_paged_attn_prompt_workspace_bytes(int batch, int rows, int q_heads, int kv_heads, int dtype) {
   if (batch < 0 || rows < 0 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads) return 0;
   size_t most = 256;
   for (const int cta_rows : {128, 256}) {  // (a CTA's rows depend on the types)
     const int items = prompt_items(batch, rows, q_heads / kv_heads, cta_rows), splits = prompt_splits(items, kv_heads);
-    if (splits > 1) most = std::max(most, (size_t)items * kv_heads * splits * cta_rows * (kHeadDim * 4 + 8));
+    if (splits > 1 || dtype == QD_KV_F32)
+      most = std::max(most, (size_t)items * kv_heads * splits * cta_rows * (kHeadDim * 4 + 8));
   }
   return most;
 }

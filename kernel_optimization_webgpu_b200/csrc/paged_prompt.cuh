@@ -8,7 +8,8 @@
 //   O += P V       -> TMEM (f32), P read from TMEM   M 128, N 128 dims, K 128 keys
 // The two tiles alternate: while one's softmax runs, the tensor cores work for the other. P
 // (One thread per row left a single softmax warp of a tile on each scheduler, and its chain of
-// dependent instructions set the pace: 1 x 8192 301 us against TODO us with two.) P
+// dependent instructions set the pace; with two the MMA warp does. Uniform operands there, see below,
+// then took 8192 causal rows of 16 heads from 301 to 266 us = 1032 TFLOP/s.) P
 // replaces its S in TMEM (S0 S1 O0 O1 = 512 columns); the MMAs of one issuer run in order, so
 // S of the next key tile may be issued right behind the product that reads P.
 //
@@ -18,7 +19,11 @@
 // relative, as the tensor cores take 16-bit operands); its sum is taken in f32 before that.
 // With f32 queries q and P are each a sum of PARTS 16-bit operands, and every product is issued that
 // many times: two f16 keep 22 bits, two bf16 only 16 (the results were 5e-6 off), so a bf16 cache
-// takes three. Three parts of P do not fit over S in TMEM, so such a CTA has one row tile.
+// takes three. Three parts of P do not fit over S in TMEM, so such a CTA has one row tile. The
+// tensor cores drop the bits below an accumulator's last place, towards zero, at every step, which
+// over a long row shows in f32: every kPpFlush tiles O moves from TMEM to sums in the workspace that
+// are added with rounding (500 rows behind 3500 keys: 1.4e-6 off, 2.5e-6 without; it costs a causal
+// prompt of 4096 rows 147 us against 125).
 //
 // K and V come page by page by TMA (128-byte swizzle; rows of a page and head are contiguous)
 // into a ring of 32 KB tiles. V rows that no query of the CTA sees are zeros in shared memory: their
@@ -44,6 +49,7 @@ constexpr int kPpRegsMany = 104, kPpRegsFew = 64;
 constexpr int kPpKeys = 128;
 constexpr int kPpTileBytes = 128 * 256;  // a 128 x 128 tile of 16-bit elements
 constexpr int kPpMaxSplits = 32;
+constexpr int kPpFlush = 4;        // tiles between two moves of O to the workspace (f32 results)
 constexpr float kPpLag = 8.0f, kPpShift = 7.0f;
 
 struct PPromptArgs {
@@ -51,8 +57,10 @@ struct PPromptArgs {
   PAttnArgs a;
   int splits;
   int cta_rows;  // 128 times the row tiles of a CTA
-  float* po;     // [item][KV head][split][cta_rows][128] unnormalised
-  float2* pml;   // [item][KV head][split][cta_rows]
+  // Unnormalised sums (f32 results, or parts > 1): [item][KV head][split][32 groups of 4 dims][cta_rows], so
+  // that a warp's rows lie side by side; and their maxima and weights: [item][KV head][split][cta_rows].
+  float4* po;
+  float2* pml;
 };
 
 template <int PARTS>
@@ -422,15 +430,19 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
     const unsigned id_s = pp_idesc<T>(false), id_o = pp_idesc<T>(true), leader = lane == 0;
     const unsigned long long dq = umma_desc_k_sw128(tc_smem(qs)), dk = umma_desc_k_sw128(tc_smem(ring));
     const unsigned long long dv = umma_desc_mn_sw128(tc_smem(ring));
-    auto scores = [&](int t, int slot) {  // S_t = Q_t K^T
+    // S_t = Q_t K^T. The smallest part goes first: the accumulator drops bits towards zero at every step,
+    // and that costs the less the smaller the sum still is (f32 results at 64 + 3500 keys: 2.0e-6 off
+    // with the largest part first, 0.9e-6 so).
+    auto scores = [&](int t, int slot) {
       const unsigned long long q0 = dq + (unsigned)(t * (kQTile >> 4)), k0 = dk + (unsigned)(slot * (kPpTileBytes >> 4));
 #pragma unroll
       for (int part = 0; part < PARTS; ++part)
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
           const unsigned off = ((ks >> 2) * (kPpTileBytes / 2) + (ks & 3) * 32) >> 4;
-          if (part == 0 && ks == 0) pp_mma_ss<false>(tmem + t * 128, q0, k0, id_s, leader);
-          else pp_mma_ss<true>(tmem + t * 128, q0 + part * (kPpTileBytes >> 4) + off, k0 + off, id_s, leader);
+          const unsigned qo = (PARTS - 1 - part) * (kPpTileBytes >> 4) + off;
+          if (part == 0 && ks == 0) pp_mma_ss<false>(tmem + t * 128, q0 + qo, k0, id_s, leader);
+          else pp_mma_ss<true>(tmem + t * 128, q0 + qo, k0 + off, id_s, leader);
         }
       pp_commit(&s_full[t], leader);
     };
@@ -457,8 +469,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         for (int part = 0; part < PARTS; ++part)
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks) {
-            if (part == 0 && ks == 0) pp_mma_ts(od, pd, v0, id_o, j > 0, leader);
-            else pp_mma_ts(od, pd + part * 64 + ks * 8, v0 + ks * (2048 >> 4), id_o, true, leader);
+            const unsigned po = (PARTS - 1 - part) * 64 + ks * 8;
+            if (part == 0 && ks == 0) pp_mma_ts(od, pd + po, v0, id_o, PARTS > 1 ? j % kPpFlush != 0 : j > 0, leader);
+            else pp_mma_ts(od, pd + po, v0 + ks * (2048 >> 4), id_o, true, leader);
           }
         pp_commit(&o_done[t], leader);
         if (t == halves - 1) pp_commit(&empty[vs], leader);
@@ -536,6 +549,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       // positions of the warp's first and last live rows
       const unsigned lv = __ballot_sync(0xffffffffu, live);
       const int pw0 = __shfl_sync(0xffffffffu, p, 0), pw1 = __shfl_sync(0xffffffffu, p, lv ? 31 - __clz(lv) : 0);
+      const long long part0 = (((long long)item * kvh + g) * pa.splits + z) * kRows;
+      float4* mine = pa.po + part0 * (kHeadDim / 4) + lr;
+      float moved = -INFINITY;  // the maximum that the sums in the workspace go by
       bool ok = true;  // (a warp that has given up still meets its partner at their barriers, where both end)
       for (int j = 0; j < nk; ++j) {
         ok = ok && __all_sync(0xffffffffu, pp_wait(&s_full[t], (unsigned)j & 1u, &failed));
@@ -604,6 +620,29 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
             }
           }
         }
+        if (PARTS > 1 && j > 0 && j % kPpFlush == 0) {
+          ok = ok && __all_sync(0xffffffffu, pp_wait(&o_done[t], (unsigned)(j - 1) & 1u, &failed));
+          tc_fence_after();
+          const float f = moved == -INFINITY ? 0.0f : exp2_fast(moved - m);
+#pragma unroll 1
+          for (int h = 0; h < 4; ++h) {
+            unsigned o[16];
+            tmem_ld16(to + 16 * h, o);
+            float4* dst = mine + (16 * hf + 4 * h) * kRows;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float4 x = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                     __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+              if (j > kPpFlush) {
+                const float4 y = dst[i * kRows];
+                x = make_float4(fmaf(y.x, f, x.x), fmaf(y.y, f, x.y), fmaf(y.z, f, x.z), fmaf(y.w, f, x.w));
+              }
+              dst[i * kRows] = x;
+            }
+          }
+          moved = m;
+          tc_fence_before();
+        }
         const float ref = m == -INFINITY ? 0.0f : kPpShift - m;
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
@@ -639,18 +678,28 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         tc_fence_after();
         const bool whole = parts == 1;
         const float f = whole ? inv_sum(l) : 1.0f;
-        const long long prow = (((long long)item * kvh + g) * pa.splits + z) * kRows + lr;
         const long long base = (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf;
-        if (!whole && hf == 0) pa.pml[prow] = make_float2(m, l);
+        if (!whole && hf == 0) pa.pml[part0 + lr] = make_float2(m, l);
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {
           float o[32];
           tmem_ld32(to + 32 * h, o);
+          if (PARTS > 1 && nk > kPpFlush) {
+            const float fm = moved == -INFINITY ? 0.0f : exp2_fast(moved - m);
+            const float4* src = mine + (16 * hf + 8 * h) * kRows;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float4 y = src[i * kRows];
+              o[4 * i] = fmaf(y.x, fm, o[4 * i]);
+              o[4 * i + 1] = fmaf(y.y, fm, o[4 * i + 1]);
+              o[4 * i + 2] = fmaf(y.z, fm, o[4 * i + 2]);
+              o[4 * i + 3] = fmaf(y.w, fm, o[4 * i + 3]);
+            }
+          }
           if (!whole) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<float4*>(pa.po + prow * kHeadDim + 64 * hf + 32 * h + i) =
-                  make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+              mine[(16 * hf + 8 * h + i / 4) * kRows] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           } else if (live) {
             if constexpr (PARTS > 1) {
 #pragma unroll
@@ -679,12 +728,13 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
   if (warp == kPpSoftmax / 32) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
-// Adds the parts of rows whose key tiles were split. One warp per row; grid: items * kv_heads * cta_rows / 8.
+// Adds the parts of rows whose key tiles were split. A CTA takes eight rows, a thread four dims of
+// one; grid: items * kv_heads * cta_rows / 8.
 __global__ void __launch_bounds__(256) k_paged_prompt_join(const __grid_constant__ PPromptArgs pa) {
   const PAttnArgs& a = pa.a;
-  const int kvh = a.kv.kv_heads, G = a.q_heads / kvh, lane = threadIdx.x & 31;
-  const int R = pa.cta_rows, per = R >> 3;
-  const int r = (blockIdx.x % per) * 8 + (threadIdx.x >> 5), ig = blockIdx.x / per, g = ig % kvh, item = ig / kvh;
+  const int kvh = a.kv.kv_heads, G = a.q_heads / kvh, R = pa.cta_rows, per = R >> 3;
+  const int r = (blockIdx.x % per) * 8 + (threadIdx.x & 7), d4 = threadIdx.x >> 3;
+  const int ig = blockIdx.x / per, g = ig % kvh, item = ig / kvh;
   pdl_wait();
   pdl_trigger();
   int seq = 0, tile = 0;
@@ -692,20 +742,21 @@ __global__ void __launch_bounds__(256) k_paged_prompt_join(const __grid_constant
   const PpItem it = pp_rows(a, G, R, seq, tile);
   const int parts = pp_parts(it.v.tiles, pa.splits), row = tile * R + r, tok = row / G;
   if (parts == 1 || row >= it.n_rows || (unsigned)(it.tok0 + tok) >= (unsigned)a.rows) return;
-  const long long p0 = ((long long)item * kvh + g) * pa.splits * R + r;
-  const float2 ml = lane < parts ? pa.pml[p0 + (long long)lane * R] : make_float2(-INFINITY, 0.0f);
-  const float M = warp_max(ml.x);
-  const float f = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - M);
-  const float L = warp_sum(ml.y * f);
+  const long long p0 = ((long long)item * kvh + g) * pa.splits * R;
+  float M = -INFINITY;
+  for (int k = 0; k < parts; ++k) M = fmaxf(M, pa.pml[p0 + k * R + r].x);
+  float L = 0.0f;
   float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
+#pragma unroll 4
   for (int k = 0; k < parts; ++k) {
-    const float fk = __shfl_sync(0xffffffffu, f, k);
-    const float4 x = *reinterpret_cast<const float4*>(pa.po + (p0 + (long long)k * R) * kHeadDim + 4 * lane);
-    y = make_float4(y.x + x.x * fk, y.y + x.y * fk, y.z + x.z * fk, y.w + x.w * fk);
+    const float2 ml = pa.pml[p0 + k * R + r];
+    const float4 x = pa.po[(p0 + (long long)k * R) * (kHeadDim / 4) + (long long)d4 * R + r];
+    const float f = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - M);
+    L = fmaf(ml.y, f, L);
+    y = make_float4(fmaf(x.x, f, y.x), fmaf(x.y, f, y.y), fmaf(x.z, f, y.z), fmaf(x.w, f, y.w));
   }
   const float zf = inv_sum(L);
-  store4(a.y, (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + row % G) * kHeadDim + 4 * lane, a.dtype,
+  store4(a.y, (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + row % G) * kHeadDim + 4 * d4, a.dtype,
          make_float4(y.x * zf, y.y * zf, y.z * zf, y.w * zf));
 }
 

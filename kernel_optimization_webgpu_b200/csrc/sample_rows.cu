@@ -46,7 +46,7 @@ constexpr int kRowsWarps = kRowsThreads / 32;
 constexpr int kRowsMaxVocab = 393216;
 constexpr int kRowsMaxCluster = 8;
 constexpr int kRowsMaxPer = kRowsMaxVocab / kRowsMaxCluster;  // tokens a CTA takes: its 32-bit sums of 16 bits fit
-constexpr int kRowsBins = 2048;       // four a thread of the leader; 1024 left 40 of 64 rows above a list's size
+constexpr int kRowsBins = 2048;       // four a thread of the leader
 constexpr int kRowsExact = kRowsBins / 2;  // bins of an exact histogram (twice the words a bin)
 constexpr int kRowsList = 1024;
 constexpr double kRowsOne = 17592186044416.0;  // weight 1 = 2^44

@@ -187,7 +187,8 @@ Tensor paged_attn_prompt(const Tensor& q, const Tensor& k, const Tensor& v, cons
   const Here here(q.device());
   const Tensor y = a.out(q, y_out);
   const Tensor ws =
-      workspace(ws_in, qd_paged_attn_prompt_workspace_bytes(a.kv.batch, rows, a.heads, a.kv.kv_heads), q.device());
+      workspace(ws_in, qd_paged_attn_prompt_workspace_bytes(a.kv.batch, rows, a.heads, a.kv.kv_heads, a.dtype),
+                q.device());
   done(qd_paged_attn_prompt(&a.kv, q.const_data_ptr(), a.dtype, a.q_stride, rows,
                             vec<int32_t>(q_starts, (int64_t)a.kv.batch + 1, at::kInt, q.device(), "q_starts"), a.heads,
                             to_int(window, "bad window"), to_int(sinks, "bad sinks"), (float)scale, y.data_ptr(),
