@@ -429,8 +429,8 @@ int qd_paged_append(const qd_paged_kv* kv, const void* qkv, int qkv_dtype, int64
 
 /* Attention of one new token per sequence (rows = batch): y[b] = softmax(scale * q[b] k^T) v
  * over the keys that position seq_lens[b] - 1 sees. q, y [batch][q_heads][128], rows q_stride /
- * y_stride elements apart (multiples of 8), 16-byte aligned; dtype (of both) QD_KV_F32 or the
- * cache's. q_heads is a multiple of kv_heads, at most 64 times it. The softmax and its sums
+ * y_stride elements apart (multiples of 8), 16-byte aligned, y apart from all that is read; dtype
+ * (of both) QD_KV_F32 or the cache's. q_heads is a multiple of kv_heads, at most 64 times it. The softmax and its sums
  * are f32; with dtype QD_KV_F32 the products keep f32 accuracy too (q and the weights go into
  * them as sums of two f16 or three bf16), with a 16-bit dtype the prompt's weights are rounded to
  * it once. scale 0 means 1/sqrt(128). The workspace holds

@@ -7,11 +7,13 @@
 //   P = exp2(S c - m)   two threads per row: maximum, weights, their sum, all in f32
 //   O += P V       -> TMEM (f32), P read from TMEM   M 128, N 128 dims, K 128 keys
 // The two tiles alternate: while one's softmax runs, the tensor cores work for the other. P
-// (One thread per row left a single softmax warp of a tile on each scheduler, and its chain of
-// dependent instructions set the pace; with two the MMA warp does. Uniform operands there, see below,
-// then took 8192 causal rows of 16 heads from 301 to 266 us = 1032 TFLOP/s.) P
 // replaces its S in TMEM (S0 S1 O0 O1 = 512 columns); the MMAs of one issuer run in order, so
-// S of the next key tile may be issued right behind the product that reads P.
+// S of the next key tile may be issued right behind the product that reads P. What bounds it:
+// 2048 cycles of products and as many of exponentials per 256 rows and 128 keys, in a loop of
+// 3460 (scores ready -> weights ready 1900, products -> next scores ready 1460, for each tile in
+// turn): 8192 causal rows of 16 heads take 266 us = 1032 TFLOP/s. One thread per row instead of
+// two: 301 us. An exp2 by polynomial for 3 to 8 of 16 weights: 269 to 287 us (the softmax warps
+// wait on each other's instructions, not on the special-function unit).
 //
 // O is rescaled only when a row's maximum has grown by more than 2^kPpLag since the last time
 // (weights then stay below 2^(kPpLag + kPpShift), inside f16); the final division makes up for
@@ -73,13 +75,25 @@ __host__ __device__ constexpr int pp_smem() {
 }
 
 // The item-th tile of rows, counted from the last (the latest rows of a prompt see the most keys
-// and start first): its sequence and tile, or false. Called by whole warps.
-__device__ __forceinline__ bool pp_item(const PAttnArgs& a, int G, int cta_rows, int item, int& seq, int& tile) {
+// and start first): its sequence, tile, first row, new tokens and length, or false. Called by
+// whole warps; up to 32 sequences take one round trip to memory.
+__device__ __forceinline__ bool pp_item(const PAttnArgs& a, int G, int cta_rows, int item, int& seq, int& tile, int& start,
+                                        int& fresh, int& asked) {
   const int lane = threadIdx.x & 31, B = a.kv.batch;
+  int n0 = 0, s0 = 0, len0 = 0;  // of the first 32 sequences
   int total = 0;
   for (int b0 = 0; b0 < B; b0 += 32) {
     const int b = b0 + lane;
-    const int n = b < B ? max(a.q_starts[b + 1] - a.q_starts[b], 0) : 0;
+    int n = 0, s = 0;
+    if (b < B) {
+      s = a.q_starts[b];
+      n = max(a.q_starts[b + 1] - s, 0);
+      if (b0 == 0) len0 = a.kv.seq_lens[b];
+    }
+    if (b0 == 0) {
+      n0 = n;
+      s0 = s;
+    }
     int t = (n * G + cta_rows - 1) / cta_rows;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
@@ -89,7 +103,7 @@ __device__ __forceinline__ bool pp_item(const PAttnArgs& a, int G, int cta_rows,
   if (want < 0) return false;
   for (int b0 = 0; b0 < B; b0 += 32) {
     const int b = b0 + lane;
-    const int n = b < B ? max(a.q_starts[b + 1] - a.q_starts[b], 0) : 0;
+    const int n = b0 == 0 ? n0 : b < B ? max(a.q_starts[b + 1] - a.q_starts[b], 0) : 0;
     const int t = (n * G + cta_rows - 1) / cta_rows;
     int incl = t;
 #pragma unroll
@@ -102,6 +116,9 @@ __device__ __forceinline__ bool pp_item(const PAttnArgs& a, int G, int cta_rows,
       const int src = __ffs(past) - 1;
       seq = b0 + src;
       tile = want - __shfl_sync(0xffffffffu, incl - t, src);
+      fresh = __shfl_sync(0xffffffffu, n, src);
+      start = b0 == 0 ? __shfl_sync(0xffffffffu, s0, src) : a.q_starts[seq];
+      asked = b0 == 0 ? __shfl_sync(0xffffffffu, len0, src) : a.kv.seq_lens[seq];
       return true;
     }
     want -= __shfl_sync(0xffffffffu, incl, 31);
@@ -114,14 +131,14 @@ struct PpItem {
   int tok0, n_rows, pos0, len, asked;  // row r: token tok0 + r / G at position pos0 + r / G
   Visible v;
 };
-__device__ __forceinline__ PpItem pp_rows(const PAttnArgs& a, int G, int cta_rows, int seq, int tile) {
+__device__ __forceinline__ PpItem pp_rows(const PAttnArgs& a, int G, int cta_rows, int tile, int start, int fresh,
+                                          int asked) {
   PpItem it;
-  const int s0 = a.q_starts[seq], n = a.q_starts[seq + 1] - s0;
-  it.asked = a.kv.seq_lens[seq];
-  it.len = paged_len(a.kv, seq);
-  it.tok0 = s0;
-  it.pos0 = it.asked - n;
-  it.n_rows = n * G;
+  it.asked = asked;
+  it.len = min(max(asked, 0), a.kv.table_width << a.kv.page_shift);
+  it.tok0 = start;
+  it.pos0 = asked - fresh;
+  it.n_rows = fresh * G;
   const int r0 = tile * cta_rows, r1 = min(r0 + cta_rows, it.n_rows);
   const int plo = it.pos0 + r0 / G, phi = it.pos0 + (r1 - 1) / G;
   Visible& v = it.v;
@@ -290,11 +307,16 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int kvh = a.kv.kv_heads, G = a.q_heads / kvh;
   const int g = blockIdx.x % kvh, z = (blockIdx.x / kvh) % pa.splits, item = blockIdx.x / (kvh * pa.splits);
+  if (tid == 0) {
+    tma_prefetch_map(&pa.tk);
+    tma_prefetch_map(&pa.tv);
+    tma_prefetch_map(&pa.tv16);
+  }
   pdl_wait();
   pdl_trigger();
-  int seq = 0, tile = 0;
-  if (!pp_item(a, G, kRows, item, seq, tile)) return;
-  const PpItem it = pp_rows(a, G, kRows, seq, tile);
+  int seq = 0, tile = 0, start = 0, fresh = 0, asked = 0;
+  if (!pp_item(a, G, kRows, item, seq, tile, start, fresh, asked)) return;
+  const PpItem it = pp_rows(a, G, kRows, tile, start, fresh, asked);
   if (it.asked > it.len && it.asked > 0 && tid == 0) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
   const int parts = pp_parts(it.v.tiles, pa.splits);
   if (z >= parts) return;
@@ -494,48 +516,53 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPpRegsMany));
     if (t < halves && nk > 0) {
       // ---- softmax: half a row per thread ----
-      // Q: K-major with the 128-byte swizzle; dead rows are zero. A negative scale changes the sign of q,
-      // so that the softmax always has a positive one.
-      {
-        const int r = tid & 127;
-        unsigned char* dst = qs + t * kQTile + hf * (kPpTileBytes / 2) + r * 128;
-        const long long base =
-            (long long)(it.tok0 + (live ? tok : 0)) * a.q_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf;
-        if constexpr (PARTS > 1) {
-#pragma unroll 4
-          for (int c = 0; c < 8; ++c) {
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-            if (live) {
-              x = load4<float>(a.q, base + 8 * c);
-              y = load4<float>(a.q, base + 8 * c + 4);
-              if (a.scale < 0.0f) {
-                x = make_float4(-x.x, -x.y, -x.z, -x.w);
-                y = make_float4(-y.x, -y.y, -y.z, -y.w);
-              }
-            }
-            unsigned u[4][PARTS];
-            split_parts<T, PARTS>(x.x, x.y, u[0]);
-            split_parts<T, PARTS>(x.z, x.w, u[1]);
-            split_parts<T, PARTS>(y.x, y.y, u[2]);
-            split_parts<T, PARTS>(y.z, y.w, u[3]);
-            const unsigned off = ((c ^ r) & 7) << 4;
+      // Q: K-major with the 128-byte swizzle; dead rows are zero. A warp copies its 32 rows' 64 dims row by
+      // row, neighbouring lanes on neighbouring chunks (a row per lane took 4.5 us of a busy GPU's
+      // time). A negative scale changes the sign of q, so that the softmax always has a positive one.
+      const int wr = (warp & 3) * 32;  // first of the warp's rows in its tile
+      unsigned char* wq = qs + t * kQTile + hf * (kPpTileBytes / 2);
+      const long long q_at =
+          live ? (long long)(it.tok0 + tok) * a.q_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf : -1;
+      if constexpr (PARTS > 1) {
+        const int c4 = lane & 15;
+#pragma unroll
+        for (int i0 = 0; i0 < 16; i0 += 8) {
+          float4 x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const long long at = __shfl_sync(0xffffffffu, q_at, 2 * (i0 + i) + (lane >> 4));
+            x[i] = at >= 0 ? load4<float>(a.q, at + 4 * c4) : make_float4(0.f, 0.f, 0.f, 0.f);
+            if (a.scale < 0.0f) x[i] = make_float4(-x[i].x, -x[i].y, -x[i].z, -x[i].w);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = wr + 2 * (i0 + i) + (lane >> 4);
+            unsigned u[2][PARTS];
+            split_parts<T, PARTS>(x[i].x, x[i].y, u[0]);
+            split_parts<T, PARTS>(x[i].z, x[i].w, u[1]);
+            const unsigned off = r * 128 + ((((c4 >> 1) ^ r) & 7) << 4) + (c4 & 1) * 8;
 #pragma unroll
             for (int part = 0; part < PARTS; ++part)
-              *reinterpret_cast<uint4*>(dst + part * kPpTileBytes + off) =
-                  make_uint4(u[0][part], u[1][part], u[2][part], u[3][part]);
-          }
-        } else {
-          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + base);
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            uint4 x = live ? src[c] : make_uint4(0, 0, 0, 0);
-            if (a.scale < 0.0f)
-              x = make_uint4(x.x ^ 0x80008000u, x.y ^ 0x80008000u, x.z ^ 0x80008000u, x.w ^ 0x80008000u);
-            *reinterpret_cast<uint4*>(dst + (((c ^ r) & 7) << 4)) = x;
+              *reinterpret_cast<uint2*>(wq + part * kPpTileBytes + off) = make_uint2(u[0][part], u[1][part]);
           }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      } else {
+        uint4 x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const long long at = __shfl_sync(0xffffffffu, q_at, 4 * i + (lane >> 3));
+          x[i] = at >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at + 8 * (lane & 7))
+                         : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (a.scale < 0.0f)
+            x[i] = make_uint4(x[i].x ^ 0x80008000u, x[i].y ^ 0x80008000u, x[i].z ^ 0x80008000u, x[i].w ^ 0x80008000u);
+          const int r = wr + 4 * i + (lane >> 3);
+          *reinterpret_cast<uint4*>(wq + r * 128 + (((lane ^ r) & 7) << 4)) = x[i];
+        }
       }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       pp_arrive(&q_full[t]);
       float m = -INFINITY, l = 0.0f;
       const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
@@ -678,8 +705,11 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         tc_fence_after();
         const bool whole = parts == 1;
         const float f = whole ? inv_sum(l) : 1.0f;
-        const long long base = (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf;
+        const long long y_at =
+            live ? (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf : -1;
         if (!whole && hf == 0) pa.pml[part0 + lr] = make_float2(m, l);
+        // Whole rows leave through the warp's part of Q's shared memory (every product that read it is done),
+        // 32 dims at a time, so that neighbouring lanes write neighbouring chunks.
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {
           float o[32];
@@ -700,20 +730,33 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
 #pragma unroll
             for (int i = 0; i < 32; i += 4)
               mine[(16 * hf + 8 * h + i / 4) * kRows] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-          } else if (live) {
-            if constexpr (PARTS > 1) {
-#pragma unroll
-              for (int i = 0; i < 32; i += 4)
-                *reinterpret_cast<float4*>(static_cast<float*>(a.y) + base + 32 * h + i) =
-                    make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; i += 8)
-                *reinterpret_cast<uint4*>(static_cast<T*>(a.y) + base + 32 * h + i) =
-                    make_uint4(pack2<T>(o[i] * f, o[i + 1] * f), pack2<T>(o[i + 2] * f, o[i + 3] * f),
-                               pack2<T>(o[i + 4] * f, o[i + 5] * f), pack2<T>(o[i + 6] * f, o[i + 7] * f));
-            }
+            continue;
           }
+          constexpr int kChunks = PARTS > 1 ? 8 : 4;  // 16-byte chunks of 32 dims
+          unsigned char* my_row = wq + (wr + lane) * 128;
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            uint4 x;
+            if constexpr (PARTS > 1)
+              x = make_uint4(__float_as_uint(o[4 * c] * f), __float_as_uint(o[4 * c + 1] * f),
+                             __float_as_uint(o[4 * c + 2] * f), __float_as_uint(o[4 * c + 3] * f));
+            else
+              x = make_uint4(pack2<T>(o[8 * c] * f, o[8 * c + 1] * f), pack2<T>(o[8 * c + 2] * f, o[8 * c + 3] * f),
+                             pack2<T>(o[8 * c + 4] * f, o[8 * c + 5] * f), pack2<T>(o[8 * c + 6] * f, o[8 * c + 7] * f));
+            *reinterpret_cast<uint4*>(my_row + (((c ^ lane) & 7) << 4)) = x;
+          }
+          __syncwarp();
+          constexpr int kAtOnce = 32 / kChunks;  // rows a step of the warp writes
+#pragma unroll
+          for (int i = 0; i < 32 / kAtOnce; ++i) {
+            const int r = i * kAtOnce + lane / kChunks, c = lane % kChunks;
+            const long long at = __shfl_sync(0xffffffffu, y_at, r);
+            const uint4 x = *reinterpret_cast<const uint4*>(wq + (wr + r) * 128 + (((c ^ r) & 7) << 4));
+            if (at >= 0)
+              *reinterpret_cast<uint4*>(static_cast<unsigned char*>(a.y) +
+                                        (at + 32 * h) * (PARTS > 1 ? 4 : (int)sizeof(T)) + 16 * c) = x;
+          }
+          __syncwarp();
         }
       }
     }
@@ -737,9 +780,9 @@ __global__ void __launch_bounds__(256) k_paged_prompt_join(const __grid_constant
   const int ig = blockIdx.x / per, g = ig % kvh, item = ig / kvh;
   pdl_wait();
   pdl_trigger();
-  int seq = 0, tile = 0;
-  if (!pp_item(a, G, R, item, seq, tile)) return;
-  const PpItem it = pp_rows(a, G, R, seq, tile);
+  int seq = 0, tile = 0, start = 0, fresh = 0, asked = 0;
+  if (!pp_item(a, G, R, item, seq, tile, start, fresh, asked)) return;
+  const PpItem it = pp_rows(a, G, R, tile, start, fresh, asked);
   const int parts = pp_parts(it.v.tiles, pa.splits), row = tile * R + r, tok = row / G;
   if (parts == 1 || row >= it.n_rows || (unsigned)(it.tok0 + tok) >= (unsigned)a.rows) return;
   const long long p0 = ((long long)item * kvh + g) * pa.splits * R;
