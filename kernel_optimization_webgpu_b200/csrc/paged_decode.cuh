@@ -20,6 +20,11 @@
 //    precision at no extra instruction. (tcgen05 wants 64 rows or more; 56 of them would idle.)
 //    Two bf16 hold only 16 of f32's 24 bits (results were 5e-6 off): with f32 queries on a bf16
 //    cache a second set of products takes the rest of both operands (THREE).
+//
+// 64 sequences of 2048 positions, 8 KV heads: 93 us for 537 MB = 5.8 TB/s; of 8192: 334 us = 6.4 TB/s.
+// About 10 us of either are the two launches and the chain of lookups before the first row (lengths,
+// table, row), which is why 1 x 32768 (134 MB) takes 33 us. Three slots and two CTAs an SM; two
+// slots and three CTAs: 112 us.
 #pragma once
 
 #include <type_traits>

@@ -11,9 +11,9 @@
 // S of the next key tile may be issued right behind the product that reads P. What bounds it:
 // 2048 cycles of products and as many of exponentials per 256 rows and 128 keys, in a loop of
 // 3460 (scores ready -> weights ready 1900, products -> next scores ready 1460, for each tile in
-// turn): 8192 causal rows of 16 heads take 266 us = 1032 TFLOP/s. One thread per row instead of
-// two: 301 us. An exp2 by polynomial for 3 to 8 of 16 weights: 269 to 287 us (the softmax warps
-// wait on each other's instructions, not on the special-function unit).
+// turn): 8192 causal rows of 16 heads take 255 us = 1077 TFLOP/s. Beside it at 266 us: one thread
+// per row instead of two 301 us, an exp2 by polynomial for 3 to 8 of 16 weights 269 to 287 us
+// (the softmax warps wait on each other's instructions, not on the special-function unit).
 //
 // O is rescaled only when a row's maximum has grown by more than 2^kPpLag since the last time
 // (weights then stay below 2^(kPpLag + kPpShift), inside f16); the final division makes up for
@@ -320,8 +320,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
   if (it.asked > it.len && it.asked > 0 && tid == 0) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
   const int parts = pp_parts(it.v.tiles, pa.splits);
   if (z >= parts) return;
-  const int t0 = (int)((long long)it.v.tiles * z / parts);
-  const int nk = __shfl_sync(0xffffffffu, (int)((long long)it.v.tiles * (z + 1) / parts) - t0, 0);
+  const int t0 = it.v.tiles * z / parts;  // (at most 2^23 tiles, 32 parts)
+  const int nk = __shfl_sync(0xffffffffu, it.v.tiles * (z + 1) / parts - t0, 0);
   const int row0 = tile * kRows;
   const int halves = __shfl_sync(0xffffffffu, kTiles == 2 && it.n_rows - row0 > 128 ? 2 : 1, 0);
 

@@ -25,6 +25,10 @@
 // is resolved alone: exact sums by step, the tokens of one step gathered and sorted, a step with
 // too many cut into finer ones by key, and where all of them are equal their order is their
 // index. The first CTA of the cluster leads: it tells the others what to do next and ends them.
+//
+// One row of 151936 f32 logits, top-k 40 and top-p 0.9: 14.4 us. 64 rows with settings of their own,
+// most of them over the whole vocabulary: 67 us (38.9 MB), two CTAs an SM in two waves; of a
+// cluster's 28 us there, 11 are the exact sums of all weights, 5 the histogram, 8 the leader's steps.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -842,16 +846,21 @@ __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_co
   if (upto <= kRowsList) {
     x.command(RowsCmd{kOpGather, 1, 0, (uint32_t)last, 0, 0, 0, cut_p && !few, 1, 0});
     int m = x.collect();
-    x.command(end);
+    const bool known = few || !cut_p;  // `last` is certain, not estimated: the other CTAs are done
+    if (known) x.command(end);
     x.sort_list(cum, m);
+    settled = true;
     if (few) m = min(m, top_k);
     if (cut_p) {
       u64 sum = 0;
       if (few) sum = cum[m - 1];
       else
         for (int c = 0; c < x.C; ++c) sum += sh.above[0][c];
-      m = min(m, x.find_entry(cum, m, min(max((u64)ceil(p_share * (double)sum), 1ull), cum[m - 1])) + 1);
+      const u64 goal = max((u64)ceil(p_share * (double)sum), 1ull);
+      settled = known || goal <= cum[m - 1] || (cut_m && last == mbin);
+      m = min(m, x.find_entry(cum, m, min(goal, cum[m - 1])) + 1);
     }
+    if (!known && settled) x.command(end);
     if (cut_m) {
       __syncthreads();
       if (tid == 0) sh.pick_at = 1;
@@ -870,7 +879,6 @@ __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_co
     const int at = x.find_entry(cum, m, min((u64)floor((double)u * (double)total), total - 1) + 1);
     id = (int)(uint32_t)x.list[at];
     logp = share(~(uint32_t)(x.list[at] >> 32));
-    settled = true;
   } else if (ranges) {
     // Both ranges in one list, in order: the draw's tokens lie at or before the border's. Where the
     // ranges overlap they are one. Running weights: exact, from those above each range.
