@@ -359,6 +359,14 @@ def test_prompt_window_and_sinks(window, sinks, io, cache):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("io,cache", [("f32", "f16"), ("f32", "bf16"), ("f16", "f16")])
+def test_long_prompt_over_many_key_tiles(io, cache):
+    """Enough rows that the keys are not split over CTAs, and up to 15 tiles of them in one row's sums."""
+    torch = _cuda()
+    run_prompt(torch, [1500, 90], [1900, 1800], (16, 8), 32, io, cache, 0, 0)
+
+
+@pytest.mark.gpu
 def test_prompt_equals_decode_for_single_tokens():
     torch = _cuda()
     from kernel_optimization_webgpu_b200 import runtime as R
