@@ -11,8 +11,9 @@
 // S of the next key tile may be issued right behind the product that reads P. What bounds it:
 // 2048 cycles of products and as many of exponentials per 256 rows and 128 keys, in a loop of
 // 3460 (scores ready -> weights ready 1900, products -> next scores ready 1460, for each tile in
-// turn): 8192 causal rows of 16 heads take 255 us = 1077 TFLOP/s. Beside it at 266 us: one thread
-// per row instead of two 301 us, an exp2 by polynomial for 3 to 8 of 16 weights 269 to 287 us
+// turn): 8192 causal rows of 16 heads take 252 us = 1090 TFLOP/s (255 before the products of the
+// first half of P's keys started ahead of the second). Beside it at 266 us: one thread per row
+// instead of two 301 us, an exp2 by polynomial for 3 to 8 of 16 weights 269 to 287 us
 // (the softmax warps wait on each other's instructions, not on the special-function unit).
 //
 // O is rescaled only when a row's maximum has grown by more than 2^kPpLag since the last time
@@ -297,7 +298,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
   unsigned char* qs =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* ring = qs + kTiles * kQTile;
-  __shared__ unsigned long long full[S], empty[S], s_full[2], p_full[2], o_done[2], q_full[2], drain;
+  __shared__ unsigned long long full[S], empty[S], s_full[2], p_half[2], p_full[2], o_done[2], q_full[2], drain;
   __shared__ unsigned bad_rows[8];  // of key tile j: bit i set where 16-key chunk i has no usable page
   __shared__ unsigned tmem_base;
   __shared__ float shared_row[256];  // between a row's two threads: a maximum (NaN: given up), then a sum
@@ -347,6 +348,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       tc_mbar_init(&s_full[i]);
       tc_mbar_init(&o_done[i]);
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 256;" ::"r"(tc_smem(&p_full[i])) : "memory");
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 256;" ::"r"(tc_smem(&p_half[i])) : "memory");
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 256;" ::"r"(tc_smem(&q_full[i])) : "memory");
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -482,19 +484,26 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       if (j + 1 < nk) ok = pp_wait(&full[ks_slot], kph, &failed) && ok;
       ok = __all_sync(0xffffffffu, ok);
       for (int t = 0; t < halves && ok; ++t) {
-        ok = __all_sync(0xffffffffu, pp_wait(&p_full[t], (unsigned)j & 1u, &failed));
-        if (!ok) break;
-        tc_fence_after();
         const unsigned long long v0 = dv + (unsigned)(vs * (kPpTileBytes >> 4));
         const unsigned od = tmem + kColO + t * 128, pd = tmem + kColP + t * 128;
 #pragma unroll
-        for (int part = 0; part < PARTS; ++part)
+        for (int half = 0; half < 2; ++half) {
+          ok = __all_sync(0xffffffffu, pp_wait(half ? &p_full[t] : &p_half[t], (unsigned)j & 1u, &failed));
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll
-          for (int ks = 0; ks < 8; ++ks) {
-            const unsigned po = (PARTS - 1 - part) * 64 + ks * 8;
-            if (part == 0 && ks == 0) pp_mma_ts(od, pd + po, v0, id_o, PARTS > 1 ? j % kPpFlush != 0 : j > 0, leader);
-            else pp_mma_ts(od, pd + po, v0 + ks * (2048 >> 4), id_o, true, leader);
-          }
+          for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int ks = 2 * half + (i & 1) + 4 * (i >> 1);  // keys 0-31 and 64-95, then the others
+              const unsigned po = (PARTS - 1 - part) * 64 + ks * 8;
+              if (half == 0 && part == 0 && i == 0)
+                pp_mma_ts(od, pd + po, v0, id_o, PARTS > 1 ? j % kPpFlush != 0 : j > 0, leader);
+              else
+                pp_mma_ts(od, pd + po, v0 + ks * (2048 >> 4), id_o, true, leader);
+            }
+        }
+        if (!ok) break;
         pp_commit(&o_done[t], leader);
         if (t == halves - 1) pp_commit(&empty[vs], leader);
         if (j + 1 < nk) {
@@ -688,6 +697,11 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
           }
 #pragma unroll
           for (int part = 0; part < PARTS; ++part) tmem_st16(tp + 64 * part + 16 * h, w[part]);
+          if (h == 0) {  // the products of the first half of both threads' keys may start
+            tmem_wait_st();
+            tc_fence_before();
+            if (ok) pp_arrive(&p_half[t]);
+          }
         }
         l += sum.x + sum.y;
         tmem_wait_st();
