@@ -107,6 +107,7 @@ struct RowsShared {
   float mx[kRowsMaxCluster], mn[kRowsMaxCluster];
   u64 part[kRowsMaxCluster];      // per-CTA sums for the leader
   u64 above[3][kRowsMaxCluster];  // kOpGather with sums: all, below lo, below lo2
+  u64 sums[3][kRowsWarps];        // of this CTA's warps
   int taken;                      // entries of this CTA's own list
   uint32_t key_min, key_max;      // leader
   int found;                      // leader: an index
@@ -129,7 +130,7 @@ struct RowsCta {
   RowsShared* sh;
   float* val;       // this CTA's tokens, filled up to a multiple of 4 with NaN
   uint32_t* hist;   // [2][kRowsBins]: counts, places; or [4][kRowsExact]: counts, and weights in three sums
-  const double* pow2;  // 2^(i / 128)
+  const double* pow2;  // 2^(44 + i / 128)
   u64* list;       // leader: {~key, index}
   int n, base, C, lg, rank;  // C = 1 << lg CTAs
   float vmax, scale, range;  // scale: places per unit of value
@@ -137,13 +138,11 @@ struct RowsCta {
   float step;             // width of a bin in the weight's logarithm to base 2
 
   // A value's place: 4096ths of a bin below the maximum, rounded by an addition of 2^23 (conversions
-  // run at an eighth of its rate). Ascending as v descends. kNoPlace for what has no weight: NaN,
-  // -inf, beyond the range; those are the last bin.
+  // run at an eighth of its rate). Ascending as v descends. kNoPlace for what has no weight (NaN,
+  // -inf, beyond the range; the scale keeps the range's end below it): those are the last bin.
   static constexpr uint32_t kNoPlace = (kRowsBins - 1) << 12;
   __device__ __forceinline__ uint32_t place(float v) const {
-    const float d = vmax - v;
-    const uint32_t u = __float_as_uint(fminf(fmaf(d, scale, 8388608.0f), 8388608.0f + (float)(kNoPlace - 1))) & 0x7fffffu;
-    return d <= range ? u : kNoPlace;
+    return __float_as_uint(fminf(fmaf(vmax - v, scale, 8388608.0f), 8388608.0f + (float)kNoPlace)) & 0x7fffffu;
   }
   __device__ __forceinline__ int bin(float v) const { return (int)(place(v) >> 12); }
   __device__ __forceinline__ int exact_bin(float v) const { return (int)(place(v) >> 13); }
@@ -151,7 +150,8 @@ struct RowsCta {
   // 2^(44 + e) 2^(i / 128) 2^(r / 128), |r| <= 1 / 2, the last factor by its Taylor sum to the fourth
   // power (the rest is below 2^-49): table-driven, after Tang, ACM TOMS 15 (1989). Roundings to
   // an integer are additions of 1.5 * 2^52 and 2^52.
-  __device__ __forceinline__ double raw_weight(float v) const {  // before the last rounding, v within the range
+  // (before the last rounding; of a value beyond the range it is meaningless)
+  __device__ __forceinline__ double raw_weight(float v) const {
     const double d = (double)v - (double)vmax;
     const double near = fma(d, z_scale, 6755399441055744.0);
     const int k = __double2loint(near);
@@ -159,7 +159,7 @@ struct RowsCta {
     constexpr double c = 0.6931471805599453 / 128.0;
     const double p = fma(fma(fma(fma(c * c * c * c / 24.0, r, c * c * c / 6.0), r, c * c / 2.0), r, c), r, 1.0);
     const double w = p * pow2[k & 127];
-    return __hiloint2double(__double2hiint(w) + (((k >> 7) + 44) << 20), __double2loint(w));
+    return __hiloint2double(__double2hiint(w) + ((k << 13) & 0xfff00000), __double2loint(w));
   }
   __device__ __forceinline__ u64 weight(float v) const {
     if (!(vmax - v <= range)) return 0ull;
@@ -302,31 +302,50 @@ struct RowsCta {
         // Each thread adds at most 96 weights below 2^45 to 2^52: additions there round every weight to an
         // integer and are exact otherwise.
         double sum[3] = {4503599627370496.0, 4503599627370496.0, 4503599627370496.0};
+        const bool two = c.lo2 <= c.hi2;
         const uint32_t lo = c.lo << 12, span = ((c.hi + 1) << 12) - lo, lo2 = c.lo2 << 12;
-        const uint32_t span2 = c.lo2 <= c.hi2 ? ((c.hi2 + 1) << 12) - lo2 : 0u;
+        const uint32_t span2 = two ? ((c.hi2 + 1) << 12) - lo2 : 0u;
         each4([&](const float (&v)[4], int i) {
+          double w[4];
+          uint32_t u[4];
           bool any = false;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t u = place(v[k]);
-            const double w = u < kNoPlace ? raw_weight(v[k]) : 0.0;
-            sum[0] += w;
-            if (u < lo) sum[1] += w;
-            if (u < lo2) sum[2] += w;
-            any = any || u - lo < span || u - lo2 < span2;
+            u[k] = place(v[k]);
+            w[k] = raw_weight(v[k]);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (u[k] < kNoPlace) sum[0] += w[k];
+            if (u[k] < lo) sum[1] += w[k];
+            any = any || u[k] - lo < span;
+          }
+          if (two) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (u[k] < lo2) sum[2] += w[k];
+              any = any || u[k] - lo2 < span2;
+            }
           }
           if (any) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t u = place(v[k]);
-              if ((u - lo < span || u - lo2 < span2) && i + k < n) keep(v[k], i + k);
-            }
+            for (int k = 0; k < 4; ++k)
+              if ((u[k] - lo < span || u[k] - lo2 < span2) && i + k < n) keep(v[k], i + k);
           }
         });
+        u64 all[3];
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
-          const u64 all = block_sum64((u64)__double_as_longlong(sum[k]) & 0xfffffffffffffull);
-          if (threadIdx.x == 0) lead->above[k][rank] = all;
+          all[k] = (u64)__double_as_longlong(sum[k]) & 0xfffffffffffffull;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) all[k] += __shfl_xor_sync(0xffffffffu, all[k], o);
+          if (lane == 0) sh->sums[k][threadIdx.x >> 5] = all[k];
+        }
+        __syncthreads();
+        if (threadIdx.x < 3) {
+          u64 total = 0;
+          for (int w = 0; w < kRowsWarps; ++w) total += sh->sums[threadIdx.x][w];
+          lead->above[threadIdx.x][rank] = total;
         }
       } else if (c.by_bin == 1) {
         const uint32_t lo = c.lo << 12, span = ((c.hi + 1) << 12) - lo;
@@ -686,7 +705,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_co
   x.base = x.rank * a.per;
   x.n = max(0, min(a.per, a.vocab - x.base));
   x.pow2 = pow2;
-  if (tid < 128) pow2[tid] = exp2(tid / 128.0);
+  if (tid < 128) pow2[tid] = exp2(tid / 128.0) * kRowsOne;
   auto started = x.cl.barrier_arrive();  // waited for before the first access to another CTA's memory
   pdl_wait();
   pdl_trigger();
@@ -775,7 +794,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_co
   x.z_scale = x.inv_t * (128.0 * 1.4426950408889634);
   // 32 T: 2^44 exp(-32) < 1/2, so that what lies beyond weighs nothing
   x.range = fminf(32.0f * temperature, mx - mn);
-  x.scale = x.range > 0.0f ? fminf((float)(RowsCta::kNoPlace) / x.range, 3.0e38f) : 0.0f;
+  x.scale = x.range > 0.0f ? fminf((float)(RowsCta::kNoPlace - 8) / x.range, 3.0e38f) : 0.0f;
   x.step = x.scale > 0.0f ? (float)(x.z_scale * (4096.0 / 128.0) / (double)x.scale) : 0.0f;
 
   // weights matter unless a top-k cut (or a min-p cut without a top-p one) leaves a short list
