@@ -21,13 +21,16 @@
 //  3. the tokens of those steps are gathered into the first CTA; in the same pass the exact
 //     weights of all tokens, and of those above each such range, are summed in registers. The
 //     leader sorts the gathered ones and finds the borders exactly.
+//     The border's range and the draw's share one such pass, or take one each where only both
+//     together are too long for the list (64 rows as below: 66 -> 65 us; a row that then needed the
+//     resolution below took 43 us, and takes 25 to 28).
 // Where a range holds more than kRowsList tokens (long classes of equal values, a large top-k), each border
 // is resolved alone: exact sums by step, the tokens of one step gathered and sorted, a step with
 // too many cut into finer ones by key, and where all of them are equal their order is their
 // index. The first CTA of the cluster leads: it tells the others what to do next and ends them.
 //
-// One row of 151936 f32 logits, top-k 40 and top-p 0.9: 14.4 us. 64 rows with settings of their own,
-// most of them over the whole vocabulary: 67 us (38.9 MB), two CTAs an SM in two waves; of a
+// One row of 151936 f32 logits, top-k 40 and top-p 0.9: 14.5 us. 64 rows with settings of their own,
+// most of them over the whole vocabulary: 65 us (38.9 MB), two CTAs an SM in two waves; of a
 // cluster's 28 us there, 11 are the exact sums of all weights, 5 the histogram, 8 the leader's steps.
 #include <cooperative_groups.h>
 
@@ -86,7 +89,8 @@ struct RowsCmd {
   uint32_t lo, hi;
   int shift;          // kOpHist by key: bin = (hi - key) >> shift
   int rank, n;        // kOpPick: CTA `rank` finds its n-th member by index
-  int sums;           // kOpGather: also the weights of all tokens, and of those in bins below lo and lo2
+  int sums;           // kOpGather: also the weights of all tokens, and of those in bins below lo and lo2;
+                      // 2: [lo2, hi2] are no members
   uint32_t lo2, hi2;  // kOpGather by bin: a second range of members (lo2 > hi2: none)
 };
 // A prefix of the row's order: every key above `key` and the first `ties` of those equal to it.
@@ -302,9 +306,9 @@ struct RowsCta {
         // Each thread adds at most 96 weights below 2^45 to 2^52: additions there round every weight to an
         // integer and are exact otherwise.
         double sum[3] = {4503599627370496.0, 4503599627370496.0, 4503599627370496.0};
-        const bool two = c.lo2 <= c.hi2;
+        const bool two = c.sums == 2 || c.lo2 <= c.hi2;
         const uint32_t lo = c.lo << 12, span = ((c.hi + 1) << 12) - lo, lo2 = c.lo2 << 12;
-        const uint32_t span2 = two ? ((c.hi2 + 1) << 12) - lo2 : 0u;
+        const uint32_t span2 = c.sums == 1 && two ? ((c.hi2 + 1) << 12) - lo2 : 0u;
         each4([&](const float (&v)[4], int i) {
           double w[4];
           uint32_t u[4];
@@ -848,11 +852,12 @@ __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_co
   }
   // without a top-k or min-p cut: the ranges of bins of the border and of the draw, if short enough
   const int p_lo = sh.at[1].bin, p_hi = last, d_lo = min(sh.at[3].bin, last), d_hi = min(sh.at[2].bin, last);
-  bool ranges = upto > kRowsList && kind == RowsCta::kPlaces && !cut_m;
+  bool ranges = upto > kRowsList && kind == RowsCta::kPlaces && !cut_m, apart = false;
   if (ranges) {
-    int found = sh.at[2].before + sh.at[2].count - sh.at[3].before;
-    if (cut_p) found += upto - sh.at[1].before;
-    ranges = found <= kRowsList;
+    const int n_draw = sh.at[2].before + sh.at[2].count - sh.at[3].before;
+    const int n_border = cut_p ? upto - sh.at[1].before : 0;
+    apart = n_draw + n_border > kRowsList;  // one after the other, if each fits alone
+    ranges = n_draw <= kRowsList && n_border <= kRowsList;
   }
   u64 total = 0;
   int id = 0;
@@ -900,9 +905,12 @@ __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_co
     logp = share(~(uint32_t)(x.list[at] >> 32));
   } else if (ranges) {
     // Both ranges in one list, in order: the draw's tokens lie at or before the border's. Where the
-    // ranges overlap they are one. Running weights: exact, from those above each range.
+    // ranges overlap they are one. Running weights: exact, from those above each range. (Apart: the
+    // border's list first, then the draw's.)
     RowsCmd c{kOpGather, 1, (uint32_t)d_lo, (uint32_t)d_hi, 0, 0, 0, 1, 1, 0};
-    if (cut_p) {
+    if (apart) {
+      c = RowsCmd{kOpGather, 1, (uint32_t)p_lo, (uint32_t)p_hi, 0, 0, 0, 2, (uint32_t)d_lo, (uint32_t)d_lo};
+    } else if (cut_p) {
       if (p_lo <= d_hi + 1) {
         c.hi = (uint32_t)p_hi;
       } else {
@@ -911,14 +919,14 @@ __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_co
       }
     }
     x.command(c);
-    const int m = x.collect();
+    int m = x.collect();
     u64 all = 0, above = 0, above2 = 0;
     for (int k = 0; k < x.C; ++k) {
       all += sh.above[0][k];
       above += sh.above[1][k];
       above2 += sh.above[2][k];
     }
-    const bool split = c.lo2 <= c.hi2;
+    const bool split = !apart && c.lo2 <= c.hi2;
     x.sort_list(cum, m);
     // entries of the first range, then what the second one's running weights lack
     int m1 = m;
@@ -935,7 +943,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_co
       __syncthreads();
       m1 = sh.pick_at;
     }
-    const u64 first = m1 > 0 ? cum[m1 - 1] : 0ull;
+    u64 first = m1 > 0 ? cum[m1 - 1] : 0ull;
     const u64 lift = split ? above2 - above - first : 0ull;  // weights between the ranges
     const u64 span = m > 0 ? above + cum[m - 1] + lift : 0ull;
     total = all;
@@ -945,6 +953,13 @@ __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_co
       const u64 from = split ? above + first + lift : above;  // before the border's range
       ok = goal > from && goal <= span;
       if (ok) total = above + lift + cum[x.find_entry(cum, m, goal - above - lift)];
+    }
+    if (ok && apart) {
+      x.command(RowsCmd{kOpGather, 1, (uint32_t)d_lo, (uint32_t)d_hi, 0, 0, 0, 0, 1, 0});
+      m = m1 = x.collect();
+      x.sort_list(cum, m);
+      above = above2;
+      first = m > 0 ? cum[m - 1] : 0ull;
     }
     if (ok) {
       const u64 goal = min((u64)floor((double)u * (double)total), total - 1) + 1;

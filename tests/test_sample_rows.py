@@ -111,6 +111,21 @@ def test_rows_match_the_definition(vocab, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("spread", [0.5, 1.0, 2.0, 4.0])
+@pytest.mark.parametrize("vocab", [1024, 1025, 151936])
+def test_borders_among_many_tokens(spread, vocab):
+    """Rows without top-k, where thousands of tokens weigh about the same: the border's and the draw's
+    neighbourhoods fit one list together, one after the other, or not at all."""
+    torch = _cuda()
+    rng = np.random.default_rng(int(spread * 10) + vocab)
+    rows = 24
+    x = torch.from_numpy(rng.standard_normal((rows, vocab)).astype(np.float32) * np.float32(spread)).cuda()
+    pick = lambda *a: [a[int(i)] for i in rng.integers(0, len(a), rows)]  # noqa: E731
+    check(torch, x, pick(1.0, 0.8, 1.3), [0] * rows, pick(1.0, 0.999, 0.95, 0.9, 0.7), [0.0] * rows,
+          rng.random(rows).tolist())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("vocab", [257, 151936])
 def test_ties_infinities_and_nan(vocab):
     torch = _cuda()
