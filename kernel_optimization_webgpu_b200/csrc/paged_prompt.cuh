@@ -11,7 +11,7 @@
 // S of the next key tile may be issued right behind the product that reads P. What bounds it:
 // 2048 cycles of products and as many of exponentials per 256 rows and 128 keys, in a loop of
 // 3460 (scores ready -> weights ready 1900, products -> next scores ready 1460, for each tile in
-// turn): 8192 causal rows of 16 heads take 252 us = 1090 TFLOP/s (255 before the products of the
+// turn): 8192 causal rows of 16 heads take 250 us = 1100 TFLOP/s (3 us more before the products of the
 // first half of P's keys started ahead of the second). Beside it at 266 us: one thread per row
 // instead of two 301 us, an exp2 by polynomial for 3 to 8 of 16 weights 269 to 287 us
 // (the softmax warps wait on each other's instructions, not on the special-function unit).
@@ -27,6 +27,12 @@
 // over a long row shows in f32: every kPpFlush tiles O moves from TMEM to sums in the workspace that
 // are added with rounding (500 rows behind 3500 keys: 1.4e-6 off, 2.5e-6 without; it costs a causal
 // prompt of 4096 rows 147 us against 125).
+//
+// Where the grid does not fit the GPU at once, a CTA goes on with the work of blocks that have not started
+// (cluster launch control), looked up by a warp of its own while the last key tiles are still on
+// their way: K and V of the next rows flow through the ring without a pause, their Q is on its
+// way into L2, and one row tile ends while the other still has products. 5 ragged chunks (480
+// blocks of 30 us, 8 of them start and end): 109 -> 98 us, 1.5 of them by Q's prefetch.
 //
 // K and V come page by page by TMA (128-byte swizzle; rows of a page and head are contiguous)
 // into a ring of 32 KB tiles. V rows that no query of the CTA sees are zeros in shared memory: their
@@ -45,7 +51,7 @@
 namespace qd {
 
 constexpr int kPpSoftmax = 512;    // softmax threads: two a row, 64 keys of a tile each
-constexpr int kPpThreads = 640;    // and the MMA warp, the copy warp and two idle ones
+constexpr int kPpThreads = 640;    // and the MMA warp, the copy warp, the scheduling warp and an idle one
 // Registers: 96 a thread at launch (61440 in all); a softmax thread holds 64 scores, so the last
 // warpgroup gives some of its share up: 512 * 104 + 128 * 64 = 61440.
 constexpr int kPpRegsMany = 104, kPpRegsFew = 64;
@@ -129,13 +135,12 @@ __device__ __forceinline__ bool pp_item(const PAttnArgs& a, int G, int cta_rows,
 
 // What the rows of an item are: first token, positions, and the keys that any of them sees.
 struct PpItem {
-  int tok0, n_rows, pos0, len, asked;  // row r: token tok0 + r / G at position pos0 + r / G
+  int seq, tok0, n_rows, pos0, len;  // row r: token tok0 + r / G at position pos0 + r / G
   Visible v;
 };
 __device__ __forceinline__ PpItem pp_rows(const PAttnArgs& a, int G, int cta_rows, int tile, int start, int fresh,
                                           int asked) {
   PpItem it;
-  it.asked = asked;
   it.len = min(max(asked, 0), a.kv.table_width << a.kv.page_shift);
   it.tok0 = start;
   it.pos0 = asked - fresh;
@@ -175,20 +180,50 @@ __device__ __forceinline__ unsigned pp_below(int n) { return n <= 0 ? 0u : n >= 
 __device__ __forceinline__ int pp_parts(int tiles, int splits) { return min(splits, max(1, tiles >> 1)); }
 
 // Bounded wait that gives up at once where another role already has.
-__device__ __forceinline__ bool pp_wait(unsigned long long* bar, unsigned parity, volatile int* failed) {
+__device__ __forceinline__ bool pp_wait(unsigned long long* bar, unsigned parity, volatile int* failed,
+                                        unsigned long long limit = kTcWaitNs) {
   if (tc_mbar_test(bar, parity)) return true;
   const unsigned long long t0 = tc_now();
   while (!tc_mbar_test(bar, parity)) {
     if (*failed) return false;
-    if (tc_now() - t0 > kTcWaitNs) {
+    if (tc_now() - t0 > limit) {
       *failed = 1;
       return false;
     }
   }
   return true;
 }
+// The limit of a wait for work of so many key tiles to come to its end (a tile takes 2 to 4 us).
+__device__ __forceinline__ unsigned long long pp_patience(int tiles) { return kTcWaitNs + 16384ull * (unsigned)tiles; }
 __device__ __forceinline__ void pp_arrive(unsigned long long* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc_smem(bar)) : "memory");
+}
+
+// What a CTA does next, as its scheduling warp writes it for the others. halves: row tiles, 0 at the end.
+struct PpWork {
+  PpItem it;
+  int item, row0, g, z, parts, t0, nk, halves;
+};
+// Takes a block of the grid that has not started yet; its index and true, or false when all have.
+__device__ __forceinline__ void pp_claim(void* answer, unsigned long long* bar) {
+  asm volatile(
+      "mbarrier.arrive.expect_tx.shared::cta.b64 _, [%1], 16;\n\t"
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+          tc_smem(answer)),
+      "r"(tc_smem(bar))
+      : "memory");
+}
+__device__ __forceinline__ bool pp_claimed(const void* answer, int& block) {
+  unsigned got, x;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\tld.shared.b128 h, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+      : "=r"(got), "=r"(x)
+      : "r"(tc_smem(answer))
+      : "memory");
+  block = (int)x;
+  return got != 0;
 }
 
 // B operand with its N index (dims) contiguous: 64-dim rows of 128 bytes, 128-byte swizzle; the
@@ -287,7 +322,8 @@ __device__ __forceinline__ void split_parts(float x, float y, unsigned (&u)[PART
   }
 }
 
-template <typename T, int PARTS>
+// CLAIM: blocks take the work of others that have not started (a grid that does not fit the GPU at once).
+template <typename T, int PARTS, bool CLAIM>
 __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_constant__ PPromptArgs pa) {
   const PAttnArgs& a = pa.a;
   constexpr int S = pp_slots<PARTS>(), kTiles = pp_tiles<PARTS>(), kRows = 128 * kTiles;
@@ -299,6 +335,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* ring = qs + kTiles * kQTile;
   __shared__ unsigned long long full[S], empty[S], s_full[2], p_half[2], p_full[2], o_done[2], q_full[2], drain;
+  __shared__ unsigned long long work_full[2], work_empty[2], ask, answered;
+  __shared__ __align__(16) uint4 answer;
+  __shared__ PpWork work[2];
   __shared__ unsigned bad_rows[8];  // of key tile j: bit i set where 16-key chunk i has no usable page
   __shared__ unsigned tmem_base;
   __shared__ float shared_row[256];  // between a row's two threads: a maximum (NaN: given up), then a sum
@@ -307,7 +346,6 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
   // in uniform registers)
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int kvh = a.kv.kv_heads, G = a.q_heads / kvh;
-  const int g = blockIdx.x % kvh, z = (blockIdx.x / kvh) % pa.splits, item = blockIdx.x / (kvh * pa.splits);
   if (tid == 0) {
     tma_prefetch_map(&pa.tk);
     tma_prefetch_map(&pa.tv);
@@ -315,22 +353,36 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
   }
   pdl_wait();
   pdl_trigger();
-  int seq = 0, tile = 0, start = 0, fresh = 0, asked = 0;
-  if (!pp_item(a, G, kRows, item, seq, tile, start, fresh, asked)) return;
-  const PpItem it = pp_rows(a, G, kRows, tile, start, fresh, asked);
-  if (it.asked > it.len && it.asked > 0 && tid == 0) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
-  const int parts = pp_parts(it.v.tiles, pa.splits);
-  if (z >= parts) return;
-  const int t0 = it.v.tiles * z / parts;  // (at most 2^23 tiles, 32 parts)
-  const int nk = __shfl_sync(0xffffffffu, it.v.tiles * (z + 1) / parts - t0, 0);
-  const int row0 = tile * kRows;
-  const int halves = __shfl_sync(0xffffffffu, kTiles == 2 && it.n_rows - row0 > 128 ? 2 : 1, 0);
-
-  // this thread's row and half of a row's keys and dims (softmax threads)
-  const int t = (tid >> 8) & 1, hf = (tid >> 7) & 1, lr = t * 128 + (tid & 127);
-  const int row = row0 + lr;
-  const int tok = row / G, hs = row - tok * G;
-  const bool live = tid < kPpSoftmax && lr < kRows && row < it.n_rows && (unsigned)(it.tok0 + tok) < (unsigned)a.rows;
+  // What block `b` of the grid is to do, if anything (whole warps).
+  auto find_work = [&](int b, PpWork& w) {
+    w.g = b % kvh;
+    w.z = (b / kvh) % pa.splits;
+    w.item = b / (kvh * pa.splits);
+    int seq = 0, tile = 0, start = 0, fresh = 0, asked = 0;
+    if (!pp_item(a, G, kRows, w.item, seq, tile, start, fresh, asked)) return false;
+    w.it = pp_rows(a, G, kRows, tile, start, fresh, asked);
+    w.it.seq = seq;
+    if (asked > w.it.len && asked > 0 && lane == 0) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
+    w.parts = pp_parts(w.it.v.tiles, pa.splits);
+    if (w.z >= w.parts) return false;
+    w.t0 = w.it.v.tiles * w.z / w.parts;  // (at most 2^23 tiles, 32 parts)
+    w.nk = w.it.v.tiles * (w.z + 1) / w.parts - w.t0;
+    w.row0 = tile * kRows;
+    w.halves = kTiles == 2 && w.it.n_rows - w.row0 > 128 ? 2 : 1;
+    return true;
+  };
+  PpWork first;
+  if (!find_work(blockIdx.x, first)) return;
+  // The n-th work of the block, when it is there (the one before has `tiles`); false: given up.
+  auto wait_work = [&](int n, int tiles) {
+    return !CLAIM ||
+           __all_sync(0xffffffffu, pp_wait(&work_full[n & 1], (unsigned)(n >> 1) & 1u, &failed, pp_patience(tiles)));
+  };
+  auto work_of = [&](int n) -> const PpWork& { return CLAIM ? work[n & 1] : first; };
+  auto work_done = [&](int n) {
+    __syncwarp();
+    if (CLAIM && lane == 0) pp_arrive(&work_empty[n & 1]);
+  };
 
   if (warp == kPpSoftmax / 32) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(&tmem_base)),
@@ -350,9 +402,18 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 256;" ::"r"(tc_smem(&p_full[i])) : "memory");
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 256;" ::"r"(tc_smem(&p_half[i])) : "memory");
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 256;" ::"r"(tc_smem(&q_full[i])) : "memory");
+      tc_mbar_init(&work_full[i]);
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(tc_smem(&work_empty[i])), "n"(kPpSoftmax / 32 + 2)
+                   : "memory");
     }
+    tc_mbar_init(&ask);
+    tc_mbar_init(&answered);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     failed = 0;
+    if (CLAIM) {
+      work[0] = first;
+      pp_arrive(&work_full[0]);
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -361,92 +422,148 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
 
   if (warp >= kPpSoftmax / 32) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPpRegsFew));
-    if (warp == kPpSoftmax / 32 + 1 && nk > 0) {
+    if (CLAIM && warp == kPpSoftmax / 32 + 2) {
+    // ---- schedule: this block's work, then that of blocks that have not started ----
+    // (asked for by the copy warp when it comes to the last tile)
+    int next = 1, claims = 0, block = 0, tiles = work[0].nk;
+    bool ok = true, more = true;
+    auto free_slot = [&] {
+      return next < 2 || __all_sync(0xffffffffu, pp_wait(&work_empty[next & 1], (unsigned)(next / 2 - 1) & 1u, &failed));
+    };
+    while (ok && more) {
+      ok = __all_sync(0xffffffffu, pp_wait(&ask, (unsigned)(next - 1) & 1u, &failed, pp_patience(tiles)));
+      if (!ok) break;
+      PpWork w;
+      do {
+        if (lane == 0) pp_claim(&answer, &answered);
+        ok = __all_sync(0xffffffffu, tc_mbar_wait(&answered, (unsigned)claims++ & 1u));
+        if (!ok) failed = 1;
+        more = ok && pp_claimed(&answer, block);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (read before the next answer lands)
+        __syncwarp();
+      } while (more && !find_work(__shfl_sync(0xffffffffu, block, 0), w));
+      if (!more) break;
+      for (int r = w.row0 + lane; r < min(w.row0 + kRows, w.it.n_rows); r += 32) {  // Q, to L2
+        const int tok = w.it.tok0 + r / G;
+        if ((unsigned)tok < (unsigned)a.rows) {
+          constexpr int kSize = PARTS > 1 ? 4 : 2;
+          const char* q = static_cast<const char*>(a.q) +
+                          ((long long)tok * a.q_stride + ((long long)w.g * G + r % G) * kHeadDim) * kSize;
+#pragma unroll
+          for (int i = 0; i < kHeadDim * kSize; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + i));
+        }
+      }
+      tiles = w.nk;
+      ok = free_slot();
+      if (ok && lane == 0) {
+        work[next & 1] = w;
+        pp_arrive(&work_full[next & 1]);
+      }
+      ++next;
+    }
+    if (ok && free_slot() && lane == 0) {
+      work[next & 1].halves = 0;
+      pp_arrive(&work_full[next & 1]);
+    }
+    } else if (warp == kPpSoftmax / 32 + 1) {
     // ---- copies: K and V tiles alternate through the ring ----
     const int ps = 1 << a.kv.page_shift, box = min(ps, kPpKeys), boxes = kPpKeys / box;
-    int issued_to = -1;
+    int issued_to = -1, done = 0;  // ring slots of the works before
     bool ok = true;
-    for (int i = 0; i < 2 * nk && ok; ++i) {
-      const int j = i >> 1, slot = i % S;
-      const bool is_v = i & 1;
-      const int k0 = it.v.tile(t0 + j) * kPpKeys;
-      // lane n: the page of the n-th box, if any row of the CTA sees it
-      int page = -1;
-      const int p0 = k0 + lane * box;
-      const bool any = lane < boxes && p0 < it.v.end && (p0 + box > it.v.lo || p0 < it.v.ns);
-      if (any) page = paged_page(a.kv, seq, p0);
-      const unsigned seen = __ballot_sync(0xffffffffu, any), good = __ballot_sync(0xffffffffu, page >= 0);
-      if (i >= S) ok = pp_wait(&empty[slot], (unsigned)(i / S - 1) & 1u, &failed);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      const bool partial = !(k0 + kPpKeys <= it.v.end && (k0 >= it.v.lo || k0 + kPpKeys <= it.v.ns)) || good != seen;
-      unsigned char* dst = ring + slot * kPpTileBytes;
-      if (lane == 0 && !is_v) {
-        unsigned bad = 0;
-        for (int n = 0; n < boxes; ++n)
-          if (((seen & ~good) >> n) & 1u) bad |= ((1u << (box / 16)) - 1u) << (n * (box / 16));
-        bad_rows[j & 7] = bad;
-        if (bad) paged_flag(a.kv, QD_PAGED_BAD_PAGE);
-      }
-      if (!(is_v && partial)) {  // whole boxes (what they hold of hidden keys gives scores that are masked)
-        if (lane == 0)
-          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc_smem(&full[slot])),
-                       "r"(__popc(good) * box * 256)
-                       : "memory");
-        __syncwarp();
-        if (page >= 0) {
-          const int y = (page * kvh + g) * ps + (p0 & (ps - 1));
-          unsigned char* d = dst + lane * box * 128;
-          tma_load_2d(d, is_v ? &pa.tv : &pa.tk, 0, y, &full[slot]);
-          tma_load_2d(d + kPpTileBytes / 2, is_v ? &pa.tv : &pa.tk, 64, y, &full[slot]);
+    for (int n = 0, nk = 0; ok && (CLAIM || n == 0); ++n) {
+      ok = wait_work(n, nk);
+      if (!ok || work_of(n).halves == 0) break;
+      const PpItem it = work_of(n).it;
+      const int seq = it.seq, g = work_of(n).g, t0 = work_of(n).t0;
+      nk = __shfl_sync(0xffffffffu, work_of(n).nk, 0);
+      if (CLAIM && nk == 0 && lane == 0) pp_arrive(&ask);
+      for (int i = 0; i < 2 * nk && ok; ++i) {
+        // the scheduling warp has the time of the ring's tiles to find the next work; earlier, a CTA would hold
+        // work that another one could begin
+        if (CLAIM && i == max(0, 2 * nk - 3) && lane == 0) pp_arrive(&ask);
+        const int j = i >> 1, at = done + i, slot = at % S;
+        const bool is_v = i & 1;
+        const int k0 = it.v.tile(t0 + j) * kPpKeys;
+        // lane n: the page of the n-th box, if any row of the CTA sees it
+        int page = -1;
+        const int p0 = k0 + lane * box;
+        const bool any = lane < boxes && p0 < it.v.end && (p0 + box > it.v.lo || p0 < it.v.ns);
+        if (any) page = paged_page(a.kv, seq, p0);
+        const unsigned seen = __ballot_sync(0xffffffffu, any), good = __ballot_sync(0xffffffffu, page >= 0);
+        if (at >= S) ok = pp_wait(&empty[slot], (unsigned)(at / S - 1) & 1u, &failed);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const bool partial = !(k0 + kPpKeys <= it.v.end && (k0 >= it.v.lo || k0 + kPpKeys <= it.v.ns)) || good != seen;
+        unsigned char* dst = ring + slot * kPpTileBytes;
+        if (lane == 0 && !is_v) {
+          unsigned bad = 0;
+          for (int n = 0; n < boxes; ++n)
+            if (((seen & ~good) >> n) & 1u) bad |= ((1u << (box / 16)) - 1u) << (n * (box / 16));
+          bad_rows[(at >> 1) & 7] = bad;
+          if (bad) paged_flag(a.kv, QD_PAGED_BAD_PAGE);
         }
-      } else {
-        // V of a tile with hidden rows, by groups of 16: TMA copies a group that is wholly visible and, from
-        // outside the tensor, the zeros of one that is wholly hidden; the rows of a group with both
-        // are copied or cleared one by one. (Clearing after the copy, row by row, cost 33 of 158 us
-        // where every row has a window: 5 ragged chunks of up to 1500 tokens.)
-        const int g0 = k0 + 16 * lane, gpage = __shfl_sync(0xffffffffu, page, (16 * (lane & 7)) / box);
-        bool all = lane < 8 && gpage >= 0, some = false;
-        if (all) {
-          some = g0 < it.v.end && (g0 + 16 > it.v.lo || g0 < it.v.ns);
-          all = g0 + 16 <= it.v.end && (g0 >= it.v.lo || g0 + 16 <= it.v.ns);
-        }
-        const unsigned edge = __ballot_sync(0xffffffffu, some && !all);
-        if (lane == 0)
-          asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(tc_smem(&full[slot])),
-                       "r"((8 - __popc(edge)) * 4096)
-                       : "memory");
-        __syncwarp();
-        if (lane < 8 && !((edge >> lane) & 1u)) {
-          const int y = all ? (gpage * kvh + g) * ps + (g0 & (ps - 1)) : -16;
-          unsigned char* d = dst + lane * 16 * 128;
-          tma_load_2d(d, &pa.tv16, 0, y, &full[slot]);
-          tma_load_2d(d + kPpTileBytes / 2, &pa.tv16, 64, y, &full[slot]);
-        }
-        for (unsigned left = edge; left; left &= left - 1) {
-          const int n = __ffs(left) - 1, q0 = k0 + 16 * n;
-          const long long row = ((long long)__shfl_sync(0xffffffffu, gpage, n) * kvh + g) * ps + (q0 & (ps - 1));
-          const char* src = static_cast<const char*>(a.kv.v) + row * 256 + (lane & 15) * 16;
-          const unsigned d = tc_smem(dst) + ((lane & 15) >> 3) * (kPpTileBytes / 2) + n * 16 * 128;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int r = 2 * e + (lane >> 4);
-            cp_async16(d + r * 128 + (((lane ^ r) & 7) << 4), src + r * 256, it.v.at(q0 + r));
-          }
-        }
-        if (edge) {
-          asm volatile("cp.async.wait_all;" ::: "memory");
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if (!(is_v && partial)) {  // whole boxes (what they hold of hidden keys gives scores that are masked)
+          if (lane == 0)
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc_smem(&full[slot])),
+                         "r"(__popc(good) * box * 256)
+                         : "memory");
           __syncwarp();
+          if (page >= 0) {
+            const int y = (page * kvh + g) * ps + (p0 & (ps - 1));
+            unsigned char* d = dst + lane * box * 128;
+            tma_load_2d(d, is_v ? &pa.tv : &pa.tk, 0, y, &full[slot]);
+            tma_load_2d(d + kPpTileBytes / 2, is_v ? &pa.tv : &pa.tk, 64, y, &full[slot]);
+          }
+        } else {
+          // V of a tile with hidden rows, by groups of 16: TMA copies a group that is wholly visible and, from
+          // outside the tensor, the zeros of one that is wholly hidden; the rows of a group with both
+          // are copied or cleared one by one. (Clearing after the copy, row by row, cost 33 of 158 us
+          // where every row has a window: 5 ragged chunks of up to 1500 tokens.)
+          const int g0 = k0 + 16 * lane, gpage = __shfl_sync(0xffffffffu, page, (16 * (lane & 7)) / box);
+          bool all = lane < 8 && gpage >= 0, some = false;
+          if (all) {
+            some = g0 < it.v.end && (g0 + 16 > it.v.lo || g0 < it.v.ns);
+            all = g0 + 16 <= it.v.end && (g0 >= it.v.lo || g0 + 16 <= it.v.ns);
+          }
+          const unsigned edge = __ballot_sync(0xffffffffu, some && !all);
+          if (lane == 0)
+            asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(tc_smem(&full[slot])),
+                         "r"((8 - __popc(edge)) * 4096)
+                         : "memory");
+          __syncwarp();
+          if (lane < 8 && !((edge >> lane) & 1u)) {
+            const int y = all ? (gpage * kvh + g) * ps + (g0 & (ps - 1)) : -16;
+            unsigned char* d = dst + lane * 16 * 128;
+            tma_load_2d(d, &pa.tv16, 0, y, &full[slot]);
+            tma_load_2d(d + kPpTileBytes / 2, &pa.tv16, 64, y, &full[slot]);
+          }
+          for (unsigned left = edge; left; left &= left - 1) {
+            const int n = __ffs(left) - 1, q0 = k0 + 16 * n;
+            const long long row = ((long long)__shfl_sync(0xffffffffu, gpage, n) * kvh + g) * ps + (q0 & (ps - 1));
+            const char* src = static_cast<const char*>(a.kv.v) + row * 256 + (lane & 15) * 16;
+            const unsigned d = tc_smem(dst) + ((lane & 15) >> 3) * (kPpTileBytes / 2) + n * 16 * 128;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int r = 2 * e + (lane >> 4);
+              cp_async16(d + r * 128 + (((lane ^ r) & 7) << 4), src + r * 256, it.v.at(q0 + r));
+            }
+          }
+          if (edge) {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
+          if (lane == 0) pp_arrive(&full[slot]);
         }
-        if (lane == 0) pp_arrive(&full[slot]);
-      }
-      issued_to = i;
+        issued_to = at;
+    }
+    done += 2 * nk;
+    work_done(n);
     }
     // nothing may still be landing when the CTA ends
     for (int i = max(0, issued_to - S + 1); i <= issued_to; ++i)
       (void)tc_mbar_wait(&full[i % S], (unsigned)(i / S) & 1u);
-  } else if (warp == kPpSoftmax / 32 && nk > 0) {
+    } else if (warp == kPpSoftmax / 32) {
     // ---- MMA issue ----
     // The whole warp runs the loop, so that the descriptors are warp-uniform values, and one lane issues.
     // (Under `if (lane == 0)` each of the 16 products of a tile and its operands took 90 cycles to issue,
@@ -470,15 +587,29 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         }
       pp_commit(&s_full[t], leader);
     };
-    bool ok = __all_sync(0xffffffffu, pp_wait(&full[0], 0, &failed));
-    for (int t = 0; t < halves && ok; ++t) {
-      ok = __all_sync(0xffffffffu, pp_wait(&q_full[t], 0, &failed));
-      tc_fence_after();
-      if (ok) scores(t, 0);
+    bool ok = true;
+    unsigned turn = 0, q_turn = 0;  // bit t: parity of row tile t's barriers before this work
+    int done = 0;                   // ring slots of the works before
+    for (int n = 0, nk = 0; ok && (CLAIM || n == 0); ++n) {
+      ok = wait_work(n, nk);
+      if (!ok) break;
+      nk = __shfl_sync(0xffffffffu, work_of(n).nk, 0);
+      const int halves = __shfl_sync(0xffffffffu, work_of(n).halves, 0);
+      work_done(n);
+      if (halves == 0) break;
+      if (nk == 0) continue;
+      auto ring_slot = [&](int i) { return (done + i) % S; };
+      auto ring_phase = [&](int i) { return (unsigned)((done + i) / S) & 1u; };
+      ok = __all_sync(0xffffffffu, pp_wait(&full[ring_slot(0)], ring_phase(0), &failed));
+      for (int t = 0; t < halves && ok; ++t) {
+        ok = __all_sync(0xffffffffu, pp_wait(&q_full[t], (q_turn >> t) & 1u, &failed));
+        tc_fence_after();
+        if (ok) scores(t, ring_slot(0));
     }
-    if (ok) pp_commit(&empty[0], leader);
-    int vs = 1 % S, ks_slot = 2 % S;       // ring slots of V of tile j and K of tile j + 1,
-    unsigned vph = 0, kph = 2 / S & 1u;    // and their phases
+    q_turn ^= halves == 2 ? 3u : 1u;
+    if (ok) pp_commit(&empty[ring_slot(0)], leader);
+    int vs = ring_slot(1), ks_slot = ring_slot(2);           // ring slots of V of tile j and K of tile j + 1,
+    unsigned vph = ring_phase(1), kph = ring_phase(2);       // and their phases
     for (int j = 0; j < nk && ok; ++j) {
       ok = pp_wait(&full[vs], vph, &failed);
       if (j + 1 < nk) ok = pp_wait(&full[ks_slot], kph, &failed) && ok;
@@ -488,7 +619,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         const unsigned od = tmem + kColO + t * 128, pd = tmem + kColP + t * 128;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          ok = __all_sync(0xffffffffu, pp_wait(half ? &p_full[t] : &p_half[t], (unsigned)j & 1u, &failed));
+          ok = __all_sync(0xffffffffu, pp_wait(half ? &p_full[t] : &p_half[t], (unsigned)(j ^ (turn >> t)) & 1u, &failed));
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
@@ -516,6 +647,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       ks_slot += 2;
       if (ks_slot >= S) ks_slot -= S, kph ^= 1u;
     }
+    done += 2 * nk;
+    if (nk & 1) turn ^= halves == 2 ? 3u : 1u;
+    }
     if (!ok) {  // given up: let what was issued finish before the CTA ends
       pp_commit(&drain, leader);
       (void)tc_mbar_wait(&drain, 0);
@@ -523,8 +657,25 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPpRegsMany));
+    // ---- softmax: half a row per thread ----
+    const int t = (tid >> 8) & 1, hf = (tid >> 7) & 1, lr = t * 128 + (tid & 127);
+    const int pair = 1 + t * 4 + (warp & 3);  // named barrier of the two warps that share 32 rows
+    int done = 0;       // key tiles of the works before
+    unsigned turn = 0;  // parity of this row tile's among them
+    bool ok = true;  // (a warp that has given up still meets its partner at their barriers, where both end)
+    for (int n = 0, nk = 0; CLAIM || n == 0; ++n) {
+      if (CLAIM) {
+        ok = ok && wait_work(n, nk);
+        if (pp_any(pair, !ok)) break;
+    }
+    const PpItem it = work_of(n).it;
+    const int item = work_of(n).item, g = work_of(n).g, z = work_of(n).z, parts = work_of(n).parts, t0 = work_of(n).t0,
+              halves = __shfl_sync(0xffffffffu, work_of(n).halves, 0);
+    nk = __shfl_sync(0xffffffffu, work_of(n).nk, 0);
+    if (halves == 0) break;
+    const int row = work_of(n).row0 + lr, tok = row / G, hs = row - tok * G;
+    const bool live = lr < kRows && row < it.n_rows && (unsigned)(it.tok0 + tok) < (unsigned)a.rows;
     if (t < halves && nk > 0) {
-      // ---- softmax: half a row per thread ----
       // Q: K-major with the 128-byte swizzle; dead rows are zero. A warp copies its 32 rows' 64 dims row by
       // row, neighbouring lanes on neighbouring chunks (a row per lane took 4.5 us of a busy GPU's
       // time). A negative scale changes the sign of q, so that the softmax always has a positive one.
@@ -577,7 +728,6 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
       const unsigned ts = tmem + t * 128 + lanes, tp = tmem + kColP + t * 128 + 32 * hf + lanes;
       const unsigned to = tmem + kColO + t * 128 + 64 * hf + lanes;
-      const int pair = 1 + t * 4 + (warp & 3);  // named barrier of the two warps that share 32 rows
       const float c = fabsf(a.scale) * kLog2e;
       const int p = live ? it.pos0 + tok : -1;
       const int pmax = min(p, it.len - 1);
@@ -588,14 +738,13 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       const long long part0 = (((long long)item * kvh + g) * pa.splits + z) * kRows;
       float4* mine = pa.po + part0 * (kHeadDim / 4) + lr;
       float moved = -INFINITY;  // the maximum that the sums in the workspace go by
-      bool ok = true;  // (a warp that has given up still meets its partner at their barriers, where both end)
       for (int j = 0; j < nk; ++j) {
-        ok = ok && __all_sync(0xffffffffu, pp_wait(&s_full[t], (unsigned)j & 1u, &failed));
+        ok = ok && __all_sync(0xffffffffu, pp_wait(&s_full[t], (unsigned)(j ^ turn) & 1u, &failed));
         tc_fence_after();
         unsigned sr[64];
         tmem_ld64(ts + 64 * hf, sr);
         const int k0 = it.v.tile(t0 + j) * kPpKeys;
-        const unsigned bad = bad_rows[j & 7];
+        const unsigned bad = bad_rows[(done + j) & 7];
         const bool inside = lv == 0xffffffffu && bad == 0 && k0 + kPpKeys - 1 <= min(pw0, it.len - 1) &&
                             (a.window == 0 || k0 > pw1 - a.window || k0 + kPpKeys <= a.sinks);
         if (!inside) {
@@ -644,7 +793,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
           m = mn;
           l *= f;
           if (j > 0) {  // the product of the tile before must have reached O
-            ok = __all_sync(0xffffffffu, pp_wait(&o_done[t], (unsigned)(j - 1) & 1u, &failed));
+            ok = __all_sync(0xffffffffu, pp_wait(&o_done[t], (unsigned)((j - 1) ^ turn) & 1u, &failed));
             tc_fence_after();
 #pragma unroll 1
             for (int h = 0; h < 4; ++h) {
@@ -657,7 +806,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
           }
         }
         if (PARTS > 1 && j > 0 && j % kPpFlush == 0) {
-          ok = ok && __all_sync(0xffffffffu, pp_wait(&o_done[t], (unsigned)(j - 1) & 1u, &failed));
+          ok = ok && __all_sync(0xffffffffu, pp_wait(&o_done[t], (unsigned)((j - 1) ^ turn) & 1u, &failed));
           tc_fence_after();
           const float f = moved == -INFINITY ? 0.0f : exp2_fast(moved - m);
 #pragma unroll 1
@@ -714,7 +863,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       if (hf == 1) shared_row[lr] += l;
       pp_meet(pair);
       l = shared_row[lr];
-      if (ok) ok = __all_sync(0xffffffffu, pp_wait(&o_done[t], (unsigned)(nk - 1) & 1u, &failed));
+      if (ok) ok = __all_sync(0xffffffffu, pp_wait(&o_done[t], (unsigned)((nk - 1) ^ turn) & 1u, &failed));
       if (ok) {
         tc_fence_after();
         const bool whole = parts == 1;
@@ -773,11 +922,16 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
           __syncwarp();
         }
       }
+      tc_fence_before();
+      turn ^= (unsigned)nk;
     }
-  }
-  if (nk == 0 && live) {  // no key is visible to any row
-    const long long base = (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf;
-    for (int i = 0; i < kHeadDim / 2; i += 4) store4(a.y, base + i, a.dtype, make_float4(0.f, 0.f, 0.f, 0.f));
+    done += nk;
+    if (nk == 0 && live) {  // no key is visible to any row
+      const long long base = (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf;
+      for (int i = 0; i < kHeadDim / 2; i += 4) store4(a.y, base + i, a.dtype, make_float4(0.f, 0.f, 0.f, 0.f));
+    }
+    work_done(n);
+    }
   }
   tc_fence_before();
   __syncthreads();

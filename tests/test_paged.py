@@ -14,6 +14,7 @@ Tolerances count roundings, relative to A = sum of |weight| |value| of an output
  - the output's own rounding, half a step of its type."""
 import ctypes as C
 import math
+import random
 
 import pytest
 
@@ -364,6 +365,43 @@ def test_long_prompt_over_many_key_tiles(io, cache):
     """Enough rows that the keys are not split over CTAs, and up to 15 tiles of them in one row's sums."""
     torch = _cuda()
     run_prompt(torch, [1500, 90], [1900, 1800], (16, 8), 32, io, cache, 0, 0)
+
+
+def many_chunks():
+    rng = random.Random(11)
+    new = [rng.choice([0, 1, 2, 33, 64, 127, 128, 129, 200]) for _ in range(60)]
+    return new, [n + rng.choice([0, 0, 5, 100, 700]) for n in new]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window,sinks", [(0, 0), (90, 3)])
+@pytest.mark.parametrize("heads", [(4, 4), (8, 4), (28, 4)], ids=lambda h: f"{h[0]}q{h[1]}kv")
+@pytest.mark.parametrize("io,cache", [("f32", "f16"), ("f16", "f16"), ("bf16", "bf16"), ("f32", "bf16")])
+def test_prompt_of_more_blocks_than_run_at_once(io, cache, heads, window, sinks):
+    torch = _cuda()
+    run_prompt(torch, *many_chunks(), heads, 16, io, cache, window, sinks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("io", ["f32", "f16"])
+def test_prompt_of_many_blocks_some_with_nothing_to_see(io):
+    """Sequences whose length says that nothing was appended give zeros; the others' rows stay as they are,
+    to the bit, and in every one of several runs."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    new, totals = many_chunks()
+    k, v, table, n = make_cache(torch, totals, 32, 4, "f16")
+    starts = torch.tensor([sum(new[:b]) for b in range(61)], dtype=torch.int32, device="cuda")
+    q = torch.randn(sum(new), 8, D, device="cuda").to(_types(torch)[io])
+    want = R.paged_attn_prompt(q, k, v, table, n, starts)
+    none = n.clone()
+    none[::3] = 0
+    hit = torch.zeros(sum(new), dtype=torch.bool, device="cuda")
+    for b in range(0, 60, 3):
+        hit[sum(new[:b]):sum(new[:b + 1])] = True
+    for _ in range(5):
+        got = R.paged_attn_prompt(q, k, v, table, none, starts)
+        assert bool((got[hit] == 0).all()) and torch.equal(got[~hit], want[~hit])
 
 
 @pytest.mark.gpu
