@@ -405,6 +405,43 @@ def test_prompt_of_many_blocks_some_with_nothing_to_see(io):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("io", ["f32", "f16"])
+def test_captured_prompts_follow_their_lengths_on_two_streams(io):
+    """A captured call over padded rows, replayed with other chunks, beside a second one on its own stream."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    rows, graphs = 6000, []
+    for seed in (0, 1):
+        new, totals = many_chunks()
+        k, v, table, n = make_cache(torch, totals, 16, 4, "f16", seed=seed)
+        starts = torch.tensor([sum(new[:b]) for b in range(61)], dtype=torch.int32, device="cuda")
+        q = torch.randn(rows, 8, D, device="cuda").to(_types(torch)[io])
+        y = torch.zeros_like(q)
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        R.paged_attn_prompt(q, k, v, table, n, starts, y=y)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            R.paged_attn_prompt(q, k, v, table, n, starts, y=y)
+        graphs.append((stream, graph, q, k, v, table, n, starts, y, new, totals))
+    for turn in range(4):
+        for stream, graph, q, k, v, table, n, starts, y, new, totals in graphs:
+            some = [c if (b + turn) % 4 else 0 for b, c in enumerate(new)]
+            starts.copy_(torch.tensor([sum(some[:b]) for b in range(61)], dtype=torch.int32))
+            n.copy_(torch.tensor([t - c + s for t, c, s in zip(totals, new, some)], dtype=torch.int32))
+            y.fill_(7.0)
+        torch.cuda.synchronize()
+        for stream, graph, *_ in graphs:
+            with torch.cuda.stream(stream):
+                for _ in range(3):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for stream, graph, q, k, v, table, n, starts, y, new, totals in graphs:
+            want = R.paged_attn_prompt(q, k, v, table, n, starts, y=torch.full_like(y, 7.0))
+            used = int(starts[-1])
+            assert torch.equal(y, want) and bool((y[used:] == 7.0).all()) and not bool((y[:used] == 7.0).any())
+
+
+@pytest.mark.gpu
 def test_prompt_equals_decode_for_single_tokens():
     torch = _cuda()
     from kernel_optimization_webgpu_b200 import runtime as R
