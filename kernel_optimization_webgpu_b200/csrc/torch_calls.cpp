@@ -5,6 +5,7 @@
 //
 // Python module kernel_optimization_webgpu_b200._torch_calls; runtime.py documents the functions.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
@@ -106,8 +107,13 @@ struct Here {
   explicit Here(c10::Device dev) : guard(dev), stream(c10::cuda::getCurrentCUDAStream(dev.index()).stream()) {}
 };
 
+// (straight from the allocator: through the dispatcher a call took 0.5 us more, of 5)
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, c10::Device dev) {
+  return at::detail::empty_cuda(sizes, type, dev, std::nullopt);
+}
+
 Tensor workspace(const Maybe& given, size_t bytes, c10::Device dev) {
-  if (!given) return at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
+  if (!given) return fresh({(int64_t)bytes}, at::kByte, dev);
   need(given->device() == dev && given->is_contiguous() && given->nbytes() >= bytes,
        "workspace must be a contiguous tensor of at least the bytes that the call asks for, on its device");
   return *given;
@@ -132,7 +138,7 @@ Tensor paged_append(const Tensor& qkv, const Tensor& k, const Tensor& v, const T
   const Here here(dev);
   need(!q_out || (q_out->device() == dev && q_out->dim() >= 1 && q_out->size(0) == rows),
        "q_out must have a row for every row of qkv, on its device");
-  const Tensor q = q_out ? *q_out : at::empty({rows, q_heads * 128}, qkv.options());
+  const Tensor q = q_out ? *q_out : fresh({rows, q_heads * 128}, qkv.scalar_type(), dev);
   done(qd_paged_append(&kv, qkv.const_data_ptr(), code(qkv, "qkv"), stride, to_int(rows, "too many rows"),
                        vec<int32_t>(q_starts, (int64_t)kv.batch + 1, at::kInt, dev, "q_starts"), (int)q_heads,
                        vec<float>(q_norm, 128, at::kFloat, dev, "q_norm"),
@@ -158,7 +164,7 @@ struct Attn {
     q_stride = row_stride(q, width, "q");
   }
   Tensor out(const Tensor& q, const Maybe& y) const {
-    if (!y) return at::empty(q.sizes(), q.options());
+    if (!y) return fresh(q.sizes(), q.scalar_type(), q.device());
     need(y->scalar_type() == q.scalar_type() && y->sizes() == q.sizes() && y->device() == q.device(),
          "y must have q's type, shape and device");
     return *y;
@@ -204,8 +210,8 @@ std::pair<Tensor, Tensor> sample_rows(const Tensor& logits, const Tensor& u, con
   need(dev.is_cuda(), "tensors must be on a CUDA device");
   const int64_t rows = logits.size(0), vocab = logits.size(1), stride = row_stride(logits, vocab, "logits");
   const Here here(dev);
-  const Tensor ids = ids_out ? *ids_out : at::empty({rows}, logits.options().dtype(at::kInt));
-  const Tensor logprobs = logprobs_out ? *logprobs_out : at::empty({rows}, logits.options().dtype(at::kFloat));
+  const Tensor ids = ids_out ? *ids_out : fresh({rows}, at::kInt, dev);
+  const Tensor logprobs = logprobs_out ? *logprobs_out : fresh({rows}, at::kFloat, dev);
   need(vocab <= UINT32_MAX, "vocab too large");
   done(qd_sample_rows(logits.const_data_ptr(), code(logits, "logits"), to_int(rows, "too many rows"), (uint32_t)vocab,
                       stride, vec<float>(temperature, rows, at::kFloat, dev, "temperature"),
