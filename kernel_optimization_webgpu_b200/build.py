@@ -1,12 +1,14 @@
 """Build recipe for the in-tree CUDA library (libqdecode.so, sm_100a).
 
 The library is compiled with nvcc directly (no torch extension machinery): it is
-a plain C-ABI shared object that JavaScript, C or Python can load. Beside it, where
-torch is installed, _torch_calls.so: the Python module through which runtime.py's paged
-operators and batched sampler take torch tensors (csrc/torch_calls.cpp).
+a plain C-ABI shared object that JavaScript, C or Python can load. Beside it, for the
+installed torch, _torch_calls.so: the Python module through which runtime.py's paged
+operators and batched sampler take torch tensors (csrc/torch_calls.cpp). It is built apart
+(build_calls), when one of them is first called: nothing else needs it.
 """
 from __future__ import annotations
 
+import hashlib
 import importlib.util
 import os
 import shutil
@@ -22,6 +24,7 @@ SOURCES = ["engine.cu", "batch.cu", "noalloc.cu", "bench_api.cu", "sample.cu", "
 DEPS = SOURCES + ["kernels.cuh", "persist.cuh", "gemm_tc.cuh", "batch.cuh", "paged.cuh", "paged_decode.cuh", "paged_prompt.cuh", "internal.cuh", "tma.cuh", "common.cuh", "json.hpp"]
 CALLS = os.path.join(PKG, "_torch_calls.so")
 CALLS_SOURCE = "torch_calls.cpp"
+CALLS_KEY = os.path.join(PKG, "_build", "torch_calls.key")  # what the module on disk was built from
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -42,7 +45,6 @@ def _stale() -> bool:
 
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not _stale():
-        build_calls()
         return LIB
     obj_dir = os.path.join(PKG, "_build")
     os.makedirs(obj_dir, exist_ok=True)
@@ -72,32 +74,51 @@ def build(force: bool = False, verbose: bool = False) -> str:
         sys.stderr.write(res.stdout + res.stderr)
         raise RuntimeError("nvcc failed linking libqdecode.so")
     os.replace(LIB + ".tmp", LIB)
-    build_calls(force)
     return LIB
 
 
+def _calls_key(torch) -> str:
+    """The torch and Python that a module built now belongs to, and its sources."""
+    h = hashlib.sha256()
+    for path in (os.path.join(CSRC, CALLS_SOURCE), os.path.join(ROOT, "include", "qdecode.h")):
+        with open(path, "rb") as f:
+            h.update(f.read())
+    return f"torch {torch.__version__} {sys.implementation.cache_tag} {h.hexdigest()}"
+
+
 def build_calls(force: bool = False) -> str:
-    """_torch_calls.so against the installed torch (nothing where there is none)."""
-    torch = importlib.util.find_spec("torch")  # found, not imported
-    if torch is None:
+    """_torch_calls.so against the installed torch and libqdecode.so ("" where there is no torch)."""
+    if importlib.util.find_spec("torch") is None:
         return ""
-    src, header = os.path.join(CSRC, CALLS_SOURCE), os.path.join(ROOT, "include", "qdecode.h")
-    if not force and os.path.exists(CALLS) and all(os.path.getmtime(p) <= os.path.getmtime(CALLS) for p in (src, header)):
-        return CALLS
-    home = torch.submodule_search_locations[0]
+    import torch
+    key = _calls_key(torch)
+    if not force and os.path.exists(CALLS) and os.path.exists(CALLS_KEY):
+        with open(CALLS_KEY) as f:
+            if f.read() == key:
+                return CALLS
+    home = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(nvcc()))
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", src, "-o", CALLS + ".tmp",
+    mine = f".{os.getpid()}.tmp"  # processes may build at once
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", os.path.join(CSRC, CALLS_SOURCE), "-o", CALLS + mine,
            "-I", os.path.join(home, "include"), "-I", os.path.join(home, "include", "torch", "csrc", "api", "include"),
            "-I", sysconfig.get_paths()["include"], "-I", os.path.join(cuda, "include"), "-L", os.path.join(home, "lib"),
            "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda", "-L", PKG, "-lqdecode", "-Wl,-rpath,$ORIGIN"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
+    try:
+        res = subprocess.run(cmd, capture_output=True, text=True)
+    except OSError as err:
+        raise RuntimeError(f"no g++ to build _torch_calls.so with: {err}") from err
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
         raise RuntimeError("g++ failed building _torch_calls.so")
-    os.replace(CALLS + ".tmp", CALLS)
+    os.replace(CALLS + mine, CALLS)
+    os.makedirs(os.path.dirname(CALLS_KEY), exist_ok=True)
+    with open(CALLS_KEY + mine, "w") as f:
+        f.write(key)
+    os.replace(CALLS_KEY + mine, CALLS_KEY)
     return CALLS
 
 
 if __name__ == "__main__":
     build(force="--force" in sys.argv, verbose="-v" in sys.argv)
+    build_calls(force="--force" in sys.argv)
     print(LIB)

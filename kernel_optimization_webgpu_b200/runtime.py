@@ -600,7 +600,9 @@ def _calls():
     global _calls_module
     if _calls_module is None:
         import torch  # noqa: F401  (the module uses torch's libraries)
+        from . import build
         _lib.load()
+        build.build_calls()
         from . import _torch_calls
         _calls_module = _torch_calls
     return _calls_module
