@@ -509,7 +509,8 @@ struct RowsCta {
     return b;
   }
   // For each goal: the bin at which the running count (by_count) or weight first reaches it, and the
-  // tokens and weight before it, in sh->at. (A goal lies within the whole sum.)
+  // tokens and weight before it, in sh->at. (A goal lies between 1 and the whole sum, as an integer:
+  // a sum beyond 2^53 that became a double may have grown.)
   __device__ void find_bins(const Bins& b, const u64* goal, int n_goals, bool by_count) {
     __syncthreads();
 #pragma unroll
@@ -835,10 +836,11 @@ __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_co
   const double d_lo_goal = uu * (cut_p ? p_goal * (1.0 - slack) : about),
                d_hi_goal = uu * (cut_p ? p_goal * (1.0 + slack) + kRowsOne : about);
   u64 goals[4];
-  goals[0] = few ? (u64)top_k : (u64)fmin(fmax(p_goal * (1.0 + slack), 1.0), about);
-  goals[1] = (u64)fmin(fmax(p_goal * (1.0 - slack), 1.0), about);
-  goals[2] = (u64)fmin(fmax(d_hi_goal * (1.0 + slack) + 1.0, 1.0), about);
-  goals[3] = (u64)fmin(fmax(d_lo_goal * (1.0 - slack), 1.0), about);
+  auto within = [&](double goal) { return min((u64)fmax(goal, 1.0), sh.whole); };
+  goals[0] = few ? (u64)top_k : within(p_goal * (1.0 + slack));
+  goals[1] = within(p_goal * (1.0 - slack));
+  goals[2] = within(d_hi_goal * (1.0 + slack) + 1.0);
+  goals[3] = within(d_lo_goal * (1.0 - slack));
   if (kind == RowsCta::kPlaces || few) x.find_bins(bins, goals, few ? 1 : 4, few);
   // the last bin that can hold a kept token, and the tokens up to it
   int last = kRowsBins - 1, upto = a.vocab;

@@ -205,3 +205,22 @@ def test_draws_follow_the_softmax():
     ids, _ = R.sample_rows(x, u.float(), temperature=torch.full((n,), 0.8, device="cuda"))
     share = torch.bincount(ids.long(), minlength=5).double() / n
     assert float((share - torch.softmax(x[0].double() / 0.8, 0)).abs().max()) <= 1.0 / n   # one stratum a border
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("u", [0.5, 0.99995, 1.0 - 2.0 ** -24])
+@pytest.mark.parametrize("tail", ["uniform", "deep"])
+def test_borders_at_the_end_of_heavy_rows(tail, u):
+    """Rows whose weights add up to thousands of times the largest one, with the border or the draw among
+    the last of them: the sum, about 2^56 units, is no exact double, and rounds up in every other row."""
+    torch = _cuda()
+    rng = np.random.default_rng(3)
+    rows, vocab = 16, 151936
+    if tail == "uniform":
+        x = rng.uniform(-25.0, 0.0, (rows, vocab))
+    else:
+        x = rng.standard_normal((rows, vocab))
+        x[:, rng.permutation(vocab)[:1000]] -= 20.0
+    x = torch.from_numpy(x.astype(np.float32)).cuda()
+    p = [[1.0, 0.9999, 0.99999, 1.0 - 2.0 ** -24][r % 4] for r in range(rows)]
+    check(torch, x, [1.0] * rows, [0] * rows, p, [0.0] * rows, [u] * rows)
