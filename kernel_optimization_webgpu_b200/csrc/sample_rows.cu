@@ -799,12 +799,17 @@ __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_co
   x.z_scale = x.inv_t * (128.0 * 1.4426950408889634);
   // 32 T: 2^44 exp(-32) < 1/2, so that what lies beyond weighs nothing
   x.range = fminf(32.0f * temperature, mx - mn);
-  x.scale = x.range > 0.0f ? fminf((float)(RowsCta::kNoPlace - 8) / x.range, 3.0e38f) : 0.0f;
+  x.scale = x.range > 0.0f ? (float)(RowsCta::kNoPlace - 8) / x.range : 0.0f;
+  // A temperature (or a row) below 1e-33 wants more places per unit than f32 has: places then still ascend,
+  // but lie close together and reach beyond the range, and tell nothing about weights. Such a row takes the
+  // exact passes.
+  const bool coarse = x.scale > 3.0e38f;
+  if (coarse) x.scale = 3.0e38f;
   x.step = x.scale > 0.0f ? (float)(x.z_scale * (4096.0 / 128.0) / (double)x.scale) : 0.0f;
 
   // weights matter unless a top-k cut (or a min-p cut without a top-p one) leaves a short list
   const bool cut_p = top_p < 1.0f, cut_m = min_p > 0.0f;
-  const RowsCta::HistKind kind = few || (cut_m && !cut_p) ? RowsCta::kCounts : RowsCta::kPlaces;
+  const RowsCta::HistKind kind = few || coarse || (cut_m && !cut_p) ? RowsCta::kCounts : RowsCta::kPlaces;
   x.histogram(RowsCmd{}, kind);
   x.cl.sync();
   if (x.rank != 0) {
@@ -844,7 +849,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_co
   if (kind == RowsCta::kPlaces || few) x.find_bins(bins, goals, few ? 1 : 4, few);
   // the last bin that can hold a kept token, and the tokens up to it
   int last = kRowsBins - 1, upto = a.vocab;
-  if (few || cut_p) {
+  if (few || (cut_p && !coarse)) {
     last = sh.at[0].bin;
     upto = sh.at[0].before + sh.at[0].count;
   }
@@ -869,7 +874,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) k_sample_rows(const __grid_co
   };
   u64* cum = reinterpret_cast<u64*>(x.hist);
   bool settled = false;
-  if (upto <= kRowsList) {
+  if (upto <= kRowsList && (few || !cut_p || !coarse)) {
     x.command(RowsCmd{kOpGather, 1, 0, (uint32_t)last, 0, 0, 0, cut_p && !few, 1, 0});
     int m = x.collect();
     const bool known = few || !cut_p;  // `last` is certain, not estimated: the other CTAs are done

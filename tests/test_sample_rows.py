@@ -224,3 +224,19 @@ def test_borders_at_the_end_of_heavy_rows(tail, u):
     x = torch.from_numpy(x.astype(np.float32)).cuda()
     p = [[1.0, 0.9999, 0.99999, 1.0 - 2.0 ** -24][r % 4] for r in range(rows)]
     check(torch, x, [1.0] * rows, [0] * rows, p, [0.0] * rows, [u] * rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [3e-33, 1e-36, 1e-40])
+@pytest.mark.parametrize("vocab", [700, 5000, 151936])
+def test_rows_and_temperatures_near_the_smallest_numbers(vocab, scale):
+    """Differences and temperatures below 1e-33, subnormal ones among them: the weights are ordinary."""
+    torch = _cuda()
+    rng = np.random.default_rng(vocab)
+    rows = 24 if vocab < 100000 else 8
+    x = rng.standard_normal((rows, vocab)) * 3.0
+    x -= np.where(rng.random(x.shape) < 0.5, rng.uniform(40.0, 4000.0, x.shape), 0.0)  # half of them weigh nothing
+    x = torch.from_numpy((x * scale).astype(np.float32)).cuda()
+    pick = lambda *a: [a[int(i)] for i in rng.integers(0, len(a), rows)]  # noqa: E731
+    check(torch, x, [(1.0, 0.3)[r % 2] * scale for r in range(rows)], pick(0, 0, 0, 40, 2000), pick(1.0, 0.9, 0.5),
+          pick(0.0, 0.0, 0.05), rng.random(rows).tolist())
