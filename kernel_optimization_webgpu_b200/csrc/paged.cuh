@@ -39,20 +39,28 @@ __device__ __forceinline__ int paged_page(const PagedArgs& a, int b, int p) {
 }
 
 // Sequence of row r: the b with q_starts[b] <= r < q_starts[b + 1], or -1 (padding rows).
-// Every lane of a warp calls it with the same r; 32 entries are compared per round trip.
-__device__ __forceinline__ int paged_find_seq(const int* q_starts, int batch, int r) {
+// Every lane of a warp calls it with the same r; 32 entries are compared per round trip. The first
+// trip tells whether the row is padding; if it is not, load() is called then, and what it
+// reads comes under the rest of the search (up to 32 sequences have none).
+template <typename F>
+__device__ __forceinline__ int paged_find_seq(const int* q_starts, int batch, int r, F&& load) {
   const int lane = threadIdx.x & 31;
   int lo = 0, hi = batch;  // entries [lo, hi] bracket the answer: q_starts[lo] <= r
-  if (r < q_starts[0] || r >= q_starts[batch]) return -1;
-  while (hi - lo > 1) {
+  bool first = true;
+  do {
     const int step = (hi - lo + 31) >> 5;
-    const int i = min(lo + (lane + 1) * step, hi);
-    const unsigned le = __ballot_sync(0xffffffffu, q_starts[i] <= r);
+    const int e = q_starts[min(lo + (lane + 1) * step, hi)];
+    const unsigned le = __ballot_sync(0xffffffffu, e <= r);
+    if (first) {
+      if (r < q_starts[0] || le >> 31) return -1;  // (the last lane holds entry hi)
+      load();
+      first = false;
+    }
     const int n = __popc(le);  // ascending entries: the lanes at or below r are a prefix
     const int nlo = lo + n * step;
     hi = min(nlo + step, hi);
     lo = min(nlo, hi - 1);
-  }
+  } while (hi - lo > 1);
   return lo;
 }
 
@@ -113,8 +121,9 @@ struct AppendArgs {
 
 // One warp per row and HEADS consecutive heads of its [q | k | v]; lane l holds dims 4l .. 4l+3, so
 // the rotation's partner dims are 16 lanes away. What it has to move bounds it (per row and head 512
-// bytes of f32 in, 512 or 256 out), so the heads' loads go out first, and the row's sequence,
-// position and page are looked up under them; the heads' sums of squares then run side by side.
+// bytes of f32 in, 512 or 256 out), so the heads' loads go out as soon as the row is known not to be
+// padding, and its sequence, position and page are looked up under them; the heads' sums of squares
+// then run side by side.
 // HEADS: 4 keep 2 KB in flight per warp at 40 warps an SM (16384 rows of 16 + 8 + 8 heads, f32, 470 MB:
 // 82 us = 5.7 TB/s, 88 with 8); with few rows 2 spread the work over more warps (1 row: 2.5 us, 3.2
 // with 4).
@@ -128,14 +137,18 @@ __global__ void __launch_bounds__(256, HEADS == 4 ? 5 : 6) k_paged_append(const 
   if (r >= a.rows) return;
   pdl_wait();
   float4 x[HEADS];
+  auto load = [&] {
 #pragma unroll
-  for (int i = 0; i < HEADS; ++i)
-    x[i] = load4<T>(a.qkv, r * a.qkv_stride + (long long)min(h0 + i, heads - 1) * kHeadDim + 4 * lane);
+    for (int i = 0; i < HEADS; ++i)
+      x[i] = load4<T>(a.qkv, r * a.qkv_stride + (long long)min(h0 + i, heads - 1) * kHeadDim + 4 * lane);
+  };
   int b = r, back = 1;
   if (a.q_starts) {
-    b = paged_find_seq(a.q_starts, a.kv.batch, r);
+    b = paged_find_seq(a.q_starts, a.kv.batch, r, load);
     if (b < 0) return;
     back = a.q_starts[b + 1] - r;
+  } else {
+    load();
   }
   const int p = a.kv.seq_lens[b] - back;
   const long long t = (long long)p * a.rope_stride + 4 * (lane & 15);

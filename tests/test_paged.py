@@ -524,6 +524,34 @@ def test_append(io, cache, out, new, totals, heads):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("batch", [1, 2, 31, 32, 33, 64, 65, 1023, 1024, 1025, 4096])
+def test_append_finds_the_rows_of_any_number_of_sequences(batch):
+    """Ragged chunks, empty ones among them, behind which the buffer ends: padding rows are not read."""
+    torch = _cuda()
+    rng = random.Random(batch)
+    new = [rng.choice([0, 0, 1, 2, 3]) for _ in range(batch)]
+    new[batch // 2] = 2
+    rows, pad = sum(new), 37
+    k, v, table, n = make_cache(torch, [m + rng.randrange(9) for m in new], 16, 1, "f16")
+    starts = torch.tensor([sum(new[:b]) for b in range(batch + 1)], dtype=torch.int32, device="cuda")
+    qkv = torch.randn(rows, 4 * D, device="cuda")              # the last rows + pad .. rows of it do not exist
+    out = torch.full((rows + pad, 2 * D), 9.0, device="cuda")
+    kv = _kv(k=k.data_ptr(), v=v.data_ptr(), num_pages=k.shape[0], kv_heads=1, batch=batch,
+             block_table=table.data_ptr(), table_width=table.shape[1], table_stride=table.shape[1],
+             seq_lens=n.data_ptr())
+    rc = _lib.load().qd_paged_append(kv, qkv.data_ptr(), _lib.QD_KV_F32, 4 * D, rows + pad, starts.data_ptr(), 2, None,
+                                     None, 1e-6, None, None, 0, 0, out.data_ptr(), _lib.QD_KV_F32, 2 * D,
+                                     torch.cuda.current_stream().cuda_stream)
+    assert rc == _lib.QD_OK
+    assert torch.equal(out[:rows], qkv[:, :2 * D]) and bool((out[rows:] == 9.0).all())
+    seq = torch.repeat_interleave(torch.arange(batch), torch.tensor(new)).cuda()
+    pos = torch.cat([torch.arange(int(t) - m, int(t)) for m, t in zip(new, n.tolist())]).cuda()
+    pg = table[seq].long().gather(1, (pos // 16)[:, None])[:, 0]
+    assert torch.equal(k[pg, 0, pos % 16], qkv[:, 2 * D:3 * D].half())
+    assert torch.equal(v[pg, 0, pos % 16], qkv[:, 3 * D:].half())
+
+
+@pytest.mark.gpu
 def test_append_in_place_without_norm_or_rotation_and_wider_table_rows():
     torch = _cuda()
     from kernel_optimization_webgpu_b200 import runtime as R
