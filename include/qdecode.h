@@ -389,7 +389,8 @@ int qd_gqa_decode_noalloc(const float* q, const void* k_cache, const void* v_cac
  * A table entry outside [0, num_pages) where a position is visible, a length beyond
  * table_width * page_size and a new token at a negative position (or, in the append, beyond
  * the rotation tables) can only be seen on the device: the position is left out (not
- * written, not attended to; the length is cut) and the bit is set in *status. */
+ * written, not attended to; the length is cut) and the bit is set in *status. (To the two
+ * attention calls a sequence of length 0 is padding: its rows get zeros and no bit is set.) */
 #define QD_PAGED_BAD_PAGE 1     /* status bits (or-ed; never cleared by the library) */
 #define QD_PAGED_BAD_LENGTH 2
 #define QD_PAGED_TIMEOUT 4      /* a device-side wait of qd_paged_attn_prompt expired: its results are void */

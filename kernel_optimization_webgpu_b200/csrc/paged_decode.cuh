@@ -216,8 +216,8 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
   }
   if (blockIdx.x == 0) {
     for (int b = tid; b <= B; b += kPdThreads) ws.first[b] = first[b];
-    for (int b = tid; b < B; b += kPdThreads)
-      if (a.kv.seq_lens[b] > paged_len(a.kv, b) && a.kv.seq_lens[b] > 0) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
+    for (int b = tid; b < B; b += kPdThreads)  // (paged_len cuts both)
+      if (a.kv.seq_lens[b] != paged_len(a.kv, b)) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
   }
   for (int b = blockIdx.x; b < B; b += gridDim.x)  // nothing visible: zeros
     if (first[b + 1] == first[b])

@@ -362,7 +362,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
     if (!pp_item(a, G, kRows, w.item, seq, tile, start, fresh, asked)) return false;
     w.it = pp_rows(a, G, kRows, tile, start, fresh, asked);
     w.it.seq = seq;
-    if (asked > w.it.len && asked > 0 && lane == 0) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
+    // beyond the table, or new tokens before position 0 (a length of 0 is a padded sequence)
+    if ((asked > w.it.len || (asked != 0 && asked < fresh)) && lane == 0) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
     w.parts = pp_parts(w.it.v.tiles, pa.splits);
     if (w.z >= w.parts) return false;
     w.t0 = w.it.v.tiles * w.z / w.parts;  // (at most 2^23 tiles, 32 parts)

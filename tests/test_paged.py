@@ -320,6 +320,31 @@ def test_bad_pages_and_lengths_are_left_out_and_flagged():
     assert bool((y[0] == 0).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("length,bits", [(0, 0), (-1, _lib.QD_PAGED_BAD_LENGTH), (-2 ** 31, _lib.QD_PAGED_BAD_LENGTH),
+                                         (2, _lib.QD_PAGED_BAD_LENGTH), (3, 0), (40, 0), (48, 0),
+                                         (49, _lib.QD_PAGED_BAD_LENGTH), (2 ** 31 - 1, _lib.QD_PAGED_BAD_LENGTH)])
+def test_lengths_that_have_no_place_are_flagged(length, bits):
+    """Three new tokens of a sequence in a table of 48 positions: the rows at positions below 0 give zeros."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    k, v, table, n = make_cache(torch, [48, 48], 16, 2, "f16")
+    q = torch.randn(5, 4, D, device="cuda")
+    starts = torch.tensor([0, 3, 5], dtype=torch.int32, device="cuda")
+    n.copy_(torch.tensor([length, 48], dtype=torch.int32))
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    y = R.paged_attn_prompt(q, k, v, table, n, starts, status=status)
+    assert int(status) == bits
+    before = min(3, max(0, 3 - length))
+    assert bool((y[:before] == 0).all()) and bool((y[before:3] != 0).any(-1).all())
+    other = R.paged_attn_prompt(q[3:], k, v, table[1:], n[1:], torch.tensor([0, 2], dtype=torch.int32, device="cuda"))
+    assert torch.equal(y[3:], other)
+    status.zero_()
+    y = R.paged_attn_decode(q[:2], k, v, table, n, status=status)
+    assert int(status) == (bits if length != 2 else 0)
+    assert bool((y[0] == 0).all()) == (length <= 0)
+
+
 # ---- attention of prompt chunks ------------------------------------------------------------
 
 CHUNKS = [([8], [8]), ([1], [1]), ([130], [130]), ([1, 0, 70, 5], [900, 40, 70, 6]), ([300, 17], [513, 1100]),
