@@ -434,8 +434,9 @@ int qd_paged_append(const qd_paged_kv* kv, const void* qkv, int qkv_dtype, int64
  * (of both) QD_KV_F32 or the cache's. q_heads is a multiple of kv_heads, at most 64 times it. The softmax and its sums
  * are f32; with dtype QD_KV_F32 the products keep f32 accuracy too (q and the weights go into
  * them as sums of two f16 or three bf16), with a 16-bit dtype the prompt's weights are rounded to
- * it once. scale 0 means 1/sqrt(128). The workspace holds
- * the joined parts' partial sums; nothing in it needs to start at zero. */
+ * it once. q and scale may have any size; what counts is the scores': beyond 2^22, where f32 cannot tell
+ * neighbouring weights apart any more, a row may come out as NaN. scale 0 means 1/sqrt(128). The workspace
+ * holds the joined parts' partial sums; nothing in it needs to start at zero. */
 size_t qd_paged_attn_decode_workspace_bytes(int batch, int q_heads);
 int qd_paged_attn_decode(const qd_paged_kv* kv, const void* q, int dtype, int64_t q_stride, int q_heads, int window,
                          int sinks, float scale, void* y, int64_t y_stride, void* workspace, void* stream);

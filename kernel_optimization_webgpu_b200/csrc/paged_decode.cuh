@@ -20,6 +20,8 @@
 //    precision at no extra instruction. (tcgen05 wants 64 rows or more; 56 of them would idle.)
 //    Two bf16 hold only 16 of f32's 24 bits (results were 5e-6 off): with f32 queries on a bf16
 //    cache a second set of products takes the rest of both operands (THREE).
+//    Two f16 hold 22 bits of what lies well inside f16's range: each head's q is brought there by a
+//    power of two, which its scores' factor takes back (f16_fit).
 //
 // 64 sequences of 2048 positions, 8 KV heads: 93 us for 537 MB = 5.8 TB/s; of 8192: 334 us = 6.4 TB/s.
 // About 10 us of either are the two launches and the chain of lookups before the first row (lengths,
@@ -137,6 +139,12 @@ __device__ __forceinline__ float2 split2_rest(float x, float y, unsigned& hi) {
                        ? __half22float2(*reinterpret_cast<const __half2*>(&hi))
                        : make_float2(__uint_as_float(hi << 16), __uint_as_float(hi & 0xffff0000u));
   return make_float2(x - f.x, y - f.y);
+}
+// The power of two that brings values whose largest has the (biased) exponent e into f16's upper range (the
+// largest to 2^13 .. 2^14), so that the second of two f16 parts keeps its bits, and its inverse.
+__device__ __forceinline__ float2 f16_fit(int e) {
+  e = min(max(e, 14), 254);  // (an infinity stays one, zeros stay zeros)
+  return make_float2(__int_as_float((267 - e) << 23), __int_as_float((e - 13) << 23));
 }
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -339,6 +347,7 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
   fetch_q(cur);
   unsigned q[8][4], q3[THREE ? 8 : 1][2];
   float o[16][4], m = -INFINITY, l = 0.0f;
+  float factor = qs;   // of q's products
   bool fresh = true;   // a new (sequence, head): take its q, clear the sums
   int seg = 0;         // segments finished by this CTA
   bool from_start = cur.t == 0;
@@ -347,16 +356,27 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
     issue();
     if (fresh) {
       fresh = false;
+      if constexpr (std::is_same<T, __half>::value) {
+        float top = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < 16; ++kk) top = fmaxf(top, fmaxf(fabsf(qn[kk].x), fabsf(qn[kk].y)));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float2 fit = f16_fit(__float_as_int(top) >> 23);
+#pragma unroll
+        for (int kk = 0; kk < 16; ++kk) qn[kk] = make_float2(qn[kk].x * fit.x, qn[kk].y * fit.x);
+        factor = qs * fit.y;
+      }
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) {
         if constexpr (THREE) {
-          const float2 x = split2_rest<T>(qn[2 * kk].x * qs, qn[2 * kk].y * qs, q[kk][0]);
-          const float2 y = split2_rest<T>(qn[2 * kk + 1].x * qs, qn[2 * kk + 1].y * qs, q[kk][2]);
+          const float2 x = split2_rest<T>(qn[2 * kk].x, qn[2 * kk].y, q[kk][0]);
+          const float2 y = split2_rest<T>(qn[2 * kk + 1].x, qn[2 * kk + 1].y, q[kk][2]);
           split2<T>(x.x, x.y, q[kk][1], q3[kk][0]);
           split2<T>(y.x, y.y, q[kk][3], q3[kk][1]);
         } else {
-          split2<T>(qn[2 * kk].x * qs, qn[2 * kk].y * qs, q[kk][0], q[kk][1]);
-          split2<T>(qn[2 * kk + 1].x * qs, qn[2 * kk + 1].y * qs, q[kk][2], q[kk][3]);
+          split2<T>(qn[2 * kk].x, qn[2 * kk].y, q[kk][0], q[kk][1]);
+          split2<T>(qn[2 * kk + 1].x, qn[2 * kk + 1].y, q[kk][2], q[kk][3]);
         }
       }
 #pragma unroll
@@ -396,7 +416,7 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) p[j][e] = (s[j][e] + s[2 + j][e]) + (s[j][2 + e] + s[2 + j][2 + e]);
+        for (int e = 0; e < 2; ++e) p[j][e] = ((s[j][e] + s[2 + j][e]) + (s[j][2 + e] + s[2 + j][2 + e])) * factor;
       if (!(p0 + 16 <= cur.v.end && (p0 >= cur.v.lo || p0 + 16 <= cur.v.ns))) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)

@@ -21,8 +21,9 @@
 // it, so the result is exact to rounding. P is rounded to the cache's 16-bit type (half a step
 // relative, as the tensor cores take 16-bit operands); its sum is taken in f32 before that.
 // With f32 queries q and P are each a sum of PARTS 16-bit operands, and every product is issued that
-// many times: two f16 keep 22 bits, two bf16 only 16 (the results were 5e-6 off), so a bf16 cache
-// takes three. Three parts of P do not fit over S in TMEM, so such a CTA has one row tile. The
+// many times: two f16 keep 22 bits (of a row of q that a power of two has brought to the upper end of f16's
+// range; the factor of the row's scores takes it back), two bf16 only 16 (the results were 5e-6 off),
+// so a bf16 cache takes three. Three parts of P do not fit over S in TMEM, so such a CTA has one row tile. The
 // tensor cores drop the bits below an accumulator's last place, towards zero, at every step, which
 // over a long row shows in f32: every kPpFlush tiles O moves from TMEM to sums in the workspace that
 // are added with rounding (500 rows behind 3500 keys: 1.4e-6 off, 2.5e-6 without; it costs a causal
@@ -684,19 +685,48 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       unsigned char* wq = qs + t * kQTile + hf * (kPpTileBytes / 2);
       const long long q_at =
           live ? (long long)(it.tok0 + tok) * a.q_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf : -1;
+      float c = fabsf(a.scale) * kLog2e;  // of the row's scores
       if constexpr (PARTS > 1) {
         const int c4 = lane & 15;
+        constexpr int N = PARTS == 2 ? 16 : 8;
 #pragma unroll
-        for (int i0 = 0; i0 < 16; i0 += 8) {
-          float4 x[8];
+        for (int i0 = 0; i0 < 16; i0 += N) {
+          float4 x[N];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+          for (int i = 0; i < N; ++i) {
             const long long at = __shfl_sync(0xffffffffu, q_at, 2 * (i0 + i) + (lane >> 4));
             x[i] = at >= 0 ? load4<float>(a.q, at + 4 * c4) : make_float4(0.f, 0.f, 0.f, 0.f);
             if (a.scale < 0.0f) x[i] = make_float4(-x[i].x, -x[i].y, -x[i].z, -x[i].w);
           }
+          if constexpr (PARTS == 2) {
+            // Each row by its own power of two to where two f16 hold 22 bits of it (f16_fit). The largest of
+            // a row's 64 dims, for the i-th pair of rows in lane i of each half; the partner warp has the others:
+            // the two exponents go to the halves of the row's word.
+            float top[16];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 16; ++i)
+              top[i] = fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+              for (int i = 0; i < o; ++i) {
+                const float theirs = lane & o ? top[i] : top[i + o], ours = lane & o ? top[i + o] : top[i];
+                top[i] = fmaxf(ours, __shfl_xor_sync(0xffffffffu, theirs, o));
+              }
+            const unsigned* tops = reinterpret_cast<const unsigned*>(shared_row) + t * 128;
+            reinterpret_cast<unsigned short*>(shared_row)[2 * (t * 128 + wr + 2 * c4 + (lane >> 4)) + hf] =
+                (unsigned short)(__float_as_int(top[0]) >> 23);
+            pp_meet(pair);
+            auto fit = [&](int r) { return f16_fit((int)max(tops[r] & 0xffffu, tops[r] >> 16)); };
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float up = fit(wr + 2 * i + (lane >> 4)).x;
+              x[i] = make_float4(x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up);
+            }
+            c = fmaxf(c * fit(wr + lane).y, 1.0e-37f);  // (never 0: a hidden key's score is -inf)
+          }
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
             const int r = wr + 2 * (i0 + i) + (lane >> 4);
             unsigned u[2][PARTS];
             split_parts<T, PARTS>(x[i].x, x[i].y, u[0]);
@@ -729,7 +759,6 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
       const unsigned ts = tmem + t * 128 + lanes, tp = tmem + kColP + t * 128 + 32 * hf + lanes;
       const unsigned to = tmem + kColO + t * 128 + 64 * hf + lanes;
-      const float c = fabsf(a.scale) * kLog2e;
       const int p = live ? it.pos0 + tok : -1;
       const int pmax = min(p, it.len - 1);
       const int phi = a.window > 0 ? p - a.window : -2;  // keys up to here are hidden, unless sinks

@@ -497,6 +497,55 @@ def test_a_causal_future_of_large_values_does_not_reach_the_past():
     assert torch.equal(before[:140], after[:140]) and bool(torch.isfinite(after).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e-20, 1e-4, 1.0, 1e5, 1e20])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+def test_f32_queries_of_any_size(size, sign, cache):
+    """The scores are ordinary, whatever share of them q and the scale hold: f32 queries keep their accuracy far
+    outside f16's range, rows of every size in one call, a few large elements in a row among them."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    new, totals = [300, 3], [330, 200]
+    k, v, table, n = make_cache(torch, totals, 32, 2, cache)
+    q = torch.randn(303, 8, D, device="cuda") * 1.5
+    q[::3] *= 0.01
+    q[1::5, :, 7] *= 300.0
+    q *= size
+    scale = sign * D ** -0.5 / size
+    y = R.paged_attn_prompt(q, k, v, table, n, torch.tensor([0, 300, 303], dtype=torch.int32, device="cuda"), scale=scale)
+    want, tol = plain_attention(torch, q, k, v, table, n, new, 0, 0, scale, "f32", cache)
+    close(torch, y, want, tol)
+    y = R.paged_attn_decode(q[:2], k, v, table, n, scale=scale)
+    want, tol = plain_attention(torch, q[:2], k, v, table, n, [1, 1], 0, 0, scale, "f32", cache)
+    close(torch, y, want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("io", ["f16", "f32"])
+def test_zero_and_large_queries_and_large_scales(io):
+    """Zeros weigh all keys alike; f16 queries times a large scale leave f16's range, not f32's."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    k, v, table, n = make_cache(torch, [90, 70], 16, 2, "f16")
+    q = (torch.randn(2, 4, D, device="cuda") * 1.5e4).clamp(-6e4, 6e4).to(_types(torch)[io])
+    q[0] = 0.0
+    starts = torch.arange(3, dtype=torch.int32, device="cuda")
+    for y in (R.paged_attn_decode(q, k, v, table, n, scale=20.0), R.paged_attn_prompt(q, k, v, table, n, starts, scale=20.0)):
+        want, tol = plain_attention(torch, q[:1], k, v, table[:1], n[:1], [1], 0, 0, 20.0, io, "f16")
+        close(torch, y[:1], want, tol)
+        # scores of 1e7 and more, thousands apart: one key has all the weight
+        j = torch.arange(70, device="cuda")
+        kk, vv = (x[table[1].long()[j // 16], :, j % 16].double().repeat_interleave(2, 1) for x in (k, v))
+        best = torch.einsum("hd,jhd->hj", q[1].double(), kk).argmax(-1)
+        want = vv[best, torch.arange(4, device="cuda")]
+        # The scores, in units of 1e7 log2 e, leave the maximum's f32 rounding (half of 2) in the exponent, so the one
+        # weight is no power of two: with 16-bit queries it is rounded to f16 once (half a step, 2^-11) where
+        # its sum is not; then the sum, a division and y's own rounding.
+        weight = 2.0 ** -11 if io == "f16" else 2.0 ** -21
+        close(torch, y[1], want, (weight + HALF_STEP[io] + 2.0 ** -22) * want.abs())
+
+
 # ---- norm + rotation + append ----------------------------------------------------------------
 
 @pytest.mark.gpu
