@@ -417,7 +417,7 @@ typedef struct qd_paged_kv {
  *   x[i], x[i+64] <- x[i] c - x[i+64] s, x[i+64] c + x[i] s,   i < 64,
  * c = cos[position * rope_stride + i], s = sin[...] (f32 tables of rope_len entries each;
  * both NULL: no rotation). q goes to q_out [rows][q_heads*128] (rows q_out_stride elements
- * apart; q_out may be qkv itself, with its type and stride), k and v to the cache. All
+ * apart; q_out may be qkv itself, with its type and stride, and is else apart from it), k and v to the cache. All
  * arithmetic in f32, rounded once to the output's type. qkv_dtype, q_out_dtype: QD_KV_F16,
  * QD_KV_F32 or QD_KV_BF16; pointers 16-byte aligned, strides multiples of 8. Two rows of one
  * call never share a position of the cache unless the block table does (then either wins).
@@ -430,7 +430,8 @@ int qd_paged_append(const qd_paged_kv* kv, const void* qkv, int qkv_dtype, int64
 
 /* Attention of one new token per sequence (rows = batch): y[b] = softmax(scale * q[b] k^T) v
  * over the keys that position seq_lens[b] - 1 sees. q, y [batch][q_heads][128], rows q_stride /
- * y_stride elements apart (multiples of 8), 16-byte aligned, y apart from all that is read; dtype
+ * y_stride elements apart (multiples of 8), 16-byte aligned, y apart from all that is read (y over q or the
+ * pools is refused; of a ragged batch, where that shows in the first row); dtype
  * (of both) QD_KV_F32 or the cache's. q_heads is a multiple of kv_heads, at most 64 times it. The softmax and its sums
  * are f32; with dtype QD_KV_F32 the products keep f32 accuracy too (q and the weights go into
  * them as sums of two f16 or three bf16), with a 16-bit dtype the prompt's weights are rounded to

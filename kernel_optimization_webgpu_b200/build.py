@@ -21,7 +21,7 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libqdecode.so")
 SOURCES = ["engine.cu", "batch.cu", "noalloc.cu", "bench_api.cu", "sample.cu", "paged.cu", "sample_rows.cu"]
-DEPS = SOURCES + ["kernels.cuh", "persist.cuh", "gemm_tc.cuh", "batch.cuh", "paged.cuh", "paged_decode.cuh", "paged_prompt.cuh", "internal.cuh", "tma.cuh", "common.cuh", "json.hpp"]
+DEPS = SOURCES + ["kernels.cuh", "persist.cuh", "gemm_tc.cuh", "batch.cuh", "paged.cuh", "paged_decode.cuh", "paged_prompt.cuh", "internal.cuh", "overlap.hpp", "tma.cuh", "common.cuh", "json.hpp"]
 CALLS = os.path.join(PKG, "_torch_calls.so")
 CALLS_SOURCE = "torch_calls.cpp"
 CALLS_KEY = os.path.join(PKG, "_build", "torch_calls.key")  # what the module on disk was built from
@@ -80,7 +80,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
 def _calls_key(torch) -> str:
     """The torch and Python that a module built now belongs to, and its sources."""
     h = hashlib.sha256()
-    for path in (os.path.join(CSRC, CALLS_SOURCE), os.path.join(ROOT, "include", "qdecode.h")):
+    for path in (os.path.join(CSRC, CALLS_SOURCE), os.path.join(CSRC, "overlap.hpp"), os.path.join(ROOT, "include", "qdecode.h")):
         with open(path, "rb") as f:
             h.update(f.read())
     return f"torch {torch.__version__} {sys.implementation.cache_tag} {h.hexdigest()}"

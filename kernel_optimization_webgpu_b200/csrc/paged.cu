@@ -5,6 +5,7 @@
 
 #include "../../include/qdecode.h"
 #include "internal.cuh"
+#include "overlap.hpp"
 #include "paged.cuh"
 #include "paged_decode.cuh"
 #include "paged_prompt.cuh"
@@ -16,6 +17,16 @@ static bool known_dtype(int d) { return d == QD_KV_F16 || d == QD_KV_F32 || d ==
 
 static void need(bool ok, const char* msg) {
   if (!ok) throw QdError{QD_E_INVALID, msg};
+}
+
+// (Rows of a ragged batch may be padding that no memory stands behind: the host is sure of the first alone.)
+static Rows rows_of(const void* p, int dtype, int64_t rows, int64_t elements, int64_t stride) {
+  const int64_t size = dtype == QD_KV_F32 ? 4 : 2;
+  return {p, rows, elements * size, stride * size};
+}
+static void need_apart_from_pools(const qd_paged_kv* kv, const Rows& x, const char* msg) {
+  const int64_t bytes = (int64_t)kv->num_pages * kv->kv_heads * kv->page_size * kHeadDim * 2;
+  need(apart(x, Rows{kv->k, 1, bytes, bytes}) && apart(x, Rows{kv->v, 1, bytes, bytes}), msg);
 }
 
 static PagedArgs check_paged(const qd_paged_kv* kv) {
@@ -48,7 +59,7 @@ static PagedArgs check_paged(const qd_paged_kv* kv) {
 }
 
 static PAttnArgs check_attn(const qd_paged_kv* kv, const void* q, int dtype, int64_t q_stride, int rows, int q_heads,
-                            int window, int sinks, float scale, void* y, int64_t y_stride) {
+                            int window, int sinks, float scale, void* y, int64_t y_stride, int sure) {
   PAttnArgs a{};
   a.kv = check_paged(kv);
   need(rows >= 0, "paged attention: negative rows");
@@ -62,6 +73,10 @@ static PAttnArgs check_attn(const qd_paged_kv* kv, const void* q, int dtype, int
   need(q_stride >= (int64_t)q_heads * kHeadDim && y_stride >= (int64_t)q_heads * kHeadDim && q_stride % 8 == 0 &&
            y_stride % 8 == 0,
        "paged attention: row strides must be multiples of 8, at least q_heads * 128");
+  // (several CTAs read a row of q, and one of them may be done first)
+  const Rows out = rows_of(y, dtype, sure, (int64_t)q_heads * kHeadDim, y_stride);
+  need(apart(out, rows_of(q, dtype, sure, (int64_t)q_heads * kHeadDim, q_stride)), "paged attention: y overlaps q");
+  need_apart_from_pools(kv, out, "paged attention: y overlaps the pools");
   a.q = q;
   a.q_stride = q_stride;
   a.rows = rows;
@@ -194,6 +209,14 @@ int qd_paged_append(const qd_paged_kv* kv, const void* qkv, int qkv_dtype, int64
     need(aligned16(qkv) && aligned16(q_out) && aligned16(cos) && aligned16(sin) && aligned16(q_norm) &&
              aligned16(k_norm),
          "qd_paged_append: pointers must be 16-byte aligned");
+    const int sure = q_starts ? std::min(rows, 1) : rows;
+    const Rows in = rows_of(qkv, qkv_dtype, sure, heads * kHeadDim, qkv_stride);
+    const Rows out = rows_of(q_out, q_out_dtype, sure, (int64_t)q_heads * kHeadDim, q_out_stride);
+    const bool in_place = q_out == qkv && q_out_dtype == qkv_dtype && (q_out_stride == qkv_stride || rows == 1);
+    need(in_place || apart(out, in),
+         "qd_paged_append: q_out overlaps qkv (it may be qkv itself, with its type and stride)");
+    need_apart_from_pools(kv, out, "qd_paged_append: q_out overlaps the pools");
+    need_apart_from_pools(kv, in, "qd_paged_append: qkv overlaps the pools");
     if (rows == 0 || kv->batch == 0) return;
     a.kv_dtype = kv->dtype;
     a.qkv = qkv;
@@ -226,7 +249,7 @@ int qd_paged_attn_decode(const qd_paged_kv* kv, const void* q, int dtype, int64_
                          int sinks, float scale, void* y, int64_t y_stride, void* workspace, void* stream) {
   return guarded([&] {
     need(kv != nullptr, "paged cache: NULL pointer");
-    PAttnArgs a = check_attn(kv, q, dtype, q_stride, kv->batch, q_heads, window, sinks, scale, y, y_stride);
+    PAttnArgs a = check_attn(kv, q, dtype, q_stride, kv->batch, q_heads, window, sinks, scale, y, y_stride, kv->batch);
     if (a.rows == 0) return;
     need(workspace != nullptr, "qd_paged_attn_decode: NULL workspace");
     need(aligned16(workspace), "qd_paged_attn_decode: the workspace must be 16-byte aligned");
@@ -252,7 +275,8 @@ int qd_paged_attn_prompt(const qd_paged_kv* kv, const void* q, int dtype, int64_
                          const int32_t* q_starts, int q_heads, int window, int sinks, float scale, void* y,
                          int64_t y_stride, void* workspace, void* stream) {
   return guarded([&] {
-    PAttnArgs a = check_attn(kv, q, dtype, q_stride, rows, q_heads, window, sinks, scale, y, y_stride);
+    PAttnArgs a =
+        check_attn(kv, q, dtype, q_stride, rows, q_heads, window, sinks, scale, y, y_stride, std::min(rows, 1));
     if (rows == 0 || kv->batch == 0) return;
     need(q_starts != nullptr, "qd_paged_attn_prompt: NULL q_starts");
     need(workspace != nullptr, "qd_paged_attn_prompt: NULL workspace");

@@ -15,6 +15,7 @@
 #include <string>
 
 #include "../../include/qdecode.h"
+#include "overlap.hpp"
 
 namespace py = pybind11;
 using at::Tensor;
@@ -65,6 +66,12 @@ int64_t row_stride(const Tensor& x, int64_t width, const char* what) {
   if (!ok || inner != width)
     throw std::invalid_argument(std::string(what) + " must have contiguous rows of " + std::to_string(width) + " elements");
   return x.size(0) > 1 ? x.stride(0) : width;
+}
+
+// The rows of a [rows, ...] tensor, `stride` elements apart (padding rows of a tensor are memory too).
+qd::Rows rows_of(const Tensor& x, int64_t width, int64_t stride) {
+  const int64_t size = x.element_size();
+  return {x.const_data_ptr(), x.size(0), width * size, stride * size};
 }
 
 int to_int(int64_t v, const char* what) {
@@ -139,13 +146,20 @@ Tensor paged_append(const Tensor& qkv, const Tensor& k, const Tensor& v, const T
   need(!q_out || (q_out->device() == dev && q_out->dim() >= 1 && q_out->size(0) == rows),
        "q_out must have a row for every row of qkv, on its device");
   const Tensor q = q_out ? *q_out : fresh({rows, q_heads * 128}, qkv.scalar_type(), dev);
+  const int64_t q_stride = row_stride(q, q_heads * 128, "q_out");
+  if (q_out) {
+    const bool in_place = q.const_data_ptr() == qkv.const_data_ptr() && q.scalar_type() == qkv.scalar_type() &&
+                          (q_stride == stride || rows == 1);
+    need(in_place || qd::apart(rows_of(q, q_heads * 128, q_stride), rows_of(qkv, (q_heads + 2 * kv.kv_heads) * 128, stride)),
+         "q_out overlaps qkv (it may be the first q_heads * 128 elements of its rows)");
+  }
   done(qd_paged_append(&kv, qkv.const_data_ptr(), code(qkv, "qkv"), stride, to_int(rows, "too many rows"),
                        vec<int32_t>(q_starts, (int64_t)kv.batch + 1, at::kInt, dev, "q_starts"), (int)q_heads,
                        vec<float>(q_norm, 128, at::kFloat, dev, "q_norm"),
                        vec<float>(k_norm, 128, at::kFloat, dev, "k_norm"), (float)eps,
                        cos ? static_cast<const float*>(cos->const_data_ptr()) : nullptr,
                        sin ? static_cast<const float*>(sin->const_data_ptr()) : nullptr, rope_len, step, q.data_ptr(),
-                       code(q, "q_out"), row_stride(q, q_heads * 128, "q_out"), here.stream));
+                       code(q, "q_out"), q_stride, here.stream));
   return q;
 }
 
@@ -167,6 +181,7 @@ struct Attn {
     if (!y) return fresh(q.sizes(), q.scalar_type(), q.device());
     need(y->scalar_type() == q.scalar_type() && y->sizes() == q.sizes() && y->device() == q.device(),
          "y must have q's type, shape and device");
+    need(qd::apart(rows_of(*y, width, row_stride(*y, width, "y")), rows_of(q, width, q_stride)), "y overlaps q");
     return *y;
   }
 };

@@ -110,6 +110,85 @@ def test_python_wrappers_refuse_before_they_enqueue():
         R.paged_append(torch.zeros(2, 700), k, k, table, lens, None, None, 2)
 
 
+BASE = 1 << 40   # (addresses that nothing is read from)
+
+
+def _refuses(call, *args):
+    """Whether a call over sequences without a row to work on is refused, and with which words."""
+    rc = call(*args)
+    assert rc in (_lib.QD_OK, _lib.QD_E_INVALID)
+    return _lib.load().qd_last_error(None).decode() if rc else ""
+
+
+@pytest.mark.parametrize("dy,stride,y_stride,batch,over", [
+    (0, 256, 256, 2, "q"), (512, 256, 256, 2, "q"), (1024, 256, 256, 2, ""), (-512, 256, 256, 2, "q"),
+    (-1024, 256, 256, 2, ""), (512, 512, 512, 2, ""), (496, 512, 512, 2, "q"), (528, 512, 512, 2, "q"),
+    (512, 520, 520, 2, ""), (1552, 520, 520, 2, ""), (512, 512, 256, 2, "q"), (512, 512, 256, 1, ""),
+    (0, 512, 256, 1, "q"), (BASE, 256, 256, 2, "the pools"), (BASE - 16, 256, 256, 2, "the pools"),
+    (BASE + 32768 - 16, 256, 256, 2, "the pools"), (BASE + 32768, 256, 256, 2, ""), (2 * BASE, 256, 256, 2, "the pools")])
+def test_attention_outputs_over_their_inputs_are_refused(dy, stride, y_stride, batch, over):
+    """q at BASE, 512-byte rows; pools of 32768 bytes at 2 and 3 BASE. A NULL workspace ends what is not refused."""
+    L = _lib.load()
+    kv = _kv(k=2 * BASE, v=3 * BASE, batch=batch, block_table=64, seq_lens=64)
+    args = (kv, BASE, _lib.QD_KV_F16, stride, 2, 0, 0, 0.0, BASE + dy, y_stride, None, None)
+    assert _refuses(L.qd_paged_attn_decode, *args) == (
+        f"paged attention: y overlaps {over}" if over else "qd_paged_attn_decode: NULL workspace")
+    # of a ragged batch the rows behind the first may be padding without memory
+    if -512 < dy < 512 or over != "q":
+        args = (kv, BASE, _lib.QD_KV_F16, stride, batch, 64, 2, 0, 0, 0.0, BASE + dy, y_stride, None, None)
+        assert _refuses(L.qd_paged_attn_prompt, *args) == (
+            f"paged attention: y overlaps {over}" if over else "qd_paged_attn_prompt: NULL workspace")
+
+
+@pytest.mark.parametrize("out,dtype,stride,over", [
+    (BASE, 1, 768, ""), (BASE, 1, 776, "q_out overlaps qkv"), (BASE, 0, 768, "q_out overlaps qkv"),
+    (BASE + 256, 1, 768, "q_out overlaps qkv"), (BASE + 768 * 4, 1, 768, "q_out overlaps qkv"),
+    (BASE + 2 * 768 * 4, 1, 768, ""), (2 * BASE, 1, 768, "q_out overlaps the pools"),
+    (3 * BASE + 32000, 0, 768, "q_out overlaps the pools")])
+def test_append_outputs_over_their_inputs_are_refused(out, dtype, stride, over):
+    """qkv at BASE, two rows of 768 f32. A cache that nothing is written to: eps ends what is not refused."""
+    kv = _kv(k=2 * BASE, v=3 * BASE, block_table=64, seq_lens=64)
+    L = _lib.load()
+
+    def call(eps):
+        return _refuses(L.qd_paged_append, kv, BASE, _lib.QD_KV_F32, 768, 2, None, 2, None, None, eps, None, None, 0, 0, out,
+                        dtype, stride, None)
+
+    assert "eps" in call(-1.0)
+    if over:
+        assert over in call(1e-6)
+    else:   # the same layout over a cache of no sequences is no error
+        kv.batch = 0
+        assert _refuses(L.qd_paged_append, kv, BASE, _lib.QD_KV_F32, 768, 2, 64, 2, None, None, 1e-6, None, None, 0, 0, out,
+                        dtype, stride, None) == ""
+
+
+@pytest.mark.gpu
+def test_outputs_beside_their_inputs_in_one_buffer():
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    k, v, table, n = make_cache(torch, [50, 3], 16, 2, "f16")
+    both = torch.randn(2, 2, 4, D, device="cuda")
+    q, y = both[:, 0], both[:, 1]
+    want = R.paged_attn_decode(q.clone(), k, v, table, n)
+    assert torch.equal(R.paged_attn_decode(q, k, v, table, n, y=y), want) and torch.equal(y, want)
+    starts = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    three = torch.randn(3, 4, D, device="cuda")
+    with pytest.raises(ValueError, match="overlaps"):
+        R.paged_attn_decode(q, k, v, table, n, y=q)
+    with pytest.raises(ValueError, match="overlaps"):
+        R.paged_attn_prompt(three[:2], k, v, table, n, starts, y=three[1:])
+    pool = k.view(torch.float32).reshape(-1)[:2 * 4 * D].view(2, 4, D)
+    with pytest.raises(_lib.QdError, match="pools"):
+        R.paged_attn_prompt(q, k, v, table, n, starts, y=pool)
+    qkv = torch.randn(1, 8 * D, device="cuda")      # one row: its stride says nothing
+    x = qkv.clone()
+    R.paged_append(qkv, k, v, table[:1], n[:1], None, None, 4, q_out=qkv[:, :4 * D])
+    assert torch.equal(qkv, x)
+    with pytest.raises(ValueError, match="overlaps"):
+        R.paged_append(qkv, k, v, table[:1], n[:1], None, None, 4, q_out=qkv[:, D:5 * D])
+
+
 # ---- the plain 64-bit forms -------------------------------------------------------------
 
 def _cuda():
