@@ -140,7 +140,12 @@ Tensor paged_append(const Tensor& qkv, const Tensor& k, const Tensor& v, const T
          "cos and sin must be contiguous float32 tables on the device of the other tensors");
   if (cos && sin) {
     rope_len = std::min(cos->numel(), sin->numel());
-    if (!rope_stride) step = cos->dim() > 1 ? cos->stride(0) : 64;
+    if (!rope_stride) {  // their own: 64 in a vector, else a row of both
+      need(cos->sizes() == sin->sizes() &&
+               (cos->dim() < 2 || (cos->size(-1) >= 64 && cos->numel() == cos->size(0) * cos->size(-1))),
+           "cos and sin must be [positions][64 or more], of one shape, where no rope_stride is given");
+      step = cos->dim() > 1 ? cos->size(-1) : 64;
+    }
   }
   const Here here(dev);
   need(!q_out || (q_out->device() == dev && q_out->dim() >= 1 && q_out->size(0) == rows),

@@ -622,8 +622,8 @@ def paged_append(qkv, k_pages, v_pages, block_table, seq_lens, cos, sin, q_heads
     """Head RMSNorm + rotation of the new tokens' q and k, and their K/V rows into the pages
     (qd_paged_append). qkv [rows][(q_heads + 2 kv_heads) * 128]; cache pools
     [pages][kv_heads][page_size][128]; cos, sin f32 tables whose row for a position is
-    rope_stride elements after the previous one's (default: their own row stride; None, None:
-    no rotation); returns q [rows][q_heads * 128] (q_out, or a new tensor of qkv's type)."""
+    rope_stride elements after the previous one's (default: their own rows, [positions][64 or more]
+    and alike; None, None: no rotation); returns q [rows][q_heads * 128] (q_out, or a new tensor of qkv's type)."""
     if stream is not None:
         with _on(stream, qkv):
             return paged_append(qkv, k_pages, v_pages, block_table, seq_lens, cos, sin, q_heads, q_norm, k_norm, eps,

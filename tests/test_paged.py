@@ -741,6 +741,27 @@ def test_append_flags_what_has_no_place():
     assert int(status) == _lib.QD_PAGED_BAD_PAGE and torch.equal(k, k0)
 
 
+@pytest.mark.gpu
+def test_rotation_tables_that_are_not_rows_by_position_are_refused():
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    k, v, table, n = make_cache(torch, [5, 9], 16, 1, "f16")
+    x = torch.randn(2, 4 * D, device="cuda")
+    rows = torch.rand(20, 64, device="cuda")
+    wide = torch.cat([rows, rows], 1).contiguous()
+    want = R.paged_append(x, k, v, table, n, rows, rows, 2)
+    for cos, sin in ((wide, wide), (rows.reshape(-1), rows.reshape(-1)), (rows[:, None], rows[:, None])):
+        assert torch.equal(R.paged_append(x, k, v, table, n, cos, sin, 2), want)
+    one = torch.as_strided(wide, (1, 64), (128, 1))       # one row: its stride says nothing
+    got = R.paged_append(x[:1], k, v, table[:1], torch.ones_like(n[:1]), one, one, 2)
+    assert torch.equal(got, R.paged_append(x[:1], k, v, table[:1], torch.ones_like(n[:1]), rows, rows, 2))
+    half = rows[:, :32].contiguous()
+    for cos, sin in ((wide, rows), (rows, wide), (half, half), (rows[None], rows[None]), (rows, rows[:10])):
+        with pytest.raises(ValueError, match="positions"):
+            R.paged_append(x, k, v, table, n, cos, sin, 2)
+    assert torch.equal(R.paged_append(x, k, v, table, n, rows, rows[:10], 2, rope_stride=64), want)
+
+
 # ---- the step as it is used -------------------------------------------------------------------
 
 @pytest.mark.gpu
