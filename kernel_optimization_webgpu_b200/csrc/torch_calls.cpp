@@ -74,6 +74,12 @@ qd::Rows rows_of(const Tensor& x, int64_t width, int64_t stride) {
   return {x.const_data_ptr(), x.size(0), width * size, stride * size};
 }
 
+// As the C ABI takes it, where 0 stands for the default: a scale that f32 cannot hold must not become that.
+float to_scale(double v) {
+  need(v == 0.0 || (float)v != 0.0f, "scale is below what float32 holds");
+  return (float)v;
+}
+
 int to_int(int64_t v, const char* what) {
   need(v >= INT32_MIN && v <= INT32_MAX, what);
   return (int)v;
@@ -200,7 +206,7 @@ Tensor paged_attn_decode(const Tensor& q, const Tensor& k, const Tensor& v, cons
   const Tensor y = a.out(q, y_out);
   const Tensor ws = workspace(ws_in, qd_paged_attn_decode_workspace_bytes(a.kv.batch, a.heads), q.device());
   done(qd_paged_attn_decode(&a.kv, q.const_data_ptr(), a.dtype, a.q_stride, a.heads, to_int(window, "bad window"),
-                            to_int(sinks, "bad sinks"), (float)scale, y.data_ptr(), row_stride(y, a.width, "y"),
+                            to_int(sinks, "bad sinks"), to_scale(scale), y.data_ptr(), row_stride(y, a.width, "y"),
                             ws.data_ptr(), here.stream));
   return y;
 }
@@ -217,7 +223,7 @@ Tensor paged_attn_prompt(const Tensor& q, const Tensor& k, const Tensor& v, cons
                 q.device());
   done(qd_paged_attn_prompt(&a.kv, q.const_data_ptr(), a.dtype, a.q_stride, rows,
                             vec<int32_t>(q_starts, (int64_t)a.kv.batch + 1, at::kInt, q.device(), "q_starts"), a.heads,
-                            to_int(window, "bad window"), to_int(sinks, "bad sinks"), (float)scale, y.data_ptr(),
+                            to_int(window, "bad window"), to_int(sinks, "bad sinks"), to_scale(scale), y.data_ptr(),
                             row_stride(y, a.width, "y"), ws.data_ptr(), here.stream));
   return y;
 }

@@ -762,6 +762,21 @@ def test_rotation_tables_that_are_not_rows_by_position_are_refused():
     assert torch.equal(R.paged_append(x, k, v, table, n, rows, rows[:10], 2, rope_stride=64), want)
 
 
+@pytest.mark.gpu
+def test_a_scale_below_float32_is_not_the_default():
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    k, v, table, n = make_cache(torch, [5, 9], 16, 1, "f16")
+    q = torch.randn(2, 2, D, device="cuda")
+    starts = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    for call in (lambda s: R.paged_attn_decode(q, k, v, table, n, scale=s),
+                 lambda s: R.paged_attn_prompt(q, k, v, table, n, starts, scale=s)):
+        with pytest.raises(ValueError, match="scale"):
+            call(1e-60)
+        mean = v[table[0, 0].long(), 0, :5].double().mean(0)      # every key alike
+        close(torch, call(1e-40)[0], mean.expand(2, D), 2.0 ** -20 * v[table[0, 0].long(), 0, :5].double().abs().mean(0))
+
+
 # ---- the step as it is used -------------------------------------------------------------------
 
 @pytest.mark.gpu
