@@ -277,7 +277,7 @@ int qd_run_full_decoder_stack_benchmark(qd_engine* e, qd_stack_bench* out);
  * The reference's only failure detection is the A/B page's uncapturederror guard
  * (src/bench/ab-page.js:158-161,181-187), which refuses results after a device error.
  * Here every device-side wait is bounded and a wait that runs out makes the call
- * return QD_E_TIMEOUT with the engine still usable. These two calls let a test make
+ * return QD_E_TIMEOUT with the engine still usable. These calls let a test make
  * one such wait run out on purpose, without any fault:
  *  - qd_engine_inject_stall: the next persistent decode launch withholds layer 0's
  *    q/k/v results, so its attention CTAs wait until their 200 ms deadline, raise the
@@ -290,6 +290,10 @@ int qd_run_full_decoder_stack_benchmark(qd_engine* e, qd_stack_bench* out);
  *    QD_E_TIMEOUT. Both only enqueue (on the engine's stream). */
 int qd_engine_inject_stall(qd_engine* e);
 int qd_batch_inject_stall(qd_batch* b);
+/*  - qd_paged_inject_stall: the calling thread's next qd_paged_attn_prompt withholds the first key
+ *    tile of its block 0, whose waits end after 1 s: QD_PAGED_TIMEOUT is set, the rows that the block
+ *    held are NaN and all others are right. (In a captured call, at every replay.) */
+void qd_paged_inject_stall(void);
 
 /* runCustomQwenGreedyPrompt over `batch` prompts of n_prompt ids each: prefill,
  * then max_new_tokens greedy tokens per prompt. ids [batch][n_prompt], out_ids
@@ -393,7 +397,7 @@ int qd_gqa_decode_noalloc(const float* q, const void* k_cache, const void* v_cac
  * attention calls a sequence of length 0 is padding: its rows get zeros and no bit is set.) */
 #define QD_PAGED_BAD_PAGE 1     /* status bits (or-ed; never cleared by the library) */
 #define QD_PAGED_BAD_LENGTH 2
-#define QD_PAGED_TIMEOUT 4      /* a device-side wait of qd_paged_attn_prompt expired: its results are void */
+#define QD_PAGED_TIMEOUT 4      /* a device-side wait of qd_paged_attn_prompt expired: rows of y are NaN */
 
 typedef struct qd_paged_kv {
   void* k;                      /* [num_pages][kv_heads][page_size][head_dim] of dtype, 16-byte aligned */

@@ -44,6 +44,7 @@ EXPORTS = (
     "qd_generate_sample", "qd_sample_workspace_bytes", "qd_sample_logits",
     "qd_paged_append", "qd_paged_attn_decode_workspace_bytes", "qd_paged_attn_decode",
     "qd_paged_attn_prompt_workspace_bytes", "qd_paged_attn_prompt", "qd_sample_rows",
+    "qd_paged_inject_stall",
 )
 
 
@@ -222,6 +223,8 @@ def load(build_if_stale: bool = True):
     L.qd_paged_attn_prompt_workspace_bytes.restype = C.c_size_t
     L.qd_paged_attn_prompt.argtypes = [kv, vp, i32, i64, i32, vp, i32, i32, i32, f32, vp, i64, vp, vp]
     L.qd_paged_attn_prompt.restype = i32
+    L.qd_paged_inject_stall.argtypes = []
+    L.qd_paged_inject_stall.restype = None
     L.qd_sample_rows.argtypes = [vp, i32, i32, u32, i64, vp, vp, vp, vp, vp, vp, vp, vp]
     L.qd_sample_rows.restype = i32
     L.qd_run_kernel_benchmarks.argtypes = [vp, C.POINTER(QdKernelBench)]

@@ -125,6 +125,8 @@ static int prompt_splits(int items, int kv_heads) {
   return n == 0 ? 1 : (int)std::max(1LL, std::min<long long>(kPpMaxSplits, current_sms() / n));
 }
 
+static thread_local bool stall_next = false;  // qd_paged_inject_stall
+
 template <typename T, int PARTS>
 static void launch_prompt(const PAttnArgs& a, const void* q_any, void* workspace, cudaStream_t s) {
   constexpr int kRows = 128 * pp_tiles<PARTS>();
@@ -132,6 +134,8 @@ static void launch_prompt(const PAttnArgs& a, const void* q_any, void* workspace
   PPromptArgs p{};
   p.a = a;
   p.cta_rows = kRows;
+  p.stall = stall_next;
+  stall_next = false;
   p.splits = prompt_splits(items, a.kv.kv_heads);
   p.po = static_cast<float4*>(workspace);
   p.pml = reinterpret_cast<float2*>(p.po + (size_t)items * a.kv.kv_heads * p.splits * kRows * (kHeadDim / 4));
@@ -292,5 +296,7 @@ int qd_paged_attn_prompt(const qd_paged_kv* kv, const void* q, int dtype, int64_
     }
   });
 }
+
+void qd_paged_inject_stall(void) { stall_next = true; }
 
 }  // extern "C"

@@ -67,6 +67,7 @@ struct PPromptArgs {
   PAttnArgs a;
   int splits;
   int cta_rows;  // 128 times the row tiles of a CTA
+  int stall;     // test hook (qd_paged_inject_stall): block 0 withholds its first key tile
   // Unnormalised sums (f32 results, or parts > 1): [item][KV head][split][32 groups of 4 dims][cta_rows], so
   // that a warp's rows lie side by side; and their maxima and weights: [item][KV head][split][cta_rows].
   float4* po;
@@ -338,7 +339,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
   __shared__ unsigned long long full[S], empty[S], s_full[2], p_half[2], p_full[2], o_done[2], q_full[2], drain;
   __shared__ unsigned long long work_full[2], work_empty[2], ask, answered;
   __shared__ __align__(16) uint4 answer;
-  __shared__ PpWork work[2];
+  __shared__ PpWork work[3];  // two in turn; one that was taken and could not be handed on
   __shared__ unsigned bad_rows[8];  // of key tile j: bit i set where 16-key chunk i has no usable page
   __shared__ unsigned tmem_base;
   __shared__ float shared_row[256];  // between a row's two threads: a maximum (NaN: given up), then a sum
@@ -412,10 +413,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
     tc_mbar_init(&answered);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     failed = 0;
-    if (CLAIM) {
-      work[0] = first;
-      pp_arrive(&work_full[0]);
-    }
+    work[0] = first;
+    work[1].halves = work[2].halves = 0;
+    if (CLAIM) pp_arrive(&work_full[0]);
   }
   tc_fence_before();
   __syncthreads();
@@ -457,9 +457,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       }
       tiles = w.nk;
       ok = free_slot();
-      if (ok && lane == 0) {
-        work[next & 1] = w;
-        pp_arrive(&work_full[next & 1]);
+      if (lane == 0) {
+        work[ok ? next & 1 : 2] = w;
+        if (ok) pp_arrive(&work_full[next & 1]);
       }
       ++next;
     }
@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
     // ---- copies: K and V tiles alternate through the ring ----
     const int ps = 1 << a.kv.page_shift, box = min(ps, kPpKeys), boxes = kPpKeys / box;
     int issued_to = -1, done = 0;  // ring slots of the works before
-    bool ok = true;
+    bool ok = !(pa.stall && blockIdx.x == 0);
     for (int n = 0, nk = 0; ok && (CLAIM || n == 0); ++n) {
       ok = wait_work(n, nk);
       if (!ok || work_of(n).halves == 0) break;
@@ -657,6 +657,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       (void)tc_mbar_wait(&drain, 0);
     }
   }
+  tc_fence_before();
+  __syncthreads();
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPpRegsMany));
     // ---- softmax: half a row per thread ----
@@ -962,10 +964,31 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
     }
     work_done(n);
     }
+    tc_fence_before();
+    __syncthreads();  // (the other roles' is at their end)
+    if (failed) {
+      // What this block held becomes NaN, so that nobody takes it for an answer. (Here, where the softmax threads'
+      // registers are, and after the barrier, behind which no work is handed on any more.)
+      if (tid == 0) paged_flag(a.kv, QD_PAGED_TIMEOUT);
+      const float gone = __int_as_float(0x7fffffff);
+#pragma unroll 1
+      for (int i = 0; i < 3; ++i) {
+        const PpWork& w = work[i];
+        if (w.halves == 0) continue;
+        const int n_rows = min(kRows, w.it.n_rows - w.row0);
+#pragma unroll 1
+        for (int e = tid; e < 32 * n_rows; e += kPpSoftmax) {
+          const int lr = e >> 5, row = w.row0 + lr, tok = w.it.tok0 + row / G;
+          if ((unsigned)tok >= (unsigned)a.rows) continue;
+          if (w.parts > 1)
+            pa.pml[(((long long)w.item * kvh + w.g) * pa.splits + w.z) * kRows + lr] = make_float2(gone, gone);
+          else
+            store4(a.y, (long long)tok * a.y_stride + ((long long)w.g * G + row % G) * kHeadDim + 4 * lane, a.dtype,
+                   make_float4(gone, gone, gone, gone));
+        }
+      }
+    }
   }
-  tc_fence_before();
-  __syncthreads();
-  if (tid == 0 && failed) paged_flag(a.kv, QD_PAGED_TIMEOUT);
   if (warp == kPpSoftmax / 32) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 

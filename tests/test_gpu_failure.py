@@ -72,3 +72,35 @@ def test_gemm_wait_runs_out_and_the_batch_recovers(tiny_runtime):
         # and a prefill afterwards is unaffected as well
         first = bt.prefill(rng.integers(0, eng.profile["vocab"], size=(3, 20)).astype(np.int32))
         assert first.shape == (3,)
+
+
+@pytest.mark.parametrize("io,cache", [("float16", "float16"), ("float32", "float16"), ("float32", "bfloat16")])
+@pytest.mark.parametrize("shape", ["one block a tile", "split keys", "blocks that take each other's work"])
+def test_a_prompts_wait_runs_out_and_its_rows_say_so(shape, io, cache):
+    """With and without a status word: rows of the block that gave up are NaN, the others as ever."""
+    T = getattr(torch, cache)
+    new, total = {"one block a tile": (300, 300), "split keys": (40, 3000),
+                  "blocks that take each other's work": (3000, 3000)}[shape]
+    batch, kvh, H, page = (1, 4, 8, 32) if new < 3000 else (2, 8, 16, 32)
+    per = -(-total // page)
+    k, v = (torch.randn(batch * per, kvh, page, 128, device="cuda").to(T) for _ in "kv")
+    table = torch.randperm(batch * per, device="cuda").to(torch.int32).view(batch, per)
+    lens = torch.full((batch,), total, dtype=torch.int32, device="cuda")
+    starts = torch.arange(batch + 1, dtype=torch.int32, device="cuda") * new
+    q = torch.randn(batch * new, H, 128, device="cuda").to(getattr(torch, io))
+    want = R.paged_attn_prompt(q, k, v, table, lens, starts)
+    assert bool(torch.isfinite(want).all())
+    for status in (None, torch.zeros(1, dtype=torch.int32, device="cuda")):
+        _lib.load().qd_paged_inject_stall()
+        t0 = time.monotonic()
+        y = R.paged_attn_prompt(q, k, v, table, lens, starts, status=status)
+        torch.cuda.synchronize()
+        assert time.monotonic() - t0 < 20.0
+        gone = torch.isnan(y).any(-1)
+        assert torch.equal(gone, torch.isnan(y).all(-1))
+        # block 0: the last rows of the last sequence, the query heads of the first KV head
+        rows = int(gone.any(1).sum())
+        assert 0 < rows <= 128 and bool(gone[-rows:, :H // kvh].all()) and int(gone.sum()) == rows * (H // kvh)
+        assert torch.equal(y[~gone], want[~gone])
+        assert status is None or int(status) == _lib.QD_PAGED_TIMEOUT
+    assert torch.equal(R.paged_attn_prompt(q, k, v, table, lens, starts), want)
