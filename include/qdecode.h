@@ -449,8 +449,9 @@ int qd_paged_attn_decode(const qd_paged_kv* kv, const void* q, int dtype, int64_
 /* The same for a ragged batch of new tokens (q_starts as above, not NULL): each row attends
  * to the keys its own position sees, the call's own new tokens among them (append them
  * first). q, y [rows][q_heads][128]. Weights of hidden keys are zeros, not left out: a V row that
- * is not finite also reaches rows of its sequence in this call that do not see it, within 128
- * positions, as it would in a plain product. The workspace's size depends on dtype (of q and
+ * is not finite also reaches rows of its sequence in this call that do not see it, as it would in a
+ * plain product, if they are less than 256 positions from a row that does (fewer with several
+ * query heads to a KV head: the 256 rows that are worked on together are tokens times these heads). The workspace's size depends on dtype (of q and
  * y): with QD_KV_F32 it holds running sums of every row. */
 size_t qd_paged_attn_prompt_workspace_bytes(int batch, int rows, int q_heads, int kv_heads, int dtype);
 int qd_paged_attn_prompt(const qd_paged_kv* kv, const void* q, int dtype, int64_t q_stride, int rows,

@@ -625,6 +625,33 @@ def test_zero_and_large_queries_and_large_scales(io):
         close(torch, y[1], want, (weight + HALF_STEP[io] + 2.0 ** -22) * want.abs())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [(2, 2), (3, 1), (16, 2)], ids=lambda h: f"{h[0]}q{h[1]}kv")
+@pytest.mark.parametrize("io,cache", [("f16", "f16"), ("f32", "f16"), ("f32", "bf16")])
+def test_how_far_a_v_row_that_is_not_finite_reaches(heads, io, cache):
+    """A NaN or an infinity in one visible V row: rows that see it, and no row 256 tokens * heads from those."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    new, at, window = 1400, 700, 40
+    k, v, table, n = make_cache(torch, [new], 16, heads[1], cache)
+    starts = torch.tensor([0, new], dtype=torch.int32, device="cuda")
+    q = torch.randn(new, heads[0], D, device="cuda").to(_types(torch)[io])
+    want = R.paged_attn_prompt(q, k, v, table, n, starts, window=window)
+    reach = -(-256 // (heads[0] // heads[1]))
+    p = torch.arange(new, device="cuda")
+    sees = (p >= at) & (p < at + window)
+    near = (p > at - reach) & (p < at + window + reach)
+    for bad in (math.nan, math.inf):
+        v2 = v.clone()
+        v2[table[0, at // 16].long(), 0, at % 16, 5] = bad
+        y = R.paged_attn_prompt(q, k, v2, table, n, starts, window=window)
+        gone = ~torch.isfinite(y)
+        assert bool(gone[sees, :heads[0] // heads[1], 5].all())
+        assert torch.equal(y[~near], want[~near]) and not bool(gone[:, heads[0] // heads[1]:].any())
+        gone[..., 5] = False
+        assert not bool(gone.any())
+
+
 # ---- norm + rotation + append ----------------------------------------------------------------
 
 @pytest.mark.gpu
