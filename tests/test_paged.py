@@ -15,6 +15,7 @@ Tolerances count roundings, relative to A = sum of |weight| |value| of an output
 import ctypes as C
 import math
 import random
+import threading
 
 import pytest
 
@@ -846,3 +847,23 @@ def test_prompt_then_decoding_steps_over_one_cache(cache, window):
     rank = int((w.cumsum(0) <= 0.9).sum())
     assert int(ids[2]) == int(logits[2].topk(50).indices[rank]) and abs(float(logp[2]) - math.log(float(w[rank]))) < 1e-5
     assert int(status) == 0
+
+
+@pytest.mark.gpu
+def test_a_thread_without_a_cuda_call_before_it():
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    k, v, table, n = make_cache(torch, [40, 7], 16, 2, "f16")
+    q = torch.randn(2, 4, D, device="cuda")
+    starts = torch.arange(3, dtype=torch.int32, device="cuda")
+    u = torch.rand(2, device="cuda")
+    calls = [lambda: R.paged_attn_prompt(q, k, v, table, n, starts), lambda: R.paged_attn_decode(q, k, v, table, n),
+             lambda: R.paged_append(q.view(1, 8 * D), k, v, table[:1], n[:1], None, None, 4),
+             lambda: R.sample_rows(q.view(2, -1), u)[0]]
+    for call in calls:
+        want, got = call(), []
+        thread = threading.Thread(target=lambda: got.append(call()))
+        thread.start()
+        thread.join()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want)
