@@ -57,15 +57,15 @@ inline void launch_ex(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t sm
 }
 
 // Raises a kernel's dynamic shared memory limit once per device (the attribute
-// belongs to the device's context).
+// belongs to the device's context). Calls come from any thread; two that set it at once do the same.
 template <typename... KArgs>
 inline void allow_smem(void (*kernel)(KArgs...), size_t bytes, unsigned long long& done_mask) {
   int dev = 0;
   QD_CK(cudaGetDevice(&dev));
   const unsigned long long bit = 1ull << (dev & 63);
-  if (done_mask & bit) return;
+  if (__atomic_load_n(&done_mask, __ATOMIC_ACQUIRE) & bit) return;
   QD_CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  done_mask |= bit;
+  __atomic_fetch_or(&done_mask, bit, __ATOMIC_RELEASE);
 }
 
 inline int sm_count(int dev) {

@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 
+#include <atomic>
 #include <cstdint>
 #include <string>
 
@@ -53,7 +54,8 @@ __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) {
 inline bool make_tmap_2d(CUtensorMap* out, const void* base, CUtensorMapDataType dtype, uint64_t inner,
                          uint64_t rows, uint64_t row_bytes, uint32_t box_inner, uint32_t box_rows,
                          CUtensorMapSwizzle swizzle, std::string* err) {
-  static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+  static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> known{nullptr};  // (calls come from any thread)
+  PFN_cuTensorMapEncodeTiled_v12000 encode = known.load();
   if (!encode) {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult q{};
@@ -63,6 +65,7 @@ inline bool make_tmap_2d(CUtensorMap* out, const void* base, CUtensorMapDataType
       return false;
     }
     encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    known.store(encode);
   }
   const cuuint64_t dims[2] = {inner, rows};
   const cuuint64_t strides[1] = {row_bytes};

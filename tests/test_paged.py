@@ -15,6 +15,9 @@ Tolerances count roundings, relative to A = sum of |weight| |value| of an output
 import ctypes as C
 import math
 import random
+import subprocess
+import sys
+import textwrap
 import threading
 
 import pytest
@@ -867,3 +870,53 @@ def test_a_thread_without_a_cuda_call_before_it():
         thread.join()
         torch.cuda.synchronize()
         assert torch.equal(got[0], want)
+
+
+@pytest.mark.gpu
+def test_calls_from_many_threads_at_once():
+    """Eight threads with streams, outputs and workspaces of their own, every entry among them; the C ABI, under
+    which Python's threads do run together, in a process that has made no call before."""
+    _cuda()
+    code = textwrap.dedent("""
+        import threading, torch
+        from kernel_optimization_webgpu_b200 import _lib, runtime as R
+        L = _lib.load()
+        torch.manual_seed(0)
+        lens = [700, 33, 64, 129]
+        per = -(-max(lens) // 32)
+        k, v = (torch.randn(4 * per, 2, 32, 128, device="cuda").half() for _ in "kv")
+        table = torch.randperm(4 * per, device="cuda").to(torch.int32).view(4, per)
+        n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        kv = _lib.QdPagedKv(k.data_ptr(), v.data_ptr(), 0, 4 * per, 32, 2, 128, 4, table.data_ptr(), per, per, n.data_ptr(), None)
+        starts = torch.tensor([0, 300, 310, 311, 400], dtype=torch.int32, device="cuda")
+        q = torch.randn(400, 8, 128, device="cuda")
+        logits, u = torch.randn(4, 5000, device="cuda"), torch.rand(4, device="cuda")
+        outs, codes, gate = [], [], threading.Barrier(8)
+        for i in range(8):
+            outs.append([torch.zeros(400, 8, 128, device="cuda"), torch.zeros(4, 8, 128, device="cuda"),
+                         torch.zeros(4, dtype=torch.int32, device="cuda"), torch.cuda.Stream(),
+                         torch.empty(L.qd_paged_attn_prompt_workspace_bytes(4, 400, 8, 2, 1), dtype=torch.uint8, device="cuda"),
+                         torch.empty(L.qd_paged_attn_decode_workspace_bytes(4, 8), dtype=torch.uint8, device="cuda")])
+        torch.cuda.synchronize()
+        def work(i):
+            yp, yd, ids, stream, wp, wd = outs[i]
+            s = stream.cuda_stream
+            gate.wait()
+            for _ in range(20):
+                codes.append(L.qd_paged_attn_prompt(kv, q.data_ptr(), 1, 1024, 400, starts.data_ptr(), 8, 0, 0, 0.0,
+                                                    yp.data_ptr(), 1024, wp.data_ptr(), s))
+                codes.append(L.qd_paged_attn_decode(kv, q.data_ptr(), 1, 1024, 8, 0, 0, 0.0, yd.data_ptr(), 1024,
+                                                    wd.data_ptr(), s))
+                codes.append(L.qd_sample_rows(logits.data_ptr(), 1, 4, 5000, 5000, None, None, None, None, u.data_ptr(),
+                                              ids.data_ptr(), None, s))
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(8)]
+        for t in threads: t.start()
+        for t in threads: t.join()
+        torch.cuda.synchronize()
+        want = (R.paged_attn_prompt(q, k, v, table, n, starts), R.paged_attn_decode(q[:4], k, v, table, n),
+                R.sample_rows(logits, u)[0])
+        assert codes == [0] * 480, codes
+        print(all(torch.equal(a, b) for o in outs for a, b in zip(o, want)))
+    """)
+    res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=_lib._build.ROOT)
+    assert res.returncode == 0 and res.stdout.split() == ["True"], res.stderr
