@@ -656,6 +656,100 @@ def test_how_far_a_v_row_that_is_not_finite_reaches(heads, io, cache):
         assert not bool(gone.any())
 
 
+# ---- the accuracy of f32 queries ---------------------------------------------------------------
+
+def two_keys(torch, n, cache):
+    """n pairs of keys, seen by one query each, whose scores are two elements of q: (q, keys, values, y in 64 bits). With
+    the scale ln 2 the factor of the scores is 1 in f32, so a kernel that keeps all of q has their exact difference."""
+    T = _types(torch)[cache]
+    g = torch.Generator().manual_seed(n)
+    a = 24 + 8 * torch.rand(n, 2, generator=g)
+    b = a + 0.7 * torch.randn(n, 2, generator=g)
+    q = torch.zeros(n, 2, D)
+    q[..., 0], q[..., 1] = a, b
+    k = torch.zeros(2, D)
+    k[0, 0] = k[1, 1] = 1.0
+    v = torch.ones(2, D)
+    v[1] = -1.0
+    return q, k.to(T), v.to(T), torch.tanh((a.double() - b.double()) * math.log(2) / 2)
+
+
+def f32_tolerance(cache):
+    """Of |w0 - w1| / (w0 + w1): the exponential (2^-22), at most 6 truncated additions of products (2^-23 each), as
+    many roundings in f32 of sums, joins and the division (2^-24). Two f16 hold 22 bits: half a step of 2^-22 of scores
+    up to 34 (in units of log2) and of the weights. Three bf16 hold all 24."""
+    return 2.0 ** -22 + 6 * 2.0 ** -23 + 6 * 2.0 ** -24 + (math.log(2) * 34 * 2.0 ** -23 + 2.0 ** -22 if cache == "f16" else 0)
+
+
+def parts(torch, x, n, T):
+    """x as a sum of n rounded parts."""
+    out = torch.zeros_like(x)
+    for _ in range(n):
+        out = out + (x - out).to(T).double()
+    return out
+
+
+def test_the_tolerance_of_f32_queries_tells_two_bf16_from_three():
+    torch = pytest.importorskip("torch")
+    q, _, _, want = two_keys(torch, 600, "bf16")
+    a, b = q[..., 0].double(), q[..., 1].double()
+    for q_parts, w_parts, passes in ((3, 3, True), (2, 3, False), (3, 2, False)):
+        x, y = parts(torch, a, q_parts, torch.bfloat16), parts(torch, b, q_parts, torch.bfloat16)
+        m = torch.maximum(x, y)
+        w0, w1 = torch.exp2(x - m + 7), torch.exp2(y - m + 7)
+        got = (parts(torch, w0, w_parts, torch.bfloat16) - parts(torch, w1, w_parts, torch.bfloat16)) / (w0 + w1)
+        assert (float((got - want).abs().max()) <= f32_tolerance("bf16")) == passes
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+def test_f32_queries_keep_their_bits(cache):
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    n = 600
+    q, keys, values, want = (x.cuda() for x in two_keys(torch, n, cache))
+    # decode: n sequences of two positions
+    k, v, table, lens = make_cache(torch, [2] * n, 16, 1, cache)
+    pg = table[:, 0].long()
+    k[pg, 0, :2], v[pg, 0, :2] = keys, values
+    y = R.paged_attn_decode(q, k, v, table, lens, scale=math.log(2))
+    close(torch, y, want[..., None].expand(n, 2, D), torch.full((1,), f32_tolerance(cache), device="cuda"))
+    # prompt: every row sees the sink and itself
+    k, v, table, lens = make_cache(torch, [n + 1], 16, 1, cache)
+    pg = table[0].long()
+    k[pg, 0], v[pg, 0] = keys[1], values[1]
+    k[pg[0], 0, 0], v[pg[0], 0, 0] = keys[0], values[0]
+    y = R.paged_attn_prompt(q, k, v, table, lens, torch.tensor([0, n], dtype=torch.int32, device="cuda"), window=1,
+                            sinks=1, scale=math.log(2))
+    close(torch, y, want[..., None].expand(n, 2, D), torch.full((1,), f32_tolerance(cache), device="cuda"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+def test_long_rows_of_f32_queries_do_not_drift(cache):
+    """Rows over 4000 keys with positive values, where every truncated addition of the tensor cores drifts the same
+    way. Scores of one product: off by its roundings, 3 * 2^-23 of scores up to 4, and (f16) half a step of 22 bits of
+    q. Weights: the exponential of arguments up to 16 (2^-21, 2^-22), their parts (2^-22). Sums: between two moves out
+    of TMEM at most 4 tiles * 8 steps * 3 parts, each of which drops up to 2^-23 of a sum that is half grown on the
+    average; then 8 moves, the sum of weights (32 chains of additions a tile) and the division, 2^-24 each."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    new, total = 600, 4000      # 80 row tiles or more: their keys are not split over CTAs
+    k, v, table, lens = make_cache(torch, [total], 32, 16, cache)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k[..., 1:] = 0
+    k[..., 0] = torch.rand(k.shape[:3], generator=g, device="cuda").to(k.dtype) * 2 - 1
+    v.copy_((1 + torch.rand(v.shape, generator=g, device="cuda")).to(v.dtype))
+    q = torch.zeros(new, 32, D, device="cuda")
+    q[..., 0] = 4 * torch.rand(new, 32, generator=g, device="cuda")
+    starts = torch.tensor([0, new], dtype=torch.int32, device="cuda")
+    y = R.paged_attn_prompt(q, k, v, table, lens, starts, scale=1.0)
+    want, _ = plain_attention(torch, q, k, v, table, lens, [new], 0, 0, 1.0, "f32", cache)
+    weights = 2 * (4 * 3 * 2.0 ** -23 + 4 * (2.0 ** -23 if cache == "f16" else 0) + 2.0 ** -21 + 2.0 ** -22 + 2.0 ** -22)
+    sums = 4 * 8 * (3 if cache == "bf16" else 2) / 2 * 2.0 ** -23 + (8 + 32 + 2) * 2.0 ** -24
+    close(torch, y, want, (weights + sums) * want)
+
+
 # ---- norm + rotation + append ----------------------------------------------------------------
 
 @pytest.mark.gpu
