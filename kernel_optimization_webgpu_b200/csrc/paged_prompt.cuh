@@ -425,240 +425,244 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
   if (warp >= kPpSoftmax / 32) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPpRegsFew));
     if (CLAIM && warp == kPpSoftmax / 32 + 2) {
-    // ---- schedule: this block's work, then that of blocks that have not started ----
-    // (asked for by the copy warp when it comes to the last tile)
-    int next = 1, claims = 0, block = 0, tiles = work[0].nk;
-    bool ok = true, more = true;
-    auto free_slot = [&] {
-      return next < 2 || __all_sync(0xffffffffu, pp_wait(&work_empty[next & 1], (unsigned)(next / 2 - 1) & 1u, &failed));
-    };
-    while (ok && more) {
-      ok = __all_sync(0xffffffffu, pp_wait(&ask, (unsigned)(next - 1) & 1u, &failed, pp_patience(tiles)));
-      if (!ok) break;
-      PpWork w;
-      do {
-        if (lane == 0) pp_claim(&answer, &answered);
-        ok = __all_sync(0xffffffffu, tc_mbar_wait(&answered, (unsigned)claims++ & 1u));
-        if (!ok) failed = 1;
-        more = ok && pp_claimed(&answer, block);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (read before the next answer lands)
-        __syncwarp();
-      } while (more && !find_work(__shfl_sync(0xffffffffu, block, 0), w));
-      if (!more) break;
-      for (int r = w.row0 + lane; r < min(w.row0 + kRows, w.it.n_rows); r += 32) {  // Q, to L2
-        const int tok = w.it.tok0 + r / G;
-        if ((unsigned)tok < (unsigned)a.rows) {
-          constexpr int kSize = PARTS > 1 ? 4 : 2;
-          const char* q = static_cast<const char*>(a.q) +
-                          ((long long)tok * a.q_stride + ((long long)w.g * G + r % G) * kHeadDim) * kSize;
+      // ---- schedule: this block's work, then that of blocks that have not started ----
+      // (asked for by the copy warp when it comes to the last tile)
+      int next = 1, claims = 0, block = 0, tiles = work[0].nk;
+      bool ok = true, more = true;
+      auto free_slot = [&] {
+        return next < 2 ||
+               __all_sync(0xffffffffu, pp_wait(&work_empty[next & 1], (unsigned)(next / 2 - 1) & 1u, &failed));
+      };
+      while (ok && more) {
+        ok = __all_sync(0xffffffffu, pp_wait(&ask, (unsigned)(next - 1) & 1u, &failed, pp_patience(tiles)));
+        if (!ok) break;
+        PpWork w;
+        do {
+          if (lane == 0) pp_claim(&answer, &answered);
+          ok = __all_sync(0xffffffffu, tc_mbar_wait(&answered, (unsigned)claims++ & 1u));
+          if (!ok) failed = 1;
+          more = ok && pp_claimed(&answer, block);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (read before the next answer lands)
+          __syncwarp();
+        } while (more && !find_work(__shfl_sync(0xffffffffu, block, 0), w));
+        if (!more) break;
+        for (int r = w.row0 + lane; r < min(w.row0 + kRows, w.it.n_rows); r += 32) {  // Q, to L2
+          const int tok = w.it.tok0 + r / G;
+          if ((unsigned)tok < (unsigned)a.rows) {
+            constexpr int kSize = PARTS > 1 ? 4 : 2;
+            const char* q = static_cast<const char*>(a.q) +
+                            ((long long)tok * a.q_stride + ((long long)w.g * G + r % G) * kHeadDim) * kSize;
 #pragma unroll
-          for (int i = 0; i < kHeadDim * kSize; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + i));
+            for (int i = 0; i < kHeadDim * kSize; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + i));
+          }
         }
+        tiles = w.nk;
+        ok = free_slot();
+        if (lane == 0) {
+          work[ok ? next & 1 : 2] = w;
+          if (ok) pp_arrive(&work_full[next & 1]);
+        }
+        ++next;
       }
-      tiles = w.nk;
-      ok = free_slot();
-      if (lane == 0) {
-        work[ok ? next & 1 : 2] = w;
-        if (ok) pp_arrive(&work_full[next & 1]);
+      if (ok && free_slot() && lane == 0) {
+        work[next & 1].halves = 0;
+        pp_arrive(&work_full[next & 1]);
       }
-      ++next;
-    }
-    if (ok && free_slot() && lane == 0) {
-      work[next & 1].halves = 0;
-      pp_arrive(&work_full[next & 1]);
-    }
     } else if (warp == kPpSoftmax / 32 + 1) {
-    // ---- copies: K and V tiles alternate through the ring ----
-    const int ps = 1 << a.kv.page_shift, box = min(ps, kPpKeys), boxes = kPpKeys / box;
-    int issued_to = -1, done = 0;  // ring slots of the works before
-    bool ok = !(pa.stall && blockIdx.x == 0);
-    for (int n = 0, nk = 0; ok && (CLAIM || n == 0); ++n) {
-      ok = wait_work(n, nk);
-      if (!ok || work_of(n).halves == 0) break;
-      const PpItem it = work_of(n).it;
-      const int seq = it.seq, g = work_of(n).g, t0 = work_of(n).t0;
-      nk = __shfl_sync(0xffffffffu, work_of(n).nk, 0);
-      if (CLAIM && nk == 0 && lane == 0) pp_arrive(&ask);
-      for (int i = 0; i < 2 * nk && ok; ++i) {
-        // the scheduling warp has the time of the ring's tiles to find the next work; earlier, a CTA would hold
-        // work that another one could begin
-        if (CLAIM && i == max(0, 2 * nk - 3) && lane == 0) pp_arrive(&ask);
-        const int j = i >> 1, at = done + i, slot = at % S;
-        const bool is_v = i & 1;
-        const int k0 = it.v.tile(t0 + j) * kPpKeys;
-        // lane n: the page of the n-th box, if any row of the CTA sees it
-        int page = -1;
-        const int p0 = k0 + lane * box;
-        const bool any = lane < boxes && p0 < it.v.end && (p0 + box > it.v.lo || p0 < it.v.ns);
-        if (any) page = paged_page(a.kv, seq, p0);
-        const unsigned seen = __ballot_sync(0xffffffffu, any), good = __ballot_sync(0xffffffffu, page >= 0);
-        if (at >= S) ok = pp_wait(&empty[slot], (unsigned)(at / S - 1) & 1u, &failed);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const bool partial = !(k0 + kPpKeys <= it.v.end && (k0 >= it.v.lo || k0 + kPpKeys <= it.v.ns)) || good != seen;
-        unsigned char* dst = ring + slot * kPpTileBytes;
-        if (lane == 0 && !is_v) {
-          unsigned bad = 0;
-          for (int n = 0; n < boxes; ++n)
-            if (((seen & ~good) >> n) & 1u) bad |= ((1u << (box / 16)) - 1u) << (n * (box / 16));
-          bad_rows[(at >> 1) & 7] = bad;
-          if (bad) paged_flag(a.kv, QD_PAGED_BAD_PAGE);
-        }
-        if (!(is_v && partial)) {  // whole boxes (what they hold of hidden keys gives scores that are masked)
-          if (lane == 0)
-            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc_smem(&full[slot])),
-                         "r"(__popc(good) * box * 256)
-                         : "memory");
-          __syncwarp();
-          if (page >= 0) {
-            const int y = (page * kvh + g) * ps + (p0 & (ps - 1));
-            unsigned char* d = dst + lane * box * 128;
-            tma_load_2d(d, is_v ? &pa.tv : &pa.tk, 0, y, &full[slot]);
-            tma_load_2d(d + kPpTileBytes / 2, is_v ? &pa.tv : &pa.tk, 64, y, &full[slot]);
-          }
-        } else {
-          // V of a tile with hidden rows, by groups of 16: TMA copies a group that is wholly visible and, from
-          // outside the tensor, the zeros of one that is wholly hidden; the rows of a group with both
-          // are copied or cleared one by one. (Clearing after the copy, row by row, cost 33 of 158 us
-          // where every row has a window: 5 ragged chunks of up to 1500 tokens.)
-          const int g0 = k0 + 16 * lane, gpage = __shfl_sync(0xffffffffu, page, (16 * (lane & 7)) / box);
-          bool all = lane < 8 && gpage >= 0, some = false;
-          if (all) {
-            some = g0 < it.v.end && (g0 + 16 > it.v.lo || g0 < it.v.ns);
-            all = g0 + 16 <= it.v.end && (g0 >= it.v.lo || g0 + 16 <= it.v.ns);
-          }
-          const unsigned edge = __ballot_sync(0xffffffffu, some && !all);
-          if (lane == 0)
-            asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(tc_smem(&full[slot])),
-                         "r"((8 - __popc(edge)) * 4096)
-                         : "memory");
-          __syncwarp();
-          if (lane < 8 && !((edge >> lane) & 1u)) {
-            const int y = all ? (gpage * kvh + g) * ps + (g0 & (ps - 1)) : -16;
-            unsigned char* d = dst + lane * 16 * 128;
-            tma_load_2d(d, &pa.tv16, 0, y, &full[slot]);
-            tma_load_2d(d + kPpTileBytes / 2, &pa.tv16, 64, y, &full[slot]);
-          }
-          for (unsigned left = edge; left; left &= left - 1) {
-            const int n = __ffs(left) - 1, q0 = k0 + 16 * n;
-            const long long row = ((long long)__shfl_sync(0xffffffffu, gpage, n) * kvh + g) * ps + (q0 & (ps - 1));
-            const char* src = static_cast<const char*>(a.kv.v) + row * 256 + (lane & 15) * 16;
-            const unsigned d = tc_smem(dst) + ((lane & 15) >> 3) * (kPpTileBytes / 2) + n * 16 * 128;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int r = 2 * e + (lane >> 4);
-              cp_async16(d + r * 128 + (((lane ^ r) & 7) << 4), src + r * 256, it.v.at(q0 + r));
-            }
-          }
-          if (edge) {
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-          }
-          if (lane == 0) pp_arrive(&full[slot]);
-        }
-        issued_to = at;
-    }
-    done += 2 * nk;
-    work_done(n);
-    }
-    // nothing may still be landing when the CTA ends
-    for (int i = max(0, issued_to - S + 1); i <= issued_to; ++i)
-      (void)tc_mbar_wait(&full[i % S], (unsigned)(i / S) & 1u);
-    } else if (warp == kPpSoftmax / 32) {
-    // ---- MMA issue ----
-    // The whole warp runs the loop, so that the descriptors are warp-uniform values, and one lane issues.
-    // (Under `if (lane == 0)` each of the 16 products of a tile and its operands took 90 cycles to issue,
-    // more than the 64 that it runs.)
-    const unsigned id_s = pp_idesc<T>(false), id_o = pp_idesc<T>(true), leader = lane == 0;
-    const unsigned long long dq = umma_desc_k_sw128(tc_smem(qs)), dk = umma_desc_k_sw128(tc_smem(ring));
-    const unsigned long long dv = umma_desc_mn_sw128(tc_smem(ring));
-    // S_t = Q_t K^T. The smallest part goes first: the accumulator drops bits towards zero at every step,
-    // and that costs the less the smaller the sum still is (f32 results at 64 + 3500 keys: 2.0e-6 off
-    // with the largest part first, 0.9e-6 so).
-    auto scores = [&](int t, int slot) {
-      const unsigned long long q0 = dq + (unsigned)(t * (kQTile >> 4)), k0 = dk + (unsigned)(slot * (kPpTileBytes >> 4));
-#pragma unroll
-      for (int part = 0; part < PARTS; ++part)
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-          const unsigned off = ((ks >> 2) * (kPpTileBytes / 2) + (ks & 3) * 32) >> 4;
-          const unsigned qo = (PARTS - 1 - part) * (kPpTileBytes >> 4) + off;
-          if (part == 0 && ks == 0) pp_mma_ss<false>(tmem + t * 128, q0 + qo, k0, id_s, leader);
-          else pp_mma_ss<true>(tmem + t * 128, q0 + qo, k0 + off, id_s, leader);
-        }
-      pp_commit(&s_full[t], leader);
-    };
-    bool ok = true;
-    unsigned turn = 0, q_turn = 0;  // bit t: parity of row tile t's barriers before this work
-    int done = 0;                   // ring slots of the works before
-    for (int n = 0, nk = 0; ok && (CLAIM || n == 0); ++n) {
-      ok = wait_work(n, nk);
-      if (!ok) break;
-      nk = __shfl_sync(0xffffffffu, work_of(n).nk, 0);
-      const int halves = __shfl_sync(0xffffffffu, work_of(n).halves, 0);
-      work_done(n);
-      if (halves == 0) break;
-      if (nk == 0) continue;
-      auto ring_slot = [&](int i) { return (done + i) % S; };
-      auto ring_phase = [&](int i) { return (unsigned)((done + i) / S) & 1u; };
-      ok = __all_sync(0xffffffffu, pp_wait(&full[ring_slot(0)], ring_phase(0), &failed));
-      for (int t = 0; t < halves && ok; ++t) {
-        ok = __all_sync(0xffffffffu, pp_wait(&q_full[t], (q_turn >> t) & 1u, &failed));
-        tc_fence_after();
-        if (ok) scores(t, ring_slot(0));
-    }
-    q_turn ^= halves == 2 ? 3u : 1u;
-    if (ok) pp_commit(&empty[ring_slot(0)], leader);
-    int vs = ring_slot(1), ks_slot = ring_slot(2);           // ring slots of V of tile j and K of tile j + 1,
-    unsigned vph = ring_phase(1), kph = ring_phase(2);       // and their phases
-    for (int j = 0; j < nk && ok; ++j) {
-      ok = pp_wait(&full[vs], vph, &failed);
-      if (j + 1 < nk) ok = pp_wait(&full[ks_slot], kph, &failed) && ok;
-      ok = __all_sync(0xffffffffu, ok);
-      for (int t = 0; t < halves && ok; ++t) {
-        const unsigned long long v0 = dv + (unsigned)(vs * (kPpTileBytes >> 4));
-        const unsigned od = tmem + kColO + t * 128, pd = tmem + kColP + t * 128;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          ok = __all_sync(0xffffffffu, pp_wait(half ? &p_full[t] : &p_half[t], (unsigned)(j ^ (turn >> t)) & 1u, &failed));
+      // ---- copies: K and V tiles alternate through the ring ----
+      const int ps = 1 << a.kv.page_shift, box = min(ps, kPpKeys), boxes = kPpKeys / box;
+      int issued_to = -1, done = 0;  // ring slots of the works before
+      bool ok = !(pa.stall && blockIdx.x == 0);
+      for (int n = 0, nk = 0; ok && (CLAIM || n == 0); ++n) {
+        ok = wait_work(n, nk);
+        if (!ok || work_of(n).halves == 0) break;
+        const PpItem it = work_of(n).it;
+        const int seq = it.seq, g = work_of(n).g, t0 = work_of(n).t0;
+        nk = __shfl_sync(0xffffffffu, work_of(n).nk, 0);
+        if (CLAIM && nk == 0 && lane == 0) pp_arrive(&ask);
+        for (int i = 0; i < 2 * nk && ok; ++i) {
+          // the scheduling warp has the time of the ring's tiles to find the next work; earlier, a CTA would hold
+          // work that another one could begin
+          if (CLAIM && i == max(0, 2 * nk - 3) && lane == 0) pp_arrive(&ask);
+          const int j = i >> 1, at = done + i, slot = at % S;
+          const bool is_v = i & 1;
+          const int k0 = it.v.tile(t0 + j) * kPpKeys;
+          // lane n: the page of the n-th box, if any row of the CTA sees it
+          int page = -1;
+          const int p0 = k0 + lane * box;
+          const bool any = lane < boxes && p0 < it.v.end && (p0 + box > it.v.lo || p0 < it.v.ns);
+          if (any) page = paged_page(a.kv, seq, p0);
+          const unsigned seen = __ballot_sync(0xffffffffu, any), good = __ballot_sync(0xffffffffu, page >= 0);
+          if (at >= S) ok = pp_wait(&empty[slot], (unsigned)(at / S - 1) & 1u, &failed);
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int part = 0; part < PARTS; ++part)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int ks = 2 * half + (i & 1) + 4 * (i >> 1);  // keys 0-31 and 64-95, then the others
-              const unsigned po = (PARTS - 1 - part) * 64 + ks * 8;
-              if (half == 0 && part == 0 && i == 0)
-                pp_mma_ts(od, pd + po, v0, id_o, PARTS > 1 ? j % kPpFlush != 0 : j > 0, leader);
-              else
-                pp_mma_ts(od, pd + po, v0 + ks * (2048 >> 4), id_o, true, leader);
+          const bool partial =
+              !(k0 + kPpKeys <= it.v.end && (k0 >= it.v.lo || k0 + kPpKeys <= it.v.ns)) || good != seen;
+          unsigned char* dst = ring + slot * kPpTileBytes;
+          if (lane == 0 && !is_v) {
+            unsigned bad = 0;
+            for (int n = 0; n < boxes; ++n)
+              if (((seen & ~good) >> n) & 1u) bad |= ((1u << (box / 16)) - 1u) << (n * (box / 16));
+            bad_rows[(at >> 1) & 7] = bad;
+            if (bad) paged_flag(a.kv, QD_PAGED_BAD_PAGE);
+          }
+          if (!(is_v && partial)) {  // whole boxes (what they hold of hidden keys gives scores that are masked)
+            if (lane == 0)
+              asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc_smem(&full[slot])),
+                           "r"(__popc(good) * box * 256)
+                           : "memory");
+            __syncwarp();
+            if (page >= 0) {
+              const int y = (page * kvh + g) * ps + (p0 & (ps - 1));
+              unsigned char* d = dst + lane * box * 128;
+              tma_load_2d(d, is_v ? &pa.tv : &pa.tk, 0, y, &full[slot]);
+              tma_load_2d(d + kPpTileBytes / 2, is_v ? &pa.tv : &pa.tk, 64, y, &full[slot]);
             }
+          } else {
+            // V of a tile with hidden rows, by groups of 16: TMA copies a group that is wholly visible and, from
+            // outside the tensor, the zeros of one that is wholly hidden; the rows of a group with both
+            // are copied or cleared one by one. (Clearing after the copy, row by row, cost 33 of 158 us
+            // where every row has a window: 5 ragged chunks of up to 1500 tokens.)
+            const int g0 = k0 + 16 * lane, gpage = __shfl_sync(0xffffffffu, page, (16 * (lane & 7)) / box);
+            bool all = lane < 8 && gpage >= 0, some = false;
+            if (all) {
+              some = g0 < it.v.end && (g0 + 16 > it.v.lo || g0 < it.v.ns);
+              all = g0 + 16 <= it.v.end && (g0 >= it.v.lo || g0 + 16 <= it.v.ns);
+            }
+            const unsigned edge = __ballot_sync(0xffffffffu, some && !all);
+            if (lane == 0)
+              asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(tc_smem(&full[slot])),
+                           "r"((8 - __popc(edge)) * 4096)
+                           : "memory");
+            __syncwarp();
+            if (lane < 8 && !((edge >> lane) & 1u)) {
+              const int y = all ? (gpage * kvh + g) * ps + (g0 & (ps - 1)) : -16;
+              unsigned char* d = dst + lane * 16 * 128;
+              tma_load_2d(d, &pa.tv16, 0, y, &full[slot]);
+              tma_load_2d(d + kPpTileBytes / 2, &pa.tv16, 64, y, &full[slot]);
+            }
+            for (unsigned left = edge; left; left &= left - 1) {
+              const int n = __ffs(left) - 1, q0 = k0 + 16 * n;
+              const long long row = ((long long)__shfl_sync(0xffffffffu, gpage, n) * kvh + g) * ps + (q0 & (ps - 1));
+              const char* src = static_cast<const char*>(a.kv.v) + row * 256 + (lane & 15) * 16;
+              const unsigned d = tc_smem(dst) + ((lane & 15) >> 3) * (kPpTileBytes / 2) + n * 16 * 128;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const int r = 2 * e + (lane >> 4);
+                cp_async16(d + r * 128 + (((lane ^ r) & 7) << 4), src + r * 256, it.v.at(q0 + r));
+              }
+            }
+            if (edge) {
+              asm volatile("cp.async.wait_all;" ::: "memory");
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+            }
+            if (lane == 0) pp_arrive(&full[slot]);
+          }
+          issued_to = at;
         }
-        if (!ok) break;
-        pp_commit(&o_done[t], leader);
-        if (t == halves - 1) pp_commit(&empty[vs], leader);
-        if (j + 1 < nk) {
-          scores(t, ks_slot);
-          if (t == halves - 1) pp_commit(&empty[ks_slot], leader);
-        }
+        done += 2 * nk;
+        work_done(n);
       }
-      vs += 2;
-      if (vs >= S) vs -= S, vph ^= 1u;
-      ks_slot += 2;
-      if (ks_slot >= S) ks_slot -= S, kph ^= 1u;
+      // nothing may still be landing when the CTA ends
+      for (int i = max(0, issued_to - S + 1); i <= issued_to; ++i)
+        (void)tc_mbar_wait(&full[i % S], (unsigned)(i / S) & 1u);
+    } else if (warp == kPpSoftmax / 32) {
+      // ---- MMA issue ----
+      // The whole warp runs the loop, so that the descriptors are warp-uniform values, and one lane issues.
+      // (Under `if (lane == 0)` each of the 16 products of a tile and its operands took 90 cycles to issue,
+      // more than the 64 that it runs.)
+      const unsigned id_s = pp_idesc<T>(false), id_o = pp_idesc<T>(true), leader = lane == 0;
+      const unsigned long long dq = umma_desc_k_sw128(tc_smem(qs)), dk = umma_desc_k_sw128(tc_smem(ring));
+      const unsigned long long dv = umma_desc_mn_sw128(tc_smem(ring));
+      // S_t = Q_t K^T. The smallest part goes first: the accumulator drops bits towards zero at every step,
+      // and that costs the less the smaller the sum still is (f32 results at 64 + 3500 keys: 2.0e-6 off
+      // with the largest part first, 0.9e-6 so).
+      auto scores = [&](int t, int slot) {
+        const unsigned long long q0 = dq + (unsigned)(t * (kQTile >> 4));
+        const unsigned long long k0 = dk + (unsigned)(slot * (kPpTileBytes >> 4));
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {
+            const unsigned off = ((ks >> 2) * (kPpTileBytes / 2) + (ks & 3) * 32) >> 4;
+            const unsigned qo = (PARTS - 1 - part) * (kPpTileBytes >> 4) + off;
+            if (part == 0 && ks == 0) pp_mma_ss<false>(tmem + t * 128, q0 + qo, k0, id_s, leader);
+            else pp_mma_ss<true>(tmem + t * 128, q0 + qo, k0 + off, id_s, leader);
+          }
+        pp_commit(&s_full[t], leader);
+      };
+      bool ok = true;
+      unsigned turn = 0, q_turn = 0;  // bit t: parity of row tile t's barriers before this work
+      int done = 0;                   // ring slots of the works before
+      for (int n = 0, nk = 0; ok && (CLAIM || n == 0); ++n) {
+        ok = wait_work(n, nk);
+        if (!ok) break;
+        nk = __shfl_sync(0xffffffffu, work_of(n).nk, 0);
+        const int halves = __shfl_sync(0xffffffffu, work_of(n).halves, 0);
+        work_done(n);
+        if (halves == 0) break;
+        if (nk == 0) continue;
+        auto ring_slot = [&](int i) { return (done + i) % S; };
+        auto ring_phase = [&](int i) { return (unsigned)((done + i) / S) & 1u; };
+        ok = __all_sync(0xffffffffu, pp_wait(&full[ring_slot(0)], ring_phase(0), &failed));
+        for (int t = 0; t < halves && ok; ++t) {
+          ok = __all_sync(0xffffffffu, pp_wait(&q_full[t], (q_turn >> t) & 1u, &failed));
+          tc_fence_after();
+          if (ok) scores(t, ring_slot(0));
+        }
+        q_turn ^= halves == 2 ? 3u : 1u;
+        if (ok) pp_commit(&empty[ring_slot(0)], leader);
+        int vs = ring_slot(1), ks_slot = ring_slot(2);           // ring slots of V of tile j and K of tile j + 1,
+        unsigned vph = ring_phase(1), kph = ring_phase(2);       // and their phases
+        for (int j = 0; j < nk && ok; ++j) {
+          ok = pp_wait(&full[vs], vph, &failed);
+          if (j + 1 < nk) ok = pp_wait(&full[ks_slot], kph, &failed) && ok;
+          ok = __all_sync(0xffffffffu, ok);
+          for (int t = 0; t < halves && ok; ++t) {
+            const unsigned long long v0 = dv + (unsigned)(vs * (kPpTileBytes >> 4));
+            const unsigned od = tmem + kColO + t * 128, pd = tmem + kColP + t * 128;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              ok = __all_sync(0xffffffffu, pp_wait(half ? &p_full[t] : &p_half[t], (unsigned)(j ^ (turn >> t)) & 1u,
+                                                   &failed));
+              if (!ok) break;
+              tc_fence_after();
+#pragma unroll
+              for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int ks = 2 * half + (i & 1) + 4 * (i >> 1);  // keys 0-31 and 64-95, then the others
+                  const unsigned po = (PARTS - 1 - part) * 64 + ks * 8;
+                  if (half == 0 && part == 0 && i == 0)
+                    pp_mma_ts(od, pd + po, v0, id_o, PARTS > 1 ? j % kPpFlush != 0 : j > 0, leader);
+                  else
+                    pp_mma_ts(od, pd + po, v0 + ks * (2048 >> 4), id_o, true, leader);
+                }
+            }
+            if (!ok) break;
+            pp_commit(&o_done[t], leader);
+            if (t == halves - 1) pp_commit(&empty[vs], leader);
+            if (j + 1 < nk) {
+              scores(t, ks_slot);
+              if (t == halves - 1) pp_commit(&empty[ks_slot], leader);
+            }
+          }
+          vs += 2;
+          if (vs >= S) vs -= S, vph ^= 1u;
+          ks_slot += 2;
+          if (ks_slot >= S) ks_slot -= S, kph ^= 1u;
+        }
+        done += 2 * nk;
+        if (nk & 1) turn ^= halves == 2 ? 3u : 1u;
+      }
+      if (!ok) {  // given up: let what was issued finish before the CTA ends
+        pp_commit(&drain, leader);
+        (void)tc_mbar_wait(&drain, 0);
+      }
     }
-    done += 2 * nk;
-    if (nk & 1) turn ^= halves == 2 ? 3u : 1u;
-    }
-    if (!ok) {  // given up: let what was issued finish before the CTA ends
-      pp_commit(&drain, leader);
-      (void)tc_mbar_wait(&drain, 0);
-    }
-  }
-  tc_fence_before();
-  __syncthreads();
+    tc_fence_before();
+    __syncthreads();
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPpRegsMany));
     // ---- softmax: half a row per thread ----
@@ -671,298 +675,300 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       if (CLAIM) {
         ok = ok && wait_work(n, nk);
         if (pp_any(pair, !ok)) break;
-    }
-    const PpItem it = work_of(n).it;
-    const int item = work_of(n).item, g = work_of(n).g, z = work_of(n).z, parts = work_of(n).parts, t0 = work_of(n).t0,
-              halves = __shfl_sync(0xffffffffu, work_of(n).halves, 0);
-    nk = __shfl_sync(0xffffffffu, work_of(n).nk, 0);
-    if (halves == 0) break;
-    const int row = work_of(n).row0 + lr, tok = row / G, hs = row - tok * G;
-    const bool live = lr < kRows && row < it.n_rows && (unsigned)(it.tok0 + tok) < (unsigned)a.rows;
-    if (t < halves && nk > 0) {
-      // Q: K-major with the 128-byte swizzle; dead rows are zero. A warp copies its 32 rows' 64 dims row by
-      // row, neighbouring lanes on neighbouring chunks (a row per lane took 4.5 us of a busy GPU's
-      // time). A negative scale changes the sign of q, so that the softmax always has a positive one.
-      const int wr = (warp & 3) * 32;  // first of the warp's rows in its tile
-      unsigned char* wq = qs + t * kQTile + hf * (kPpTileBytes / 2);
-      const long long q_at =
-          live ? (long long)(it.tok0 + tok) * a.q_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf : -1;
-      float c = fabsf(a.scale) * kLog2e;  // of the row's scores
-      if constexpr (PARTS > 1) {
-        const int c4 = lane & 15;
-        constexpr int N = PARTS == 2 ? 16 : 8;
-#pragma unroll
-        for (int i0 = 0; i0 < 16; i0 += N) {
-          float4 x[N];
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const long long at = __shfl_sync(0xffffffffu, q_at, 2 * (i0 + i) + (lane >> 4));
-            x[i] = at >= 0 ? load4<float>(a.q, at + 4 * c4) : make_float4(0.f, 0.f, 0.f, 0.f);
-            if (a.scale < 0.0f) x[i] = make_float4(-x[i].x, -x[i].y, -x[i].z, -x[i].w);
-          }
-          if constexpr (PARTS == 2) {
-            // Each row by its own power of two to where two f16 hold 22 bits of it (f16_fit). The largest of
-            // a row's 64 dims, for the i-th pair of rows in lane i of each half; the partner warp has the others:
-            // the two exponents go to the halves of the row's word.
-            float top[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              top[i] = fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1)
-#pragma unroll
-              for (int i = 0; i < o; ++i) {
-                const float theirs = lane & o ? top[i] : top[i + o], ours = lane & o ? top[i + o] : top[i];
-                top[i] = fmaxf(ours, __shfl_xor_sync(0xffffffffu, theirs, o));
-              }
-            const unsigned* tops = reinterpret_cast<const unsigned*>(shared_row) + t * 128;
-            reinterpret_cast<unsigned short*>(shared_row)[2 * (t * 128 + wr + 2 * c4 + (lane >> 4)) + hf] =
-                (unsigned short)(__float_as_int(top[0]) >> 23);
-            pp_meet(pair);
-            auto fit = [&](int r) { return f16_fit((int)max(tops[r] & 0xffffu, tops[r] >> 16)); };
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float up = fit(wr + 2 * i + (lane >> 4)).x;
-              x[i] = make_float4(x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up);
-            }
-            c = fmaxf(c * fit(wr + lane).y, 1.0e-37f);  // (never 0: a hidden key's score is -inf)
-          }
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const int r = wr + 2 * (i0 + i) + (lane >> 4);
-            unsigned u[2][PARTS];
-            split_parts<T, PARTS>(x[i].x, x[i].y, u[0]);
-            split_parts<T, PARTS>(x[i].z, x[i].w, u[1]);
-            const unsigned off = r * 128 + ((((c4 >> 1) ^ r) & 7) << 4) + (c4 & 1) * 8;
-#pragma unroll
-            for (int part = 0; part < PARTS; ++part)
-              *reinterpret_cast<uint2*>(wq + part * kPpTileBytes + off) = make_uint2(u[0][part], u[1][part]);
-          }
-        }
-      } else {
-        uint4 x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const long long at = __shfl_sync(0xffffffffu, q_at, 4 * i + (lane >> 3));
-          x[i] = at >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at + 8 * (lane & 7))
-                         : make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (a.scale < 0.0f)
-            x[i] = make_uint4(x[i].x ^ 0x80008000u, x[i].y ^ 0x80008000u, x[i].z ^ 0x80008000u, x[i].w ^ 0x80008000u);
-          const int r = wr + 4 * i + (lane >> 3);
-          *reinterpret_cast<uint4*>(wq + r * 128 + (((lane ^ r) & 7) << 4)) = x[i];
-        }
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      pp_arrive(&q_full[t]);
-      float m = -INFINITY, l = 0.0f;
-      const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
-      const unsigned ts = tmem + t * 128 + lanes, tp = tmem + kColP + t * 128 + 32 * hf + lanes;
-      const unsigned to = tmem + kColO + t * 128 + 64 * hf + lanes;
-      const int p = live ? it.pos0 + tok : -1;
-      const int pmax = min(p, it.len - 1);
-      const int phi = a.window > 0 ? p - a.window : -2;  // keys up to here are hidden, unless sinks
-      // positions of the warp's first and last live rows
-      const unsigned lv = __ballot_sync(0xffffffffu, live);
-      const int pw0 = __shfl_sync(0xffffffffu, p, 0), pw1 = __shfl_sync(0xffffffffu, p, lv ? 31 - __clz(lv) : 0);
-      const long long part0 = (((long long)item * kvh + g) * pa.splits + z) * kRows;
-      float4* mine = pa.po + part0 * (kHeadDim / 4) + lr;
-      float moved = -INFINITY;  // the maximum that the sums in the workspace go by
-      for (int j = 0; j < nk; ++j) {
-        ok = ok && __all_sync(0xffffffffu, pp_wait(&s_full[t], (unsigned)(j ^ turn) & 1u, &failed));
-        tc_fence_after();
-        unsigned sr[64];
-        tmem_ld64(ts + 64 * hf, sr);
-        const int k0 = it.v.tile(t0 + j) * kPpKeys;
-        const unsigned bad = bad_rows[(done + j) & 7];
-        const bool inside = lv == 0xffffffffu && bad == 0 && k0 + kPpKeys - 1 <= min(pw0, it.len - 1) &&
-                            (a.window == 0 || k0 > pw1 - a.window || k0 + kPpKeys <= a.sinks);
-        if (!inside) {
-          // bit i of a word: key at + i is visible to this row
+      const PpItem it = work_of(n).it;
+      const int item = work_of(n).item, g = work_of(n).g, z = work_of(n).z, parts = work_of(n).parts,
+                t0 = work_of(n).t0, halves = __shfl_sync(0xffffffffu, work_of(n).halves, 0);
+      nk = __shfl_sync(0xffffffffu, work_of(n).nk, 0);
+      if (halves == 0) break;
+      const int row = work_of(n).row0 + lr, tok = row / G, hs = row - tok * G;
+      const bool live = lr < kRows && row < it.n_rows && (unsigned)(it.tok0 + tok) < (unsigned)a.rows;
+      if (t < halves && nk > 0) {
+        // Q: K-major with the 128-byte swizzle; dead rows are zero. A warp copies its 32 rows' 64 dims row by
+        // row, neighbouring lanes on neighbouring chunks (a row per lane took 4.5 us of a busy GPU's
+        // time). A negative scale changes the sign of q, so that the softmax always has a positive one.
+        const int wr = (warp & 3) * 32;  // first of the warp's rows in its tile
+        unsigned char* wq = qs + t * kQTile + hf * (kPpTileBytes / 2);
+        const long long q_at =
+            live ? (long long)(it.tok0 + tok) * a.q_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf : -1;
+        float c = fabsf(a.scale) * kLog2e;  // of the row's scores
+        if constexpr (PARTS > 1) {
+          const int c4 = lane & 15;
+          constexpr int N = PARTS == 2 ? 16 : 8;
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const int at = k0 + 64 * hf + 32 * w, b = bad >> (4 * hf + 2 * w);
-            unsigned see = pp_below(pmax + 1 - at) & (~pp_below(phi + 1 - at) | pp_below(a.sinks - at));
-            if (b & 1) see &= 0xffff0000u;
-            if (b & 2) see &= 0x0000ffffu;
+          for (int i0 = 0; i0 < 16; i0 += N) {
+            float4 x[N];
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!((see >> i) & 1u)) sr[32 * w + i] = 0xff800000u;
+            for (int i = 0; i < N; ++i) {
+              const long long at = __shfl_sync(0xffffffffu, q_at, 2 * (i0 + i) + (lane >> 4));
+              x[i] = at >= 0 ? load4<float>(a.q, at + 4 * c4) : make_float4(0.f, 0.f, 0.f, 0.f);
+              if (a.scale < 0.0f) x[i] = make_float4(-x[i].x, -x[i].y, -x[i].z, -x[i].w);
+            }
+            if constexpr (PARTS == 2) {
+              // Each row by its own power of two to where two f16 hold 22 bits of it (f16_fit). The largest of
+              // a row's 64 dims, for the i-th pair of rows in lane i of each half; the partner warp has the others:
+              // the two exponents go to the halves of the row's word.
+              float top[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                top[i] = fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
+#pragma unroll
+              for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+                for (int i = 0; i < o; ++i) {
+                  const float theirs = lane & o ? top[i] : top[i + o], ours = lane & o ? top[i + o] : top[i];
+                  top[i] = fmaxf(ours, __shfl_xor_sync(0xffffffffu, theirs, o));
+                }
+              const unsigned* tops = reinterpret_cast<const unsigned*>(shared_row) + t * 128;
+              reinterpret_cast<unsigned short*>(shared_row)[2 * (t * 128 + wr + 2 * c4 + (lane >> 4)) + hf] =
+                  (unsigned short)(__float_as_int(top[0]) >> 23);
+              pp_meet(pair);
+              auto fit = [&](int r) { return f16_fit((int)max(tops[r] & 0xffffu, tops[r] >> 16)); };
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float up = fit(wr + 2 * i + (lane >> 4)).x;
+                x[i] = make_float4(x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up);
+              }
+              c = fmaxf(c * fit(wr + lane).y, 1.0e-37f);  // (never 0: a hidden key's score is -inf)
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              const int r = wr + 2 * (i0 + i) + (lane >> 4);
+              unsigned u[2][PARTS];
+              split_parts<T, PARTS>(x[i].x, x[i].y, u[0]);
+              split_parts<T, PARTS>(x[i].z, x[i].w, u[1]);
+              const unsigned off = r * 128 + ((((c4 >> 1) ^ r) & 7) << 4) + (c4 & 1) * 8;
+#pragma unroll
+              for (int part = 0; part < PARTS; ++part)
+                *reinterpret_cast<uint2*>(wq + part * kPpTileBytes + off) = make_uint2(u[0][part], u[1][part]);
+            }
+          }
+        } else {
+          uint4 x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const long long at = __shfl_sync(0xffffffffu, q_at, 4 * i + (lane >> 3));
+            x[i] = at >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at + 8 * (lane & 7))
+                           : make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (a.scale < 0.0f)
+              x[i] = make_uint4(x[i].x ^ 0x80008000u, x[i].y ^ 0x80008000u, x[i].z ^ 0x80008000u, x[i].w ^ 0x80008000u);
+            const int r = wr + 4 * i + (lane >> 3);
+            *reinterpret_cast<uint4*>(wq + r * 128 + (((lane ^ r) & 7) << 4)) = x[i];
           }
         }
-        float mx[4];
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        pp_arrive(&q_full[t]);
+        float m = -INFINITY, l = 0.0f;
+        const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
+        const unsigned ts = tmem + t * 128 + lanes, tp = tmem + kColP + t * 128 + 32 * hf + lanes;
+        const unsigned to = tmem + kColO + t * 128 + 64 * hf + lanes;
+        const int p = live ? it.pos0 + tok : -1;
+        const int pmax = min(p, it.len - 1);
+        const int phi = a.window > 0 ? p - a.window : -2;  // keys up to here are hidden, unless sinks
+        // positions of the warp's first and last live rows
+        const unsigned lv = __ballot_sync(0xffffffffu, live);
+        const int pw0 = __shfl_sync(0xffffffffu, p, 0), pw1 = __shfl_sync(0xffffffffu, p, lv ? 31 - __clz(lv) : 0);
+        const long long part0 = (((long long)item * kvh + g) * pa.splits + z) * kRows;
+        float4* mine = pa.po + part0 * (kHeadDim / 4) + lr;
+        float moved = -INFINITY;  // the maximum that the sums in the workspace go by
+        for (int j = 0; j < nk; ++j) {
+          ok = ok && __all_sync(0xffffffffu, pp_wait(&s_full[t], (unsigned)(j ^ turn) & 1u, &failed));
+          tc_fence_after();
+          unsigned sr[64];
+          tmem_ld64(ts + 64 * hf, sr);
+          const int k0 = it.v.tile(t0 + j) * kPpKeys;
+          const unsigned bad = bad_rows[(done + j) & 7];
+          const bool inside = lv == 0xffffffffu && bad == 0 && k0 + kPpKeys - 1 <= min(pw0, it.len - 1) &&
+                              (a.window == 0 || k0 > pw1 - a.window || k0 + kPpKeys <= a.sinks);
+          if (!inside) {
+            // bit i of a word: key at + i is visible to this row
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(sr[e]);
+            for (int w = 0; w < 2; ++w) {
+              const int at = k0 + 64 * hf + 32 * w, b = bad >> (4 * hf + 2 * w);
+              unsigned see = pp_below(pmax + 1 - at) & (~pp_below(phi + 1 - at) | pp_below(a.sinks - at));
+              if (b & 1) see &= 0xffff0000u;
+              if (b & 2) see &= 0x0000ffffu;
 #pragma unroll
-        for (int i = 4; i < 60; i += 8)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sr[i + e]), __uint_as_float(sr[i + 4 + e]));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sr[60 + e]), -INFINITY);
-        float mt = max3(max3(mx[0], mx[1], mx[2]), mx[3], -INFINITY) * c;  // NaN where a score is
-        // This barrier also stands between every read of S and the writes of P over it.
-        if (pp_any(pair, !ok || mt > m + kPpLag)) {
-          // The first thread's maximum to the second, the larger one back. (A NaN maximum moves nothing: its
-          // row becomes NaN by its weights.)
-          const float gone = __int_as_float(0x7fffffff);
-          if (!(mt == mt)) mt = -INFINITY;
-          if (hf == 0) shared_row[lr] = ok ? mt : gone;
-          pp_meet(pair);
-          if (hf == 1) {
-            const float other = shared_row[lr];
-            shared_row[lr] = ok && other == other ? fmaxf(mt, other) : gone;
+              for (int i = 0; i < 32; ++i)
+                if (!((see >> i) & 1u)) sr[32 * w + i] = 0xff800000u;
+            }
           }
-          pp_meet(pair);
-          mt = shared_row[lr];
-          ok = __all_sync(0xffffffffu, mt == mt);
-          if (!ok) break;
-          // each row by its own maximum (a factor of 1 where it has not moved), so that a row's result
-          // does not depend on the rows beside it
-          const float mn = mt > m + kPpLag ? mt : m;
-          const float f = m == -INFINITY ? 0.0f : exp2_fast(m - mn);
-          m = mn;
-          l *= f;
-          if (j > 0) {  // the product of the tile before must have reached O
-            ok = __all_sync(0xffffffffu, pp_wait(&o_done[t], (unsigned)((j - 1) ^ turn) & 1u, &failed));
+          float mx[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(sr[e]);
+#pragma unroll
+          for (int i = 4; i < 60; i += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sr[i + e]), __uint_as_float(sr[i + 4 + e]));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sr[60 + e]), -INFINITY);
+          float mt = max3(max3(mx[0], mx[1], mx[2]), mx[3], -INFINITY) * c;  // NaN where a score is
+          // This barrier also stands between every read of S and the writes of P over it.
+          if (pp_any(pair, !ok || mt > m + kPpLag)) {
+            // The first thread's maximum to the second, the larger one back. (A NaN maximum moves nothing: its
+            // row becomes NaN by its weights.)
+            const float gone = __int_as_float(0x7fffffff);
+            if (!(mt == mt)) mt = -INFINITY;
+            if (hf == 0) shared_row[lr] = ok ? mt : gone;
+            pp_meet(pair);
+            if (hf == 1) {
+              const float other = shared_row[lr];
+              shared_row[lr] = ok && other == other ? fmaxf(mt, other) : gone;
+            }
+            pp_meet(pair);
+            mt = shared_row[lr];
+            ok = __all_sync(0xffffffffu, mt == mt);
+            if (!ok) break;
+            // each row by its own maximum (a factor of 1 where it has not moved), so that a row's result
+            // does not depend on the rows beside it
+            const float mn = mt > m + kPpLag ? mt : m;
+            const float f = m == -INFINITY ? 0.0f : exp2_fast(m - mn);
+            m = mn;
+            l *= f;
+            if (j > 0) {  // the product of the tile before must have reached O
+              ok = __all_sync(0xffffffffu, pp_wait(&o_done[t], (unsigned)((j - 1) ^ turn) & 1u, &failed));
+              tc_fence_after();
+#pragma unroll 1
+              for (int h = 0; h < 4; ++h) {
+                unsigned o[16];
+                tmem_ld16(to + 16 * h, o);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tmem_st16(to + 16 * h, o);
+              }
+            }
+          }
+          if (PARTS > 1 && j > 0 && j % kPpFlush == 0) {
+            ok = ok && __all_sync(0xffffffffu, pp_wait(&o_done[t], (unsigned)((j - 1) ^ turn) & 1u, &failed));
             tc_fence_after();
+            const float f = moved == -INFINITY ? 0.0f : exp2_fast(moved - m);
 #pragma unroll 1
             for (int h = 0; h < 4; ++h) {
               unsigned o[16];
               tmem_ld16(to + 16 * h, o);
+              float4* dst = mine + (16 * hf + 4 * h) * kRows;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              tmem_st16(to + 16 * h, o);
-            }
-          }
-        }
-        if (PARTS > 1 && j > 0 && j % kPpFlush == 0) {
-          ok = ok && __all_sync(0xffffffffu, pp_wait(&o_done[t], (unsigned)((j - 1) ^ turn) & 1u, &failed));
-          tc_fence_after();
-          const float f = moved == -INFINITY ? 0.0f : exp2_fast(moved - m);
-#pragma unroll 1
-          for (int h = 0; h < 4; ++h) {
-            unsigned o[16];
-            tmem_ld16(to + 16 * h, o);
-            float4* dst = mine + (16 * hf + 4 * h) * kRows;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float4 x = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                     __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
-              if (j > kPpFlush) {
-                const float4 y = dst[i * kRows];
-                x = make_float4(fmaf(y.x, f, x.x), fmaf(y.y, f, x.y), fmaf(y.z, f, x.z), fmaf(y.w, f, x.w));
+              for (int i = 0; i < 4; ++i) {
+                float4 x = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                       __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+                if (j > kPpFlush) {
+                  const float4 y = dst[i * kRows];
+                  x = make_float4(fmaf(y.x, f, x.x), fmaf(y.y, f, x.y), fmaf(y.z, f, x.z), fmaf(y.w, f, x.w));
+                }
+                dst[i * kRows] = x;
               }
-              dst[i * kRows] = x;
             }
-          }
-          moved = m;
-          tc_fence_before();
-        }
-        const float ref = m == -INFINITY ? 0.0f : kPpShift - m;
-        float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {  // 32 keys: 16 packed columns
-          unsigned w[PARTS][16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float s0 = __uint_as_float(sr[32 * h + 2 * i]), s1 = __uint_as_float(sr[32 * h + 2 * i + 1]);
-            float2 e = __ffma2_rn(make_float2(s0, s1), make_float2(c, c), make_float2(ref, ref));
-            e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-            sum = __fadd2_rn(sum, e);
-            unsigned u[PARTS];
-            split_parts<T, PARTS>(e.x, e.y, u);
-#pragma unroll
-            for (int part = 0; part < PARTS; ++part) w[part][i] = u[part];
-          }
-#pragma unroll
-          for (int part = 0; part < PARTS; ++part) tmem_st16(tp + 64 * part + 16 * h, w[part]);
-          if (h == 0) {  // the products of the first half of both threads' keys may start
-            tmem_wait_st();
+            moved = m;
             tc_fence_before();
-            if (ok) pp_arrive(&p_half[t]);
           }
-        }
-        l += sum.x + sum.y;
-        tmem_wait_st();
-        tc_fence_before();
-        if (ok) pp_arrive(&p_full[t]);
-      }
-      pp_meet(pair);  // (the last maximum has been read)
-      if (hf == 0) shared_row[lr] = l;
-      pp_meet(pair);
-      if (hf == 1) shared_row[lr] += l;
-      pp_meet(pair);
-      l = shared_row[lr];
-      if (ok) ok = __all_sync(0xffffffffu, pp_wait(&o_done[t], (unsigned)((nk - 1) ^ turn) & 1u, &failed));
-      if (ok) {
-        tc_fence_after();
-        const bool whole = parts == 1;
-        const float f = whole ? inv_sum(l) : 1.0f;
-        const long long y_at =
-            live ? (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf : -1;
-        if (!whole && hf == 0) pa.pml[part0 + lr] = make_float2(m, l);
-        // Whole rows leave through the warp's part of Q's shared memory (every product that read it is done),
-        // 32 dims at a time, so that neighbouring lanes write neighbouring chunks.
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          float o[32];
-          tmem_ld32(to + 32 * h, o);
-          if (PARTS > 1 && nk > kPpFlush) {
-            const float fm = moved == -INFINITY ? 0.0f : exp2_fast(moved - m);
-            const float4* src = mine + (16 * hf + 8 * h) * kRows;
+          const float ref = m == -INFINITY ? 0.0f : kPpShift - m;
+          float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 y = src[i * kRows];
-              o[4 * i] = fmaf(y.x, fm, o[4 * i]);
-              o[4 * i + 1] = fmaf(y.y, fm, o[4 * i + 1]);
-              o[4 * i + 2] = fmaf(y.z, fm, o[4 * i + 2]);
-              o[4 * i + 3] = fmaf(y.w, fm, o[4 * i + 3]);
+          for (int h = 0; h < 2; ++h) {  // 32 keys: 16 packed columns
+            unsigned w[PARTS][16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float s0 = __uint_as_float(sr[32 * h + 2 * i]), s1 = __uint_as_float(sr[32 * h + 2 * i + 1]);
+              float2 e = __ffma2_rn(make_float2(s0, s1), make_float2(c, c), make_float2(ref, ref));
+              e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+              sum = __fadd2_rn(sum, e);
+              unsigned u[PARTS];
+              split_parts<T, PARTS>(e.x, e.y, u);
+#pragma unroll
+              for (int part = 0; part < PARTS; ++part) w[part][i] = u[part];
+            }
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) tmem_st16(tp + 64 * part + 16 * h, w[part]);
+            if (h == 0) {  // the products of the first half of both threads' keys may start
+              tmem_wait_st();
+              tc_fence_before();
+              if (ok) pp_arrive(&p_half[t]);
             }
           }
-          if (!whole) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              mine[(16 * hf + 8 * h + i / 4) * kRows] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-            continue;
-          }
-          constexpr int kChunks = PARTS > 1 ? 8 : 4;  // 16-byte chunks of 32 dims
-          unsigned char* my_row = wq + (wr + lane) * 128;
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
-            uint4 x;
-            if constexpr (PARTS > 1)
-              x = make_uint4(__float_as_uint(o[4 * c] * f), __float_as_uint(o[4 * c + 1] * f),
-                             __float_as_uint(o[4 * c + 2] * f), __float_as_uint(o[4 * c + 3] * f));
-            else
-              x = make_uint4(pack2<T>(o[8 * c] * f, o[8 * c + 1] * f), pack2<T>(o[8 * c + 2] * f, o[8 * c + 3] * f),
-                             pack2<T>(o[8 * c + 4] * f, o[8 * c + 5] * f), pack2<T>(o[8 * c + 6] * f, o[8 * c + 7] * f));
-            *reinterpret_cast<uint4*>(my_row + (((c ^ lane) & 7) << 4)) = x;
-          }
-          __syncwarp();
-          constexpr int kAtOnce = 32 / kChunks;  // rows a step of the warp writes
-#pragma unroll
-          for (int i = 0; i < 32 / kAtOnce; ++i) {
-            const int r = i * kAtOnce + lane / kChunks, c = lane % kChunks;
-            const long long at = __shfl_sync(0xffffffffu, y_at, r);
-            const uint4 x = *reinterpret_cast<const uint4*>(wq + (wr + r) * 128 + (((c ^ r) & 7) << 4));
-            if (at >= 0)
-              *reinterpret_cast<uint4*>(static_cast<unsigned char*>(a.y) +
-                                        (at + 32 * h) * (PARTS > 1 ? 4 : (int)sizeof(T)) + 16 * c) = x;
-          }
-          __syncwarp();
+          l += sum.x + sum.y;
+          tmem_wait_st();
+          tc_fence_before();
+          if (ok) pp_arrive(&p_full[t]);
         }
+        pp_meet(pair);  // (the last maximum has been read)
+        if (hf == 0) shared_row[lr] = l;
+        pp_meet(pair);
+        if (hf == 1) shared_row[lr] += l;
+        pp_meet(pair);
+        l = shared_row[lr];
+        if (ok) ok = __all_sync(0xffffffffu, pp_wait(&o_done[t], (unsigned)((nk - 1) ^ turn) & 1u, &failed));
+        if (ok) {
+          tc_fence_after();
+          const bool whole = parts == 1;
+          const float f = whole ? inv_sum(l) : 1.0f;
+          const long long y_at =
+              live ? (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf : -1;
+          if (!whole && hf == 0) pa.pml[part0 + lr] = make_float2(m, l);
+          // Whole rows leave through the warp's part of Q's shared memory (every product that read it is done),
+          // 32 dims at a time, so that neighbouring lanes write neighbouring chunks.
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            float o[32];
+            tmem_ld32(to + 32 * h, o);
+            if (PARTS > 1 && nk > kPpFlush) {
+              const float fm = moved == -INFINITY ? 0.0f : exp2_fast(moved - m);
+              const float4* src = mine + (16 * hf + 8 * h) * kRows;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float4 y = src[i * kRows];
+                o[4 * i] = fmaf(y.x, fm, o[4 * i]);
+                o[4 * i + 1] = fmaf(y.y, fm, o[4 * i + 1]);
+                o[4 * i + 2] = fmaf(y.z, fm, o[4 * i + 2]);
+                o[4 * i + 3] = fmaf(y.w, fm, o[4 * i + 3]);
+              }
+            }
+            if (!whole) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4)
+                mine[(16 * hf + 8 * h + i / 4) * kRows] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+              continue;
+            }
+            constexpr int kChunks = PARTS > 1 ? 8 : 4;  // 16-byte chunks of 32 dims
+            unsigned char* my_row = wq + (wr + lane) * 128;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+              uint4 x;
+              if constexpr (PARTS > 1)
+                x = make_uint4(__float_as_uint(o[4 * c] * f), __float_as_uint(o[4 * c + 1] * f),
+                               __float_as_uint(o[4 * c + 2] * f), __float_as_uint(o[4 * c + 3] * f));
+              else
+                x = make_uint4(pack2<T>(o[8 * c] * f, o[8 * c + 1] * f),
+                               pack2<T>(o[8 * c + 2] * f, o[8 * c + 3] * f),
+                               pack2<T>(o[8 * c + 4] * f, o[8 * c + 5] * f),
+                               pack2<T>(o[8 * c + 6] * f, o[8 * c + 7] * f));
+              *reinterpret_cast<uint4*>(my_row + (((c ^ lane) & 7) << 4)) = x;
+            }
+            __syncwarp();
+            constexpr int kAtOnce = 32 / kChunks;  // rows a step of the warp writes
+#pragma unroll
+            for (int i = 0; i < 32 / kAtOnce; ++i) {
+              const int r = i * kAtOnce + lane / kChunks, c = lane % kChunks;
+              const long long at = __shfl_sync(0xffffffffu, y_at, r);
+              const uint4 x = *reinterpret_cast<const uint4*>(wq + (wr + r) * 128 + (((c ^ r) & 7) << 4));
+              if (at >= 0)
+                *reinterpret_cast<uint4*>(static_cast<unsigned char*>(a.y) +
+                                          (at + 32 * h) * (PARTS > 1 ? 4 : (int)sizeof(T)) + 16 * c) = x;
+            }
+            __syncwarp();
+          }
+        }
+        tc_fence_before();
+        turn ^= (unsigned)nk;
       }
-      tc_fence_before();
-      turn ^= (unsigned)nk;
-    }
-    done += nk;
-    if (nk == 0 && live) {  // no key is visible to any row
-      const long long base = (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf;
-      for (int i = 0; i < kHeadDim / 2; i += 4) store4(a.y, base + i, a.dtype, make_float4(0.f, 0.f, 0.f, 0.f));
-    }
-    work_done(n);
+      done += nk;
+      if (nk == 0 && live) {  // no key is visible to any row
+        const long long base = (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf;
+        for (int i = 0; i < kHeadDim / 2; i += 4) store4(a.y, base + i, a.dtype, make_float4(0.f, 0.f, 0.f, 0.f));
+      }
+      work_done(n);
     }
     tc_fence_before();
     __syncthreads();  // (the other roles' is at their end)
