@@ -947,6 +947,42 @@ def test_prompt_then_decoding_steps_over_one_cache(cache, window):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("io", ["f16", "f32"])
+def test_offsets_beyond_32_bits(io):
+    """Pools of 5.2 GB whose used pages lie at both ends, and rows 4.4 GB apart."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    pages, kvh, page, H = 40000, 8, 64, 16
+    T = _types(torch)[io]
+    k, v = (torch.empty(pages, kvh, page, D, dtype=torch.float16, device="cuda") for _ in "kv")
+    small_k, small_v, small, n = make_cache(torch, [300, 131], page, kvh, "f16")
+    used = torch.unique(small[small >= 0]).long()
+    far = torch.where(used % 2 == 0, pages - 1 - used, used)
+    k[far], v[far] = small_k[used], small_v[used]
+    table = small.clone()
+    for a, b in zip(used.tolist(), far.tolist()):
+        table[small == a] = b
+    wide = (2 ** 32 + 2 ** 28) // T.itemsize          # elements between two rows
+    store = torch.empty(wide + 64 * D, dtype=T, device="cuda")
+    qkv = store.as_strided((2, (H + 2 * kvh) * D), (wide, 1))
+    qkv.copy_(torch.randn(2, (H + 2 * kvh) * D, device="cuda"))
+    near = qkv.clone()
+    want = R.paged_append(near, small_k, small_v, small, n, None, None, H)
+    got = R.paged_append(qkv, k, v, table, n, None, None, H, q_out=qkv[:, :H * D])
+    assert torch.equal(got, want) and torch.equal(k[far], small_k[used]) and torch.equal(v[far], small_v[used])
+    starts = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    y = store.as_strided((2, H, D), (wide, D, 1), (H + 2 * kvh) * D)
+    big = R.paged_attn_decode(got.unflatten(1, (H, D)), k, v, table, n, y=y)
+    assert torch.equal(big, R.paged_attn_decode(want.unflatten(1, (H, D)), small_k, small_v, small, n))
+    big = R.paged_attn_prompt(got.unflatten(1, (H, D)), k, v, table, n, starts, y=y)
+    assert torch.equal(big, R.paged_attn_prompt(want.unflatten(1, (H, D)), small_k, small_v, small, n, starts))
+    u = torch.rand(2, device="cuda")
+    ids, logp = R.sample_rows(qkv, u)
+    want_ids, want_logp = R.sample_rows(qkv.clone(), u)
+    assert torch.equal(ids, want_ids) and torch.equal(logp, want_logp)
+
+
+@pytest.mark.gpu
 def test_a_thread_without_a_cuda_call_before_it():
     torch = _cuda()
     from kernel_optimization_webgpu_b200 import runtime as R
