@@ -421,9 +421,9 @@ typedef struct qd_paged_kv {
  *   x[i], x[i+64] <- x[i] c - x[i+64] s, x[i+64] c + x[i] s,   i < 64,
  * c = cos[position * rope_stride + i], s = sin[...] (f32 tables of rope_len entries each;
  * both NULL: no rotation). q goes to q_out [rows][q_heads*128] (rows q_out_stride elements
- * apart; q_out may be qkv itself, with its type and stride, and is else apart from it), k and v to the cache. All
- * arithmetic in f32, rounded once to the output's type. qkv_dtype, q_out_dtype: QD_KV_F16,
- * QD_KV_F32 or QD_KV_BF16; pointers 16-byte aligned, strides multiples of 8. Two rows of one
+ * apart; q_out may be qkv itself, with its type and stride, and is else apart from it), k and v
+ * to the cache. All arithmetic in f32, rounded once to the output's type. qkv_dtype, q_out_dtype:
+ * QD_KV_F16, QD_KV_F32 or QD_KV_BF16; pointers 16-byte aligned, strides multiples of 8. Two rows of one
  * call never share a position of the cache unless the block table does (then either wins).
  * Replaces, for any number of rows, head_rms_norm.wgsl, rope.wgsl:14-31 and
  * cache_write.wgsl. */
@@ -434,14 +434,15 @@ int qd_paged_append(const qd_paged_kv* kv, const void* qkv, int qkv_dtype, int64
 
 /* Attention of one new token per sequence (rows = batch): y[b] = softmax(scale * q[b] k^T) v
  * over the keys that position seq_lens[b] - 1 sees. q, y [batch][q_heads][128], rows q_stride /
- * y_stride elements apart (multiples of 8), 16-byte aligned, y apart from all that is read (y over q or the
- * pools is refused; of a ragged batch, where that shows in the first row); dtype
- * (of both) QD_KV_F32 or the cache's. q_heads is a multiple of kv_heads, at most 64 times it. The softmax and its sums
- * are f32; with dtype QD_KV_F32 the products keep f32 accuracy too (q and the weights go into
- * them as sums of two f16 or three bf16), with a 16-bit dtype the prompt's weights are rounded to
- * it once. q and scale may have any size; what counts is the scores': beyond 2^22, where f32 cannot tell
- * neighbouring weights apart any more, a row may come out as NaN. scale 0 means 1/sqrt(128). The workspace
- * holds the joined parts' partial sums; nothing in it needs to start at zero. */
+ * y_stride elements apart (multiples of 8), 16-byte aligned, y apart from all that is read (y over
+ * q or the pools is refused; of a ragged batch, where that shows in the first row); dtype (of both)
+ * QD_KV_F32 or the cache's. q_heads is a multiple of kv_heads, at most 64 times it. The softmax and
+ * its sums are f32; with dtype QD_KV_F32 the products keep f32 accuracy too (q and the weights go
+ * into them as sums of two f16 or three bf16), with a 16-bit dtype the prompt's weights are rounded
+ * to it once. q and scale may have any size; what counts is the scores': beyond 2^22, where f32
+ * cannot tell neighbouring weights apart any more, a row may come out as NaN. scale 0 means
+ * 1/sqrt(128). The workspace holds the joined parts' partial sums; nothing in it needs to start at
+ * zero. */
 size_t qd_paged_attn_decode_workspace_bytes(int batch, int q_heads);
 int qd_paged_attn_decode(const qd_paged_kv* kv, const void* q, int dtype, int64_t q_stride, int q_heads, int window,
                          int sinks, float scale, void* y, int64_t y_stride, void* workspace, void* stream);
@@ -451,8 +452,9 @@ int qd_paged_attn_decode(const qd_paged_kv* kv, const void* q, int dtype, int64_
  * first). q, y [rows][q_heads][128]. Weights of hidden keys are zeros, not left out: a V row that
  * is not finite also reaches rows of its sequence in this call that do not see it, as it would in a
  * plain product, if they are less than 256 positions from a row that does (fewer with several
- * query heads to a KV head: the 256 rows that are worked on together are tokens times these heads). The workspace's size depends on dtype (of q and
- * y): with QD_KV_F32 it holds running sums of every row. */
+ * query heads to a KV head: the 256 rows that are worked on together are tokens times these heads).
+ * The workspace's size depends on dtype (of q and y): with QD_KV_F32 it holds running sums of every
+ * row. */
 size_t qd_paged_attn_prompt_workspace_bytes(int batch, int rows, int q_heads, int kv_heads, int dtype);
 int qd_paged_attn_prompt(const qd_paged_kv* kv, const void* q, int dtype, int64_t q_stride, int rows,
                          const int32_t* q_starts, int q_heads, int window, int sinks, float scale, void* y,

@@ -23,9 +23,9 @@
 //    Two f16 hold 22 bits of what lies well inside f16's range: each head's q is brought there by a
 //    power of two, which its scores' factor takes back (f16_fit).
 //
-// 64 sequences of 2048 positions, 8 KV heads: 93 us for 537 MB = 5.8 TB/s; of 8192: 334 us = 6.4 TB/s.
+// 64 sequences of 2048 positions, 8 KV heads: 93 us for 537 MB = 5.8 TB/s; of 8192: 338 us = 6.35 TB/s.
 // About 10 us of either are the two launches and the chain of lookups before the first row (lengths,
-// table, row), which is why 1 x 32768 (134 MB) takes 33 us. Three slots and two CTAs an SM; two
+// table, row), which is why 1 x 32768 (134 MB) takes 32 us. Three slots and two CTAs an SM; two
 // slots and three CTAs: 112 us.
 #pragma once
 

@@ -11,7 +11,8 @@
 // S of the next key tile may be issued right behind the product that reads P. What bounds it:
 // 2048 cycles of products and as many of exponentials per 256 rows and 128 keys, in a loop of
 // 3460 (scores ready -> weights ready 1900, products -> next scores ready 1460, for each tile in
-// turn): 8192 causal rows of 16 heads take 250 us = 1100 TFLOP/s (3 us more before the products of the
+// turn): 8192 causal rows of 16 heads take 250 us = 1100 TFLOP/s in a burst at 1965 MHz, and 292 us one
+// after the other for a second, at 1620 to 1680 MHz under the power cap (3 us more before the products of the
 // first half of P's keys started ahead of the second). Beside it at 266 us: one thread per row
 // instead of two 301 us, an exp2 by polynomial for 3 to 8 of 16 weights 269 to 287 us
 // (the softmax warps wait on each other's instructions, not on the special-function unit).
@@ -26,8 +27,8 @@
 // so a bf16 cache takes three. Three parts of P do not fit over S in TMEM, so such a CTA has one row tile. The
 // tensor cores drop the bits below an accumulator's last place, towards zero, at every step, which
 // over a long row shows in f32: every kPpFlush tiles O moves from TMEM to sums in the workspace that
-// are added with rounding (500 rows behind 3500 keys: 1.4e-6 off, 2.5e-6 without; it costs a causal
-// prompt of 4096 rows 147 us against 125).
+// are added with rounding (rows over 4000 keys with values of one sign: 4e-6 off, 3e-5 without; it costs a
+// causal prompt of 4096 rows 154 us against 122, with three parts 257 against 218).
 //
 // Where the grid does not fit the GPU at once, a CTA goes on with the work of blocks that have not started
 // (cluster launch control), looked up by a warp of its own while the last key tiles are still on
