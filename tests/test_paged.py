@@ -404,6 +404,28 @@ def test_bad_pages_and_lengths_are_left_out_and_flagged():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("io,cache", [("f32", "f16"), ("f16", "f16"), ("bf16", "bf16"), ("f32", "bf16")])
+@pytest.mark.parametrize("pages", [0, 4])
+def test_sequences_without_a_single_usable_page(io, cache, pages):
+    """No pool, or entries that name no page of it: zeros, flagged, and nothing is written."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    T = _types(torch)
+    k, v = (torch.full((pages, 2, 64, D), math.nan, dtype=T[cache], device="cuda") for _ in "kv")
+    table = torch.full((2, 3), pages, dtype=torch.int32, device="cuda")
+    n = torch.tensor([150, 2], dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0, 140, 142], dtype=torch.int32, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    q = torch.randn(142, 4, D, device="cuda").to(T[io])
+    for call in (lambda: R.paged_attn_prompt(q, k, v, table, n, starts, status=status),
+                 lambda: R.paged_attn_decode(q[:2], k, v, table, n, status=status)):
+        assert bool((call() == 0).all()) and int(status) == _lib.QD_PAGED_BAD_PAGE
+        status.zero_()
+    R.paged_append(torch.randn(142, 8 * D, device="cuda"), k, v, table, n, None, None, 4, q_starts=starts, status=status)
+    assert int(status) == _lib.QD_PAGED_BAD_PAGE and bool(torch.isnan(k).all()) and bool(torch.isnan(v).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("length,bits", [(0, 0), (-1, _lib.QD_PAGED_BAD_LENGTH), (-2 ** 31, _lib.QD_PAGED_BAD_LENGTH),
                                          (2, _lib.QD_PAGED_BAD_LENGTH), (3, 0), (40, 0), (48, 0),
                                          (49, _lib.QD_PAGED_BAD_LENGTH), (2 ** 31 - 1, _lib.QD_PAGED_BAD_LENGTH)])
