@@ -460,6 +460,66 @@ int qd_paged_attn_prompt(const qd_paged_kv* kv, const void* q, int dtype, int64_
                          const int32_t* q_starts, int q_heads, int window, int sinks, float scale, void* y,
                          int64_t y_stride, void* workspace, void* stream);
 
+/* Decode attention of groups of sequences that share their first positions (several answers to one
+ * prompt, say): group i is the sequences group_starts[i] .. group_starts[i + 1] - 1 (groups + 1
+ * ascending device entries from 0; sequences from group_starts[groups] on are padding: their rows of y are left as
+ * they were). Sequence b sees
+ * its first shared_lens[b] positions (device, [batch]; at most seq_lens[b] count, negative: none)
+ * through the block table's row of its group's first sequence, the others through its own row;
+ * only the pages that it uses so are looked up. Otherwise as
+ * qd_paged_attn_decode without a window, whose results these are to rounding where the table's
+ * rows agree; the shared positions are read once per group. groups: 0..batch. (Weights of
+ * positions that a sequence does not see but others of its group do are zeros, not left out: a V row
+ * among them that is not finite reaches it, as in qd_paged_attn_prompt.) A device-side wait that
+ * expires makes rows NaN and sets QD_PAGED_TIMEOUT. */
+size_t qd_paged_attn_decode_shared_workspace_bytes(int batch, int groups, int q_heads, int kv_heads);
+int qd_paged_attn_decode_shared(const qd_paged_kv* kv, const void* q, int dtype, int64_t q_stride, int q_heads,
+                                int groups, const int32_t* group_starts, const int32_t* shared_lens, float scale,
+                                void* y, int64_t y_stride, void* workspace, void* stream);
+
+/* ---- the same cache in 8 bits ------------------------------------------------------
+ * Rows of 128 8-bit integers with one f32 scale each: element i stands for n[i] * scale. 132
+ * bytes a row against 256. The block table, lengths and status as in qd_paged_kv. */
+typedef struct qd_paged_q8 {
+  int8_t* k;                    /* [num_pages][kv_heads][page_size][head_dim], 16-byte aligned */
+  int8_t* v;
+  float* k_scale;               /* [num_pages][kv_heads][page_size], 16-byte aligned, not negative */
+  float* v_scale;
+  int num_pages;
+  int page_size;                /* a power of two, 16..256 */
+  int kv_heads;
+  int head_dim;                 /* 128 */
+  int batch;                    /* sequences, 0..4096 */
+  const int32_t* block_table;   /* [batch][table_stride], table_width entries of each row used */
+  int table_width, table_stride;
+  const int32_t* seq_lens;      /* [batch]: positions held, the new tokens included */
+  int32_t* status;              /* device word of QD_PAGED_* bits, or NULL */
+} qd_paged_q8;
+
+/* qd_paged_append into such a cache: what it would write of a K or V row x (in f32) is written as
+ * scale = max|x| / 127 and n = x / scale rounded to the nearest integer, -127..127. A row with an
+ * element that is not finite gets a NaN scale, one whose largest magnitude is below 2^-100 a
+ * scale of 0 and zeros. */
+int qd_paged_append_q8(const qd_paged_q8* kv, const void* qkv, int qkv_dtype, int64_t qkv_stride, int rows,
+                       const int32_t* q_starts, int q_heads, const float* q_norm, const float* k_norm, float eps,
+                       const float* cos, const float* sin, int64_t rope_len, int64_t rope_stride, void* q_out,
+                       int q_out_dtype, int64_t q_out_stride, void* stream);
+
+/* Positions first[b] .. seq_lens[b] - 1 of every sequence (first: device, [batch]; NULL or
+ * negative: from 0) read back into the pages of a 16-bit cache, n * scale rounded once to its
+ * type: position p goes to page to->block_table[b][p / to->page_size]. qd_paged_attn_prompt can
+ * then run over `to`. Both caches have the same batch and kv_heads; page sizes may differ;
+ * to->seq_lens and to->status are not used. No other row of `to` is written. A bad page of either (its
+ * positions are left out) and a length beyond either table (cut) set the bits in *kv->status. */
+int qd_paged_read_q8(const qd_paged_q8* kv, const int32_t* first, const qd_paged_kv* to, void* stream);
+
+/* qd_paged_attn_decode over such a cache; dtype (of q and y) is QD_KV_F32, QD_KV_F16 or
+ * QD_KV_BF16. The products keep f32 accuracy for every dtype (the integers are exact operands; q and
+ * the weights are sums of two f16, the weights times V's scales with a common exponent of their own). The
+ * workspace is qd_paged_attn_decode_workspace_bytes(batch, q_heads). */
+int qd_paged_attn_decode_q8(const qd_paged_q8* kv, const void* q, int dtype, int64_t q_stride, int q_heads, int window,
+                            int sinks, float scale, void* y, int64_t y_stride, void* workspace, void* stream);
+
 /* ---- sampling of a batch of rows -------------------------------------------------- */
 
 /* One token per row of logits [rows][vocab] (device, dtype QD_KV_F32 / F16 / BF16, rows
@@ -483,6 +543,19 @@ int qd_paged_attn_prompt(const qd_paged_kv* kv, const void* q, int dtype, int64_
 int qd_sample_rows(const void* logits, int dtype, int rows, uint32_t vocab, int64_t row_stride,
                    const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                    const float* u, int32_t* ids, float* logprobs, void* stream);
+
+/* What a softmax over each row of logits [rows][vocab] (device, dtype QD_KV_F32 / F16 / BF16,
+ * rows row_stride elements apart) says, with p = softmax(row):
+ *  - logprobs[r] = log p[tokens[r]] (tokens: device int32; NaN for one outside [0, vocab));
+ *  - entropy[r] (NULL: left out) = -sum p log p, 0 log 0 = 0;
+ *  - top_ids[r][top], top_logprobs[r][top] (contiguous; top 0..64, at most vocab): the `top` first
+ *    tokens in the order of qd_sample_rows (by value, ties to the lower index, NaN last) and their
+ *    logarithms.
+ * Sums are f32. -inf is a token of probability 0 (logarithm -inf). A row that holds NaN or +inf,
+ * or -inf only, has no softmax: its logprobs and entropy are NaN (top_ids is by the order all the
+ * same). Enqueues only; needs no workspace. */
+int qd_score_rows(const void* logits, int dtype, int rows, uint32_t vocab, int64_t row_stride, const int32_t* tokens,
+                  int top, float* logprobs, float* entropy, int32_t* top_ids, float* top_logprobs, void* stream);
 
 #ifdef __cplusplus
 }

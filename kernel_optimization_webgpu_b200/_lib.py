@@ -45,6 +45,8 @@ EXPORTS = (
     "qd_paged_append", "qd_paged_attn_decode_workspace_bytes", "qd_paged_attn_decode",
     "qd_paged_attn_prompt_workspace_bytes", "qd_paged_attn_prompt", "qd_sample_rows",
     "qd_paged_inject_stall",
+    "qd_paged_append_q8", "qd_paged_read_q8", "qd_paged_attn_decode_q8",
+    "qd_paged_attn_decode_shared_workspace_bytes", "qd_paged_attn_decode_shared", "qd_score_rows",
 )
 
 
@@ -74,6 +76,13 @@ class QdPagedKv(C.Structure):
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int), ("num_pages", C.c_int),
                 ("page_size", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("batch", C.c_int),
                 ("block_table", C.c_void_p), ("table_width", C.c_int), ("table_stride", C.c_int),
+                ("seq_lens", C.c_void_p), ("status", C.c_void_p)]
+
+
+class QdPagedQ8(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("num_pages", C.c_int), ("page_size", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("batch", C.c_int), ("block_table", C.c_void_p), ("table_width", C.c_int), ("table_stride", C.c_int),
                 ("seq_lens", C.c_void_p), ("status", C.c_void_p)]
 
 
@@ -227,6 +236,19 @@ def load(build_if_stale: bool = True):
     L.qd_paged_inject_stall.restype = None
     L.qd_sample_rows.argtypes = [vp, i32, i32, u32, i64, vp, vp, vp, vp, vp, vp, vp, vp]
     L.qd_sample_rows.restype = i32
+    q8 = C.POINTER(QdPagedQ8)
+    L.qd_paged_append_q8.argtypes = [q8, *L.qd_paged_append.argtypes[1:]]
+    L.qd_paged_append_q8.restype = i32
+    L.qd_paged_read_q8.argtypes = [q8, vp, kv, vp]
+    L.qd_paged_read_q8.restype = i32
+    L.qd_paged_attn_decode_q8.argtypes = [q8, *L.qd_paged_attn_decode.argtypes[1:]]
+    L.qd_paged_attn_decode_q8.restype = i32
+    L.qd_paged_attn_decode_shared_workspace_bytes.argtypes = [i32, i32, i32, i32]
+    L.qd_paged_attn_decode_shared_workspace_bytes.restype = C.c_size_t
+    L.qd_paged_attn_decode_shared.argtypes = [kv, vp, i32, i64, i32, i32, vp, vp, f32, vp, i64, vp, vp]
+    L.qd_paged_attn_decode_shared.restype = i32
+    L.qd_score_rows.argtypes = [vp, i32, i32, u32, i64, vp, i32, vp, vp, vp, vp, vp]
+    L.qd_score_rows.restype = i32
     L.qd_run_kernel_benchmarks.argtypes = [vp, C.POINTER(QdKernelBench)]
     L.qd_run_kernel_benchmarks.restype = i32
     L.qd_run_full_decoder_stack_benchmark.argtypes = [vp, C.POINTER(QdStackBench)]

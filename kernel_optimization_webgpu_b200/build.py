@@ -20,8 +20,9 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libqdecode.so")
-SOURCES = ["engine.cu", "batch.cu", "noalloc.cu", "bench_api.cu", "sample.cu", "paged.cu", "sample_rows.cu"]
-DEPS = SOURCES + ["kernels.cuh", "persist.cuh", "gemm_tc.cuh", "batch.cuh", "paged.cuh", "paged_decode.cuh", "paged_prompt.cuh", "internal.cuh", "overlap.hpp", "tma.cuh", "common.cuh", "json.hpp"]
+SOURCES = ["engine.cu", "batch.cu", "noalloc.cu", "bench_api.cu", "sample.cu", "paged.cu", "sample_rows.cu",
+           "score_rows.cu"]
+DEPS = SOURCES + ["kernels.cuh", "persist.cuh", "gemm_tc.cuh", "batch.cuh", "paged.cuh", "paged_decode.cuh", "paged_prompt.cuh", "paged_q8.cuh", "paged_shared.cuh", "rows.cuh", "internal.cuh", "overlap.hpp", "tma.cuh", "common.cuh", "json.hpp"]
 CALLS = os.path.join(PKG, "_torch_calls.so")
 CALLS_SOURCE = "torch_calls.cpp"
 CALLS_KEY = os.path.join(PKG, "_build", "torch_calls.key")  # what the module on disk was built from

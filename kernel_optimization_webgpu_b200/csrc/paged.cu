@@ -9,6 +9,8 @@
 #include "paged.cuh"
 #include "paged_decode.cuh"
 #include "paged_prompt.cuh"
+#include "paged_q8.cuh"
+#include "paged_shared.cuh"
 
 namespace qd {
 
@@ -58,13 +60,30 @@ static PagedArgs check_paged(const qd_paged_kv* kv) {
   return a;
 }
 
+static PagedArgs check_q8(const qd_paged_q8* kv) {
+  need(kv != nullptr, "paged cache: NULL pointer");
+  const qd_paged_kv same{kv->k, kv->v, QD_KV_F16, kv->num_pages, kv->page_size, kv->kv_heads, kv->head_dim, kv->batch,
+                         kv->block_table, kv->table_width, kv->table_stride, kv->seq_lens, kv->status};
+  const PagedArgs a = check_paged(&same);
+  need(kv->num_pages == 0 || (kv->k_scale && kv->v_scale), "paged cache: NULL scales");
+  need(aligned16(kv->k_scale) && aligned16(kv->v_scale), "paged cache: scales must be 16-byte aligned");
+  return a;
+}
+static void need_apart_from_q8(const qd_paged_q8* kv, const Rows& x, const char* msg) {
+  const int64_t rows = (int64_t)kv->num_pages * kv->kv_heads * kv->page_size;
+  for (const void* pool : {kv->k, kv->v}) need(apart(x, Rows{pool, 1, rows * kHeadDim, rows * kHeadDim}), msg);
+  for (const void* scales : {kv->k_scale, kv->v_scale}) need(apart(x, Rows{scales, 1, rows * 4, rows * 4}), msg);
+}
+
 static PAttnArgs check_attn(const qd_paged_kv* kv, const void* q, int dtype, int64_t q_stride, int rows, int q_heads,
-                            int window, int sinks, float scale, void* y, int64_t y_stride, int sure) {
+                            int window, int sinks, float scale, void* y, int64_t y_stride, int sure,
+                            const qd_paged_q8* q8 = nullptr) {
   PAttnArgs a{};
-  a.kv = check_paged(kv);
+  a.kv = q8 ? check_q8(q8) : check_paged(kv);
   need(rows >= 0, "paged attention: negative rows");
-  need(dtype == QD_KV_F32 || dtype == kv->dtype, "paged attention: q and y are QD_KV_F32 or of the cache's dtype");
-  need(q_heads >= 1 && q_heads % kv->kv_heads == 0 && q_heads / kv->kv_heads <= 64,
+  need(q8 ? known_dtype(dtype) : dtype == QD_KV_F32 || dtype == kv->dtype,
+       q8 ? "paged attention: unknown dtype" : "paged attention: q and y are QD_KV_F32 or of the cache's dtype");
+  need(q_heads >= 1 && q_heads % a.kv.kv_heads == 0 && q_heads / a.kv.kv_heads <= 64,
        "paged attention: q_heads must be a multiple of kv_heads, at most 64 times it");
   need(window >= 0 && sinks >= 0, "paged attention: window and sinks must not be negative");
   need(std::isfinite(scale), "paged attention: scale must be finite");
@@ -76,7 +95,8 @@ static PAttnArgs check_attn(const qd_paged_kv* kv, const void* q, int dtype, int
   // (several CTAs read a row of q, and one of them may be done first)
   const Rows out = rows_of(y, dtype, sure, (int64_t)q_heads * kHeadDim, y_stride);
   need(apart(out, rows_of(q, dtype, sure, (int64_t)q_heads * kHeadDim, q_stride)), "paged attention: y overlaps q");
-  need_apart_from_pools(kv, out, "paged attention: y overlaps the pools");
+  if (q8) need_apart_from_q8(q8, out, "paged attention: y overlaps the pools");
+  else need_apart_from_pools(kv, out, "paged attention: y overlaps the pools");
   a.q = q;
   a.q_stride = q_stride;
   a.rows = rows;
@@ -90,14 +110,75 @@ static PAttnArgs check_attn(const qd_paged_kv* kv, const void* q, int dtype, int
   return a;
 }
 
-template <int HEADS>
+template <int HEADS, bool Q8>
 static void launch_append(const AppendArgs& a, int qkv_dtype, long long heads, cudaStream_t s) {
   const long long warps = a.rows * ((heads + HEADS - 1) / HEADS);
   need(warps <= 0x7fffffffLL, "qd_paged_append: too many rows");
   const dim3 grid((unsigned)((warps + 7) / 8)), block(256);
-  if (qkv_dtype == QD_KV_F32) launch_ex(k_paged_append<float, HEADS>, grid, block, 0, s, a);
-  else if (qkv_dtype == QD_KV_F16) launch_ex(k_paged_append<__half, HEADS>, grid, block, 0, s, a);
-  else launch_ex(k_paged_append<__nv_bfloat16, HEADS>, grid, block, 0, s, a);
+  if (qkv_dtype == QD_KV_F32) launch_ex(k_paged_append<float, HEADS, Q8>, grid, block, 0, s, a);
+  else if (qkv_dtype == QD_KV_F16) launch_ex(k_paged_append<__half, HEADS, Q8>, grid, block, 0, s, a);
+  else launch_ex(k_paged_append<__nv_bfloat16, HEADS, Q8>, grid, block, 0, s, a);
+}
+
+// The append calls, over a checked cache; need_apart refuses rows that lie over it.
+struct Scales {
+  float *k, *v;
+};
+template <bool Q8, typename F>
+static void append(const PagedArgs& kv, int kv_dtype, Scales scales, F&& need_apart, const void* qkv, int qkv_dtype,
+                   int64_t qkv_stride, int rows, const int32_t* q_starts, int q_heads, const float* q_norm,
+                   const float* k_norm, float eps, const float* cos, const float* sin, int64_t rope_len,
+                   int64_t rope_stride, void* q_out, int q_out_dtype, int64_t q_out_stride, void* stream) {
+  need(rows >= 0, "qd_paged_append: negative rows");
+  need(q_starts || rows == kv.batch, "qd_paged_append: without q_starts rows must equal the batch");
+  need(known_dtype(qkv_dtype) && known_dtype(q_out_dtype), "qd_paged_append: unknown dtype");
+  need(q_heads >= 0 && q_heads <= 65536, "qd_paged_append: bad q_heads");
+  const int64_t heads = (int64_t)q_heads + 2 * kv.kv_heads;
+  need(qkv_stride >= heads * kHeadDim && qkv_stride % 8 == 0,
+       "qd_paged_append: qkv_stride must be a multiple of 8, at least (q_heads + 2 kv_heads) * 128");
+  need(q_heads == 0 || (q_out_stride >= (int64_t)q_heads * kHeadDim && q_out_stride % 8 == 0),
+       "qd_paged_append: q_out_stride must be a multiple of 8, at least q_heads * 128");
+  need(std::isfinite(eps) && eps >= 0.0f, "qd_paged_append: eps must be finite and not negative");
+  need((cos == nullptr) == (sin == nullptr), "qd_paged_append: cos and sin go together");
+  need(!cos || (rope_len >= 0 && rope_stride >= 0 && rope_stride % 4 == 0),
+       "qd_paged_append: rope_stride must be a multiple of 4, not negative");
+  need(rows == 0 || (qkv && (q_out || q_heads == 0)), "qd_paged_append: NULL pointer");
+  need(aligned16(qkv) && aligned16(q_out) && aligned16(cos) && aligned16(sin) && aligned16(q_norm) &&
+           aligned16(k_norm),
+       "qd_paged_append: pointers must be 16-byte aligned");
+  const int sure = q_starts ? std::min(rows, 1) : rows;
+  const Rows in = rows_of(qkv, qkv_dtype, sure, heads * kHeadDim, qkv_stride);
+  const Rows out = rows_of(q_out, q_out_dtype, sure, (int64_t)q_heads * kHeadDim, q_out_stride);
+  const bool in_place = q_out == qkv && q_out_dtype == qkv_dtype && (q_out_stride == qkv_stride || rows == 1);
+  need(in_place || apart(out, in),
+       "qd_paged_append: q_out overlaps qkv (it may be qkv itself, with its type and stride)");
+  need_apart(out, "qd_paged_append: q_out overlaps the pools");
+  need_apart(in, "qd_paged_append: qkv overlaps the pools");
+  if (rows == 0 || kv.batch == 0) return;
+  AppendArgs a{};
+  a.kv = kv;
+  a.kv_dtype = kv_dtype;
+  a.k_scale = scales.k;
+  a.v_scale = scales.v;
+  a.qkv = qkv;
+  a.qkv_stride = qkv_stride;
+  a.rows = rows;
+  a.q_starts = q_starts;
+  a.q_heads = q_heads;
+  a.q_norm = q_norm;
+  a.k_norm = k_norm;
+  a.eps = eps;
+  a.cos_t = cos;
+  a.sin_t = sin;
+  a.rope_len = rope_len;
+  a.rope_stride = rope_stride;
+  a.q_out = q_out;
+  a.q_out_dtype = q_out_dtype;
+  a.q_out_stride = q_out_stride;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  // four heads a warp once that gives every SM four CTAs, else two
+  if (rows * ((heads + 3) / 4) >= 32LL * current_sms()) launch_append<4, Q8>(a, qkv_dtype, heads, s);
+  else launch_append<2, Q8>(a, qkv_dtype, heads, s);
 }
 
 template <typename T, bool THREE>
@@ -115,6 +196,20 @@ static void launch_decode(const PAttnArgs& a, void* workspace, cudaStream_t s) {
     launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas);
 }
 
+static void launch_decode_q8(const PAttnArgs& a, PagedScales scale, void* workspace, cudaStream_t s) {
+  const int nh = a.kv.kv_heads * ((a.q_heads / a.kv.kv_heads + 7) / 8);
+  const long long most = (long long)a.kv.batch * nh * (((long long)a.kv.table_width << a.kv.page_shift) / kQ8Tile + 1);
+  if (most > 0x7fffffffLL)
+    throw QdError{QD_E_RANGE, "qd_paged_attn_decode_q8: batch * heads * table beyond 2^31 units"};
+  static unsigned long long smem_set = 0;
+  allow_smem(k_paged_decode_q8, pq8_smem(4096), smem_set);
+  const int ctas = (int)std::max(1LL, std::min<long long>(most, std::min(2 * current_sms(), kPdMaxCtas)));
+  launch_ex(k_paged_decode_q8, dim3(ctas), dim3(kPdThreads), (size_t)pq8_smem(a.kv.batch), s, a, scale, workspace);
+  // (a table of one unit leaves nothing to join)
+  if ((a.kv.table_width << a.kv.page_shift) > kQ8Tile)
+    launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas);
+}
+
 // Row tiles of a call (at most), and the parts that their keys are split into: enough to give
 // every SM a CTA, none where the row tiles alone do.
 static int prompt_items(int batch, int rows, int group, int cta_rows) {
@@ -126,6 +221,25 @@ static int prompt_splits(int items, int kv_heads) {
 }
 
 static thread_local bool stall_next = false;  // qd_paged_inject_stall
+
+template <typename T>
+static void pool_maps(PPromptArgs& p, const void* any, const char* too_large) {
+  const PagedArgs& kv = p.a.kv;
+  const CUtensorMapDataType type =
+      std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const unsigned box = std::min(1 << kv.page_shift, kPpKeys);
+  // (an empty pool has no page that could be copied: any address will do)
+  const uint64_t pool = std::max<uint64_t>((uint64_t)kv.num_pages * kv.kv_heads << kv.page_shift, box);
+  if (pool > 0x7fffffffULL) throw QdError{QD_E_RANGE, too_large};
+  std::string err;
+  if (!make_tmap_2d(&p.tk, kv.num_pages ? kv.k : any, type, kHeadDim, pool, kHeadDim * 2, 64, box,
+                    CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
+      !make_tmap_2d(&p.tv, kv.num_pages ? kv.v : any, type, kHeadDim, pool, kHeadDim * 2, 64, box,
+                    CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
+      !make_tmap_2d(&p.tv16, kv.num_pages ? kv.v : any, type, kHeadDim, pool, kHeadDim * 2, 64, 16,
+                    CU_TENSOR_MAP_SWIZZLE_128B, &err))
+    throw QdError{QD_E_CUDA, err};
+}
 
 template <typename T, int PARTS>
 static void launch_prompt(const PAttnArgs& a, const void* q_any, void* workspace, cudaStream_t s) {
@@ -144,20 +258,7 @@ static void launch_prompt(const PAttnArgs& a, const void* q_any, void* workspace
   p.splits = (int)std::max(1LL, std::min<long long>(p.splits, tiles / 2));
   const long long grid = (long long)items * a.kv.kv_heads * p.splits;
   if (grid * 32 > 0x7fffffffLL) throw QdError{QD_E_RANGE, "qd_paged_attn_prompt: too many rows"};
-  const CUtensorMapDataType type =
-      std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const unsigned box = std::min(1 << a.kv.page_shift, kPpKeys);
-  // (an empty pool has no page that could be copied: any address will do)
-  const uint64_t pool = std::max<uint64_t>((uint64_t)a.kv.num_pages * a.kv.kv_heads << a.kv.page_shift, box);
-  if (pool > 0x7fffffffULL) throw QdError{QD_E_RANGE, "qd_paged_attn_prompt: a pool beyond 2^31 rows"};
-  std::string err;
-  if (!make_tmap_2d(&p.tk, a.kv.num_pages ? a.kv.k : q_any, type, kHeadDim, pool, kHeadDim * 2, 64, box,
-                    CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
-      !make_tmap_2d(&p.tv, a.kv.num_pages ? a.kv.v : q_any, type, kHeadDim, pool, kHeadDim * 2, 64, box,
-                    CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
-      !make_tmap_2d(&p.tv16, a.kv.num_pages ? a.kv.v : q_any, type, kHeadDim, pool, kHeadDim * 2, 64, 16,
-                    CU_TENSOR_MAP_SWIZZLE_128B, &err))
-    throw QdError{QD_E_CUDA, err};
+  pool_maps<T>(p, q_any, "qd_paged_attn_prompt: a pool beyond 2^31 rows");
   // More blocks than SMs: they take each other's work (5 ragged chunks in 480 blocks 109 -> 98 us; a prompt of
   // 8 rows, whose blocks have nothing to take, 9.6 us without that and 10.8 with it).
   static unsigned long long smem_set[2] = {};
@@ -166,6 +267,75 @@ static void launch_prompt(const PAttnArgs& a, const void* q_any, void* workspace
   allow_smem(kernel, pp_smem<PARTS>(), smem_set[claim]);
   launch_ex(kernel, dim3((unsigned)grid), dim3(kPpThreads), (size_t)pp_smem<PARTS>(), s, p);
   if (p.splits > 1) launch_ex(k_paged_prompt_join, dim3(items * a.kv.kv_heads * (kRows / 8)), dim3(256), 0, s, p);
+}
+
+// Attention over shared prefixes: its workspace is the sums of both kinds of positions.
+struct SharedWs {
+  size_t po, pml, rows, tail_o, tail_ml, decode, bytes;
+};
+static SharedWs shared_ws(int batch, int groups, int q_heads, int kv_heads, int cta_rows) {
+  const int G = q_heads / kv_heads, items = prompt_items(groups, batch, G, cta_rows);
+  const size_t rows = (size_t)items * kv_heads * prompt_splits(items, kv_heads) * cta_rows;
+  SharedWs w{};
+  const auto take = [&](size_t n) {
+    const size_t at = w.bytes;
+    w.bytes += (n + 255) / 256 * 256;
+    return at;
+  };
+  w.po = take(rows * kHeadDim * 4);
+  w.pml = take(rows * 8);
+  w.rows = take((size_t)batch * G * 8);
+  w.tail_o = take((size_t)batch * q_heads * kHeadDim * 4);
+  w.tail_ml = take((size_t)batch * q_heads * 8);
+  w.decode = take(pd_ws_bytes(batch));
+  return w;
+}
+
+template <typename T, int PARTS>
+static void launch_shared(const PAttnArgs& a, void* workspace, cudaStream_t s) {
+  constexpr int kRows = 128 * pp_tiles<PARTS>();
+  const int B = a.kv.batch, kvh = a.kv.kv_heads, G = a.q_heads / kvh, subs = (G + 7) / 8;
+  const long long most = (long long)B * kvh * subs * (((long long)a.kv.table_width << a.kv.page_shift) / kPdTile + 1);
+  if (most > 0x7fffffffLL)
+    throw QdError{QD_E_RANGE, "qd_paged_attn_decode_shared: batch * heads * table beyond 2^31 units"};
+  const SharedWs w = shared_ws(B, a.groups, a.q_heads, kvh, kRows);
+  char* base = static_cast<char*>(workspace);
+  PPromptArgs p{};
+  p.a = a;
+  p.a.kv.batch = a.groups;
+  p.cta_rows = kRows;
+  const int items = prompt_items(a.groups, B, G, kRows);
+  p.splits = prompt_splits(items, kvh);
+  p.po = reinterpret_cast<float4*>(base + w.po);
+  p.pml = reinterpret_cast<float2*>(base + w.pml);
+  p.rows = reinterpret_cast<int2*>(base + w.rows);
+  const long long grid = (long long)items * kvh * p.splits;
+  if (grid * 32 > 0x7fffffffLL) throw QdError{QD_E_RANGE, "qd_paged_attn_decode_shared: too many rows"};
+  pool_maps<T>(p, a.q, "qd_paged_attn_decode_shared: a pool beyond 2^31 rows");
+  if (grid > 0) {
+    static unsigned long long smem_set[2] = {};
+    const bool claim = grid > current_sms();
+    auto kernel = claim ? k_paged_prompt<T, PARTS, true, true> : k_paged_prompt<T, PARTS, false, true>;
+    allow_smem(kernel, pp_smem<PARTS>(), smem_set[claim]);
+    launch_ex(kernel, dim3((unsigned)grid), dim3(kPpThreads), (size_t)pp_smem<PARTS>(), s, p);
+  }
+  PSharedArgs j{};
+  j.a = a;
+  j.a.tail_o = reinterpret_cast<float*>(base + w.tail_o);
+  j.a.tail_ml = reinterpret_cast<float2*>(base + w.tail_ml);
+  j.po = p.po;
+  j.pml = p.pml;
+  j.rows = p.rows;
+  j.splits = p.splits;
+  j.cta_rows = kRows;
+  j.all_rows = items * kRows;
+  j.decode_ws = base + w.decode;
+  j.ctas = (int)std::max(1LL, std::min<long long>(most, std::min(2 * current_sms(), kPdMaxCtas)));
+  static unsigned long long smem_set = 0;
+  allow_smem(k_paged_decode<T, PARTS == 3, true>, pd_smem(4096), smem_set);
+  launch_ex(k_paged_decode<T, PARTS == 3, true>, dim3(j.ctas), dim3(kPdThreads), (size_t)pd_smem(B), s, j.a,
+            (void*)j.decode_ws);
+  launch_ex(k_paged_shared_join, dim3((B * G + 7) / 8, kvh), dim3(256), 0, s, j);
 }
 
 }  // namespace qd
@@ -194,54 +364,51 @@ int qd_paged_append(const qd_paged_kv* kv, const void* qkv, int qkv_dtype, int64
                     const float* cos, const float* sin, int64_t rope_len, int64_t rope_stride, void* q_out,
                     int q_out_dtype, int64_t q_out_stride, void* stream) {
   return guarded([&] {
-    AppendArgs a{};
-    a.kv = check_paged(kv);
-    need(rows >= 0, "qd_paged_append: negative rows");
-    need(q_starts || rows == kv->batch, "qd_paged_append: without q_starts rows must equal the batch");
-    need(known_dtype(qkv_dtype) && known_dtype(q_out_dtype), "qd_paged_append: unknown dtype");
-    need(q_heads >= 0 && q_heads <= 65536, "qd_paged_append: bad q_heads");
-    const int64_t heads = (int64_t)q_heads + 2 * kv->kv_heads;
-    need(qkv_stride >= heads * kHeadDim && qkv_stride % 8 == 0,
-         "qd_paged_append: qkv_stride must be a multiple of 8, at least (q_heads + 2 kv_heads) * 128");
-    need(q_heads == 0 || (q_out_stride >= (int64_t)q_heads * kHeadDim && q_out_stride % 8 == 0),
-         "qd_paged_append: q_out_stride must be a multiple of 8, at least q_heads * 128");
-    need(std::isfinite(eps) && eps >= 0.0f, "qd_paged_append: eps must be finite and not negative");
-    need((cos == nullptr) == (sin == nullptr), "qd_paged_append: cos and sin go together");
-    need(!cos || (rope_len >= 0 && rope_stride >= 0 && rope_stride % 4 == 0),
-         "qd_paged_append: rope_stride must be a multiple of 4, not negative");
-    need(rows == 0 || (qkv && (q_out || q_heads == 0)), "qd_paged_append: NULL pointer");
-    need(aligned16(qkv) && aligned16(q_out) && aligned16(cos) && aligned16(sin) && aligned16(q_norm) &&
-             aligned16(k_norm),
-         "qd_paged_append: pointers must be 16-byte aligned");
-    const int sure = q_starts ? std::min(rows, 1) : rows;
-    const Rows in = rows_of(qkv, qkv_dtype, sure, heads * kHeadDim, qkv_stride);
-    const Rows out = rows_of(q_out, q_out_dtype, sure, (int64_t)q_heads * kHeadDim, q_out_stride);
-    const bool in_place = q_out == qkv && q_out_dtype == qkv_dtype && (q_out_stride == qkv_stride || rows == 1);
-    need(in_place || apart(out, in),
-         "qd_paged_append: q_out overlaps qkv (it may be qkv itself, with its type and stride)");
-    need_apart_from_pools(kv, out, "qd_paged_append: q_out overlaps the pools");
-    need_apart_from_pools(kv, in, "qd_paged_append: qkv overlaps the pools");
-    if (rows == 0 || kv->batch == 0) return;
-    a.kv_dtype = kv->dtype;
-    a.qkv = qkv;
-    a.qkv_stride = qkv_stride;
-    a.rows = rows;
-    a.q_starts = q_starts;
-    a.q_heads = q_heads;
-    a.q_norm = q_norm;
-    a.k_norm = k_norm;
-    a.eps = eps;
-    a.cos_t = cos;
-    a.sin_t = sin;
-    a.rope_len = rope_len;
-    a.rope_stride = rope_stride;
-    a.q_out = q_out;
-    a.q_out_dtype = q_out_dtype;
-    a.q_out_stride = q_out_stride;
+    const PagedArgs cache = check_paged(kv);
+    append<false>(cache, kv->dtype, {}, [&](const Rows& x, const char* msg) { need_apart_from_pools(kv, x, msg); }, qkv, qkv_dtype,
+                  qkv_stride, rows, q_starts, q_heads, q_norm, k_norm, eps, cos, sin, rope_len, rope_stride, q_out,
+                  q_out_dtype, q_out_stride, stream);
+  });
+}
+
+int qd_paged_append_q8(const qd_paged_q8* kv, const void* qkv, int qkv_dtype, int64_t qkv_stride, int rows,
+                       const int32_t* q_starts, int q_heads, const float* q_norm, const float* k_norm, float eps,
+                       const float* cos, const float* sin, int64_t rope_len, int64_t rope_stride, void* q_out,
+                       int q_out_dtype, int64_t q_out_stride, void* stream) {
+  return guarded([&] {
+    const PagedArgs cache = check_q8(kv);
+    append<true>(cache, QD_KV_F16, {kv->k_scale, kv->v_scale},
+                 [&](const Rows& x, const char* msg) { need_apart_from_q8(kv, x, msg); }, qkv, qkv_dtype, qkv_stride, rows,
+                 q_starts, q_heads, q_norm, k_norm, eps, cos, sin, rope_len, rope_stride, q_out, q_out_dtype,
+                 q_out_stride, stream);
+  });
+}
+
+int qd_paged_read_q8(const qd_paged_q8* kv, const int32_t* first, const qd_paged_kv* to, void* stream) {
+  return guarded([&] {
+    ReadArgs a{};
+    a.src = check_q8(kv);
+    need(to != nullptr, "paged cache: NULL pointer");
+    qd_paged_kv out = *to;
+    out.seq_lens = kv->seq_lens;  // (those of `to` are not looked at)
+    a.dst = check_paged(&out);
+    need(to->batch == kv->batch && to->kv_heads == kv->kv_heads,
+         "qd_paged_read_q8: both caches must have the same batch and kv_heads");
+    for (const void* pool : {to->k, to->v}) {
+      const int64_t bytes = (int64_t)to->num_pages * to->kv_heads * to->page_size * kHeadDim * 2;
+      need_apart_from_q8(kv, Rows{pool, 1, bytes, bytes}, "qd_paged_read_q8: the 16-bit pools overlap the 8-bit ones");
+    }
+    a.scale = {kv->k_scale, kv->v_scale};
+    a.first = first;
+    a.dtype = to->dtype;
+    if (kv->batch == 0) return;
+    const long long most = (long long)kv->batch * kv->kv_heads * (((long long)kv->table_width << a.src.page_shift) / 16 + 1);
+    if (most > 0x7fffffffLL) throw QdError{QD_E_RANGE, "qd_paged_read_q8: batch * heads * table beyond 2^31 units"};
+    const int ctas = (int)std::max(1LL, std::min<long long>((most + 3) / 4, 8 * current_sms()));
+    const size_t smem = (size_t)(kv->batch + 1) * 4;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    // four heads a warp once that gives every SM four CTAs, else two
-    if (rows * ((heads + 3) / 4) >= 32LL * current_sms()) launch_append<4>(a, qkv_dtype, heads, s);
-    else launch_append<2>(a, qkv_dtype, heads, s);
+    if (to->dtype == QD_KV_F16) launch_ex(k_paged_read_q8<__half>, dim3(ctas), dim3(kPdThreads), smem, s, a);
+    else launch_ex(k_paged_read_q8<__nv_bfloat16>, dim3(ctas), dim3(kPdThreads), smem, s, a);
   });
 }
 
@@ -261,6 +428,50 @@ int qd_paged_attn_decode(const qd_paged_kv* kv, const void* q, int dtype, int64_
     if (kv->dtype == QD_KV_F16) launch_decode<__half, false>(a, workspace, s);
     else if (dtype == QD_KV_F32) launch_decode<__nv_bfloat16, true>(a, workspace, s);
     else launch_decode<__nv_bfloat16, false>(a, workspace, s);
+  });
+}
+
+int qd_paged_attn_decode_q8(const qd_paged_q8* kv, const void* q, int dtype, int64_t q_stride, int q_heads, int window,
+                            int sinks, float scale, void* y, int64_t y_stride, void* workspace, void* stream) {
+  return guarded([&] {
+    need(kv != nullptr, "paged cache: NULL pointer");
+    PAttnArgs a =
+        check_attn(nullptr, q, dtype, q_stride, kv->batch, q_heads, window, sinks, scale, y, y_stride, kv->batch, kv);
+    if (a.rows == 0) return;
+    need(workspace != nullptr, "qd_paged_attn_decode_q8: NULL workspace");
+    need(aligned16(workspace), "qd_paged_attn_decode_q8: the workspace must be 16-byte aligned");
+    launch_decode_q8(a, {kv->k_scale, kv->v_scale}, workspace, static_cast<cudaStream_t>(stream));
+  });
+}
+
+size_t qd_paged_attn_decode_shared_workspace_bytes(int batch, int groups, int q_heads, int kv_heads) {
+  if (batch < 0 || groups < 0 || groups > batch || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads) return 0;
+  return std::max(shared_ws(batch, groups, q_heads, kv_heads, 128).bytes,
+                  shared_ws(batch, groups, q_heads, kv_heads, 256).bytes);  // (a CTA's rows depend on the types)
+}
+
+int qd_paged_attn_decode_shared(const qd_paged_kv* kv, const void* q, int dtype, int64_t q_stride, int q_heads,
+                                int groups, const int32_t* group_starts, const int32_t* shared_lens, float scale,
+                                void* y, int64_t y_stride, void* workspace, void* stream) {
+  return guarded([&] {
+    need(kv != nullptr, "paged cache: NULL pointer");
+    PAttnArgs a = check_attn(kv, q, dtype, q_stride, kv->batch, q_heads, 0, 0, scale, y, y_stride, kv->batch);
+    need(groups >= 0 && groups <= kv->batch, "qd_paged_attn_decode_shared: groups must be 0..batch");
+    if (a.rows == 0 || groups == 0) return;
+    need(group_starts && shared_lens, "qd_paged_attn_decode_shared: NULL group_starts or shared_lens");
+    need(workspace != nullptr, "qd_paged_attn_decode_shared: NULL workspace");
+    need(aligned16(workspace), "qd_paged_attn_decode_shared: the workspace must be 16-byte aligned");
+    a.q_starts = group_starts;
+    a.groups = groups;
+    a.shared_lens = shared_lens;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (kv->dtype == QD_KV_F16) {
+      if (dtype == QD_KV_F32) launch_shared<__half, 2>(a, workspace, s);
+      else launch_shared<__half, 1>(a, workspace, s);
+    } else {
+      if (dtype == QD_KV_F32) launch_shared<__nv_bfloat16, 3>(a, workspace, s);
+      else launch_shared<__nv_bfloat16, 1>(a, workspace, s);
+    }
   });
 }
 

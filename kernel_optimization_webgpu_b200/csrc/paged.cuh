@@ -117,7 +117,32 @@ struct AppendArgs {
   void* q_out;
   int q_out_dtype;
   long long q_out_stride;
+  float *k_scale, *v_scale;  // of an 8-bit cache
 };
+
+// A row of 128 elements (four a lane) as 8-bit integers n with one scale: n = round(x / scale), scale = the
+// largest magnitude / 127, so that each element is at most half a scale (1/254 of the largest) off. A row
+// with an element that is not finite gets a NaN scale (all of it reads as NaN), one whose largest is below 2^-100
+// a scale of 0. The rounding is that of an addition of 1.5 * 2^23, whose sum's low byte is n.
+__device__ __forceinline__ void store_q8(int8_t* rows, float* scales, long long row, int lane, float4 x) {
+  const unsigned none = 0x7fffffffu;
+  const unsigned mine = max(max(__float_as_uint(x.x) & none, __float_as_uint(x.y) & none),
+                            max(__float_as_uint(x.z) & none, __float_as_uint(x.w) & none));
+  const unsigned top = __reduce_max_sync(0xffffffffu, mine);  // (NaN above infinity above every number)
+  float scale = 0.0f;
+  unsigned n = 0;
+  if (top >= 0x7f800000u) {
+    scale = __uint_as_float(0x7fffffffu);
+  } else if (top >= 27u << 23) {
+    const float most = __uint_as_float(top), up = 127.0f / most, magic = 12582912.0f;
+    scale = most / 127.0f;
+    const unsigned a = __float_as_uint(fmaf(x.x, up, magic)), b = __float_as_uint(fmaf(x.y, up, magic));
+    const unsigned c = __float_as_uint(fmaf(x.z, up, magic)), d = __float_as_uint(fmaf(x.w, up, magic));
+    n = __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+  }
+  reinterpret_cast<unsigned*>(rows + row * kHeadDim)[lane] = n;
+  if (lane == 0) scales[row] = scale;
+}
 
 // One warp per row and HEADS consecutive heads of its [q | k | v]; lane l holds dims 4l .. 4l+3, so
 // the rotation's partner dims are 16 lanes away. What it has to move bounds it (per row and head 512
@@ -127,7 +152,8 @@ struct AppendArgs {
 // HEADS: 4 keep 2 KB in flight per warp at 40 warps an SM (16384 rows of 16 + 8 + 8 heads, f32, 470 MB:
 // 82 us = 5.7 TB/s, 88 with 8); with few rows 2 spread the work over more warps (1 row: 2.5 us, 3.2
 // with 4).
-template <typename T, int HEADS>
+// Q8: the K and V rows go to an 8-bit cache (store_q8).
+template <typename T, int HEADS, bool Q8 = false>
 __global__ void __launch_bounds__(256, HEADS == 4 ? 5 : 6) k_paged_append(const __grid_constant__ AppendArgs a) {
   const int lane = threadIdx.x & 31;
   const int heads = a.q_heads + 2 * a.kv.kv_heads;
@@ -202,7 +228,10 @@ __global__ void __launch_bounds__(256, HEADS == 4 ? 5 : 6) k_paged_append(const 
     } else if (page >= 0) {
       const int g = h < v0 ? h - k0 : h - v0;
       const long long row = (((long long)page * a.kv.kv_heads + g) << a.kv.page_shift) + in_page;
-      store4(h < v0 ? a.kv.k : a.kv.v, row * kHeadDim + 4 * lane, a.kv_dtype, y);
+      if constexpr (Q8)
+        store_q8(static_cast<int8_t*>(h < v0 ? a.kv.k : a.kv.v), h < v0 ? a.k_scale : a.v_scale, row, lane, y);
+      else
+        store4(h < v0 ? a.kv.k : a.kv.v, row * kHeadDim + 4 * lane, a.kv_dtype, y);
     }
   }
 }
@@ -220,6 +249,11 @@ struct PAttnArgs {
   void* y;
   int dtype;  // of q and y
   long long y_stride;
+  // Shared prefixes: q_starts holds the groups' first sequences (groups + 1 entries).
+  int groups;
+  const int* shared_lens;  // [batch]
+  float* tail_o;           // [batch][q_heads][128]: unnormalised sums of the positions behind them,
+  float2* tail_ml;         // [batch][q_heads]: with their maxima and weights
 };
 
 }  // namespace qd

@@ -80,6 +80,17 @@ __device__ __forceinline__ Visible visible(int asked, int len, int window, int s
   return v;
 }
 
+// The positions of sequence b from its shared_lens[b]-th on.
+template <int TILE>
+__device__ __forceinline__ Visible tail(const PAttnArgs& a, int b) {
+  Visible v{};
+  v.end = paged_len(a.kv, b);
+  v.lo = min(max(a.shared_lens[b], 0), v.end);
+  v.w0 = v.lo / TILE;
+  v.tiles = v.lo < v.end ? (v.end + TILE - 1) / TILE - v.w0 : 0;
+  return v;
+}
+
 __device__ __forceinline__ void cp_async16(unsigned dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
@@ -174,6 +185,71 @@ struct PdCursor {
   Visible v;
 };
 
+// Units before each sequence: first[0 .. B], an exclusive scan of the sequences' tile counts by a CTA of
+// kPdThreads. see(b): what sequence b shows.
+template <typename See>
+__device__ __forceinline__ void pd_units(int B, int* first, See&& see) {
+  __shared__ int wsum[4];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (B + kPdThreads - 1) / kPdThreads;
+  const int b0 = min(tid * per, B), b1 = min(b0 + per, B);
+  int n = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int t = see(b).tiles;
+    first[b] = t;
+    n += t;
+  }
+  int incl = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += x;
+  }
+  if (lane == 31) wsum[warp] = incl;
+  __syncthreads();
+  int at = incl - n;
+  for (int w = 0; w < warp; ++w) at += wsum[w];
+  for (int b = b0; b < b1; ++b) {
+    const int t = first[b];
+    first[b] = at;
+    at += t;
+  }
+  if (tid == kPdThreads - 1) first[B] = wsum[0] + wsum[1] + wsum[2] + wsum[3];
+  __syncthreads();
+}
+// The place of unit u.
+template <typename See>
+__device__ __forceinline__ PdCursor pd_place(int B, const int* first, int nh, int subs, int u, See&& see) {
+  PdCursor c;
+  int lo = 0, hi = B;  // the last sequence whose units start at or before u
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if ((long long)first[mid] * nh <= u) lo = mid;
+    else hi = mid;
+  }
+  c.b = lo;
+  c.v = see(lo);
+  const int rest = u - first[lo] * nh;
+  const int h = rest / c.v.tiles;
+  c.t = rest - h * c.v.tiles;
+  c.g = h / subs;
+  c.sub = h - c.g * subs;
+  return c;
+}
+// To the next unit (there is one).
+template <typename See>
+__device__ __forceinline__ void pd_step(PdCursor& c, const int* first, int kv_heads, int subs, See&& see) {
+  if (++c.t < c.v.tiles) return;
+  c.t = 0;
+  if (++c.sub < subs) return;
+  c.sub = 0;
+  if (++c.g < kv_heads) return;
+  c.g = 0;
+  do ++c.b;
+  while (first[c.b + 1] == first[c.b]);
+  c.v = see(c.b);
+}
+
 // Dynamic shared memory: 4 rings | units before each sequence. Where a (sequence, head) ends, each
 // warp's sums go to the ring slot it has just read, rows kPdSumRow floats apart (8 heads on
 // distinct banks).
@@ -181,7 +257,9 @@ constexpr int kPdSumRow = 136;
 static_assert(8 * kPdSumRow * 4 <= kPdSlot, "a slot holds eight heads' sums");
 __host__ __device__ constexpr int pd_smem(int batch) { return 4 * kPdStages * kPdSlot + (batch + 1) * 4; }
 
-template <typename T, bool THREE>
+// TAIL: the positions behind those that a sequence shares (paged_shared.cuh). All sums go to the workspace, a
+// (sequence, head) that one CTA holds whole to a place of its own.
+template <typename T, bool THREE, bool TAIL = false>
 __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_constant__ PAttnArgs a, void* workspace) {
   extern __shared__ __align__(128) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -192,42 +270,19 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
   const PDecodeWs ws = pd_ws(workspace);
   pdl_wait();
   pdl_trigger();
+  const int held = TAIL ? min(a.q_starts[a.groups], B) : B;  // sequences behind the last group are padding
 
-  // units before each sequence (an exclusive scan of the tile counts)
-  {
-    __shared__ int wsum[4];
-    const int per = (B + kPdThreads - 1) / kPdThreads;
-    const int b0 = min(tid * per, B), b1 = min(b0 + per, B);
-    int n = 0;
-    for (int b = b0; b < b1; ++b) {
-      const int t = visible<kPdTile>(a.kv.seq_lens[b], paged_len(a.kv, b), a.window, a.sinks).tiles;
-      first[b] = t;
-      n += t;
-    }
-    int incl = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += x;
-    }
-    if (lane == 31) wsum[warp] = incl;
-    __syncthreads();
-    int at = incl - n;
-    for (int w = 0; w < warp; ++w) at += wsum[w];
-    for (int b = b0; b < b1; ++b) {
-      const int t = first[b];
-      first[b] = at;
-      at += t;
-    }
-    if (tid == kPdThreads - 1) first[B] = wsum[0] + wsum[1] + wsum[2] + wsum[3];
-    __syncthreads();
-  }
+  auto see = [&](int b) {
+    if constexpr (TAIL) return b < held ? tail<kPdTile>(a, b) : Visible{};
+    else return visible<kPdTile>(a.kv.seq_lens[b], paged_len(a.kv, b), a.window, a.sinks);
+  };
+  pd_units(B, first, see);
   if (blockIdx.x == 0) {
     for (int b = tid; b <= B; b += kPdThreads) ws.first[b] = first[b];
-    for (int b = tid; b < B; b += kPdThreads)  // (paged_len cuts both)
+    for (int b = tid; b < held; b += kPdThreads)  // (paged_len cuts both)
       if (a.kv.seq_lens[b] != paged_len(a.kv, b)) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
   }
-  for (int b = blockIdx.x; b < B; b += gridDim.x)  // nothing visible: zeros
+  for (int b = blockIdx.x; !TAIL && b < B; b += gridDim.x)  // nothing visible: zeros
     if (first[b + 1] == first[b])
       for (int i = tid; i < a.q_heads * kHeadDim; i += kPdThreads) store1(a.y, b * a.y_stride + i, a.dtype, 0.0f);
   const long long U = (long long)first[B] * nh;
@@ -235,36 +290,8 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
   if ((int)blockIdx.x >= ctas) return;
   const int u0 = (int)(U * blockIdx.x / ctas), u1 = (int)(U * (blockIdx.x + 1) / ctas);
 
-  auto see = [&](PdCursor& c) {
-    c.v = visible<kPdTile>(a.kv.seq_lens[c.b], paged_len(a.kv, c.b), a.window, a.sinks);
-  };
-  auto step = [&](PdCursor& c) {  // to the next unit (there is one)
-    if (++c.t < c.v.tiles) return;
-    c.t = 0;
-    if (++c.sub < subs) return;
-    c.sub = 0;
-    if (++c.g < a.kv.kv_heads) return;
-    c.g = 0;
-    do ++c.b;
-    while (first[c.b + 1] == first[c.b]);
-    see(c);
-  };
-  PdCursor cur;
-  {
-    int lo = 0, hi = B;  // the last sequence whose units start at or before u0
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if ((long long)first[mid] * nh <= u0) lo = mid;
-      else hi = mid;
-    }
-    cur.b = lo;
-    see(cur);
-    const int rest = u0 - first[lo] * nh;
-    const int h = rest / cur.v.tiles;
-    cur.t = rest - h * cur.v.tiles;
-    cur.g = h / subs;
-    cur.sub = h - cur.g * subs;
-  }
+  auto step = [&](PdCursor& c) { pd_step(c, first, a.kv.kv_heads, subs, see); };
+  PdCursor cur = pd_place(B, first, nh, subs, u0, see);
   PdCursor pre = cur;  // the copies run ahead of the sums
   const int n_units = u1 - u0;
 
@@ -493,7 +520,11 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
           L += sml[w][h].y * f;
           x += reinterpret_cast<const float*>(smem + (w * kPdStages + slot) * kPdSlot)[h * kPdSumRow + tid] * f;
         }
-        if (whole) {
+        if (whole && TAIL) {
+          const long long at = (long long)cur.b * a.q_heads + cur.g * G + cur.sub * 8 + h;
+          a.tail_o[at * kHeadDim + tid] = x;
+          if (tid == 0) a.tail_ml[at] = make_float2(M, L);
+        } else if (whole) {
           store1(a.y, out + h * kHeadDim, a.dtype, x * inv_sum(L));
         } else {
           ws.o[(part + h) * kHeadDim + tid] = x;

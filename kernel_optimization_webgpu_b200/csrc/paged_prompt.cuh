@@ -73,6 +73,7 @@ struct PPromptArgs {
   // that a warp's rows lie side by side; and their maxima and weights: [item][KV head][split][cta_rows].
   float4* po;
   float2* pml;
+  int2* rows;    // SHARED: [batch][query heads of a KV head]: where a row's sums are (item * cta_rows + row), its parts
 };
 
 template <int PARTS>
@@ -157,6 +158,24 @@ __device__ __forceinline__ PpItem pp_rows(const PAttnArgs& a, int G, int cta_row
   v.st = (v.ns + kPpKeys - 1) / kPpKeys;
   v.w0 = max(v.lo / kPpKeys, v.st);
   v.tiles = v.st + max(0, (v.end + kPpKeys - 1) / kPpKeys - v.w0);
+  return it;
+}
+// The same for queries of a group of sequences over the positions that they share with its first: row r belongs to
+// sequence tok0 + r / G and sees what of them its own length leaves (pp_shares). Whole warps.
+__device__ __forceinline__ int pp_shares(const PAttnArgs& a, int seq) {
+  return max(0, min(paged_len(a.kv, seq), a.shared_lens[seq]));
+}
+__device__ __forceinline__ PpItem pp_shared_rows(const PAttnArgs& a, int G, int cta_rows, int tile, int start, int n) {
+  PpItem it;
+  it.tok0 = start;
+  it.pos0 = 0;
+  it.n_rows = n * G;
+  const int r0 = tile * cta_rows, r1 = min(r0 + cta_rows, it.n_rows);
+  int most = 0;
+  for (int s = start + r0 / G + (threadIdx.x & 31); s <= start + (r1 - 1) / G; s += 32)
+    if ((unsigned)s < (unsigned)a.rows) most = max(most, pp_shares(a, s));
+  it.len = __reduce_max_sync(0xffffffffu, most);
+  it.v = Visible{it.len, 0, 0, 0, 0, (it.len + kPpKeys - 1) / kPpKeys};
   return it;
 }
 // Largest of three, NaN if one of them is.
@@ -326,7 +345,9 @@ __device__ __forceinline__ void split_parts(float x, float y, unsigned (&u)[PART
 }
 
 // CLAIM: blocks take the work of others that have not started (a grid that does not fit the GPU at once).
-template <typename T, int PARTS, bool CLAIM>
+// SHARED: the rows of a "sequence" are the queries of a group, all of which see the positions that the group shares
+// (a.q_starts: the groups' first sequences, a.kv.batch of them); every row's sums go to the workspace.
+template <typename T, int PARTS, bool CLAIM, bool SHARED = false>
 __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_constant__ PPromptArgs pa) {
   const PAttnArgs& a = pa.a;
   constexpr int S = pp_slots<PARTS>(), kTiles = pp_tiles<PARTS>(), kRows = 128 * kTiles;
@@ -363,10 +384,16 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
     w.item = b / (kvh * pa.splits);
     int seq = 0, tile = 0, start = 0, fresh = 0, asked = 0;
     if (!pp_item(a, G, kRows, w.item, seq, tile, start, fresh, asked)) return false;
-    w.it = pp_rows(a, G, kRows, tile, start, fresh, asked);
+    if constexpr (SHARED) {
+      if ((unsigned)start >= (unsigned)a.rows) return false;  // (no such sequence)
+      w.it = pp_shared_rows(a, G, kRows, tile, start, fresh);
+      seq = start;  // (whose pages are the group's)
+    } else {
+      w.it = pp_rows(a, G, kRows, tile, start, fresh, asked);
+    }
     w.it.seq = seq;
     // beyond the table, or new tokens before position 0 (a length of 0 is a padded sequence)
-    if ((asked > w.it.len || (asked != 0 && asked < fresh)) && lane == 0) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
+    if (!SHARED && (asked > w.it.len || (asked != 0 && asked < fresh)) && lane == 0) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
     w.parts = pp_parts(w.it.v.tiles, pa.splits);
     if (w.z >= w.parts) return false;
     w.t0 = w.it.v.tiles * w.z / w.parts;  // (at most 2^23 tiles, 32 parts)
@@ -766,12 +793,12 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
         const unsigned ts = tmem + t * 128 + lanes, tp = tmem + kColP + t * 128 + 32 * hf + lanes;
         const unsigned to = tmem + kColO + t * 128 + 64 * hf + lanes;
-        const int p = live ? it.pos0 + tok : -1;
+        const int p = !live ? -1 : SHARED ? pp_shares(a, it.tok0 + tok) - 1 : it.pos0 + tok;
         const int pmax = min(p, it.len - 1);
         const int phi = a.window > 0 ? p - a.window : -2;  // keys up to here are hidden, unless sinks
         // positions of the warp's first and last live rows
         const unsigned lv = __ballot_sync(0xffffffffu, live);
-        const int pw0 = __shfl_sync(0xffffffffu, p, 0), pw1 = __shfl_sync(0xffffffffu, p, lv ? 31 - __clz(lv) : 0);
+        const int pw0 = SHARED ? __reduce_min_sync(0xffffffffu, p) : __shfl_sync(0xffffffffu, p, 0), pw1 = __shfl_sync(0xffffffffu, p, lv ? 31 - __clz(lv) : 0);
         const long long part0 = (((long long)item * kvh + g) * pa.splits + z) * kRows;
         float4* mine = pa.po + part0 * (kHeadDim / 4) + lr;
         float moved = -INFINITY;  // the maximum that the sums in the workspace go by
@@ -903,7 +930,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         if (ok) ok = __all_sync(0xffffffffu, pp_wait(&o_done[t], (unsigned)((nk - 1) ^ turn) & 1u, &failed));
         if (ok) {
           tc_fence_after();
-          const bool whole = parts == 1;
+          const bool whole = !SHARED && parts == 1;
           const float f = whole ? inv_sum(l) : 1.0f;
           const long long y_at =
               live ? (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf : -1;
@@ -965,7 +992,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         turn ^= (unsigned)nk;
       }
       done += nk;
-      if (nk == 0 && live) {  // no key is visible to any row
+      if (SHARED && live && hf == 0 && g == 0 && z == 0)
+        pa.rows[(long long)(it.tok0 + tok) * G + hs] = make_int2(item * kRows + lr, nk == 0 ? 0 : parts);
+      if (!SHARED && nk == 0 && live) {  // no key is visible to any row
         const long long base = (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf;
         for (int i = 0; i < kHeadDim / 2; i += 4) store4(a.y, base + i, a.dtype, make_float4(0.f, 0.f, 0.f, 0.f));
       }
@@ -987,7 +1016,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         for (int e = tid; e < 32 * n_rows; e += kPpSoftmax) {
           const int lr = e >> 5, row = w.row0 + lr, tok = w.it.tok0 + row / G;
           if ((unsigned)tok >= (unsigned)a.rows) continue;
-          if (w.parts > 1)
+          if (SHARED || w.parts > 1)
             pa.pml[(((long long)w.item * kvh + w.g) * pa.splits + w.z) * kRows + lr] = make_float2(gone, gone);
           else
             store4(a.y, (long long)tok * a.y_stride + ((long long)w.g * G + row % G) * kHeadDim + 4 * lane, a.dtype,

@@ -669,7 +669,72 @@ def sample_rows(logits, u, temperature=None, top_k=None, top_p=None, min_p=None,
     return (_calls_module or _calls()).sample_rows(logits, u, temperature, top_k, top_p, min_p, ids, logprobs)
 
 
+def paged_append_q8(qkv, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, cos, sin, q_heads: int,
+                    q_norm=None, k_norm=None, eps: float = 1e-6, q_starts=None, q_out=None,
+                    rope_stride: Optional[int] = None, status=None, stream=None):
+    """paged_append into a cache of 8-bit integers (qd_paged_append_q8): pools int8
+    [pages][kv_heads][page_size][128] with f32 scales [pages][kv_heads][page_size], a row x being held as
+    scale = max|x| / 127 and x / scale rounded. Returns q."""
+    if stream is not None:
+        with _on(stream, qkv):
+            return paged_append_q8(qkv, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, cos, sin, q_heads,
+                                   q_norm, k_norm, eps, q_starts, q_out, rope_stride, status)
+    return (_calls_module or _calls()).paged_append_q8(qkv, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens,
+                                                       cos, sin, q_heads, q_norm, k_norm, eps, q_starts, q_out,
+                                                       rope_stride, status)
+
+
+def paged_read_q8(k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, k_out, v_out, out_table, first=None,
+                  status=None, stream=None):
+    """Positions first[b] (default 0) .. seq_lens[b] - 1 of every sequence of an 8-bit cache read back into
+    16-bit pools under a table of their own (qd_paged_read_q8), over which paged_attn_prompt can run; their
+    page size may differ. Writes nothing else of k_out, v_out; returns them."""
+    if stream is not None:
+        with _on(stream, k_pages):
+            return paged_read_q8(k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, k_out, v_out, out_table,
+                                 first, status)
+    return (_calls_module or _calls()).paged_read_q8(k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, k_out,
+                                                     v_out, out_table, first, status)
+
+
+def paged_attn_decode_q8(q, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, window: int = 0, sinks: int = 0,
+                         scale: float = 0.0, y=None, workspace=None, status=None, stream=None):
+    """paged_attn_decode over an 8-bit cache (qd_paged_attn_decode_q8); q f32, f16 or bf16."""
+    if stream is not None:
+        with _on(stream, q):
+            return paged_attn_decode_q8(q, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, window, sinks,
+                                        scale, y, workspace, status)
+    return (_calls_module or _calls()).paged_attn_decode_q8(q, k_pages, v_pages, k_scales, v_scales, block_table,
+                                                            seq_lens, window, sinks, scale, y, workspace, status)
+
+
+def paged_attn_decode_shared(q, k_pages, v_pages, block_table, seq_lens, group_starts, shared_lens, scale: float = 0.0,
+                             y=None, workspace=None, status=None, stream=None):
+    """paged_attn_decode for groups of sequences that share their first positions
+    (qd_paged_attn_decode_shared): group i is the sequences group_starts[i] .. group_starts[i + 1] - 1 (int32,
+    groups + 1 entries from 0), sequence b's first shared_lens[b] (int32) positions are those of its
+    group's first sequence and are read once for all of the group. Sequences behind the last group are padding; y
+    keeps what it held there. workspace: qd_paged_attn_decode_shared_workspace_bytes."""
+    if stream is not None:
+        with _on(stream, q):
+            return paged_attn_decode_shared(q, k_pages, v_pages, block_table, seq_lens, group_starts, shared_lens, scale,
+                                            y, workspace, status)
+    return (_calls_module or _calls()).paged_attn_decode_shared(q, k_pages, v_pages, block_table, seq_lens, group_starts,
+                                                                shared_lens, scale, y, workspace, status)
+
+
+def score_rows(logits, tokens, top: int = 0, logprobs=None, entropy=None, top_ids=None, top_logprobs=None, stream=None):
+    """Log probability of one given token (int32) per row of logits [rows][vocab] (f32, f16 or bf16), the
+    row's entropy and its `top` (0..64) likeliest tokens with their log probabilities, as qd_score_rows defines
+    them. Returns (logprobs [rows], entropy [rows], top_ids [rows][top] int32, top_logprobs [rows][top])."""
+    if stream is not None:
+        with _on(stream, logits):
+            return score_rows(logits, tokens, top, logprobs, entropy, top_ids, top_logprobs)
+    return (_calls_module or _calls()).score_rows(logits, tokens, top, logprobs, entropy, top_ids, top_logprobs)
+
+
 __all__ = ["Engine", "QdError", "createWebGpuContext", "runCustomQwenGreedyPrompt", "runKernelBenchmarks",
            "runFullDecoderStackBenchmark", "qwen_profile",
            "qwenProfile", "q4_matvec", "lm_head_argmax", "gqa_decode", "LmHeadWorkspace",
-           "paged_append", "paged_attn_decode", "paged_attn_prompt", "sample_rows"]
+           "paged_append", "paged_attn_decode", "paged_attn_prompt", "sample_rows",
+           "paged_append_q8", "paged_read_q8", "paged_attn_decode_q8", "paged_attn_decode_shared", "score_rows"]
