@@ -3,11 +3,16 @@
 //   log p_t = x_t - m - log S,  H = log S - sum (x - m) e^(x - m) / S,  S = sum e^(x - m),  m = max x
 //
 // One thread-block cluster per row, a contiguous share per CTA, read once from memory: each thread keeps a running
-// maximum, S and the entropy's sum by it (in base 2), joined over warps, CTAs and the cluster at the end. The
-// largest tokens need a border first, below which nothing has to be looked at: the row's threads form 128 groups,
-// and the top-th largest of the groups' maxima is a value that at least `top` tokens reach and that
-// hardly more than those do. A second look at the CTA's share (in L1 by now) lists what reaches it; the lists, a few
-// tokens each, are put in order by counting.
+// maximum and both sums by it, joined over warps and the cluster at the end. The largest tokens need a border first,
+// below which nothing has to be looked at: the row's threads form 128 groups, and the top-th largest of the groups'
+// maxima is a value that at least `top` tokens reach and that hardly more than those do. Of the batches of loads whose
+// maximum (kept in shared memory) reaches it, a few dozen, the tokens are listed, and the list is put in order by
+// counting.
+//
+// Many rows: bound by the latency of the loads and, with 16-bit logits, by the exponentials (one per token: 17 of
+// 39 us of the special-function unit), so the next batch is on its way while one is worked on. 512 x 151936 bf16 with 20
+// alternatives: 39 us (156 MB, 4.0 TB/s; 35 without alternatives), 256 x 151936 f32: 27 us (5.75 TB/s). One row of f32:
+// 7.8 us, of which a chain of loads, barriers of the cluster and the border's search, not bytes.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -23,13 +28,13 @@ namespace qd {
 namespace cg = cooperative_groups;
 typedef unsigned long long u64;
 
-constexpr int kScoreThreads = 512;
-constexpr int kScoreWarps = kScoreThreads / 32;
+constexpr int kScoreThreads = 256;
 constexpr int kScoreCluster = 8;
-constexpr int kScoreTop = 64;     // largest `top`
+constexpr int kScoreTop = 64;      // largest `top`
 constexpr int kScoreGroups = 128;  // of a row's threads: at least kScoreTop
-constexpr int kScoreList = 1024;  // tokens at or above the border that a CTA lists
-constexpr int kScoreUnroll = 4;   // 16-byte loads in flight per thread
+constexpr int kScoreList = 1024;   // tokens at or above the border that a CTA lists
+constexpr int kScoreUnroll = 4;    // 16-byte loads of a thread's batch
+constexpr int kScoreSlots = 12;    // batches whose maxima are kept apart
 
 struct ScoreArgs {
   const void* logits;
@@ -43,7 +48,9 @@ struct ScoreArgs {
   float* top_logprobs;
 };
 
-// Sums by a maximum: s0 = sum 2^y, s1 = sum y 2^y, y = (x - m) log2 e.
+constexpr float kLog2E = 1.4426950408889634f;
+
+// Sums by a maximum: s0 = sum e^d, s1 = sum d e^d, d = x - m.
 struct ScoreSums {
   float m, s0, s1;
 };
@@ -52,83 +59,142 @@ __device__ __forceinline__ float score_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// The same sums by the maximum mn >= s.m.
-__device__ __forceinline__ ScoreSums score_by(ScoreSums s, float mn) {
-  const float d = s.m == mn || s.m == -INFINITY ? 0.0f : fmaxf((s.m - mn) * 1.4426950408889634f, -200.0f);
-  const float f = s.m == -INFINITY ? 0.0f : score_exp2(d);
-  return ScoreSums{mn, s.s0 * f, fmaf(d, s.s0, s.s1) * f};
+// The factor of sums by the maximum m, for sums by mn >= m: e^d.
+__device__ __forceinline__ float score_shift(float m, float mn, float& d) {
+  d = m == mn || m == -INFINITY ? 0.0f : fmaxf(m - mn, -150.0f);
+  return m == -INFINITY ? 0.0f : score_exp2(d * kLog2E);
 }
-__device__ __forceinline__ ScoreSums score_join(ScoreSums a, ScoreSums b) {
-  const float mn = fmaxf(a.m, b.m);
-  a = score_by(a, mn);
-  b = score_by(b, mn);
-  return ScoreSums{mn, a.s0 + b.s0, a.s1 + b.s1};
+// The sums of a warp's lanes, in all of them.
+__device__ __forceinline__ ScoreSums score_join(ScoreSums s) {
+  float mn = s.m, d;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+  const float f = score_shift(s.m, mn, d);
+  s = ScoreSums{mn, s.s0 * f, fmaf(d, s.s0, s.s1) * f};
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s.s0 += __shfl_xor_sync(0xffffffffu, s.s0, o);
+    s.s1 += __shfl_xor_sync(0xffffffffu, s.s1, o);
+  }
+  return s;
 }
-__device__ __forceinline__ float score_max_nan(float x, float y) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
-  return r;
-}
-
+// A row as 16-byte vectors of VE tokens; what of its first and last one lies outside is -inf.
 template <typename T>
 struct ScoreRow {
   static constexpr int VE = 16 / sizeof(T);
-  const char* base;  // 16-byte boundary at or below the row's first element
-  int head, vocab;   // elements between them
-  // Vector v: elements v * VE - head ..; what lies outside the row is -inf.
+  const char* base;  // 16-byte boundary at or below the row's first token
+  int head, vocab;   // tokens between them
   __device__ __forceinline__ bool whole(int v) const { return v * VE >= head && v * VE - head + VE <= vocab; }
-  __device__ __forceinline__ void load(int v, float (&x)[VE]) const {
-    if (whole(v)) {
-      const uint4 u = *reinterpret_cast<const uint4*>(base + (long long)v * 16);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  __device__ __forceinline__ uint4 load(int v) const {
+    if (whole(v)) return *reinterpret_cast<const uint4*>(base + (long long)v * 16);
+    uint32_t w[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 4) {
-          x[i] = __uint_as_float(w[i]);
-        } else if constexpr (std::is_same<T, __half>::value) {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-          x[2 * i] = f.x;
-          x[2 * i + 1] = f.y;
-        } else {
-          x[2 * i] = __uint_as_float(w[i] << 16);
-          x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        const int e = v * VE - head + i;
+        w[i] = e >= 0 && e < vocab ? reinterpret_cast<const uint32_t*>(base)[(long long)v * VE + i] : kNone;
+      } else {
+        w[i] = kNone;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int e = v * VE - head + 2 * i + h;
+          if (e >= 0 && e < vocab)
+            w[i] = __byte_perm(w[i], reinterpret_cast<const uint16_t*>(base)[(long long)v * VE + 2 * i + h],
+                               h ? 0x5410 : 0x3254);
         }
       }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  // -inf, or a pair of them
+  static constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+  static __device__ __forceinline__ uint4 none() { return make_uint4(kNone, kNone, kNone, kNone); }
+  // Pair i of a vector.
+  static __device__ __forceinline__ float2 pair(const uint4& u, int i) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    else if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    else return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+  }
+  static __device__ __forceinline__ float2 pair_at(const uint4& u, int i) {  // (an index of run time)
+    const uint32_t w = i & 2 ? (i & 1 ? u.w : u.z) : (i & 1 ? u.y : u.x);
+    if constexpr (sizeof(T) == 4) return i ? make_float2(__uint_as_float(u.z), __uint_as_float(u.w)) : pair(u, 0);
+    else return pair(make_uint4(w, 0, 0, 0), 0);
+  }
+  // A bound below which a weight by the maximum m is 0, as a pair of T: a finite one, so that d e^d is 0 there too.
+  // (There is none for a maximum next to the type's lowest value.)
+  static constexpr float kLow = sizeof(T) == 4 ? -3.402823466e38f : std::is_same<T, __half>::value ? -65504.0f : -3.389531389e38f;
+  static __device__ __forceinline__ bool has_floor(float m) { return m - kLow > 150.0f; }
+  static __device__ __forceinline__ uint32_t floor_of(float m) {
+    const float f = fmaxf(m - fmaf(fabsf(m), 0.125f, 1.0e4f), kLow);
+    if constexpr (sizeof(T) == 4) {
+      return __float_as_uint(f);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const __half2 h = __float2half2_rn(f);
+      return *reinterpret_cast<const uint32_t*>(&h);
     } else {
-#pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        const int e = v * VE - head + i;
-        x[i] = e >= 0 && e < vocab ? rows_value<T>(base, (long long)v * VE + i) : -INFINITY;
-      }
+      const __nv_bfloat162 h = __float2bfloat162_rn(f);
+      return *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  // Word i of a vector, its numbers at least `floor` (NaN stays).
+  static __device__ __forceinline__ uint32_t lifted(uint32_t w, uint32_t floor) {
+    if constexpr (sizeof(T) == 4) {
+      float r;
+      asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(w)), "f"(__uint_as_float(floor)));
+      return __float_as_uint(r);
+    } else {
+      using V = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+      const V h = __hmax2_nan(*reinterpret_cast<const V*>(&w), *reinterpret_cast<const V*>(&floor));
+      return *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  // The largest of a vector that is a number (-inf where none is).
+  static __device__ __forceinline__ float most(const uint4& u) {
+    if constexpr (sizeof(T) == 4) {
+      return fmaxf(fmaxf(fmaxf(__uint_as_float(u.x), -INFINITY), __uint_as_float(u.y)),
+                   fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+    } else {
+      using V = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+      const V a = __hmax2(*reinterpret_cast<const V*>(&u.x), *reinterpret_cast<const V*>(&u.y));
+      const V b = __hmax2(*reinterpret_cast<const V*>(&u.z), *reinterpret_cast<const V*>(&u.w));
+      const V c = __hmax2(a, b);
+      const float2 f = pair(make_uint4(*reinterpret_cast<const uint32_t*>(&c), 0, 0, 0), 0);
+      return fmaxf(fmaxf(f.x, -INFINITY), f.y);
     }
   }
 };
 
 struct ScoreShared {
-  ScoreSums sums;               // this CTA's
-  ScoreSums warp[kScoreWarps];
-  float groups[kScoreGroups];   // this CTA's maxima (kScoreGroups / C of them)
-  u64 best[kScoreTop];          // this CTA's largest tokens in order, 0 behind the last
-  float all[kScoreGroups];      // the row's
-  float border;
-  int listed;
-  u64 red[kScoreWarps];
+  ScoreSums warp[kScoreThreads / 32];
+  float groups[kScoreGroups];  // this CTA's maxima
+  u64 best[kScoreTop];         // this CTA's largest tokens in order, 0 behind the last
+  float border, M, log_s;
+  int listed, batches;
+  u64 red[kScoreThreads / 32];
   u64 list[kScoreList];
+  float most[kScoreSlots][kScoreThreads];              // of each thread's batches
+  unsigned short again[kScoreSlots * kScoreThreads];   // batches that hold what reaches the border
 };
 
 // Position in the order of sample_rows: larger first.
 __device__ __forceinline__ u64 score_key(float x, int i) { return (u64)row_key(x) << 32 | (uint32_t)~i; }
 
 template <typename T>
-__global__ void __launch_bounds__(kScoreThreads, 2) k_score_rows(const __grid_constant__ ScoreArgs a) {
-  constexpr int VE = 16 / sizeof(T), U = kScoreUnroll;
+__global__ void __launch_bounds__(kScoreThreads, 4) k_score_rows(const __grid_constant__ ScoreArgs a) {
+  using Row = ScoreRow<T>;
+  constexpr int VE = Row::VE, U = kScoreUnroll, kSlots = kScoreSlots, N = kScoreThreads;
   __shared__ ScoreShared sh;
   cg::cluster_group cl = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank(), r = blockIdx.x / C, K = a.top;
+  auto meet = [&] {  // of the row's CTAs
+    if (C > 1) cl.sync();
+    else __syncthreads();
+  };
   pdl_wait();
   pdl_trigger();
-  ScoreRow<T> row;
+  Row row;
   {
     const char* at = static_cast<const char*>(a.logits) + r * a.row_stride * (long long)sizeof(T);
     const int off = (int)(reinterpret_cast<uintptr_t>(at) & 15);
@@ -140,85 +206,125 @@ __global__ void __launch_bounds__(kScoreThreads, 2) k_score_rows(const __grid_co
   const int v0 = min(rank * a.per, nv), v1 = min(v0 + a.per, nv);
   float given = 0.0f;
   int token = 0;
-  if (rank == 0 && tid == 0) {
+  if (rank == 0 && tid == 32) {
     token = a.tokens[r];
     if ((unsigned)token < (unsigned)a.vocab) given = rows_value<T>(row.base, (long long)row.head + token);
   }
 
   ScoreSums s{-INFINITY, 0.0f, 0.0f};
-  for (int v = v0 + tid; v < v1; v += U * kScoreThreads) {
-    float x[U][VE];
+  {
+    float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+    int slot = 0;
+    // vectors [vb, ve) lie wholly inside the row and this share
+    const int vb = max(v0, row.head > 0), ve = row.whole(nv - 1) ? v1 : min(v1, nv - 1);
+    uint4 next[U];
+    auto fetch = [&](int v) {
+      if (v >= vb && v + (U - 1) * N < ve) {
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      if (v + k * kScoreThreads < v1) {
-        row.load(v + k * kScoreThreads, x[k]);
+        for (int k = 0; k < U; ++k) next[k] = *reinterpret_cast<const uint4*>(row.base + (long long)(v + k * N) * 16);
       } else {
 #pragma unroll
-        for (int i = 0; i < VE; ++i) x[k][i] = -INFINITY;
+        for (int k = 0; k < U; ++k) next[k] = v + k * N < v1 ? row.load(v + k * N) : Row::none();
+      }
+    };
+    fetch(v0 + tid);
+    for (int v = v0 + tid; v < v1; v += U * N) {
+      uint4 x[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) x[k] = next[k];
+      if (v + U * N < v1) fetch(v + U * N);
+      float mx = Row::most(x[0]);
+#pragma unroll
+      for (int k = 1; k < U; ++k) mx = fmaxf(mx, Row::most(x[k]));
+      // (more batches than slots: a slot stands for several)
+      sh.most[slot][tid] = v - (v0 + tid) < kSlots * U * N ? mx : fmaxf(mx, sh.most[slot][tid]);
+      slot = slot + 1 == kSlots ? 0 : slot + 1;
+      if (mx > s.m) {
+        float d;
+        const float f = score_shift(s.m, mx, d);
+        s1 = make_float2(fmaf(d, s0.x, s1.x) * f, fmaf(d, s0.y, s1.y) * f);
+        s0 = make_float2(s0.x * f, s0.y * f);
+        s.m = mx;
+      }
+      // (before the first finite value: everything -inf, or NaN, which stays NaN)
+      const float m = s.m == -INFINITY ? 0.0f : s.m;
+      if (!Row::has_floor(m)) {  // (a mask of the lowest value that covers the whole batch)
+        for (int k = 0; k < U * VE / 2; ++k) {
+          const int w = v + k / (VE / 2) * N;
+          const float2 f = w < v1 ? Row::pair_at(row.load(w), k % (VE / 2)) : make_float2(-INFINITY, -INFINITY);
+          const float dx = f.x - m, dy = f.y - m, ex = score_exp2(dx * kLog2E), ey = score_exp2(dy * kLog2E);
+          s0 = __fadd2_rn(s0, make_float2(ex, ey));
+          s1 = __fadd2_rn(s1, make_float2(ex > 0.0f ? dx * ex : 0.0f, ey > 0.0f ? dy * ey : 0.0f));
+        }
+        continue;
+      }
+      const uint32_t floor = Row::floor_of(m);
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const uint4 u = make_uint4(Row::lifted(x[k].x, floor), Row::lifted(x[k].y, floor), Row::lifted(x[k].z, floor),
+                                   Row::lifted(x[k].w, floor));
+#pragma unroll
+        for (int i = 0; i < VE / 2; ++i) {
+          const float2 d = __fadd2_rn(Row::pair(u, i), make_float2(-m, -m));
+          const float2 y = __fmul2_rn(d, make_float2(kLog2E, kLog2E));
+          const float2 e = make_float2(score_exp2(y.x), score_exp2(y.y));
+          s0 = __fadd2_rn(s0, e);
+          s1 = __ffma2_rn(d, e, s1);
+        }
       }
     }
-    float mx = x[0][0];
-#pragma unroll
-    for (int k = 0; k < U; ++k)
-#pragma unroll
-      for (int i = 0; i < VE; ++i) mx = fmaxf(mx, x[k][i]);
-    if (mx > s.m) s = score_by(s, mx);
-    // (before the first finite value: everything -inf, or NaN, which stays NaN)
-    const float m = s.m == -INFINITY ? 0.0f : s.m;
-#pragma unroll
-    for (int k = 0; k < U; ++k)
-#pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        // below 2^-126 a weight is as good as none, and its place in the entropy's sum stays finite
-        const float y = score_max_nan((x[k][i] - m) * 1.4426950408889634f, -126.0f);
-        const float e = score_exp2(y);
-        s.s0 += e;
-        s.s1 = fmaf(y, e, s.s1);
-      }
+    s.s0 = s0.x + s0.y;
+    s.s1 = s1.x + s1.y;
   }
-  // maxima of the row's 128 groups of 4 C neighbouring threads
+  // maxima of the row's groups of `per` neighbouring threads
+  const int per = N * C / kScoreGroups, mine = N / per;  // (groups of this CTA)
   float top = s.m;
-  for (int o = 1; o < 4 * C; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane % (4 * C) == 0) sh.groups[tid / (4 * C)] = top;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    s = score_join(s, ScoreSums{__shfl_xor_sync(0xffffffffu, s.m, o), __shfl_xor_sync(0xffffffffu, s.s0, o),
-                                __shfl_xor_sync(0xffffffffu, s.s1, o)});
+  for (int o = 1; o < per; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane % per == 0) sh.groups[tid / per] = top;
+  s = score_join(s);
   if (lane == 0) sh.warp[warp] = s;
-  __syncthreads();
-  if (warp == 0) {
-    s = sh.warp[lane % kScoreWarps];
-#pragma unroll
-    for (int o = kScoreWarps / 2; o > 0; o >>= 1)
-      s = score_join(s, ScoreSums{__shfl_xor_sync(0xffffffffu, s.m, o), __shfl_xor_sync(0xffffffffu, s.s0, o),
-                                  __shfl_xor_sync(0xffffffffu, s.s1, o)});
-    if (lane == 0) sh.sums = s;
-  }
-  cl.sync();
+  if (tid == 0) sh.listed = sh.batches = 0;
+  if (tid < kScoreTop) sh.best[tid] = 0;
+  meet();
 
-  float M = 0.0f, log_s = 0.0f;
-  if (rank == 0) {  // the whole row's sums, in the order of the CTAs
-    s = cl.map_shared_rank(&sh, 0)->sums;
-    for (int c = 1; c < C; ++c) s = score_join(s, cl.map_shared_rank(&sh, c)->sums);
-    M = s.m;
-    log_s = logf(s.s0);
-    if (tid == 0) {
-      const float none = __int_as_float(0x7fffffff);
-      a.logprobs[r] = (unsigned)token < (unsigned)a.vocab ? (given - M) - log_s : none;
-      const float h = fmaf(-0.6931471805599453f, s.s1 / s.s0, log_s);
-      if (a.entropy) a.entropy[r] = M == -INFINITY ? none : h < 0.0f ? 0.0f : h;  // (NaN stays)
+  if (warp == 1 && rank == 0) {  // the whole row's sums
+    s = ScoreSums{-INFINITY, 0.0f, 0.0f};
+    for (int i = lane; i < C * (N / 32); i += 32) {
+      const ScoreSums o = cl.map_shared_rank(&sh, i / (N / 32))->warp[i % (N / 32)];
+      const float mn = fmaxf(s.m, o.m);
+      float ds, d;
+      const float fs = score_shift(s.m, mn, ds), f = score_shift(o.m, mn, d);
+      s = ScoreSums{mn, s.s0 * fs + o.s0 * f, fmaf(ds, s.s0, s.s1) * fs + fmaf(d, o.s0, o.s1) * f};
+    }
+    s = score_join(s);
+    const float log_s = logf(s.s0);
+    if (lane == 0) {
+      const float none = __int_as_float(0x7fffffff), h = log_s - s.s1 / s.s0;
+      a.logprobs[r] = (unsigned)token < (unsigned)a.vocab ? (given - s.m) - log_s : none;
+      if (a.entropy) a.entropy[r] = s.m == -INFINITY ? none : h < 0.0f ? 0.0f : h;  // (NaN stays)
+      sh.M = s.m;
+      sh.log_s = log_s;
     }
   }
   if (K > 0) {
-    if (tid < kScoreGroups) sh.all[tid] = cl.map_shared_rank(&sh, tid / (kScoreGroups / C))->groups[tid % (kScoreGroups / C)];
-    if (tid < kScoreTop) sh.best[tid] = 0;
-    if (tid == 0) sh.listed = 0;
-    __syncthreads();
-    if (tid < kScoreGroups) {
-      const float mine = sh.all[tid];
-      int before = 0;
-      for (int j = 0; j < kScoreGroups; ++j) before += sh.all[j] > mine || (sh.all[j] == mine && j < tid);
-      if (before == K - 1) sh.border = mine;
+    if (warp == 0) {
+      // The border: the largest key of 16 bits that K groups reach.
+      uint32_t key[kScoreGroups / 32];
+#pragma unroll
+      for (int i = 0; i < kScoreGroups / 32; ++i) {
+        const int at = i * 32 + lane;
+        key[i] = row_key(cl.map_shared_rank(&sh, at / mine)->groups[at % mine]);
+      }
+      uint32_t low = 0;
+#pragma unroll
+      for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t want = low | 1u << bit;
+        int reach = 0;
+#pragma unroll
+        for (int i = 0; i < kScoreGroups / 32; ++i) reach += key[i] >= want;
+        if (__reduce_add_sync(0xffffffffu, reach) >= K) low = want;
+      }
+      if (lane == 0) sh.border = low > 0x007fffffu ? row_key_value(low) : -INFINITY;  // (the key of -inf)
     }
     __syncthreads();
     const float border = sh.border;
@@ -226,45 +332,60 @@ __global__ void __launch_bounds__(kScoreThreads, 2) k_score_rows(const __grid_co
     // what is not, the first few by index, which is their order.
     const bool few = border == -INFINITY;
     const int first = v0 * VE - row.head, last = min(v1 * VE - row.head, a.vocab);  // this CTA's tokens (first may be < 0)
+    auto put = [&](int at, u64 key) {
+      a.top_ids[(long long)r * K + at] = (int)~(uint32_t)key;
+      a.top_logprobs[(long long)r * K + at] = (row_key_value((uint32_t)(key >> 32)) - sh.M) - sh.log_s;
+    };
     auto list = [&](float x, int i) {
       const int at = atomicAdd(&sh.listed, 1);
       if (at < kScoreList) sh.list[at] = score_key(x, i);
     };
-    for (int v = v0 + tid; v < v1; v += kScoreThreads) {
-      float x[VE];
-      row.load(v, x);
-      float mx = x[0];
+    // The batches that reach it, and then their vectors side by side (one trip to memory, where a thread's own
+    // batches in turn took a trip per vector: 512 rows of bf16 60 us).
+    for (int i = 0; i < kSlots && v0 + tid + i * U * N < v1; ++i)
+      if (sh.most[i][tid] >= border) sh.again[atomicAdd(&sh.batches, 1)] = (unsigned short)(i * N + tid);
+    __syncthreads();
+    for (int j = tid; j < sh.batches * U; j += N) {
+      const int at = sh.again[j / U];
+      for (int w = v0 + at % N + (at / N * U + j % U) * N; w < v1; w += kSlots * U * N) {
+        const uint4 x = row.load(w);
+        if (!(Row::most(x) >= border)) continue;
 #pragma unroll
-      for (int i = 1; i < VE; ++i) mx = fmaxf(mx, x[i]);
-      if (mx >= border) {
+        for (int c = 0; c < VE / 2; ++c) {
+          const float2 f = Row::pair(x, c);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) {
-          const int e = v * VE - row.head + i;
-          if (few ? x[i] > -INFINITY || (x[i] == -INFINITY && e >= 0 && e < last && e < first + kScoreList / 2) : x[i] >= border)
-            list(x[i], e);
+          for (int h = 0; h < 2; ++h) {
+            const float y = h ? f.y : f.x;
+            const int e = w * VE - row.head + 2 * c + h;
+            if (few ? y > -INFINITY || (y == -INFINITY && e >= 0 && e < last && e < first + kScoreList / 2) : y >= border)
+              list(y, e);
+          }
         }
       }
     }
     __syncthreads();
     const int n = sh.listed;
     if (n <= kScoreList && (!few || n >= K || n == last - max(first, 0))) {
-      for (int i = tid; i < n; i += kScoreThreads) {
+      for (int i = tid; i < n; i += N) {
         const u64 mine = sh.list[i];
         int before = 0;
         for (int j = 0; j < n; ++j) before += sh.list[j] > mine;
-        if (before < K) sh.best[before] = mine;
+        if (before < K) {
+          if (C == 1) put(before, mine);
+          else sh.best[before] = mine;
+        }
       }
     } else {  // too many tokens reach the border (long classes of equal values): one after the other
       u64 below = ~0ull;
       for (int k = 0; k < K; ++k) {
         u64 best = 0;
-        for (int v = v0 + tid; v < v1; v += kScoreThreads) {
-          float x[VE];
-          row.load(v, x);
+        for (int v = v0 + tid; v < v1; v += N) {
+          const uint4 x = row.load(v);
 #pragma unroll
           for (int i = 0; i < VE; ++i) {
             const int e = v * VE - row.head + i;
-            const u64 key = score_key(x[i], e);
+            const float2 f = Row::pair(x, i / 2);
+            const u64 key = score_key(i & 1 ? f.y : f.x, e);
             if (e >= 0 && e < last && key < below && key > best) best = key;
           }
         }
@@ -272,41 +393,41 @@ __global__ void __launch_bounds__(kScoreThreads, 2) k_score_rows(const __grid_co
         for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
         if (lane == 0) sh.red[warp] = best;
         __syncthreads();
-        best = sh.red[lane % kScoreWarps];
+        best = sh.red[lane % (N / 32)];
 #pragma unroll
-        for (int o = kScoreWarps / 2; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+        for (int o = (N / 32) / 2; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
         if (best == 0) break;  // (the same in every thread)
-        if (tid == 0) sh.best[k] = best;
+        if (tid == 0) {
+          if (C == 1) put(k, best);
+          else sh.best[k] = best;
+        }
         below = best;
         __syncthreads();
       }
     }
-    cl.sync();
-    if (rank == 0) {  // the CTAs' largest in order
+    if (C > 1) cl.sync();
+    if (C > 1 && rank == 0) {  // the CTAs' largest in order
       const int m = C * K;
-      if (tid < m) sh.list[tid] = cl.map_shared_rank(&sh, tid / K)->best[tid % K];
+      for (int i = tid; i < m; i += N) sh.list[i] = cl.map_shared_rank(&sh, i / K)->best[i % K];
       __syncthreads();
-      if (tid < m) {
-        const u64 mine = sh.list[tid];
+      for (int i = tid; i < m; i += N) {
+        const u64 mine = sh.list[i];
         int before = 0;
         for (int j = 0; j < m; ++j) before += sh.list[j] > mine;
-        if (mine != 0 && before < K) {
-          a.top_ids[(long long)r * K + before] = (int)~(uint32_t)mine;
-          a.top_logprobs[(long long)r * K + before] = (row_key_value((uint32_t)(mine >> 32)) - M) - log_s;
-        }
+        if (mine != 0 && before < K) put(before, mine);
       }
     }
   }
-  cl.sync();  // shared memory is read by others until here
+  if (C > 1) cl.sync();  // shared memory is read by others until here
 }
 
 template <typename T>
 static void launch_score_rows(ScoreArgs a, int rows, cudaStream_t s) {
   constexpr int VE = 16 / sizeof(T);
+  // CTAs per row: as many as fill the GPU twice (a CTA pays 4 us beside its loads: 512 rows of bf16 40 us with one,
+  // 44 with two, 94 with eight; 64 rows of f32 37, 23 and 15.5), none below 2048 tokens.
   int C = 1;
-  while (C < kScoreCluster && ((a.vocab + C - 1) / C > 20480 ||
-                               ((long long)rows * C < 2 * current_sms() && (a.vocab + C - 1) / C > 2048)))
-    C *= 2;
+  while (C < kScoreCluster && (long long)rows * C < 2 * current_sms() && (a.vocab + C - 1) / C > 2048) C *= 2;
   a.per = ((a.vocab + VE - 1) / VE + 1 + C - 1) / C;  // (a row that starts inside a vector has one more)
   if ((long long)rows * C > 0x7fffffffLL) throw QdError{QD_E_RANGE, "qd_score_rows: too many rows"};
   cudaLaunchConfig_t cfg = {};
@@ -324,7 +445,6 @@ static void launch_score_rows(ScoreArgs a, int rows, cudaStream_t s) {
   cfg.numAttrs = 2;
   QD_CK(cudaLaunchKernelEx(&cfg, k_score_rows<T>, a));
 }
-
 }  // namespace qd
 
 extern "C" int qd_score_rows(const void* logits, int dtype, int rows, uint32_t vocab, int64_t row_stride,
