@@ -196,15 +196,26 @@ static void launch_decode(const PAttnArgs& a, void* workspace, cudaStream_t s) {
     launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas);
 }
 
-static void launch_decode_q8(const PAttnArgs& a, PagedScales scale, void* workspace, cudaStream_t s) {
+template <int SETS>
+static void launch_decode_q8(Q8Args q, void* workspace, cudaStream_t s) {
+  const PAttnArgs& a = q.a;
   const int nh = a.kv.kv_heads * ((a.q_heads / a.kv.kv_heads + 7) / 8);
   const long long most = (long long)a.kv.batch * nh * (((long long)a.kv.table_width << a.kv.page_shift) / kQ8Tile + 1);
   if (most > 0x7fffffffLL)
     throw QdError{QD_E_RANGE, "qd_paged_attn_decode_q8: batch * heads * table beyond 2^31 units"};
+  // (an empty pool has no page that could be copied: any address will do)
+  const uint64_t pool = std::max<uint64_t>((uint64_t)a.kv.num_pages * a.kv.kv_heads << a.kv.page_shift, 16);
+  if (pool > 0x7fffffffULL) throw QdError{QD_E_RANGE, "qd_paged_attn_decode_q8: a pool beyond 2^31 rows"};
+  std::string err;
+  for (const bool v : {false, true})
+    if (!make_tmap_2d(v ? &q.tv : &q.tk, a.kv.num_pages == 0 ? a.q : v ? a.kv.v : a.kv.k, CU_TENSOR_MAP_DATA_TYPE_UINT8,
+                      kHeadDim, pool, kHeadDim, kHeadDim, 16, CU_TENSOR_MAP_SWIZZLE_128B, &err))
+      throw QdError{QD_E_CUDA, err};
   static unsigned long long smem_set = 0;
-  allow_smem(k_paged_decode_q8, pq8_smem(4096), smem_set);
-  const int ctas = (int)std::max(1LL, std::min<long long>(most, std::min(2 * current_sms(), kPdMaxCtas)));
-  launch_ex(k_paged_decode_q8, dim3(ctas), dim3(kPdThreads), (size_t)pq8_smem(a.kv.batch), s, a, scale, workspace);
+  allow_smem(k_paged_decode_q8<SETS>, pq8_smem(4096), smem_set);
+  const int per_sm = SETS == 1 ? kQ8PerSm : 2;
+  const int ctas = (int)std::max(1LL, std::min<long long>(most, std::min(per_sm * current_sms(), kPdMaxCtas)));
+  launch_ex(k_paged_decode_q8<SETS>, dim3(ctas), dim3(kPdThreads), (size_t)pq8_smem(a.kv.batch), s, q, workspace);
   // (a table of one unit leaves nothing to join)
   if ((a.kv.table_width << a.kv.page_shift) > kQ8Tile)
     launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas);
@@ -440,7 +451,12 @@ int qd_paged_attn_decode_q8(const qd_paged_q8* kv, const void* q, int dtype, int
     if (a.rows == 0) return;
     need(workspace != nullptr, "qd_paged_attn_decode_q8: NULL workspace");
     need(aligned16(workspace), "qd_paged_attn_decode_q8: the workspace must be 16-byte aligned");
-    launch_decode_q8(a, {kv->k_scale, kv->v_scale}, workspace, static_cast<cudaStream_t>(stream));
+    Q8Args args{};
+    args.a = a;
+    args.scale = {kv->k_scale, kv->v_scale};
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (q_heads / kv->kv_heads <= 4) launch_decode_q8<1>(args, workspace, s);
+    else launch_decode_q8<2>(args, workspace, s);
   });
 }
 

@@ -39,7 +39,7 @@ constexpr int kPdThreads = 128;
 constexpr int kPdTile = 64;          // positions per unit
 constexpr int kPdStages = 3;
 constexpr int kPdSlot = 2 * 16 * 256;  // K and V rows of 16 positions
-constexpr int kPdMaxCtas = 320;
+constexpr int kPdMaxCtas = 480;
 constexpr float kPdLag = 8.0f;       // log2 a running maximum may fall behind before the sums are rescaled
 constexpr float kPdShift = 7.0f;     // weights are kept times 2^7: with the lag below 2^15 < 65504, and small
                                      // weights stay in f16's normal range down to 2^-21 of the largest

@@ -99,25 +99,38 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_read_q8(const __grid_const
 }
 
 // ---- attention of one new token per sequence ---------------------------------------------------
-// As k_paged_decode (units in equal runs per CTA, a ring of copies per warp, hi / lo operand rows on mma.sync,
-// parts joined by k_paged_decode_join), over half the bytes, so a warp takes 32 positions of a unit of 128:
+// As k_paged_decode (units in equal runs per CTA, a ring of copies per warp, parts joined by
+// k_paged_decode_join), over half the bytes, which leaves instructions as the next bound, so:
+//  - A warp takes 32 positions of a unit of 128. TMA copies them, 16 rows of one page at a time, with the swizzle
+//    that the loads from shared memory want; one lane per 16 rows asks for them.
 //  - The integers are exact in f16 and feed the products as they are (byte permutes and one subtraction per pair, in
 //    registers). A K row's scale multiplies its scores, a V row's its weight: y = sum_j (p_j vs_j) n_j.
-//  - Products may take the contraction's index in any order that both operands share. Thread t of a quad takes dims
-//    32 t .. 32 t + 31 of a K row (two 16-byte loads, no transposition) and of V, for the quad's
-//    8 dim groups, 16 consecutive dims of its own four positions of 16.
+//  - mma.sync m16n8k16 with keys (dims of V) as the 16 rows and query heads as the 8 columns: four heads, each as a
+//    column of its 16-bit part and one of the rest, which meet in one thread, so that nothing is
+//    spent on the eight rows that two heads would leave empty the other way round (82 us for the 64 sequences below).
+//    The contraction's index may have any order that both operands share: thread t of a quad takes dims 32 t .. + 31
+//    of a K row (two 16-byte loads) and 16 consecutive dims of four positions of V. The weights'
+//    fragments are those of the scores transposed (movmatrix).
 //  - The weights p_j vs_j go into f16 parts, and a V row's scale may have any size beside its weight (the first
 //    token's V is small in many models, and its weight large), so they have a running maximum of their own, of
 //    s_j + log2 vs_j, next to that of s_j, by which the weights' sum goes.
-constexpr int kQ8Tile = 128, kQ8Stages = 3;
-constexpr int kQ8Rows = 32;                                  // positions of a warp
-constexpr int kQ8Slot = 2 * kQ8Rows * 128 + 2 * kQ8Rows * 4;  // K, V, their scales
+// SETS: column sets of four heads; one for up to four query heads to a KV head, else two.
+constexpr int kQ8Tile = 128, kQ8Stages = 2;
+constexpr int kQ8Rows = 32;                 // positions of a warp
+constexpr int kQ8Slot = 2 * kQ8Rows * 128;  // K and V
+constexpr int kQ8Scales = 2 * kQ8Rows * 4;  // their scales
+constexpr int kQ8PerSm = 3;                 // CTAs
 static_assert(8 * kPdSumRow * 4 <= kQ8Slot, "a slot holds eight heads' sums");
-__host__ __device__ constexpr int pq8_smem(int batch) { return 4 * kQ8Stages * kQ8Slot + (batch + 1) * 4; }
-
-__device__ __forceinline__ void cp_async4(unsigned dst, const void* src, bool live) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
+__host__ __device__ constexpr int pq8_smem(int batch) {
+  return 1024 + 4 * kQ8Stages * (kQ8Slot + kQ8Scales) + (batch + 1) * 4;
 }
+
+struct Q8Args {
+  CUtensorMap tk, tv;  // boxes of 16 rows
+  PAttnArgs a;
+  PagedScales scale;
+};
+
 __device__ __forceinline__ float log2_fast(float x) {
   float y;
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -128,27 +141,43 @@ __device__ __forceinline__ uint4 lds128(unsigned addr) {
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr));
   return r;
 }
-__device__ __forceinline__ float2 lds64f(unsigned addr) {
-  float2 r;
-  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(r.x), "=f"(r.y) : "r"(addr));
+__device__ __forceinline__ float lds32f(unsigned addr) {
+  float r;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(addr));
   return r;
 }
+__device__ __forceinline__ unsigned transpose_b16(unsigned x) {  // an 8 x 8 matrix over the warp
+  unsigned y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 
-__global__ void __launch_bounds__(kPdThreads) k_paged_decode_q8(const __grid_constant__ PAttnArgs a,
-                                                                const __grid_constant__ PagedScales scale,
-                                                                void* workspace) {
-  extern __shared__ __align__(128) unsigned char smem[];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+template <int SETS>
+__global__ void __launch_bounds__(kPdThreads, SETS == 1 ? kQ8PerSm : 2) k_paged_decode_q8(const __grid_constant__ Q8Args qa,
+                                                                                       void* workspace) {
+  const PAttnArgs& a = qa.a;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   unsigned char* ring = smem + warp * kQ8Stages * kQ8Slot;
-  int* first = reinterpret_cast<int*>(smem + 4 * kQ8Stages * kQ8Slot);
+  unsigned char* scales = smem + 4 * kQ8Stages * kQ8Slot + warp * kQ8Stages * kQ8Scales;
+  int* first = reinterpret_cast<int*>(smem + 4 * kQ8Stages * (kQ8Slot + kQ8Scales));
+  __shared__ unsigned long long full[4][kQ8Stages];
   __shared__ float2 sml[4][8];  // maximum and sum of weights of each warp and head,
   __shared__ float smo[4][8];   // the maximum that its sums go by
   const int G = a.q_heads / a.kv.kv_heads, subs = (G + 7) >> 3, nh = a.kv.kv_heads * subs, B = a.kv.batch;
   const PDecodeWs ws = pd_ws(workspace);
+  if (tid == 0) {
+    tma_prefetch_map(&qa.tk);
+    tma_prefetch_map(&qa.tv);
+    for (int i = 0; i < 4 * kQ8Stages; ++i) tc_mbar_init(&full[0][0] + i);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   pdl_wait();
   pdl_trigger();
   auto see = [&](int b) { return visible<kQ8Tile>(a.kv.seq_lens[b], paged_len(a.kv, b), a.window, a.sinks); };
-  pd_units(B, first, see);
+  pd_units(B, first, see);  // (its barriers are the mbarriers' too)
   if (blockIdx.x == 0) {
     for (int b = tid; b <= B; b += kPdThreads) ws.first[b] = first[b];
     for (int b = tid; b < B; b += kPdThreads)  // (paged_len cuts both)
@@ -166,7 +195,7 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode_q8(const __grid_con
   PdCursor pre = cur;  // the copies run ahead of the sums
   const int n_units = u1 - u0;
 
-  // page of the 16 positions that this half of the warp copies of the unit at `pre`; -1: nothing visible there, -2: bad
+  // page of the 16 positions that this half of the warp asks for of the unit at `pre`; -1: nothing visible there, -2: bad
   auto page_of = [&](const PdCursor& c) {
     const int p0 = c.v.tile(c.t) * kQ8Tile + kQ8Rows * warp + (lane & 16);
     const bool any = p0 < c.v.end && (p0 + 16 > c.v.lo || p0 < c.v.ns);
@@ -176,214 +205,224 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode_q8(const __grid_con
   };
   int next_page = page_of(pre);
   unsigned live_ring = 0;  // bits 2 i, 2 i + 1: the halves of slot i hold rows
+  unsigned phases = 0;     // bit i: parity of slot i's barrier
   int issued = 0, in_slot = 0;
-  const int pmask = (1 << a.kv.page_shift) - 1;
-  const unsigned ring_s = (unsigned)__cvta_generic_to_shared(ring);
-  // lane l copies chunk l % 8 of rows 4 i + l / 8; chunk c of row r sits at c ^ (r % 8). Scales: lane l row l.
-  unsigned to[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = 4 * i + (lane >> 3);
-    to[i] = ring_s + r * 128 + (((lane & 7) ^ (r & 7)) << 4);
-  }
+  bool gone = false;  // a copy has not come in time
   auto issue = [&]() {
-    if (issued < n_units) {
-      const int page = next_page;
-      const unsigned good = __ballot_sync(0xffffffffu, page >= 0);
-      const unsigned halves = (good & 1u) | ((good >> 16 & 1u) << 1);
-      live_ring = (live_ring & ~(3u << (2 * in_slot))) | halves << (2 * in_slot);
-      if (page == -2 && (lane & 15) == 0) paged_flag(a.kv, QD_PAGED_BAD_PAGE);
-      const int p0 = pre.v.tile(pre.t) * kQ8Tile + kQ8Rows * warp;
-      const unsigned dst = in_slot * kQ8Slot;
-      // first row of this lane's half (of its scale), and of both halves
-      const long long mine = (((long long)max(page, 0) * a.kv.kv_heads + pre.g) << a.kv.page_shift) + ((p0 + (lane & 16)) & pmask);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const long long row0 = __shfl_sync(0xffffffffu, mine, 16 * h);
-        if (!(halves >> h & 1u)) continue;
-        const char* ks = static_cast<const char*>(a.kv.k) + row0 * 128 + lane * 16;
-        const char* vs = static_cast<const char*>(a.kv.v) + row0 * 128 + lane * 16;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool ok = pre.v.at(p0 + 16 * h + 4 * i + (lane >> 3));
-          cp_async16(to[i & 1] + dst + 2048 * h + (i >> 1) * 1024, ks + i * 512, ok);
-          cp_async16(to[i & 1] + dst + 2048 * h + (i >> 1) * 1024 + 4096, vs + i * 512, ok);
-        }
-      }
-      if (page >= 0) {
-        const bool ok = pre.v.at(p0 + lane);
-        cp_async4(ring_s + dst + 8192 + lane * 4, scale.k + mine + (lane & 15), ok);
-        cp_async4(ring_s + dst + 8320 + lane * 4, scale.v + mine + (lane & 15), ok);
-      }
-      ++issued;
-      in_slot = in_slot + 1 == kQ8Stages ? 0 : in_slot + 1;
-      if (issued < n_units) {
-        step(pre);
-        next_page = page_of(pre);
-      }
+    if (issued >= n_units || gone) return;
+    const int page = next_page;
+    const unsigned good = __ballot_sync(0xffffffffu, page >= 0);
+    const unsigned halves = (good & 1u) | (good >> 16 & 1u) << 1;
+    live_ring = (live_ring & ~(3u << (2 * in_slot))) | halves << (2 * in_slot);
+    if (page == -2 && (lane & 15) == 0) paged_flag(a.kv, QD_PAGED_BAD_PAGE);
+    unsigned long long* bar = &full[warp][in_slot];
+    if (lane == 0 && halves)
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc_smem(bar)),
+                   "r"((halves == 3u ? 2 : 1) * (2 * 16 * 128 + 2 * 16 * 4))
+                   : "memory");
+    __syncwarp();
+    if ((lane & 15) == 0 && page >= 0) {
+      const int p0 = pre.v.tile(pre.t) * kQ8Tile + kQ8Rows * warp + lane;
+      const int row = ((page * a.kv.kv_heads + pre.g) << a.kv.page_shift) + (p0 & ((1 << a.kv.page_shift) - 1));
+      unsigned char* d = ring + in_slot * kQ8Slot + lane * 128;
+      unsigned char* s = scales + in_slot * kQ8Scales + lane * 4;
+      tma_load_2d(d, &qa.tk, 0, row, bar);
+      tma_load_2d(d + kQ8Rows * 128, &qa.tv, 0, row, bar);
+      bulk_load(s, qa.scale.k + row, 64, bar);
+      bulk_load(s + kQ8Rows * 4, qa.scale.v + row, 64, bar);
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    ++issued;
+    in_slot = in_slot + 1 == kQ8Stages ? 0 : in_slot + 1;
+    if (issued < n_units) {
+      step(pre);
+      next_page = page_of(pre);
+    }
   };
 #pragma unroll
   for (int i = 0; i < kQ8Stages - 1; ++i) issue();
 
-  // The queries of a (sequence, head), fetched a unit before they are needed: lane l has head l / 4, dims
-  // 32 (l % 4) .. + 31, pairs qn[i] of them.
+  // The queries of a (sequence, head): lane l has column l / 4 of the products (of set s head 4 s + l / 8, its 16-bit part
+  // or the rest), dims 32 (l % 4) .. + 31; the scores and sums of head 4 s + l % 4.
   const float qs = a.scale * kLog2e;
   const int t4 = lane & 3, g8 = lane >> 2;
-  float2 qn[16];
-  auto fetch_q = [&](const PdCursor& c) {
-    const int hs = c.sub * 8 + g8;
-    const bool live = hs < G;
-    const long long base = c.b * a.q_stride + ((long long)c.g * G + (live ? hs : 0)) * kHeadDim + 32 * t4;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) qn[i] = load2(a.q, base + 2 * i, a.dtype);
-    if (!live) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) qn[i] = make_float2(0.f, 0.f);
-    }
-  };
-  fetch_q(cur);
-  unsigned q[8][4];
-  float o[16][4], m = -INFINITY, mo = -INFINITY, l = 0.0f;
-  float factor = qs;   // of q's products
-  bool fresh = true;   // a new (sequence, head): take its q, clear the sums
-  int seg = 0;         // segments finished by this CTA
+  unsigned q[SETS][8][2];
+  float o[SETS][8][4], m[SETS], mo[SETS], l[SETS], factor[SETS];
+  bool fresh = true;  // a new (sequence, head): take its q, clear the sums
+  int seg = 0;        // segments finished by this CTA
   bool from_start = cur.t == 0;
   int slot = 0;
   for (int i = 0; i < n_units; ++i) {
     issue();
     if (fresh) {
       fresh = false;
-      float top = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 16; ++k) top = fmaxf(top, fmaxf(fabsf(qn[k].x), fabsf(qn[k].y)));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float2 fit = f16_fit(__float_as_int(top) >> 23);
-      factor = qs * fit.y;
+      for (int n = 0; n < SETS; ++n) {
+        const int hs = cur.sub * 8 + 4 * n + (g8 >> 1);
+        const bool live = hs < G;
+        const long long base = cur.b * a.q_stride + ((long long)cur.g * G + (live ? hs : 0)) * kHeadDim + 32 * t4;
+        float2 x[16];
+        float top = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        split2<__half>(qn[2 * k].x * fit.x, qn[2 * k].y * fit.x, q[k][0], q[k][1]);
-        split2<__half>(qn[2 * k + 1].x * fit.x, qn[2 * k + 1].y * fit.x, q[k][2], q[k][3]);
+        for (int k = 0; k < 16; ++k) x[k] = load2(a.q, base + 2 * k, a.dtype);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          if (!live) x[k] = make_float2(0.f, 0.f);
+          top = fmaxf(top, fmaxf(fabsf(x[k].x), fabsf(x[k].y)));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float2 fit = f16_fit(__float_as_int(top) >> 23);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            unsigned hi, lo;
+            split2<__half>(x[2 * k + e].x * fit.x, x[2 * k + e].y * fit.x, hi, lo);
+            q[n][k][e] = g8 & 1 ? lo : hi;
+          }
+        factor[n] = qs * __shfl_sync(0xffffffffu, fit.y, 8 * t4);  // of head t4: columns 2 t4, 2 t4 + 1
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.0f;
+        m[n] = mo[n] = -INFINITY;
+        l[n] = 0.0f;
       }
-#pragma unroll
-      for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-      m = mo = -INFINITY;
-      l = 0.0f;
     }
     const bool last_t = cur.t + 1 == cur.v.tiles, more = i + 1 < n_units;
-    PdCursor nxt = cur;
-    if (more) {
-      step(nxt);
-      if (last_t) fetch_q(nxt);
+    unsigned halves = live_ring >> (2 * slot) & 3u;
+    if (halves && !gone) {
+      gone = !__all_sync(0xffffffffu, tc_mbar_wait(&full[warp][slot], phases >> slot & 1u));
+      if (gone) {
+        if (lane == 0) paged_flag(a.kv, QD_PAGED_TIMEOUT);
+      } else {
+        phases ^= 1u << slot;
+        live_ring &= ~(3u << (2 * slot));
+      }
     }
-    const unsigned halves = live_ring >> (2 * slot) & 3u;
-    asm volatile("cp.async.wait_group %0;" ::"n"(kQ8Stages - 1) : "memory");
-    __syncwarp();
+    if (gone) {  // what this warp held becomes NaN
+      halves = 0;
+#pragma unroll
+      for (int n = 0; n < SETS; ++n) l[n] = __int_as_float(0x7fffffff);
+    }
     if (halves) {
-      const unsigned kb = ring_s + slot * kQ8Slot, vb = kb + 4096;
+      const unsigned kb = tc_smem(ring) + slot * kQ8Slot, vb = kb + kQ8Rows * 128;
+      const unsigned sb = tc_smem(scales) + slot * kQ8Scales + g8 * 4;
       const int p0 = cur.v.tile(cur.t) * kQ8Tile + kQ8Rows * warp;
       const bool inside = halves == 3u && p0 + 32 <= cur.v.end && (p0 >= cur.v.lo || p0 + 32 <= cur.v.ns);
-      float p[4][2], u[4][2];  // of positions 8 j + 2 t + {0, 1}: scores, and with V's scale
+      float p[SETS][4], u[SETS][4];  // of positions 8 j + g8: scores, and with V's scale
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float s[2][4];
+      for (int h = 0; h < 2; ++h) {
+        float s[SETS][2][4];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) s[e][0] = s[e][1] = s[e][2] = s[e][3] = 0.0f;
-        const unsigned row = kb + (8 * j + g8) * 128;
+        for (int n = 0; n < SETS; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) s[n][e][0] = s[n][e][1] = s[n][e][2] = s[n][e][3] = 0.0f;
+        const unsigned row = kb + (16 * h + g8) * 128;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const uint4 x = lds128(row + (((2 * t4 + c) ^ g8) << 4));
-          const unsigned w[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
+          const unsigned at = row + (((2 * t4 + c) ^ g8) << 4);
+          const uint4 x = lds128(at), y = lds128(at + 1024);
+          const unsigned xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_16816<__half>(s[c], q[4 * c + k], q8_half2(w[k], kQ8Lo), q8_half2(w[k], kQ8Hi));
+          for (int k = 0; k < 4; ++k) {
+            const unsigned v = xw[k] ^ 0x80808080u, w = yw[k] ^ 0x80808080u;
+            const unsigned f[4] = {q8_half2(v, kQ8Lo), q8_half2(w, kQ8Lo), q8_half2(v, kQ8Hi), q8_half2(w, kQ8Hi)};
+#pragma unroll
+            for (int n = 0; n < SETS; ++n) mma_16816<__half>(s[n][k & 1], f, q[n][4 * c + k][0], q[n][4 * c + k][1]);
+          }
         }
-        const float2 ks = lds64f(kb + 8192 + (8 * j + 2 * t4) * 4), vs = lds64f(kb + 8320 + (8 * j + 2 * t4) * 4);
-        p[j][0] = ((s[0][0] + s[1][0]) + (s[0][2] + s[1][2])) * (factor * ks.x);
-        p[j][1] = ((s[0][1] + s[1][1]) + (s[0][3] + s[1][3])) * (factor * ks.y);
-        u[j][0] = p[j][0] + log2_fast(vs.x);
-        u[j][1] = p[j][1] + log2_fast(vs.y);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int j = 2 * h + e;
+          const float ks = lds32f(sb + 32 * j), lv = log2_fast(lds32f(sb + 32 * j + kQ8Rows * 4));
+#pragma unroll
+          for (int n = 0; n < SETS; ++n) {
+            p[n][j] = ((s[n][0][2 * e] + s[n][1][2 * e]) + (s[n][0][2 * e + 1] + s[n][1][2 * e + 1])) * (factor[n] * ks);
+            u[n][j] = p[n][j] + lv;
+          }
+        }
       }
       if (!inside) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
+          if (!(halves >> (j >> 1) & 1u) || !cur.v.at(p0 + 8 * j + g8))
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (!(halves >> (j >> 1) & 1u) || !cur.v.at(p0 + 8 * j + 2 * t4 + e)) p[j][e] = u[j][e] = -INFINITY;
+            for (int n = 0; n < SETS; ++n) p[n][j] = u[n][j] = -INFINITY;
       }
-      float mt = -INFINITY, ut = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        mt = fmaxf(mt, fmaxf(p[j][0], p[j][1]));
-        ut = fmaxf(ut, fmaxf(u[j][0], u[j][1]));
-      }
-      mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
-      ut = fmaxf(ut, __shfl_xor_sync(0xffffffffu, ut, 1));
-      mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
-      ut = fmaxf(ut, __shfl_xor_sync(0xffffffffu, ut, 2));
-      if (__any_sync(0xffffffffu, mt > m + kPdLag || ut > mo + kPdLag)) {  // some head's maximum moved: rescale
-        const float mn = mt > m + kPdLag ? mt : m, un = ut > mo + kPdLag ? ut : mo;
-        l *= m == -INFINITY ? 0.0f : exp2_fast(m - mn);
-        const float f = mo == -INFINITY ? 0.0f : exp2_fast(mo - un);
-        m = mn;
-        mo = un;
+      for (int n = 0; n < SETS; ++n) {
+        float mt = fmaxf(fmaxf(p[n][0], p[n][1]), fmaxf(p[n][2], p[n][3]));
+        float ut = fmaxf(fmaxf(u[n][0], u[n][1]), fmaxf(u[n][2], u[n][3]));
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          o[j][0] *= f;
-          o[j][1] *= f;
-          o[j][2] *= f;
-          o[j][3] *= f;
+        for (int x = 4; x < 32; x <<= 1) {
+          mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
+          ut = fmaxf(ut, __shfl_xor_sync(0xffffffffu, ut, x));
+        }
+        if (__any_sync(0xffffffffu, mt > m[n] + kPdLag || ut > mo[n] + kPdLag)) {  // some head's maximum moved: rescale
+          const float mn = mt > m[n] + kPdLag ? mt : m[n], un = ut > mo[n] + kPdLag ? ut : mo[n];
+          l[n] *= m[n] == -INFINITY ? 0.0f : exp2_fast(m[n] - mn);
+          const float f = mo[n] == -INFINITY ? 0.0f : exp2_fast(mo[n] - un);
+          m[n] = mn;
+          mo[n] = un;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][j][e] *= f;
+        }
+        const float ref = m[n] == -INFINITY ? 0.0f : m[n], uref = mo[n] == -INFINITY ? 0.0f : mo[n] - kPdShift;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          l[n] += exp2_fast(p[n][j] - ref);
+          u[n][j] = exp2_fast(u[n][j] - uref);
         }
       }
-      const float ref = m == -INFINITY ? 0.0f : m, uref = mo == -INFINITY ? 0.0f : mo - kPdShift;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          l += exp2_fast(p[j][e] - ref);
-          u[j][e] = exp2_fast(u[j][e] - uref);
-        }
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
-        unsigned w[4];
-        split2<__half>(u[2 * st][0], u[2 * st][1], w[0], w[1]);
-        split2<__half>(u[2 * st + 1][0], u[2 * st + 1][1], w[2], w[3]);
+        unsigned w[SETS][2];
+#pragma unroll
+        for (int n = 0; n < SETS; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {  // a weight as its 16-bit part and the rest, for the columns of its head
+            const float x = u[n][2 * st + e];
+            const float hi = __half2float(__float2half_rn(x));
+            w[n][e] = transpose_b16(pack2<__half>(hi, x - hi));
+          }
         // rows 16 st + 2 t + {0, 1, 8, 9}, chunk g8
-        const int r = 2 * t4;
-        const unsigned row = vb + (16 * st + r) * 128;
-        const uint4 x0 = lds128(row + ((g8 ^ r) << 4)), x1 = lds128(row + 128 + ((g8 ^ (r + 1)) << 4));
-        const uint4 x2 = lds128(row + 1024 + ((g8 ^ r) << 4)), x3 = lds128(row + 1152 + ((g8 ^ (r + 1)) << 4));
-        const unsigned va[4] = {x0.x, x0.y, x0.z, x0.w}, vbb[4] = {x1.x, x1.y, x1.z, x1.w};
-        const unsigned vc[4] = {x2.x, x2.y, x2.z, x2.w}, vd[4] = {x3.x, x3.y, x3.z, x3.w};
+        const unsigned row = vb + (16 * st + 2 * t4) * 128, c0 = (g8 ^ (2 * t4)) << 4, c1 = (g8 ^ (2 * t4 + 1)) << 4;
+        const uint4 x0 = lds128(row + c0), x1 = lds128(row + 128 + c1);
+        const uint4 x2 = lds128(row + 1024 + c0), x3 = lds128(row + 1152 + c1);
+        const unsigned va[4] = {x0.x, x0.y, x0.z, x0.w}, vc[4] = {x1.x, x1.y, x1.z, x1.w};
+        const unsigned vd[4] = {x2.x, x2.y, x2.z, x2.w}, ve[4] = {x3.x, x3.y, x3.z, x3.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const unsigned a0 = __byte_perm(va[k], vbb[k], 0x5140) ^ 0x80808080u, a1 = __byte_perm(va[k], vbb[k], 0x7362) ^ 0x80808080u;
-          const unsigned b0 = __byte_perm(vc[k], vd[k], 0x5140) ^ 0x80808080u, b1 = __byte_perm(vc[k], vd[k], 0x7362) ^ 0x80808080u;
-          mma_16816<__half>(o[4 * k], w, q8_half2(a0, kQ8Lo), q8_half2(b0, kQ8Lo));
-          mma_16816<__half>(o[4 * k + 1], w, q8_half2(a0, kQ8Hi), q8_half2(b0, kQ8Hi));
-          mma_16816<__half>(o[4 * k + 2], w, q8_half2(a1, kQ8Lo), q8_half2(b1, kQ8Lo));
-          mma_16816<__half>(o[4 * k + 3], w, q8_half2(a1, kQ8Hi), q8_half2(b1, kQ8Hi));
+          const unsigned a0 = __byte_perm(va[k], vc[k], 0x5140) ^ 0x80808080u, a1 = __byte_perm(va[k], vc[k], 0x7362) ^ 0x80808080u;
+          const unsigned b0 = __byte_perm(vd[k], ve[k], 0x5140) ^ 0x80808080u, b1 = __byte_perm(vd[k], ve[k], 0x7362) ^ 0x80808080u;
+          const unsigned f[4] = {q8_half2(a0, kQ8Lo), q8_half2(a0, kQ8Hi), q8_half2(b0, kQ8Lo), q8_half2(b0, kQ8Hi)};
+          const unsigned f2[4] = {q8_half2(a1, kQ8Lo), q8_half2(a1, kQ8Hi), q8_half2(b1, kQ8Lo), q8_half2(b1, kQ8Hi)};
+#pragma unroll
+          for (int n = 0; n < SETS; ++n) {
+            mma_16816<__half>(o[n][2 * k], f, w[n][0], w[n][1]);
+            mma_16816<__half>(o[n][2 * k + 1], f2, w[n][0], w[n][1]);
+          }
         }
       }
     }
     __syncwarp();  // the slot may be refilled
     if (last_t || !more) {
-      // The (sequence, head), or this CTA's part of it, ends: join the four warps.
-      l += __shfl_xor_sync(0xffffffffu, l, 1);
-      l += __shfl_xor_sync(0xffffffffu, l, 2);
-      float* mine = reinterpret_cast<float*>(ring + slot * kQ8Slot) + g8 * kPdSumRow + 32 * t4;
+      // The (sequence, head), or this CTA's part of it, ends: join the four warps. The sums go to the slot that has
+      // just been read: dims 16 g8 .. + 15 of head t4 of each set.
 #pragma unroll
-      for (int j = 0; j < 16; j += 4) {
-        *reinterpret_cast<float4*>(mine + j) = make_float4(o[j][0] + o[j][2], o[j + 1][0] + o[j + 1][2],
-                                                           o[j + 2][0] + o[j + 2][2], o[j + 3][0] + o[j + 3][2]);
-        *reinterpret_cast<float4*>(mine + 16 + j) = make_float4(o[j][1] + o[j][3], o[j + 1][1] + o[j + 1][3],
-                                                                o[j + 2][1] + o[j + 2][3], o[j + 3][1] + o[j + 3][3]);
-      }
-      if (t4 == 0) {
-        sml[warp][g8] = make_float2(m, l);
-        smo[warp][g8] = mo;
+      for (int n = 0; n < SETS; ++n) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[n] += __shfl_xor_sync(0xffffffffu, l[n], x);
+        float* mine = reinterpret_cast<float*>(ring + slot * kQ8Slot) + (4 * n + t4) * kPdSumRow + 16 * g8;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2)
+          *reinterpret_cast<float4*>(mine + 2 * j) = make_float4(o[n][j][0] + o[n][j][1], o[n][j][2] + o[n][j][3],
+                                                                 o[n][j + 1][0] + o[n][j + 1][1], o[n][j + 1][2] + o[n][j + 1][3]);
+        if (g8 == 0) {
+          sml[warp][4 * n + t4] = make_float2(m[n], l[n]);
+          smo[warp][4 * n + t4] = mo[n];
+        }
       }
       __syncthreads();
       const int live = min(8, G - cur.sub * 8);
@@ -395,7 +434,7 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode_q8(const __grid_con
         float L = 0.0f, x = 0.0f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          L += sml[w][h].x == -INFINITY ? sml[w][h].y * 0.0f : sml[w][h].y * exp2_fast(sml[w][h].x - M);
+          L += sml[w][h].y * (sml[w][h].x == -INFINITY ? 0.0f : exp2_fast(sml[w][h].x - M));  // (NaN stays)
           const float f = smo[w][h] == -INFINITY ? 0.0f : exp2_fast(smo[w][h] - kPdShift - M);
           x += reinterpret_cast<const float*>(smem + (w * kQ8Stages + slot) * kQ8Slot)[h * kPdSumRow + tid] * f;
         }
@@ -406,14 +445,18 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode_q8(const __grid_con
           if (tid == 0) ws.ml[part + h] = make_float2(M, L);
         }
       }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncthreads();  // before the slots are refilled
       ++seg;
       fresh = true;
       from_start = true;
     }
-    cur = nxt;
+    if (more) step(cur);
     slot = slot + 1 == kQ8Stages ? 0 : slot + 1;
   }
+  if (gone)  // nothing may still be landing when the CTA ends
+    for (int i = 0; i < kQ8Stages; ++i)
+      if (live_ring >> (2 * i) & 3u) (void)tc_mbar_wait(&full[warp][i], phases >> i & 1u);
 }
 
 }  // namespace qd
