@@ -196,7 +196,7 @@ static void launch_decode(const PAttnArgs& a, void* workspace, cudaStream_t s) {
     launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas);
 }
 
-template <int SETS>
+template <typename Heads>
 static void launch_decode_q8(Q8Args q, void* workspace, cudaStream_t s) {
   const PAttnArgs& a = q.a;
   const int nh = a.kv.kv_heads * ((a.q_heads / a.kv.kv_heads + 7) / 8);
@@ -212,10 +212,9 @@ static void launch_decode_q8(Q8Args q, void* workspace, cudaStream_t s) {
                       kHeadDim, pool, kHeadDim, kHeadDim, 16, CU_TENSOR_MAP_SWIZZLE_128B, &err))
       throw QdError{QD_E_CUDA, err};
   static unsigned long long smem_set = 0;
-  allow_smem(k_paged_decode_q8<SETS>, pq8_smem(4096), smem_set);
-  const int per_sm = SETS == 1 ? kQ8PerSm : 2;
-  const int ctas = (int)std::max(1LL, std::min<long long>(most, std::min(per_sm * current_sms(), kPdMaxCtas)));
-  launch_ex(k_paged_decode_q8<SETS>, dim3(ctas), dim3(kPdThreads), (size_t)pq8_smem(a.kv.batch), s, q, workspace);
+  allow_smem(k_paged_decode_q8<Heads>, pq8_smem(4096), smem_set);
+  const int ctas = (int)std::max(1LL, std::min<long long>(most, std::min(Heads::kCtas * current_sms(), kPdMaxCtas)));
+  launch_ex(k_paged_decode_q8<Heads>, dim3(ctas), dim3(kPdThreads), (size_t)pq8_smem(a.kv.batch), s, q, workspace);
   // (a table of one unit leaves nothing to join)
   if ((a.kv.table_width << a.kv.page_shift) > kQ8Tile)
     launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas);
@@ -455,8 +454,10 @@ int qd_paged_attn_decode_q8(const qd_paged_q8* kv, const void* q, int dtype, int
     args.a = a;
     args.scale = {kv->k_scale, kv->v_scale};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (q_heads / kv->kv_heads <= 4) launch_decode_q8<1>(args, workspace, s);
-    else launch_decode_q8<2>(args, workspace, s);
+    const int group = q_heads / kv->kv_heads;
+    if (group <= 2) launch_decode_q8<Q8Whole<1>>(args, workspace, s);
+    else if (group <= 4) launch_decode_q8<Q8Whole<2>>(args, workspace, s);
+    else launch_decode_q8<Q8Half>(args, workspace, s);
   });
 }
 

@@ -103,23 +103,25 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_read_q8(const __grid_const
 // k_paged_decode_join), over half the bytes, which leaves instructions as the next bound, so:
 //  - A warp takes 32 positions of a unit of 128. TMA copies them, 16 rows of one page at a time, with the swizzle
 //    that the loads from shared memory want; one lane per 16 rows asks for them.
-//  - The integers are exact in f16 and feed the products as they are (byte permutes and one subtraction per pair, in
-//    registers). A K row's scale multiplies its scores, a V row's its weight: y = sum_j (p_j vs_j) n_j.
-//  - mma.sync m16n8k16 with keys (dims of V) as the 16 rows and query heads as the 8 columns: four heads, each as a
-//    column of its 16-bit part and one of the rest, which meet in one thread, so that nothing is
-//    spent on the eight rows that two heads would leave empty the other way round (82 us for the 64 sequences below).
-//    The contraction's index may have any order that both operands share: thread t of a quad takes dims 32 t .. + 31
-//    of a K row (two 16-byte loads) and 16 consecutive dims of four positions of V. The weights'
-//    fragments are those of the scores transposed (movmatrix).
-//  - The weights p_j vs_j go into f16 parts, and a V row's scale may have any size beside its weight (the first
-//    token's V is small in many models, and its weight large), so they have a running maximum of their own, of
-//    s_j + log2 vs_j, next to that of s_j, by which the weights' sum goes.
-// SETS: column sets of four heads; one for up to four query heads to a KV head, else two.
+//  - mma.sync with keys (dims of V) as the 16 rows and query heads as the 8 columns, so that nothing is spent on
+//    the eight rows that two heads would leave empty the other way round.
+//  - A K row's scale multiplies its scores, a V row's its weight: y = sum_j (p_j vs_j) n_j. The products take the
+//    cache's integers, and the other operand as a sum of parts that are columns side by side:
+//      up to four heads to a KV head (Q8Whole): m16n8k32 of 8-bit integers, q and the weights as 31-bit fixed-point
+//      numbers in four signed bytes, exact sums in 32 bits. K goes into it as it lies in memory, V transposed by bytes
+//      in registers;
+//      more heads (Q8Half): m16n8k16 of f16, the integers made f16 (byte permutes and a subtraction per pair), q and the
+//      weights as two f16. Its products are for four heads what the others are for two, and its sums
+//      need a third of the registers.
+//  - The contraction's index may have any order that both operands share: thread t of a quad takes dims
+//    32 t .. + 31 of a K row (two 16-byte loads) and 16 consecutive dims of some positions of V.
+//  - A V row's scale may have any size beside its weight (the first token's V is small in many models, and its weight
+//    large), so the weights p_j vs_j have a running maximum of their own, of s_j + log2 vs_j, next to that of s_j, by
+//    which the weights' sum goes.
 constexpr int kQ8Tile = 128, kQ8Stages = 2;
 constexpr int kQ8Rows = 32;                 // positions of a warp
 constexpr int kQ8Slot = 2 * kQ8Rows * 128;  // K and V
 constexpr int kQ8Scales = 2 * kQ8Rows * 4;  // their scales
-constexpr int kQ8PerSm = 3;                 // CTAs
 static_assert(8 * kPdSumRow * 4 <= kQ8Slot, "a slot holds eight heads' sums");
 __host__ __device__ constexpr int pq8_smem(int batch) {
   return 1024 + 4 * kQ8Stages * (kQ8Slot + kQ8Scales) + (batch + 1) * 4;
@@ -136,15 +138,11 @@ __device__ __forceinline__ float log2_fast(float x) {
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint4 lds128(unsigned addr) {
-  uint4 r;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr));
-  return r;
-}
-__device__ __forceinline__ float lds32f(unsigned addr) {
-  float r;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(addr));
-  return r;
+// (not volatile: the loads and products of a unit may be interleaved as their latencies ask)
+__device__ __forceinline__ void q8_mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ unsigned transpose_b16(unsigned x) {  // an 8 x 8 matrix over the warp
   unsigned y;
@@ -152,9 +150,403 @@ __device__ __forceinline__ unsigned transpose_b16(unsigned x) {  // an 8 x 8 mat
   return y;
 }
 
+// What both kinds share of a unit: the visible positions of the warp's 32.
+struct Q8Seen {
+  bool inside;      // all of them
+  unsigned halves;  // bit i: rows 16 i .. + 15 are there
+  int p0;
+  Visible v;
+  __device__ __forceinline__ bool at(int i) const { return (halves >> (i >> 4) & 1u) && v.at(p0 + i); }
+};
+__device__ __forceinline__ uint4 q8_lds(const unsigned char* at) { return *reinterpret_cast<const uint4*>(at); }
+
+// Up to 2 * SETS heads. Set n has heads 2 n and 2 n + 1: columns 4 (h % 2) + part, part 3 the most significant byte. Thread
+// (g8, t4) has the scores of head 2 n + t4 / 2 at positions order(g8) + 8 j, j < 4 (as its neighbour t4 ^ 1 has), and
+// dims 16 g8 .. + 15 of two of the head's parts. Positions are taken in an order for which the rows that a quarter warp reads
+// from shared memory lie on distinct banks.
 template <int SETS>
-__global__ void __launch_bounds__(kPdThreads, SETS == 1 ? kQ8PerSm : 2) k_paged_decode_q8(const __grid_constant__ Q8Args qa,
-                                                                                       void* workspace) {
+struct Q8Whole {
+  static constexpr int kHeads = 2 * SETS, kCtas = SETS == 1 ? 3 : 2;  // CTAs per SM
+  static constexpr float kLag = 1.0f;     // log2 that a weights' maximum may fall behind
+  static constexpr float kShift = 29.0f;  // weights are kept times 2^29: with the lag at most 2^30, the largest off by 2^-30
+  static constexpr int kFlush = 2048;     // units after which the 32-bit sums are moved (each adds below 2^19)
+  unsigned q[SETS][4][2];
+  int acc[SETS][8][4];
+  float o[SETS][16], m[SETS], mo[SETS], l[SETS], factor[SETS];
+  int since;
+
+  static __device__ __forceinline__ int order(int c) { return 2 * (c & 3) + ((c ^ (c >> 2)) & 1); }
+  // A number of at most 2^30 in size as four signed bytes.
+  static __device__ __forceinline__ unsigned digits(int x) { return (unsigned)(x + 0x00808080) ^ 0x00808080u; }
+  // Four words as the columns of their bytes.
+  static __device__ __forceinline__ void turn(unsigned a, unsigned b, unsigned c, unsigned d, unsigned (&r)[4]) {
+    const unsigned ab0 = __byte_perm(a, b, 0x5140), ab1 = __byte_perm(a, b, 0x7362);
+    const unsigned cd0 = __byte_perm(c, d, 0x5140), cd1 = __byte_perm(c, d, 0x7362);
+    r[0] = __byte_perm(ab0, cd0, 0x5410);
+    r[1] = __byte_perm(ab0, cd0, 0x7632);
+    r[2] = __byte_perm(ab1, cd1, 0x5410);
+    r[3] = __byte_perm(ab1, cd1, 0x7632);
+  }
+  static __device__ __forceinline__ void mma(int (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
+                                             unsigned b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+
+  __device__ __forceinline__ void start(const PAttnArgs& a, const PdCursor& c, int G, int g8, int t4) {
+    since = 0;
+#pragma unroll
+    for (int n = 0; n < SETS; ++n) {
+      const int hs = c.sub * 8 + 2 * n + (g8 >> 2);
+      const bool live = hs < G;
+      const long long base = c.b * a.q_stride + ((long long)c.g * G + (live ? hs : 0)) * kHeadDim + 32 * t4;
+      float2 x[16];
+      unsigned top = 0;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) x[k] = load2(a.q, base + 2 * k, a.dtype);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        if (!live) x[k] = make_float2(0.f, 0.f);
+        top = max(top, max(__float_as_uint(x[k].x) & 0x7fffffffu, __float_as_uint(x[k].y) & 0x7fffffffu));
+      }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // by a power of two (in two steps from very small ones) to below 2^30
+      const int e = (int)(top >> 23), small = e < 60;
+      const float up0 = small ? 18446744073709551616.0f : 1.0f, down0 = small ? 5.421010862427522e-20f : 1.0f;
+      const int f = min(small ? e + 64 : e, 254);
+      const float up = __int_as_float((283 - f) << 23), down = __int_as_float((f - 29) << 23);
+      const unsigned sel = 0x0040u + 0x11u * (g8 & 3);  // byte g8 % 4 of two words
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        unsigned d[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float y = i & 1 ? x[2 * k + (i >> 1)].y : x[2 * k + (i >> 1)].x;
+          d[i] = digits(__float2int_rn(y * up0 * up));
+        }
+        q[n][k >> 1][k & 1] = __byte_perm(__byte_perm(d[0], d[1], sel), __byte_perm(d[2], d[3], sel), 0x5410);
+      }
+      // of the head whose scores this thread has; not finite: its scores are NaN
+      const float mine = e == 255 ? __int_as_float(0x7fffffff) : a.scale * kLog2e * down0 * down;
+      factor[n] = __shfl_sync(0xffffffffu, mine, 16 * (t4 >> 1));
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[n][j] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[n][j][0] = acc[n][j][1] = acc[n][j][2] = acc[n][j][3] = 0;
+      m[n] = mo[n] = -INFINITY;
+      l[n] = 0.0f;
+    }
+  }
+  // Moves the 32-bit sums to the f32 ones, times f.
+  __device__ __forceinline__ void flush(int n, float f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        o[n][2 * j + e] = (o[n][2 * j + e] + fmaf((float)acc[n][j][2 * e + 1], 256.0f, (float)acc[n][j][2 * e])) * f;
+        acc[n][j][2 * e] = acc[n][j][2 * e + 1] = 0;
+      }
+  }
+  __device__ __forceinline__ void unit(const unsigned char* kb, const unsigned char* vb, const float* ks, const float* vs,
+                                       const Q8Seen& seen, int g8, int t4) {
+    const int r0 = order(g8);
+    float p[SETS][4], u[SETS][4];  // of positions r0 + 8 j: scores, and with V's scale
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      int s[SETS][4];
+#pragma unroll
+      for (int n = 0; n < SETS; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0;
+      const unsigned char* row = kb + (16 * h + r0) * 128;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const unsigned char* at = row + (((2 * t4 + c) ^ r0) << 4);
+        const uint4 x = q8_lds(at), y = q8_lds(at + 1024);
+#pragma unroll
+        for (int n = 0; n < SETS; ++n) {
+          mma(s[n], x.x, y.x, x.y, y.y, q[n][2 * c][0], q[n][2 * c][1]);
+          mma(s[n], x.z, y.z, x.w, y.w, q[n][2 * c + 1][0], q[n][2 * c + 1][1]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int j = 2 * h + e;
+        const float sc = ks[r0 + 8 * j], lv = log2_fast(vs[r0 + 8 * j]);
+#pragma unroll
+        for (int n = 0; n < SETS; ++n) {  // two bytes of q here (below 2^30 together), two in the neighbour
+          const float x = (float)(s[n][2 * e] + 256 * s[n][2 * e + 1]) * (t4 & 1 ? 65536.0f : 1.0f);
+          p[n][j] = (x + __shfl_xor_sync(0xffffffffu, x, 1)) * (factor[n] * sc);
+          u[n][j] = p[n][j] + lv;
+        }
+      }
+    }
+    if (!seen.inside) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (!seen.at(r0 + 8 * j))
+#pragma unroll
+          for (int n = 0; n < SETS; ++n) p[n][j] = u[n][j] = -INFINITY;
+    }
+    const bool full = ++since == kFlush;
+    if (full) since = 0;
+    unsigned w[SETS][2];
+#pragma unroll
+    for (int n = 0; n < SETS; ++n) {
+      float mt = fmaxf(fmaxf(p[n][0], p[n][1]), fmaxf(p[n][2], p[n][3]));
+      float ut = fmaxf(fmaxf(u[n][0], u[n][1]), fmaxf(u[n][2], u[n][3]));
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) {
+        mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
+        ut = fmaxf(ut, __shfl_xor_sync(0xffffffffu, ut, x));
+      }
+      if (__any_sync(0xffffffffu, full || mt > m[n] + kPdLag || ut > mo[n] + kLag)) {  // some head's maximum moved
+        const float mn = mt > m[n] + kPdLag ? mt : m[n], un = ut > mo[n] + kLag ? ut : mo[n];
+        l[n] *= m[n] == -INFINITY ? 0.0f : exp2_fast(m[n] - mn);
+        flush(n, mo[n] == -INFINITY ? 0.0f : exp2_fast(mo[n] - un));
+        m[n] = mn;
+        mo[n] = un;
+      }
+      const float ref = m[n] == -INFINITY ? 0.0f : m[n], uref = mo[n] == -INFINITY ? 0.0f : mo[n] - kShift;
+      unsigned d[4], r[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = exp2_fast(u[n][j] - uref);
+        l[n] = fmaf(x, 0.0f, l[n]) + exp2_fast(p[n][j] - ref);  // (a NaN weight is no integer)
+        d[j] = digits(__float2int_rn(x));
+      }
+      // the parts of four positions each; thread (g8, t4) wants part g8 % 4 of head g8 / 4 of those that rows t4 and t4 + 4 have
+      turn(d[0], d[1], d[2], d[3], r);
+      const unsigned even = t4 & 1 ? r[2] : r[0], odd = t4 & 1 ? r[3] : r[1];
+      const int from = 4 * t4 + 2 * (g8 >> 2) + ((g8 >> 1) & 1);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const unsigned x = __shfl_sync(0xffffffffu, even, from + 16 * e), y = __shfl_sync(0xffffffffu, odd, from + 16 * e);
+        w[n][e] = g8 & 1 ? y : x;
+      }
+    }
+    // V: positions order(t4) + 8 j and order(t4 + 4) + 8 j, dims 16 g8 .. + 15
+    const int ra = order(t4), rb = order(t4 + 4);
+    const unsigned char *va = vb + ra * 128 + ((g8 ^ ra) << 4), *vc = vb + rb * 128 + ((g8 ^ rb) << 4);
+    uint4 x[4], y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[j] = q8_lds(va + 1024 * j);
+      y[j] = q8_lds(vc + 1024 * j);
+    }
+    auto dims = [&](int k, unsigned xa, unsigned xb, unsigned xc, unsigned xd, unsigned ya, unsigned yb, unsigned yc,
+                    unsigned yd) {  // 4 k .. + 3 of both
+      unsigned e[4], f[4];
+      turn(xa, xb, xc, xd, e);
+      turn(ya, yb, yc, yd, f);
+#pragma unroll
+      for (int n = 0; n < SETS; ++n) {
+        mma(acc[n][2 * k], e[0], e[1], f[0], f[1], w[n][0], w[n][1]);
+        mma(acc[n][2 * k + 1], e[2], e[3], f[2], f[3], w[n][0], w[n][1]);
+      }
+    };
+    dims(0, x[0].x, x[1].x, x[2].x, x[3].x, y[0].x, y[1].x, y[2].x, y[3].x);
+    dims(1, x[0].y, x[1].y, x[2].y, x[3].y, y[0].y, y[1].y, y[2].y, y[3].y);
+    dims(2, x[0].z, x[1].z, x[2].z, x[3].z, y[0].z, y[1].z, y[2].z, y[3].z);
+    dims(3, x[0].w, x[1].w, x[2].w, x[3].w, y[0].w, y[1].w, y[2].w, y[3].w);
+  }
+  __device__ __forceinline__ void give_up() {
+#pragma unroll
+    for (int n = 0; n < SETS; ++n) l[n] = __int_as_float(0x7fffffff);
+  }
+  // The warp's sums of head h to sums[h * kPdSumRow + dim], maximum and weights to ml[h], the maximum of the sums to mos[h].
+  __device__ __forceinline__ void finish(float* sums, float2* ml, float* mos, int g8, int t4) {
+#pragma unroll
+    for (int n = 0; n < SETS; ++n) {
+      flush(n, 1.0f);
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l[n] += __shfl_xor_sync(0xffffffffu, l[n], x);
+      float y[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float x = o[n][j] * (t4 & 1 ? 65536.0f : 1.0f);
+        y[j] = x + __shfl_xor_sync(0xffffffffu, x, 1);
+      }
+      const int h = 2 * n + (t4 >> 1);
+      float* mine = sums + h * kPdSumRow + 16 * g8 + 8 * (t4 & 1);
+#pragma unroll
+      for (int j = 0; j < 8; j += 4)
+        *reinterpret_cast<float4*>(mine + j) = t4 & 1 ? make_float4(y[8 + j], y[9 + j], y[10 + j], y[11 + j])
+                                                     : make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
+      if (g8 == 0 && !(t4 & 1)) {
+        ml[h] = make_float2(m[n], l[n]);
+        mos[h] = mo[n];
+      }
+    }
+  }
+};
+
+// Up to eight heads. Set n has heads 4 n .. + 3: columns 2 (h % 4) (the 16-bit part) and + 1 (the rest). Thread (g8, t4) has
+// the scores of head 4 n + t4 at positions g8 + 8 j, and its dims 16 g8 .. + 15.
+struct Q8Half {
+  static constexpr int kHeads = 8, kCtas = 2, SETS = 2;
+  static constexpr float kShift = kPdShift;
+  unsigned q[SETS][8][2];
+  float o[SETS][8][4], m[SETS], mo[SETS], l[SETS], factor[SETS];
+
+  __device__ __forceinline__ void start(const PAttnArgs& a, const PdCursor& c, int G, int g8, int t4) {
+#pragma unroll
+    for (int n = 0; n < SETS; ++n) {
+      const int hs = c.sub * 8 + 4 * n + (g8 >> 1);
+      const bool live = hs < G;
+      const long long base = c.b * a.q_stride + ((long long)c.g * G + (live ? hs : 0)) * kHeadDim + 32 * t4;
+      float2 x[16];
+      float top = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) x[k] = load2(a.q, base + 2 * k, a.dtype);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        if (!live) x[k] = make_float2(0.f, 0.f);
+        top = fmaxf(top, fmaxf(fabsf(x[k].x), fabsf(x[k].y)));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const float2 fit = f16_fit(__float_as_int(top) >> 23);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          unsigned hi, lo;
+          split2<__half>(x[2 * k + e].x * fit.x, x[2 * k + e].y * fit.x, hi, lo);
+          q[n][k][e] = g8 & 1 ? lo : hi;
+        }
+      factor[n] = a.scale * kLog2e * __shfl_sync(0xffffffffu, fit.y, 8 * t4);  // of head t4: columns 2 t4, 2 t4 + 1
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.0f;
+      m[n] = mo[n] = -INFINITY;
+      l[n] = 0.0f;
+    }
+  }
+  __device__ __forceinline__ void unit(const unsigned char* kb, const unsigned char* vb, const float* ks, const float* vs,
+                                       const Q8Seen& seen, int g8, int t4) {
+    float p[SETS][4], u[SETS][4];  // of positions 8 j + g8: scores, and with V's scale
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float s[SETS][2][4];
+#pragma unroll
+      for (int n = 0; n < SETS; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) s[n][e][0] = s[n][e][1] = s[n][e][2] = s[n][e][3] = 0.0f;
+      const unsigned char* row = kb + (16 * h + g8) * 128;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const unsigned char* at = row + (((2 * t4 + c) ^ g8) << 4);
+        const uint4 x = q8_lds(at), y = q8_lds(at + 1024);
+        const unsigned xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const unsigned v = xw[k] ^ 0x80808080u, w = yw[k] ^ 0x80808080u;
+          const unsigned f[4] = {q8_half2(v, kQ8Lo), q8_half2(w, kQ8Lo), q8_half2(v, kQ8Hi), q8_half2(w, kQ8Hi)};
+#pragma unroll
+          for (int n = 0; n < SETS; ++n) q8_mma(s[n][k & 1], f, q[n][4 * c + k][0], q[n][4 * c + k][1]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int j = 2 * h + e;
+        const float sc = ks[8 * j + g8], lv = log2_fast(vs[8 * j + g8]);
+#pragma unroll
+        for (int n = 0; n < SETS; ++n) {
+          p[n][j] = ((s[n][0][2 * e] + s[n][1][2 * e]) + (s[n][0][2 * e + 1] + s[n][1][2 * e + 1])) * (factor[n] * sc);
+          u[n][j] = p[n][j] + lv;
+        }
+      }
+    }
+    if (!seen.inside) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (!seen.at(8 * j + g8))
+#pragma unroll
+          for (int n = 0; n < SETS; ++n) p[n][j] = u[n][j] = -INFINITY;
+    }
+#pragma unroll
+    for (int n = 0; n < SETS; ++n) {
+      float mt = fmaxf(fmaxf(p[n][0], p[n][1]), fmaxf(p[n][2], p[n][3]));
+      float ut = fmaxf(fmaxf(u[n][0], u[n][1]), fmaxf(u[n][2], u[n][3]));
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) {
+        mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
+        ut = fmaxf(ut, __shfl_xor_sync(0xffffffffu, ut, x));
+      }
+      if (__any_sync(0xffffffffu, mt > m[n] + kPdLag || ut > mo[n] + kPdLag)) {  // some head's maximum moved: rescale
+        const float mn = mt > m[n] + kPdLag ? mt : m[n], un = ut > mo[n] + kPdLag ? ut : mo[n];
+        l[n] *= m[n] == -INFINITY ? 0.0f : exp2_fast(m[n] - mn);
+        const float f = mo[n] == -INFINITY ? 0.0f : exp2_fast(mo[n] - un);
+        m[n] = mn;
+        mo[n] = un;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][j][e] *= f;
+      }
+      const float ref = m[n] == -INFINITY ? 0.0f : m[n], uref = mo[n] == -INFINITY ? 0.0f : mo[n] - kPdShift;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        l[n] += exp2_fast(p[n][j] - ref);
+        u[n][j] = exp2_fast(u[n][j] - uref);
+      }
+    }
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      unsigned w[SETS][2];
+#pragma unroll
+      for (int n = 0; n < SETS; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {  // a weight as its 16-bit part and the rest, for the columns of its head
+          const float x = u[n][2 * st + e];
+          const float hi = __half2float(__float2half_rn(x));
+          w[n][e] = transpose_b16(pack2<__half>(hi, x - hi));
+        }
+      // rows 16 st + 2 t + {0, 1, 8, 9}, chunk g8
+      const unsigned char* row = vb + (16 * st + 2 * t4) * 128;
+      const unsigned c0 = (g8 ^ (2 * t4)) << 4, c1 = (g8 ^ (2 * t4 + 1)) << 4;
+      const uint4 x0 = q8_lds(row + c0), x1 = q8_lds(row + 128 + c1);
+      const uint4 x2 = q8_lds(row + 1024 + c0), x3 = q8_lds(row + 1152 + c1);
+      const unsigned va[4] = {x0.x, x0.y, x0.z, x0.w}, vc[4] = {x1.x, x1.y, x1.z, x1.w};
+      const unsigned vd[4] = {x2.x, x2.y, x2.z, x2.w}, ve[4] = {x3.x, x3.y, x3.z, x3.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const unsigned a0 = __byte_perm(va[k], vc[k], 0x5140) ^ 0x80808080u, a1 = __byte_perm(va[k], vc[k], 0x7362) ^ 0x80808080u;
+        const unsigned b0 = __byte_perm(vd[k], ve[k], 0x5140) ^ 0x80808080u, b1 = __byte_perm(vd[k], ve[k], 0x7362) ^ 0x80808080u;
+        const unsigned f[4] = {q8_half2(a0, kQ8Lo), q8_half2(a0, kQ8Hi), q8_half2(b0, kQ8Lo), q8_half2(b0, kQ8Hi)};
+        const unsigned f2[4] = {q8_half2(a1, kQ8Lo), q8_half2(a1, kQ8Hi), q8_half2(b1, kQ8Lo), q8_half2(b1, kQ8Hi)};
+#pragma unroll
+        for (int n = 0; n < SETS; ++n) {
+          q8_mma(o[n][2 * k], f, w[n][0], w[n][1]);
+          q8_mma(o[n][2 * k + 1], f2, w[n][0], w[n][1]);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void give_up() {
+#pragma unroll
+    for (int n = 0; n < SETS; ++n) l[n] = __int_as_float(0x7fffffff);
+  }
+  __device__ __forceinline__ void finish(float* sums, float2* ml, float* mos, int g8, int t4) {
+#pragma unroll
+    for (int n = 0; n < SETS; ++n) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l[n] += __shfl_xor_sync(0xffffffffu, l[n], x);
+      float* mine = sums + (4 * n + t4) * kPdSumRow + 16 * g8;
+#pragma unroll
+      for (int j = 0; j < 8; j += 2)
+        *reinterpret_cast<float4*>(mine + 2 * j) = make_float4(o[n][j][0] + o[n][j][1], o[n][j][2] + o[n][j][3],
+                                                               o[n][j + 1][0] + o[n][j + 1][1], o[n][j + 1][2] + o[n][j + 1][3]);
+      if (g8 == 0) {
+        ml[4 * n + t4] = make_float2(m[n], l[n]);
+        mos[4 * n + t4] = mo[n];
+      }
+    }
+  }
+};
+
+template <typename Heads>
+__global__ void __launch_bounds__(kPdThreads, Heads::kCtas) k_paged_decode_q8(const __grid_constant__ Q8Args qa, void* workspace) {
   const PAttnArgs& a = qa.a;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
@@ -178,18 +570,23 @@ __global__ void __launch_bounds__(kPdThreads, SETS == 1 ? kQ8PerSm : 2) k_paged_
   pdl_trigger();
   auto see = [&](int b) { return visible<kQ8Tile>(a.kv.seq_lens[b], paged_len(a.kv, b), a.window, a.sinks); };
   pd_units(B, first, see);  // (its barriers are the mbarriers' too)
-  if (blockIdx.x == 0) {
-    for (int b = tid; b <= B; b += kPdThreads) ws.first[b] = first[b];
-    for (int b = tid; b < B; b += kPdThreads)  // (paged_len cuts both)
-      if (a.kv.seq_lens[b] != paged_len(a.kv, b)) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
-  }
-  for (int b = blockIdx.x; b < B; b += gridDim.x)  // nothing visible: zeros
-    if (first[b + 1] == first[b])
-      for (int i = tid; i < a.q_heads * kHeadDim; i += kPdThreads) store1(a.y, b * a.y_stride + i, a.dtype, 0.0f);
   const long long U = (long long)first[B] * nh;
   const int ctas = (int)min((long long)gridDim.x, U);  // none of them empty
-  if ((int)blockIdx.x >= ctas) return;
-  const int u0 = (int)(U * blockIdx.x / ctas), u1 = (int)(U * (blockIdx.x + 1) / ctas);
+  auto aside = [&] {  // what is not on the way to the first copies
+    if (blockIdx.x == 0) {
+      for (int b = tid; b <= B; b += kPdThreads) ws.first[b] = first[b];
+      for (int b = tid; b < B; b += kPdThreads)  // (paged_len cuts both)
+        if (a.kv.seq_lens[b] != paged_len(a.kv, b)) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
+    }
+    for (int b = blockIdx.x; b < B; b += gridDim.x)  // nothing visible: zeros
+      if (first[b + 1] == first[b])
+        for (int i = tid; i < a.q_heads * kHeadDim; i += kPdThreads) store1(a.y, b * a.y_stride + i, a.dtype, 0.0f);
+  };
+  if ((int)blockIdx.x >= ctas) {
+    aside();
+    return;
+  }
+  const int u0 = pd_div(U * blockIdx.x, ctas), u1 = pd_div(U * (blockIdx.x + 1), ctas);
   auto step = [&](PdCursor& c) { pd_step(c, first, a.kv.kv_heads, subs, see); };
   PdCursor cur = pd_place(B, first, nh, subs, u0, see);
   PdCursor pre = cur;  // the copies run ahead of the sums
@@ -203,7 +600,14 @@ __global__ void __launch_bounds__(kPdThreads, SETS == 1 ? kQ8PerSm : 2) k_paged_
     const int page = paged_page(a.kv, c.b, p0);
     return page < 0 ? -2 : page;
   };
+  // the queries of a (sequence, head) brought near before they are needed
+  const int q_bytes = a.dtype == QD_KV_F32 ? 4 : 2;
+  auto near_q = [&](const PdCursor& c) {
+    const char* at = static_cast<const char*>(a.q) + (c.b * a.q_stride + ((long long)c.g * G + c.sub * 8) * kHeadDim) * q_bytes;
+    if (lane * 128 < min(8, G - c.sub * 8) * kHeadDim * q_bytes) asm volatile("prefetch.global.L1 [%0];" ::"l"(at + lane * 128));
+  };
   int next_page = page_of(pre);
+  near_q(pre);
   unsigned live_ring = 0;  // bits 2 i, 2 i + 1: the halves of slot i hold rows
   unsigned phases = 0;     // bit i: parity of slot i's barrier
   int issued = 0, in_slot = 0;
@@ -236,57 +640,23 @@ __global__ void __launch_bounds__(kPdThreads, SETS == 1 ? kQ8PerSm : 2) k_paged_
     if (issued < n_units) {
       step(pre);
       next_page = page_of(pre);
+      if (pre.t == 0) near_q(pre);
     }
   };
 #pragma unroll
   for (int i = 0; i < kQ8Stages - 1; ++i) issue();
+  aside();
 
-  // The queries of a (sequence, head): lane l has column l / 4 of the products (of set s head 4 s + l / 8, its 16-bit part
-  // or the rest), dims 32 (l % 4) .. + 31; the scores and sums of head 4 s + l % 4.
-  const float qs = a.scale * kLog2e;
   const int t4 = lane & 3, g8 = lane >> 2;
-  unsigned q[SETS][8][2];
-  float o[SETS][8][4], m[SETS], mo[SETS], l[SETS], factor[SETS];
+  Heads heads;
   bool fresh = true;  // a new (sequence, head): take its q, clear the sums
   int seg = 0;        // segments finished by this CTA
   bool from_start = cur.t == 0;
   int slot = 0;
   for (int i = 0; i < n_units; ++i) {
     issue();
-    if (fresh) {
-      fresh = false;
-#pragma unroll
-      for (int n = 0; n < SETS; ++n) {
-        const int hs = cur.sub * 8 + 4 * n + (g8 >> 1);
-        const bool live = hs < G;
-        const long long base = cur.b * a.q_stride + ((long long)cur.g * G + (live ? hs : 0)) * kHeadDim + 32 * t4;
-        float2 x[16];
-        float top = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) x[k] = load2(a.q, base + 2 * k, a.dtype);
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          if (!live) x[k] = make_float2(0.f, 0.f);
-          top = fmaxf(top, fmaxf(fabsf(x[k].x), fabsf(x[k].y)));
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float2 fit = f16_fit(__float_as_int(top) >> 23);
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            unsigned hi, lo;
-            split2<__half>(x[2 * k + e].x * fit.x, x[2 * k + e].y * fit.x, hi, lo);
-            q[n][k][e] = g8 & 1 ? lo : hi;
-          }
-        factor[n] = qs * __shfl_sync(0xffffffffu, fit.y, 8 * t4);  // of head t4: columns 2 t4, 2 t4 + 1
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.0f;
-        m[n] = mo[n] = -INFINITY;
-        l[n] = 0.0f;
-      }
-    }
+    if (fresh) heads.start(a, cur, G, g8, t4);
+    fresh = false;
     const bool last_t = cur.t + 1 == cur.v.tiles, more = i + 1 < n_units;
     unsigned halves = live_ring >> (2 * slot) & 3u;
     if (halves && !gone) {
@@ -300,130 +670,20 @@ __global__ void __launch_bounds__(kPdThreads, SETS == 1 ? kQ8PerSm : 2) k_paged_
     }
     if (gone) {  // what this warp held becomes NaN
       halves = 0;
-#pragma unroll
-      for (int n = 0; n < SETS; ++n) l[n] = __int_as_float(0x7fffffff);
+      heads.give_up();
     }
     if (halves) {
-      const unsigned kb = tc_smem(ring) + slot * kQ8Slot, vb = kb + kQ8Rows * 128;
-      const unsigned sb = tc_smem(scales) + slot * kQ8Scales + g8 * 4;
-      const int p0 = cur.v.tile(cur.t) * kQ8Tile + kQ8Rows * warp;
-      const bool inside = halves == 3u && p0 + 32 <= cur.v.end && (p0 >= cur.v.lo || p0 + 32 <= cur.v.ns);
-      float p[SETS][4], u[SETS][4];  // of positions 8 j + g8: scores, and with V's scale
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float s[SETS][2][4];
-#pragma unroll
-        for (int n = 0; n < SETS; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) s[n][e][0] = s[n][e][1] = s[n][e][2] = s[n][e][3] = 0.0f;
-        const unsigned row = kb + (16 * h + g8) * 128;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const unsigned at = row + (((2 * t4 + c) ^ g8) << 4);
-          const uint4 x = lds128(at), y = lds128(at + 1024);
-          const unsigned xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const unsigned v = xw[k] ^ 0x80808080u, w = yw[k] ^ 0x80808080u;
-            const unsigned f[4] = {q8_half2(v, kQ8Lo), q8_half2(w, kQ8Lo), q8_half2(v, kQ8Hi), q8_half2(w, kQ8Hi)};
-#pragma unroll
-            for (int n = 0; n < SETS; ++n) mma_16816<__half>(s[n][k & 1], f, q[n][4 * c + k][0], q[n][4 * c + k][1]);
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int j = 2 * h + e;
-          const float ks = lds32f(sb + 32 * j), lv = log2_fast(lds32f(sb + 32 * j + kQ8Rows * 4));
-#pragma unroll
-          for (int n = 0; n < SETS; ++n) {
-            p[n][j] = ((s[n][0][2 * e] + s[n][1][2 * e]) + (s[n][0][2 * e + 1] + s[n][1][2 * e + 1])) * (factor[n] * ks);
-            u[n][j] = p[n][j] + lv;
-          }
-        }
-      }
-      if (!inside) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (!(halves >> (j >> 1) & 1u) || !cur.v.at(p0 + 8 * j + g8))
-#pragma unroll
-            for (int n = 0; n < SETS; ++n) p[n][j] = u[n][j] = -INFINITY;
-      }
-#pragma unroll
-      for (int n = 0; n < SETS; ++n) {
-        float mt = fmaxf(fmaxf(p[n][0], p[n][1]), fmaxf(p[n][2], p[n][3]));
-        float ut = fmaxf(fmaxf(u[n][0], u[n][1]), fmaxf(u[n][2], u[n][3]));
-#pragma unroll
-        for (int x = 4; x < 32; x <<= 1) {
-          mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
-          ut = fmaxf(ut, __shfl_xor_sync(0xffffffffu, ut, x));
-        }
-        if (__any_sync(0xffffffffu, mt > m[n] + kPdLag || ut > mo[n] + kPdLag)) {  // some head's maximum moved: rescale
-          const float mn = mt > m[n] + kPdLag ? mt : m[n], un = ut > mo[n] + kPdLag ? ut : mo[n];
-          l[n] *= m[n] == -INFINITY ? 0.0f : exp2_fast(m[n] - mn);
-          const float f = mo[n] == -INFINITY ? 0.0f : exp2_fast(mo[n] - un);
-          m[n] = mn;
-          mo[n] = un;
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][j][e] *= f;
-        }
-        const float ref = m[n] == -INFINITY ? 0.0f : m[n], uref = mo[n] == -INFINITY ? 0.0f : mo[n] - kPdShift;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          l[n] += exp2_fast(p[n][j] - ref);
-          u[n][j] = exp2_fast(u[n][j] - uref);
-        }
-      }
-#pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        unsigned w[SETS][2];
-#pragma unroll
-        for (int n = 0; n < SETS; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {  // a weight as its 16-bit part and the rest, for the columns of its head
-            const float x = u[n][2 * st + e];
-            const float hi = __half2float(__float2half_rn(x));
-            w[n][e] = transpose_b16(pack2<__half>(hi, x - hi));
-          }
-        // rows 16 st + 2 t + {0, 1, 8, 9}, chunk g8
-        const unsigned row = vb + (16 * st + 2 * t4) * 128, c0 = (g8 ^ (2 * t4)) << 4, c1 = (g8 ^ (2 * t4 + 1)) << 4;
-        const uint4 x0 = lds128(row + c0), x1 = lds128(row + 128 + c1);
-        const uint4 x2 = lds128(row + 1024 + c0), x3 = lds128(row + 1152 + c1);
-        const unsigned va[4] = {x0.x, x0.y, x0.z, x0.w}, vc[4] = {x1.x, x1.y, x1.z, x1.w};
-        const unsigned vd[4] = {x2.x, x2.y, x2.z, x2.w}, ve[4] = {x3.x, x3.y, x3.z, x3.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const unsigned a0 = __byte_perm(va[k], vc[k], 0x5140) ^ 0x80808080u, a1 = __byte_perm(va[k], vc[k], 0x7362) ^ 0x80808080u;
-          const unsigned b0 = __byte_perm(vd[k], ve[k], 0x5140) ^ 0x80808080u, b1 = __byte_perm(vd[k], ve[k], 0x7362) ^ 0x80808080u;
-          const unsigned f[4] = {q8_half2(a0, kQ8Lo), q8_half2(a0, kQ8Hi), q8_half2(b0, kQ8Lo), q8_half2(b0, kQ8Hi)};
-          const unsigned f2[4] = {q8_half2(a1, kQ8Lo), q8_half2(a1, kQ8Hi), q8_half2(b1, kQ8Lo), q8_half2(b1, kQ8Hi)};
-#pragma unroll
-          for (int n = 0; n < SETS; ++n) {
-            mma_16816<__half>(o[n][2 * k], f, w[n][0], w[n][1]);
-            mma_16816<__half>(o[n][2 * k + 1], f2, w[n][0], w[n][1]);
-          }
-        }
-      }
+      const unsigned char* kb = ring + slot * kQ8Slot;
+      const float* ks = reinterpret_cast<const float*>(scales + slot * kQ8Scales);
+      Q8Seen seen{false, halves, cur.v.tile(cur.t) * kQ8Tile + kQ8Rows * warp, cur.v};
+      seen.inside = halves == 3u && seen.p0 + 32 <= cur.v.end && (seen.p0 >= cur.v.lo || seen.p0 + 32 <= cur.v.ns);
+      heads.unit(kb, kb + kQ8Rows * 128, ks, ks + kQ8Rows, seen, g8, t4);
     }
     __syncwarp();  // the slot may be refilled
     if (last_t || !more) {
       // The (sequence, head), or this CTA's part of it, ends: join the four warps. The sums go to the slot that has
-      // just been read: dims 16 g8 .. + 15 of head t4 of each set.
-#pragma unroll
-      for (int n = 0; n < SETS; ++n) {
-#pragma unroll
-        for (int x = 4; x < 32; x <<= 1) l[n] += __shfl_xor_sync(0xffffffffu, l[n], x);
-        float* mine = reinterpret_cast<float*>(ring + slot * kQ8Slot) + (4 * n + t4) * kPdSumRow + 16 * g8;
-#pragma unroll
-        for (int j = 0; j < 8; j += 2)
-          *reinterpret_cast<float4*>(mine + 2 * j) = make_float4(o[n][j][0] + o[n][j][1], o[n][j][2] + o[n][j][3],
-                                                                 o[n][j + 1][0] + o[n][j + 1][1], o[n][j + 1][2] + o[n][j + 1][3]);
-        if (g8 == 0) {
-          sml[warp][4 * n + t4] = make_float2(m[n], l[n]);
-          smo[warp][4 * n + t4] = mo[n];
-        }
-      }
+      // just been read.
+      heads.finish(reinterpret_cast<float*>(ring + slot * kQ8Slot), sml[warp], smo[warp], g8, t4);
       __syncthreads();
       const int live = min(8, G - cur.sub * 8);
       const bool whole = from_start && last_t;
@@ -435,7 +695,7 @@ __global__ void __launch_bounds__(kPdThreads, SETS == 1 ? kQ8PerSm : 2) k_paged_
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           L += sml[w][h].y * (sml[w][h].x == -INFINITY ? 0.0f : exp2_fast(sml[w][h].x - M));  // (NaN stays)
-          const float f = smo[w][h] == -INFINITY ? 0.0f : exp2_fast(smo[w][h] - kPdShift - M);
+          const float f = smo[w][h] == -INFINITY ? 0.0f : exp2_fast(smo[w][h] - Heads::kShift - M);
           x += reinterpret_cast<const float*>(smem + (w * kQ8Stages + slot) * kQ8Slot)[h * kPdSumRow + tid] * f;
         }
         if (whole) {

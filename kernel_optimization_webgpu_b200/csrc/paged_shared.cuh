@@ -63,13 +63,13 @@ __global__ void __launch_bounds__(256) k_paged_shared_join(const __grid_constant
     const long long U = (long long)ws.first[a.kv.batch] * nh;
     const int ctas = (int)min((long long)pa.ctas, U);
     const long long v0 = (long long)f0 * nh + (long long)(g * subs + (hs >> 3)) * tiles, v1 = v0 + tiles;
-    const int c0 = (int)(((v0 + 1) * ctas - 1) / U), c1 = (int)((v1 * ctas - 1) / U);
+    const int c0 = pd_div((v0 + 1) * ctas - 1, U), c1 = pd_div(v1 * ctas - 1, U);
     if (c0 == c1) {
       const long long i = (long long)b * a.q_heads + g * G + hs;
       ps_add(s, a.tail_ml[i], *reinterpret_cast<const float4*>(a.tail_o + i * kHeadDim + 4 * d4));
     } else {
       for (int c = c0; c <= c1; ++c) {
-        const long long i = (2ll * c + (U * c / ctas >= v0 ? 0 : 1)) * 8 + (hs & 7);
+        const long long i = (2ll * c + (pd_div(U * c, ctas) >= v0 ? 0 : 1)) * 8 + (hs & 7);
         ps_add(s, ws.ml[i], *reinterpret_cast<const float4*>(ws.o + i * kHeadDim + 4 * d4));
       }
     }
