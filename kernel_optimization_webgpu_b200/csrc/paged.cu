@@ -345,7 +345,7 @@ static void launch_shared(const PAttnArgs& a, void* workspace, cudaStream_t s) {
   allow_smem(k_paged_decode<T, PARTS == 3, true>, pd_smem(4096), smem_set);
   launch_ex(k_paged_decode<T, PARTS == 3, true>, dim3(j.ctas), dim3(kPdThreads), (size_t)pd_smem(B), s, j.a,
             (void*)j.decode_ws);
-  launch_ex(k_paged_shared_join, dim3((B * G + 7) / 8, kvh), dim3(256), 0, s, j);
+  launch_ex(k_paged_shared_join, dim3((B * G + 7) / 8, kvh), dim3(kPsThreads), 0, s, j);
 }
 
 }  // namespace qd

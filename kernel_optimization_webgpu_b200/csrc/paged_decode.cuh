@@ -80,14 +80,16 @@ __device__ __forceinline__ Visible visible(int asked, int len, int window, int s
   return v;
 }
 
-// The positions of sequence b from its shared_lens[b]-th on.
+// The positions of sequence b from its shared_lens[b]-th on, and kPdEnds tiles without any: what a (sequence,
+// head)'s end costs a CTA beside its tiles, so that a run of many short ones is shared out over more CTAs.
+constexpr int kPdEnds = 2;
 template <int TILE>
 __device__ __forceinline__ Visible tail(const PAttnArgs& a, int b) {
   Visible v{};
   v.end = paged_len(a.kv, b);
   v.lo = min(max(a.shared_lens[b], 0), v.end);
   v.w0 = v.lo / TILE;
-  v.tiles = v.lo < v.end ? (v.end + TILE - 1) / TILE - v.w0 : 0;
+  v.tiles = v.lo < v.end ? (v.end + TILE - 1) / TILE - v.w0 + kPdEnds : 0;
   return v;
 }
 
