@@ -283,9 +283,14 @@ static void launch_prompt(const PAttnArgs& a, const void* q_any, void* workspace
 struct SharedWs {
   size_t po, pml, rows, tail_o, tail_ml, decode, bytes;
 };
-static SharedWs shared_ws(int batch, int groups, int q_heads, int kv_heads, int cta_rows) {
-  const int G = q_heads / kv_heads, items = prompt_items(groups, batch, G, cta_rows);
-  const size_t rows = (size_t)items * kv_heads * prompt_splits(items, kv_heads) * cta_rows;
+constexpr int kSharedRows = 128;  // rows of a CTA (sequences times query heads of a KV head)
+// Row tiles of the groups, at most.
+static int shared_items(int batch, int groups, int group) {
+  return (int)(((long long)batch * group + (long long)groups * (kSharedRows - 1)) / kSharedRows);
+}
+static SharedWs shared_ws(int batch, int groups, int q_heads, int kv_heads) {
+  const int G = q_heads / kv_heads, items = shared_items(batch, groups, G);
+  const size_t rows = (size_t)items * kv_heads * prompt_splits(items, kv_heads) * 2 * kSharedRows;  // (two sets)
   SharedWs w{};
   const auto take = [&](size_t n) {
     const size_t at = w.bytes;
@@ -303,18 +308,18 @@ static SharedWs shared_ws(int batch, int groups, int q_heads, int kv_heads, int 
 
 template <typename T, int PARTS>
 static void launch_shared(const PAttnArgs& a, void* workspace, cudaStream_t s) {
-  constexpr int kRows = 128 * pp_tiles<PARTS>();
+  constexpr int kSets = pp_tiles<PARTS>();
   const int B = a.kv.batch, kvh = a.kv.kv_heads, G = a.q_heads / kvh, subs = (G + 7) / 8;
   const long long most = (long long)B * kvh * subs * (((long long)a.kv.table_width << a.kv.page_shift) / kPdTile + 1);
   if (most > 0x7fffffffLL)
     throw QdError{QD_E_RANGE, "qd_paged_attn_decode_shared: batch * heads * table beyond 2^31 units"};
-  const SharedWs w = shared_ws(B, a.groups, a.q_heads, kvh, kRows);
+  const SharedWs w = shared_ws(B, a.groups, a.q_heads, kvh);
   char* base = static_cast<char*>(workspace);
   PPromptArgs p{};
   p.a = a;
   p.a.kv.batch = a.groups;
-  p.cta_rows = kRows;
-  const int items = prompt_items(a.groups, B, G, kRows);
+  p.cta_rows = kSharedRows;
+  const int items = shared_items(B, a.groups, G);
   p.splits = prompt_splits(items, kvh);
   p.po = reinterpret_cast<float4*>(base + w.po);
   p.pml = reinterpret_cast<float2*>(base + w.pml);
@@ -336,9 +341,9 @@ static void launch_shared(const PAttnArgs& a, void* workspace, cudaStream_t s) {
   j.po = p.po;
   j.pml = p.pml;
   j.rows = p.rows;
-  j.splits = p.splits;
-  j.cta_rows = kRows;
-  j.all_rows = items * kRows;
+  j.splits = p.splits * kSets;
+  j.cta_rows = kSharedRows;
+  j.all_rows = items * kSharedRows;
   j.decode_ws = base + w.decode;
   j.ctas = (int)std::max(1LL, std::min<long long>(most, std::min(2 * current_sms(), kPdMaxCtas)));
   static unsigned long long smem_set = 0;
@@ -463,8 +468,7 @@ int qd_paged_attn_decode_q8(const qd_paged_q8* kv, const void* q, int dtype, int
 
 size_t qd_paged_attn_decode_shared_workspace_bytes(int batch, int groups, int q_heads, int kv_heads) {
   if (batch < 0 || groups < 0 || groups > batch || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads) return 0;
-  return std::max(shared_ws(batch, groups, q_heads, kv_heads, 128).bytes,
-                  shared_ws(batch, groups, q_heads, kv_heads, 256).bytes);  // (a CTA's rows depend on the types)
+  return shared_ws(batch, groups, q_heads, kv_heads).bytes;
 }
 
 int qd_paged_attn_decode_shared(const qd_paged_kv* kv, const void* q, int dtype, int64_t q_stride, int q_heads,

@@ -84,6 +84,9 @@ template <int PARTS>
 __host__ __device__ constexpr int pp_smem() {
   return (pp_tiles<PARTS>() * PARTS + pp_slots<PARTS>()) * kPpTileBytes + 1024;
 }
+// With SHARED: one tile of queries, the rest of that memory goes to the ring.
+template <int PARTS>
+__host__ __device__ constexpr int pp_shared_slots() { return pp_slots<PARTS>() + (pp_tiles<PARTS>() - 1) * PARTS; }
 
 // The item-th tile of rows, counted from the last (the latest rows of a prompt see the most keys
 // and start first): its sequence, tile, first row, new tokens and length, or false. Called by
@@ -346,18 +349,23 @@ __device__ __forceinline__ void split_parts(float x, float y, unsigned (&u)[PART
 
 // CLAIM: blocks take the work of others that have not started (a grid that does not fit the GPU at once).
 // SHARED: the rows of a "sequence" are the queries of a group, all of which see the positions that the group shares
-// (a.q_starts: the groups' first sequences, a.kv.batch of them); every row's sums go to the workspace.
+// (a.q_starts: the groups' first sequences, a.kv.batch of them); every row's sums go to the workspace. A CTA has one
+// tile of 128 rows, as few queries share a prefix, and its two sets of softmax threads take every other key
+// tile of it: S_t = Q K_j^T for t = j % 2, with a maximum, sums and an O of their own, joined like the parts of
+// several CTAs (64 queries of 2 heads behind 16384 keys: 7 key tiles a CTA in X us, Y with one set).
 template <typename T, int PARTS, bool CLAIM, bool SHARED = false>
 __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_constant__ PPromptArgs pa) {
   const PAttnArgs& a = pa.a;
-  constexpr int S = pp_slots<PARTS>(), kTiles = pp_tiles<PARTS>(), kRows = 128 * kTiles;
+  constexpr int kTiles = pp_tiles<PARTS>(), kQTiles = SHARED ? 1 : kTiles, kRows = 128 * kQTiles;
+  constexpr int S = SHARED ? pp_shared_slots<PARTS>() : pp_slots<PARTS>();
+  constexpr int kAlt = SHARED ? kTiles : 1;  // sets that share the key tiles of a row
   constexpr int kQTile = PARTS * kPpTileBytes;  // the parts of 128 rows
   // TMEM columns: S_t | O_t with P over S, or S | P (three parts) | O
   constexpr unsigned kColP = kTiles == 2 ? 0 : 128, kColO = kTiles == 2 ? 256 : 384;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* qs =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  unsigned char* ring = qs + kTiles * kQTile;
+  unsigned char* ring = qs + kQTiles * kQTile;
   __shared__ unsigned long long full[S], empty[S], s_full[2], p_half[2], p_full[2], o_done[2], q_full[2], drain;
   __shared__ unsigned long long work_full[2], work_empty[2], ask, answered;
   __shared__ __align__(16) uint4 answer;
@@ -365,6 +373,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
   __shared__ unsigned bad_rows[8];  // of key tile j: bit i set where 16-key chunk i has no usable page
   __shared__ unsigned tmem_base;
   __shared__ float shared_row[256];  // between a row's two threads: a maximum (NaN: given up), then a sum
+  __shared__ unsigned char q_exp[2][SHARED ? 128 : 1];  // largest exponents of the queries, for the other set
   __shared__ int failed;
   // (values read back from lane 0 are warp-uniform to the compiler: the MMA warp's operands then live
   // in uniform registers)
@@ -399,7 +408,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
     w.t0 = w.it.v.tiles * w.z / w.parts;  // (at most 2^23 tiles, 32 parts)
     w.nk = w.it.v.tiles * (w.z + 1) / w.parts - w.t0;
     w.row0 = tile * kRows;
-    w.halves = kTiles == 2 && w.it.n_rows - w.row0 > 128 ? 2 : 1;
+    w.halves = kTiles == 2 && (SHARED ? w.nk > 1 : w.it.n_rows - w.row0 > 128) ? 2 : 1;
     return true;
   };
   PpWork first;
@@ -607,7 +616,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       // and that costs the less the smaller the sum still is (f32 results at 64 + 3500 keys: 2.0e-6 off
       // with the largest part first, 0.9e-6 so).
       auto scores = [&](int t, int slot) {
-        const unsigned long long q0 = dq + (unsigned)(t * (kQTile >> 4));
+        const unsigned long long q0 = dq + (SHARED ? 0u : (unsigned)(t * (kQTile >> 4)));
         const unsigned long long k0 = dk + (unsigned)(slot * (kPpTileBytes >> 4));
 #pragma unroll
         for (int part = 0; part < PARTS; ++part)
@@ -633,6 +642,55 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         if (nk == 0) continue;
         auto ring_slot = [&](int i) { return (done + i) % S; };
         auto ring_phase = [&](int i) { return (unsigned)((done + i) / S) & 1u; };
+        // O_t += P_t V for the n-th tile of row tile t
+        auto product = [&](int t, int n, int slot) {
+          const unsigned long long v0 = dv + (unsigned)(slot * (kPpTileBytes >> 4));
+          const unsigned od = tmem + kColO + t * 128, pd = tmem + kColP + t * 128;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            ok = __all_sync(0xffffffffu,
+                            pp_wait(half ? &p_full[t] : &p_half[t], (unsigned)(n ^ (turn >> t)) & 1u, &failed));
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int ks = 2 * half + (i & 1) + 4 * (i >> 1);  // keys 0-31 and 64-95, then the others
+                const unsigned po = (PARTS - 1 - part) * 64 + ks * 8;
+                if (half == 0 && part == 0 && i == 0)
+                  pp_mma_ts(od, pd + po, v0, id_o, PARTS > 1 ? n % kPpFlush != 0 : n > 0, leader);
+                else
+                  pp_mma_ts(od, pd + po, v0 + ks * (2048 >> 4), id_o, true, leader);
+              }
+          }
+        };
+        if constexpr (SHARED) {
+          auto landed = [&](int i) { return __all_sync(0xffffffffu, pp_wait(&full[ring_slot(i)], ring_phase(i), &failed)); };
+          auto scores_of = [&](int j) {
+            ok = ok && landed(2 * j);
+            tc_fence_after();
+            if (!ok) return;
+            scores(j % kAlt, ring_slot(2 * j));
+            pp_commit(&empty[ring_slot(2 * j)], leader);
+          };
+          ok = __all_sync(0xffffffffu, pp_wait(&q_full[0], q_turn & 1u, &failed));
+          q_turn ^= 1u;
+          for (int j = 0; j < halves; ++j) scores_of(j);
+          for (int j = 0; j < nk && ok; ++j) {
+            const int t = j % kAlt;
+            ok = landed(2 * j + 1);
+            if (ok) product(t, j / kAlt, ring_slot(2 * j + 1));
+            if (!ok) break;
+            pp_commit(&o_done[t], leader);
+            pp_commit(&empty[ring_slot(2 * j + 1)], leader);
+            if (j + kAlt < nk) scores_of(j + kAlt);
+          }
+          done += 2 * nk;
+          for (int t = 0; t < kAlt; ++t)
+            if ((nk + kAlt - 1 - t) / kAlt & 1) turn ^= 1u << t;
+          continue;
+        }
         ok = __all_sync(0xffffffffu, pp_wait(&full[ring_slot(0)], ring_phase(0), &failed));
         for (int t = 0; t < halves && ok; ++t) {
           ok = __all_sync(0xffffffffu, pp_wait(&q_full[t], (q_turn >> t) & 1u, &failed));
@@ -648,26 +706,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
           if (j + 1 < nk) ok = pp_wait(&full[ks_slot], kph, &failed) && ok;
           ok = __all_sync(0xffffffffu, ok);
           for (int t = 0; t < halves && ok; ++t) {
-            const unsigned long long v0 = dv + (unsigned)(vs * (kPpTileBytes >> 4));
-            const unsigned od = tmem + kColO + t * 128, pd = tmem + kColP + t * 128;
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              ok = __all_sync(0xffffffffu, pp_wait(half ? &p_full[t] : &p_half[t], (unsigned)(j ^ (turn >> t)) & 1u,
-                                                   &failed));
-              if (!ok) break;
-              tc_fence_after();
-#pragma unroll
-              for (int part = 0; part < PARTS; ++part)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const int ks = 2 * half + (i & 1) + 4 * (i >> 1);  // keys 0-31 and 64-95, then the others
-                  const unsigned po = (PARTS - 1 - part) * 64 + ks * 8;
-                  if (half == 0 && part == 0 && i == 0)
-                    pp_mma_ts(od, pd + po, v0, id_o, PARTS > 1 ? j % kPpFlush != 0 : j > 0, leader);
-                  else
-                    pp_mma_ts(od, pd + po, v0 + ks * (2048 >> 4), id_o, true, leader);
-                }
-            }
+            product(t, j, vs);
             if (!ok) break;
             pp_commit(&o_done[t], leader);
             if (t == halves - 1) pp_commit(&empty[vs], leader);
@@ -694,9 +733,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPpRegsMany));
     // ---- softmax: half a row per thread ----
-    const int t = (tid >> 8) & 1, hf = (tid >> 7) & 1, lr = t * 128 + (tid & 127);
+    const int t = (tid >> 8) & 1, hf = (tid >> 7) & 1, own = t * 128 + (tid & 127), lr = SHARED ? tid & 127 : own;
     const int pair = 1 + t * 4 + (warp & 3);  // named barrier of the two warps that share 32 rows
     int done = 0;       // key tiles of the works before
+    int works = 0;      // those with any
     unsigned turn = 0;  // parity of this row tile's among them
     bool ok = true;  // (a warp that has given up still meets its partner at their barriers, where both end)
     for (int n = 0, nk = 0; CLAIM || n == 0; ++n) {
@@ -711,15 +751,21 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       if (halves == 0) break;
       const int row = work_of(n).row0 + lr, tok = row / G, hs = row - tok * G;
       const bool live = lr < kRows && row < it.n_rows && (unsigned)(it.tok0 + tok) < (unsigned)a.rows;
+      // key tiles of this set: all, or every other one
+      const int mine_nk = kAlt == 2 ? (nk + 1 - t) >> 1 : nk;
       if (t < halves && nk > 0) {
         // Q: K-major with the 128-byte swizzle; dead rows are zero. A warp copies its 32 rows' 64 dims row by
         // row, neighbouring lanes on neighbouring chunks (a row per lane took 4.5 us of a busy GPU's
         // time). A negative scale changes the sign of q, so that the softmax always has a positive one.
         const int wr = (warp & 3) * 32;  // first of the warp's rows in its tile
-        unsigned char* wq = qs + t * kQTile + hf * (kPpTileBytes / 2);
+        unsigned char* wq = qs + (SHARED ? 0 : t * kQTile) + hf * (kPpTileBytes / 2);
         const long long q_at =
             live ? (long long)(it.tok0 + tok) * a.q_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf : -1;
         float c = fabsf(a.scale) * kLog2e;  // of the row's scores
+        if (SHARED && t == 1) {  // the other set brings the queries
+          ok = ok && __all_sync(0xffffffffu, pp_wait(&q_full[0], (unsigned)works & 1u, &failed));
+          if constexpr (PARTS == 2) c = fmaxf(c * f16_fit(q_exp[works & 1][wr + lane]).y, 1.0e-37f);
+        } else {
         if constexpr (PARTS > 1) {
           const int c4 = lane & 15;
           constexpr int N = PARTS == 2 ? 16 : 8;
@@ -758,6 +804,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                 x[i] = make_float4(x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up);
               }
               c = fmaxf(c * fit(wr + lane).y, 1.0e-37f);  // (never 0: a hidden key's score is -inf)
+              if (SHARED && hf == 0) {
+                const unsigned both = tops[wr + lane];
+                q_exp[works & 1][wr + lane] = (unsigned char)max(both & 0xffffu, both >> 16);
+              }
             }
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -789,6 +839,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         pp_arrive(&q_full[t]);
+        }
         float m = -INFINITY, l = 0.0f;
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
         const unsigned ts = tmem + t * 128 + lanes, tp = tmem + kColP + t * 128 + 32 * hf + lanes;
@@ -799,16 +850,17 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         // positions of the warp's first and last live rows
         const unsigned lv = __ballot_sync(0xffffffffu, live);
         const int pw0 = SHARED ? __reduce_min_sync(0xffffffffu, p) : __shfl_sync(0xffffffffu, p, 0), pw1 = __shfl_sync(0xffffffffu, p, lv ? 31 - __clz(lv) : 0);
-        const long long part0 = (((long long)item * kvh + g) * pa.splits + z) * kRows;
+        const long long part0 = ((((long long)item * kvh + g) * pa.splits + z) * kAlt + (kAlt == 2 ? t : 0)) * kRows;
         float4* mine = pa.po + part0 * (kHeadDim / 4) + lr;
         float moved = -INFINITY;  // the maximum that the sums in the workspace go by
-        for (int j = 0; j < nk; ++j) {
+        for (int j = 0; j < mine_nk; ++j) {
+          const int jt = kAlt == 2 ? 2 * j + t : j;  // of the work's tiles
           ok = ok && __all_sync(0xffffffffu, pp_wait(&s_full[t], (unsigned)(j ^ turn) & 1u, &failed));
           tc_fence_after();
           unsigned sr[64];
           tmem_ld64(ts + 64 * hf, sr);
-          const int k0 = it.v.tile(t0 + j) * kPpKeys;
-          const unsigned bad = bad_rows[(done + j) & 7];
+          const int k0 = it.v.tile(t0 + jt) * kPpKeys;
+          const unsigned bad = bad_rows[(done + jt) & 7];
           const bool inside = lv == 0xffffffffu && bad == 0 && k0 + kPpKeys - 1 <= min(pw0, it.len - 1) &&
                               (a.window == 0 || k0 > pw1 - a.window || k0 + kPpKeys <= a.sinks);
           if (!inside) {
@@ -840,14 +892,14 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
             // row becomes NaN by its weights.)
             const float gone = __int_as_float(0x7fffffff);
             if (!(mt == mt)) mt = -INFINITY;
-            if (hf == 0) shared_row[lr] = ok ? mt : gone;
+            if (hf == 0) shared_row[own] = ok ? mt : gone;
             pp_meet(pair);
             if (hf == 1) {
-              const float other = shared_row[lr];
-              shared_row[lr] = ok && other == other ? fmaxf(mt, other) : gone;
+              const float other = shared_row[own];
+              shared_row[own] = ok && other == other ? fmaxf(mt, other) : gone;
             }
             pp_meet(pair);
-            mt = shared_row[lr];
+            mt = shared_row[own];
             ok = __all_sync(0xffffffffu, mt == mt);
             if (!ok) break;
             // each row by its own maximum (a factor of 1 where it has not moved), so that a row's result
@@ -922,12 +974,12 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
           if (ok) pp_arrive(&p_full[t]);
         }
         pp_meet(pair);  // (the last maximum has been read)
-        if (hf == 0) shared_row[lr] = l;
+        if (hf == 0) shared_row[own] = l;
         pp_meet(pair);
-        if (hf == 1) shared_row[lr] += l;
+        if (hf == 1) shared_row[own] += l;
         pp_meet(pair);
-        l = shared_row[lr];
-        if (ok) ok = __all_sync(0xffffffffu, pp_wait(&o_done[t], (unsigned)((nk - 1) ^ turn) & 1u, &failed));
+        l = shared_row[own];
+        if (ok) ok = __all_sync(0xffffffffu, pp_wait(&o_done[t], (unsigned)((mine_nk - 1) ^ turn) & 1u, &failed));
         if (ok) {
           tc_fence_after();
           const bool whole = !SHARED && parts == 1;
@@ -941,7 +993,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
           for (int h = 0; h < 2; ++h) {
             float o[32];
             tmem_ld32(to + 32 * h, o);
-            if (PARTS > 1 && nk > kPpFlush) {
+            if (PARTS > 1 && mine_nk > kPpFlush) {
               const float fm = moved == -INFINITY ? 0.0f : exp2_fast(moved - m);
               const float4* src = mine + (16 * hf + 8 * h) * kRows;
 #pragma unroll
@@ -989,11 +1041,12 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
           }
         }
         tc_fence_before();
-        turn ^= (unsigned)nk;
+        turn ^= (unsigned)mine_nk;
       }
       done += nk;
-      if (SHARED && live && hf == 0 && g == 0 && z == 0)
-        pa.rows[(long long)(it.tok0 + tok) * G + hs] = make_int2(item * kRows + lr, nk == 0 ? 0 : parts);
+      if (nk > 0) ++works;
+      if (SHARED && live && t == 0 && hf == 0 && g == 0 && z == 0)
+        pa.rows[(long long)(it.tok0 + tok) * G + hs] = make_int2(item * kRows + lr, it.v.tiles < 2 ? it.v.tiles : parts * kAlt);
       if (!SHARED && nk == 0 && live) {  // no key is visible to any row
         const long long base = (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf;
         for (int i = 0; i < kHeadDim / 2; i += 4) store4(a.y, base + i, a.dtype, make_float4(0.f, 0.f, 0.f, 0.f));
@@ -1017,7 +1070,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
           const int lr = e >> 5, row = w.row0 + lr, tok = w.it.tok0 + row / G;
           if ((unsigned)tok >= (unsigned)a.rows) continue;
           if (SHARED || w.parts > 1)
-            pa.pml[(((long long)w.item * kvh + w.g) * pa.splits + w.z) * kRows + lr] = make_float2(gone, gone);
+            for (int x = 0; x < kAlt; ++x)
+              pa.pml[((((long long)w.item * kvh + w.g) * pa.splits + w.z) * kAlt + x) * kRows + lr] = make_float2(gone, gone);
           else
             store4(a.y, (long long)tok * a.y_stride + ((long long)w.g * G + row % G) * kHeadDim + 4 * lane, a.dtype,
                    make_float4(gone, gone, gone, gone));
