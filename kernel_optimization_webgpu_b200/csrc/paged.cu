@@ -336,6 +336,7 @@ static void launch_shared(const PAttnArgs& a, void* workspace, cudaStream_t s) {
   }
   PSharedArgs j{};
   j.a = a;
+  j.a.beside = grid > 0;
   j.a.tail_o = reinterpret_cast<float*>(base + w.tail_o);
   j.a.tail_ml = reinterpret_cast<float2*>(base + w.tail_ml);
   j.po = p.po;

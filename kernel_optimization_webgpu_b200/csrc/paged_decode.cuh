@@ -264,7 +264,9 @@ static_assert(8 * kPdSumRow * 4 <= kPdSlot, "a slot holds eight heads' sums");
 __host__ __device__ constexpr int pd_smem(int batch) { return 4 * kPdStages * kPdSlot + (batch + 1) * 4; }
 
 // TAIL: the positions behind those that a sequence shares (paged_shared.cuh). All sums go to the workspace, a
-// (sequence, head) that one CTA holds whole to a place of its own.
+// (sequence, head) that one CTA holds whole to a place of its own. The launch before it, over the shared positions, may
+// still run (a.beside: it wrote nothing that is read here, and it began after all before it had ended), so it is
+// waited for at the end only; a fence clears L1 of what that launch may have found there.
 template <typename T, bool THREE, bool TAIL = false>
 __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_constant__ PAttnArgs a, void* workspace) {
   extern __shared__ __align__(128) unsigned char smem[];
@@ -274,7 +276,8 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
   __shared__ float2 sml[4][8];  // maximum and sum of each warp and head
   const int G = a.q_heads / a.kv.kv_heads, subs = (G + 7) >> 3, nh = a.kv.kv_heads * subs, B = a.kv.batch;
   const PDecodeWs ws = pd_ws(workspace);
-  pdl_wait();
+  if (!TAIL || !a.beside) pdl_wait();
+  else __threadfence();
   pdl_trigger();
   const int held = TAIL ? min(a.q_starts[a.groups], B) : B;  // sequences behind the last group are padding
 
@@ -293,7 +296,10 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
       for (int i = tid; i < a.q_heads * kHeadDim; i += kPdThreads) store1(a.y, b * a.y_stride + i, a.dtype, 0.0f);
   const long long U = (long long)first[B] * nh;
   const int ctas = (int)min((long long)gridDim.x, U);  // none of them empty
-  if ((int)blockIdx.x >= ctas) return;
+  if ((int)blockIdx.x >= ctas) {
+    if (TAIL) pdl_wait();
+    return;
+  }
   const int u0 = pd_div(U * blockIdx.x, ctas), u1 = pd_div(U * (blockIdx.x + 1), ctas);
 
   auto step = [&](PdCursor& c) { pd_step(c, first, a.kv.kv_heads, subs, see); };
@@ -545,6 +551,7 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
     cur = nxt;
     slot = slot + 1 == kPdStages ? 0 : slot + 1;
   }
+  if (TAIL) pdl_wait();
 }
 
 // Joins the parts of each (sequence, query group) that several CTAs hold. Grid: batch * nh. Warp w takes head w / per of the group
