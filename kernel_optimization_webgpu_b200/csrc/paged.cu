@@ -115,9 +115,15 @@ static void launch_append(const AppendArgs& a, int qkv_dtype, long long heads, c
   const long long warps = a.rows * ((heads + HEADS - 1) / HEADS);
   need(warps <= 0x7fffffffLL, "qd_paged_append: too many rows");
   const dim3 grid((unsigned)((warps + 7) / 8)), block(256);
-  if (qkv_dtype == QD_KV_F32) launch_ex(k_paged_append<float, HEADS, Q8>, grid, block, 0, s, a);
-  else if (qkv_dtype == QD_KV_F16) launch_ex(k_paged_append<__half, HEADS, Q8>, grid, block, 0, s, a);
-  else launch_ex(k_paged_append<__nv_bfloat16, HEADS, Q8>, grid, block, 0, s, a);
+  if constexpr (Q8) {
+    if (qkv_dtype == QD_KV_F32) launch_ex(k_paged_append_q8<float, HEADS / 2>, grid, block, 0, s, a);
+    else if (qkv_dtype == QD_KV_F16) launch_ex(k_paged_append_q8<__half, HEADS / 2>, grid, block, 0, s, a);
+    else launch_ex(k_paged_append_q8<__nv_bfloat16, HEADS / 2>, grid, block, 0, s, a);
+  } else {
+    if (qkv_dtype == QD_KV_F32) launch_ex(k_paged_append<float, HEADS>, grid, block, 0, s, a);
+    else if (qkv_dtype == QD_KV_F16) launch_ex(k_paged_append<__half, HEADS>, grid, block, 0, s, a);
+    else launch_ex(k_paged_append<__nv_bfloat16, HEADS>, grid, block, 0, s, a);
+  }
 }
 
 // The append calls, over a checked cache; need_apart refuses rows that lie over it.
@@ -193,13 +199,13 @@ static void launch_decode(const PAttnArgs& a, void* workspace, cudaStream_t s) {
   launch_ex(k_paged_decode<T, THREE>, dim3(ctas), dim3(kPdThreads), (size_t)pd_smem(a.kv.batch), s, a, workspace);
   // (a table of one unit leaves nothing to join)
   if ((a.kv.table_width << a.kv.page_shift) > kPdTile)
-    launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas);
+    launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas, 8);
 }
 
 template <typename Heads>
 static void launch_decode_q8(Q8Args q, void* workspace, cudaStream_t s) {
   const PAttnArgs& a = q.a;
-  const int nh = a.kv.kv_heads * ((a.q_heads / a.kv.kv_heads + 7) / 8);
+  const int nh = a.kv.kv_heads * ((a.q_heads / a.kv.kv_heads + Heads::kHeads - 1) / Heads::kHeads);
   const long long most = (long long)a.kv.batch * nh * (((long long)a.kv.table_width << a.kv.page_shift) / kQ8Tile + 1);
   if (most > 0x7fffffffLL)
     throw QdError{QD_E_RANGE, "qd_paged_attn_decode_q8: batch * heads * table beyond 2^31 units"};
@@ -217,7 +223,7 @@ static void launch_decode_q8(Q8Args q, void* workspace, cudaStream_t s) {
   launch_ex(k_paged_decode_q8<Heads>, dim3(ctas), dim3(kPdThreads), (size_t)pq8_smem(a.kv.batch), s, q, workspace);
   // (a table of one unit leaves nothing to join)
   if ((a.kv.table_width << a.kv.page_shift) > kQ8Tile)
-    launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas);
+    launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas, Heads::kHeads);
 }
 
 // Row tiles of a call (at most), and the parts that their keys are split into: enough to give
@@ -420,7 +426,7 @@ int qd_paged_read_q8(const qd_paged_q8* kv, const int32_t* first, const qd_paged
     if (kv->batch == 0) return;
     const long long most = (long long)kv->batch * kv->kv_heads * (((long long)kv->table_width << a.src.page_shift) / 16 + 1);
     if (most > 0x7fffffffLL) throw QdError{QD_E_RANGE, "qd_paged_read_q8: batch * heads * table beyond 2^31 units"};
-    const int ctas = (int)std::max(1LL, std::min<long long>((most + 3) / 4, 8 * current_sms()));
+    const int ctas = (int)std::max(1LL, std::min<long long>((most + 3) / 4, 32 * current_sms()));
     const size_t smem = (size_t)(kv->batch + 1) * 4;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (to->dtype == QD_KV_F16) launch_ex(k_paged_read_q8<__half>, dim3(ctas), dim3(kPdThreads), smem, s, a);
@@ -461,9 +467,9 @@ int qd_paged_attn_decode_q8(const qd_paged_q8* kv, const void* q, int dtype, int
     args.scale = {kv->k_scale, kv->v_scale};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int group = q_heads / kv->kv_heads;
-    if (group <= 2) launch_decode_q8<Q8Whole<1>>(args, workspace, s);
-    else if (group <= 4) launch_decode_q8<Q8Whole<2>>(args, workspace, s);
-    else launch_decode_q8<Q8Half>(args, workspace, s);
+    if (group <= 2) launch_decode_q8<Q8Whole>(args, workspace, s);
+    else if (group <= 4) launch_decode_q8<Q8Half<1>>(args, workspace, s);
+    else launch_decode_q8<Q8Half<2>>(args, workspace, s);
   });
 }
 

@@ -120,30 +120,6 @@ struct AppendArgs {
   float *k_scale, *v_scale;  // of an 8-bit cache
 };
 
-// A row of 128 elements (four a lane) as 8-bit integers n with one scale: n = round(x / scale), scale = the
-// largest magnitude / 127, so that each element is at most half a scale (1/254 of the largest) off. A row
-// with an element that is not finite gets a NaN scale (all of it reads as NaN), one whose largest is below 2^-100
-// a scale of 0. The rounding is that of an addition of 1.5 * 2^23, whose sum's low byte is n.
-__device__ __forceinline__ void store_q8(int8_t* rows, float* scales, long long row, int lane, float4 x) {
-  const unsigned none = 0x7fffffffu;
-  const unsigned mine = max(max(__float_as_uint(x.x) & none, __float_as_uint(x.y) & none),
-                            max(__float_as_uint(x.z) & none, __float_as_uint(x.w) & none));
-  const unsigned top = __reduce_max_sync(0xffffffffu, mine);  // (NaN above infinity above every number)
-  float scale = 0.0f;
-  unsigned n = 0;
-  if (top >= 0x7f800000u) {
-    scale = __uint_as_float(0x7fffffffu);
-  } else if (top >= 27u << 23) {
-    const float most = __uint_as_float(top), up = 127.0f / most, magic = 12582912.0f;
-    scale = most / 127.0f;
-    const unsigned a = __float_as_uint(fmaf(x.x, up, magic)), b = __float_as_uint(fmaf(x.y, up, magic));
-    const unsigned c = __float_as_uint(fmaf(x.z, up, magic)), d = __float_as_uint(fmaf(x.w, up, magic));
-    n = __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
-  }
-  reinterpret_cast<unsigned*>(rows + row * kHeadDim)[lane] = n;
-  if (lane == 0) scales[row] = scale;
-}
-
 // One warp per row and HEADS consecutive heads of its [q | k | v]; lane l holds dims 4l .. 4l+3, so
 // the rotation's partner dims are 16 lanes away. What it has to move bounds it (per row and head 512
 // bytes of f32 in, 512 or 256 out), so the heads' loads go out as soon as the row is known not to be
@@ -152,8 +128,7 @@ __device__ __forceinline__ void store_q8(int8_t* rows, float* scales, long long 
 // HEADS: 4 keep 2 KB in flight per warp at 40 warps an SM (16384 rows of 16 + 8 + 8 heads, f32, 470 MB:
 // 82 us = 5.7 TB/s, 88 with 8); with few rows 2 spread the work over more warps (1 row: 2.5 us, 3.2
 // with 4).
-// Q8: the K and V rows go to an 8-bit cache (store_q8).
-template <typename T, int HEADS, bool Q8 = false>
+template <typename T, int HEADS>
 __global__ void __launch_bounds__(256, HEADS == 4 ? 5 : 6) k_paged_append(const __grid_constant__ AppendArgs a) {
   const int lane = threadIdx.x & 31;
   const int heads = a.q_heads + 2 * a.kv.kv_heads;
@@ -228,11 +203,138 @@ __global__ void __launch_bounds__(256, HEADS == 4 ? 5 : 6) k_paged_append(const 
     } else if (page >= 0) {
       const int g = h < v0 ? h - k0 : h - v0;
       const long long row = (((long long)page * a.kv.kv_heads + g) << a.kv.page_shift) + in_page;
-      if constexpr (Q8)
-        store_q8(static_cast<int8_t*>(h < v0 ? a.kv.k : a.kv.v), h < v0 ? a.k_scale : a.v_scale, row, lane, y);
-      else
-        store4(h < v0 ? a.kv.k : a.kv.v, row * kHeadDim + 4 * lane, a.kv_dtype, y);
+      store4(h < v0 ? a.kv.k : a.kv.v, row * kHeadDim + 4 * lane, a.kv_dtype, y);
     }
+  }
+}
+
+// The same into a cache of 8-bit integers n with a scale per row: scale = the largest magnitude / 127, n = x / scale
+// rounded, by an addition of 1.5 * 2^23 whose sum's low byte is n: each element is at most half a scale (1/254 of
+// the largest) off, but for roundings that move a border by 127 * 2^-22 of a scale. A row with an element that is not
+// finite gets a NaN scale (all of it reads as NaN), one whose largest is below 2^-100 a scale of 0.
+//
+// Half a warp per head: lane h of it holds dims 4 h .. + 3 and 64 + 4 h .. + 3, which the rotation turns into
+// each other, and a sum or maximum takes four steps for two heads at once. (The other kernel's lanes, with the rows'
+// maxima and divisions added, were bound by instructions: 16384 rows of 16 + 8 + 8 heads, f32, 437 MB, 98 us; so 71 us = 6.1 TB/s.)
+// Sums run in that kernel's order: q comes out the same to the bit.
+template <typename T, int PAIRS>
+__global__ void __launch_bounds__(256, PAIRS == 2 ? 5 : 6) k_paged_append_q8(const __grid_constant__ AppendArgs a) {
+  const int lane = threadIdx.x & 31, hl = lane & 15, half = lane >> 4;
+  const int heads = a.q_heads + 2 * a.kv.kv_heads, k0 = a.q_heads, v0 = a.q_heads + a.kv.kv_heads;
+  const unsigned per_row = (unsigned)(heads + 2 * PAIRS - 1) / (2 * PAIRS);
+  const unsigned w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int r = (int)(w / per_row), h0 = (int)(w % per_row) * (2 * PAIRS);
+  if (r >= a.rows) return;
+  pdl_wait();
+  float4 x[PAIRS][2];
+  auto load = [&] {
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+      const long long at = r * a.qkv_stride + (long long)min(h0 + 2 * i + half, heads - 1) * kHeadDim + 4 * hl;
+      x[i][0] = load4<T>(a.qkv, at);
+      x[i][1] = load4<T>(a.qkv, at + kHeadDim / 2);
+    }
+  };
+  int b = r, back = 1;
+  if (a.q_starts) {
+    b = paged_find_seq(a.q_starts, a.kv.batch, r, load);
+    if (b < 0) return;
+    back = a.q_starts[b + 1] - r;
+  } else {
+    load();
+  }
+  const int p = a.kv.seq_lens[b] - back;
+  const long long t = (long long)p * a.rope_stride + 4 * hl;
+  const bool turned = a.cos_t != nullptr;
+  const bool live = p >= 0 && p < (a.kv.table_width << a.kv.page_shift) &&
+                    (!turned || (long long)p * a.rope_stride + kHeadDim / 2 <= a.rope_len);
+  if (!live) {
+    if (lane == 0) paged_flag(a.kv, QD_PAGED_BAD_LENGTH);
+    return;
+  }
+  float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (turned && h0 < v0) {
+    c = *reinterpret_cast<const float4*>(a.cos_t + t);
+    s = *reinterpret_cast<const float4*>(a.sin_t + t);
+  }
+  int page = -1;
+  if (h0 + 2 * PAIRS > k0) {
+    page = paged_page(a.kv, b, p);
+    if (page < 0 && lane == 0) paged_flag(a.kv, QD_PAGED_BAD_PAGE);
+  }
+  if (h0 < v0) {  // (warp-uniform: V rows are written as they are)
+    float ss[PAIRS];
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+      const float4 u = x[i][0], v = x[i][1];
+      const float su = fmaf(u.w, u.w, fmaf(u.z, u.z, fmaf(u.x, u.x, u.y * u.y)));
+      const float sv = fmaf(v.w, v.w, fmaf(v.z, v.z, fmaf(v.x, v.x, v.y * v.y)));
+      ss[i] = su + sv;
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) ss[i] += __shfl_xor_sync(0xffffffffu, ss[i], o);
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+      const int h = h0 + 2 * i + half;
+      if (h >= v0) continue;
+      float4 u = x[i][0], v = x[i][1];
+      const float* wn = h < k0 ? a.q_norm : a.k_norm;
+      if (wn) {
+        const float f = rsqrtf(ss[i] * (1.0f / kHeadDim) + a.eps);
+        const float4 n = *reinterpret_cast<const float4*>(wn + 4 * hl);
+        const float4 m = *reinterpret_cast<const float4*>(wn + kHeadDim / 2 + 4 * hl);
+        u = make_float4(u.x * f * n.x, u.y * f * n.y, u.z * f * n.z, u.w * f * n.w);
+        v = make_float4(v.x * f * m.x, v.y * f * m.y, v.z * f * m.z, v.w * f * m.w);
+      }
+      if (turned) {
+        // (which product is rounded, as in the other kernel)
+        x[i][0] = make_float4(fmaf(u.x, c.x, v.x * -s.x), fmaf(u.y, c.y, v.y * -s.y), fmaf(u.z, c.z, v.z * -s.z),
+                              fmaf(u.w, c.w, v.w * -s.w));
+        x[i][1] = make_float4(fmaf(v.x, c.x, u.x * s.x), fmaf(v.y, c.y, u.y * s.y), fmaf(v.z, c.z, u.z * s.z),
+                              fmaf(v.w, c.w, u.w * s.w));
+      } else {
+        x[i][0] = u;
+        x[i][1] = v;
+      }
+      if (h < k0) {
+        const long long at = r * a.q_out_stride + (long long)h * kHeadDim + 4 * hl;
+        store4(a.q_out, at, a.q_out_dtype, x[i][0]);
+        store4(a.q_out, at + kHeadDim / 2, a.q_out_dtype, x[i][1]);
+      }
+    }
+  }
+  if (page < 0) return;
+  const int in_page = p & ((1 << a.kv.page_shift) - 1);
+  const unsigned none = 0x7fffffffu;
+#pragma unroll
+  for (int i = 0; i < PAIRS; ++i) {
+    if (h0 + 2 * i + 1 < k0) continue;  // (both heads are q's)
+    const float4 u = x[i][0], v = x[i][1];
+    // the largest magnitude (NaN above infinity above every number)
+    unsigned top = max(max(max(__float_as_uint(u.x) & none, __float_as_uint(u.y) & none),
+                           max(__float_as_uint(u.z) & none, __float_as_uint(u.w) & none)),
+                       max(max(__float_as_uint(v.x) & none, __float_as_uint(v.y) & none),
+                           max(__float_as_uint(v.z) & none, __float_as_uint(v.w) & none)));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float scale = __uint_as_float(top) * (1.0f / 127.0f), magic = 12582912.0f;
+    const float up = __fdividef(1.0f, scale);
+    auto bytes = [&](float4 y) {
+      const unsigned d0 = __float_as_uint(fmaf(y.x, up, magic)), d1 = __float_as_uint(fmaf(y.y, up, magic));
+      const unsigned d2 = __float_as_uint(fmaf(y.z, up, magic)), d3 = __float_as_uint(fmaf(y.w, up, magic));
+      return __byte_perm(__byte_perm(d0, d1, 0x0040), __byte_perm(d2, d3, 0x0040), 0x5410);
+    };
+    const int h = h0 + 2 * i + half;
+    if (h < k0 || h >= heads) continue;
+    const bool fits = top < 0x7f800000u && top >= 27u << 23;
+    const int g = h < v0 ? h - k0 : h - v0;
+    const long long row = (((long long)page * a.kv.kv_heads + g) << a.kv.page_shift) + in_page;
+    unsigned* n = reinterpret_cast<unsigned*>(static_cast<int8_t*>(h < v0 ? a.kv.k : a.kv.v) + row * kHeadDim) + hl;
+    n[0] = fits ? bytes(u) : 0u;
+    n[16] = fits ? bytes(v) : 0u;
+    if (hl == 0) (h < v0 ? a.k_scale : a.v_scale)[row] = fits ? scale : top >= 0x7f800000u ? __uint_as_float(none) : 0.0f;
   }
 }
 

@@ -38,9 +38,10 @@ __device__ __forceinline__ float4 q8_float4(unsigned w, float s) {
   return make_float4(a.x * s, a.y * s, b.x * s, b.y * s);
 }
 // A warp takes 16 positions (which one page holds) of one sequence and KV head, K and V: lane l the eight elements
-// 8 (l % 16) of every other row, all sixteen loads before the first store. What it has to move bounds it (132 bytes
-// of a row in, 256 out). Units are counted through a scan of the lengths, so that a table wider than they are costs
-// nothing.
+// 8 (l % 16) of every other row, all sixteen loads together, and while they are on their way it finds the next 16 and looks
+// up their pages. What it has to move bounds it (132 bytes of a row in, 256 out): 24 sequences of up to 9001 positions, 527 MB,
+// 86 us = 6.1 TB/s. Units are counted through a scan of the lengths, so that a table wider than they are costs nothing, and
+// shared out over more CTAs than run at once (32 per SM; 93 us with 8), as the SMs' share of the memory's rate is not even.
 template <typename T>
 __global__ void __launch_bounds__(kPdThreads) k_paged_read_q8(const __grid_constant__ ReadArgs a) {
   extern __shared__ int first[];
@@ -59,7 +60,10 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_read_q8(const __grid_const
       if (a.src.seq_lens[b] != end_of(b)) paged_flag(a.src, QD_PAGED_BAD_LENGTH);
   const long long units = (long long)first[B] * kvh;
   const int warps = gridDim.x * (kPdThreads / 32);
-  for (long long u = blockIdx.x * (kPdThreads / 32) + (tid >> 5); u < units; u += warps) {
+  struct Unit {
+    int g, f, end, p0, ps, pd;  // its positions are those of p0 .. p0 + 15 in [f, end); entries of both tables
+  };
+  auto find = [&](long long u) {
     int lo = 0, hi = B;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -67,34 +71,57 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_read_q8(const __grid_const
       else hi = mid;
     }
     const int rest = (int)(u - (long long)first[lo] * kvh), tiles = first[lo + 1] - first[lo];
-    const int g = rest / tiles, f = from(lo), end = end_of(lo), p0 = (f / 16 + rest % tiles) * 16;
-    const int ps = paged_page(a.src, lo, p0), pd = paged_page(a.dst, lo, p0);
-    if (ps < 0 || pd < 0) {
-      if (lane == 0) paged_flag(a.src, QD_PAGED_BAD_PAGE);
-      continue;
-    }
-    const long long rs = (((long long)ps * kvh + g) << a.src.page_shift) + (p0 & ((1 << a.src.page_shift) - 1));
-    const long long rd = (((long long)pd * kvh + g) << a.dst.page_shift) + (p0 & ((1 << a.dst.page_shift) - 1));
-    const int r0 = lane >> 4, c = lane & 15;
-    // lane l: the scale of row l % 16, of K in the first half, of V in the second (rows of the page that no
-    // sequence holds are memory too, and their values are not used)
-    const float mine = (lane < 16 ? a.scale.k : a.scale.v)[rs + c];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const uint2* src = reinterpret_cast<const uint2*>(static_cast<const int8_t*>(x ? a.src.v : a.src.k) + rs * kHeadDim) + lane;
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(x ? a.dst.v : a.dst.k) + rd * kHeadDim) + lane;
-      uint2 w[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = src[i * 32];
+    Unit x;
+    x.g = rest / tiles;
+    x.f = from(lo);
+    x.end = end_of(lo);
+    x.p0 = (x.f / 16 + rest - x.g * tiles) * 16;
+    x.ps = a.src.table[(long long)lo * a.src.table_stride + (x.p0 >> a.src.page_shift)];
+    x.pd = a.dst.table[(long long)lo * a.dst.table_stride + (x.p0 >> a.dst.page_shift)];
+    return x;
+  };
+  long long u = blockIdx.x * (kPdThreads / 32) + (tid >> 5);
+  if (u >= units) return;
+  const int r0 = lane >> 4, c = lane & 15;
+  for (Unit x = find(u);;) {
+    const bool ok = (unsigned)x.ps < (unsigned)a.src.num_pages && (unsigned)x.pd < (unsigned)a.dst.num_pages;
+    uint2 w[2][8];
+    float mine = 0.0f;
+    if (ok) {
+      const long long rs = (((long long)x.ps * kvh + x.g) << a.src.page_shift) + (x.p0 & ((1 << a.src.page_shift) - 1));
+      // lane l: the scale of row l % 16, of K in the first half, of V in the second (rows of the page that no
+      // sequence holds are memory too, and their values are not used)
+      mine = (lane < 16 ? a.scale.k : a.scale.v)[rs + c];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int p = p0 + 2 * i + r0;
-        const float s = __shfl_sync(0xffffffffu, mine, 16 * x + 2 * i + r0);
-        const float4 y = q8_float4(w[i].x ^ 0x80808080u, s), z = q8_float4(w[i].y ^ 0x80808080u, s);
-        if (p >= f && p < end)
-          dst[i * 32] = make_uint4(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w), pack2<T>(z.x, z.y), pack2<T>(z.z, z.w));
+        w[0][i] = reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.src.k) + rs * kHeadDim)[i * 32 + lane];
+        w[1][i] = reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.src.v) + rs * kHeadDim)[i * 32 + lane];
+      }
+    } else if (lane == 0) {
+      paged_flag(a.src, QD_PAGED_BAD_PAGE);
+    }
+    u += warps;
+    const bool more = u < units;
+    Unit next = x;
+    if (more) next = find(u);
+    if (ok) {
+      const long long rd = (((long long)x.pd * kvh + x.g) << a.dst.page_shift) + (x.p0 & ((1 << a.dst.page_shift) - 1));
+      const bool all = x.p0 >= x.f && x.p0 + 16 <= x.end;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(n ? a.dst.v : a.dst.k) + rd * kHeadDim) + lane;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int p = x.p0 + 2 * i + r0;
+          const float s = __shfl_sync(0xffffffffu, mine, 16 * n + 2 * i + r0);
+          const float4 y = q8_float4(w[n][i].x ^ 0x80808080u, s), z = q8_float4(w[n][i].y ^ 0x80808080u, s);
+          if (all || (p >= x.f && p < x.end))
+            dst[i * 32] = make_uint4(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w), pack2<T>(z.x, z.y), pack2<T>(z.z, z.w));
+        }
       }
     }
+    if (!more) break;
+    x = next;
   }
 }
 
@@ -107,12 +134,13 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_read_q8(const __grid_const
 //    the eight rows that two heads would leave empty the other way round.
 //  - A K row's scale multiplies its scores, a V row's its weight: y = sum_j (p_j vs_j) n_j. The products take the
 //    cache's integers, and the other operand as a sum of parts that are columns side by side:
-//      up to four heads to a KV head (Q8Whole): m16n8k32 of 8-bit integers, q and the weights as 31-bit fixed-point
+//      one or two heads to a KV head (Q8Whole): m16n8k32 of 8-bit integers, q and the weights as 31-bit fixed-point
 //      numbers in four signed bytes, exact sums in 32 bits. K goes into it as it lies in memory, V transposed by bytes
 //      in registers;
 //      more heads (Q8Half): m16n8k16 of f16, the integers made f16 (byte permutes and a subtraction per pair), q and the
-//      weights as two f16. Its products are for four heads what the others are for two, and its sums
-//      need a third of the registers.
+//      weights as two f16. Its columns hold twice the heads, and its sums take a third of the registers.
+//    64 sequences of 2048 positions, 8 KV heads: 16 query heads 55 us with Q8Whole and 58 with Q8Half; 32 query heads 71 and
+//    63 (with four heads in Q8Whole); 4 KV heads and 32 query heads 50 with Q8Half, 75 with Q8Whole twice.
 //  - The contraction's index may have any order that both operands share: thread t of a quad takes dims
 //    32 t .. + 31 of a K row (two 16-byte loads) and 16 consecutive dims of some positions of V.
 //  - A V row's scale may have any size beside its weight (the first token's V is small in many models, and its weight
@@ -160,19 +188,17 @@ struct Q8Seen {
 };
 __device__ __forceinline__ uint4 q8_lds(const unsigned char* at) { return *reinterpret_cast<const uint4*>(at); }
 
-// Up to 2 * SETS heads. Set n has heads 2 n and 2 n + 1: columns 4 (h % 2) + part, part 3 the most significant byte. Thread
-// (g8, t4) has the scores of head 2 n + t4 / 2 at positions order(g8) + 8 j, j < 4 (as its neighbour t4 ^ 1 has), and
-// dims 16 g8 .. + 15 of two of the head's parts. Positions are taken in an order for which the rows that a quarter warp reads
-// from shared memory lie on distinct banks.
-template <int SETS>
+// One or two heads: columns 4 h + part, part 3 the most significant byte. Thread (g8, t4) has the scores of head t4 / 2 at
+// positions order(g8) + 8 j, j < 4 (as its neighbour t4 ^ 1 has), and dims 16 g8 .. + 15 of two of the head's parts.
+// Positions are taken in an order for which the rows that a quarter warp reads from shared memory lie on distinct banks.
 struct Q8Whole {
-  static constexpr int kHeads = 2 * SETS, kCtas = SETS == 1 ? 3 : 2;  // CTAs per SM
-  static constexpr float kLag = 1.0f;     // log2 that a weights' maximum may fall behind
-  static constexpr float kShift = 29.0f;  // weights are kept times 2^29: with the lag at most 2^30, the largest off by 2^-30
-  static constexpr int kFlush = 2048;     // units after which the 32-bit sums are moved (each adds below 2^19)
-  unsigned q[SETS][4][2];
-  int acc[SETS][8][4];
-  float o[SETS][16], m[SETS], mo[SETS], l[SETS], factor[SETS];
+  static constexpr int kHeads = 2, kCtas = 3;  // heads, CTAs per SM
+  static constexpr float kLag = 1.0f;          // log2 that a weights' maximum may fall behind
+  static constexpr float kShift = 29.0f;       // weights are kept times 2^29 (with the lag at most 2^30), off by 2^-30 of the largest
+  static constexpr int kFlush = 2048;          // units after which the 32-bit sums are moved (each adds below 2^19)
+  unsigned q[4][2];
+  int acc[8][4];
+  float o[16], m, mo, l, factor;
   int since;
 
   static __device__ __forceinline__ int order(int c) { return 2 * (c & 3) + ((c ^ (c >> 2)) & 1); }
@@ -196,134 +222,119 @@ struct Q8Whole {
 
   __device__ __forceinline__ void start(const PAttnArgs& a, const PdCursor& c, int G, int g8, int t4) {
     since = 0;
+    const int hs = c.sub * kHeads + (g8 >> 2);
+    const bool live = hs < G;
+    const long long base = c.b * a.q_stride + ((long long)c.g * G + (live ? hs : 0)) * kHeadDim + 32 * t4;
+    float2 x[16];
+    unsigned top = 0;
 #pragma unroll
-    for (int n = 0; n < SETS; ++n) {
-      const int hs = c.sub * 8 + 2 * n + (g8 >> 2);
-      const bool live = hs < G;
-      const long long base = c.b * a.q_stride + ((long long)c.g * G + (live ? hs : 0)) * kHeadDim + 32 * t4;
-      float2 x[16];
-      unsigned top = 0;
+    for (int k = 0; k < 16; ++k) x[k] = load2(a.q, base + 2 * k, a.dtype);
 #pragma unroll
-      for (int k = 0; k < 16; ++k) x[k] = load2(a.q, base + 2 * k, a.dtype);
-#pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        if (!live) x[k] = make_float2(0.f, 0.f);
-        top = max(top, max(__float_as_uint(x[k].x) & 0x7fffffffu, __float_as_uint(x[k].y) & 0x7fffffffu));
-      }
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // by a power of two (in two steps from very small ones) to below 2^30
-      const int e = (int)(top >> 23), small = e < 60;
-      const float up0 = small ? 18446744073709551616.0f : 1.0f, down0 = small ? 5.421010862427522e-20f : 1.0f;
-      const int f = min(small ? e + 64 : e, 254);
-      const float up = __int_as_float((283 - f) << 23), down = __int_as_float((f - 29) << 23);
-      const unsigned sel = 0x0040u + 0x11u * (g8 & 3);  // byte g8 % 4 of two words
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        unsigned d[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float y = i & 1 ? x[2 * k + (i >> 1)].y : x[2 * k + (i >> 1)].x;
-          d[i] = digits(__float2int_rn(y * up0 * up));
-        }
-        q[n][k >> 1][k & 1] = __byte_perm(__byte_perm(d[0], d[1], sel), __byte_perm(d[2], d[3], sel), 0x5410);
-      }
-      // of the head whose scores this thread has; not finite: its scores are NaN
-      const float mine = e == 255 ? __int_as_float(0x7fffffff) : a.scale * kLog2e * down0 * down;
-      factor[n] = __shfl_sync(0xffffffffu, mine, 16 * (t4 >> 1));
-#pragma unroll
-      for (int j = 0; j < 16; ++j) o[n][j] = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) acc[n][j][0] = acc[n][j][1] = acc[n][j][2] = acc[n][j][3] = 0;
-      m[n] = mo[n] = -INFINITY;
-      l[n] = 0.0f;
+    for (int k = 0; k < 16; ++k) {
+      if (!live) x[k] = make_float2(0.f, 0.f);
+      top = max(top, max(__float_as_uint(x[k].x) & 0x7fffffffu, __float_as_uint(x[k].y) & 0x7fffffffu));
     }
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // by a power of two (in two steps from very small ones) to below 2^30
+    const int e = (int)(top >> 23), small = e < 60;
+    const float up0 = small ? 18446744073709551616.0f : 1.0f, down0 = small ? 5.421010862427522e-20f : 1.0f;
+    const int f = min(small ? e + 64 : e, 254);
+    const float up = __int_as_float((283 - f) << 23), down = __int_as_float((f - 29) << 23);
+    const unsigned sel = 0x0040u + 0x11u * (g8 & 3);  // byte g8 % 4 of two words
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      unsigned d[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float y = i & 1 ? x[2 * k + (i >> 1)].y : x[2 * k + (i >> 1)].x;
+        d[i] = digits(__float2int_rn(y * up0 * up));
+      }
+      q[k >> 1][k & 1] = __byte_perm(__byte_perm(d[0], d[1], sel), __byte_perm(d[2], d[3], sel), 0x5410);
+    }
+    // of the head whose scores this thread has; not finite: its scores are NaN
+    const float mine = e == 255 ? __int_as_float(0x7fffffff) : a.scale * kLog2e * down0 * down;
+    factor = __shfl_sync(0xffffffffu, mine, 16 * (t4 >> 1));
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[j] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0;
+    m = mo = -INFINITY;
+    l = 0.0f;
   }
   // Moves the 32-bit sums to the f32 ones, times f.
-  __device__ __forceinline__ void flush(int n, float f) {
+  __device__ __forceinline__ void flush(float f) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        o[n][2 * j + e] = (o[n][2 * j + e] + fmaf((float)acc[n][j][2 * e + 1], 256.0f, (float)acc[n][j][2 * e])) * f;
-        acc[n][j][2 * e] = acc[n][j][2 * e + 1] = 0;
+        o[2 * j + e] = (o[2 * j + e] + fmaf((float)acc[j][2 * e + 1], 256.0f, (float)acc[j][2 * e])) * f;
+        acc[j][2 * e] = acc[j][2 * e + 1] = 0;
       }
   }
   __device__ __forceinline__ void unit(const unsigned char* kb, const unsigned char* vb, const float* ks, const float* vs,
                                        const Q8Seen& seen, int g8, int t4) {
     const int r0 = order(g8);
-    float p[SETS][4], u[SETS][4];  // of positions r0 + 8 j: scores, and with V's scale
+    float p[4], u[4];  // of positions r0 + 8 j: scores, and with V's scale
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      int s[SETS][4];
-#pragma unroll
-      for (int n = 0; n < SETS; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0;
+      int s[4] = {0, 0, 0, 0};
       const unsigned char* row = kb + (16 * h + r0) * 128;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const unsigned char* at = row + (((2 * t4 + c) ^ r0) << 4);
         const uint4 x = q8_lds(at), y = q8_lds(at + 1024);
-#pragma unroll
-        for (int n = 0; n < SETS; ++n) {
-          mma(s[n], x.x, y.x, x.y, y.y, q[n][2 * c][0], q[n][2 * c][1]);
-          mma(s[n], x.z, y.z, x.w, y.w, q[n][2 * c + 1][0], q[n][2 * c + 1][1]);
-        }
+        mma(s, x.x, y.x, x.y, y.y, q[2 * c][0], q[2 * c][1]);
+        mma(s, x.z, y.z, x.w, y.w, q[2 * c + 1][0], q[2 * c + 1][1]);
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int j = 2 * h + e;
         const float sc = ks[r0 + 8 * j], lv = log2_fast(vs[r0 + 8 * j]);
-#pragma unroll
-        for (int n = 0; n < SETS; ++n) {  // two bytes of q here (below 2^30 together), two in the neighbour
-          const float x = (float)(s[n][2 * e] + 256 * s[n][2 * e + 1]) * (t4 & 1 ? 65536.0f : 1.0f);
-          p[n][j] = (x + __shfl_xor_sync(0xffffffffu, x, 1)) * (factor[n] * sc);
-          u[n][j] = p[n][j] + lv;
-        }
+        // two bytes of q here (below 2^30 together), two in the neighbour
+        const float x = (float)(s[2 * e] + 256 * s[2 * e + 1]) * (t4 & 1 ? 65536.0f : 1.0f);
+        p[j] = (x + __shfl_xor_sync(0xffffffffu, x, 1)) * (factor * sc);
+        u[j] = p[j] + lv;
       }
     }
     if (!seen.inside) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (!seen.at(r0 + 8 * j))
-#pragma unroll
-          for (int n = 0; n < SETS; ++n) p[n][j] = u[n][j] = -INFINITY;
+        if (!seen.at(r0 + 8 * j)) p[j] = u[j] = -INFINITY;
     }
     const bool full = ++since == kFlush;
     if (full) since = 0;
-    unsigned w[SETS][2];
+    unsigned w[2];
+    float mt = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
+    float ut = fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3]));
 #pragma unroll
-    for (int n = 0; n < SETS; ++n) {
-      float mt = fmaxf(fmaxf(p[n][0], p[n][1]), fmaxf(p[n][2], p[n][3]));
-      float ut = fmaxf(fmaxf(u[n][0], u[n][1]), fmaxf(u[n][2], u[n][3]));
+    for (int x = 4; x < 32; x <<= 1) {
+      mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
+      ut = fmaxf(ut, __shfl_xor_sync(0xffffffffu, ut, x));
+    }
+    if (__any_sync(0xffffffffu, full || mt > m + kPdLag || ut > mo + kLag)) {  // some head's maximum moved
+      const float mn = mt > m + kPdLag ? mt : m, un = ut > mo + kLag ? ut : mo;
+      l *= m == -INFINITY ? 0.0f : exp2_fast(m - mn);
+      flush(mo == -INFINITY ? 0.0f : exp2_fast(mo - un));
+      m = mn;
+      mo = un;
+    }
+    const float ref = m == -INFINITY ? 0.0f : m, uref = mo == -INFINITY ? 0.0f : mo - kShift;
+    unsigned d[4], r[4];
 #pragma unroll
-      for (int x = 4; x < 32; x <<= 1) {
-        mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
-        ut = fmaxf(ut, __shfl_xor_sync(0xffffffffu, ut, x));
-      }
-      if (__any_sync(0xffffffffu, full || mt > m[n] + kPdLag || ut > mo[n] + kLag)) {  // some head's maximum moved
-        const float mn = mt > m[n] + kPdLag ? mt : m[n], un = ut > mo[n] + kLag ? ut : mo[n];
-        l[n] *= m[n] == -INFINITY ? 0.0f : exp2_fast(m[n] - mn);
-        flush(n, mo[n] == -INFINITY ? 0.0f : exp2_fast(mo[n] - un));
-        m[n] = mn;
-        mo[n] = un;
-      }
-      const float ref = m[n] == -INFINITY ? 0.0f : m[n], uref = mo[n] == -INFINITY ? 0.0f : mo[n] - kShift;
-      unsigned d[4], r[4];
+    for (int j = 0; j < 4; ++j) {
+      const float x = exp2_fast(u[j] - uref);
+      l = fmaf(x, 0.0f, l) + exp2_fast(p[j] - ref);  // (a NaN weight is no integer)
+      d[j] = digits(__float2int_rn(x));
+    }
+    // the parts of four positions each; thread (g8, t4) wants part g8 % 4 of head g8 / 4 of those that rows t4 and t4 + 4 have
+    turn(d[0], d[1], d[2], d[3], r);
+    const unsigned even = t4 & 1 ? r[2] : r[0], odd = t4 & 1 ? r[3] : r[1];
+    const int from = 4 * t4 + 2 * (g8 >> 2) + ((g8 >> 1) & 1);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float x = exp2_fast(u[n][j] - uref);
-        l[n] = fmaf(x, 0.0f, l[n]) + exp2_fast(p[n][j] - ref);  // (a NaN weight is no integer)
-        d[j] = digits(__float2int_rn(x));
-      }
-      // the parts of four positions each; thread (g8, t4) wants part g8 % 4 of head g8 / 4 of those that rows t4 and t4 + 4 have
-      turn(d[0], d[1], d[2], d[3], r);
-      const unsigned even = t4 & 1 ? r[2] : r[0], odd = t4 & 1 ? r[3] : r[1];
-      const int from = 4 * t4 + 2 * (g8 >> 2) + ((g8 >> 1) & 1);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const unsigned x = __shfl_sync(0xffffffffu, even, from + 16 * e), y = __shfl_sync(0xffffffffu, odd, from + 16 * e);
-        w[n][e] = g8 & 1 ? y : x;
-      }
+    for (int e = 0; e < 2; ++e) {
+      const unsigned x = __shfl_sync(0xffffffffu, even, from + 16 * e), y = __shfl_sync(0xffffffffu, odd, from + 16 * e);
+      w[e] = g8 & 1 ? y : x;
     }
     // V: positions order(t4) + 8 j and order(t4 + 4) + 8 j, dims 16 g8 .. + 15
     const int ra = order(t4), rb = order(t4 + 4);
@@ -339,52 +350,44 @@ struct Q8Whole {
       unsigned e[4], f[4];
       turn(xa, xb, xc, xd, e);
       turn(ya, yb, yc, yd, f);
-#pragma unroll
-      for (int n = 0; n < SETS; ++n) {
-        mma(acc[n][2 * k], e[0], e[1], f[0], f[1], w[n][0], w[n][1]);
-        mma(acc[n][2 * k + 1], e[2], e[3], f[2], f[3], w[n][0], w[n][1]);
-      }
+      mma(acc[2 * k], e[0], e[1], f[0], f[1], w[0], w[1]);
+      mma(acc[2 * k + 1], e[2], e[3], f[2], f[3], w[0], w[1]);
     };
     dims(0, x[0].x, x[1].x, x[2].x, x[3].x, y[0].x, y[1].x, y[2].x, y[3].x);
     dims(1, x[0].y, x[1].y, x[2].y, x[3].y, y[0].y, y[1].y, y[2].y, y[3].y);
     dims(2, x[0].z, x[1].z, x[2].z, x[3].z, y[0].z, y[1].z, y[2].z, y[3].z);
     dims(3, x[0].w, x[1].w, x[2].w, x[3].w, y[0].w, y[1].w, y[2].w, y[3].w);
   }
-  __device__ __forceinline__ void give_up() {
-#pragma unroll
-    for (int n = 0; n < SETS; ++n) l[n] = __int_as_float(0x7fffffff);
-  }
+  __device__ __forceinline__ void give_up() { l = __int_as_float(0x7fffffff); }
   // The warp's sums of head h to sums[h * kPdSumRow + dim], maximum and weights to ml[h], the maximum of the sums to mos[h].
   __device__ __forceinline__ void finish(float* sums, float2* ml, float* mos, int g8, int t4) {
+    flush(1.0f);
 #pragma unroll
-    for (int n = 0; n < SETS; ++n) {
-      flush(n, 1.0f);
+    for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+    float y[16];
 #pragma unroll
-      for (int x = 4; x < 32; x <<= 1) l[n] += __shfl_xor_sync(0xffffffffu, l[n], x);
-      float y[16];
+    for (int j = 0; j < 16; ++j) {
+      const float x = o[j] * (t4 & 1 ? 65536.0f : 1.0f);
+      y[j] = x + __shfl_xor_sync(0xffffffffu, x, 1);
+    }
+    const int h = t4 >> 1;
+    float* mine = sums + h * kPdSumRow + 16 * g8 + 8 * (t4 & 1);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float x = o[n][j] * (t4 & 1 ? 65536.0f : 1.0f);
-        y[j] = x + __shfl_xor_sync(0xffffffffu, x, 1);
-      }
-      const int h = 2 * n + (t4 >> 1);
-      float* mine = sums + h * kPdSumRow + 16 * g8 + 8 * (t4 & 1);
-#pragma unroll
-      for (int j = 0; j < 8; j += 4)
-        *reinterpret_cast<float4*>(mine + j) = t4 & 1 ? make_float4(y[8 + j], y[9 + j], y[10 + j], y[11 + j])
-                                                     : make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
-      if (g8 == 0 && !(t4 & 1)) {
-        ml[h] = make_float2(m[n], l[n]);
-        mos[h] = mo[n];
-      }
+    for (int j = 0; j < 8; j += 4)
+      *reinterpret_cast<float4*>(mine + j) = t4 & 1 ? make_float4(y[8 + j], y[9 + j], y[10 + j], y[11 + j])
+                                                   : make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
+    if (g8 == 0 && !(t4 & 1)) {
+      ml[h] = make_float2(m, l);
+      mos[h] = mo;
     }
   }
 };
 
-// Up to eight heads. Set n has heads 4 n .. + 3: columns 2 (h % 4) (the 16-bit part) and + 1 (the rest). Thread (g8, t4) has
+// Up to 4 * SETS heads. Set n has heads 4 n .. + 3: columns 2 (h % 4) (the 16-bit part) and + 1 (the rest). Thread (g8, t4) has
 // the scores of head 4 n + t4 at positions g8 + 8 j, and its dims 16 g8 .. + 15.
+template <int SETS>
 struct Q8Half {
-  static constexpr int kHeads = 8, kCtas = 2, SETS = 2;
+  static constexpr int kHeads = 4 * SETS, kCtas = SETS == 1 ? 3 : 2;
   static constexpr float kShift = kPdShift;
   unsigned q[SETS][8][2];
   float o[SETS][8][4], m[SETS], mo[SETS], l[SETS], factor[SETS];
@@ -392,7 +395,7 @@ struct Q8Half {
   __device__ __forceinline__ void start(const PAttnArgs& a, const PdCursor& c, int G, int g8, int t4) {
 #pragma unroll
     for (int n = 0; n < SETS; ++n) {
-      const int hs = c.sub * 8 + 4 * n + (g8 >> 1);
+      const int hs = c.sub * kHeads + 4 * n + (g8 >> 1);
       const bool live = hs < G;
       const long long base = c.b * a.q_stride + ((long long)c.g * G + (live ? hs : 0)) * kHeadDim + 32 * t4;
       float2 x[16];
@@ -558,7 +561,7 @@ __global__ void __launch_bounds__(kPdThreads, Heads::kCtas) k_paged_decode_q8(co
   __shared__ unsigned long long full[4][kQ8Stages];
   __shared__ float2 sml[4][8];  // maximum and sum of weights of each warp and head,
   __shared__ float smo[4][8];   // the maximum that its sums go by
-  const int G = a.q_heads / a.kv.kv_heads, subs = (G + 7) >> 3, nh = a.kv.kv_heads * subs, B = a.kv.batch;
+  const int G = a.q_heads / a.kv.kv_heads, subs = (G + Heads::kHeads - 1) / Heads::kHeads, nh = a.kv.kv_heads * subs, B = a.kv.batch;
   const PDecodeWs ws = pd_ws(workspace);
   if (tid == 0) {
     tma_prefetch_map(&qa.tk);
@@ -603,8 +606,8 @@ __global__ void __launch_bounds__(kPdThreads, Heads::kCtas) k_paged_decode_q8(co
   // the queries of a (sequence, head) brought near before they are needed
   const int q_bytes = a.dtype == QD_KV_F32 ? 4 : 2;
   auto near_q = [&](const PdCursor& c) {
-    const char* at = static_cast<const char*>(a.q) + (c.b * a.q_stride + ((long long)c.g * G + c.sub * 8) * kHeadDim) * q_bytes;
-    if (lane * 128 < min(8, G - c.sub * 8) * kHeadDim * q_bytes) asm volatile("prefetch.global.L1 [%0];" ::"l"(at + lane * 128));
+    const char* at = static_cast<const char*>(a.q) + (c.b * a.q_stride + ((long long)c.g * G + c.sub * Heads::kHeads) * kHeadDim) * q_bytes;
+    if (lane * 128 < min(Heads::kHeads, G - c.sub * Heads::kHeads) * kHeadDim * q_bytes) asm volatile("prefetch.global.L1 [%0];" ::"l"(at + lane * 128));
   };
   int next_page = page_of(pre);
   near_q(pre);
@@ -685,9 +688,9 @@ __global__ void __launch_bounds__(kPdThreads, Heads::kCtas) k_paged_decode_q8(co
       // just been read.
       heads.finish(reinterpret_cast<float*>(ring + slot * kQ8Slot), sml[warp], smo[warp], g8, t4);
       __syncthreads();
-      const int live = min(8, G - cur.sub * 8);
+      const int live = min(Heads::kHeads, G - cur.sub * Heads::kHeads);
       const bool whole = from_start && last_t;
-      const long long out = cur.b * a.y_stride + ((long long)cur.g * G + cur.sub * 8) * kHeadDim + tid;
+      const long long out = cur.b * a.y_stride + ((long long)cur.g * G + cur.sub * Heads::kHeads) * kHeadDim + tid;
       const long long part = (2ll * blockIdx.x + (seg ? 1 : 0)) * 8;
       for (int h = 0; h < live; ++h) {  // thread tid: dim tid
         const float M = fmaxf(fmaxf(sml[0][h].x, sml[1][h].x), fmaxf(sml[2][h].x, sml[3][h].x));

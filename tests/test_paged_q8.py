@@ -150,12 +150,12 @@ def plain(torch, q, k, v, ks, vs, table, lens, window, sinks, scale, io):
         eps = (2 * S * (2.0 ** -19 + 2.0 ** -21 + 2.0 ** -22) + 2.0 ** -20 + 2.0 ** -21 + lg * 2.0 ** -22
                + (1.45 * S + lg) * 2.0 ** -24 + t / 16 * 2.0 ** -23 + 2.0 ** -19)
         # A weight times its scale is a sum of two f16, whose last step is 2^-24, where the largest of them stands at 2^7
-        # or above (off by 2^-25 at most, 2^-32 of the largest), or, with up to four heads to a KV head, a whole number
+        # or above (off by 2^-25 at most, 2^-32 of the largest), or, with one or two heads to a KV head, a whole number
         # where the largest stands at 2^29 or above: off by half, 2^-30 of the largest. That shows where the heavy rows'
         # integers are 0.
         vsc = vs[pg, :, j % page].double().T.repeat_interleave(H // kvh, 0)
         ints = v[pg, :, j % page].double().abs().sum(0).repeat_interleave(H // kvh, 0)
-        small = 2.0 ** (-30 if H // kvh <= 4 else -32) * (w * vsc).amax(-1, keepdim=True) * ints
+        small = 2.0 ** (-30 if H // kvh <= 2 else -32) * (w * vsc).amax(-1, keepdim=True) * ints
         ys.append(y)
         tols.append(small + 2 * A * eps + HALF_STEP[io] * y.abs() + (2.0 ** -25 if io == "f16" else 1e-30))
     return torch.stack(ys), torch.stack(tols)
