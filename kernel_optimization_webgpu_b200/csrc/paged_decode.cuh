@@ -80,9 +80,9 @@ __device__ __forceinline__ Visible visible(int asked, int len, int window, int s
   return v;
 }
 
-// The positions of sequence b from its shared_lens[b]-th on, and kPdEnds tiles without any: what a (sequence,
+// The positions of sequence b from its shared_lens[b]-th on, and kPdEnds tile without any: what a (sequence,
 // head)'s end costs a CTA beside its tiles, so that a run of many short ones is shared out over more CTAs.
-constexpr int kPdEnds = 2;
+constexpr int kPdEnds = 1;
 template <int TILE>
 __device__ __forceinline__ Visible tail(const PAttnArgs& a, int b) {
   Visible v{};

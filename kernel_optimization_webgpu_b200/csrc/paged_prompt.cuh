@@ -359,6 +359,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
   constexpr int kTiles = pp_tiles<PARTS>(), kQTiles = SHARED ? 1 : kTiles, kRows = 128 * kQTiles;
   constexpr int S = SHARED ? pp_shared_slots<PARTS>() : pp_slots<PARTS>();
   constexpr int kAlt = SHARED ? kTiles : 1;  // sets that share the key tiles of a row
+  // (with three parts and one set, a tile's 24 products into O cost 1.7e-6 of the result with moves every four tiles, 1.0e-6 so)
+  constexpr int kFlush = SHARED && PARTS == 3 ? 2 : kPpFlush;
   constexpr int kQTile = PARTS * kPpTileBytes;  // the parts of 128 rows
   // TMEM columns: S_t | O_t with P over S, or S | P (three parts) | O
   constexpr unsigned kColP = kTiles == 2 ? 0 : 128, kColO = kTiles == 2 ? 256 : 384;
@@ -659,7 +661,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                 const int ks = 2 * half + (i & 1) + 4 * (i >> 1);  // keys 0-31 and 64-95, then the others
                 const unsigned po = (PARTS - 1 - part) * 64 + ks * 8;
                 if (half == 0 && part == 0 && i == 0)
-                  pp_mma_ts(od, pd + po, v0, id_o, PARTS > 1 ? n % kPpFlush != 0 : n > 0, leader);
+                  pp_mma_ts(od, pd + po, v0, id_o, PARTS > 1 ? n % kFlush != 0 : n > 0, leader);
                 else
                   pp_mma_ts(od, pd + po, v0 + ks * (2048 >> 4), id_o, true, leader);
               }
@@ -921,7 +923,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
               }
             }
           }
-          if (PARTS > 1 && j > 0 && j % kPpFlush == 0) {
+          if (PARTS > 1 && j > 0 && j % kFlush == 0) {
             ok = ok && __all_sync(0xffffffffu, pp_wait(&o_done[t], (unsigned)((j - 1) ^ turn) & 1u, &failed));
             tc_fence_after();
             const float f = moved == -INFINITY ? 0.0f : exp2_fast(moved - m);
@@ -934,7 +936,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
               for (int i = 0; i < 4; ++i) {
                 float4 x = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
                                        __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
-                if (j > kPpFlush) {
+                if (j > kFlush) {
                   const float4 y = dst[i * kRows];
                   x = make_float4(fmaf(y.x, f, x.x), fmaf(y.y, f, x.y), fmaf(y.z, f, x.z), fmaf(y.w, f, x.w));
                 }
@@ -993,7 +995,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
           for (int h = 0; h < 2; ++h) {
             float o[32];
             tmem_ld32(to + 32 * h, o);
-            if (PARTS > 1 && mine_nk > kPpFlush) {
+            if (PARTS > 1 && mine_nk > kFlush) {
               const float fm = moved == -INFINITY ? 0.0f : exp2_fast(moved - m);
               const float4* src = mine + (16 * hf + 8 * h) * kRows;
 #pragma unroll
