@@ -290,9 +290,10 @@ int qd_run_full_decoder_stack_benchmark(qd_engine* e, qd_stack_bench* out);
  *    QD_E_TIMEOUT. Both only enqueue (on the engine's stream). */
 int qd_engine_inject_stall(qd_engine* e);
 int qd_batch_inject_stall(qd_batch* b);
-/*  - qd_paged_inject_stall: the calling thread's next qd_paged_attn_prompt withholds the first key
- *    tile of its block 0, whose waits end after 1 s: QD_PAGED_TIMEOUT is set, the rows that the block
- *    held are NaN and all others are right. (In a captured call, at every replay.) */
+/*  - qd_paged_inject_stall: the calling thread's next qd_paged_attn_prompt, qd_paged_attn_decode_shared or
+ *    qd_paged_attn_decode_q8 withholds the first key tile of its block 0, whose waits end after 1 s:
+ *    QD_PAGED_TIMEOUT is set, the rows that the block held are NaN and all others are right. (In a
+ *    captured call, at every replay.) */
 void qd_paged_inject_stall(void);
 
 /* runCustomQwenGreedyPrompt over `batch` prompts of n_prompt ids each: prefill,
@@ -397,7 +398,7 @@ int qd_gqa_decode_noalloc(const float* q, const void* k_cache, const void* v_cac
  * attention calls a sequence of length 0 is padding: its rows get zeros and no bit is set.) */
 #define QD_PAGED_BAD_PAGE 1     /* status bits (or-ed; never cleared by the library) */
 #define QD_PAGED_BAD_LENGTH 2
-#define QD_PAGED_TIMEOUT 4      /* a device-side wait of qd_paged_attn_prompt expired: rows of y are NaN */
+#define QD_PAGED_TIMEOUT 4      /* a device-side wait of an attention call expired: rows of y are NaN */
 
 typedef struct qd_paged_kv {
   void* k;                      /* [num_pages][kv_heads][page_size][head_dim] of dtype, 16-byte aligned */
@@ -497,9 +498,10 @@ typedef struct qd_paged_q8 {
 } qd_paged_q8;
 
 /* qd_paged_append into such a cache: what it would write of a K or V row x (in f32) is written as
- * scale = max|x| / 127 and n = x / scale rounded to the nearest integer, -127..127. A row with an
- * element that is not finite gets a NaN scale, one whose largest magnitude is below 2^-100 a
- * scale of 0 and zeros. */
+ * scale = max|x| / 127 and n = x / scale rounded to the nearest integer, -127..127 (to f32: a
+ * border between two integers may lie 2^-15 of a step aside). A row with an element that is not
+ * finite gets a NaN scale, one whose largest magnitude is below 2^-100 a scale of 0 and zeros. Where the
+ * block table makes two new rows share a position, what is left there may mix both. */
 int qd_paged_append_q8(const qd_paged_q8* kv, const void* qkv, int qkv_dtype, int64_t qkv_stride, int rows,
                        const int32_t* q_starts, int q_heads, const float* q_norm, const float* k_norm, float eps,
                        const float* cos, const float* sin, int64_t rope_len, int64_t rope_stride, void* q_out,
@@ -514,9 +516,11 @@ int qd_paged_append_q8(const qd_paged_q8* kv, const void* qkv, int qkv_dtype, in
 int qd_paged_read_q8(const qd_paged_q8* kv, const int32_t* first, const qd_paged_kv* to, void* stream);
 
 /* qd_paged_attn_decode over such a cache; dtype (of q and y) is QD_KV_F32, QD_KV_F16 or
- * QD_KV_BF16. The products keep f32 accuracy for every dtype (the integers are exact operands; q and
- * the weights are sums of two f16, the weights times V's scales with a common exponent of their own). The
- * workspace is qd_paged_attn_decode_workspace_bytes(batch, q_heads). */
+ * QD_KV_BF16. The products keep f32 accuracy for every dtype: the integers are exact operands, q is
+ * held to 2^-22 of each element or 2^-30 of its head's largest, a weight times its V row's scale to
+ * 2^-22 of itself or 2^-30 of the largest such product. Scales must not be negative. A device-side
+ * wait that expires makes rows NaN and sets QD_PAGED_TIMEOUT. The workspace is
+ * qd_paged_attn_decode_workspace_bytes(batch, q_heads). */
 int qd_paged_attn_decode_q8(const qd_paged_q8* kv, const void* q, int dtype, int64_t q_stride, int q_heads, int window,
                             int sinks, float scale, void* y, int64_t y_stride, void* workspace, void* stream);
 

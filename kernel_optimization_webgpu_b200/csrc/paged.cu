@@ -199,7 +199,15 @@ static void launch_decode(const PAttnArgs& a, void* workspace, cudaStream_t s) {
   launch_ex(k_paged_decode<T, THREE>, dim3(ctas), dim3(kPdThreads), (size_t)pd_smem(a.kv.batch), s, a, workspace);
   // (a table of one unit leaves nothing to join)
   if ((a.kv.table_width << a.kv.page_shift) > kPdTile)
-    launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas, 8);
+    launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas, 8, true);
+}
+
+// qd_paged_inject_stall, taken by the thread's next call.
+static thread_local bool stall_next = false;
+static bool take_stall() {
+  const bool stall = stall_next;
+  stall_next = false;
+  return stall;
 }
 
 template <typename Heads>
@@ -222,8 +230,11 @@ static void launch_decode_q8(Q8Args q, void* workspace, cudaStream_t s) {
   const int ctas = (int)std::max(1LL, std::min<long long>(most, std::min(Heads::kCtas * current_sms(), kPdMaxCtas)));
   launch_ex(k_paged_decode_q8<Heads>, dim3(ctas), dim3(kPdThreads), (size_t)pq8_smem(a.kv.batch), s, q, workspace);
   // (a table of one unit leaves nothing to join)
+  // What follows starts when the join's CTAs have left: three CTAs of the next call fill an SM, and among the join's some
+  // did not find their place in one piece until others had ended (64 sequences of 2048 positions, call after call: 70 us
+  // instead of 56).
   if ((a.kv.table_width << a.kv.page_shift) > kQ8Tile)
-    launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas, Heads::kHeads);
+    launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas, Heads::kHeads, false);
 }
 
 // Row tiles of a call (at most), and the parts that their keys are split into: enough to give
@@ -235,8 +246,6 @@ static int prompt_splits(int items, int kv_heads) {
   const long long n = (long long)items * kv_heads;
   return n == 0 ? 1 : (int)std::max(1LL, std::min<long long>(kPpMaxSplits, current_sms() / n));
 }
-
-static thread_local bool stall_next = false;  // qd_paged_inject_stall
 
 template <typename T>
 static void pool_maps(PPromptArgs& p, const void* any, const char* too_large) {
@@ -264,8 +273,7 @@ static void launch_prompt(const PAttnArgs& a, const void* q_any, void* workspace
   PPromptArgs p{};
   p.a = a;
   p.cta_rows = kRows;
-  p.stall = stall_next;
-  stall_next = false;
+  p.stall = take_stall();
   p.splits = prompt_splits(items, a.kv.kv_heads);
   p.po = static_cast<float4*>(workspace);
   p.pml = reinterpret_cast<float2*>(p.po + (size_t)items * a.kv.kv_heads * p.splits * kRows * (kHeadDim / 4));
@@ -324,6 +332,7 @@ static void launch_shared(const PAttnArgs& a, void* workspace, cudaStream_t s) {
   PPromptArgs p{};
   p.a = a;
   p.a.kv.batch = a.groups;
+  p.stall = take_stall();
   p.cta_rows = kSharedRows;
   const int items = shared_items(B, a.groups, G);
   p.splits = prompt_splits(items, kvh);
@@ -465,6 +474,7 @@ int qd_paged_attn_decode_q8(const qd_paged_q8* kv, const void* q, int dtype, int
     Q8Args args{};
     args.a = a;
     args.scale = {kv->k_scale, kv->v_scale};
+    args.stall = take_stall();
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int group = q_heads / kv->kv_heads;
     if (group <= 2) launch_decode_q8<Q8Whole>(args, workspace, s);

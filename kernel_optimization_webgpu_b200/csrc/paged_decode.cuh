@@ -554,17 +554,17 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
   if (TAIL) pdl_wait();
 }
 
-// per_sub: heads of a query group (at most 8). Joins the parts of each (sequence, query group) that several CTAs hold. Grid: batch * nh. Warp w takes head w / per of the group
+// per_sub: heads of a query group (at most 8). early: what follows may start before this has ended. Joins the parts of each (sequence, query group) that several CTAs hold. Grid: batch * nh. Warp w takes head w / per of the group
 // and every per-th part (per = 8 / heads, a power of two): each lane's loads of up to eight
 // parts are in flight together (with one warp per head, 37 parts took 6 us).
 __global__ void __launch_bounds__(256) k_paged_decode_join(const __grid_constant__ PAttnArgs a, void* workspace,
-                                                           int grid, int per_sub) {
+                                                           int grid, int per_sub, bool early) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int G = a.q_heads / a.kv.kv_heads, subs = (G + per_sub - 1) / per_sub, nh = a.kv.kv_heads * subs;
   const int b = blockIdx.x / nh, h = blockIdx.x % nh, heads = min(per_sub, G - (h % subs) * per_sub);
   const PDecodeWs ws = pd_ws(workspace);
   pdl_wait();
-  pdl_trigger();
+  if (early) pdl_trigger();
   const int f0 = ws.first[b], tiles = ws.first[b + 1] - f0;
   const long long U = (long long)ws.first[a.kv.batch] * nh;
   const int ctas = (int)min((long long)grid, U);

@@ -159,6 +159,7 @@ struct Q8Args {
   CUtensorMap tk, tv;  // boxes of 16 rows
   PAttnArgs a;
   PagedScales scale;
+  int stall;  // test hook (qd_paged_inject_stall): block 0's first warp withholds its first copies
 };
 
 __device__ __forceinline__ float log2_fast(float x) {
@@ -628,7 +629,7 @@ __global__ void __launch_bounds__(kPdThreads, Heads::kCtas) k_paged_decode_q8(co
                    "r"((halves == 3u ? 2 : 1) * (2 * 16 * 128 + 2 * 16 * 4))
                    : "memory");
     __syncwarp();
-    if ((lane & 15) == 0 && page >= 0) {
+    if ((lane & 15) == 0 && page >= 0 && !(qa.stall && issued == 0 && warp == 0 && blockIdx.x == 0)) {
       const int p0 = pre.v.tile(pre.t) * kQ8Tile + kQ8Rows * warp + lane;
       const int row = ((page * a.kv.kv_heads + pre.g) << a.kv.page_shift) + (p0 & ((1 << a.kv.page_shift) - 1));
       unsigned char* d = ring + in_slot * kQ8Slot + lane * 128;

@@ -21,6 +21,7 @@
 
 #include "../../include/qdecode.h"
 #include "internal.cuh"
+#include "overlap.hpp"
 #include "rows.cuh"
 
 namespace qd {
@@ -462,6 +463,13 @@ extern "C" int qd_score_rows(const void* logits, int dtype, int rows, uint32_t v
     if (rows == 0) return QD_OK;
     if (!logits || !tokens || !logprobs || (top && (!top_ids || !top_logprobs)))
       throw QdError{QD_E_INVALID, "qd_score_rows: NULL argument"};
+    const int64_t size = dtype == QD_KV_F32 ? 4 : 2, n = rows;
+    const Rows in{logits, n, (int64_t)vocab * size, row_stride * size}, given{tokens, 1, n * 4, n * 4};
+    for (const Rows& out : {Rows{logprobs, 1, n * 4, n * 4}, Rows{entropy, entropy ? 1 : 0, n * 4, n * 4},
+                            Rows{top_ids, top ? 1 : 0, n * top * 4, n * top * 4},
+                            Rows{top_logprobs, top ? 1 : 0, n * top * 4, n * top * 4}})
+      if (!apart(out, in) || !apart(out, given))
+        throw QdError{QD_E_INVALID, "qd_score_rows: an output overlaps logits or tokens"};
     ScoreArgs a{logits, (int)vocab, 0, row_stride, tokens, top, logprobs, entropy, top_ids, top_logprobs};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == QD_KV_F32) launch_score_rows<float>(a, rows, s);

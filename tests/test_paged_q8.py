@@ -294,6 +294,27 @@ def test_strides_workspace_stream_and_replay():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("heads", [(4, 2), (8, 2), (16, 2)], ids=lambda h: f"{h[0]}q{h[1]}kv")
+def test_copies_that_do_not_come_end_in_nan_and_a_status(heads):
+    """Block 0's first warp withholds its first copies: its waits end after a second."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    cache = make_q8(torch, [2000, 700, 40], 64, heads[1])
+    q = torch.randn(3, heads[0], D, device="cuda")
+    want = R.paged_attn_decode_q8(q, *cache)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    _lib.load().qd_paged_inject_stall()
+    y = R.paged_attn_decode_q8(q, *cache, status=status)
+    gone = y.isnan().any(-1)
+    assert int(status) == _lib.QD_PAGED_TIMEOUT and torch.equal(gone, y.isnan().all(-1))
+    # block 0: units of the first sequence's first KV head
+    assert bool(gone[0, :heads[0] // heads[1]].all()) and int(gone.sum()) < gone.numel()
+    assert torch.equal(y[~gone], want[~gone])
+    status.zero_()
+    assert torch.equal(R.paged_attn_decode_q8(q, *cache, status=status), want) and int(status) == 0
+
+
+@pytest.mark.gpu
 def test_bad_pages_and_lengths_are_left_out_and_flagged():
     torch = _cuda()
     from kernel_optimization_webgpu_b200 import runtime as R

@@ -194,6 +194,28 @@ def test_bad_pages_and_lengths_are_left_out_and_flagged():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("io,cache", [("f32", "f16"), ("f16", "f16"), ("f32", "bf16")])
+@pytest.mark.parametrize("groups", [2, 60])
+def test_a_block_that_gives_up_leaves_nan_and_a_status(io, cache, groups):
+    """Block 0 (the last rows of the last group, the first KV head) withholds its first key tile. 60 groups: blocks take
+    the work of others."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    k, v, table, n, starts, shared, _ = make_shared(torch, [3] * groups, [900] * groups, [9] * (3 * groups), 64, 4, cache)
+    q = torch.randn(3 * groups, 8, D, device="cuda").to(_types(torch)[io])
+    want = R.paged_attn_decode_shared(q, k, v, table, n, starts, shared)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    _lib.load().qd_paged_inject_stall()
+    y = R.paged_attn_decode_shared(q, k, v, table, n, starts, shared, status=status)
+    gone = y.isnan().any(-1)
+    assert int(status) == _lib.QD_PAGED_TIMEOUT and torch.equal(gone, y.isnan().all(-1))
+    assert bool(gone[-3:, :2].all()) and int(gone.sum()) == 6
+    assert torch.equal(y[~gone], want[~gone])
+    status.zero_()
+    assert torch.equal(R.paged_attn_decode_shared(q, k, v, table, n, starts, shared, status=status), want) and int(status) == 0
+
+
+@pytest.mark.gpu
 def test_replays_follow_lengths_and_groups():
     """Two graphs with workspaces of their own; the groups and lengths change between replays."""
     torch = _cuda()

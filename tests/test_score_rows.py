@@ -31,6 +31,22 @@ def test_arguments_are_refused():
     assert call(rows=0, logits=None, tokens=None, logp=None) == _lib.QD_OK
 
 
+def test_outputs_over_their_inputs_are_refused():
+    """Two rows of ten f32 logits, 48 bytes apart, at 1 << 40; tokens at 1 << 41. (What is not refused is ended by vocab.)"""
+    L = _lib.load()
+    at, far = 1 << 40, 1 << 42
+    ok = dict(logits=at, tokens=1 << 41, logp=far, ent=far + 64, ids=far + 128, tops=far + 192)
+
+    def call(vocab=10, **kw):
+        c = {**ok, **kw}
+        rc = L.qd_score_rows(c["logits"], 1, 2, vocab, 12, c["tokens"], 2, c["logp"], c["ent"], c["ids"], c["tops"], None)
+        return rc, L.qd_last_error(None)
+
+    for bad in (dict(logp=at), dict(ent=at + 84), dict(ids=at - 12), dict(tops=at + 60), dict(logp=1 << 41), dict(ids=(1 << 41) - 8)):
+        rc, said = call(**bad)
+        assert rc == _lib.QD_E_INVALID and b"overlaps" in said, bad
+
+
 def test_python_wrapper_refuses():
     torch = pytest.importorskip("torch")
     from kernel_optimization_webgpu_b200 import runtime as R
