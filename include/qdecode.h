@@ -484,7 +484,7 @@ int qd_paged_attn_decode_shared(const qd_paged_kv* kv, const void* q, int dtype,
 typedef struct qd_paged_q8 {
   int8_t* k;                    /* [num_pages][kv_heads][page_size][head_dim], 16-byte aligned */
   int8_t* v;
-  float* k_scale;               /* [num_pages][kv_heads][page_size], 16-byte aligned, not negative */
+  float* k_scale;               /* [num_pages][kv_heads][page_size], 16-byte aligned */
   float* v_scale;
   int num_pages;
   int page_size;                /* a power of two, 16..256 */
@@ -518,7 +518,7 @@ int qd_paged_read_q8(const qd_paged_q8* kv, const int32_t* first, const qd_paged
 /* qd_paged_attn_decode over such a cache; dtype (of q and y) is QD_KV_F32, QD_KV_F16 or
  * QD_KV_BF16. The products keep f32 accuracy for every dtype: the integers are exact operands, q is
  * held to 2^-22 of each element or 2^-30 of its head's largest, a weight times its V row's scale to
- * 2^-22 of itself or 2^-30 of the largest such product. Scales must not be negative. A device-side
+ * 2^-22 of itself or 2^-30 of the largest such product. V scales below 2^-126 count as 0. A device-side
  * wait that expires makes rows NaN and sets QD_PAGED_TIMEOUT. The workspace is
  * qd_paged_attn_decode_workspace_bytes(batch, q_heads). */
 int qd_paged_attn_decode_q8(const qd_paged_q8* kv, const void* q, int dtype, int64_t q_stride, int q_heads, int window,

@@ -144,8 +144,8 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_read_q8(const __grid_const
 //  - The contraction's index may have any order that both operands share: thread t of a quad takes dims
 //    32 t .. + 31 of a K row (two 16-byte loads) and 16 consecutive dims of some positions of V.
 //  - A V row's scale may have any size beside its weight (the first token's V is small in many models, and its weight
-//    large), so the weights p_j vs_j have a running maximum of their own, of s_j + log2 vs_j, next to that of s_j, by
-//    which the weights' sum goes.
+//    large), so the weights p_j vs_j have a running maximum of their own, of s_j and the scale's exponent, next to that
+//    of s_j, by which the weights' sum goes.
 constexpr int kQ8Tile = 128, kQ8Stages = 2;
 constexpr int kQ8Rows = 32;                 // positions of a warp
 constexpr int kQ8Slot = 2 * kQ8Rows * 128;  // K and V
@@ -162,10 +162,13 @@ struct Q8Args {
   int stall;  // test hook (qd_paged_inject_stall): block 0's first warp withholds its first copies
 };
 
-__device__ __forceinline__ float log2_fast(float x) {
-  float y;
-  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+// A scale as f * 2^k, 1 <= |f| < 2 (0 and below 2^-126: k is -inf; not finite: f is the scale itself). A weight times it is
+// exp2(s + k - reference) f: the sum with k loses less than one with a logarithm does (f32 queries on 1 x 31
+// positions: 9e-7 off with a logarithm, 2 - 4e-7 so; 64 x 2048: the same time).
+__device__ __forceinline__ void q8_scale(float s, float& k, float& f) {
+  const unsigned u = __float_as_uint(s), e = (u >> 23) & 255u;
+  k = e == 0u ? -INFINITY : __uint_as_float(0x4b000000u | e) - 8388735.0f;  // (2^23 + e less 2^23 + 127)
+  f = e == 255u ? s : __uint_as_float((u & 0x807fffffu) | 0x3f800000u);
 }
 // (not volatile: the loads and products of a unit may be interleaved as their latencies ask)
 __device__ __forceinline__ void q8_mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
@@ -194,8 +197,7 @@ __device__ __forceinline__ uint4 q8_lds(const unsigned char* at) { return *reint
 // Positions are taken in an order for which the rows that a quarter warp reads from shared memory lie on distinct banks.
 struct Q8Whole {
   static constexpr int kHeads = 2, kCtas = 3;  // heads, CTAs per SM
-  static constexpr float kLag = 1.0f;          // log2 that a weights' maximum may fall behind
-  static constexpr float kShift = 29.0f;       // weights are kept times 2^29 (with the lag at most 2^30), off by 2^-30 of the largest
+  static constexpr float kShift = 29.0f;       // weights are kept times 2^29 (below 2^30), off by 2^-30 of the largest
   static constexpr int kFlush = 2048;          // units after which the 32-bit sums are moved (each adds below 2^19)
   unsigned q[4][2];
   int acc[8][4];
@@ -276,7 +278,7 @@ struct Q8Whole {
   __device__ __forceinline__ void unit(const unsigned char* kb, const unsigned char* vb, const float* ks, const float* vs,
                                        const Q8Seen& seen, int g8, int t4) {
     const int r0 = order(g8);
-    float p[4], u[4];  // of positions r0 + 8 j: scores, and with V's scale
+    float p[4], u[4], vf[4];  // of positions r0 + 8 j: scores, and with V's scale but for its factor vf
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       int s[4] = {0, 0, 0, 0};
@@ -291,17 +293,19 @@ struct Q8Whole {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int j = 2 * h + e;
-        const float sc = ks[r0 + 8 * j], lv = log2_fast(vs[r0 + 8 * j]);
+        const float sc = ks[r0 + 8 * j];
+        float k;
+        q8_scale(vs[r0 + 8 * j], k, vf[j]);
         // two bytes of q here (below 2^30 together), two in the neighbour
         const float x = (float)(s[2 * e] + 256 * s[2 * e + 1]) * (t4 & 1 ? 65536.0f : 1.0f);
         p[j] = (x + __shfl_xor_sync(0xffffffffu, x, 1)) * (factor * sc);
-        u[j] = p[j] + lv;
+        u[j] = p[j] + k;
       }
     }
     if (!seen.inside) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (!seen.at(r0 + 8 * j)) p[j] = u[j] = -INFINITY;
+        if (!seen.at(r0 + 8 * j)) p[j] = u[j] = -INFINITY, vf[j] = 0.0f;  // (what lies there may be no scale)
     }
     const bool full = ++since == kFlush;
     if (full) since = 0;
@@ -313,8 +317,8 @@ struct Q8Whole {
       mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
       ut = fmaxf(ut, __shfl_xor_sync(0xffffffffu, ut, x));
     }
-    if (__any_sync(0xffffffffu, full || mt > m + kPdLag || ut > mo + kLag)) {  // some head's maximum moved
-      const float mn = mt > m + kPdLag ? mt : m, un = ut > mo + kLag ? ut : mo;
+    if (__any_sync(0xffffffffu, full || mt > m + kPdLag || ut > mo)) {  // some head's maximum moved
+      const float mn = mt > m + kPdLag ? mt : m, un = ut > mo ? ut : mo;
       l *= m == -INFINITY ? 0.0f : exp2_fast(m - mn);
       flush(mo == -INFINITY ? 0.0f : exp2_fast(mo - un));
       m = mn;
@@ -324,7 +328,7 @@ struct Q8Whole {
     unsigned d[4], r[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float x = exp2_fast(u[j] - uref);
+      const float x = exp2_fast(u[j] - uref) * vf[j];
       l = fmaf(x, 0.0f, l) + exp2_fast(p[j] - ref);  // (a NaN weight is no integer)
       d[j] = digits(__float2int_rn(x));
     }
@@ -389,7 +393,8 @@ struct Q8Whole {
 template <int SETS>
 struct Q8Half {
   static constexpr int kHeads = 4 * SETS, kCtas = SETS == 1 ? 3 : 2;
-  static constexpr float kShift = kPdShift;
+  // a maximum may fall behind by 2^7: weights, and their scales' factors below 2, then stay below 2^15
+  static constexpr float kLag = 7.0f, kShift = kPdShift;
   unsigned q[SETS][8][2];
   float o[SETS][8][4], m[SETS], mo[SETS], l[SETS], factor[SETS];
 
@@ -428,7 +433,7 @@ struct Q8Half {
   }
   __device__ __forceinline__ void unit(const unsigned char* kb, const unsigned char* vb, const float* ks, const float* vs,
                                        const Q8Seen& seen, int g8, int t4) {
-    float p[SETS][4], u[SETS][4];  // of positions 8 j + g8: scores, and with V's scale
+    float p[SETS][4], u[SETS][4], vf[4];  // of positions 8 j + g8: scores, and with V's scale
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float s[SETS][2][4];
@@ -453,20 +458,24 @@ struct Q8Half {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int j = 2 * h + e;
-        const float sc = ks[8 * j + g8], lv = log2_fast(vs[8 * j + g8]);
+        const float sc = ks[8 * j + g8];
+        float kv;
+        q8_scale(vs[8 * j + g8], kv, vf[j]);
 #pragma unroll
         for (int n = 0; n < SETS; ++n) {
           p[n][j] = ((s[n][0][2 * e] + s[n][1][2 * e]) + (s[n][0][2 * e + 1] + s[n][1][2 * e + 1])) * (factor[n] * sc);
-          u[n][j] = p[n][j] + lv;
+          u[n][j] = p[n][j] + kv;
         }
       }
     }
     if (!seen.inside) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (!seen.at(8 * j + g8))
+        if (!seen.at(8 * j + g8)) {
+          vf[j] = 0.0f;  // (what lies there may be no scale)
 #pragma unroll
           for (int n = 0; n < SETS; ++n) p[n][j] = u[n][j] = -INFINITY;
+        }
     }
 #pragma unroll
     for (int n = 0; n < SETS; ++n) {
@@ -477,8 +486,8 @@ struct Q8Half {
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
         ut = fmaxf(ut, __shfl_xor_sync(0xffffffffu, ut, x));
       }
-      if (__any_sync(0xffffffffu, mt > m[n] + kPdLag || ut > mo[n] + kPdLag)) {  // some head's maximum moved: rescale
-        const float mn = mt > m[n] + kPdLag ? mt : m[n], un = ut > mo[n] + kPdLag ? ut : mo[n];
+      if (__any_sync(0xffffffffu, mt > m[n] + kPdLag || ut > mo[n] + kLag)) {  // some head's maximum moved: rescale
+        const float mn = mt > m[n] + kPdLag ? mt : m[n], un = ut > mo[n] + kLag ? ut : mo[n];
         l[n] *= m[n] == -INFINITY ? 0.0f : exp2_fast(m[n] - mn);
         const float f = mo[n] == -INFINITY ? 0.0f : exp2_fast(mo[n] - un);
         m[n] = mn;
@@ -492,7 +501,7 @@ struct Q8Half {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         l[n] += exp2_fast(p[n][j] - ref);
-        u[n][j] = exp2_fast(u[n][j] - uref);
+        u[n][j] = exp2_fast(u[n][j] - uref) * vf[j];
       }
     }
 #pragma unroll

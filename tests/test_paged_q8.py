@@ -4,8 +4,10 @@ host (no GPU), and the CUDA path against plain 64-bit evaluations.
 Tolerances count roundings. Of the attention, relative to A = sum of |weight| |value| of an output:
  - scores: as in test_paged.py (f32 sums and q as two f16: S (2^-19 + 2^-21)), and the product with the query's factor
    and the row's scale: S 2^-22;
- - weights: twice that, 2^-20 for the exponential, 2^-21 for two f16 parts; log2 of V's scale, |lg| <= L, is off by
-   2^-22 L and the sum with the score by 2^-24 (1.45 S + L);
+ - weights: twice that, 2^-20 for the exponential, 2^-21 for two f16 parts; V's scale goes in by its exponent, at
+   most L + 1 in size for |log2 scale| <= L, whose sum with the score is off by 2^-24 (1.45 S + L + 1), and by its
+   factor, off by 2^-24: together less than the 2^-22 L + 2^-24 (1.45 S + L) that a logarithm would cost, or, for
+   L < 1, than what 2^-20 leaves over;
  - sums over n keys in f32: n / 16 * 2^-23 + 2^-19; the output's own rounding.
 Of a row written in 8 bits: n is x / scale rounded, so |x - n scale| <= scale / 2 but for f32 roundings: of x itself
 (its tolerance), of the scale and its inverse (2^-23 of 127 steps)."""
