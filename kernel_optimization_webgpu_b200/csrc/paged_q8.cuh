@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_read_q8(const __grid_const
 //      more heads (Q8Half): m16n8k16 of f16, the integers made f16 (byte permutes and a subtraction per pair), q and the
 //      weights as two f16. Its columns hold twice the heads, and its sums take a third of the registers.
 //    64 sequences of 2048 positions, 8 KV heads: 16 query heads 55 us with Q8Whole and 58 with Q8Half; 32 query heads 71 and
-//    63 (with four heads in Q8Whole); 4 KV heads and 32 query heads 50 with Q8Half, 75 with Q8Whole twice.
+//    66 (with four heads in Q8Whole); 4 KV heads and 32 query heads 52 with Q8Half, 75 with Q8Whole twice.
 //  - The contraction's index may have any order that both operands share: thread t of a quad takes dims
 //    32 t .. + 31 of a K row (two 16-byte loads) and 16 consecutive dims of some positions of V.
 //  - A V row's scale may have any size beside its weight (the first token's V is small in many models, and its weight
@@ -164,7 +164,7 @@ struct Q8Args {
 
 // A scale as f * 2^k, 1 <= |f| < 2 (0 and below 2^-126: k is -inf; not finite: f is the scale itself). A weight times it is
 // exp2(s + k - reference) f: the sum with k loses less than one with a logarithm does (f32 queries on 1 x 31
-// positions: 9e-7 off with a logarithm, 2 - 4e-7 so; 64 x 2048: the same time).
+// positions: 9e-7 off with a logarithm, 2 - 4e-7 so; 64 x 2048: 54.2 -> 55.3 us, 64 x 8192: 182 -> 177).
 __device__ __forceinline__ void q8_scale(float s, float& k, float& f) {
   const unsigned u = __float_as_uint(s), e = (u >> 23) & 255u;
   k = e == 0u ? -INFINITY : __uint_as_float(0x4b000000u | e) - 8388735.0f;  // (2^23 + e less 2^23 + 127)
