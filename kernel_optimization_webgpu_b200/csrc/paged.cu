@@ -339,19 +339,16 @@ static void launch_shared(const PAttnArgs& a, void* workspace, cudaStream_t s) {
   p.po = reinterpret_cast<float4*>(base + w.po);
   p.pml = reinterpret_cast<float2*>(base + w.pml);
   p.rows = reinterpret_cast<int2*>(base + w.rows);
-  const long long grid = (long long)items * kvh * p.splits;
+  const long long grid = (long long)items * kvh * p.splits;  // (at least one)
   if (grid * 32 > 0x7fffffffLL) throw QdError{QD_E_RANGE, "qd_paged_attn_decode_shared: too many rows"};
   pool_maps<T>(p, a.q, "qd_paged_attn_decode_shared: a pool beyond 2^31 rows");
-  if (grid > 0) {
-    static unsigned long long smem_set[2] = {};
-    const bool claim = grid > current_sms();
-    auto kernel = claim ? k_paged_prompt<T, PARTS, true, true> : k_paged_prompt<T, PARTS, false, true>;
-    allow_smem(kernel, pp_smem<PARTS>(), smem_set[claim]);
-    launch_ex(kernel, dim3((unsigned)grid), dim3(kPpThreads), (size_t)pp_smem<PARTS>(), s, p);
-  }
+  static unsigned long long prefix_set[2] = {}, tail_set = 0;
+  const bool claim = grid > current_sms();
+  auto prefix = claim ? k_paged_prompt<T, PARTS, true, true> : k_paged_prompt<T, PARTS, false, true>;
+  allow_smem(prefix, pp_smem<PARTS>(), prefix_set[claim]);
+  launch_ex(prefix, dim3((unsigned)grid), dim3(kPpThreads), (size_t)pp_smem<PARTS>(), s, p);
   PSharedArgs j{};
   j.a = a;
-  j.a.beside = grid > 0;
   j.a.tail_o = reinterpret_cast<float*>(base + w.tail_o);
   j.a.tail_ml = reinterpret_cast<float2*>(base + w.tail_ml);
   j.po = p.po;
@@ -362,8 +359,7 @@ static void launch_shared(const PAttnArgs& a, void* workspace, cudaStream_t s) {
   j.all_rows = items * kSharedRows;
   j.decode_ws = base + w.decode;
   j.ctas = (int)std::max(1LL, std::min<long long>(most, std::min(2 * current_sms(), kPdMaxCtas)));
-  static unsigned long long smem_set = 0;
-  allow_smem(k_paged_decode<T, PARTS == 3, true>, pd_smem(4096), smem_set);
+  allow_smem(k_paged_decode<T, PARTS == 3, true>, pd_smem(4096), tail_set);
   launch_ex(k_paged_decode<T, PARTS == 3, true>, dim3(j.ctas), dim3(kPdThreads), (size_t)pd_smem(B), s, j.a,
             (void*)j.decode_ws);
   launch_ex(k_paged_shared_join, dim3((B * G + 7) / 8, kvh), dim3(kPsThreads), 0, s, j);

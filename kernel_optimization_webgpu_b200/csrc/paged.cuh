@@ -353,7 +353,6 @@ struct PAttnArgs {
   long long y_stride;
   // Shared prefixes: q_starts holds the groups' first sequences (groups + 1 entries).
   int groups;
-  bool beside;             // (k_paged_decode) the launch before works on the shared positions
   const int* shared_lens;  // [batch]
   float* tail_o;           // [batch][q_heads][128]: unnormalised sums of the positions behind them,
   float2* tail_ml;         // [batch][q_heads]: with their maxima and weights

@@ -265,7 +265,7 @@ __host__ __device__ constexpr int pd_smem(int batch) { return 4 * kPdStages * kP
 
 // TAIL: the positions behind those that a sequence shares (paged_shared.cuh). All sums go to the workspace, a
 // (sequence, head) that one CTA holds whole to a place of its own. The launch before it, over the shared positions, may
-// still run (a.beside: it wrote nothing that is read here, and it began after all before it had ended), so it is
+// still run (it wrote nothing that is read here, and it began after all before it had ended), so it is
 // waited for at the end only; a fence clears L1 of what that launch may have found there.
 template <typename T, bool THREE, bool TAIL = false>
 __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_constant__ PAttnArgs a, void* workspace) {
@@ -276,8 +276,8 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
   __shared__ float2 sml[4][8];  // maximum and sum of each warp and head
   const int G = a.q_heads / a.kv.kv_heads, subs = (G + 7) >> 3, nh = a.kv.kv_heads * subs, B = a.kv.batch;
   const PDecodeWs ws = pd_ws(workspace);
-  if (!TAIL || !a.beside) pdl_wait();
-  else __threadfence();
+  if (TAIL) __threadfence();
+  else pdl_wait();
   pdl_trigger();
   const int held = TAIL ? min(a.q_starts[a.groups], B) : B;  // sequences behind the last group are padding
 
@@ -554,7 +554,8 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
   if (TAIL) pdl_wait();
 }
 
-// per_sub: heads of a query group (at most 8). early: what follows may start before this has ended. Joins the parts of each (sequence, query group) that several CTAs hold. Grid: batch * nh. Warp w takes head w / per of the group
+// per_sub: heads of a query group (at most 8). early: what follows may start before this has ended.
+// Joins the parts of each (sequence, query group) that several CTAs hold. Grid: batch * nh. Warp w takes head w / per of the group
 // and every per-th part (per = 8 / heads, a power of two): each lane's loads of up to eight
 // parts are in flight together (with one warp per head, 37 parts took 6 us).
 __global__ void __launch_bounds__(256) k_paged_decode_join(const __grid_constant__ PAttnArgs a, void* workspace,
