@@ -363,6 +363,14 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
   // (with three parts and one set, a tile's 24 products into O cost 1.7e-6 of the result with moves every four tiles, 1.0e-6 so)
   constexpr int kFlush = SHARED && PARTS == 3 ? 2 : kPpFlush;
   constexpr int kQTile = PARTS * kPpTileBytes;  // the parts of 128 rows
+  // Parts of a weight: those of q, but two for 16-bit queries over shared positions, as k_paged_decode takes them for
+  // the positions behind and for all of a sequence alone. With one, f16 results were 2.8e-4 off and bf16 results
+  // 2.0e-3, where their own rounding is 2.1e-4 and 1.7e-3; 64 of 16384 took 49 us, 7 groups of bf16 56 (51 and 59 with two).
+  constexpr int kParts = SHARED && PARTS == 1 ? 2 : PARTS;
+  // O moves to the workspace every kFlush tiles. Not for 16-bit results: what the products drop on the way, 3e-5 of
+  // a sum of 8192 values of one sign that one CTA takes, is a sixth of their rounding (moves every 4 tiles: 3e-6, 65
+  // us for the 7 groups; every 16: 1.4e-5, 60 us).
+  constexpr bool kMoves = PARTS > 1;
   // TMEM columns: S_t | O_t with P over S, or S | P (three parts) | O
   constexpr unsigned kColP = kTiles == 2 ? 0 : 128, kColO = kTiles == 2 ? 256 : 384;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -656,13 +664,13 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
-            for (int part = 0; part < PARTS; ++part)
+            for (int part = 0; part < kParts; ++part)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int ks = 2 * half + (i & 1) + 4 * (i >> 1);  // keys 0-31 and 64-95, then the others
-                const unsigned po = (PARTS - 1 - part) * 64 + ks * 8;
+                const unsigned po = (kParts - 1 - part) * 64 + ks * 8;
                 if (half == 0 && part == 0 && i == 0)
-                  pp_mma_ts(od, pd + po, v0, id_o, PARTS > 1 ? n % kFlush != 0 : n > 0, leader);
+                  pp_mma_ts(od, pd + po, v0, id_o, kMoves ? n % kFlush != 0 : n > 0, leader);
                 else
                   pp_mma_ts(od, pd + po, v0 + ks * (2048 >> 4), id_o, true, leader);
               }
@@ -924,7 +932,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
               }
             }
           }
-          if (PARTS > 1 && j > 0 && j % kFlush == 0) {
+          if (kMoves && j > 0 && j % kFlush == 0) {
             ok = ok && __all_sync(0xffffffffu, pp_wait(&o_done[t], (unsigned)((j - 1) ^ turn) & 1u, &failed));
             tc_fence_after();
             const float f = moved == -INFINITY ? 0.0f : exp2_fast(moved - m);
@@ -951,20 +959,20 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
           float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {  // 32 keys: 16 packed columns
-            unsigned w[PARTS][16];
+            unsigned w[kParts][16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const float s0 = __uint_as_float(sr[32 * h + 2 * i]), s1 = __uint_as_float(sr[32 * h + 2 * i + 1]);
               float2 e = __ffma2_rn(make_float2(s0, s1), make_float2(c, c), make_float2(ref, ref));
               e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
               sum = __fadd2_rn(sum, e);
-              unsigned u[PARTS];
-              split_parts<T, PARTS>(e.x, e.y, u);
+              unsigned u[kParts];
+              split_parts<T, kParts>(e.x, e.y, u);
 #pragma unroll
-              for (int part = 0; part < PARTS; ++part) w[part][i] = u[part];
+              for (int part = 0; part < kParts; ++part) w[part][i] = u[part];
             }
 #pragma unroll
-            for (int part = 0; part < PARTS; ++part) tmem_st16(tp + 64 * part + 16 * h, w[part]);
+            for (int part = 0; part < kParts; ++part) tmem_st16(tp + 64 * part + 16 * h, w[part]);
             if (h == 0) {  // the products of the first half of both threads' keys may start
               tmem_wait_st();
               tc_fence_before();
@@ -996,7 +1004,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
           for (int h = 0; h < 2; ++h) {
             float o[32];
             tmem_ld32(to + 32 * h, o);
-            if (PARTS > 1 && mine_nk > kFlush) {
+            if (kMoves && mine_nk > kFlush) {
               const float fm = moved == -INFINITY ? 0.0f : exp2_fast(moved - m);
               const float4* src = mine + (16 * hf + 8 * h) * kRows;
 #pragma unroll

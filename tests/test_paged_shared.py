@@ -6,7 +6,7 @@ import math
 import pytest
 
 from kernel_optimization_webgpu_b200 import _lib
-from test_paged import BAD_CACHES, BASE, D, HEADS, _cuda, _kv, _types, close, make_cache, plain_attention
+from test_paged import BAD_CACHES, BASE, D, HALF_STEP, HEADS, _cuda, _kv, _types, close, make_cache, plain_attention
 
 
 def test_arguments_are_refused():
@@ -287,3 +287,24 @@ def test_answers_to_one_prompt_step_by_step():
         assert float((logp - exact.gather(1, ids.long()[:, None])[:, 0]).abs().max()) < 1e-5
         assert torch.equal(top[:, 0].long(), logits.argmax(-1))
     assert int(status) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes,prefix", [([3], [200]), ([40], [600]), ([2] * 40, [130 + 3 * i for i in range(40)])],
+                         ids=["one", "wide", "many"])
+@pytest.mark.parametrize("io", ["f16", "bf16"])
+def test_16_bit_queries_keep_both_parts_of_a_weight(sizes, prefix, io):
+    """Values of alternating sign under nearly equal weights: what rounding a weight to 16 bits (2^-11, 2^-8) would
+    leave does not cancel, the output and its own rounding do. The tolerance is that of two parts (f32 queries' terms),
+    and the output's half step."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    k, v, table, n, starts, shared, whole = make_shared(torch, sizes, prefix, [1 + b % 5 for b in range(sum(sizes))], 16, 2, io)
+    v[:, :, ::2] = v[:, :, ::2].abs()
+    v[:, :, 1::2] = -v[:, :, 1::2].abs()
+    q = (torch.randn(sum(sizes), 8, D, device="cuda") * 0.02).to(_types(torch)[io])
+    y = R.paged_attn_decode_shared(q, k, v, table, n, starts, shared)
+    want, tol = plain_attention(torch, q, k, v, whole, n, [1] * sum(sizes), 0, 0, D ** -0.5, "f32", io)
+    tol = tol + HALF_STEP[io] * want.abs() + (2.0 ** -25 if io == "f16" else 0.0) + 2.0 ** -20 * want.abs().amax(-1, keepdim=True)
+    close(torch, R.paged_attn_decode(q, k, v, whole, n), want, tol)
+    close(torch, y, want, tol)
