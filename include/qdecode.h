@@ -498,8 +498,8 @@ typedef struct qd_paged_q8 {
 } qd_paged_q8;
 
 /* qd_paged_append into such a cache: what it would write of a K or V row x (in f32) is written as
- * scale = max|x| / 127 and n = x / scale rounded to the nearest integer, -127..127 (to f32: a
- * border between two integers may lie 2^-15 of a step aside). A row with an element that is not
+ * scale = max|x| / 127 and n = 127 x / max|x| rounded to the nearest integer, halves to even, -127..127 (to
+ * f32: a border between two integers may lie 2^-16 of a step aside, a half is one). A row with an element that is not
  * finite gets a NaN scale, one whose largest magnitude is below 2^-100 a scale of 0 and zeros. Where the
  * block table makes two new rows share a position, what is left there may mix both. */
 int qd_paged_append_q8(const qd_paged_q8* kv, const void* qkv, int qkv_dtype, int64_t qkv_stride, int rows,

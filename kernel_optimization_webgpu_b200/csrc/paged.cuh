@@ -208,14 +208,19 @@ __global__ void __launch_bounds__(256, HEADS == 4 ? 5 : 6) k_paged_append(const 
   }
 }
 
-// The same into a cache of 8-bit integers n with a scale per row: scale = the largest magnitude / 127, n = x / scale
-// rounded, by an addition of 1.5 * 2^23 whose sum's low byte is n: each element is at most half a scale (1/254 of
-// the largest) off, but for roundings that move a border by 127 * 2^-22 of a scale. A row with an element that is not
+// The same into a cache of 8-bit integers n with a scale per row: scale = the largest magnitude / 127, n = 127 x / the largest
+// rounded, halves to even, by an addition of 1.5 * 2^23 whose sum's low byte is n. Halves are common (any element that
+// is half the largest), so the quotient q = x / scale gets one residual: q + (127 x - q max) / max is off by no more than its
+// own rounding, 2^-17 of a step, and a half comes out as one. (Without it about half of the halves of 16-bit rows went to
+// the other integer: read back in f16, V was 6.5e-4 off from bf16 rows and 3.7e-4 from f16 rows, both 2.0e-4 so; it takes 2.3
+// us of 16384 rows.) With f32 rows 127 x is the product and what it rounds off. All of it over 128, so that no product
+// leaves f32. A row with an element that is not
 // finite gets a NaN scale (all of it reads as NaN), one whose largest is below 2^-100 a scale of 0.
 //
 // Half a warp per head: lane h of it holds dims 4 h .. + 3 and 64 + 4 h .. + 3, which the rotation turns into
 // each other, and a sum or maximum takes four steps for two heads at once. (The other kernel's lanes, with the rows'
-// maxima and divisions added, were bound by instructions: 16384 rows of 16 + 8 + 8 heads, f32, 437 MB, 98 us; so 71 us = 6.1 TB/s.)
+// maxima and divisions added, were bound by instructions: 16384 rows of 16 + 8 + 8 heads, f32, 437 MB, 98 us; so 73 us = 6.0 TB/s.
+// Rows of f16 or bf16, 236 MB, take 73 us too: their bound is the instructions still.)
 // Sums run in that kernel's order: q comes out the same to the bit.
 template <typename T, int PAIRS>
 __global__ void __launch_bounds__(256, PAIRS == 2 ? 5 : 6) k_paged_append_q8(const __grid_constant__ AppendArgs a) {
@@ -319,12 +324,20 @@ __global__ void __launch_bounds__(256, PAIRS == 2 ? 5 : 6) k_paged_append_q8(con
                            max(__float_as_uint(v.z) & none, __float_as_uint(v.w) & none)));
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float scale = __uint_as_float(top) * (1.0f / 127.0f), magic = 12582912.0f;
-    const float up = __fdividef(1.0f, scale);
+    const float most = __uint_as_float(top), near = most * (1.0f / 127.0f);
+    const float scale = fmaf(fmaf(-near, 127.0f, most), 1.0f / 127.0f, near);
+    const float up = __fdividef(1.0f, scale), most7 = most * 0.0078125f, up7 = up * (128.0f / 127.0f);
+    auto both = [](float y) { return make_float2(y, y); };
+    auto whole = [&](float2 y) {
+      const float2 q = __fmul2_rn(y, both(up)), z = __fmul2_rn(y, both(0.9921875f));  // 127 / 128
+      float2 rest = __ffma2_rn(make_float2(-q.x, -q.y), both(most7), z);
+      if constexpr (sizeof(T) == 4) rest = __fadd2_rn(rest, __ffma2_rn(y, both(0.9921875f), make_float2(-z.x, -z.y)));
+      return __fadd2_rn(__ffma2_rn(rest, both(up7), q), both(12582912.0f));
+    };
     auto bytes = [&](float4 y) {
-      const unsigned d0 = __float_as_uint(fmaf(y.x, up, magic)), d1 = __float_as_uint(fmaf(y.y, up, magic));
-      const unsigned d2 = __float_as_uint(fmaf(y.z, up, magic)), d3 = __float_as_uint(fmaf(y.w, up, magic));
-      return __byte_perm(__byte_perm(d0, d1, 0x0040), __byte_perm(d2, d3, 0x0040), 0x5410);
+      const float2 d = whole(make_float2(y.x, y.y)), e = whole(make_float2(y.z, y.w));
+      return __byte_perm(__byte_perm(__float_as_uint(d.x), __float_as_uint(d.y), 0x0040),
+                         __byte_perm(__float_as_uint(e.x), __float_as_uint(e.y), 0x0040), 0x5410);
     };
     const int h = h0 + 2 * i + half;
     if (h < k0 || h >= heads) continue;

@@ -562,3 +562,38 @@ def test_offsets_beyond_32_bits():
     R.paged_read_q8(k, v, ks, vs, table, n, *outs[0], to)
     R.paged_read_q8(*small, *outs[1], to)
     assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("io", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("size", [1.0, 1e-3, 200.0])
+def test_integers_are_the_quotients_rounded(io, size):
+    """n = 127 x / max|x| rounded, halves to even: every integer of rows in which many elements are halves (of the largest,
+    and between any two integers of rows whose largest is 127 times a power of two). In 16 bits no quotient comes nearer
+    to a half than 2^-19 of itself without being one, and a quotient is off by 2^-24 of itself; in f32 only the
+    halves, and what lies 2^-16 of a step from one, are compared."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    rows, kvh = 300, 4
+    T = _types(torch)[io]
+    g = torch.Generator(device="cuda").manual_seed(11)
+    x = (torch.randn(rows, 2 * kvh, D, generator=g, device="cuda") * size).to(T)
+    top = x.abs().amax(-1, keepdim=True)
+    x[:, :, 5:40:3] = top * 0.5 * torch.randn(rows, 2 * kvh, 12, generator=g, device="cuda").sign().to(T)
+    odd = 2 * torch.randint(-127, 127, (rows // 2, 2 * kvh, D), generator=g, device="cuda") + 1
+    x[::2] = (odd * 0.5 if size == 1.0 else odd * 0.0625).to(T)   # at most 126.5 or an eighth of it, exact in 8 bits and more
+    x[::2, :, 9] = 127.0 if size == 1.0 else -127.0 / 8
+    k8, v8, ks, vs, table, n = make_q8(torch, [rows], 64, kvh, fill=False)
+    starts = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    R.paged_append_q8(x.flatten(1), k8, v8, ks, vs, table, n, None, None, 0, q_starts=starts)
+    at = torch.arange(rows, device="cuda")
+    pg = table[0].long()[at // 64]
+    ints = torch.cat([k8[pg, :, at % 64], v8[pg, :, at % 64]], 1)
+    scales = torch.cat([ks[pg, :, at % 64], vs[pg, :, at % 64]], 1)
+    most = x.double().abs().amax(-1)
+    assert bool(((scales.double() * 127 - most).abs() <= 2.0 ** -24 * 1.001 * most).all())   # half a step
+    q = x.double() * 127 / most[..., None]
+    off = ((q - q.floor()) - 0.5).abs()
+    assert int((off == 0).sum()) > rows * kvh * 32
+    sure = (off == 0) | (off > 2.0 ** -16) if io == "f32" else torch.ones_like(off, dtype=torch.bool)
+    assert torch.equal(ints[sure].double(), q.round()[sure])
