@@ -293,8 +293,14 @@ int qd_batch_inject_stall(qd_batch* b);
 /*  - qd_paged_inject_stall: the calling thread's next qd_paged_attn_prompt, qd_paged_attn_decode_shared or
  *    qd_paged_attn_decode_q8 withholds the first key tile of its block 0, whose waits end after 1 s:
  *    QD_PAGED_TIMEOUT is set, the rows that the block held are NaN and all others are right. (In a
- *    captured call, at every replay.) */
+ *    captured call, at every replay.)
+ *  - qd_paged_inject_stall_at: the same at a place: QD_PAGED_STALL_FIRST as above;
+ *    QD_PAGED_STALL_LATE (qd_paged_attn_decode_shared): nothing is withheld, but half of the threads of every
+ *    block begin each of its row tiles 40 us after the others, which must not change a result. */
+#define QD_PAGED_STALL_FIRST 1
+#define QD_PAGED_STALL_LATE 2
 void qd_paged_inject_stall(void);
+int qd_paged_inject_stall_at(int where);
 
 /* runCustomQwenGreedyPrompt over `batch` prompts of n_prompt ids each: prefill,
  * then max_new_tokens greedy tokens per prompt. ids [batch][n_prompt], out_ids

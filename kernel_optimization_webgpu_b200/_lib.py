@@ -24,6 +24,8 @@ QD_KV_BF16 = 2
 QD_PAGED_BAD_PAGE = 1
 QD_PAGED_BAD_LENGTH = 2
 QD_PAGED_TIMEOUT = 4
+QD_PAGED_STALL_FIRST = 1
+QD_PAGED_STALL_LATE = 2
 
 # Every function include/qdecode.h declares (checked by the tests).
 EXPORTS = (
@@ -44,7 +46,7 @@ EXPORTS = (
     "qd_generate_sample", "qd_sample_workspace_bytes", "qd_sample_logits",
     "qd_paged_append", "qd_paged_attn_decode_workspace_bytes", "qd_paged_attn_decode",
     "qd_paged_attn_prompt_workspace_bytes", "qd_paged_attn_prompt", "qd_sample_rows",
-    "qd_paged_inject_stall",
+    "qd_paged_inject_stall", "qd_paged_inject_stall_at",
     "qd_paged_append_q8", "qd_paged_read_q8", "qd_paged_attn_decode_q8",
     "qd_paged_attn_decode_shared_workspace_bytes", "qd_paged_attn_decode_shared", "qd_score_rows",
 )
@@ -234,6 +236,8 @@ def load(build_if_stale: bool = True):
     L.qd_paged_attn_prompt.restype = i32
     L.qd_paged_inject_stall.argtypes = []
     L.qd_paged_inject_stall.restype = None
+    L.qd_paged_inject_stall_at.argtypes = [i32]
+    L.qd_paged_inject_stall_at.restype = i32
     L.qd_sample_rows.argtypes = [vp, i32, i32, u32, i64, vp, vp, vp, vp, vp, vp, vp, vp]
     L.qd_sample_rows.restype = i32
     q8 = C.POINTER(QdPagedQ8)

@@ -202,11 +202,11 @@ static void launch_decode(const PAttnArgs& a, void* workspace, cudaStream_t s) {
     launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas, 8, true);
 }
 
-// qd_paged_inject_stall, taken by the thread's next call.
-static thread_local bool stall_next = false;
-static bool take_stall() {
-  const bool stall = stall_next;
-  stall_next = false;
+// qd_paged_inject_stall and qd_paged_inject_stall_at, taken by the thread's next call.
+static thread_local int stall_next = kPpStallNone;
+static int take_stall() {
+  const int stall = stall_next;
+  stall_next = kPpStallNone;
   return stall;
 }
 
@@ -470,7 +470,7 @@ int qd_paged_attn_decode_q8(const qd_paged_q8* kv, const void* q, int dtype, int
     Q8Args args{};
     args.a = a;
     args.scale = {kv->k_scale, kv->v_scale};
-    args.stall = take_stall();
+    args.stall = take_stall() == kPpStallFirst;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int group = q_heads / kv->kv_heads;
     if (group <= 2) launch_decode_q8<Q8Whole>(args, workspace, s);
@@ -542,6 +542,12 @@ int qd_paged_attn_prompt(const qd_paged_kv* kv, const void* q, int dtype, int64_
   });
 }
 
-void qd_paged_inject_stall(void) { stall_next = true; }
+void qd_paged_inject_stall(void) { stall_next = kPpStallFirst; }
+int qd_paged_inject_stall_at(int where) {
+  return guarded([&] {
+    need(where == kPpStallFirst || where == kPpStallLate, "qd_paged_inject_stall_at: no such place");
+    stall_next = where;
+  });
+}
 
 }  // extern "C"

@@ -63,12 +63,14 @@ constexpr int kPpMaxSplits = 32;
 constexpr int kPpFlush = 4;        // tiles between two moves of O to the workspace (f32 results)
 constexpr float kPpLag = 8.0f, kPpShift = 7.0f;
 
+// kFirst: block 0 withholds its first key tile. kLate (SHARED): the second softmax set begins each work 40 us late.
+enum PpStall : int { kPpStallNone = 0, kPpStallFirst = 1, kPpStallLate = 2 };
 struct PPromptArgs {
   CUtensorMap tk, tv, tv16;  // boxes of a page (at most 128 rows), and of 16 rows
   PAttnArgs a;
   int splits;
   int cta_rows;  // 128 times the row tiles of a CTA
-  int stall;     // test hook (qd_paged_inject_stall): block 0 withholds its first key tile
+  int stall;     // test hook (qd_paged_inject_stall, qd_paged_inject_stall_at), one of PpStall
   // Unnormalised sums (f32 results, or parts > 1): [item][KV head][split][32 groups of 4 dims][cta_rows], so
   // that a warp's rows lie side by side; and their maxima and weights: [item][KV head][split][cta_rows].
   float4* po;
@@ -520,7 +522,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       // ---- copies: K and V tiles alternate through the ring ----
       const int ps = 1 << a.kv.page_shift, box = min(ps, kPpKeys), boxes = kPpKeys / box;
       int issued_to = -1, done = 0;  // ring slots of the works before
-      bool ok = !(pa.stall && blockIdx.x == 0);
+      bool ok = !(pa.stall == kPpStallFirst && blockIdx.x == 0);
       for (int n = 0, nk = 0; ok && (CLAIM || n == 0); ++n) {
         ok = wait_work(n, nk);
         if (!ok || work_of(n).halves == 0) break;
@@ -641,7 +643,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         pp_commit(&s_full[t], leader);
       };
       bool ok = true;
-      unsigned turn = 0, q_turn = 0;  // bit t: parity of row tile t's barriers before this work
+      unsigned turn = 0, q_turn = 0;  // bit t: parity of row tile t's barriers before this work (SHARED: works in q_turn)
       int done = 0;                   // ring slots of the works before
       for (int n = 0, nk = 0; ok && (CLAIM || n == 0); ++n) {
         ok = wait_work(n, nk);
@@ -685,8 +687,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
             scores(j % kAlt, ring_slot(2 * j));
             pp_commit(&empty[ring_slot(2 * j)], leader);
           };
-          ok = __all_sync(0xffffffffu, pp_wait(&q_full[0], q_turn & 1u, &failed));
-          q_turn ^= 1u;
+          ok = __all_sync(0xffffffffu, pp_wait(&q_full[q_turn & 1u], q_turn >> 1 & 1u, &failed));
+          ++q_turn;
           for (int j = 0; j < halves; ++j) scores_of(j);
           for (int j = 0; j < nk && ok; ++j) {
             const int t = j % kAlt;
@@ -773,8 +775,12 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         const long long q_at =
             live ? (long long)(it.tok0 + tok) * a.q_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf : -1;
         float c = fabsf(a.scale) * kLog2e;  // of the row's scores
-        if (SHARED && t == 1) {  // the other set brings the queries
-          ok = ok && __all_sync(0xffffffffu, pp_wait(&q_full[0], (unsigned)works & 1u, &failed));
+        if (SHARED && t == 1) {
+          // The other set brings the queries. It may end this work and bring the next one's before this set has looked
+          // (of two key tiles it waits for its own only), so works have two barriers in turn; the work behind the
+          // next is handed out when this one has been left.
+          if (pa.stall == kPpStallLate) __nanosleep(40000);
+          ok = ok && __all_sync(0xffffffffu, pp_wait(&q_full[works & 1], (unsigned)works >> 1 & 1u, &failed));
           if constexpr (PARTS == 2) c = fmaxf(c * f16_fit(q_exp[works & 1][wr + lane]).y, 1.0e-37f);
         } else {
         if constexpr (PARTS > 1) {
@@ -849,7 +855,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        pp_arrive(&q_full[t]);
+        pp_arrive(&q_full[SHARED ? works & 1 : t]);
         }
         float m = -INFINITY, l = 0.0f;
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;

@@ -308,3 +308,28 @@ def test_16_bit_queries_keep_both_parts_of_a_weight(sizes, prefix, io):
     tol = tol + HALF_STEP[io] * want.abs() + (2.0 ** -25 if io == "f16" else 0.0) + 2.0 ** -20 * want.abs().amax(-1, keepdim=True)
     close(torch, R.paged_attn_decode(q, k, v, whole, n), want, tol)
     close(torch, y, want, tol)
+
+
+def test_places_to_stall_at_are_checked():
+    L = _lib.load()
+    for bad in (0, -1, 99):
+        assert L.qd_paged_inject_stall_at(bad) == _lib.QD_E_INVALID
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("io,cache", [("f32", "f16"), ("f16", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("prefix", [200, 400, [100 + 40 * (i % 9) for i in range(120)]], ids=["two", "four", "ragged"])
+def test_threads_that_begin_late_change_nothing(io, cache, prefix):
+    """One set of a block's threads may be a whole row tile ahead of the other: here it has 40 us at every tile, more
+    than a tile of 2 to 4 key tiles takes. 120 groups of 4 KV heads: blocks take others' work."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    groups = 120
+    prefix = [prefix] * groups if isinstance(prefix, int) else prefix
+    k, v, table, n, starts, shared, _ = make_shared(torch, [2] * groups, prefix, [3] * (2 * groups), 64, 4, cache)
+    q = torch.randn(2 * groups, 8, D, device="cuda").to(_types(torch)[io])
+    want = R.paged_attn_decode_shared(q, k, v, table, n, starts, shared)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert _lib.load().qd_paged_inject_stall_at(_lib.QD_PAGED_STALL_LATE) == _lib.QD_OK
+    y = R.paged_attn_decode_shared(q, k, v, table, n, starts, shared, status=status)
+    assert int(status) == 0 and torch.equal(y, want)
