@@ -296,9 +296,12 @@ int qd_batch_inject_stall(qd_batch* b);
  *    captured call, at every replay.)
  *  - qd_paged_inject_stall_at: the same at a place: QD_PAGED_STALL_FIRST as above;
  *    QD_PAGED_STALL_LATE (qd_paged_attn_decode_shared): nothing is withheld, but half of the threads of every
- *    block begin each of its row tiles 40 us after the others, which must not change a result. */
+ *    block begin each of its row tiles 40 us after the others, which must not change a result;
+ *    QD_PAGED_STALL_LAST (prompts and shared prefixes): block 0 withholds the last key tile of its first rows, after
+ *    it has taken other rows over (where there are more blocks than the GPU runs at once). */
 #define QD_PAGED_STALL_FIRST 1
 #define QD_PAGED_STALL_LATE 2
+#define QD_PAGED_STALL_LAST 3
 void qd_paged_inject_stall(void);
 int qd_paged_inject_stall_at(int where);
 

@@ -26,6 +26,7 @@ QD_PAGED_BAD_LENGTH = 2
 QD_PAGED_TIMEOUT = 4
 QD_PAGED_STALL_FIRST = 1
 QD_PAGED_STALL_LATE = 2
+QD_PAGED_STALL_LAST = 3
 
 # Every function include/qdecode.h declares (checked by the tests).
 EXPORTS = (

@@ -545,7 +545,7 @@ int qd_paged_attn_prompt(const qd_paged_kv* kv, const void* q, int dtype, int64_
 void qd_paged_inject_stall(void) { stall_next = kPpStallFirst; }
 int qd_paged_inject_stall_at(int where) {
   return guarded([&] {
-    need(where == kPpStallFirst || where == kPpStallLate, "qd_paged_inject_stall_at: no such place");
+    need(where == kPpStallFirst || where == kPpStallLate || where == kPpStallLast, "qd_paged_inject_stall_at: no such place");
     stall_next = where;
   });
 }

@@ -63,8 +63,9 @@ constexpr int kPpMaxSplits = 32;
 constexpr int kPpFlush = 4;        // tiles between two moves of O to the workspace (f32 results)
 constexpr float kPpLag = 8.0f, kPpShift = 7.0f;
 
-// kFirst: block 0 withholds its first key tile. kLate (SHARED): the second softmax set begins each work 40 us late.
-enum PpStall : int { kPpStallNone = 0, kPpStallFirst = 1, kPpStallLate = 2 };
+// First: block 0 withholds its first key tile. Late (SHARED): the second softmax set begins each work 40 us late. Last:
+// block 0 withholds the last key tile of its first work, whose successor it has then taken.
+enum PpStall : int { kPpStallNone = 0, kPpStallFirst = 1, kPpStallLate = 2, kPpStallLast = 3 };
 struct PPromptArgs {
   CUtensorMap tk, tv, tv16;  // boxes of a page (at most 128 rows), and of 16 rows
   PAttnArgs a;
@@ -431,6 +432,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
     return !CLAIM ||
            __all_sync(0xffffffffu, pp_wait(&work_full[n & 1], (unsigned)(n >> 1) & 1u, &failed, pp_patience(tiles)));
   };
+  // SHARED: where a work's row has its sums, and how many of them.
+  auto place = [&](const PpWork& w, int lr) {
+    return make_int2(w.item * kRows + lr, w.it.v.tiles < 2 ? w.it.v.tiles : w.parts * kAlt);
+  };
   auto work_of = [&](int n) -> const PpWork& { return CLAIM ? work[n & 1] : first; };
   auto work_done = [&](int n) {
     __syncwarp();
@@ -534,6 +539,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
           // the scheduling warp has the time of the ring's tiles to find the next work; earlier, a CTA would hold
           // work that another one could begin
           if (CLAIM && i == max(0, 2 * nk - 3) && lane == 0) pp_arrive(&ask);
+          if (pa.stall == kPpStallLast && blockIdx.x == 0 && n == 0 && i == 2 * nk - 2) {
+            ok = false;
+            break;
+          }
           const int j = i >> 1, at = done + i, slot = at % S;
           const bool is_v = i & 1;
           const int k0 = it.v.tile(t0 + j) * kPpKeys;
@@ -1063,7 +1072,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
       done += nk;
       if (nk > 0) ++works;
       if (SHARED && live && t == 0 && hf == 0 && g == 0 && z == 0)
-        pa.rows[(long long)(it.tok0 + tok) * G + hs] = make_int2(item * kRows + lr, it.v.tiles < 2 ? it.v.tiles : parts * kAlt);
+        pa.rows[(long long)(it.tok0 + tok) * G + hs] = place(work_of(n), lr);
       if (!SHARED && nk == 0 && live) {  // no key is visible to any row
         const long long base = (long long)(it.tok0 + tok) * a.y_stride + ((long long)g * G + hs) * kHeadDim + 64 * hf;
         for (int i = 0; i < kHeadDim / 2; i += 4) store4(a.y, base + i, a.dtype, make_float4(0.f, 0.f, 0.f, 0.f));
@@ -1086,6 +1095,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         for (int e = tid; e < 32 * n_rows; e += kPpSoftmax) {
           const int lr = e >> 5, row = w.row0 + lr, tok = w.it.tok0 + row / G;
           if ((unsigned)tok >= (unsigned)a.rows) continue;
+          // (and where the rows of a work are that was taken and not begun)
+          if (SHARED && w.g == 0 && w.z == 0 && lane == 0) pa.rows[(long long)tok * G + row % G] = place(w, lr);
           if (SHARED || w.parts > 1)
             for (int x = 0; x < kAlt; ++x)
               pa.pml[((((long long)w.item * kvh + w.g) * pa.splits + w.z) * kAlt + x) * kRows + lr] = make_float2(gone, gone);

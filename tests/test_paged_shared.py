@@ -333,3 +333,32 @@ def test_threads_that_begin_late_change_nothing(io, cache, prefix):
     assert _lib.load().qd_paged_inject_stall_at(_lib.QD_PAGED_STALL_LATE) == _lib.QD_OK
     y = R.paged_attn_decode_shared(q, k, v, table, n, starts, shared, status=status)
     assert int(status) == 0 and torch.equal(y, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("io,cache", [("f32", "f16"), ("f16", "f16"), ("f32", "bf16")])
+@pytest.mark.parametrize("prefix", [100, 900])
+@pytest.mark.parametrize("groups", [200, 700])
+def test_rows_that_a_block_took_and_could_not_begin_are_nan(io, cache, prefix, groups):
+    """Groups of one KV head: block 0 has the last group's rows and takes another group's before it gives up (of 700
+    for certain: 148 blocks run and ask once each while 552 are left; of 200, 52 are left for all who ask, and it may
+    come too late). The workspace holds zeros, as a place among the sums zero of them."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    k, v, table, n, starts, shared, _ = make_shared(torch, [3] * groups, [prefix] * groups, [9] * (3 * groups), 64, 1, cache)
+    q = torch.randn(3 * groups, 4, D, device="cuda").to(_types(torch)[io])
+    want = R.paged_attn_decode_shared(q, k, v, table, n, starts, shared)
+    ws = torch.zeros(_lib.load().qd_paged_attn_decode_shared_workspace_bytes(3 * groups, groups, 4, 1), dtype=torch.uint8, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert _lib.load().qd_paged_inject_stall_at(_lib.QD_PAGED_STALL_LAST) == _lib.QD_OK
+    y = R.paged_attn_decode_shared(q, k, v, table, n, starts, shared, workspace=ws, status=status)
+    assert int(status) == _lib.QD_PAGED_TIMEOUT
+    gone = y.isnan().all(-1).view(groups, 12)
+    assert torch.equal(gone, y.isnan().any(-1).view(groups, 12))
+    assert bool(gone[-1].all()) and torch.equal(gone.any(-1), gone.all(-1))
+    assert int(gone.any(-1).sum()) in ((1, 2) if groups == 200 else (2,))
+    keep = ~gone.view(-1, 4)
+    assert torch.equal(y[keep], want[keep])
+    status.zero_()
+    assert torch.equal(R.paged_attn_decode_shared(q, k, v, table, n, starts, shared, workspace=ws, status=status), want)
+    assert int(status) == 0
