@@ -1,5 +1,6 @@
 // Host entries of the paged key-value cache operators (kernels: paged.cuh).
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <string>
 
@@ -295,7 +296,7 @@ static void launch_prompt(const PAttnArgs& a, const void* q_any, void* workspace
 
 // Attention over shared prefixes: its workspace is the sums of both kinds of positions.
 struct SharedWs {
-  size_t po, pml, rows, tail_o, tail_ml, decode, bytes;
+  size_t po, pml, rows, tail_o, tail_ml, mark, decode, bytes;
 };
 constexpr int kSharedRows = 128;  // rows of a CTA (sequences times query heads of a KV head)
 // Row tiles of the groups, at most.
@@ -316,12 +317,19 @@ static SharedWs shared_ws(int batch, int groups, int q_heads, int kv_heads) {
   w.rows = take((size_t)batch * G * 8);
   w.tail_o = take((size_t)batch * q_heads * kHeadDim * 4);
   w.tail_ml = take((size_t)batch * q_heads * 8);
+  w.mark = take(8);
   w.decode = take(pd_ws_bytes(batch));
   return w;
 }
 
+// A number that no call had before and that a workspace's old contents will hardly be.
+static uint64_t next_ticket() {
+  static std::atomic<uint64_t> calls{0};
+  return (calls.fetch_add(1, std::memory_order_relaxed) + 1) * 0x9e3779b97f4a7c15ull;
+}
+
 template <typename T, int PARTS>
-static void launch_shared(const PAttnArgs& a, void* workspace, cudaStream_t s) {
+static void launch_shared(PAttnArgs a, void* workspace, cudaStream_t s) {
   constexpr int kSets = pp_tiles<PARTS>();
   const int B = a.kv.batch, kvh = a.kv.kv_heads, G = a.q_heads / kvh, subs = (G + 7) / 8;
   const long long most = (long long)B * kvh * subs * (((long long)a.kv.table_width << a.kv.page_shift) / kPdTile + 1);
@@ -329,6 +337,8 @@ static void launch_shared(const PAttnArgs& a, void* workspace, cudaStream_t s) {
     throw QdError{QD_E_RANGE, "qd_paged_attn_decode_shared: batch * heads * table beyond 2^31 units"};
   const SharedWs w = shared_ws(B, a.groups, a.q_heads, kvh);
   char* base = static_cast<char*>(workspace);
+  a.mark = reinterpret_cast<unsigned long long*>(base + w.mark);
+  a.ticket = next_ticket();
   PPromptArgs p{};
   p.a = a;
   p.a.kv.batch = a.groups;

@@ -369,6 +369,8 @@ struct PAttnArgs {
   const int* shared_lens;  // [batch]
   float* tail_o;           // [batch][q_heads][128]: unnormalised sums of the positions behind them,
   float2* tail_ml;         // [batch][q_heads]: with their maxima and weights
+  // The launch over the shared positions writes the call's ticket here when all before it is done, the join clears it.
+  unsigned long long *mark, ticket;
 };
 
 }  // namespace qd

@@ -265,8 +265,11 @@ __host__ __device__ constexpr int pd_smem(int batch) { return 4 * kPdStages * kP
 
 // TAIL: the positions behind those that a sequence shares (paged_shared.cuh). All sums go to the workspace, a
 // (sequence, head) that one CTA holds whole to a place of its own. The launch before it, over the shared positions, may
-// still run (it wrote nothing that is read here, and it began after all before it had ended), so it is
-// waited for at the end only; a fence clears L1 of what that launch may have found there.
+// still run: it writes nothing that is read here, so it is waited for at the end only. What came before that
+// launch is ordered by a word in memory: its first thread has waited for all of it and then releases the call's ticket,
+// which every thread here acquires before it reads anything. (That launch's blocks have all passed their wait when
+// this one starts, so the ticket is there; a thread that does not find it waits for the launch to end. With that wait in
+// every call 64 of 16384 take 55 us instead of 52, 4 of 1000 23 instead of 19.)
 template <typename T, bool THREE, bool TAIL = false>
 __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_constant__ PAttnArgs a, void* workspace) {
   extern __shared__ __align__(128) unsigned char smem[];
@@ -276,8 +279,13 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_decode(const __grid_consta
   __shared__ float2 sml[4][8];  // maximum and sum of each warp and head
   const int G = a.q_heads / a.kv.kv_heads, subs = (G + 7) >> 3, nh = a.kv.kv_heads * subs, B = a.kv.batch;
   const PDecodeWs ws = pd_ws(workspace);
-  if (TAIL) __threadfence();
-  else pdl_wait();
+  if (TAIL) {
+    unsigned long long found;
+    asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(found) : "l"(a.mark) : "memory");
+    if (found != a.ticket) pdl_wait();
+  } else {
+    pdl_wait();
+  }
   pdl_trigger();
   const int held = TAIL ? min(a.q_starts[a.groups], B) : B;  // sequences behind the last group are padding
 

@@ -399,6 +399,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
     tma_prefetch_map(&pa.tv16);
   }
   pdl_wait();
+  if (SHARED && blockIdx.x == 0 && tid == 0)
+    asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(a.mark), "l"(a.ticket) : "memory");
   pdl_trigger();
   // What block `b` of the grid is to do, if anything (whole warps).
   auto find_work = [&](int b, PpWork& w) {

@@ -40,6 +40,7 @@ __global__ void __launch_bounds__(kPsThreads) k_paged_shared_join(const __grid_c
   const int b = min(row / G, a.kv.batch - 1), hs = row % G;
   pdl_wait();
   pdl_trigger();
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.mark = 0;  // (a captured call has one ticket for all replays)
   const PDecodeWs ws = pd_ws(pa.decode_ws);
   int2 at = pa.rows[min(row, a.kv.batch * G - 1)];
   const int f0 = ws.first[b], f1 = ws.first[b + 1], all = ws.first[a.kv.batch];

@@ -362,3 +362,49 @@ def test_rows_that_a_block_took_and_could_not_begin_are_nan(io, cache, prefix, g
     status.zero_()
     assert torch.equal(R.paged_attn_decode_shared(q, k, v, table, n, starts, shared, workspace=ws, status=status), want)
     assert int(status) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("captured", [False, True])
+def test_what_was_written_right_before_is_seen(captured):
+    """Steps of append and attention without a pause, each step's new rows, lengths and queries written by the launches
+    just before: the results of the same calls made one at a time. One workspace for all, with old contents."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    H, kvh, B, steps = 8, 2, 24, 40
+    k, v, table, n, starts, shared, whole = make_shared(torch, [10, 14], [300, 77], [1] * B, 16, kvh, "f16")
+    grown = torch.arange(k.shape[0], k.shape[0] + 4 * B, dtype=torch.int32, device="cuda").view(B, 4)   # pages to grow into
+    k, v = (torch.cat([x, torch.zeros(4 * B, kvh, 16, D, dtype=x.dtype, device="cuda")]) for x in (k, v))
+    table = torch.cat([table, torch.full((B, 4), -1, dtype=torch.int32, device="cuda")], 1)
+    for b in range(B):
+        used = -(-int(n[b]) // 16)
+        table[b, used:used + 4] = grown[b]
+    qkv = torch.randn(steps, B, (H + 2 * kvh) * D, device="cuda")
+    ws = torch.full((_lib.load().qd_paged_attn_decode_shared_workspace_bytes(B, 2, H, kvh),), 255, dtype=torch.uint8, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    keep = [x.clone() for x in (k, v, n)]
+
+    def run(pause):
+        ys = []
+        for i in range(steps):
+            n.add_(1)
+            q = R.paged_append(qkv[i], k, v, table, n, None, None, H, status=status)
+            pause()
+            ys.append(R.paged_attn_decode_shared(q.view(B, H, D), k, v, table, n, starts, shared, workspace=ws, status=status))
+            pause()
+        return torch.stack(ys)
+
+    want = run(torch.cuda.synchronize)
+    graph = torch.cuda.CUDAGraph()
+    if captured:
+        with torch.cuda.graph(graph):
+            ys = run(lambda: None)
+    for _ in range(5):
+        for x, old in zip((k, v, n), keep):
+            x.copy_(old)
+        if captured:
+            ys.zero_()
+            graph.replay()
+        else:
+            ys = run(lambda: None)
+        assert torch.equal(ys, want) and int(status) == 0
