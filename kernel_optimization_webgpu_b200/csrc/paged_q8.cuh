@@ -708,8 +708,11 @@ __global__ void __launch_bounds__(kPdThreads, Heads::kCtas) k_paged_decode_q8(co
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           L += sml[w][h].y * (sml[w][h].x == -INFINITY ? 0.0f : exp2_fast(sml[w][h].x - M));  // (NaN stays)
-          const float f = smo[w][h] == -INFINITY ? 0.0f : exp2_fast(smo[w][h] - Heads::kShift - M);
-          x += reinterpret_cast<const float*>(smem + (w * kQ8Stages + slot) * kQ8Slot)[h * kPdSumRow + tid] * f;
+          // (the exponential has no results below 2^-126, the sums may: V scales go down to there)
+          const float e = smo[w][h] - M, lift = e < -64.0f ? 64.0f : 0.0f;
+          const float f = smo[w][h] == -INFINITY ? 0.0f : exp2_fast(e + lift);
+          const float sum = reinterpret_cast<const float*>(smem + (w * kQ8Stages + slot) * kQ8Slot)[h * kPdSumRow + tid];
+          x += sum * (1.0f / (1 << (int)Heads::kShift)) * f * (lift == 0.0f ? 1.0f : 0x1p-64f);
         }
         if (whole) {
           store1(a.y, out + h * kHeadDim, a.dtype, x * inv_sum(L));

@@ -597,3 +597,23 @@ def test_integers_are_the_quotients_rounded(io, size):
     assert int((off == 0).sum()) > rows * kvh * 32
     sure = (off == 0) | (off > 2.0 ** -16) if io == "f32" else torch.ones_like(off, dtype=torch.bool)
     assert torch.equal(ints[sure].double(), q.round()[sure])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("exponent", [-125, -118, -105, -97, -90, 0, 100])
+@pytest.mark.parametrize("heads", [4, 8, 16], ids=lambda h: f"{h}q2kv")
+def test_v_scales_down_to_the_smallest(exponent, heads):
+    """Every V scale within a factor of 2 of 2^exponent: results go down to 2^-126 and are not flushed. (The tolerance's
+    term for the smallest numbers makes place for 4 of f32's last ones.)"""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    lens = [300, 1, 5000, 17]
+    k, v, ks, vs, table, n = make_q8(torch, lens, 32, 2, seed=21, spread=1.0)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    vs *= 0.0
+    vs += torch.ldexp(1 + torch.rand(vs.shape, generator=g, device="cuda"), torch.tensor(exponent, device="cuda"))
+    q = torch.randn(len(lens), heads, D, device="cuda")
+    y = R.paged_attn_decode_q8(q, k, v, ks, vs, table, n)
+    want, tol = plain(torch, q, k, v, ks, vs, table, n, 0, 0, D ** -0.5, "f32")
+    close(torch, y, want, tol - 1e-30 + 2.0 ** -147)
+    assert bool((y != 0).any(-1).all())
