@@ -309,7 +309,10 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score_rows(const __grid_co
   }
   if (K > 0) {
     if (warp == 0) {
-      // The border: the largest key of 16 bits that K groups reach.
+      // The border, from the top bit down: the largest key that K groups reach, or one that no more than K do. (To the
+      // type's last bit: with f32 keys of 16 bits a row whose values lie close together beside their size, as under a
+      // common offset, had tens of thousands of tokens at the border, and each of the largest took a pass.)
+      constexpr int kLast = sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 13 : 16;
       uint32_t key[kScoreGroups / 32];
 #pragma unroll
       for (int i = 0; i < kScoreGroups / 32; ++i) {
@@ -318,12 +321,14 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score_rows(const __grid_co
       }
       uint32_t low = 0;
 #pragma unroll
-      for (int bit = 31; bit >= 16; --bit) {
+      for (int bit = 31; bit >= kLast; --bit) {
         const uint32_t want = low | 1u << bit;
         int reach = 0;
 #pragma unroll
         for (int i = 0; i < kScoreGroups / 32; ++i) reach += key[i] >= want;
-        if (__reduce_add_sync(0xffffffffu, reach) >= K) low = want;
+        reach = __reduce_add_sync(0xffffffffu, reach);
+        if (reach >= K) low = want;
+        if (reach == K) break;
       }
       if (lane == 0) sh.border = low > 0x007fffffu ? row_key_value(low) : -INFINITY;  // (the key of -inf)
     }
@@ -376,7 +381,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score_rows(const __grid_co
           else sh.best[before] = mine;
         }
       }
-    } else {  // too many tokens reach the border (long classes of equal values): one after the other
+    } else {  // too many tokens reach the border (values that occur a thousand times): one after the other
       u64 below = ~0ull;
       for (int k = 0; k < K; ++k) {
         u64 best = 0;
@@ -426,7 +431,7 @@ template <typename T>
 static void launch_score_rows(ScoreArgs a, int rows, cudaStream_t s) {
   constexpr int VE = 16 / sizeof(T);
   // CTAs per row: as many as fill the GPU twice (a CTA pays 4 us beside its loads: 512 rows of bf16 40 us with one,
-  // 44 with two, 94 with eight; 64 rows of f32 37, 23 and 15.5), none below 2048 tokens.
+  // 44 with two, 94 with eight; 64 rows of f32 37, 23 and 15.5), but 2048 tokens are not split.
   int C = 1;
   while (C < kScoreCluster && (long long)rows * C < 2 * current_sms() && (a.vocab + C - 1) / C > 2048) C *= 2;
   a.per = ((a.vocab + VE - 1) / VE + 1 + C - 1) / C;  // (a row that starts inside a vector has one more)

@@ -214,6 +214,36 @@ def test_scores_of_draws_are_the_samplers():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("offset,size", [(1000.0, 4.0), (-30000.0, 1.0), (3.0e6, 100.0), (0.0, 1e-30)])
+@pytest.mark.parametrize("top", [1, 20, 64])
+def test_rows_with_a_common_offset(offset, size, top):
+    """A softmax does not change under an offset, and the time does not either: distinct values next to each other are
+    told apart by their last bits, not one pass after the other (which took more than ten times as long)."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    g = torch.Generator(device="cuda").manual_seed(3)
+    plain = torch.randn(6, 151936, generator=g, device="cuda")
+    x = plain * size + offset
+    tokens = [5, 151935, 0, int(x[3].argmax()), 77, 1000]
+    check(torch, x, tokens, top)
+    t = torch.tensor(tokens, dtype=torch.int32, device="cuda")
+
+    def us(rows):
+        best = math.inf
+        for _ in range(10):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(20):
+                R.score_rows(rows, t, top=top)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    assert us(x) < 2 * us(plain)
+
+
+@pytest.mark.gpu
 def test_offsets_beyond_32_bits():
     """Rows 4.4 GB apart."""
     torch = _cuda()
