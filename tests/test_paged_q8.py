@@ -617,3 +617,87 @@ def test_v_scales_down_to_the_smallest(exponent, heads):
     want, tol = plain(torch, q, k, v, ks, vs, table, n, 0, 0, D ** -0.5, "f32")
     close(torch, y, want, tol - 1e-30 + 2.0 ** -147)
     assert bool((y != 0).any(-1).all())
+
+
+KERNELS = pytest.mark.parametrize("heads", [4, 8, 16], ids=lambda h: f"{h}q2kv")   # one for each kernel behind the call
+
+
+@pytest.mark.gpu
+@KERNELS
+@pytest.mark.parametrize("spread", [30.0, 60.0])
+@pytest.mark.parametrize("heavy", [False, True])
+def test_scales_of_any_size_in_every_kernel(heads, spread, heavy):
+    """V rows 2^120 apart, some of them zeros; heavy: the likeliest key's V is the smallest, for every head."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    lens = [300, 17, 1000]
+    k, v, ks, vs, table, n = make_q8(torch, lens, 32, 2, seed=3, spread=1.0)
+    g = torch.Generator(device="cuda").manual_seed(9)
+    vs *= 2.0 ** ((torch.rand(vs.shape, generator=g, device="cuda") * 2 - 1) * spread)
+    vs[:, 1, ::3] = torch.where(vs[:, 1, ::3].isnan(), vs[:, 1, ::3], 0.0)
+    q = torch.randn(3, heads, D, device="cuda")
+    if heavy:
+        q = q[:, ::heads // 2].repeat_interleave(heads // 2, 1) + 0.1 * q
+        for b in range(3):
+            k[table[b, 0], :, 0] = (q[b, ::heads // 2] * 30).clamp(-127, 127).to(torch.int8)
+            ks[table[b, 0], :, 0] = 0.2
+            vs[table[b, 0], :, 0] = 2.0 ** -spread
+    y = R.paged_attn_decode_q8(q, k, v, ks, vs, table, n)
+    want, tol = plain(torch, q, k, v, ks, vs, table, n, 0, 0, D ** -0.5, "f32")
+    close(torch, y, want, tol)
+
+
+@pytest.mark.gpu
+@KERNELS
+@pytest.mark.parametrize("size", [0.0, 1e-20, 1e5, 1e20])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_queries_of_any_size_in_every_kernel(heads, size, sign):
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    cache = make_q8(torch, [200, 65], 16, 2, seed=5)
+    q = torch.randn(2, heads, D, device="cuda") * size
+    scale = sign * D ** -0.5 / (size or 1.0)
+    y = R.paged_attn_decode_q8(q, *cache, scale=scale)
+    want, tol = plain(torch, q, *cache, 0, 0, torch.tensor(scale, dtype=torch.float32).double().item(), "f32")
+    close(torch, y, want, tol)
+
+
+@pytest.mark.gpu
+@KERNELS
+def test_rows_that_are_not_finite_in_every_kernel(heads):
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    k, v, ks, vs, table, n = make_q8(torch, [100, 100], 16, 2)
+    q = torch.randn(2, heads, D, device="cuda")
+    G = heads // 2
+    clean = R.paged_attn_decode_q8(q, k, v, ks, vs, table, n)
+    for scales in (ks, vs):
+        keep = scales.clone()
+        for bad in (math.nan, math.inf):
+            scales[table[1, 3], 1, 5] = bad
+            y = R.paged_attn_decode_q8(q, k, v, ks, vs, table, n)
+            assert torch.equal(y[0], clean[0]) and torch.equal(y[1, :G], clean[1, :G])
+            if bad != bad or scales is vs:   # (an infinite key may have a weight of 0)
+                assert not bool(torch.isfinite(y[1, G:]).any())
+            y = R.paged_attn_decode_q8(q, k, v, ks, vs, table, n, window=30, sinks=4)   # out of its sight
+            assert bool(torch.isfinite(y).all())
+        scales.copy_(keep)
+    q[0, 1, 3] = math.nan   # a query of its own
+    y = R.paged_attn_decode_q8(q, k, v, ks, vs, table, n)
+    assert bool(y[0, 1].isnan().all()) and bool(torch.isfinite(y[0, 0]).all()) and torch.equal(y[1], clean[1])
+
+
+@pytest.mark.gpu
+@KERNELS
+@pytest.mark.parametrize("window,sinks", [(1, 0), (17, 4), (64, 65), (130, 3000)])
+def test_window_and_sinks_in_every_kernel(heads, window, sinks):
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    lens = [1500, 3, 150, 64, 1, 129]
+    cache = make_q8(torch, lens, 16, 2)
+    q = torch.randn(len(lens), heads, D, device="cuda") * 1.5
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    y = R.paged_attn_decode_q8(q, *cache, window=window, sinks=sinks, status=status)
+    want, tol = plain(torch, q, *cache, window, sinks, D ** -0.5, "f32")
+    close(torch, y, want, tol)
+    assert int(status) == 0
