@@ -200,7 +200,7 @@ static void launch_decode(const PAttnArgs& a, void* workspace, cudaStream_t s) {
   launch_ex(k_paged_decode<T, THREE>, dim3(ctas), dim3(kPdThreads), (size_t)pd_smem(a.kv.batch), s, a, workspace);
   // (a table of one unit leaves nothing to join)
   if ((a.kv.table_width << a.kv.page_shift) > kPdTile)
-    launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas, 8, true);
+    launch_ex(k_paged_decode_join<8, true>, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas);
 }
 
 // qd_paged_inject_stall and qd_paged_inject_stall_at, taken by the thread's next call.
@@ -235,7 +235,7 @@ static void launch_decode_q8(Q8Args q, void* workspace, cudaStream_t s) {
   // did not find their place in one piece until others had ended (64 sequences of 2048 positions, call after call: 70 us
   // instead of 56).
   if ((a.kv.table_width << a.kv.page_shift) > kQ8Tile)
-    launch_ex(k_paged_decode_join, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas, Heads::kHeads, false);
+    launch_ex(k_paged_decode_join<Heads::kHeads, false>, dim3(a.kv.batch * nh), dim3(256), 0, s, a, workspace, ctas);
 }
 
 // Row tiles of a call (at most), and the parts that their keys are split into: enough to give

@@ -51,7 +51,8 @@ __global__ void __launch_bounds__(kPdThreads) k_paged_read_q8(const __grid_const
   auto end_of = [&](int b) { return min(paged_len(a.src, b), a.dst.table_width << a.dst.page_shift); };
   auto from = [&](int b) { return a.first ? max(a.first[b], 0) : 0; };
   struct Tiles { int tiles; };
-  pd_units(B, first, [&](int b) {
+  __shared__ int wsum[4];
+  pd_units(B, first, tid, lane, tid >> 5, wsum, [&](int b) {
     const int n = end_of(b), f = min(from(b), n);
     return Tiles{f < n ? (n + 15) / 16 - f / 16 : 0};
   });
@@ -582,7 +583,8 @@ __global__ void __launch_bounds__(kPdThreads, Heads::kCtas) k_paged_decode_q8(co
   pdl_wait();
   pdl_trigger();
   auto see = [&](int b) { return visible<kQ8Tile>(a.kv.seq_lens[b], paged_len(a.kv, b), a.window, a.sinks); };
-  pd_units(B, first, see);  // (its barriers are the mbarriers' too)
+  __shared__ int wsum[4];
+  pd_units(B, first, tid, lane, warp, wsum, see);  // (its barriers are the mbarriers' too)
   const long long U = (long long)first[B] * nh;
   const int ctas = (int)min((long long)gridDim.x, U);  // none of them empty
   auto aside = [&] {  // what is not on the way to the first copies
