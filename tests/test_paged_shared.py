@@ -408,3 +408,26 @@ def test_what_was_written_right_before_is_seen(captured):
         else:
             ys = run(lambda: None)
         assert torch.equal(ys, want) and int(status) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("io,cache", [("f32", "f16"), ("bf16", "bf16")])
+def test_prompt_rows_that_a_block_took_are_nan(io, cache):
+    """The same of qd_paged_attn_prompt: 700 prompts of 20 rows, of which block 0 holds the last and another one."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    B, new = 700, 20
+    k, v, table, n = make_cache(torch, [300] * B, 64, 1, cache)
+    starts = torch.arange(B + 1, dtype=torch.int32, device="cuda") * new
+    q = torch.randn(B * new, 4, D, device="cuda").to(_types(torch)[io])
+    want = R.paged_attn_prompt(q, k, v, table, n, starts)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert _lib.load().qd_paged_inject_stall_at(_lib.QD_PAGED_STALL_LAST) == _lib.QD_OK
+    y = R.paged_attn_prompt(q, k, v, table, n, starts, status=status)
+    gone = y.isnan().any(-1).view(B, new * 4)
+    assert int(status) == _lib.QD_PAGED_TIMEOUT and torch.equal(gone.any(-1), gone.all(-1))
+    assert bool(gone[-1].all()) and int(gone.any(-1).sum()) == 2
+    keep = ~gone.view(-1, 4)
+    assert torch.equal(y[keep], want[keep]) and bool(y[~keep].isnan().all())
+    status.zero_()
+    assert torch.equal(R.paged_attn_prompt(q, k, v, table, n, starts, status=status), want) and int(status) == 0
