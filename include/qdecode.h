@@ -478,8 +478,12 @@ int qd_paged_attn_prompt(const qd_paged_kv* kv, const void* q, int dtype, int64_
  * through the block table's row of its group's first sequence, the others through its own row;
  * only the pages that it uses so are looked up. Otherwise as
  * qd_paged_attn_decode without a window, whose results these are to rounding where the table's
- * rows agree; the shared positions are read once per group. groups: 0..batch. (Weights of
- * positions that a sequence does not see but others of its group do are zeros, not left out: a V row
+ * rows agree. A group's shared positions are read once for every 128 rows of queries (sequences times query heads of
+ * a KV head), so it pays from about 60 to 100 MB of K and V that are not read again, (sequences - 1) *
+ * shared positions * kv_heads * 512 bytes; below that qd_paged_attn_decode over a full table is the faster call: 16 query and
+ * 8 KV heads, f16, tails of 64, this call / that one: 4 sequences behind 1000 16 / 13 us, behind 16000 33 / 38; 16 behind
+ * 1000 22 / 19, behind 4000 26 / 38; 64 behind 256 27 / 24, behind 1000 30 / 44. The choice is the caller's. groups:
+ * 0..batch. (Weights of positions that a sequence does not see but others of its group do are zeros, not left out: a V row
  * among them that is not finite reaches it, as in qd_paged_attn_prompt.) A device-side wait that
  * expires makes rows NaN and sets QD_PAGED_TIMEOUT. */
 size_t qd_paged_attn_decode_shared_workspace_bytes(int batch, int groups, int q_heads, int kv_heads);

@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(256, HEADS == 4 ? 5 : 6) k_paged_append(const 
 // Half a warp per head: lane h of it holds dims 4 h .. + 3 and 64 + 4 h .. + 3, which the rotation turns into
 // each other, and a sum or maximum takes four steps for two heads at once. (The other kernel's lanes, with the rows'
 // maxima and divisions added, were bound by instructions: 16384 rows of 16 + 8 + 8 heads, f32, 437 MB, 98 us; so 73 us = 6.0 TB/s.
-// Rows of f16 or bf16, 236 MB, take 73 us too: their bound is the instructions still.)
+// Rows of f16 or bf16, 236 MB, take 73 us too: 75 % of the issue slots are taken with either.)
 // Sums run in that kernel's order: q comes out the same to the bit.
 template <typename T, int PAIRS>
 __global__ void __launch_bounds__(256, PAIRS == 2 ? 5 : 6) k_paged_append_q8(const __grid_constant__ AppendArgs a) {

@@ -5,7 +5,7 @@
 //   y = (sum over both of exp(s_j - m) v_j) / (sum over both of exp(s_j - m)),
 // and each sum is taken where its keys are cheapest:
 //  - the shared ones once for all the group's queries (k_paged_prompt with SHARED: the queries of a KV head of all
-//    the group's sequences are the rows of its 128-row tiles, so the prefix is read once a group, and what was
+//    the group's sequences are the rows of its 128-row tiles, so the prefix is read once a tile, and what was
 //    4 * 128 operations per byte of K and V becomes as many for each of the group's queries, on tcgen05);
 //  - each sequence's own by k_paged_decode with TAIL, in equal runs of units per CTA;
 //  - k_paged_shared_join adds the parts of a row in order: those of the shared positions, then its own.

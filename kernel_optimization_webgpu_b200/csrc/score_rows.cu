@@ -12,7 +12,7 @@
 // Many rows: bound by the latency of the loads and, with 16-bit logits, by the exponentials (one per token: 17 of
 // 39 us of the special-function unit), so the next batch is on its way while one is worked on. 512 x 151936 bf16 with 20
 // alternatives: 39 us (156 MB, 4.0 TB/s; 35 without alternatives), 256 x 151936 f32: 27 us (5.75 TB/s). One row of f32:
-// 7.8 us, of which a chain of loads, barriers of the cluster and the border's search, not bytes.
+// 8.0 us, of which a chain of loads, barriers of the cluster and the border's search, not bytes.
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -674,7 +674,7 @@ def paged_append_q8(qkv, k_pages, v_pages, k_scales, v_scales, block_table, seq_
                     rope_stride: Optional[int] = None, status=None, stream=None):
     """paged_append into a cache of 8-bit integers (qd_paged_append_q8): pools int8
     [pages][kv_heads][page_size][128] with f32 scales [pages][kv_heads][page_size], a row x being held as
-    scale = max|x| / 127 and x / scale rounded. Returns q."""
+    scale = max|x| / 127 and 127 x / max|x| rounded. Returns q."""
     if stream is not None:
         with _on(stream, qkv):
             return paged_append_q8(qkv, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, cos, sin, q_heads,
@@ -713,7 +713,8 @@ def paged_attn_decode_shared(q, k_pages, v_pages, block_table, seq_lens, group_s
     """paged_attn_decode for groups of sequences that share their first positions
     (qd_paged_attn_decode_shared): group i is the sequences group_starts[i] .. group_starts[i + 1] - 1 (int32,
     groups + 1 entries from 0), sequence b's first shared_lens[b] (int32) positions are those of its
-    group's first sequence and are read once for all of the group. Sequences behind the last group are padding; y
+    group's first sequence and are read once per 128 rows of queries (the header says from which sizes on that is the
+    faster call). Sequences behind the last group are padding; y
     keeps what it held there. workspace: qd_paged_attn_decode_shared_workspace_bytes."""
     if stream is not None:
         with _on(stream, q):
