@@ -12,7 +12,7 @@
 // Many rows: bound by the latency of the loads and, with 16-bit logits, by the exponentials (one per token: 17 of
 // 39 us of the special-function unit), so the next batch is on its way while one is worked on. 512 x 151936 bf16 with 20
 // alternatives: 39 us (156 MB, 4.0 TB/s; 35 without alternatives), 256 x 151936 f32: 27 us (5.75 TB/s). One row of f32:
-// 8.0 us, of which a chain of loads, barriers of the cluster and the border's search, not bytes.
+// 7.9 us, of which a chain of loads, barriers of the cluster and the border's search, not bytes.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -309,9 +309,10 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score_rows(const __grid_co
   }
   if (K > 0) {
     if (warp == 0) {
-      // The border, from the top bit down: the largest key that K groups reach, or one that no more than K do. (To the
-      // type's last bit: with f32 keys of 16 bits a row whose values lie close together beside their size, as under a
-      // common offset, had tens of thousands of tokens at the border, and each of the largest took a pass.)
+      // The border, from the top bit down: the largest key that K groups reach, or of 12 bits or more one that no other
+      // group reaches. (To the type's last bit: with f32 keys of 16 bits a row whose values lie close together beside
+      // their size, as under a common offset, had tens of thousands of tokens at the border, and each of the largest
+      // took a pass.)
       constexpr int kLast = sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 13 : 16;
       uint32_t key[kScoreGroups / 32];
 #pragma unroll
@@ -328,7 +329,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score_rows(const __grid_co
         for (int i = 0; i < kScoreGroups / 32; ++i) reach += key[i] >= want;
         reach = __reduce_add_sync(0xffffffffu, reach);
         if (reach >= K) low = want;
-        if (reach == K) break;
+        if (bit <= 20 && reach == K) break;
       }
       if (lane == 0) sh.border = low > 0x007fffffu ? row_key_value(low) : -INFINITY;  // (the key of -inf)
     }
@@ -370,8 +371,51 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score_rows(const __grid_co
       }
     }
     __syncthreads();
-    const int n = sh.listed;
-    if (n <= kScoreList && (!few || n >= K || n == last - max(first, 0))) {
+    int n = sh.listed;
+    bool whole = n <= kScoreList && (!few || n >= K || n == last - max(first, 0));
+    if (!whole) {
+      // Too many (a mask that leaves much of this CTA's share and little else, say): all of the share once more, with a
+      // border of its own, the top-th largest of its threads' maxima. (600 rows of 32000 tokens of which 5000 are
+      // held by 40 threads: one after the other, as below, the largest 20 took 615 us instead of 20.)
+      __syncthreads();
+      if (warp == 0) {
+        uint32_t key[N / 32], low = 0;
+        for (int k = 0; k < N / 32; ++k) {
+          const int t = 32 * k + lane;
+          float most = -INFINITY;
+          for (int i = 0; i < kSlots && v0 + t + i * U * N < v1; ++i) most = fmaxf(most, sh.most[i][t]);
+          key[k] = row_key(most);
+        }
+#pragma unroll 1
+        for (int bit = 31; bit >= 0; --bit) {
+          const uint32_t want = low | 1u << bit;
+          int reach = 0;
+          for (int k = 0; k < N / 32; ++k) reach += key[k] >= want;
+          if (__reduce_add_sync(0xffffffffu, reach) >= K) low = want;
+        }
+        if (lane == 0) {
+          sh.border = low > 0x007fffffu ? row_key_value(low) : -INFINITY;
+          sh.listed = 0;
+        }
+      }
+      __syncthreads();
+      const float own = sh.border;
+      if (own > -INFINITY) {
+        for (int v = v0 + tid; v < v1; v += N) {
+          const uint4 x = row.load(v);
+          if (!(Row::most(x) >= own)) continue;
+          for (int i = 0; i < VE; ++i) {
+            const float2 f = Row::pair_at(x, i / 2);
+            const float y = i & 1 ? f.y : f.x;
+            if (y >= own) list(y, v * VE - row.head + i);
+          }
+        }
+      }
+      __syncthreads();
+      n = sh.listed;
+      whole = own > -INFINITY && n <= kScoreList;
+    }
+    if (whole) {
       for (int i = tid; i < n; i += N) {
         const u64 mine = sh.list[i];
         int before = 0;
@@ -381,7 +425,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score_rows(const __grid_co
           else sh.best[before] = mine;
         }
       }
-    } else {  // too many tokens reach the border (values that occur a thousand times): one after the other
+    } else {  // values that occur a thousand times: one after the other
       u64 below = ~0ull;
       for (int k = 0; k < K; ++k) {
         u64 best = 0;

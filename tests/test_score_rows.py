@@ -244,6 +244,40 @@ def test_rows_with_a_common_offset(offset, size, top):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("top", [19, 20, 21, 40])
+def test_many_tokens_above_nothing(top):
+    """Positive tokens in 20 of the 128 groups of a row's threads, and 40 of the 256 threads, only (columns 0..159 of
+    every 1024), all others negative: they are not looked through one after the other, which took 30 to 60 times the time
+    of other rows. Twice covers the second look at them, as much again the ordering of up to 1024 that are listed."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    g = torch.Generator(device="cuda").manual_seed(8)
+    rows = 600   # one block a row
+    plain = torch.randn(rows, 32000, generator=g, device="cuda")
+    x = plain.abs() + 0.1
+    x[:, torch.arange(32000, device="cuda") % 1024 >= 160] *= -1
+    t = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    ids = R.score_rows(x, t, top=top)[2]
+    want = x.topk(top, -1)
+    assert torch.equal(x.gather(1, ids.long()), want.values)
+    check(torch, x[:3], [0, 1, 2], top)
+
+    def us(rows):
+        best = math.inf
+        for _ in range(10):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(10):
+                R.score_rows(rows, t, top=top)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    assert us(x) < 4 * us(plain)
+
+
+@pytest.mark.gpu
 def test_offsets_beyond_32_bits():
     """Rows 4.4 GB apart."""
     torch = _cuda()
@@ -254,3 +288,18 @@ def test_offsets_beyond_32_bits():
     t = torch.tensor([3, 4], dtype=torch.int32, device="cuda")
     for a, b in zip(R.score_rows(x, t, top=4), R.score_rows(x.contiguous(), t, top=4)):
         assert torch.allclose(a, b, atol=1e-5) if a.is_floating_point() else torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab,allowed", [(151936, 5000), (151936, 1500), (151936, 1030), (40000, 3000)])
+@pytest.mark.parametrize("top", [5, 20, 64])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_masks_that_leave_neighbours(vocab, allowed, top, dtype):
+    """A mask that leaves a range of token ids, which few of a row's groups of threads hold."""
+    torch = _cuda()
+    g = torch.Generator(device="cuda").manual_seed(allowed)
+    x = torch.full((6, vocab), -math.inf, device="cuda")
+    for r, first in enumerate((0, 7, 20001, vocab - allowed, 19000, 100)):
+        x[r, first:first + allowed] = torch.randn(allowed, generator=g, device="cuda") * 3
+    x[5, 100:100 + allowed:2] = 2.0   # half of them alike
+    check(torch, x.to({"f32": torch.float32, "bf16": torch.bfloat16}[dtype]), [1, 8, 20002, vocab - 1, 19000, 100], top)
