@@ -375,8 +375,9 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score_rows(const __grid_co
     bool whole = n <= kScoreList && (!few || n >= K || n == last - max(first, 0));
     if (!whole) {
       // Too many (a mask that leaves much of this CTA's share and little else, say): all of the share once more, with a
-      // border of its own, the top-th largest of its threads' maxima. (600 rows of 32000 tokens of which 5000 are
-      // held by 40 threads: one after the other, as below, the largest 20 took 615 us instead of 20.)
+      // border of its own, the top-th largest of its threads' maxima. (6 rows of 151936 tokens of which a mask leaves 5000
+      // neighbours: one after the other, as below, the largest 20 took 105 us, so 30. 600 rows of 32000 whose positive
+      // tokens 40 threads hold, the largest 21: 657 and 51 us.)
       __syncthreads();
       if (warp == 0) {
         uint32_t key[N / 32], low = 0;
