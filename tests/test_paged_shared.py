@@ -431,3 +431,27 @@ def test_prompt_rows_that_a_block_took_are_nan(io, cache):
     assert torch.equal(y[keep], want[keep]) and bool(y[~keep].isnan().all())
     status.zero_()
     assert torch.equal(R.paged_attn_prompt(q, k, v, table, n, starts, status=status), want) and int(status) == 0
+
+
+@pytest.mark.gpu
+def test_calls_on_several_streams_at_once():
+    """Five streams with calls of their own, none waiting for another: every result is the one of the call alone."""
+    torch = _cuda()
+    from kernel_optimization_webgpu_b200 import runtime as R
+    work = []
+    for i, (sizes, prefix, heads, io) in enumerate([([40], [3000], 8, "f16"), ([2] * 60, [200 + i for i in range(60)], 8, "f32"),
+                                                    ([1], [50], 2, "f16"), ([9, 1, 30], [700, 0, 1500], 16, "f32"), ([5], [129], 4, "f16")]):
+        c = make_shared(torch, sizes, prefix, [1 + 7 * b % 90 for b in range(sum(sizes))], 32, 2, "f16", seed=i)
+        work.append((torch.randn(sum(sizes), heads, D, device="cuda").to(_types(torch)[io]), *c[:6]))
+    want = [R.paged_attn_decode_shared(*w) for w in work]
+    streams = [torch.cuda.Stream() for _ in work]
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    got = [[] for _ in work]
+    for _ in range(30):
+        for i, s in enumerate(streams):
+            got[i].append(R.paged_attn_decode_shared(*work[i], status=status, stream=s))
+    torch.cuda.synchronize()
+    assert int(status) == 0
+    for ys, y in zip(got, want):
+        assert all(torch.equal(x, y) for x in ys)
